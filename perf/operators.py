@@ -219,7 +219,7 @@ def _own_token_logprobs(c, s):
     r = ops.token_logprobs(s["logits"], s["tokens"], top=c["top"], scale=c["scale"])
     out = [r.logp, r.entropy] + ([r.top_logp, r.top_index] if c["top"] else [])
     if c["train"]:
-        out.append(ops.token_logprobs_grad(s["logits"], s["tokens"], r.lse, r.entropy, s["g_logp"], s["g_entropy"],
+        out.append(ops.token_logprobs_grad(s["logits"], s["tokens"], r.stats, s["g_logp"], s["g_entropy"],
                                            scale=c["scale"]))
     return out
 

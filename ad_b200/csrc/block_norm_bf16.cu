@@ -1,0 +1,8 @@
+// The kernels of block_norm.cuh for __nv_bfloat16 (one type a file: they compile side by side).
+#include "block_norm.cuh"
+
+namespace adops {
+cudaError_t start_norm_bf16(const NormArgs& a, bool grad, bool gen, bool vec, unsigned blocks, cudaStream_t s) {
+  return start_norm_typed<__nv_bfloat16>(a, grad, gen, vec, blocks, s);
+}
+}  // namespace adops

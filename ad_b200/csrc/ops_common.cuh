@@ -1,0 +1,120 @@
+// What the language-model operators share: element types, vector loads and
+// stores, warp reductions, and the checks of their C entry points.
+#ifndef AD_B200_OPS_COMMON_CUH
+#define AD_B200_OPS_COMMON_CUH
+
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <cuda_runtime.h>
+
+#include <cstdarg>
+#include <cstdint>
+#include <cstdio>
+
+#include "../../include/ad_b200.h"
+
+namespace ad_b200_internal {
+void set_error(const char* msg);  // runtime.cu: the message ad_last_error() returns
+}
+
+namespace adops {
+
+inline int fail(const char* fmt, ...) {
+  char buf[512];
+  va_list ap;
+  va_start(ap, fmt);
+  vsnprintf(buf, sizeof(buf), fmt, ap);
+  va_end(ap);
+  ad_b200_internal::set_error(buf);
+  return 1;
+}
+
+// Makes `device` current for one call (-1: the current one) and puts the
+// caller's device back at its end.
+class DeviceGuard {
+ public:
+  explicit DeviceGuard(int device) {
+    err_ = cudaGetDevice(&prev_);
+    dev_ = device < 0 ? prev_ : device;
+    if (err_ == cudaSuccess && dev_ != prev_) {
+      err_ = cudaSetDevice(dev_);
+      moved_ = err_ == cudaSuccess;
+    }
+  }
+  ~DeviceGuard() {
+    if (moved_) cudaSetDevice(prev_);
+  }
+  cudaError_t error() const { return err_; }
+  int device() const { return dev_; }
+
+ private:
+  int prev_ = 0, dev_ = 0;
+  bool moved_ = false;
+  cudaError_t err_ = cudaSuccess;
+};
+
+// Multiprocessors of a device, asked for once; 0 with an error set on failure.
+inline int sm_count(int device) {
+  static int known[64] = {};
+  if (device >= 0 && device < 64 && known[device]) return known[device];
+  int n = 0;
+  if (cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, device) != cudaSuccess) return 0;
+  if (device >= 0 && device < 64) known[device] = n;
+  return n;
+}
+
+inline int elem_size(int dtype) { return dtype == AD_F32 ? 4 : 2; }
+inline bool aligned(const void* p, size_t n) { return (reinterpret_cast<uintptr_t>(p) & (n - 1)) == 0; }
+
+// ---------------------------------------------------------------- elements
+__device__ __forceinline__ float to_float(float x) { return x; }
+__device__ __forceinline__ float to_float(__nv_bfloat16 x) { return __bfloat162float(x); }
+__device__ __forceinline__ float to_float(__half x) { return __half2float(x); }
+template <typename T>
+__device__ __forceinline__ T from_float(float x);
+template <>
+__device__ __forceinline__ float from_float<float>(float x) { return x; }
+template <>
+__device__ __forceinline__ __nv_bfloat16 from_float<__nv_bfloat16>(float x) { return __float2bfloat16_rn(x); }
+template <>
+__device__ __forceinline__ __half from_float<__half>(float x) { return __float2half_rn(x); }
+
+// V elements moved by one load or store (V * sizeof(T) <= 16 bytes).
+template <typename T, int V>
+struct alignas(sizeof(T) * V) Vec {
+  T v[V];
+};
+template <typename T, int V>
+__device__ __forceinline__ Vec<T, V> load_vec(const T* p) {
+  return *reinterpret_cast<const Vec<T, V>*>(p);
+}
+template <typename T, int V>
+__device__ __forceinline__ void store_vec(T* p, const Vec<T, V>& x) {
+  *reinterpret_cast<Vec<T, V>*>(p) = x;
+}
+
+// Element i of an array whose type (AD_F32, AD_BF16, AD_F16) is known at run
+// time only: parameters that are read a few times a block.
+__device__ __forceinline__ float load_any(const void* p, int dtype, long long i) {
+  if (dtype == AD_F32) return static_cast<const float*>(p)[i];
+  if (dtype == AD_BF16) return to_float(static_cast<const __nv_bfloat16*>(p)[i]);
+  return to_float(static_cast<const __half*>(p)[i]);
+}
+__device__ __forceinline__ void store_any(void* p, int dtype, long long i, float x) {
+  if (dtype == AD_F32)
+    static_cast<float*>(p)[i] = x;
+  else if (dtype == AD_BF16)
+    static_cast<__nv_bfloat16*>(p)[i] = from_float<__nv_bfloat16>(x);
+  else
+    static_cast<__half*>(p)[i] = from_float<__half>(x);
+}
+
+__device__ __forceinline__ float warp_sum(float x) {
+#pragma unroll
+  for (int o = 16; o; o >>= 1) x += __shfl_xor_sync(0xffffffffu, x, o);
+  return x;
+}
+
+}  // namespace adops
+
+#endif

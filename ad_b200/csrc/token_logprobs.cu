@@ -1,0 +1,489 @@
+// Log probabilities of given tokens with entropy and best alternatives:
+// ad_token_logprobs and its gradient ad_token_logprobs_grad.
+//
+// With x a row of logits, k the factor on them (the reciprocal temperature),
+// m = max x, s = sum exp(k (x - m)), p = exp(k (x - m)) / s:
+//
+//   logp    = k (x[token] - m) - ln s
+//   entropy = ln s - sum p k (x - m)       (both terms are positive: no cancellation)
+//   d loss / d x_j = k (g (1[j = token] - p_j) - e p_j (ln p_j + entropy))
+//
+// for the gradients g of logp and e of the entropy.
+//
+// Bound by memory: the row is read once, every thread keeping a running
+// maximum, sum and weighted sum that are rescaled together when the maximum
+// grows (once for several vectors, not once a value).  Few rows over a large
+// vocabulary are split over a cluster of blocks that join through distributed
+// shared memory.  The best alternatives come from the same pass: a warp keeps
+// its 32 best in registers, one a lane, sorted; values above the worst of the
+// wanted ones so far are queued in shared memory and merged 32 at a time.  The
+// order is that of (logit, then lower index), a total one, so that the result
+// does not depend on scheduling.
+//
+// A NaN among the logits makes logp, entropy and gradient NaN; it is no alternative.
+// Values masked with -inf or the type's lowest value have p = 0; a row with
+// nothing but -inf has logp = -inf, entropy 0 and no gradient.
+#include <cooperative_groups.h>
+
+#include <cfloat>
+
+#include "ops_common.cuh"
+
+namespace {
+
+using namespace adops;
+namespace cg = cooperative_groups;
+
+constexpr int MAX_TOP = 32;
+constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.6931471805599453f;
+constexpr float GONE = -200.0f;  // 2^GONE is 0 in 32 bits
+
+__device__ __forceinline__ float exp2_approx(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+// max that keeps a NaN
+__device__ __forceinline__ float max_nan(float a, float b) {
+  float y;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(y) : "f"(a), "f"(b));
+  return y;
+}
+
+// Running softmax statistics: largest value, sum and sum weighted with the
+// exponent to base 2, both relative to the largest.  -FLT_MAX rather than -inf
+// at the start: -inf values then lie infinitely below it and count for nothing.
+struct Soft {
+  float m = -FLT_MAX, s = 0.0f, w = 0.0f;
+  __device__ __forceinline__ void raise(float to, float k) {
+    const float d = max_nan((m - to) * k, GONE), f = exp2_approx(d);
+    w = f * fmaf(d, s, w);
+    s *= f;
+    m = to;
+  }
+  __device__ __forceinline__ void add(float x, float k) {
+    const float d = max_nan((x - m) * k, GONE), e = exp2_approx(d);
+    s += e;
+    w = fmaf(e, d, w);
+  }
+  __device__ __forceinline__ void join(float om, float os, float ow, float k) {
+    const float to = fmaxf(m, om);
+    raise(to, k);
+    Soft o;
+    o.m = om, o.s = os, o.w = ow;
+    o.raise(to, k);
+    s += o.s;
+    w += o.w;
+  }
+};
+
+// Alternatives order by this: larger logit first, then lower index.
+__device__ __forceinline__ unsigned order_of(float x) {
+  const unsigned u = __float_as_uint(x + 0.0f);  // -0 counts as +0
+  return u ^ (static_cast<unsigned>(static_cast<int>(u) >> 31) | 0x80000000u);
+}
+__device__ __forceinline__ float value_of(unsigned o) {
+  return __uint_as_float(o & 0x80000000u ? o ^ 0x80000000u : ~o);
+}
+typedef unsigned long long u64;
+__device__ __forceinline__ u64 entry_of(float x, unsigned index) {
+  return static_cast<u64>(order_of(x)) << 32 | (0xffffffffu - index);
+}
+
+__device__ __forceinline__ u64 exchange(u64 v, int o, bool keep_larger) {
+  const u64 other = __shfl_xor_sync(0xffffffffu, v, o);
+  return (v > other) == keep_larger ? v : other;
+}
+// Largest first over the lanes of a warp.
+__device__ __forceinline__ u64 sort_warp(u64 v) {
+  const int lane = threadIdx.x & 31;
+#pragma unroll
+  for (int size = 2; size <= 32; size <<= 1)
+#pragma unroll
+    for (int o = size >> 1; o; o >>= 1) v = exchange(v, o, ((lane & o) == 0) == ((lane & size) == 0 || size == 32));
+  return v;
+}
+// The 32 largest of two descending lists, descending.
+__device__ __forceinline__ u64 merge_warp(u64 a, u64 b) {
+  const int lane = threadIdx.x & 31;
+  const u64 r = __shfl_sync(0xffffffffu, b, 31 - lane);
+  u64 v = a > r ? a : r;
+#pragma unroll
+  for (int o = 16; o; o >>= 1) v = exchange(v, o, (lane & o) == 0);
+  return v;
+}
+
+struct LogprobArgs {
+  const void* logits;
+  long long ld;
+  long long rows;
+  int vocab, top, tok64;
+  const void* tokens;
+  float scale;
+  float *logp, *entropy, *stats, *top_logp;
+  long long* top_index;
+};
+
+constexpr int QUEUE = 64;  // entries of a warp's queue: under 32 left over and 32 new
+
+// A warp's best so far.
+struct Best {
+  u64 list = 0;  // lane i: the i-th best
+  u64 bar = 0;   // a value has to pass this to be among the wanted ones
+  int queued = 0;
+
+  __device__ __forceinline__ void flush(u64* queue, u64* shared_bar, int top) {
+    const int lane = threadIdx.x & 31;
+    __syncwarp();
+    const int n = queued < 32 ? queued : 32;
+    const u64 v = lane < n ? queue[lane] : 0;
+    const u64 rest = lane + 32 < queued ? queue[lane + 32] : 0;
+    __syncwarp();
+    if (lane + 32 < queued) queue[lane] = rest;
+    queued -= n;
+    list = merge_warp(list, sort_warp(v));
+    const u64 mine = __shfl_sync(0xffffffffu, list, top - 1);
+    if (lane == 0 && mine > *reinterpret_cast<volatile u64*>(shared_bar)) atomicMax(shared_bar, mine);
+    __syncwarp();
+    const u64 all = *reinterpret_cast<volatile u64*>(shared_bar);
+    bar = mine > all ? mine : all;
+    bar = __shfl_sync(0xffffffffu, bar, 0);
+  }
+  // All lanes call; `x` counts where `valid`.
+  __device__ __forceinline__ void offer(float x, unsigned index, bool valid, u64* queue, u64* shared_bar, int top) {
+    const u64 e = entry_of(x, index);
+    const bool in = valid && x == x && e > bar;
+    const unsigned who = __ballot_sync(0xffffffffu, in);
+    if (!who) return;
+    if (in) queue[queued + __popc(who & ((1u << (threadIdx.x & 31)) - 1))] = e;
+    queued += __popc(who);
+    if (queued >= 32) flush(queue, shared_bar, top);
+  }
+};
+
+constexpr int MAX_WARPS = 16;
+
+struct Shared {
+  float m[MAX_WARPS], s[MAX_WARPS], w[MAX_WARPS];
+  u64 bar;
+  u64 queue[MAX_WARPS][QUEUE];
+  u64 list[MAX_WARPS][32];
+  // this block's result, read by the first block of the cluster
+  float bm, bs, bw;
+  u64 blist[32];
+};
+
+template <typename T, bool TOP>
+__global__ void __launch_bounds__(512) logprob_kernel(const __grid_constant__ LogprobArgs a) {
+  constexpr int V = 16 / sizeof(T), U = 4;  // vectors in flight
+  __shared__ Shared sh;
+  cg::cluster_group cluster = cg::this_cluster();
+  const int parts = cluster.num_blocks(), part = cluster.block_rank();
+  const long long row = blockIdx.x / parts;
+  const T* x = static_cast<const T*>(a.logits) + row * a.ld;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
+  const float k = a.scale * LOG2E;
+  if (TOP) {
+    if (threadIdx.x == 0) sh.bar = 0;
+    __syncthreads();
+  }
+  // The row as unaligned head, vectors, tail.
+  const int off = static_cast<int>((reinterpret_cast<uintptr_t>(x) & 15) / sizeof(T));
+  const int head = min(a.vocab, off ? V - off : 0);
+  const int vecs = (a.vocab - head) / V, tail0 = head + vecs * V;
+  const int share = (vecs + parts - 1) / parts;
+  const int v0 = min(vecs, part * share), v1 = min(vecs, v0 + share);
+  Soft soft;
+  Best best;
+  u64* queue = sh.queue[warp];
+
+  // warp-uniform trip count: the lanes of a warp stay together for the votes
+  for (int base = v0 + warp * 32; base < v1; base += blockDim.x * U) {
+    Vec<T, V> r[U];
+#pragma unroll
+    for (int q = 0; q < U; ++q) {
+      const int v = base + q * blockDim.x + lane;
+      if (v < v1) {
+        r[q] = load_vec<T, V>(x + head + static_cast<long long>(v) * V);
+      } else {
+#pragma unroll
+        for (int j = 0; j < V; ++j) r[q].v[j] = from_float<T>(-INFINITY);
+      }
+    }
+    float big = -FLT_MAX;
+#pragma unroll
+    for (int q = 0; q < U; ++q)
+#pragma unroll
+      for (int j = 0; j < V; ++j) big = fmaxf(big, to_float(r[q].v[j]));
+    if (big > soft.m) soft.raise(big, k);
+#pragma unroll
+    for (int q = 0; q < U; ++q)
+#pragma unroll
+      for (int j = 0; j < V; ++j) soft.add(to_float(r[q].v[j]), k);
+    if (TOP) {
+      // The first values: the wanted number of lanes' maxima reach `seed`, so no
+      // alternative lies below it.
+      if (best.bar == 0) {
+        const unsigned seed = __shfl_sync(0xffffffffu, static_cast<unsigned>(sort_warp(order_of(big))), a.top - 1);
+        if (seed > order_of(-FLT_MAX)) best.bar = static_cast<u64>(seed) << 32;
+      }
+      const float bar = best.bar ? value_of(static_cast<unsigned>(best.bar >> 32)) : -INFINITY;
+      if (__any_sync(0xffffffffu, big >= bar || best.bar == 0)) {
+        unsigned pass = 0;
+#pragma unroll
+        for (int q = 0; q < U; ++q)
+#pragma unroll
+          for (int j = 0; j < V; ++j)
+            if (base + q * blockDim.x + lane < v1 && to_float(r[q].v[j]) >= bar) pass |= 1u << (q * V + j);
+        // one a lane at a time, read again: registers cannot be indexed
+        while (__any_sync(0xffffffffu, pass != 0)) {
+          const int bit = __ffs(pass) - 1;
+          pass &= pass - 1;
+          const int i = head + (base + (bit / V) * static_cast<int>(blockDim.x) + lane) * V + bit % V;
+          best.offer(bit >= 0 ? to_float(x[i]) : 0.0f, i, bit >= 0, queue, &sh.bar, a.top);
+        }
+      }
+    }
+  }
+  // Head and tail: fewer than a vector each, by the first block's first warp.
+  if (part == 0 && warp == 0) {
+    const int rest = head + (a.vocab - tail0);
+    const bool has = lane < rest;
+    const int i = lane < head ? lane : tail0 + (lane - head);
+    const float xi = has ? to_float(x[i]) : -INFINITY;
+    if (has) {
+      if (xi > soft.m) soft.raise(xi, k);
+      soft.add(xi, k);
+    }
+    if (TOP) best.offer(xi, i, has, queue, &sh.bar, a.top);
+  }
+  // Lanes, warps, blocks.
+#pragma unroll
+  for (int o = 16; o; o >>= 1) {
+    const float m = __shfl_xor_sync(0xffffffffu, soft.m, o), s = __shfl_xor_sync(0xffffffffu, soft.s, o),
+                w = __shfl_xor_sync(0xffffffffu, soft.w, o);
+    soft.join(m, s, w, k);
+  }
+  if (lane == 0) sh.m[warp] = soft.m, sh.s[warp] = soft.s, sh.w[warp] = soft.w;
+  if (TOP) {
+    while (best.queued) best.flush(queue, &sh.bar, a.top);
+    sh.list[warp][lane] = best.list;
+  }
+  __syncthreads();
+  if (warp == 0) {
+    Soft t;
+    for (int i = 0; i < warps; ++i) t.join(sh.m[i], sh.s[i], sh.w[i], k);
+    if (TOP)
+      for (int i = 1; i < warps; ++i) best.list = merge_warp(best.list, sh.list[i][lane]);
+    soft = t;
+    if (parts > 1) {
+      if (lane == 0) sh.bm = t.m, sh.bs = t.s, sh.bw = t.w;
+      if (TOP) sh.blist[lane] = best.list;
+    }
+  }
+  if (parts > 1) {
+    cluster.sync();
+    if (part == 0 && warp == 0) {
+      for (int i = 1; i < parts; ++i) {
+        const Shared* o = cluster.map_shared_rank(&sh, i);
+        soft.join(o->bm, o->bs, o->bw, k);
+        if (TOP) best.list = merge_warp(best.list, o->blist[lane]);
+      }
+    }
+    cluster.sync();  // no block ends while its shared memory is read
+  }
+  if (part == 0 && warp == 0) {
+    const bool empty = soft.s == 0.0f;
+    const float ln_s = empty ? 0.0f : logf(soft.s);
+    if (lane == 0) {
+      const long long t =
+          a.tok64 ? static_cast<const long long*>(a.tokens)[row] : static_cast<const int*>(a.tokens)[row];
+      float lp = 0.0f;
+      if (t >= a.vocab)
+        lp = __int_as_float(0x7fffffff);
+      else if (t >= 0)
+        lp = empty ? -INFINITY : (to_float(x[t]) - soft.m) * a.scale - ln_s;
+      const float h = empty ? 0.0f : ln_s - LN2 * (soft.w / soft.s);
+      a.logp[row] = lp;
+      a.entropy[row] = h;
+      reinterpret_cast<float4*>(a.stats)[row] =
+          make_float4(soft.m, soft.s, h, empty ? -INFINITY : fmaf(soft.m, a.scale, ln_s));
+    }
+    if (TOP && lane < a.top) {
+      const float v = value_of(static_cast<unsigned>(best.list >> 32));
+      a.top_logp[row * a.top + lane] = empty ? -INFINITY : (v - soft.m) * a.scale - ln_s;
+      a.top_index[row * a.top + lane] =
+          best.list ? static_cast<long long>(0xffffffffu - static_cast<unsigned>(best.list)) : -1ll;
+    }
+  }
+}
+
+struct LogprobGradArgs {
+  const void* logits;
+  void* out;
+  long long ld, ldo;
+  long long rows;
+  int vocab, segments, tok64;
+  const void* tokens;
+  float scale;
+  const float *stats, *g_logp, *g_entropy;
+};
+
+constexpr int GRAD_THREADS = 256, GRAD_VECS = 4;  // a block's share of a row: so many vectors a thread
+
+// V = 1 where rows of the result are not aligned as those of the logits are.
+template <typename T, int V>
+__global__ void __launch_bounds__(GRAD_THREADS) logprob_grad_kernel(const __grid_constant__ LogprobGradArgs a) {
+  const long long row = blockIdx.x / a.segments;
+  const int seg = static_cast<int>(blockIdx.x - row * a.segments);
+  const T* x = static_cast<const T*>(a.logits) + row * a.ld;
+  T* y = static_cast<T*>(a.out) + row * a.ldo;
+  const int off = static_cast<int>((reinterpret_cast<uintptr_t>(x) & 15) / sizeof(T));
+  const int head = V == 1 ? 0 : min(a.vocab, off ? V - off : 0);
+  const int vecs = (a.vocab - head) / V, tail0 = head + vecs * V;
+  Vec<T, V> r[GRAD_VECS];
+  const int first = seg * (GRAD_THREADS * GRAD_VECS) + threadIdx.x;
+#pragma unroll
+  for (int q = 0; q < GRAD_VECS; ++q) {
+    const int v = first + q * GRAD_THREADS;
+    if (v < vecs) r[q] = load_vec<T, V>(x + head + static_cast<long long>(v) * V);
+  }
+  const float4 st = reinterpret_cast<const float4*>(a.stats)[row];
+  const long long t = a.tok64 ? static_cast<const long long*>(a.tokens)[row] : static_cast<const int*>(a.tokens)[row];
+  const bool empty = st.w == -INFINITY;
+  float g = t >= 0 && a.g_logp ? a.g_logp[row] : 0.0f;
+  const float e = a.g_entropy ? a.g_entropy[row] : 0.0f;
+  if (t >= a.vocab) g *= __int_as_float(0x7fffffff);
+  const float hot = empty ? 0.0f : g * a.scale;
+  // with l = k (x - m): -k p (g + e (l - ln s + H)) = q exp(l) (g' + e l)
+  const float k = a.scale * LOG2E, el = e * LN2;
+  const float c = empty ? 0.0f : -a.scale / st.y, b = empty ? 0.0f : g + e * (st.z - logf(st.y));
+  auto grad = [&](float v) {
+    const float d = max_nan((v - st.x) * k, GONE);
+    return c * exp2_approx(d) * fmaf(el, d, b);
+  };
+#pragma unroll
+  for (int q = 0; q < GRAD_VECS; ++q) {
+    const int v = first + q * GRAD_THREADS;
+    if (v >= vecs) continue;
+    const int i = head + v * V;
+    float o[V];
+#pragma unroll
+    for (int j = 0; j < V; ++j) o[j] = grad(to_float(r[q].v[j]));
+    if (t >= i && t < i + V) {
+#pragma unroll
+      for (int j = 0; j < V; ++j)
+        if (t == i + j) o[j] += hot;
+    }
+    Vec<T, V> w;
+#pragma unroll
+    for (int j = 0; j < V; ++j) w.v[j] = from_float<T>(o[j]);
+    store_vec<T, V>(y + i, w);
+  }
+  const int rest = head + (a.vocab - tail0);
+  if (seg == 0 && static_cast<int>(threadIdx.x) < rest) {
+    const int i = static_cast<int>(threadIdx.x) < head ? threadIdx.x : tail0 + (threadIdx.x - head);
+    y[i] = from_float<T>(grad(to_float(x[i])) + (t == i ? hot : 0.0f));
+  }
+}
+
+template <typename T>
+cudaError_t forward(const LogprobArgs& a, int sms, cudaStream_t s) {
+  const int vecs = a.vocab / (16 / static_cast<int>(sizeof(T)));
+  // Threads for four vectors each, blocks of a cluster while the rows leave
+  // multiprocessors without work and a block keeps a vector a thread.
+  int threads = 64;
+  while (threads < 512 && threads * 4 < vecs) threads *= 2;
+  int parts = 1;
+  while (parts < 8 && a.rows * parts * 2 <= sms && parts * 2 * threads <= vecs) parts *= 2;
+  cudaLaunchConfig_t c = {};
+  c.gridDim = dim3(static_cast<unsigned>(a.rows * parts));
+  c.blockDim = dim3(threads);
+  c.stream = s;
+  cudaLaunchAttribute at[1];
+  at[0].id = cudaLaunchAttributeClusterDimension;
+  at[0].val.clusterDim.x = parts;
+  at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
+  c.attrs = at;
+  c.numAttrs = 1;
+  return a.top ? cudaLaunchKernelEx(&c, logprob_kernel<T, true>, a) : cudaLaunchKernelEx(&c, logprob_kernel<T, false>, a);
+}
+
+template <typename T>
+cudaError_t backward(LogprobGradArgs a, cudaStream_t s) {
+  constexpr int V = 16 / sizeof(T);
+  const bool same = ((reinterpret_cast<uintptr_t>(a.logits) ^ reinterpret_cast<uintptr_t>(a.out)) & 15) == 0 &&
+                    ((a.ld - a.ldo) * static_cast<long long>(sizeof(T))) % 16 == 0;
+  const long long per = static_cast<long long>(GRAD_THREADS) * GRAD_VECS * (same ? V : 1);
+  a.segments = static_cast<int>((a.vocab + per - 1) / per);
+  const long long blocks = a.rows * a.segments;
+  if (blocks > 0x7fffffffll) return cudaErrorInvalidValue;
+  if (same)
+    logprob_grad_kernel<T, V><<<static_cast<unsigned>(blocks), GRAD_THREADS, 0, s>>>(a);
+  else
+    logprob_grad_kernel<T, 1><<<static_cast<unsigned>(blocks), GRAD_THREADS, 0, s>>>(a);
+  return cudaGetLastError();
+}
+
+int check(const char* who, int dtype, const void* logits, int64_t ld, int64_t rows, int64_t vocab, const void* tokens,
+          float scale) {
+  if (dtype < AD_F32 || dtype > AD_F16) return fail("%s: unknown element type %d", who, dtype);
+  if (rows < 0 || vocab < 1 || vocab > 0x7fff0000ll) return fail("%s: %lld rows of %lld logits", who, (long long)rows, (long long)vocab);
+  if (rows > 0x0fffffffll) return fail("%s: %lld rows in one call", who, (long long)rows);
+  if (!(scale > 0.0f) || scale > FLT_MAX) return fail("%s: the factor %g is not a positive number", who, scale);
+  if (rows && (!logits || !tokens)) return fail("%s: null operand", who);
+  if (rows > 1 && ld < vocab) return fail("%s: rows overlap", who);
+  if (!aligned(logits, elem_size(dtype))) return fail("%s: unaligned logits", who);
+  return 0;
+}
+
+}  // namespace
+
+extern "C" int ad_token_logprobs(int device, int dtype, const void* logits, int64_t ld, int64_t rows, int64_t vocab,
+                                 const void* tokens, int tok64, float scale, int top, float* logp, float* entropy,
+                                 float* stats, float* top_logp, int64_t* top_index, void* stream) {
+  if (check("ad_token_logprobs", dtype, logits, ld, rows, vocab, tokens, scale)) return 1;
+  if (top < 0 || top > MAX_TOP || top > vocab)
+    return fail("ad_token_logprobs: %d alternatives (at most %d, and no more than logits)", top, MAX_TOP);
+  if (rows == 0) return 0;
+  if (!logp || !entropy || !stats || !aligned(stats, 16) || (top && (!top_logp || !top_index)))
+    return fail("ad_token_logprobs: null or unaligned result");
+  DeviceGuard g(device);
+  if (g.error() != cudaSuccess) return fail("ad_token_logprobs: %s", cudaGetErrorString(g.error()));
+  const int sms = sm_count(g.device());
+  if (!sms) return fail("ad_token_logprobs: no device properties");
+  LogprobArgs a = {};
+  a.logits = logits, a.ld = ld, a.rows = rows, a.vocab = static_cast<int>(vocab), a.top = top;
+  a.tokens = tokens, a.tok64 = tok64, a.scale = scale;
+  a.logp = logp, a.entropy = entropy, a.stats = stats, a.top_logp = top_logp;
+  a.top_index = reinterpret_cast<long long*>(top_index);
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  const cudaError_t e = dtype == AD_F32    ? forward<float>(a, sms, s)
+                        : dtype == AD_BF16 ? forward<__nv_bfloat16>(a, sms, s)
+                                           : forward<__half>(a, sms, s);
+  if (e != cudaSuccess) return fail("ad_token_logprobs: %s", cudaGetErrorString(e));
+  return 0;
+}
+
+extern "C" int ad_token_logprobs_grad(int device, int dtype, const void* logits, int64_t ld, int64_t rows,
+                                      int64_t vocab, const void* tokens, int tok64, float scale, const float* stats,
+                                      const float* g_logp, const float* g_entropy, void* grad, int64_t ld_grad,
+                                      void* stream) {
+  if (check("ad_token_logprobs_grad", dtype, logits, ld, rows, vocab, tokens, scale)) return 1;
+  if (rows == 0) return 0;
+  if (!stats || !aligned(stats, 16) || !grad || !aligned(grad, elem_size(dtype)))
+    return fail("ad_token_logprobs_grad: null or unaligned operand");
+  if (rows > 1 && ld_grad < vocab) return fail("ad_token_logprobs_grad: rows of the gradient overlap");
+  DeviceGuard g(device);
+  if (g.error() != cudaSuccess) return fail("ad_token_logprobs_grad: %s", cudaGetErrorString(g.error()));
+  LogprobGradArgs a = {};
+  a.logits = logits, a.out = grad, a.ld = ld, a.ldo = ld_grad, a.rows = rows, a.vocab = static_cast<int>(vocab);
+  a.tokens = tokens, a.tok64 = tok64, a.scale = scale;
+  a.stats = stats, a.g_logp = g_logp, a.g_entropy = g_entropy;
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  const cudaError_t e = dtype == AD_F32    ? backward<float>(a, s)
+                        : dtype == AD_BF16 ? backward<__nv_bfloat16>(a, s)
+                                           : backward<__half>(a, s);
+  if (e != cudaSuccess) return fail("ad_token_logprobs_grad: %s", cudaGetErrorString(e));
+  return 0;
+}

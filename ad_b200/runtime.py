@@ -20,6 +20,8 @@ c_uint = ctypes.c_uint
 c_size_t = ctypes.c_size_t
 c_u64 = ctypes.c_uint64
 c_u32 = ctypes.c_uint32
+c_i64 = ctypes.c_int64
+c_float = ctypes.c_float
 c_char_p = ctypes.c_char_p
 
 # name -> (restype, argtypes); must match include/ad_b200.h
@@ -74,6 +76,22 @@ SIGNATURES = {
     "ad_peer_close": (c_int, [c_void_p]),
     "ad_profiler_range": (c_int, [c_int]),
     "ad_dot_tf32x3_noalloc": (c_int, [c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_void_p]),
+    "ad_rotary": (c_int, [c_int, c_int, c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_void_p, c_void_p, c_void_p,
+                          c_void_p, c_int, c_i64, c_i64, c_int, c_int, c_int, c_int, c_void_p, c_void_p, c_i64,
+                          c_void_p, c_int, c_i64, c_i64, c_void_p]),
+    "ad_block_norm": (c_int, [c_int, c_int, c_int, c_int, c_void_p, c_i64, c_void_p, c_i64, c_void_p, c_i64, c_i64,
+                              c_int, c_void_p, c_void_p, c_void_p, c_void_p, c_float, c_float, c_i64, c_int, c_void_p,
+                              c_i64, c_void_p, c_i64, c_void_p, c_void_p]),
+    "ad_block_norm_grad_workspace": (c_int, [c_int, c_i64, c_int, c_i64, ctypes.POINTER(c_size_t)]),
+    "ad_block_norm_grad": (c_int, [c_int, c_int, c_int, c_int, c_void_p, c_i64, c_void_p, c_i64, c_void_p, c_i64,
+                                   c_void_p, c_i64, c_void_p, c_i64, c_i64, c_int, c_void_p, c_void_p, c_void_p,
+                                   c_void_p, c_float, c_void_p, c_i64, c_int, c_void_p, c_i64, c_void_p, c_i64,
+                                   c_void_p, c_i64, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_size_t,
+                                   c_void_p]),
+    "ad_token_logprobs": (c_int, [c_int, c_int, c_void_p, c_i64, c_i64, c_i64, c_void_p, c_int, c_float, c_int,
+                                  c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p]),
+    "ad_token_logprobs_grad": (c_int, [c_int, c_int, c_void_p, c_i64, c_i64, c_i64, c_void_p, c_int, c_float,
+                                       c_void_p, c_void_p, c_void_p, c_void_p, c_i64, c_void_p]),
 }
 
 

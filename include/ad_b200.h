@@ -162,6 +162,81 @@ int ad_profiler_range(int on);
 int ad_dot_tf32x3_noalloc(const float* A, const float* B, float* C, int M, int N, int K,
                           int b_is_nk, void* stream);
 
+/* ---- Operators of language models (no reference counterpart: the reference
+ * composes such steps from its elementwise, reduce and dot nodes) ------------
+ *
+ * They work on the caller's device memory, allocate nothing, launch on
+ * `stream` (a cudaStream_t; NULL = the legacy default stream) and return
+ * without waiting.  `device`: the device that the memory and the stream belong
+ * to, or -1 for the current one.  Element types are AD_F32, AD_BF16, AD_F16;
+ * strides count elements, not bytes, and a row's elements are adjacent.  Sums
+ * are held in 32 bits or more and results do not depend on scheduling.
+ * Results may not overlap operands unless a call allows it. */
+#define AD_F32 0
+#define AD_BF16 1
+#define AD_F16 2
+
+/* Rotary positions of queries and keys (k_heads or q_heads may be 0).
+ * Operands are [sequences][tokens][heads][dim] with the strides of the first
+ * three axes; results may be their operands.  The first `rotary` elements of a
+ * head are rotary / 2 pairs: (x[i], x[i + rotary/2]) with layout 0,
+ * (x[2i], x[2i+1]) with layout 1; pair (u, v) becomes (u c - v s, v c + u s)
+ * with c, s from row positions[token] of the [table_rows][rotary / 2] tables
+ * (s negated when `inverse`: also the gradient).  A position outside the
+ * tables makes NaNs.  Positions are of 64 bits when pos64, else of 32. */
+int ad_rotary(int device, int dtype, const void* q, const int64_t* q_strides, void* q_out,
+              const int64_t* q_out_strides, int q_heads, const void* k, const int64_t* k_strides,
+              void* k_out, const int64_t* k_out_strides, int k_heads, int64_t sequences,
+              int64_t tokens, int dim, int rotary, int layout, int inverse, const float* cos,
+              const float* sin, int64_t table_rows, const void* positions, int pos64,
+              int64_t pos_seq_stride, int64_t pos_tok_stride, void* stream);
+
+/* Norms around a block with its gate and the scaled residual sum:
+ *   u = norm(z) wa + ba (u = z when wa is NULL),
+ *   h = scale x + act(gate) u (h = scale x + u when gate is NULL),
+ *   y = norm(h) wb + bb (no y when wb is NULL).
+ * kind 0: v / sqrt(mean v^2 + eps); 1: LayerNorm.  act is the sigmoid when
+ * gate_sigmoid, else the identity.  Gate row r belongs to the rows
+ * [r rows_per_gate, (r + 1) rows_per_gate).  Weights and biases are of type
+ * wtype: AD_F32 or dtype.  stats: rows * 4 floats (16-byte aligned) for the
+ * gradient.  h may be x or z, y may be the other one. */
+int ad_block_norm(int device, int dtype, int wtype, int kind, const void* x, int64_t ldx,
+                  const void* z, int64_t ldz, const void* gate, int64_t ldg,
+                  int64_t rows_per_gate, int gate_sigmoid, const void* wa, const void* ba,
+                  const void* wb, const void* bb, float scale, float eps, int64_t rows, int width,
+                  void* h, int64_t ldh, void* y, int64_t ldy, float* stats, void* stream);
+/* Bytes of workspace that ad_block_norm_grad needs; rows_per_gate 0: no gate. */
+int ad_block_norm_grad_workspace(int device, int64_t rows, int width, int64_t rows_per_gate,
+                                 size_t* bytes);
+/* The gradients of ad_block_norm's operands from those of h and y: dx, dz, the
+ * gate's (of its shape) and, of type wtype, the weights' and biases'. */
+int ad_block_norm_grad(int device, int dtype, int wtype, int kind, const void* dh, int64_t lddh,
+                       const void* dy, int64_t lddy, const void* x, int64_t ldx, const void* z,
+                       int64_t ldz, const void* gate, int64_t ldg, int64_t rows_per_gate,
+                       int gate_sigmoid, const void* wa, const void* ba, const void* wb,
+                       const void* bb, float scale, const float* stats, int64_t rows, int width,
+                       void* dx, int64_t lddx, void* dz, int64_t lddz, void* dgate, int64_t lddg,
+                       void* dwa, void* dba, void* dwb, void* dbb, void* workspace,
+                       size_t workspace_bytes, void* stream);
+
+/* Of each row of scale * logits: the log probability of its token (0 for a
+ * negative token, NaN for one past the vocabulary), the entropy of its
+ * distribution, and the `top` (at most 32) most likely tokens with their log
+ * probabilities, the lower index first among equal logits (-1 where fewer than
+ * `top` logits are numbers).  Tokens are of 64 bits when tok64, else of 32.
+ * stats: rows * 4 floats (16-byte aligned): the largest logit, the sum of
+ * exp(scale (x - largest)), the entropy, the log of the sum of exp(scale x). */
+int ad_token_logprobs(int device, int dtype, const void* logits, int64_t ld, int64_t rows,
+                      int64_t vocab, const void* tokens, int tok64, float scale, int top,
+                      float* logp, float* entropy, float* stats, float* top_logp,
+                      int64_t* top_index, void* stream);
+/* The gradient of the logits from g_logp and g_entropy (rows floats each; NULL:
+ * zeros).  `grad` may be the logits themselves. */
+int ad_token_logprobs_grad(int device, int dtype, const void* logits, int64_t ld, int64_t rows,
+                           int64_t vocab, const void* tokens, int tok64, float scale,
+                           const float* stats, const float* g_logp, const float* g_entropy,
+                           void* grad, int64_t ld_grad, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

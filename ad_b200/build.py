@@ -16,7 +16,7 @@ ROOT = os.path.dirname(PKG)
 LIB = os.path.join(PKG, "libad_b200.so")
 SOURCES = [os.path.join(PKG, "csrc", f) for f in (
     "runtime.cu", "noalloc.cu", "rotary.cu", "block_norm.cu", "block_norm_f32.cu", "block_norm_bf16.cu",
-    "block_norm_f16.cu", "token_logprobs.cu")]
+    "block_norm_f16.cu", "token_logprobs.cu", "orthogonalize.cu")]
 HEADERS = [os.path.join(ROOT, "include", "ad_b200.h"), os.path.join(PKG, "csrc", "ops_common.cuh"),
            os.path.join(PKG, "csrc", "block_norm.cuh")]
 NVCC = os.environ.get("NVCC", "/usr/local/cuda/bin/nvcc")

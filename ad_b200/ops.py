@@ -5,6 +5,7 @@
   and the norm before the next block
 * ``token_logprobs`` / ``token_logprobs_grad``: log probabilities of given tokens, entropy and the
   best alternatives of rows of logits
+* ``orthogonalize``: Newton-Schulz orthogonalisation of matrix updates
 
 Operands are device arrays: torch CUDA tensors, or ``DeviceArray`` views of memory from
 ``runtime.Context.malloc`` (this module imports no framework by itself).  Elements are float32,
@@ -581,4 +582,65 @@ def token_logprobs_grad(logits, tokens, stats, g_logp=None, g_entropy=None, *, s
     rt.check(rt.lib().ad_token_logprobs_grad(
         dev, dt, logits.data_ptr(), ld, rows, vocab, tokens.data_ptr(), t64, scale, stats.data_ptr(), _ptr(g_logp),
         _ptr(g_entropy), out.data_ptr(), ldo, s))
+    return out
+
+
+# ------------------------------------------------------------------ orthogonalised updates
+
+NEWTON_SCHULZ = (3.4445, -4.7750, 2.0315)  # a quintic that brings singular values near 1 in a few steps
+
+
+def orthogonalize_workspace(count: int, rows: int, cols: int) -> int:
+    """Bytes of workspace that ``orthogonalize`` needs."""
+    n = rt.c_size_t()
+    rt.check(rt.lib().ad_orthogonalize_workspace(count, rows, cols, ctypes.byref(n)), "ad_orthogonalize_workspace")
+    return n.value
+
+
+def orthogonalize(g, *, steps: int = 5, coefficients=NEWTON_SCHULZ, eps: float = 1e-7, out=None, workspace=None,
+                  stream=None):
+    """Newton-Schulz orthogonalisation of an update: of each matrix of ``g`` ([rows, cols] or [count,
+    rows, cols], any strides), X = G / (|G| + eps), then ``steps`` times X = a X + (b A + c A A) X with
+    A = X X^T (taken from the side with fewer rows).  ``coefficients``: (a, b, c), or one such triple a
+    step.  Products have operands of 11 bits and sums of 32, so the result is within about 1e-3
+    (norm-wise) of the exact iteration; it is bfloat16, or of ``out``'s type.  A zero matrix gives
+    zeros, one with a NaN or an infinity NaNs.  ``workspace``: adjacent elements at a 256-byte
+    boundary, ``orthogonalize_workspace`` bytes or more."""
+    dt = _float(g, "g")
+    dev = _device(g, "g")
+    shape, st = g.shape, g.stride()
+    if len(shape) == 2:
+        count, (rows, cols), sb, (sr, sc) = 1, shape, 0, st
+    elif len(shape) == 3:
+        (count, rows, cols), (sb, sr, sc) = shape, st
+    else:
+        raise ValueError(f"g: expected [rows, cols] or [count, rows, cols], got {tuple(shape)}")
+    if not 0 <= steps <= 32:
+        raise ValueError(f"steps: {steps} (0 to 32)")
+    coef = list(coefficients)
+    if len(coef) == 3 and not hasattr(coef[0], "__len__"):
+        coef = coef * steps
+    else:
+        if len(coef) != steps or any(len(c) != 3 for c in coef):
+            raise ValueError(f"coefficients: expected a triple, or {steps} of them")
+        coef = [v for c in coef for v in c]
+    s = _stream(dev, stream, g, out is None or workspace is None)
+    if out is None:
+        out = _empty(shape, g, "bfloat16")
+    ot = _float(out, "out")
+    _same_shape(out, shape, "out")
+    _on(dev, out, "out")
+    so = out.stride()
+    if any(n > 1 and not m for n, m in zip(shape, so)):
+        raise ValueError(f"out: elements share memory (strides {tuple(so)})")
+    need = orthogonalize_workspace(count, rows, cols)
+    if workspace is None:
+        workspace = _empty((need,), g, "uint8")
+        have = need
+    else:
+        _on(dev, workspace, "workspace")
+        have = _nbytes(workspace, "workspace")
+    rt.check(rt.lib().ad_orthogonalize(
+        dev, dt, g.data_ptr(), count, rows, cols, sb, sr, sc, steps, (rt.c_float * max(1, len(coef)))(*coef), eps, ot,
+        out.data_ptr(), so[0] if len(so) == 3 else 0, so[-2], so[-1], workspace.data_ptr(), have, s))
     return out

@@ -92,6 +92,9 @@ SIGNATURES = {
                                   c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p]),
     "ad_token_logprobs_grad": (c_int, [c_int, c_int, c_void_p, c_i64, c_i64, c_i64, c_void_p, c_int, c_float,
                                        c_void_p, c_void_p, c_void_p, c_void_p, c_i64, c_void_p]),
+    "ad_orthogonalize_workspace": (c_int, [c_i64, c_i64, c_i64, ctypes.POINTER(c_size_t)]),
+    "ad_orthogonalize": (c_int, [c_int, c_int, c_void_p, c_i64, c_i64, c_i64, c_i64, c_i64, c_i64, c_int, c_void_p,
+                                 c_float, c_int, c_void_p, c_i64, c_i64, c_i64, c_void_p, c_size_t, c_void_p]),
 }
 
 

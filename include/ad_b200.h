@@ -237,6 +237,21 @@ int ad_token_logprobs_grad(int device, int dtype, const void* logits, int64_t ld
                            const float* stats, const float* g_logp, const float* g_entropy,
                            void* grad, int64_t ld_grad, void* stream);
 
+/* Newton-Schulz orthogonalisation of `count` matrices G of rows x cols:
+ * X = G / (|G|_F + eps), then `steps` (0 to 32) times X = a X + (b A + c A A) X
+ * with A = X X^T and three coefficients a, b, c a step (host memory), from the
+ * side with fewer rows.  Any strides; the result must not overlap G.  Products
+ * take operands of 11 bits and accumulate in 32: the result is within about
+ * 1e-3 (norm-wise) of the exact iteration.  Coefficients that let a singular
+ * value grow past 1024 are refused.  A zero matrix gives zeros, one with NaN or
+ * infinity NaNs.  The workspace is 256-byte aligned. */
+int ad_orthogonalize_workspace(int64_t count, int64_t rows, int64_t cols, size_t* bytes);
+int ad_orthogonalize(int device, int dtype, const void* g, int64_t count, int64_t rows,
+                     int64_t cols, int64_t batch_stride, int64_t row_stride, int64_t col_stride,
+                     int steps, const float* coefficients, float eps, int out_dtype, void* out,
+                     int64_t out_batch_stride, int64_t out_row_stride, int64_t out_col_stride,
+                     void* workspace, size_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

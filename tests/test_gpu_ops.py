@@ -602,3 +602,123 @@ def test_graph_capture_and_repeats(ops):
     again = step()
     for a, b, c in zip(first, held, again):
         assert torch.equal(a, b) and torch.equal(a, c)
+
+
+# ------------------------------------------------------------------ orthogonalised updates
+
+def orthogonal64(g, steps, coef, eps):
+    out = []
+    for x in g.double():
+        x = x / (x.square().sum().sqrt() + eps)
+        for k in range(steps):
+            a, b, c = coef[k]
+            if x.shape[0] <= x.shape[1]:
+                p = x @ x.T
+                x = a * x + (b * p + c * (p @ p)) @ x
+            else:
+                p = x.T @ x
+                x = a * x + x @ (b * p + c * (p @ p))
+        out.append(x)
+    return torch.stack(out)
+
+
+# A step rounds three operands (X, A, B) to 11 bits: 2^-11 / sqrt(3) of their norms each (the
+# root mean square of the rounding), added up over the steps as if none cancelled; then the result.
+def check_orthogonal(got, want, steps, t):
+    rms = 3 * steps * 2.0 ** -11 / math.sqrt(3) + U[t] / math.sqrt(3) + 2.0 ** -20
+    for a, b in zip(got.double(), want):
+        assert float((a - b).norm()) <= rms * float(b.norm()) + 1e-30, (float((a - b).norm() / b.norm()), rms)
+
+
+def update(gen, count, rows, cols, kind, t):
+    r = min(rows, cols)
+    if kind == "noise":
+        g = torch.randn(count, rows, cols, generator=gen, dtype=torch.float64)
+    elif kind == "decay":
+        g = (torch.randn(count, rows, r, generator=gen, dtype=torch.float64) / torch.arange(1, r + 1)) @ torch.randn(
+            count, r, cols, generator=gen, dtype=torch.float64)
+    else:
+        g = torch.randn(count, rows, 1, generator=gen, dtype=torch.float64) @ torch.randn(
+            count, 1, cols, generator=gen, dtype=torch.float64)
+    return (1e-3 * g).to(dtype(t)).cuda()
+
+
+@pytest.mark.parametrize("kind", ["noise", "decay", "rank one"])
+@pytest.mark.parametrize("t", ["float32", "bfloat16"])
+@pytest.mark.parametrize("count,rows,cols", [(1, 128, 128), (3, 64, 256), (2, 300, 130), (1, 513, 1000), (2, 7, 5),
+                                             (1, 1, 70), (1, 90, 1), (5, 129, 127), (1, 1100, 400)])
+def test_orthogonalize(ops, kind, t, count, rows, cols):
+    gen = seeded(count, rows, cols, len(kind))
+    g = update(gen, count, rows, cols, kind, t)
+    want = orthogonal64(g, 5, [ops.NEWTON_SCHULZ] * 5, 1e-7)
+    check_orthogonal(ops.orthogonalize(g), want, 5, "bfloat16")
+    out = torch.full((count, rows, cols), math.nan, device="cuda")
+    assert ops.orthogonalize(g, out=out) is out
+    check_orthogonal(out, want, 5, "float32")
+
+
+def test_orthogonalize_steps_and_coefficients(ops):
+    gen = seeded(40)
+    g = update(gen, 2, 200, 310, "noise", "float32")
+    cubic, quintic = (1.5, -0.5, 0.0), (3.4445, -4.7750, 2.0315)
+    for coef in ([], [quintic], [quintic] * 3 + [cubic] * 5, [(2.0, -1.5, 0.5)] * 12):
+        out = torch.empty((2, 200, 310), device="cuda")
+        ops.orthogonalize(g, steps=len(coef), coefficients=coef, out=out)
+        check_orthogonal(out, orthogonal64(g, len(coef), coef, 1e-7), len(coef), "float32")
+    # enough steps bring every singular value to 1
+    s = torch.linalg.svdvals(ops.orthogonalize(g, steps=13, coefficients=[quintic] * 5 + [cubic] * 8,
+                                               out=torch.empty((2, 200, 310), device="cuda")))
+    assert float((s - 1).abs().max()) < 0.01
+
+
+def test_orthogonalize_strides(ops):
+    gen = seeded(41)
+    wide = update(gen, 3, 150, 210, "noise", "float32")
+    want = ops.orthogonalize(wide[:, :133, 3:100].contiguous())
+    assert torch.equal(ops.orthogonalize(wide[:, :133, 3:100]), want)
+    turned = wide[:, :133, 3:100].transpose(1, 2).contiguous().transpose(1, 2)
+    assert torch.equal(ops.orthogonalize(turned), want)
+    spread = torch.zeros(3, 266, 194, device="cuda")
+    spread[:, ::2, ::2] = wide[:, :133, 3:100]
+    assert torch.equal(ops.orthogonalize(spread[:, ::2, ::2]), want)
+    out = torch.zeros(3, 97, 140, device="cuda", dtype=torch.bfloat16)
+    ops.orthogonalize(wide[:, :133, 3:100], out=out[:, :, :133].transpose(1, 2))
+    assert torch.equal(out[:, :, :133].transpose(1, 2), want) and not out[:, :, 133:].any()
+    assert torch.equal(ops.orthogonalize(wide[1, :133, 3:100]), want[1])
+    # one matrix for all of a batch
+    same = ops.orthogonalize(wide[:1, :133, 3:100].expand(3, 133, 97))
+    assert torch.equal(same[2], want[0])
+
+
+def test_orthogonalize_zero_nan_and_scale(ops):
+    gen = seeded(42)
+    g = update(gen, 5, 140, 96, "noise", "float32")
+    clean = ops.orthogonalize(g)
+    g[1] = 0
+    g[2, 5, 7] = math.nan
+    g[3, 0, 0] = math.inf
+    y = ops.orthogonalize(g)
+    assert not y[1].any() and torch.isnan(y[2]).any() and torch.isnan(y[3]).any()
+    assert torch.equal(y[0], clean[0]) and torch.equal(y[4], clean[4])
+    for big in (1e30, 1e-25):  # squares out of the range of 32 bits
+        z = ops.orthogonalize(g[:1] * big, eps=0.0)
+        check_orthogonal(z, orthogonal64(g[:1] * big, 5, [ops.NEWTON_SCHULZ] * 5, 0.0), 5, "bfloat16")
+
+
+def test_orthogonalize_given_workspace_and_repeats(ops):
+    gen = seeded(43)
+    g = update(gen, 2, 257, 640, "decay", "bfloat16")
+    first = ops.orthogonalize(g)
+    n = ops.orthogonalize_workspace(2, 257, 640)
+    ws = torch.full((n,), 255, dtype=torch.uint8, device="cuda")
+    out = torch.empty_like(first)
+    for _ in range(2):
+        ops.orthogonalize(g, out=out, workspace=ws)
+        assert torch.equal(out, first)
+    assert ops.orthogonalize(g[:0]).shape == (0, 257, 640)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        held = ops.orthogonalize(g)
+    graph.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(held, first)

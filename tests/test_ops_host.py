@@ -234,3 +234,27 @@ def test_c_entries_refuse():
     refused(logp(top=11), b"alternatives")
     refused(logp(stats=None), b"null or unaligned")
     assert logp(rows=0) == 0
+
+
+@pytest.mark.parametrize("kw,error,text", [
+    (dict(g=arr((4, 8), "int64")), TypeError, "g"),
+    (dict(g=arr((8,))), ValueError, "expected"),
+    (dict(steps=33), ValueError, "steps"),
+    (dict(coefficients=[(1.0, 2.0, 3.0)] * 4), ValueError, "coefficients"),
+    (dict(coefficients=[(1.0, 2.0)] * 5), ValueError, "coefficients"),
+    (dict(out=arr((4, 9))), ValueError, "out"),
+    (dict(out=arr((4, 8), strides=(0, 1))), ValueError, "share memory"),
+    (dict(out=None), ValueError, "have to be given"),
+    (dict(workspace=None), ValueError, "have to be given"),
+    (dict(workspace=arr((4,))), rt.ADError, "bytes of workspace"),
+    (dict(workspace=arr((1 << 20,), ptr=4100)), rt.ADError, "256-byte aligned"),
+    (dict(coefficients=(50.0, 0.0, 0.0)), rt.ADError, "past 1024"),
+    (dict(coefficients=(math.nan, 0.0, 0.0)), rt.ADError, "not a number"),
+    (dict(eps=-1.0), rt.ADError, "eps"),
+    (dict(g=arr((4, 70000)), out=arr((4, 70000))), rt.ADError, "at most"),
+])
+def test_orthogonalize_refuses(kw, error, text):
+    a = dict(g=arr((4, 8)), out=arr((4, 8), "bfloat16"), workspace=arr((1 << 20,)))
+    a.update(kw)
+    with pytest.raises(error, match=text):
+        ops.orthogonalize(**a)

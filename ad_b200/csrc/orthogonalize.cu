@@ -18,10 +18,20 @@
 // epilogues.  The result is then within about 1e-3 (norm-wise) of the exact
 // iteration, rank-one matrices included.
 //
-// Operands are K-major tiles brought by TMA: rows of X for X X^T, rows of the
-// symmetric A for A A, rows of B and of X^T for B X.  The last product's
-// epilogue writes X both ways; with a row of the accumulator to each lane the
-// transposed store is the coalesced one.
+// One kernel makes all products.  Its blocks (or pairs of blocks, whose tensor
+// cores share a tile of 256 x 256) stay resident and take every so-many-th tile
+// of one list: the steps in order, in a step the three products, in a product
+// the matrices.  A tile waits only for the previous product of its own matrix, by
+// a counter in memory, so that a batch leaves no gaps between products.  Within
+// a block one warp brings operands by TMA, one issues the products into one of
+// two accumulators, eight work on the other: read it from tensor memory,
+// apply the epilogue, write.  A and B are symmetric: tiles on one side of the
+// diagonal are computed and written twice.
+//
+// Operands: rows of X for X X^T and of the symmetric A for A A, K-major; for
+// B X the rows of B, K-major, and X itself as it lies, N-major.  X is held as
+// the sum of two f16 numbers, the larger of which is the operand: X crosses the
+// bus as 2 + 2 bytes in each direction.
 #include <cuda.h>
 
 #include <cmath>
@@ -33,34 +43,58 @@ namespace {
 
 using namespace adops;
 
-constexpr int BM = 128, BK = 64;  // tile rows; elements of K a stage (128 bytes, the swizzle's width)
-constexpr int STAGES = 4;
+constexpr int BK = 64;  // elements of K a stage: 128 bytes, the swizzle's width
+constexpr int BOX = 64 * BK * 2;  // bytes of a TMA box: 64 rows
+constexpr int EPI_WARPS = 8;
+constexpr int THREADS = 64 + 32 * EPI_WARPS;
 constexpr int MAX_STEPS = 32;
 constexpr int NORM_BLOCKS = 64;  // blocks that share a matrix's norm
 
-enum Mode { GRAM = 0, POLY = 1, UPDATE = 2 };
+enum Phase { GRAM = 0, POLY = 1, UPDATE = 2 };
 
-struct Step {  // one product's epilogue
-  int m, n;        // of X
-  int ldx, ldt, lda;  // rows of X, of X^T, of A and B (elements)
-  float scale;     // GRAM: of the accumulator; POLY, UPDATE: see the epilogue
-  float p, q;
-  __half *a, *b, *xh, *xt_next;  // X^T is an operand of the product that replaces it: two of them
-  float *xf, *da, *db;
-  void* out;       // UPDATE: the result, when this is the last step
-  int out_type;
+// Tiles: CTAS blocks work on one of 128 CTAS rows and BN columns.
+template <int CTAS, int BN>
+struct Tile {
+  static constexpr int M = 128 * CTAS, N = BN;
+  static constexpr int QN = BN / CTAS;  // columns whose operand a block holds
+  static constexpr int P_BYTES = 128 * BK * 2, Q_BYTES = QN * BK * 2, STAGE = P_BYTES + Q_BYTES;
+  static constexpr int STAGES = 192 * 1024 / STAGE;
+  static constexpr int SMEM = STAGES * STAGE + 1024 + 512;
+  static constexpr int RATIO = M / N;  // column tiles beside a row tile on the diagonal
+};
+
+struct StepScale {
+  float gram, poly_p, poly_q, up_p, up_q;
+};
+
+struct NsArgs {
+  int count, m, n, steps;
+  int ldx, lda;       // rows of X, and of A and B (elements)
+  int sym, up;        // tiles of a matrix in GRAM and POLY, in UPDATE
+  int row_tiles, sym_cols;
+  __half *hi[2], *lo, *a, *b;
+  float *da, *db;
+  void* out;
+  int out_type, out_vec;
   long long out_batch, out_row, out_col;
   float out_scale;
   int* err;
+  unsigned* ready;  // a matrix's finished tiles (counted once a block)
+  StepScale step[MAX_STEPS];
 };
 
 __device__ __forceinline__ unsigned smem_u32(const void* p) {
   return static_cast<unsigned>(__cvta_generic_to_shared(p));
 }
+__device__ __forceinline__ unsigned in_block(unsigned addr, unsigned rank) {
+  unsigned r;
+  asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(addr), "r"(rank));
+  return r;
+}
 __device__ __forceinline__ bool bar_try(unsigned long long* b, unsigned phase) {
   unsigned ok;
   asm volatile(
-      "{\n .reg .pred p;\n mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n"
+      "{\n .reg .pred p;\n mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n"
       " selp.u32 %0, 1, 0, p;\n}"
       : "=r"(ok)
       : "r"(smem_u32(b)), "r"(phase)
@@ -72,21 +106,44 @@ __device__ __forceinline__ unsigned long long now() {
   asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(t));
   return t;
 }
-// Bounded wait (2 s): false when the phase never completed.
-__device__ __noinline__ bool bar_wait(unsigned long long* b, unsigned phase) {
-  if (bar_try(b, phase)) return true;
+constexpr unsigned long long PATIENCE = 2000000000ull;  // every wait ends after 2 s
+
+// False when the phase never completed, or at once when another role gave up.
+__device__ __noinline__ bool bar_wait_slow(unsigned long long* b, unsigned phase, volatile int* gave_up) {
   const unsigned long long t0 = now();
   while (true) {
-    for (int i = 0; i < 256; ++i)
+    for (int i = 0; i < 64; ++i)
       if (bar_try(b, phase)) return true;
-    if (now() - t0 > 2000000000ull) return false;
+    if (*gave_up || now() - t0 > PATIENCE) return false;
   }
 }
-// K-major tile with 128-byte rows, 128-byte swizzle.
-__device__ __forceinline__ unsigned long long tile_desc(const void* p) {
-  const unsigned long long a = (smem_u32(p) >> 4) & 0x3FFFull;
-  return a | (1ull << 16) | ((1024ull >> 4) << 32) | (1ull << 46) | (2ull << 61);
+__device__ __forceinline__ bool bar_wait(unsigned long long* b, unsigned phase, volatile int* gave_up) {
+  return bar_try(b, phase) || bar_wait_slow(b, phase, gave_up);
 }
+__device__ __forceinline__ unsigned load_acquire(const unsigned* p) {
+  unsigned v;
+  asm volatile("ld.acquire.gpu.global.u32 %0, [%1];" : "=r"(v) : "l"(p) : "memory");
+  return v;
+}
+__device__ __noinline__ bool count_wait(const unsigned* p, unsigned need, volatile int* gave_up) {
+  const unsigned long long t0 = now();
+  while (load_acquire(p) < need) {
+    if (*gave_up || now() - t0 > PATIENCE) return false;
+  }
+  return true;
+}
+
+// Shared-memory descriptors, 128-byte swizzle.  K-major: 8 rows of 128 bytes
+// make a group.  N-major: 64 columns to a row of 128 bytes, a row for each k;
+// the next 64 columns lie a box further.
+__device__ __forceinline__ unsigned long long desc_k(const void* p) {
+  return ((smem_u32(p) >> 4) & 0x3FFFull) | (1ull << 16) | ((1024ull >> 4) << 32) | (1ull << 46) | (2ull << 61);
+}
+__device__ __forceinline__ unsigned long long desc_n(const void* p) {
+  return ((smem_u32(p) >> 4) & 0x3FFFull) | ((static_cast<unsigned long long>(BOX) >> 4) << 16) |
+         ((1024ull >> 4) << 32) | (1ull << 46) | (2ull << 61);
+}
+
 __device__ __forceinline__ void tmem_ld32(unsigned taddr, unsigned (&r)[32]) {
   asm volatile(
       "tcgen05.ld.sync.aligned.32x32b.x32.b32 "
@@ -97,245 +154,429 @@ __device__ __forceinline__ void tmem_ld32(unsigned taddr, unsigned (&r)[32]) {
         "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]),
         "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
       : "r"(taddr));
-  asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
 }
 
-// 32 values of a row: 16 bytes at a time where all are inside.
-__device__ __forceinline__ void store_half32(__half* p, const float (&v)[32], int inside) {
-  if (inside >= 32) {
+// 32 elements of a row as eight 8-byte words a half; words past the end are
+// zero.  From L2: other multiprocessors wrote them.
+struct Row32 {
+  uint4 q[4];
+};
+__device__ __forceinline__ Row32 load_row32(const __half* p, int inside) {
+  Row32 r;
 #pragma unroll
-    for (int k = 0; k < 32; k += 8) {
+  for (int k = 0; k < 4; ++k)
+    r.q[k] = 8 * k < inside ? __ldcg(reinterpret_cast<const uint4*>(p) + k) : make_uint4(0, 0, 0, 0);
+  return r;
+}
+__device__ __forceinline__ float2 pair_of(const Row32& r, int i) {  // elements 2 i, 2 i + 1
+  const uint4 q = r.q[i / 4];
+  const unsigned w = i % 4 == 0 ? q.x : i % 4 == 1 ? q.y : i % 4 == 2 ? q.z : q.w;
+  return __half22float2(*reinterpret_cast<const __half2*>(&w));
+}
+__device__ __forceinline__ void store_half32(__half* p, const float (&v)[32], int inside) {
+#pragma unroll
+  for (int k = 0; k < 32; k += 8) {
+    if (k + 8 <= inside) {
       Vec<__half, 8> w;
 #pragma unroll
       for (int j = 0; j < 8; ++j) w.v[j] = __float2half_rn(v[k + j]);
       store_vec<__half, 8>(p + k, w);
+    } else {
+#pragma unroll
+      for (int j = 0; j < 8; ++j)
+        if (k + j < inside) p[k + j] = __float2half_rn(v[k + j]);
+    }
+  }
+}
+// The same elements as a column of the transposed matrix: lanes hold adjacent rows.
+__device__ __forceinline__ void store_turned32(__half* p, long long ld, const float (&v)[32], int inside) {
+#pragma unroll
+  for (int j = 0; j < 32; ++j)
+    if (j < inside) p[j * ld] = __float2half_rn(v[j]);
+}
+
+// Part of a row of the result.
+__device__ __forceinline__ void store_result(const NsArgs& a, long long mat, int row, int col0, float (&v)[32], int inside) {
+  const long long at = mat * a.out_batch + row * a.out_row + col0 * a.out_col;
+#pragma unroll
+  for (int j = 0; j < 32; ++j) v[j] *= a.out_scale;
+  if (a.out_vec && inside >= 32) {
+#pragma unroll
+    for (int k = 0; k < 32; k += 8) {
+      if (a.out_type == AD_F32) {
+        float* p = static_cast<float*>(a.out) + at + k;
+        store_vec<float, 4>(p, {{v[k], v[k + 1], v[k + 2], v[k + 3]}});
+        store_vec<float, 4>(p + 4, {{v[k + 4], v[k + 5], v[k + 6], v[k + 7]}});
+      } else if (a.out_type == AD_BF16) {
+        Vec<__nv_bfloat16, 8> w;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) w.v[j] = from_float<__nv_bfloat16>(v[k + j]);
+        store_vec<__nv_bfloat16, 8>(static_cast<__nv_bfloat16*>(a.out) + at + k, w);
+      } else {
+        Vec<__half, 8> w;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) w.v[j] = from_float<__half>(v[k + j]);
+        store_vec<__half, 8>(static_cast<__half*>(a.out) + at + k, w);
+      }
     }
   } else {
 #pragma unroll
     for (int j = 0; j < 32; ++j)
-      if (j < inside) p[j] = __float2half_rn(v[j]);
+      if (j < inside) store_any(a.out, a.out_type, at + j * a.out_col, v[j]);
   }
 }
 
-template <int MODE>
-__device__ __forceinline__ void epilogue32(const Step& s, long long mat, int row, int col0, const unsigned (&acc)[32]) {
-  const int width = MODE == UPDATE ? s.n : s.m;
-  const int inside = row < s.m ? width - col0 : 0;
-  float v[32];
-  if (MODE == GRAM) {
-    if (inside <= 0) return;
-#pragma unroll
-    for (int j = 0; j < 32; ++j) {
-      v[j] = __uint_as_float(acc[j]) * s.scale;
-      if (col0 + j == row) {
-        s.da[mat * s.m + row] = v[j];
-        v[j] = 0.0f;
-      }
+// One item of the list.
+struct Item {
+  int step, phase, mat, row, col;  // row, col: of tiles
+};
+template <typename TILE>
+__device__ __forceinline__ Item item_of(const NsArgs& a, int t) {
+  Item i;
+  const int sym_all = a.count * a.sym, per_step = 2 * sym_all + a.count * a.up;
+  i.step = t / per_step;
+  int r = t - i.step * per_step;
+  if (r < 2 * sym_all) {
+    i.phase = r >= sym_all ? POLY : GRAM;
+    r -= i.phase * sym_all;
+    i.mat = r / a.sym;
+    r -= i.mat * a.sym;
+    for (i.row = 0;; ++i.row) {
+      const int n = min((i.row + 1) * TILE::RATIO, a.sym_cols);
+      if (r < n) break;
+      r -= n;
     }
-    store_half32(s.a + (mat * s.m + row) * s.lda + col0, v, inside);
-  } else if (MODE == POLY) {
-    // B = p A + q (A_o A_o + (d_row + d_col) A_o), A_o without its diagonal d
-    if (inside <= 0) return;
-    const __half* a = s.a + (mat * s.m + row) * s.lda + col0;
-    const float* d = s.da + mat * s.m;
-    const float dr = d[row];
-#pragma unroll
-    for (int k = 0; k < 32; k += 8) {
-      if (k >= inside) break;
-      const Vec<__half, 8> w = load_vec<__half, 8>(a + k);  // the row's padding is readable
-#pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        const int c = col0 + k + j;
-        const float ao = to_float(w.v[j]), dc = k + j < inside ? d[c] : 0.0f;
-        v[k + j] = s.p * ao + s.q * (__uint_as_float(acc[k + j]) + (dr + dc) * ao);
-        if (c == row) {
-          s.db[mat * s.m + row] = s.p * dr + s.q * (__uint_as_float(acc[k + j]) + dr * dr);
-          v[k + j] = 0.0f;
-        }
-      }
-    }
-    store_half32(s.b + (mat * s.m + row) * s.lda + col0, v, inside);
+    i.col = r;
   } else {
-    // X = p X + q (B_o X_h + d X_h)
-    const long long at = (mat * s.m + row) * s.ldx + col0;
-    const float d = inside > 0 ? s.db[mat * s.m + row] : 0.0f;
-#pragma unroll
-    for (int j = 0; j < 32; ++j) v[j] = 0.0f;
-#pragma unroll
-    for (int k = 0; k < 32; k += 4) {
-      if (k >= inside) break;
-      const Vec<float, 4> w = load_vec<float, 4>(s.xf + at + k);  // the row's padding is readable
-#pragma unroll
-      for (int j = 0; j < 4; ++j)
-        v[k + j] = s.p * w.v[j] + s.q * (__uint_as_float(acc[k + j]) + d * __half2float(__float2half_rn(w.v[j])));
-    }
-    if (s.out) {
-#pragma unroll
-      for (int j = 0; j < 32; ++j)
-        if (j < inside)
-          store_any(s.out, s.out_type, mat * s.out_batch + row * s.out_row + (col0 + j) * s.out_col, v[j] * s.out_scale);
-      return;
-    }
-    if (inside > 0) {
-#pragma unroll
-      for (int k = 0; k < 32; k += 4) {
-        if (k + 4 <= inside) {
-          Vec<float, 4> w;
-#pragma unroll
-          for (int j = 0; j < 4; ++j) w.v[j] = v[k + j];
-          store_vec<float, 4>(s.xf + at + k, w);
-        } else {
-#pragma unroll
-          for (int j = 0; j < 4; ++j)
-            if (k + j < inside) s.xf[at + k + j] = v[k + j];
-        }
-      }
-      store_half32(s.xh + at, v, inside);
-#pragma unroll
-      for (int j = 0; j < 32; ++j)
-        if (j < inside) s.xt_next[(mat * s.n + col0 + j) * s.ldt + row] = __float2half_rn(v[j]);
-    }
+    i.phase = UPDATE;
+    r -= 2 * sym_all;
+    i.mat = r / a.up;
+    r -= i.mat * a.up;
+    i.col = r / a.row_tiles;
+    i.row = r - i.col * a.row_tiles;
   }
+  return i;
 }
 
-template <int BN>
-constexpr int gemm_smem() {
-  return STAGES * (BM + BN) * BK * 2 + 1024 + 256;
-}
-
-// C = P Q^T over one tile: P [m rows][k], Q [n rows][k], both K-major.
-// tp, tq: maps over all matrices' rows; prow, qrow: rows of one matrix.
-template <int MODE, int BN>
-__global__ void __launch_bounds__(128, 1)
-    ns_gemm(const __grid_constant__ CUtensorMap tp, const __grid_constant__ CUtensorMap tq, int prow, int qrow,
-            int kblocks, const __grid_constant__ Step s) {
+template <int CTAS, int BN>
+__global__ void __launch_bounds__(THREADS, 1)
+    ns_kernel(const __grid_constant__ CUtensorMap tx0, const __grid_constant__ CUtensorMap tx1,
+              const __grid_constant__ CUtensorMap ta, const __grid_constant__ CUtensorMap tb,
+              const __grid_constant__ NsArgs a) {
+  using TILE = Tile<CTAS, BN>;
+  constexpr int STAGES = TILE::STAGES;
   extern __shared__ __align__(1024) unsigned char raw[];
   unsigned char* smem = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~uintptr_t(1023));
-  constexpr unsigned P_BYTES = BM * BK * 2, Q_BYTES = BN * BK * 2, STAGE = P_BYTES + Q_BYTES;
-  unsigned long long* full = reinterpret_cast<unsigned long long*>(smem + STAGES * STAGE);
+  unsigned long long* full = reinterpret_cast<unsigned long long*>(smem + STAGES * TILE::STAGE);
   unsigned long long* empty = full + STAGES;
-  unsigned long long* accb = empty + STAGES;
-  unsigned* tmem_slot = reinterpret_cast<unsigned*>(accb + 1);
-  volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
-  volatile int* consumed = abort_flag + 1;
+  unsigned long long* acc_full = empty + STAGES;
+  unsigned long long* acc_empty = acc_full + 2;
+  unsigned* tmem_slot = reinterpret_cast<unsigned*>(acc_empty + 2);
+  volatile int* gave_up = reinterpret_cast<volatile int*>(tmem_slot + 1);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int m0 = blockIdx.y * BM, n0 = blockIdx.x * BN;
-  const long long mat = blockIdx.z;
+  const int rank = CTAS == 1 ? 0 : blockIdx.x & 1;
+  const int first = blockIdx.x / CTAS, stride = gridDim.x / CTAS;
+  const int items = a.steps * a.count * (2 * a.sym + a.up);
 
   if (threadIdx.x == 0) {
     for (int i = 0; i < STAGES; ++i) {
       asm volatile("mbarrier.init.shared::cta.b64 [%0], 1;" ::"r"(smem_u32(&full[i])));
       asm volatile("mbarrier.init.shared::cta.b64 [%0], 1;" ::"r"(smem_u32(&empty[i])));
     }
-    asm volatile("mbarrier.init.shared::cta.b64 [%0], 1;" ::"r"(smem_u32(accb)));
-    *abort_flag = 0;
-    *consumed = 0;
+    for (int i = 0; i < 2; ++i) {
+      asm volatile("mbarrier.init.shared::cta.b64 [%0], 1;" ::"r"(smem_u32(&acc_full[i])));
+      asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(smem_u32(&acc_empty[i])), "r"(CTAS * EPI_WARPS));
+    }
+    *gave_up = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
   }
-  if (warp == 0) {
-    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)), "r"(BN)
-                 : "memory");
-    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+  if (warp == 1) {
+    if (CTAS == 1) {
+      asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)),
+                   "r"(2 * BN)
+                   : "memory");
+      asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    } else {
+      asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)),
+                   "r"(2 * BN)
+                   : "memory");
+      asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+    }
   }
   asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
   __syncthreads();
+  if (CTAS == 2) {
+    asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+    asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+  }
   asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
   const unsigned tmem = *tmem_slot;
 
-  if (warp == 0 && lane == 0) {
-    int issued = 0;
-    for (int kb = 0; kb < kblocks; ++kb) {
-      const int i = kb % STAGES;
-      if (kb >= STAGES && !bar_wait(&empty[i], ((kb / STAGES) - 1) & 1)) {
-        *abort_flag = 1;
-        atomicExch(s.err, 1);
-        break;
-      }
-      if (*abort_flag) break;
-      unsigned char* st = smem + i * STAGE;
-      asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(smem_u32(&full[i])), "r"(STAGE)
-                   : "memory");
-      asm volatile(
-          "cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], [%2];" ::"r"(
-              smem_u32(st)),
-          "l"(reinterpret_cast<unsigned long long>(&tp)), "r"(smem_u32(&full[i])), "r"(kb * BK),
-          "r"(static_cast<int>(mat * prow) + m0)
-          : "memory");
-      asm volatile(
-          "cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], [%2];" ::"r"(
-              smem_u32(st + P_BYTES)),
-          "l"(reinterpret_cast<unsigned long long>(&tq)), "r"(smem_u32(&full[i])), "r"(kb * BK),
-          "r"(static_cast<int>(mat * qrow) + n0)
-          : "memory");
-      issued = kb + 1;
-    }
-    if (*abort_flag)
-      for (int kb = *consumed; kb < issued; ++kb) bar_wait(&full[kb % STAGES], (kb / STAGES) & 1);
-  } else if (warp == 1 && lane == 0) {
-    // D f32, A and B f16, both K-major
-    constexpr unsigned IDESC = (1u << 4) | (static_cast<unsigned>(BN >> 3) << 17) | ((128u >> 4) << 24);
-    for (int kb = 0; kb < kblocks; ++kb) {
-      const int i = kb % STAGES;
-      if (!bar_wait(&full[i], (kb / STAGES) & 1)) {
-        *abort_flag = 1;
-        atomicExch(s.err, 2);
-        break;
-      }
-      if (*abort_flag) break;
-      asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-      unsigned char* st = smem + i * STAGE;
-      const unsigned long long pd = tile_desc(st), qd = tile_desc(st + P_BYTES);
+  if (warp == 0) {
+    if (lane == 0) {  // operands
+      int n = 0;      // stages used so far
+      for (int t = first; t < items; t += stride) {
+        const Item it = item_of<TILE>(a, t);
+        const unsigned need = static_cast<unsigned>(CTAS) *
+                              (it.step * (2 * a.sym + a.up) + (it.phase == GRAM ? 0 : it.phase == POLY ? a.sym : 2 * a.sym));
+        if (!count_wait(a.ready + it.mat, need, gave_up)) {
+          *gave_up = 1;
+          atomicExch(a.err, 1);
+          break;
+        }
+        // what others wrote through the generic proxy is read through the async one
+        asm volatile("fence.proxy.async;" ::: "memory");
+        const CUtensorMap* x = it.step & 1 ? &tx1 : &tx0;
+        const CUtensorMap* p = it.phase == GRAM ? x : it.phase == POLY ? &ta : &tb;
+        const CUtensorMap* q = it.phase == POLY ? &ta : x;
+        const int kblocks = ((it.phase == GRAM ? a.n : a.m) + BK - 1) / BK;
+        const int p0 = it.row * TILE::M + rank * 128;
+        const int q0 = it.col * BN + rank * TILE::QN;
+        bool stop = false;
+        for (int kb = 0; kb < kblocks; ++kb, ++n) {
+          const int i = n % STAGES;
+          if (n >= STAGES && !bar_wait(&empty[i], (n / STAGES - 1) & 1, gave_up)) {
+            *gave_up = 1;
+            atomicExch(a.err, 2);
+            stop = true;
+            break;
+          }
+          unsigned char* st = smem + i * TILE::STAGE;
+          unsigned bar = smem_u32(&full[i]);
+          if (rank == 0)
+            asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(CTAS * TILE::STAGE)
+                         : "memory");
+          if (CTAS == 2) bar = in_block(bar, 0);
+          auto load = [&](const CUtensorMap* map, unsigned char* to, int x0, int y0) {
+            if (CTAS == 1)
+              asm volatile(
+                  "cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], "
+                  "[%2];" ::"r"(smem_u32(to)),
+                  "l"(reinterpret_cast<unsigned long long>(map)), "r"(bar), "r"(x0), "r"(y0), "r"(it.mat)
+                  : "memory");
+            else
+              asm volatile(
+                  "cp.async.bulk.tensor.3d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], "
+                  "[%1, {%3, %4, %5}], [%2];" ::"r"(smem_u32(to)),
+                  "l"(reinterpret_cast<unsigned long long>(map)), "r"(bar), "r"(x0), "r"(y0), "r"(it.mat)
+                  : "memory");
+          };
+          load(p, st, kb * BK, p0);
+          load(p, st + BOX, kb * BK, p0 + 64);
+          unsigned char* sq = st + TILE::P_BYTES;
 #pragma unroll
-      for (int k = 0; k < BK / 16; ++k) {
-        const unsigned long long adv = static_cast<unsigned long long>(k * 32) >> 4;
-        const unsigned more = (kb > 0 || k > 0) ? 1u : 0u;
-        asm volatile(
-            "{\n .reg .pred p;\n setp.ne.u32 p, %4, 0;\n"
-            " tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}" ::"r"(tmem),
-            "l"(pd + adv), "l"(qd + adv), "r"(IDESC), "r"(more)
-            : "memory");
+          for (int h = 0; h < TILE::QN / 64; ++h) {
+            if (it.phase == UPDATE)
+              load(q, sq + h * BOX, q0 + h * 64, kb * BK);
+            else
+              load(q, sq + h * BOX, kb * BK, q0 + h * 64);
+          }
+        }
+        if (stop) break;
       }
-      asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(
-                       smem_u32(&empty[i]))
-                   : "memory");
-      *consumed = kb + 1;
     }
-    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_u32(accb))
-                 : "memory");
+  } else if (warp == 1) {
+    if (lane == 0 && rank == 0) {  // products
+      // D f32, operands f16; bit 16: the right operand is N-major
+      constexpr unsigned IDESC =
+          (1u << 4) | (static_cast<unsigned>(BN >> 3) << 17) | (static_cast<unsigned>(TILE::M >> 4) << 24);
+      int n = 0, c = 0;  // stages, accumulators used so far
+      for (int t = first; t < items; t += stride, ++c) {
+        const Item it = item_of<TILE>(a, t);
+        const int kblocks = ((it.phase == GRAM ? a.n : a.m) + BK - 1) / BK;
+        if (c >= 2 && !bar_wait(&acc_empty[c & 1], (c / 2 - 1) & 1, gave_up)) {
+          *gave_up = 1;
+          atomicExch(a.err, 3);
+          break;
+        }
+        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+        const unsigned acc = tmem + (c & 1) * BN;
+        const unsigned idesc = IDESC | (it.phase == UPDATE ? 1u << 16 : 0u);
+        const unsigned long long q_step = it.phase == UPDATE ? (16 * 128) >> 4 : 32 >> 4;
+        bool stop = false;
+        for (int kb = 0; kb < kblocks; ++kb, ++n) {
+          const int i = n % STAGES;
+          if (!bar_wait(&full[i], (n / STAGES) & 1, gave_up)) {
+            *gave_up = 1;
+            atomicExch(a.err, 4);
+            stop = true;
+            break;
+          }
+          asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+          unsigned char* st = smem + i * TILE::STAGE;
+          const unsigned long long pd = desc_k(st);
+          const unsigned long long qd = it.phase == UPDATE ? desc_n(st + TILE::P_BYTES) : desc_k(st + TILE::P_BYTES);
+#pragma unroll
+          for (int k = 0; k < BK / 16; ++k) {
+            const unsigned more = (kb > 0 || k > 0) ? 1u : 0u;
+            if (CTAS == 1)
+              asm volatile(
+                  "{\n .reg .pred p;\n setp.ne.u32 p, %4, 0;\n"
+                  " tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}" ::"r"(acc),
+                  "l"(pd + k * (32 >> 4)), "l"(qd + k * q_step), "r"(idesc), "r"(more)
+                  : "memory");
+            else
+              asm volatile(
+                  "{\n .reg .pred p;\n setp.ne.u32 p, %4, 0;\n"
+                  " tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n}" ::"r"(acc),
+                  "l"(pd + k * (32 >> 4)), "l"(qd + k * q_step), "r"(idesc), "r"(more)
+                  : "memory");
+          }
+          auto commit = [&](unsigned long long* bar) {
+            if (CTAS == 1)
+              asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(
+                               smem_u32(bar))
+                           : "memory");
+            else
+              asm volatile(
+                  "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], "
+                  "%1;" ::"r"(smem_u32(bar)),
+                  "h"(static_cast<unsigned short>(3))
+                  : "memory");
+          };
+          commit(&empty[i]);
+          if (kb + 1 == kblocks) commit(&acc_full[c & 1]);
+        }
+        if (stop) break;
+      }
+    }
+  } else {  // epilogues
+    const int quad = warp & 3, part = (warp - 2) >> 2;
+    constexpr int CHUNKS = BN / 64;  // of 32 columns, a warp's share
+    int c = 0;
+    bool dead = false;  // a wait ran out: the rest of the list is walked without work, the result shows it
+    for (int t = first; t < items; t += stride, ++c) {
+      const Item it = item_of<TILE>(a, t);
+      const int row = it.row * TILE::M + rank * 128 + quad * 32 + lane;
+      const int col_first = it.col * BN + part * (BN / 2);
+      const int width = it.phase == UPDATE ? a.n : a.m;
+      const bool row_in = row < a.m;
+      const long long row_all = static_cast<long long>(it.mat) * a.m + row;
+      const __half* hi_in = a.hi[it.step & 1];
+      __half* hi_out = a.hi[(it.step + 1) & 1];
+      const StepScale sc = a.step[it.step];
+      if (!dead && !bar_wait(&acc_full[c & 1], (c / 2) & 1, gave_up)) {
+        *gave_up = 1;
+        atomicExch(a.err, 5);
+        dead = true;
+      }
+      asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+      const bool last = it.phase == UPDATE && it.step + 1 == a.steps;
+      const bool mirror = it.phase != UPDATE && it.col / TILE::RATIO != it.row;
+      const float d = !row_in ? 0.0f
+                      : it.phase == POLY ? __ldcg(a.da + row_all)
+                      : it.phase == UPDATE ? __ldcg(a.db + row_all) : 0.0f;
+      for (int ch = 0; ch < CHUNKS; ++ch) {
+        const int col0 = col_first + ch * 32;
+        const int inside = row_in ? width - col0 : 0;
+        unsigned acc[32];
+        tmem_ld32(tmem + (static_cast<unsigned>(quad * 32) << 16) + (c & 1) * BN + part * (BN / 2) + ch * 32, acc);
+        float v[32];
+        if (dead) {
+          asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+#pragma unroll
+          for (int j = 0; j < 32; ++j) v[j] = __int_as_float(0x7fffffff);
+          if (last && inside > 0) store_result(a, it.mat, row, col0, v, inside);
+        } else if (it.phase == GRAM) {
+          asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+#pragma unroll
+          for (int j = 0; j < 32; ++j) {
+            v[j] = __uint_as_float(acc[j]) * sc.gram;
+            if (col0 + j == row && inside > 0) {
+              a.da[row_all] = v[j];
+              v[j] = 0.0f;
+            }
+          }
+          if (inside > 0) {
+            store_half32(a.a + row_all * a.lda + col0, v, inside);
+            if (mirror) store_turned32(a.a + (static_cast<long long>(it.mat) * a.m + col0) * a.lda + row, a.lda, v, inside);
+          }
+        } else if (it.phase == POLY) {
+          // B = p A + q (A_o A_o + (d_row + d_col) A_o), A_o without its diagonal d
+          const Row32 ao = load_row32(a.a + row_all * a.lda + col0, inside);
+          const float* dc = a.da + static_cast<long long>(it.mat) * a.m + col0;
+          const float mine = col0 + lane < a.m ? __ldcg(dc + lane) : 0.0f;  // lane j holds column j's
+          asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+#pragma unroll
+          for (int j = 0; j < 32; ++j) {
+            const float2 w = pair_of(ao, j / 2);
+            const float x = j & 1 ? w.y : w.x, s = __uint_as_float(acc[j]);
+            v[j] = sc.poly_p * x + sc.poly_q * (s + (d + __shfl_sync(0xffffffffu, mine, j)) * x);
+            if (col0 + j == row && inside > 0) {
+              a.db[row_all] = sc.poly_p * d + sc.poly_q * (s + d * d);
+              v[j] = 0.0f;
+            }
+          }
+          if (inside > 0) {
+            store_half32(a.b + row_all * a.lda + col0, v, inside);
+            if (mirror) store_turned32(a.b + (static_cast<long long>(it.mat) * a.m + col0) * a.lda + row, a.lda, v, inside);
+          }
+        } else {
+          // X = p X + q (B_o X_hi + d X_hi)
+          const Row32 h = load_row32(hi_in + row_all * a.ldx + col0, inside);
+          const Row32 l = load_row32(a.lo + row_all * a.ldx + col0, inside);
+          asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+#pragma unroll
+          for (int j = 0; j < 32; j += 2) {
+            const float2 x = pair_of(h, j / 2), y = pair_of(l, j / 2);
+            v[j] = sc.up_p * (x.x + y.x) + sc.up_q * (__uint_as_float(acc[j]) + d * x.x);
+            v[j + 1] = sc.up_p * (x.y + y.y) + sc.up_q * (__uint_as_float(acc[j + 1]) + d * x.y);
+          }
+          if (inside > 0 && last) {
+            store_result(a, it.mat, row, col0, v, inside);
+          } else if (inside > 0) {
+            store_half32(hi_out + row_all * a.ldx + col0, v, inside);
+#pragma unroll
+            for (int j = 0; j < 32; ++j) v[j] -= __half2float(__float2half_rn(v[j]));
+            store_half32(a.lo + row_all * a.ldx + col0, v, inside);
+          }
+        }
+      }
+      // the accumulator is free, and what was written is there for other blocks' copies
+      asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+      __threadfence();
+      asm volatile("fence.proxy.async;" ::: "memory");
+      __syncwarp();
+      if (lane == 0 && !dead) {
+        const unsigned bar = CTAS == 1 ? smem_u32(&acc_empty[c & 1]) : in_block(smem_u32(&acc_empty[c & 1]), 0);
+        asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
+      }
+      asm volatile("bar.sync 1, %0;" ::"n"(32 * EPI_WARPS) : "memory");
+      if (warp == 2 && lane == 0 && !dead)
+        asm volatile("red.release.gpu.global.add.u32 [%0], 1;" ::"l"(a.ready + it.mat) : "memory");
+    }
   }
   __syncwarp();
-
-  const bool ok = bar_wait(accb, 0);
-  if (!ok) atomicExch(s.err, 3);
-  asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+  // A role that gave up leaves copies and products in flight: let them land
+  // before shared and tensor memory are given back.
   __syncthreads();
-  const bool good = ok && !*abort_flag && *reinterpret_cast<volatile int*>(s.err) == 0;
-  const int row = m0 + warp * 32 + lane;
-  for (int c = 0; c < BN / 32; ++c) {
-    unsigned r[32];
-    tmem_ld32(tmem + (static_cast<unsigned>(warp * 32) << 16) + static_cast<unsigned>(c * 32), r);
-    if (!good) {  // a wait ran out: the result shows it
-#pragma unroll
-      for (int j = 0; j < 32; ++j) r[j] = 0x7fffffffu;
+  if (*gave_up) {
+    const unsigned long long t0 = now();
+    while (now() - t0 < 5000000ull) {
     }
-    epilogue32<MODE>(s, mat, row, n0 + c * 32, r);
   }
-  asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
-  __syncthreads();
-  if (warp == 0)
-    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(BN) : "memory");
+  if (CTAS == 2) {
+    asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+    asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+  }
+  asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+  if (warp == 1) {
+    if (CTAS == 1)
+      asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(2 * BN) : "memory");
+    else
+      asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(2 * BN) : "memory");
+  }
 }
 
 struct LoadArgs {
   const void* g;
   int type;
   long long batch, row, col;  // strides of G seen as m x n
-  int m, n, ldx, ldt;
+  int m, n, ldx;
   float eps, scale;
   double* part;
-  __half *xh, *xt;
-  float* xf;
+  __half *hi, *lo;
 };
 
 // A share of a matrix's sum of squares, in 64 bits: no scale of the update overflows.
@@ -361,7 +602,7 @@ __global__ void __launch_bounds__(256) ns_norm(const __grid_constant__ LoadArgs 
   }
 }
 
-// X = G scale / (|G| + eps), in 32 bits, as operand, and transposed as operand.
+// X = G scale / (|G| + eps) as the sum of two f16 numbers.
 __global__ void __launch_bounds__(256) ns_load(const __grid_constant__ LoadArgs a) {
   __shared__ float t[32][33];
   const long long mat = blockIdx.z;
@@ -379,44 +620,45 @@ __global__ void __launch_bounds__(256) ns_load(const __grid_constant__ LoadArgs 
   for (int k = ty; k < 32; k += 8) {
     if (r0 + k < a.m && c0 + tx < a.n) {
       const long long at = (mat * a.m + r0 + k) * a.ldx + c0 + tx;
-      a.xf[at] = t[k][tx];
-      a.xh[at] = __float2half_rn(t[k][tx]);
+      const __half h = __float2half_rn(t[k][tx]);
+      a.hi[at] = h;
+      a.lo[at] = __float2half_rn(t[k][tx] - __half2float(h));
     }
-    if (c0 + k < a.n && r0 + tx < a.m) a.xt[(mat * a.n + c0 + k) * a.ldt + r0 + tx] = __float2half_rn(t[tx][k]);
   }
 }
 
 // No steps: the normalised matrix itself.
-__global__ void ns_copy(const __grid_constant__ Step s) {
+__global__ void ns_copy(const __grid_constant__ NsArgs s) {
   const long long mat = blockIdx.y;
   const long long n = static_cast<long long>(s.m) * s.n;
   for (long long i = blockIdx.x * 256ll + threadIdx.x; i < n; i += gridDim.x * 256ll) {
     const int r = static_cast<int>(i / s.n), c = static_cast<int>(i - static_cast<long long>(r) * s.n);
+    const long long at = (mat * s.m + r) * s.ldx + c;
     store_any(s.out, s.out_type, mat * s.out_batch + r * s.out_row + c * s.out_col,
-              s.xf[(mat * s.m + r) * s.ldx + c] * s.out_scale);
+              (__half2float(s.hi[0][at]) + __half2float(s.lo[at])) * s.out_scale);
   }
 }
 
 struct Layout {
-  long long m, n, ldx, ldt, lda;
-  size_t part, xf, xh, xt[2], a, b, da, db, total;
+  long long m, n, ldx, lda;
+  size_t head, part, hi[2], lo, a, b, da, db, total;
 };
 Layout plan(long long count, long long rows, long long cols) {
   Layout l;
   l.m = rows < cols ? rows : cols;
   l.n = rows < cols ? cols : rows;
   l.ldx = (l.n + 7) / 8 * 8;
-  l.ldt = l.lda = (l.m + 7) / 8 * 8;
-  size_t at = 256;  // the error word
+  l.lda = (l.m + 7) / 8 * 8;
+  size_t at = 0;
   auto take = [&](size_t bytes) {
     const size_t here = at;
     at += (bytes + 255) / 256 * 256;
     return here;
   };
+  l.head = take(256 + 4ull * count);  // the error word, then the counters: zeros at the start
   l.part = take(sizeof(double) * NORM_BLOCKS * count);
-  l.xf = take(4ull * count * l.m * l.ldx);
-  l.xh = take(2ull * count * l.m * l.ldx);
-  for (size_t& t : l.xt) t = take(2ull * count * l.n * l.ldt);
+  for (size_t& t : l.hi) t = take(2ull * count * l.m * l.ldx);
+  l.lo = take(2ull * count * l.m * l.ldx);
   l.a = take(2ull * count * l.m * l.lda);
   l.b = take(2ull * count * l.m * l.lda);
   l.da = take(4ull * count * l.m);
@@ -465,20 +707,58 @@ Scales scales_for(int steps, const float* coef) {
   return s;
 }
 
-template <int MODE, int BN>
-cudaError_t gemm(const CUtensorMap& tp, const CUtensorMap& tq, int prow, int qrow, int m, int n, int k, int count,
-                 const Step& s, cudaStream_t st) {
+// The list's tiles for one tile size, and its time in clocks as estimated from
+// the cost of 64 elements of K and of a wait for another block's tile: the work
+// shared by all blocks, or one matrix's products one after the other.
+struct Tiling {
+  long long sym, up;
+  int row_tiles, sym_cols;
+  double clocks;
+};
+template <typename TILE>
+Tiling tiling(long long count, long long m, long long n, int workers, double per_kblock) {
+  Tiling t;
+  t.row_tiles = static_cast<int>((m + TILE::M - 1) / TILE::M);
+  t.sym_cols = static_cast<int>((m + TILE::N - 1) / TILE::N);
+  t.sym = 0;
+  for (int i = 0; i < t.row_tiles; ++i) t.sym += std::min(static_cast<long long>(i + 1) * TILE::RATIO, static_cast<long long>(t.sym_cols));
+  t.up = t.row_tiles * ((n + TILE::N - 1) / TILE::N);
+  const double kn = static_cast<double>((n + BK - 1) / BK), km = static_cast<double>((m + BK - 1) / BK);
+  const double shared = per_kblock * count * (t.sym * (kn + km) + t.up * km) / workers;
+  auto rounds = [&](long long tiles) { return static_cast<double>((tiles + workers - 1) / workers); };
+  const double alone = per_kblock * (rounds(t.sym) * (kn + km) + rounds(t.up) * km) + 3 * 3500.0;
+  t.clocks = std::fmax(shared, alone);
+  return t;
+}
+
+template <int CTAS, int BN>
+cudaError_t start(const CUtensorMap (&maps)[4], NsArgs& a, const Tiling& t, int sms, int device, cudaStream_t st) {
+  using TILE = Tile<CTAS, BN>;
   static bool ready[64] = {};
-  int dev = 0;
-  cudaGetDevice(&dev);
-  if (dev < 0 || dev >= 64 || !ready[dev]) {
-    const cudaError_t e = cudaFuncSetAttribute(ns_gemm<MODE, BN>, cudaFuncAttributeMaxDynamicSharedMemorySize, gemm_smem<BN>());
+  if (device >= 64 || !ready[device]) {
+    const cudaError_t e =
+        cudaFuncSetAttribute(ns_kernel<CTAS, BN>, cudaFuncAttributeMaxDynamicSharedMemorySize, TILE::SMEM);
     if (e != cudaSuccess) return e;
-    if (dev >= 0 && dev < 64) ready[dev] = true;
+    if (device < 64) ready[device] = true;
   }
-  ns_gemm<MODE, BN><<<dim3((n + BN - 1) / BN, (m + BM - 1) / BM, count), 128, gemm_smem<BN>(), st>>>(
-      tp, tq, prow, qrow, (k + BK - 1) / BK, s);
-  return cudaGetLastError();
+  a.sym = static_cast<int>(t.sym), a.up = static_cast<int>(t.up);
+  a.row_tiles = t.row_tiles, a.sym_cols = t.sym_cols;
+  const long long most = a.count * std::max(t.sym, t.up);  // tiles of one product
+  const int workers = static_cast<int>(std::min<long long>(sms / CTAS, most));
+  cudaLaunchConfig_t c = {};
+  c.gridDim = dim3(workers * CTAS);
+  c.blockDim = dim3(THREADS);
+  c.dynamicSmemBytes = TILE::SMEM;
+  c.stream = st;
+  cudaLaunchAttribute at[2];
+  at[0].id = cudaLaunchAttributeCooperative;  // blocks wait for one another: all of them have to be resident
+  at[0].val.cooperative = 1;
+  at[1].id = cudaLaunchAttributeClusterDimension;
+  at[1].val.clusterDim.x = CTAS;
+  at[1].val.clusterDim.y = at[1].val.clusterDim.z = 1;
+  c.attrs = at;
+  c.numAttrs = CTAS == 1 ? 1 : 2;
+  return cudaLaunchKernelEx(&c, ns_kernel<CTAS, BN>, maps[0], maps[1], maps[2], maps[3], a);
 }
 
 }  // namespace
@@ -523,71 +803,62 @@ extern "C" int ad_orthogonalize(int device, int dtype, const void* g, int64_t co
   LoadArgs la = {};
   la.g = g, la.type = dtype;
   la.batch = batch_stride, la.row = tall ? col_stride : row_stride, la.col = tall ? row_stride : col_stride;
-  la.m = m, la.n = n, la.ldx = static_cast<int>(l.ldx), la.ldt = static_cast<int>(l.ldt);
+  la.m = m, la.n = n, la.ldx = static_cast<int>(l.ldx);
   la.eps = eps, la.scale = static_cast<float>(sc.x[0]);
   la.part = reinterpret_cast<double*>(w + l.part);
-  la.xf = reinterpret_cast<float*>(w + l.xf);
-  la.xh = reinterpret_cast<__half*>(w + l.xh);
-  la.xt = reinterpret_cast<__half*>(w + l.xt[0]);
-  cudaError_t e = cudaMemsetAsync(w, 0, 256, st);
+  la.hi = reinterpret_cast<__half*>(w + l.hi[0]);
+  la.lo = reinterpret_cast<__half*>(w + l.lo);
+  cudaError_t e = cudaMemsetAsync(w, 0, 256 + 4ull * count, st);
   if (e != cudaSuccess) return fail("ad_orthogonalize: %s", cudaGetErrorString(e));
   ns_norm<<<dim3(NORM_BLOCKS, num), 256, 0, st>>>(la);
   ns_load<<<dim3((n + 31) / 32, (m + 31) / 32, num), dim3(32, 8), 0, st>>>(la);
   e = cudaGetLastError();
   if (e != cudaSuccess) return fail("ad_orthogonalize: %s", cudaGetErrorString(e));
 
-  Step s = {};
-  s.m = m, s.n = n, s.ldx = la.ldx, s.ldt = la.ldt, s.lda = static_cast<int>(l.lda);
+  NsArgs s = {};
+  s.count = num, s.m = m, s.n = n, s.steps = steps;
+  s.ldx = la.ldx, s.lda = static_cast<int>(l.lda);
+  for (int k = 0; k < 2; ++k) s.hi[k] = reinterpret_cast<__half*>(w + l.hi[k]);
+  s.lo = la.lo;
   s.a = reinterpret_cast<__half*>(w + l.a);
   s.b = reinterpret_cast<__half*>(w + l.b);
-  s.xf = la.xf, s.xh = la.xh;
   s.da = reinterpret_cast<float*>(w + l.da);
   s.db = reinterpret_cast<float*>(w + l.db);
   s.err = reinterpret_cast<int*>(w);
-  s.out_type = out_dtype;
+  s.ready = reinterpret_cast<unsigned*>(w + 256);
+  s.out = out, s.out_type = out_dtype;
   s.out_batch = out_batch_stride;
   s.out_row = tall ? out_col_stride : out_row_stride, s.out_col = tall ? out_row_stride : out_col_stride;
+  s.out_scale = static_cast<float>(1.0 / sc.x[steps]);
+  const int per16 = 16 / elem_size(out_dtype);
+  s.out_vec = s.out_col == 1 && s.out_row % per16 == 0 && s.out_batch % per16 == 0 && aligned(out, 16);
   if (steps == 0) {
-    s.out = out;
-    s.out_scale = static_cast<float>(1.0 / sc.x[0]);
     ns_copy<<<dim3(256, num), 256, 0, st>>>(s);
     e = cudaGetLastError();
     if (e != cudaSuccess) return fail("ad_orthogonalize: %s", cudaGetErrorString(e));
     return 0;
   }
-  constexpr int BN = 128;
-  // maps of X, A, B as left operands (128 rows a box), X, A and X^T as right ones
-  alignas(64) CUtensorMap tx, ta, tb, txq, taq, tt[2];
-  struct {
-    CUtensorMap* map;
-    const void* base;
-    long long rows, cols, ld;
-    int box;
-  } const maps[7] = {{&tx, s.xh, count * m, n, l.ldx, BM},  {&ta, s.a, count * m, m, l.lda, BM},
-                     {&tb, s.b, count * m, m, l.lda, BM},   {&txq, s.xh, count * m, n, l.ldx, BN},
-                     {&taq, s.a, count * m, m, l.lda, BN},  {&tt[0], w + l.xt[0], count * n, m, l.ldt, BN},
-                     {&tt[1], w + l.xt[1], count * n, m, l.ldt, BN}};
-  for (const auto& t : maps)
-    if (ad_tmap_2d(reinterpret_cast<uint64_t>(t.base), t.rows, t.cols, 2ull * t.ld, t.box, BK, 2, 128, t.map)) return 1;
   for (int k = 0; k < steps; ++k) {
     const double a = coefficients[3 * k], b = coefficients[3 * k + 1], c = coefficients[3 * k + 2];
-    const double sx = sc.x[k], sa = sc.a[k], sb = sc.b[k];
-    s.scale = static_cast<float>(sa / (sx * sx));
-    e = gemm<GRAM, BN>(tx, txq, m, m, m, m, n, num, s, st);
-    if (e == cudaSuccess) {
-      s.p = static_cast<float>(b * sb / sa);
-      s.q = static_cast<float>(c * sb / (sa * sa));
-      e = gemm<POLY, BN>(ta, taq, m, m, m, m, m, num, s, st);
-    }
-    if (e == cudaSuccess) {
-      const double up = sc.x[k + 1] / sx;
-      s.p = static_cast<float>(a * up);
-      s.q = static_cast<float>(up / sb);
-      if (k + 1 == steps) s.out = out, s.out_scale = static_cast<float>(1.0 / sc.x[steps]);
-      s.xt_next = reinterpret_cast<__half*>(w + l.xt[(k + 1) & 1]);
-      e = gemm<UPDATE, BN>(tb, tt[k & 1], m, n, m, n, m, num, s, st);
-    }
-    if (e != cudaSuccess) return fail("ad_orthogonalize: %s", cudaGetErrorString(e));
+    const double sx = sc.x[k], sa = sc.a[k], sb = sc.b[k], up = sc.x[k + 1] / sx;
+    s.step[k] = {static_cast<float>(sa / (sx * sx)), static_cast<float>(b * sb / sa), static_cast<float>(c * sb / (sa * sa)),
+                 static_cast<float>(a * up), static_cast<float>(up / sb)};
   }
+  alignas(64) CUtensorMap maps[4];  // X twice, A, B
+  const void* const base[4] = {s.hi[0], s.hi[1], s.a, s.b};
+  for (int k = 0; k < 4; ++k)
+    if (ad_b200_internal::tmap_3d_16(base[k], count, m, k < 2 ? n : m, k < 2 ? l.ldx : l.lda, 64, BK, &maps[k])) return 1;
+
+  const int sms = sm_count(guard.device());
+  if (!sms) return fail("ad_orthogonalize: no device properties");
+  const Tiling big = tiling<Tile<2, 256>>(count, m, n, sms / 2, 512.0);
+  const Tiling mid = tiling<Tile<1, 128>>(count, m, n, sms, 307.0);
+  const Tiling small = tiling<Tile<1, 64>>(count, m, n, sms, 192.0);
+  const Tiling& best = big.clocks <= mid.clocks && big.clocks <= small.clocks ? big : mid.clocks <= small.clocks ? mid : small;
+  if (steps * count * (2 * best.sym + best.up) > 0x3fffffffll) return fail("ad_orthogonalize: too many tiles in one call");
+  e = &best == &big   ? start<2, 256>(maps, s, best, sms, guard.device(), st)
+      : &best == &mid ? start<1, 128>(maps, s, best, sms, guard.device(), st)
+                      : start<1, 64>(maps, s, best, sms, guard.device(), st);
+  if (e != cudaSuccess) return fail("ad_orthogonalize: %s", cudaGetErrorString(e));
   return 0;
 }

@@ -722,3 +722,13 @@ def test_orthogonalize_given_workspace_and_repeats(ops):
     graph.replay()
     torch.cuda.synchronize()
     assert torch.equal(held, first)
+
+
+@pytest.mark.parametrize("count,rows,cols", [(6, 1024, 2048), (5, 2100, 1001), (74, 257, 300), (1, 2048, 2040),
+                                             (40, 300, 520)])
+def test_orthogonalize_large(ops, count, rows, cols):
+    """Sizes that each of the tilings is chosen for."""
+    gen = seeded(count, rows, cols)
+    g = update(gen, count, rows, cols, "decay", "float32")
+    g += 1e-5 * torch.randn(g.shape, device="cuda", generator=torch.Generator("cuda").manual_seed(1))
+    check_orthogonal(ops.orthogonalize(g), orthogonal64(g, 5, [ops.NEWTON_SCHULZ] * 5, 1e-7), 5, "bfloat16")

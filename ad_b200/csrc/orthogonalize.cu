@@ -24,9 +24,12 @@
 // the matrices.  A tile waits only for the previous product of its own matrix, by
 // a counter in memory, so that a batch leaves no gaps between products.  Within
 // a block one warp brings operands by TMA, one issues the products into one of
-// two accumulators, eight work on the other: read it from tensor memory,
-// apply the epilogue, write.  A and B are symmetric: tiles on one side of the
-// diagonal are computed and written twice.
+// two accumulators, eight work on the other: 64 columns at a time they join
+// the accumulator with what the epilogue needs of X or A, which a further warp
+// has brought into shared memory ahead of them, and leave the result in its
+// place, from where the last warp sends it off by TMA (lanes hold rows, so that
+// direct loads and stores would touch 32 lines each).  A and B are symmetric:
+// tiles on one side of the diagonal are computed and written twice.
 //
 // Operands: rows of X for X X^T and of the symmetric A for A A, K-major; for
 // B X the rows of B, K-major, and X itself as it lies, N-major.  X is held as
@@ -46,7 +49,9 @@ using namespace adops;
 constexpr int BK = 64;  // elements of K a stage: 128 bytes, the swizzle's width
 constexpr int BOX = 64 * BK * 2;  // bytes of a TMA box: 64 rows
 constexpr int EPI_WARPS = 8;
-constexpr int THREADS = 64 + 32 * EPI_WARPS;
+constexpr int LOADER = 2 + EPI_WARPS, STORER = LOADER + 1;  // warps that serve the epilogues
+constexpr int THREADS = 32 * (STORER + 1);
+constexpr int CHUNK = 2 * BOX;  // 128 rows of 64 columns of 16 bits
 constexpr int MAX_STEPS = 32;
 constexpr int NORM_BLOCKS = 64;  // blocks that share a matrix's norm
 
@@ -58,8 +63,8 @@ struct Tile {
   static constexpr int M = 128 * CTAS, N = BN;
   static constexpr int QN = BN / CTAS;  // columns whose operand a block holds
   static constexpr int P_BYTES = 128 * BK * 2, Q_BYTES = QN * BK * 2, STAGE = P_BYTES + Q_BYTES;
-  static constexpr int STAGES = 192 * 1024 / STAGE;
-  static constexpr int SMEM = STAGES * STAGE + 1024 + 512;
+  static constexpr int STAGES = 160 * 1024 / STAGE;
+  static constexpr int SMEM = STAGES * STAGE + 4 * CHUNK + 1024 + 512;
   static constexpr int RATIO = M / N;  // column tiles beside a row tile on the diagonal
 };
 
@@ -69,10 +74,10 @@ struct StepScale {
 
 struct NsArgs {
   int count, m, n, steps;
-  int ldx, lda;       // rows of X, and of A and B (elements)
+  int ldx;            // a row of X (elements)
   int sym, up;        // tiles of a matrix in GRAM and POLY, in UPDATE
   int row_tiles, sym_cols;
-  __half *hi[2], *lo, *a, *b;
+  __half *hi[2], *lo;
   float *da, *db;
   void* out;
   int out_type, out_vec;
@@ -156,43 +161,42 @@ __device__ __forceinline__ void tmem_ld32(unsigned taddr, unsigned (&r)[32]) {
       : "r"(taddr));
 }
 
-// 32 elements of a row as eight 8-byte words a half; words past the end are
-// zero.  From L2: other multiprocessors wrote them.
-struct Row32 {
-  uint4 q[4];
-};
-__device__ __forceinline__ Row32 load_row32(const __half* p, int inside) {
-  Row32 r;
-#pragma unroll
-  for (int k = 0; k < 4; ++k)
-    r.q[k] = 8 * k < inside ? __ldcg(reinterpret_cast<const uint4*>(p) + k) : make_uint4(0, 0, 0, 0);
-  return r;
+__device__ __forceinline__ uint4 lds128(unsigned addr) {
+  uint4 v;
+  asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(addr));
+  return v;
 }
-__device__ __forceinline__ float2 pair_of(const Row32& r, int i) {  // elements 2 i, 2 i + 1
-  const uint4 q = r.q[i / 4];
-  const unsigned w = i % 4 == 0 ? q.x : i % 4 == 1 ? q.y : i % 4 == 2 ? q.z : q.w;
-  return __half22float2(*reinterpret_cast<const __half2*>(&w));
+__device__ __forceinline__ void sts128(unsigned addr, uint4 v) {
+  asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" ::"r"(addr), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w) : "memory");
 }
-__device__ __forceinline__ void store_half32(__half* p, const float (&v)[32], int inside) {
-#pragma unroll
-  for (int k = 0; k < 32; k += 8) {
-    if (k + 8 <= inside) {
-      Vec<__half, 8> w;
-#pragma unroll
-      for (int j = 0; j < 8; ++j) w.v[j] = __float2half_rn(v[k + j]);
-      store_vec<__half, 8>(p + k, w);
-    } else {
-#pragma unroll
-      for (int j = 0; j < 8; ++j)
-        if (k + j < inside) p[k + j] = __float2half_rn(v[k + j]);
-    }
-  }
+__device__ __forceinline__ void sts16(unsigned addr, float v) {
+  asm volatile("st.shared.b16 [%0], %1;" ::"r"(addr), "h"(__half_as_ushort(__float2half_rn(v))) : "memory");
 }
-// The same elements as a column of the transposed matrix: lanes hold adjacent rows.
-__device__ __forceinline__ void store_turned32(__half* p, long long ld, const float (&v)[32], int inside) {
-#pragma unroll
-  for (int j = 0; j < 32; ++j)
-    if (j < inside) p[j * ld] = __float2half_rn(v[j]);
+__device__ __forceinline__ float2 halves(unsigned w) { return __half22float2(*reinterpret_cast<const __half2*>(&w)); }
+__device__ __forceinline__ unsigned packed(float a, float b) {
+  const __half2 h = __floats2half2_rn(a, b);
+  return *reinterpret_cast<const unsigned*>(&h);
+}
+
+// A box of 64 rows and 64 columns from or to a matrix.
+__device__ __forceinline__ void box_load(const CUtensorMap* map, unsigned to, unsigned bar, int col, int row, int mat) {
+  asm volatile(
+      "cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], [%2];" ::"r"(
+          to),
+      "l"(reinterpret_cast<unsigned long long>(map)), "r"(bar), "r"(col), "r"(row), "r"(mat)
+      : "memory");
+}
+__device__ __forceinline__ void box_store(const CUtensorMap* map, unsigned from, int col, int row, int mat) {
+  asm volatile("cp.async.bulk.tensor.3d.global.shared::cta.bulk_group [%0, {%2, %3, %4}], [%1];" ::"l"(
+                   reinterpret_cast<unsigned long long>(map)),
+               "r"(from), "r"(col), "r"(row), "r"(mat)
+               : "memory");
+}
+__device__ __forceinline__ void bar_expect(unsigned long long* bar, unsigned bytes) {
+  asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(smem_u32(bar)), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ void bar_arrive(unsigned long long* bar) {
+  asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(bar)) : "memory");
 }
 
 // Part of a row of the result.
@@ -258,20 +262,36 @@ __device__ __forceinline__ Item item_of(const NsArgs& a, int t) {
   return i;
 }
 
+// Chunks of 64 columns of an item's tile that are not wholly past the matrix.
+template <typename TILE>
+__device__ __forceinline__ int chunks_of(const NsArgs& a, const Item& i) {
+  const int width = (i.phase == UPDATE ? a.n : a.m) - i.col * TILE::N;
+  return min(TILE::N, width + 63) / 64;
+}
+// Tiles of its matrix that have to be finished before an item's operands are there.
+__device__ __forceinline__ unsigned needed(const NsArgs& a, const Item& i, int ctas) {
+  return static_cast<unsigned>(ctas) * (i.step * (2 * a.sym + a.up) + i.phase * a.sym);
+}
+
 template <int CTAS, int BN>
 __global__ void __launch_bounds__(THREADS, 1)
     ns_kernel(const __grid_constant__ CUtensorMap tx0, const __grid_constant__ CUtensorMap tx1,
-              const __grid_constant__ CUtensorMap ta, const __grid_constant__ CUtensorMap tb,
-              const __grid_constant__ NsArgs a) {
+              const __grid_constant__ CUtensorMap tl, const __grid_constant__ CUtensorMap ta,
+              const __grid_constant__ CUtensorMap tb, const __grid_constant__ NsArgs a) {
   using TILE = Tile<CTAS, BN>;
   constexpr int STAGES = TILE::STAGES;
   extern __shared__ __align__(1024) unsigned char raw[];
   unsigned char* smem = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~uintptr_t(1023));
-  unsigned long long* full = reinterpret_cast<unsigned long long*>(smem + STAGES * TILE::STAGE);
+  // two buffers of two chunks for the epilogues behind the operands' stages
+  unsigned char* side = smem + STAGES * TILE::STAGE;
+  unsigned long long* full = reinterpret_cast<unsigned long long*>(side + 4 * CHUNK);
   unsigned long long* empty = full + STAGES;
   unsigned long long* acc_full = empty + STAGES;
   unsigned long long* acc_empty = acc_full + 2;
-  unsigned* tmem_slot = reinterpret_cast<unsigned*>(acc_empty + 2);
+  unsigned long long* side_full = acc_empty + 2;   // a buffer holds what the epilogue needs
+  unsigned long long* side_done = side_full + 2;   // ... and then its results
+  unsigned long long* side_empty = side_done + 2;  // ... which are under way
+  unsigned* tmem_slot = reinterpret_cast<unsigned*>(side_empty + 2);
   volatile int* gave_up = reinterpret_cast<volatile int*>(tmem_slot + 1);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int rank = CTAS == 1 ? 0 : blockIdx.x & 1;
@@ -286,6 +306,9 @@ __global__ void __launch_bounds__(THREADS, 1)
     for (int i = 0; i < 2; ++i) {
       asm volatile("mbarrier.init.shared::cta.b64 [%0], 1;" ::"r"(smem_u32(&acc_full[i])));
       asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(smem_u32(&acc_empty[i])), "r"(CTAS * EPI_WARPS));
+      asm volatile("mbarrier.init.shared::cta.b64 [%0], 1;" ::"r"(smem_u32(&side_full[i])));
+      asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(smem_u32(&side_done[i])), "r"(EPI_WARPS));
+      asm volatile("mbarrier.init.shared::cta.b64 [%0], 1;" ::"r"(smem_u32(&side_empty[i])));
     }
     *gave_up = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -318,9 +341,7 @@ __global__ void __launch_bounds__(THREADS, 1)
       int n = 0;      // stages used so far
       for (int t = first; t < items; t += stride) {
         const Item it = item_of<TILE>(a, t);
-        const unsigned need = static_cast<unsigned>(CTAS) *
-                              (it.step * (2 * a.sym + a.up) + (it.phase == GRAM ? 0 : it.phase == POLY ? a.sym : 2 * a.sym));
-        if (!count_wait(a.ready + it.mat, need, gave_up)) {
+        if (!count_wait(a.ready + it.mat, needed(a, it, CTAS), gave_up)) {
           *gave_up = 1;
           atomicExch(a.err, 1);
           break;
@@ -441,110 +462,210 @@ __global__ void __launch_bounds__(THREADS, 1)
         if (stop) break;
       }
     }
-  } else {  // epilogues
-    const int quad = warp & 3, part = (warp - 2) >> 2;
-    constexpr int CHUNKS = BN / 64;  // of 32 columns, a warp's share
-    int c = 0;
+  } else if (warp < LOADER) {  // epilogues
+    const int quad = warp & 3, part = (warp - 2) >> 2;  // 32 rows, 32 columns of a chunk
+    const int r = quad * 32 + lane;
+    const unsigned swizzle = (r & 7) << 4;
+    int c = 0, e = 0;   // accumulators, chunks used so far
     bool dead = false;  // a wait ran out: the rest of the list is walked without work, the result shows it
     for (int t = first; t < items; t += stride, ++c) {
       const Item it = item_of<TILE>(a, t);
-      const int row = it.row * TILE::M + rank * 128 + quad * 32 + lane;
-      const int col_first = it.col * BN + part * (BN / 2);
-      const int width = it.phase == UPDATE ? a.n : a.m;
+      const int chunks = chunks_of<TILE>(a, it);
+      const int row = it.row * TILE::M + rank * 128 + r;
       const bool row_in = row < a.m;
       const long long row_all = static_cast<long long>(it.mat) * a.m + row;
-      const __half* hi_in = a.hi[it.step & 1];
-      __half* hi_out = a.hi[(it.step + 1) & 1];
-      const StepScale sc = a.step[it.step];
-      if (!dead && !bar_wait(&acc_full[c & 1], (c / 2) & 1, gave_up)) {
-        *gave_up = 1;
-        atomicExch(a.err, 5);
-        dead = true;
-      }
-      asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
       const bool last = it.phase == UPDATE && it.step + 1 == a.steps;
       const bool mirror = it.phase != UPDATE && it.col / TILE::RATIO != it.row;
-      const float d = !row_in ? 0.0f
-                      : it.phase == POLY ? __ldcg(a.da + row_all)
-                      : it.phase == UPDATE ? __ldcg(a.db + row_all) : 0.0f;
-      for (int ch = 0; ch < CHUNKS; ++ch) {
-        const int col0 = col_first + ch * 32;
-        const int inside = row_in ? width - col0 : 0;
-        unsigned acc[32];
-        tmem_ld32(tmem + (static_cast<unsigned>(quad * 32) << 16) + (c & 1) * BN + part * (BN / 2) + ch * 32, acc);
-        float v[32];
+      const StepScale sc = a.step[it.step];
+      float d = 0.0f;
+      for (int ch = 0; ch < chunks; ++ch, ++e) {
+        const int b = e & 1;
+        if (!dead && !bar_wait(&side_full[b], (e / 2) & 1, gave_up)) dead = true;
+        if (ch == 0) {
+          if (row_in && it.phase != GRAM) d = __ldcg((it.phase == POLY ? a.da : a.db) + row_all);
+          if (!dead && !bar_wait(&acc_full[c & 1], (c / 2) & 1, gave_up)) dead = true;
+        }
         if (dead) {
-          asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+          *gave_up = 1;
+          atomicExch(a.err, 5);
+        }
+        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+        const int col0 = it.col * BN + ch * 64 + part * 32;
+        unsigned acc[32];
+        tmem_ld32(tmem + (static_cast<unsigned>(quad * 32) << 16) + (c & 1) * BN + ch * 64 + part * 32, acc);
+        const float mine = it.phase == POLY && col0 + lane < a.m
+                               ? __ldcg(a.da + static_cast<long long>(it.mat) * a.m + col0 + lane)
+                               : 0.0f;  // lane j: column j's diagonal element
+        asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+        if (ch + 1 == chunks) {  // the accumulator is free
+          asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+          __syncwarp();
+          if (lane == 0 && !dead) {
+            const unsigned bar = CTAS == 1 ? smem_u32(&acc_empty[c & 1]) : in_block(smem_u32(&acc_empty[c & 1]), 0);
+            asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
+          }
+        }
+        const unsigned s0 = smem_u32(side) + b * (2 * CHUNK), s1 = s0 + CHUNK;
+        float v[32];
 #pragma unroll
-          for (int j = 0; j < 32; ++j) v[j] = __int_as_float(0x7fffffff);
-          if (last && inside > 0) store_result(a, it.mat, row, col0, v, inside);
-        } else if (it.phase == GRAM) {
-          asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+        for (int g = 0; g < 4; ++g) {  // 8 columns
+          const unsigned at = r * 128 + ((part * 64 + g * 16) ^ swizzle);
+          uint4 x = make_uint4(0, 0, 0, 0), y = x;
+          if (it.phase != GRAM) x = lds128(s0 + at);
+          if (it.phase == UPDATE) y = lds128(s1 + at);
+          unsigned xs[4] = {x.x, x.y, x.z, x.w}, ys[4] = {y.x, y.y, y.z, y.w};
 #pragma unroll
-          for (int j = 0; j < 32; ++j) {
-            v[j] = __uint_as_float(acc[j]) * sc.gram;
-            if (col0 + j == row && inside > 0) {
-              a.da[row_all] = v[j];
-              v[j] = 0.0f;
+          for (int k = 0; k < 4; ++k) {
+            const int j = 8 * g + 2 * k;
+            const float2 xh = halves(xs[k]), xl = halves(ys[k]);
+            const float s_0 = __uint_as_float(acc[j]), s_1 = __uint_as_float(acc[j + 1]);
+            if (it.phase == GRAM) {
+              v[j] = s_0 * sc.gram;
+              v[j + 1] = s_1 * sc.gram;
+            } else if (it.phase == POLY) {
+              // B = p A + q (A_o A_o + (d_row + d_col) A_o), A_o without its diagonal d
+              v[j] = sc.poly_p * xh.x + sc.poly_q * (s_0 + (d + __shfl_sync(0xffffffffu, mine, j)) * xh.x);
+              v[j + 1] = sc.poly_p * xh.y + sc.poly_q * (s_1 + (d + __shfl_sync(0xffffffffu, mine, j + 1)) * xh.y);
+            } else {
+              // X = p X + q (B_o X_hi + d X_hi)
+              v[j] = sc.up_p * (xh.x + xl.x) + sc.up_q * (s_0 + d * xh.x);
+              v[j + 1] = sc.up_p * (xh.y + xl.y) + sc.up_q * (s_1 + d * xh.y);
             }
           }
-          if (inside > 0) {
-            store_half32(a.a + row_all * a.lda + col0, v, inside);
-            if (mirror) store_turned32(a.a + (static_cast<long long>(it.mat) * a.m + col0) * a.lda + row, a.lda, v, inside);
-          }
-        } else if (it.phase == POLY) {
-          // B = p A + q (A_o A_o + (d_row + d_col) A_o), A_o without its diagonal d
-          const Row32 ao = load_row32(a.a + row_all * a.lda + col0, inside);
-          const float* dc = a.da + static_cast<long long>(it.mat) * a.m + col0;
-          const float mine = col0 + lane < a.m ? __ldcg(dc + lane) : 0.0f;  // lane j holds column j's
-          asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+        }
+        if (it.phase != UPDATE && row >= col0 && row < col0 + 32) {  // this row's diagonal element
 #pragma unroll
-          for (int j = 0; j < 32; ++j) {
-            const float2 w = pair_of(ao, j / 2);
-            const float x = j & 1 ? w.y : w.x, s = __uint_as_float(acc[j]);
-            v[j] = sc.poly_p * x + sc.poly_q * (s + (d + __shfl_sync(0xffffffffu, mine, j)) * x);
-            if (col0 + j == row && inside > 0) {
-              a.db[row_all] = sc.poly_p * d + sc.poly_q * (s + d * d);
+          for (int j = 0; j < 32; ++j)
+            if (col0 + j == row) {
+              if (row_in) {
+                if (it.phase == GRAM)
+                  a.da[row_all] = v[j];
+                else
+                  a.db[row_all] = sc.poly_p * d + sc.poly_q * (__uint_as_float(acc[j]) + d * d);
+              }
               v[j] = 0.0f;
             }
+        }
+        if (last) {
+          const int inside = row_in ? a.n - col0 : 0;
+          if (dead) {
+#pragma unroll
+            for (int j = 0; j < 32; ++j) v[j] = __int_as_float(0x7fffffff);
           }
-          if (inside > 0) {
-            store_half32(a.b + row_all * a.lda + col0, v, inside);
-            if (mirror) store_turned32(a.b + (static_cast<long long>(it.mat) * a.m + col0) * a.lda + row, a.lda, v, inside);
-          }
+          if (inside > 0) store_result(a, it.mat, row, col0, v, inside);
         } else {
-          // X = p X + q (B_o X_hi + d X_hi)
-          const Row32 h = load_row32(hi_in + row_all * a.ldx + col0, inside);
-          const Row32 l = load_row32(a.lo + row_all * a.ldx + col0, inside);
-          asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
 #pragma unroll
-          for (int j = 0; j < 32; j += 2) {
-            const float2 x = pair_of(h, j / 2), y = pair_of(l, j / 2);
-            v[j] = sc.up_p * (x.x + y.x) + sc.up_q * (__uint_as_float(acc[j]) + d * x.x);
-            v[j + 1] = sc.up_p * (x.y + y.y) + sc.up_q * (__uint_as_float(acc[j + 1]) + d * x.y);
+          for (int g = 0; g < 4; ++g) {
+            const unsigned at = r * 128 + ((part * 64 + g * 16) ^ swizzle);
+            unsigned w[4];
+#pragma unroll
+            for (int k = 0; k < 4; ++k) w[k] = packed(v[8 * g + 2 * k], v[8 * g + 2 * k + 1]);
+            sts128(s0 + at, make_uint4(w[0], w[1], w[2], w[3]));
+            if (it.phase == UPDATE) {
+#pragma unroll
+              for (int k = 0; k < 4; ++k) {
+                const float2 h = halves(w[k]);
+                w[k] = packed(v[8 * g + 2 * k] - h.x, v[8 * g + 2 * k + 1] - h.y);
+              }
+              sts128(s1 + at, make_uint4(w[0], w[1], w[2], w[3]));
+            }
           }
-          if (inside > 0 && last) {
-            store_result(a, it.mat, row, col0, v, inside);
-          } else if (inside > 0) {
-            store_half32(hi_out + row_all * a.ldx + col0, v, inside);
+          if (mirror) {  // rows and columns exchanged: a box for each 64 rows
 #pragma unroll
-            for (int j = 0; j < 32; ++j) v[j] -= __half2float(__float2half_rn(v[j]));
-            store_half32(a.lo + row_all * a.ldx + col0, v, inside);
+            for (int j = 0; j < 32; ++j) {
+              const unsigned cc = part * 32 + j;
+              sts16(s1 + (r >> 6) * BOX + cc * 128 + (((r & 63) * 2) ^ ((cc & 7) << 4)), v[j]);
+            }
+          }
+          asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+        }
+        __syncwarp();
+        if (lane == 0) bar_arrive(&side_done[b]);
+      }
+    }
+  } else if (warp == LOADER) {
+    if (lane == 0) {  // what the epilogues need of X or A
+      int e = 0;
+      bool stop = false;
+      for (int t = first; t < items && !stop; t += stride) {
+        const Item it = item_of<TILE>(a, t);
+        const int chunks = chunks_of<TILE>(a, it);
+        if (!count_wait(a.ready + it.mat, needed(a, it, CTAS), gave_up)) {
+          *gave_up = 1;
+          atomicExch(a.err, 6);
+          break;
+        }
+        asm volatile("fence.proxy.async;" ::: "memory");
+        const int row = it.row * TILE::M + rank * 128;
+        for (int ch = 0; ch < chunks; ++ch, ++e) {
+          const int b = e & 1;
+          if (e >= 2 && !bar_wait(&side_empty[b], (e / 2 - 1) & 1, gave_up)) {
+            *gave_up = 1;
+            atomicExch(a.err, 7);
+            stop = true;
+            break;
+          }
+          const unsigned s0 = smem_u32(side) + b * (2 * CHUNK), bar = smem_u32(&side_full[b]);
+          const int col = it.col * BN + ch * 64;
+          if (it.phase == GRAM) {
+            bar_arrive(&side_full[b]);
+          } else if (it.phase == POLY) {
+            bar_expect(&side_full[b], CHUNK);
+            for (int h = 0; h < 2; ++h) box_load(&ta, s0 + h * BOX, bar, col, row + 64 * h, it.mat);
+          } else {
+            bar_expect(&side_full[b], 2 * CHUNK);
+            const CUtensorMap* x = it.step & 1 ? &tx1 : &tx0;
+            for (int h = 0; h < 2; ++h) box_load(x, s0 + h * BOX, bar, col, row + 64 * h, it.mat);
+            for (int h = 0; h < 2; ++h) box_load(&tl, s0 + CHUNK + h * BOX, bar, col, row + 64 * h, it.mat);
           }
         }
       }
-      // the accumulator is free, and what was written is there for other blocks' copies
-      asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
-      __threadfence();
-      asm volatile("fence.proxy.async;" ::: "memory");
-      __syncwarp();
-      if (lane == 0 && !dead) {
-        const unsigned bar = CTAS == 1 ? smem_u32(&acc_empty[c & 1]) : in_block(smem_u32(&acc_empty[c & 1]), 0);
-        asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
+    }
+  } else {
+    if (lane == 0) {  // their results
+      int e = 0;
+      bool stop = false;
+      for (int t = first; t < items && !stop; t += stride) {
+        const Item it = item_of<TILE>(a, t);
+        const int chunks = chunks_of<TILE>(a, it);
+        const bool last = it.phase == UPDATE && it.step + 1 == a.steps;
+        const bool mirror = it.phase != UPDATE && it.col / TILE::RATIO != it.row;
+        const int row = it.row * TILE::M + rank * 128;
+        const CUtensorMap* to = it.phase == GRAM ? &ta : it.phase == POLY ? &tb : it.step & 1 ? &tx0 : &tx1;
+        for (int ch = 0; ch < chunks; ++ch, ++e) {
+          const int b = e & 1;
+          if (!bar_wait(&side_done[b], (e / 2) & 1, gave_up)) {
+            *gave_up = 1;
+            atomicExch(a.err, 8);
+            stop = true;
+            break;
+          }
+          if (*gave_up) {
+            stop = true;
+            break;
+          }
+          if (!last) {
+            const unsigned s0 = smem_u32(side) + b * (2 * CHUNK), s1 = s0 + CHUNK;
+            const int col = it.col * BN + ch * 64;
+            for (int h = 0; h < 2; ++h)
+              if (row + 64 * h < a.m) {
+                box_store(to, s0 + h * BOX, col, row + 64 * h, it.mat);
+                if (it.phase == UPDATE) box_store(&tl, s1 + h * BOX, col, row + 64 * h, it.mat);
+                if (mirror) box_store(to, s1 + h * BOX, row + 64 * h, col, it.mat);
+              }
+            asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+            asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
+          }
+          bar_arrive(&side_empty[b]);
+        }
+        if (!stop && !last) {
+          // written, and there for other blocks' copies
+          asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
+          asm volatile("fence.proxy.async;" ::: "memory");
+          asm volatile("red.release.gpu.global.add.u32 [%0], 1;" ::"l"(a.ready + it.mat) : "memory");
+        }
       }
-      asm volatile("bar.sync 1, %0;" ::"n"(32 * EPI_WARPS) : "memory");
-      if (warp == 2 && lane == 0 && !dead)
-        asm volatile("red.release.gpu.global.add.u32 [%0], 1;" ::"l"(a.ready + it.mat) : "memory");
+      asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
     }
   }
   __syncwarp();
@@ -571,27 +692,58 @@ __global__ void __launch_bounds__(THREADS, 1)
 
 struct LoadArgs {
   const void* g;
-  int type;
-  long long batch, row, col;  // strides of G seen as m x n
+  long long batch, outer_stride, inner_stride;  // G as `outer` runs of `inner` elements, adjacent ones where there are any
+  int outer, inner;
+  int turned;  // runs are columns of X, not rows
   int m, n, ldx;
   float eps, scale;
   double* part;
   __half *hi, *lo;
 };
 
+// V adjacent elements of a run.
+template <typename T, int V>
+__device__ __forceinline__ void load_run(const LoadArgs& a, const T* p, float (&x)[V]) {
+  if (V == 1) {
+    x[0] = to_float(*p);
+  } else {
+    const Vec<T, V> w = load_vec<T, V>(p);
+#pragma unroll
+    for (int j = 0; j < V; ++j) x[j] = to_float(w.v[j]);
+  }
+}
+
 // A share of a matrix's sum of squares, in 64 bits: no scale of the update overflows.
+template <typename T, int V>
 __global__ void __launch_bounds__(256) ns_norm(const __grid_constant__ LoadArgs a) {
+  constexpr int U = 4;  // loads in flight
   __shared__ double buf[8];
   const long long mat = blockIdx.y;
-  const bool by_row = a.col == 1 || a.row != 1;  // along the axis of adjacent elements
-  const int outer = by_row ? a.m : a.n, inner = by_row ? a.n : a.m;
-  const long long so = by_row ? a.row : a.col, si = by_row ? a.col : a.row;
+  const T* g = static_cast<const T*>(a.g) + mat * a.batch;
+  const unsigned per = a.inner / V;
+  const long long total = static_cast<long long>(a.outer) * per, step = static_cast<long long>(gridDim.x) * 256;
   double s = 0.0;
-  for (int o = blockIdx.x; o < outer; o += gridDim.x)
-    for (int i = threadIdx.x; i < inner; i += blockDim.x) {
-      const double x = load_any(a.g, a.type, mat * a.batch + o * so + i * si);
-      s += x * x;
+  for (long long i = blockIdx.x * 256ll + threadIdx.x; i < total; i += U * step) {
+    float x[U][V];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const long long k = i + u * step;
+      if (k < total) {
+        const long long o = k / per;
+        load_run<T, V>(a, g + o * a.outer_stride + (k - o * per) * V * a.inner_stride, x[u]);
+      } else {
+#pragma unroll
+        for (int j = 0; j < V; ++j) x[u][j] = 0.0f;
+      }
     }
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+#pragma unroll
+      for (int j = 0; j < V; ++j) {
+        const double y = x[u][j];
+        s = fma(y, y, s);
+      }
+  }
 #pragma unroll
   for (int o = 16; o; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
   if ((threadIdx.x & 31) == 0) buf[threadIdx.x >> 5] = s;
@@ -602,29 +754,66 @@ __global__ void __launch_bounds__(256) ns_norm(const __grid_constant__ LoadArgs 
   }
 }
 
-// X = G scale / (|G| + eps) as the sum of two f16 numbers.
+// X = G scale / (|G| + eps) as the sum of two f16 numbers, 64 x 64 elements a
+// block.  The last matrices first: the norm's pass has left them in L2.
+template <typename T, int V>
 __global__ void __launch_bounds__(256) ns_load(const __grid_constant__ LoadArgs a) {
-  __shared__ float t[32][33];
-  const long long mat = blockIdx.z;
-  const int c0 = blockIdx.x * 32, r0 = blockIdx.y * 32, tx = threadIdx.x, ty = threadIdx.y;
-  double sum = 0.0;
-  for (int k = 0; k < NORM_BLOCKS; ++k) sum += a.part[mat * NORM_BLOCKS + k];
-  const float f = static_cast<float>(a.scale / (sqrt(sum) + a.eps));
-  const bool by_row = a.col == 1 || a.row != 1;
-  for (int k = ty; k < 32; k += 8) {
-    const int r = by_row ? r0 + k : r0 + tx, c = by_row ? c0 + tx : c0 + k;
-    const float x = r < a.m && c < a.n ? load_any(a.g, a.type, mat * a.batch + r * a.row + c * a.col) * f : 0.0f;
-    t[r - r0][c - c0] = x;
-  }
-  __syncthreads();
-  for (int k = ty; k < 32; k += 8) {
-    if (r0 + k < a.m && c0 + tx < a.n) {
-      const long long at = (mat * a.m + r0 + k) * a.ldx + c0 + tx;
-      const __half h = __float2half_rn(t[k][tx]);
-      a.hi[at] = h;
-      a.lo[at] = __float2half_rn(t[k][tx] - __half2float(h));
+  __shared__ float t[64][65];
+  __shared__ float factor;
+  const long long mat = gridDim.z - 1 - blockIdx.z;
+  const T* g = static_cast<const T*>(a.g) + mat * a.batch;
+  const int i0 = blockIdx.x * 64, o0 = blockIdx.y * 64;  // along a run, of runs
+  constexpr int PER = 64 / V;                            // vectors of a run here
+  constexpr int N = 64 * PER / 256;
+  float x[N][V];
+#pragma unroll
+  for (int k = 0; k < N; ++k) {
+    const int at = k * 256 + threadIdx.x, o = o0 + at / PER, i = i0 + at % PER * V;
+    if (o < a.outer && i < a.inner) {
+      load_run<T, V>(a, g + o * a.outer_stride + i * a.inner_stride, x[k]);
+    } else {
+#pragma unroll
+      for (int j = 0; j < V; ++j) x[k][j] = 0.0f;
     }
   }
+  if (threadIdx.x < 32) {
+    double s = 0.0;
+    for (int k = threadIdx.x; k < NORM_BLOCKS; k += 32) s += a.part[mat * NORM_BLOCKS + k];
+#pragma unroll
+    for (int o = 16; o; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+    if (threadIdx.x == 0) factor = static_cast<float>(a.scale / (sqrt(s) + a.eps));
+  }
+#pragma unroll
+  for (int k = 0; k < N; ++k) {
+    const int at = k * 256 + threadIdx.x, o = at / PER, i = at % PER * V;
+#pragma unroll
+    for (int j = 0; j < V; ++j) t[a.turned ? i + j : o][a.turned ? o : i + j] = x[k][j];
+  }
+  __syncthreads();
+  const float f = factor;
+  const int r0 = a.turned ? i0 : o0, c0 = a.turned ? o0 : i0;
+#pragma unroll
+  for (int k = 0; k < 2; ++k) {  // 8 adjacent elements of a row of X
+    const int at = k * 256 + threadIdx.x, r = at / 8, c = at % 8 * 8;
+    if (r0 + r >= a.m || c0 + c >= a.n) continue;
+    Vec<__half, 8> h, l;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      const float y = t[r][c + j] * f;
+      h.v[j] = __float2half_rn(y);
+      l.v[j] = __float2half_rn(y - __half2float(h.v[j]));
+    }
+    const long long to = (mat * a.m + r0 + r) * a.ldx + c0 + c;  // the row's padding takes zeros
+    store_vec<__half, 8>(a.hi + to, h);
+    store_vec<__half, 8>(a.lo + to, l);
+  }
+}
+
+template <typename T, int V>
+cudaError_t load(const LoadArgs& a, int count, cudaStream_t st) {
+  ns_norm<T, V><<<dim3(NORM_BLOCKS, count), 256, 0, st>>>(a);
+  ns_load<T, V><<<dim3((a.inner + 63) / 64, (a.outer + 63) / 64, count), 256, 0, st>>>(a);
+  return cudaGetLastError();
 }
 
 // No steps: the normalised matrix itself.
@@ -732,7 +921,7 @@ Tiling tiling(long long count, long long m, long long n, int workers, double per
 }
 
 template <int CTAS, int BN>
-cudaError_t start(const CUtensorMap (&maps)[4], NsArgs& a, const Tiling& t, int sms, int device, cudaStream_t st) {
+cudaError_t start(const CUtensorMap (&maps)[5], NsArgs& a, const Tiling& t, int sms, int device, cudaStream_t st) {
   using TILE = Tile<CTAS, BN>;
   static bool ready[64] = {};
   if (device >= 64 || !ready[device]) {
@@ -758,7 +947,7 @@ cudaError_t start(const CUtensorMap (&maps)[4], NsArgs& a, const Tiling& t, int 
   at[1].val.clusterDim.y = at[1].val.clusterDim.z = 1;
   c.attrs = at;
   c.numAttrs = CTAS == 1 ? 1 : 2;
-  return cudaLaunchKernelEx(&c, ns_kernel<CTAS, BN>, maps[0], maps[1], maps[2], maps[3], a);
+  return cudaLaunchKernelEx(&c, ns_kernel<CTAS, BN>, maps[0], maps[1], maps[2], maps[3], maps[4], a);
 }
 
 }  // namespace
@@ -801,27 +990,30 @@ extern "C" int ad_orthogonalize(int device, int dtype, const void* g, int64_t co
   const int m = static_cast<int>(l.m), n = static_cast<int>(l.n), num = static_cast<int>(count);
 
   LoadArgs la = {};
-  la.g = g, la.type = dtype;
-  la.batch = batch_stride, la.row = tall ? col_stride : row_stride, la.col = tall ? row_stride : col_stride;
+  la.g = g, la.batch = batch_stride;
+  const bool by_row = col_stride == 1 || row_stride != 1;
+  la.outer = static_cast<int>(by_row ? rows : cols), la.inner = static_cast<int>(by_row ? cols : rows);
+  la.outer_stride = by_row ? row_stride : col_stride, la.inner_stride = by_row ? col_stride : row_stride;
+  la.turned = by_row == tall;
   la.m = m, la.n = n, la.ldx = static_cast<int>(l.ldx);
   la.eps = eps, la.scale = static_cast<float>(sc.x[0]);
   la.part = reinterpret_cast<double*>(w + l.part);
   la.hi = reinterpret_cast<__half*>(w + l.hi[0]);
   la.lo = reinterpret_cast<__half*>(w + l.lo);
+  const bool vec = la.inner_stride == 1 && la.inner % 4 == 0 && la.outer_stride % 4 == 0 && batch_stride % 4 == 0 &&
+                   aligned(g, 4 * elem_size(dtype));
   cudaError_t e = cudaMemsetAsync(w, 0, 256 + 4ull * count, st);
-  if (e != cudaSuccess) return fail("ad_orthogonalize: %s", cudaGetErrorString(e));
-  ns_norm<<<dim3(NORM_BLOCKS, num), 256, 0, st>>>(la);
-  ns_load<<<dim3((n + 31) / 32, (m + 31) / 32, num), dim3(32, 8), 0, st>>>(la);
-  e = cudaGetLastError();
+  if (e == cudaSuccess)
+    e = dtype == AD_F32    ? (vec ? load<float, 4>(la, num, st) : load<float, 1>(la, num, st))
+        : dtype == AD_BF16 ? (vec ? load<__nv_bfloat16, 4>(la, num, st) : load<__nv_bfloat16, 1>(la, num, st))
+                           : (vec ? load<__half, 4>(la, num, st) : load<__half, 1>(la, num, st));
   if (e != cudaSuccess) return fail("ad_orthogonalize: %s", cudaGetErrorString(e));
 
   NsArgs s = {};
   s.count = num, s.m = m, s.n = n, s.steps = steps;
-  s.ldx = la.ldx, s.lda = static_cast<int>(l.lda);
+  s.ldx = la.ldx;
   for (int k = 0; k < 2; ++k) s.hi[k] = reinterpret_cast<__half*>(w + l.hi[k]);
   s.lo = la.lo;
-  s.a = reinterpret_cast<__half*>(w + l.a);
-  s.b = reinterpret_cast<__half*>(w + l.b);
   s.da = reinterpret_cast<float*>(w + l.da);
   s.db = reinterpret_cast<float*>(w + l.db);
   s.err = reinterpret_cast<int*>(w);
@@ -844,10 +1036,10 @@ extern "C" int ad_orthogonalize(int device, int dtype, const void* g, int64_t co
     s.step[k] = {static_cast<float>(sa / (sx * sx)), static_cast<float>(b * sb / sa), static_cast<float>(c * sb / (sa * sa)),
                  static_cast<float>(a * up), static_cast<float>(up / sb)};
   }
-  alignas(64) CUtensorMap maps[4];  // X twice, A, B
-  const void* const base[4] = {s.hi[0], s.hi[1], s.a, s.b};
-  for (int k = 0; k < 4; ++k)
-    if (ad_b200_internal::tmap_3d_16(base[k], count, m, k < 2 ? n : m, k < 2 ? l.ldx : l.lda, 64, BK, &maps[k])) return 1;
+  alignas(64) CUtensorMap maps[5];  // X's larger part twice, the smaller, A, B
+  const void* const base[5] = {s.hi[0], s.hi[1], s.lo, w + l.a, w + l.b};
+  for (int k = 0; k < 5; ++k)
+    if (ad_b200_internal::tmap_3d_16(base[k], count, m, k < 3 ? n : m, k < 3 ? l.ldx : l.lda, 64, BK, &maps[k])) return 1;
 
   const int sms = sm_count(guard.device());
   if (!sms) return fail("ad_orthogonalize: no device properties");

@@ -63,8 +63,11 @@ struct Tile {
   static constexpr int M = 128 * CTAS, N = BN;
   static constexpr int QN = BN / CTAS;  // columns whose operand a block holds
   static constexpr int P_BYTES = 128 * BK * 2, Q_BYTES = QN * BK * 2, STAGE = P_BYTES + Q_BYTES;
-  static constexpr int STAGES = 160 * 1024 / STAGE;
-  static constexpr int SMEM = STAGES * STAGE + 4 * CHUNK + 1024 + 512;
+  // buffers of two chunks for the epilogues: a large tile's updates keep three
+  // busy (10.0 us a tile with two, beside 7 us for its products)
+  static constexpr int SIDES = CTAS == 2 ? 3 : 2;
+  static constexpr int STAGES = (224 * 1024 - SIDES * 2 * CHUNK) / STAGE;
+  static constexpr int SMEM = STAGES * STAGE + SIDES * 2 * CHUNK + 1024 + 512;
   static constexpr int RATIO = M / N;  // column tiles beside a row tile on the diagonal
 };
 
@@ -86,6 +89,13 @@ struct NsArgs {
   int* err;
   unsigned* ready;  // a matrix's finished tiles (counted once a block)
   StepScale step[MAX_STEPS];
+};
+
+// Boxes of 64 rows: X's larger part twice (a step reads one and writes the
+// other), its smaller part, A, B; of 128 rows: the same without the smaller part.
+enum { MAP_X = 0, MAP_LO = 2, MAP_A = 3, MAP_B = 4, WIDE_X = 5, WIDE_A = 7, WIDE_B = 8, MAPS = 9 };
+struct Maps {
+  CUtensorMap m[MAPS];
 };
 
 __device__ __forceinline__ unsigned smem_u32(const void* p) {
@@ -275,23 +285,21 @@ __device__ __forceinline__ unsigned needed(const NsArgs& a, const Item& i, int c
 
 template <int CTAS, int BN>
 __global__ void __launch_bounds__(THREADS, 1)
-    ns_kernel(const __grid_constant__ CUtensorMap tx0, const __grid_constant__ CUtensorMap tx1,
-              const __grid_constant__ CUtensorMap tl, const __grid_constant__ CUtensorMap ta,
-              const __grid_constant__ CUtensorMap tb, const __grid_constant__ NsArgs a) {
+    ns_kernel(const __grid_constant__ Maps maps, const __grid_constant__ NsArgs a) {
   using TILE = Tile<CTAS, BN>;
-  constexpr int STAGES = TILE::STAGES;
+  constexpr int STAGES = TILE::STAGES, SIDES = TILE::SIDES;
   extern __shared__ __align__(1024) unsigned char raw[];
   unsigned char* smem = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~uintptr_t(1023));
-  // two buffers of two chunks for the epilogues behind the operands' stages
+  // the epilogues' buffers behind the operands' stages
   unsigned char* side = smem + STAGES * TILE::STAGE;
-  unsigned long long* full = reinterpret_cast<unsigned long long*>(side + 4 * CHUNK);
+  unsigned long long* full = reinterpret_cast<unsigned long long*>(side + SIDES * 2 * CHUNK);
   unsigned long long* empty = full + STAGES;
   unsigned long long* acc_full = empty + STAGES;
   unsigned long long* acc_empty = acc_full + 2;
   unsigned long long* side_full = acc_empty + 2;   // a buffer holds what the epilogue needs
-  unsigned long long* side_done = side_full + 2;   // ... and then its results
-  unsigned long long* side_empty = side_done + 2;  // ... which are under way
-  unsigned* tmem_slot = reinterpret_cast<unsigned*>(side_empty + 2);
+  unsigned long long* side_done = side_full + SIDES;   // ... and then its results
+  unsigned long long* side_empty = side_done + SIDES;  // ... which are under way
+  unsigned* tmem_slot = reinterpret_cast<unsigned*>(side_empty + SIDES);
   volatile int* gave_up = reinterpret_cast<volatile int*>(tmem_slot + 1);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int rank = CTAS == 1 ? 0 : blockIdx.x & 1;
@@ -306,6 +314,8 @@ __global__ void __launch_bounds__(THREADS, 1)
     for (int i = 0; i < 2; ++i) {
       asm volatile("mbarrier.init.shared::cta.b64 [%0], 1;" ::"r"(smem_u32(&acc_full[i])));
       asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(smem_u32(&acc_empty[i])), "r"(CTAS * EPI_WARPS));
+    }
+    for (int i = 0; i < SIDES; ++i) {
       asm volatile("mbarrier.init.shared::cta.b64 [%0], 1;" ::"r"(smem_u32(&side_full[i])));
       asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(smem_u32(&side_done[i])), "r"(EPI_WARPS));
       asm volatile("mbarrier.init.shared::cta.b64 [%0], 1;" ::"r"(smem_u32(&side_empty[i])));
@@ -348,9 +358,11 @@ __global__ void __launch_bounds__(THREADS, 1)
         }
         // what others wrote through the generic proxy is read through the async one
         asm volatile("fence.proxy.async;" ::: "memory");
-        const CUtensorMap* x = it.step & 1 ? &tx1 : &tx0;
-        const CUtensorMap* p = it.phase == GRAM ? x : it.phase == POLY ? &ta : &tb;
-        const CUtensorMap* q = it.phase == POLY ? &ta : x;
+        const int x = it.step & 1;
+        const CUtensorMap* p = &maps.m[it.phase == GRAM ? WIDE_X + x : it.phase == POLY ? WIDE_A : WIDE_B];
+        const CUtensorMap* q = it.phase == UPDATE ? &maps.m[MAP_X + x]
+                               : TILE::QN == 128  ? p
+                                                  : &maps.m[it.phase == GRAM ? MAP_X + x : MAP_A];
         const int kblocks = ((it.phase == GRAM ? a.n : a.m) + BK - 1) / BK;
         const int p0 = it.row * TILE::M + rank * 128;
         const int q0 = it.col * BN + rank * TILE::QN;
@@ -384,14 +396,12 @@ __global__ void __launch_bounds__(THREADS, 1)
                   : "memory");
           };
           load(p, st, kb * BK, p0);
-          load(p, st + BOX, kb * BK, p0 + 64);
           unsigned char* sq = st + TILE::P_BYTES;
+          if (it.phase == UPDATE) {
 #pragma unroll
-          for (int h = 0; h < TILE::QN / 64; ++h) {
-            if (it.phase == UPDATE)
-              load(q, sq + h * BOX, q0 + h * 64, kb * BK);
-            else
-              load(q, sq + h * BOX, kb * BK, q0 + h * 64);
+            for (int h = 0; h < TILE::QN / 64; ++h) load(q, sq + h * BOX, q0 + h * 64, kb * BK);
+          } else {
+            load(q, sq, kb * BK, q0);
           }
         }
         if (stop) break;
@@ -479,8 +489,8 @@ __global__ void __launch_bounds__(THREADS, 1)
       const StepScale sc = a.step[it.step];
       float d = 0.0f;
       for (int ch = 0; ch < chunks; ++ch, ++e) {
-        const int b = e & 1;
-        if (!dead && !bar_wait(&side_full[b], (e / 2) & 1, gave_up)) dead = true;
+        const int b = e % SIDES;
+        if (!dead && !bar_wait(&side_full[b], (e / SIDES) & 1, gave_up)) dead = true;
         if (ch == 0) {
           if (row_in && it.phase != GRAM) d = __ldcg((it.phase == POLY ? a.da : a.db) + row_all);
           if (!dead && !bar_wait(&acc_full[c & 1], (c / 2) & 1, gave_up)) dead = true;
@@ -598,8 +608,8 @@ __global__ void __launch_bounds__(THREADS, 1)
         asm volatile("fence.proxy.async;" ::: "memory");
         const int row = it.row * TILE::M + rank * 128;
         for (int ch = 0; ch < chunks; ++ch, ++e) {
-          const int b = e & 1;
-          if (e >= 2 && !bar_wait(&side_empty[b], (e / 2 - 1) & 1, gave_up)) {
+          const int b = e % SIDES;
+          if (e >= SIDES && !bar_wait(&side_empty[b], (e / SIDES - 1) & 1, gave_up)) {
             *gave_up = 1;
             atomicExch(a.err, 7);
             stop = true;
@@ -611,12 +621,12 @@ __global__ void __launch_bounds__(THREADS, 1)
             bar_arrive(&side_full[b]);
           } else if (it.phase == POLY) {
             bar_expect(&side_full[b], CHUNK);
-            for (int h = 0; h < 2; ++h) box_load(&ta, s0 + h * BOX, bar, col, row + 64 * h, it.mat);
+            for (int h = 0; h < 2; ++h) box_load(&maps.m[MAP_A], s0 + h * BOX, bar, col, row + 64 * h, it.mat);
           } else {
             bar_expect(&side_full[b], 2 * CHUNK);
-            const CUtensorMap* x = it.step & 1 ? &tx1 : &tx0;
+            const CUtensorMap* x = &maps.m[MAP_X + (it.step & 1)];
             for (int h = 0; h < 2; ++h) box_load(x, s0 + h * BOX, bar, col, row + 64 * h, it.mat);
-            for (int h = 0; h < 2; ++h) box_load(&tl, s0 + CHUNK + h * BOX, bar, col, row + 64 * h, it.mat);
+            for (int h = 0; h < 2; ++h) box_load(&maps.m[MAP_LO], s0 + CHUNK + h * BOX, bar, col, row + 64 * h, it.mat);
           }
         }
       }
@@ -631,10 +641,11 @@ __global__ void __launch_bounds__(THREADS, 1)
         const bool last = it.phase == UPDATE && it.step + 1 == a.steps;
         const bool mirror = it.phase != UPDATE && it.col / TILE::RATIO != it.row;
         const int row = it.row * TILE::M + rank * 128;
-        const CUtensorMap* to = it.phase == GRAM ? &ta : it.phase == POLY ? &tb : it.step & 1 ? &tx0 : &tx1;
+        const CUtensorMap* to =
+            &maps.m[it.phase == GRAM ? MAP_A : it.phase == POLY ? MAP_B : MAP_X + ((it.step + 1) & 1)];
         for (int ch = 0; ch < chunks; ++ch, ++e) {
-          const int b = e & 1;
-          if (!bar_wait(&side_done[b], (e / 2) & 1, gave_up)) {
+          const int b = e % SIDES;
+          if (!bar_wait(&side_done[b], (e / SIDES) & 1, gave_up)) {
             *gave_up = 1;
             atomicExch(a.err, 8);
             stop = true;
@@ -650,7 +661,7 @@ __global__ void __launch_bounds__(THREADS, 1)
             for (int h = 0; h < 2; ++h)
               if (row + 64 * h < a.m) {
                 box_store(to, s0 + h * BOX, col, row + 64 * h, it.mat);
-                if (it.phase == UPDATE) box_store(&tl, s1 + h * BOX, col, row + 64 * h, it.mat);
+                if (it.phase == UPDATE) box_store(&maps.m[MAP_LO], s1 + h * BOX, col, row + 64 * h, it.mat);
                 if (mirror) box_store(to, s1 + h * BOX, row + 64 * h, col, it.mat);
               }
             asm volatile("cp.async.bulk.commit_group;" ::: "memory");
@@ -921,7 +932,7 @@ Tiling tiling(long long count, long long m, long long n, int workers, double per
 }
 
 template <int CTAS, int BN>
-cudaError_t start(const CUtensorMap (&maps)[5], NsArgs& a, const Tiling& t, int sms, int device, cudaStream_t st) {
+cudaError_t start(const Maps& maps, NsArgs& a, const Tiling& t, int sms, int device, cudaStream_t st) {
   using TILE = Tile<CTAS, BN>;
   static bool ready[64] = {};
   if (device >= 64 || !ready[device]) {
@@ -947,7 +958,7 @@ cudaError_t start(const CUtensorMap (&maps)[5], NsArgs& a, const Tiling& t, int 
   at[1].val.clusterDim.y = at[1].val.clusterDim.z = 1;
   c.attrs = at;
   c.numAttrs = CTAS == 1 ? 1 : 2;
-  return cudaLaunchKernelEx(&c, ns_kernel<CTAS, BN>, maps[0], maps[1], maps[2], maps[3], maps[4], a);
+  return cudaLaunchKernelEx(&c, ns_kernel<CTAS, BN>, maps, a);
 }
 
 }  // namespace
@@ -1036,10 +1047,13 @@ extern "C" int ad_orthogonalize(int device, int dtype, const void* g, int64_t co
     s.step[k] = {static_cast<float>(sa / (sx * sx)), static_cast<float>(b * sb / sa), static_cast<float>(c * sb / (sa * sa)),
                  static_cast<float>(a * up), static_cast<float>(up / sb)};
   }
-  alignas(64) CUtensorMap maps[5];  // X's larger part twice, the smaller, A, B
-  const void* const base[5] = {s.hi[0], s.hi[1], s.lo, w + l.a, w + l.b};
-  for (int k = 0; k < 5; ++k)
-    if (ad_b200_internal::tmap_3d_16(base[k], count, m, k < 3 ? n : m, k < 3 ? l.ldx : l.lda, 64, BK, &maps[k])) return 1;
+  Maps maps;
+  const void* const base[MAPS] = {s.hi[0], s.hi[1], s.lo, w + l.a, w + l.b, s.hi[0], s.hi[1], w + l.a, w + l.b};
+  for (int k = 0; k < MAPS; ++k) {
+    const bool of_x = k <= MAP_LO || k == WIDE_X || k == WIDE_X + 1;
+    if (ad_b200_internal::tmap_3d_16(base[k], count, m, of_x ? n : m, of_x ? l.ldx : l.lda, k < WIDE_X ? 64 : 128, BK, &maps.m[k]))
+      return 1;
+  }
 
   const int sms = sm_count(guard.device());
   if (!sms) return fail("ad_orthogonalize: no device properties");

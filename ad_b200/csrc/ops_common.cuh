@@ -17,10 +17,10 @@ namespace ad_b200_internal {
 // runtime.cu:
 void set_error(const char* msg);  // the message ad_last_error() returns
 // TMA descriptor of `count` row-major matrices of 16-bit elements stacked in
-// memory (row stride `ld` elements), 128-byte swizzle, boxes of one matrix's
-// rows; what lies outside a matrix reads as zero.  0, or 1 with an error set.
+// memory (row stride `ld` elements), swizzled over 64 or 128 bytes, boxes of one
+// matrix's rows; what lies outside a matrix reads as zero.  0, or 1 with an error set.
 int tmap_3d_16(const void* base, uint64_t count, uint64_t rows, uint64_t cols, uint64_t ld, uint32_t box_rows,
-               uint32_t box_cols, void* out128);
+               uint32_t box_cols, int swizzle_bytes, void* out128);
 }
 
 namespace adops {

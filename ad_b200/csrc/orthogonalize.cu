@@ -24,7 +24,7 @@
 // the matrices.  A tile waits only for the previous product of its own matrix, by
 // a counter in memory, so that a batch leaves no gaps between products.  Within
 // a block one warp brings operands by TMA, one issues the products into one of
-// two accumulators, eight work on the other: 64 columns at a time they join
+// two accumulators, eight work on the other: 32 columns at a time they join
 // the accumulator with what the epilogue needs of X or A, which a further warp
 // has brought into shared memory ahead of them, and leave the result in its
 // place, from where the last warp sends it off by TMA (lanes hold rows, so that
@@ -51,7 +51,7 @@ constexpr int BOX = 64 * BK * 2;  // bytes of a TMA box: 64 rows
 constexpr int EPI_WARPS = 8;
 constexpr int LOADER = 2 + EPI_WARPS, STORER = LOADER + 1;  // warps that serve the epilogues
 constexpr int THREADS = 32 * (STORER + 1);
-constexpr int CHUNK = 2 * BOX;  // 128 rows of 64 columns of 16 bits
+constexpr int CHUNK_COLS = 32, CHUNK = 128 * CHUNK_COLS * 2;  // what an epilogue takes at a time: 128 rows of 16 bits
 constexpr int MAX_STEPS = 32;
 constexpr int NORM_BLOCKS = 64;  // blocks that share a matrix's norm
 
@@ -63,9 +63,8 @@ struct Tile {
   static constexpr int M = 128 * CTAS, N = BN;
   static constexpr int QN = BN / CTAS;  // columns whose operand a block holds
   static constexpr int P_BYTES = 128 * BK * 2, Q_BYTES = QN * BK * 2, STAGE = P_BYTES + Q_BYTES;
-  // buffers of two chunks for the epilogues: a large tile's updates keep three
-  // busy (10.0 us a tile with two, beside 7 us for its products)
-  static constexpr int SIDES = CTAS == 2 ? 3 : 2;
+  // buffers of two chunks for the epilogues, by turns for each half of their warps
+  static constexpr int SIDES = CTAS == 2 ? 6 : 4;
   static constexpr int STAGES = (224 * 1024 - SIDES * 2 * CHUNK) / STAGE;
   static constexpr int SMEM = STAGES * STAGE + SIDES * 2 * CHUNK + 1024 + 512;
   static constexpr int RATIO = M / N;  // column tiles beside a row tile on the diagonal
@@ -91,9 +90,14 @@ struct NsArgs {
   StepScale step[MAX_STEPS];
 };
 
-// Boxes of 64 rows: X's larger part twice (a step reads one and writes the
-// other), its smaller part, A, B; of 128 rows: the same without the smaller part.
-enum { MAP_X = 0, MAP_LO = 2, MAP_A = 3, MAP_B = 4, WIDE_X = 5, WIDE_A = 7, WIDE_B = 8, MAPS = 9 };
+// TMA maps.  Operands, swizzled over 128 bytes: boxes of 64 elements of K by 128
+// rows, and by 64 (also 64 rows of K by 64 columns).  Chunks for the epilogues:
+// boxes of 32 columns by 128 rows, swizzled over 64 bytes; transposed ones: 64
+// columns by 32 rows.  X's larger part is there twice: a step reads one, writes the other.
+enum {
+  WIDE_X = 0, WIDE_A = 2, WIDE_B = 3, NARROW_X = 4, NARROW_A = 6,
+  CHUNK_X = 7, CHUNK_LO = 9, CHUNK_A = 10, CHUNK_B = 11, TURNED_A = 12, TURNED_B = 13, MAPS = 14
+};
 struct Maps {
   CUtensorMap m[MAPS];
 };
@@ -159,16 +163,14 @@ __device__ __forceinline__ unsigned long long desc_n(const void* p) {
          ((1024ull >> 4) << 32) | (1ull << 46) | (2ull << 61);
 }
 
-__device__ __forceinline__ void tmem_ld32(unsigned taddr, unsigned (&r)[32]) {
-  asm volatile(
-      "tcgen05.ld.sync.aligned.32x32b.x32.b32 "
-      "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
-      "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
-      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
-        "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]),
-        "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]),
-        "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
-      : "r"(taddr));
+__device__ __forceinline__ void tmem_ld8(unsigned taddr, float (&r)[8]) {
+  unsigned q[8];
+  asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
+               : "=r"(q[0]), "=r"(q[1]), "=r"(q[2]), "=r"(q[3]), "=r"(q[4]), "=r"(q[5]), "=r"(q[6]), "=r"(q[7])
+               : "r"(taddr));
+  asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+#pragma unroll
+  for (int j = 0; j < 8; ++j) r[j] = __uint_as_float(q[j]);
 }
 
 __device__ __forceinline__ uint4 lds128(unsigned addr) {
@@ -209,33 +211,30 @@ __device__ __forceinline__ void bar_arrive(unsigned long long* bar) {
   asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(bar)) : "memory");
 }
 
-// Part of a row of the result.
-__device__ __forceinline__ void store_result(const NsArgs& a, long long mat, int row, int col0, float (&v)[32], int inside) {
+// Eight elements of a row of the result.
+__device__ __forceinline__ void store_result(const NsArgs& a, long long mat, int row, int col0, float (&v)[8], int inside) {
   const long long at = mat * a.out_batch + row * a.out_row + col0 * a.out_col;
 #pragma unroll
-  for (int j = 0; j < 32; ++j) v[j] *= a.out_scale;
-  if (a.out_vec && inside >= 32) {
+  for (int j = 0; j < 8; ++j) v[j] *= a.out_scale;
+  if (a.out_vec && inside >= 8) {
+    if (a.out_type == AD_F32) {
+      float* p = static_cast<float*>(a.out) + at;
+      store_vec<float, 4>(p, {{v[0], v[1], v[2], v[3]}});
+      store_vec<float, 4>(p + 4, {{v[4], v[5], v[6], v[7]}});
+    } else if (a.out_type == AD_BF16) {
+      Vec<__nv_bfloat16, 8> w;
 #pragma unroll
-    for (int k = 0; k < 32; k += 8) {
-      if (a.out_type == AD_F32) {
-        float* p = static_cast<float*>(a.out) + at + k;
-        store_vec<float, 4>(p, {{v[k], v[k + 1], v[k + 2], v[k + 3]}});
-        store_vec<float, 4>(p + 4, {{v[k + 4], v[k + 5], v[k + 6], v[k + 7]}});
-      } else if (a.out_type == AD_BF16) {
-        Vec<__nv_bfloat16, 8> w;
+      for (int j = 0; j < 8; ++j) w.v[j] = from_float<__nv_bfloat16>(v[j]);
+      store_vec<__nv_bfloat16, 8>(static_cast<__nv_bfloat16*>(a.out) + at, w);
+    } else {
+      Vec<__half, 8> w;
 #pragma unroll
-        for (int j = 0; j < 8; ++j) w.v[j] = from_float<__nv_bfloat16>(v[k + j]);
-        store_vec<__nv_bfloat16, 8>(static_cast<__nv_bfloat16*>(a.out) + at + k, w);
-      } else {
-        Vec<__half, 8> w;
-#pragma unroll
-        for (int j = 0; j < 8; ++j) w.v[j] = from_float<__half>(v[k + j]);
-        store_vec<__half, 8>(static_cast<__half*>(a.out) + at + k, w);
-      }
+      for (int j = 0; j < 8; ++j) w.v[j] = from_float<__half>(v[j]);
+      store_vec<__half, 8>(static_cast<__half*>(a.out) + at, w);
     }
   } else {
 #pragma unroll
-    for (int j = 0; j < 32; ++j)
+    for (int j = 0; j < 8; ++j)
       if (j < inside) store_any(a.out, a.out_type, at + j * a.out_col, v[j]);
   }
 }
@@ -272,11 +271,11 @@ __device__ __forceinline__ Item item_of(const NsArgs& a, int t) {
   return i;
 }
 
-// Chunks of 64 columns of an item's tile that are not wholly past the matrix.
+// Chunks of an item's tile that are not wholly past the matrix.
 template <typename TILE>
 __device__ __forceinline__ int chunks_of(const NsArgs& a, const Item& i) {
   const int width = (i.phase == UPDATE ? a.n : a.m) - i.col * TILE::N;
-  return min(TILE::N, width + 63) / 64;
+  return min(TILE::N, width + CHUNK_COLS - 1) / CHUNK_COLS;
 }
 // Tiles of its matrix that have to be finished before an item's operands are there.
 __device__ __forceinline__ unsigned needed(const NsArgs& a, const Item& i, int ctas) {
@@ -317,7 +316,7 @@ __global__ void __launch_bounds__(THREADS, 1)
     }
     for (int i = 0; i < SIDES; ++i) {
       asm volatile("mbarrier.init.shared::cta.b64 [%0], 1;" ::"r"(smem_u32(&side_full[i])));
-      asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(smem_u32(&side_done[i])), "r"(EPI_WARPS));
+      asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(smem_u32(&side_done[i])), "r"(EPI_WARPS / 2));
       asm volatile("mbarrier.init.shared::cta.b64 [%0], 1;" ::"r"(smem_u32(&side_empty[i])));
     }
     *gave_up = 0;
@@ -360,9 +359,9 @@ __global__ void __launch_bounds__(THREADS, 1)
         asm volatile("fence.proxy.async;" ::: "memory");
         const int x = it.step & 1;
         const CUtensorMap* p = &maps.m[it.phase == GRAM ? WIDE_X + x : it.phase == POLY ? WIDE_A : WIDE_B];
-        const CUtensorMap* q = it.phase == UPDATE ? &maps.m[MAP_X + x]
+        const CUtensorMap* q = it.phase == UPDATE ? &maps.m[NARROW_X + x]
                                : TILE::QN == 128  ? p
-                                                  : &maps.m[it.phase == GRAM ? MAP_X + x : MAP_A];
+                                                  : &maps.m[it.phase == GRAM ? NARROW_X + x : NARROW_A];
         const int kblocks = ((it.phase == GRAM ? a.n : a.m) + BK - 1) / BK;
         const int p0 = it.row * TILE::M + rank * 128;
         const int q0 = it.col * BN + rank * TILE::QN;
@@ -473,9 +472,9 @@ __global__ void __launch_bounds__(THREADS, 1)
       }
     }
   } else if (warp < LOADER) {  // epilogues
-    const int quad = warp & 3, part = (warp - 2) >> 2;  // 32 rows, 32 columns of a chunk
+    const int quad = warp & 3, part = (warp - 2) >> 2;  // 32 rows; every other chunk
     const int r = quad * 32 + lane;
-    const unsigned swizzle = (r & 7) << 4;
+    const unsigned swizzle = ((r >> 1) & 3) << 4;
     int c = 0, e = 0;   // accumulators, chunks used so far
     bool dead = false;  // a wait ran out: the rest of the list is walked without work, the result shows it
     for (int t = first; t < items; t += stride, ++c) {
@@ -486,111 +485,98 @@ __global__ void __launch_bounds__(THREADS, 1)
       const long long row_all = static_cast<long long>(it.mat) * a.m + row;
       const bool last = it.phase == UPDATE && it.step + 1 == a.steps;
       const bool mirror = it.phase != UPDATE && it.col / TILE::RATIO != it.row;
-      const StepScale sc = a.step[it.step];
-      float d = 0.0f;
-      for (int ch = 0; ch < chunks; ++ch, ++e) {
-        const int b = e % SIDES;
-        if (!dead && !bar_wait(&side_full[b], (e / SIDES) & 1, gave_up)) dead = true;
-        if (ch == 0) {
-          if (row_in && it.phase != GRAM) d = __ldcg((it.phase == POLY ? a.da : a.db) + row_all);
-          if (!dead && !bar_wait(&acc_full[c & 1], (c / 2) & 1, gave_up)) dead = true;
+      // X = p X + q (acc + d X_hi);  B = p A + q (acc + (d_row + d_col) A);  A = q acc
+      const StepScale& sc = a.step[it.step];
+      const float p = it.phase == UPDATE ? sc.up_p : sc.poly_p;
+      const float q = it.phase == UPDATE ? sc.up_q : it.phase == POLY ? sc.poly_q : sc.gram;
+      bool waited = false;  // for the accumulator: after the loads below are under way
+      auto wait_acc = [&] {
+        if (!dead && !bar_wait(&acc_full[c & 1], (c / 2) & 1, gave_up)) dead = true;
+        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+        waited = true;
+      };
+      const unsigned acc = tmem + (static_cast<unsigned>(quad * 32) << 16) + (c & 1) * BN;
+      for (int ch = (e ^ part) & 1; ch < chunks; ch += 2) {
+        const int b = (e + ch) % SIDES;
+        if (!dead && !bar_wait(&side_full[b], ((e + ch) / SIDES) & 1, gave_up)) dead = true;
+        const int col0 = it.col * BN + ch * CHUNK_COLS;
+        const unsigned s0 = smem_u32(side) + b * (2 * CHUNK), s1 = s0 + CHUNK;
+        float d = 0.0f, mine = 0.0f;  // the row's diagonal element; lane j: column j's
+        if (it.phase != GRAM) {
+          if (row_in) d = __ldcg((it.phase == POLY ? a.da : a.db) + row_all);
+          if (it.phase == POLY && col0 + lane < a.m) mine = __ldcg(a.da + static_cast<long long>(it.mat) * a.m + col0 + lane);
         }
+        if (!waited) wait_acc();
         if (dead) {
           *gave_up = 1;
           atomicExch(a.err, 5);
         }
-        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-        const int col0 = it.col * BN + ch * 64 + part * 32;
-        unsigned acc[32];
-        tmem_ld32(tmem + (static_cast<unsigned>(quad * 32) << 16) + (c & 1) * BN + ch * 64 + part * 32, acc);
-        const float mine = it.phase == POLY && col0 + lane < a.m
-                               ? __ldcg(a.da + static_cast<long long>(it.mat) * a.m + col0 + lane)
-                               : 0.0f;  // lane j: column j's diagonal element
-        asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
-        if (ch + 1 == chunks) {  // the accumulator is free
-          asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
-          __syncwarp();
-          if (lane == 0 && !dead) {
-            const unsigned bar = CTAS == 1 ? smem_u32(&acc_empty[c & 1]) : in_block(smem_u32(&acc_empty[c & 1]), 0);
-            asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
-          }
-        }
-        const unsigned s0 = smem_u32(side) + b * (2 * CHUNK), s1 = s0 + CHUNK;
-        float v[32];
-#pragma unroll
-        for (int g = 0; g < 4; ++g) {  // 8 columns
-          const unsigned at = r * 128 + ((part * 64 + g * 16) ^ swizzle);
+#pragma unroll 1
+        for (int g = 0; g < CHUNK_COLS / 8; ++g) {
+          float v[8];
+          tmem_ld8(acc + ch * CHUNK_COLS + g * 8, v);
+          const unsigned at = r * (2 * CHUNK_COLS) + ((g * 16) ^ swizzle);
           uint4 x = make_uint4(0, 0, 0, 0), y = x;
           if (it.phase != GRAM) x = lds128(s0 + at);
           if (it.phase == UPDATE) y = lds128(s1 + at);
-          unsigned xs[4] = {x.x, x.y, x.z, x.w}, ys[4] = {y.x, y.y, y.z, y.w};
+          const unsigned xs[4] = {x.x, x.y, x.z, x.w}, ys[4] = {y.x, y.y, y.z, y.w};
+          const int diagonal = it.phase == UPDATE ? -1 : row - col0 - g * 8;  // which of the 8, if one
+          float on_diagonal = 0.0f;
 #pragma unroll
-          for (int k = 0; k < 4; ++k) {
-            const int j = 8 * g + 2 * k;
-            const float2 xh = halves(xs[k]), xl = halves(ys[k]);
-            const float s_0 = __uint_as_float(acc[j]), s_1 = __uint_as_float(acc[j + 1]);
-            if (it.phase == GRAM) {
-              v[j] = s_0 * sc.gram;
-              v[j + 1] = s_1 * sc.gram;
-            } else if (it.phase == POLY) {
-              // B = p A + q (A_o A_o + (d_row + d_col) A_o), A_o without its diagonal d
-              v[j] = sc.poly_p * xh.x + sc.poly_q * (s_0 + (d + __shfl_sync(0xffffffffu, mine, j)) * xh.x);
-              v[j + 1] = sc.poly_p * xh.y + sc.poly_q * (s_1 + (d + __shfl_sync(0xffffffffu, mine, j + 1)) * xh.y);
-            } else {
-              // X = p X + q (B_o X_hi + d X_hi)
-              v[j] = sc.up_p * (xh.x + xl.x) + sc.up_q * (s_0 + d * xh.x);
-              v[j + 1] = sc.up_p * (xh.y + xl.y) + sc.up_q * (s_1 + d * xh.y);
+          for (int k = 0; k < 8; k += 2) {
+            const float2 xh = halves(xs[k / 2]), xl = halves(ys[k / 2]);
+            if (k == diagonal) on_diagonal = v[k];
+            if (k + 1 == diagonal) on_diagonal = v[k + 1];
+            const float d0 = it.phase == POLY ? d + __shfl_sync(0xffffffffu, mine, g * 8 + k) : d;
+            const float d1 = it.phase == POLY ? d + __shfl_sync(0xffffffffu, mine, g * 8 + k + 1) : d;
+            v[k] = fmaf(p, xh.x + xl.x, q * fmaf(d0, xh.x, v[k]));
+            v[k + 1] = fmaf(p, xh.y + xl.y, q * fmaf(d1, xh.y, v[k + 1]));
+            if (k == diagonal) v[k] = 0.0f;
+            if (k + 1 == diagonal) v[k + 1] = 0.0f;
+          }
+          if (diagonal >= 0 && diagonal < 8 && row_in) {
+            if (it.phase == GRAM)
+              a.da[row_all] = q * on_diagonal;
+            else
+              a.db[row_all] = fmaf(p, d, q * fmaf(d, d, on_diagonal));
+          }
+          if (last) {
+            if (dead) {
+#pragma unroll
+              for (int j = 0; j < 8; ++j) v[j] = __int_as_float(0x7fffffff);
             }
+            const int inside = row_in ? a.n - col0 - g * 8 : 0;
+            if (inside > 0) store_result(a, it.mat, row, col0 + g * 8, v, inside);
+            continue;
+          }
+          unsigned w[4];
+#pragma unroll
+          for (int k = 0; k < 4; ++k) w[k] = packed(v[2 * k], v[2 * k + 1]);
+          sts128(s0 + at, make_uint4(w[0], w[1], w[2], w[3]));
+          if (it.phase == UPDATE) {
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+              const float2 h = halves(w[k]);
+              w[k] = packed(v[2 * k] - h.x, v[2 * k + 1] - h.y);
+            }
+            sts128(s1 + at, make_uint4(w[0], w[1], w[2], w[3]));
+          } else if (mirror) {  // rows and columns exchanged: 32 rows of 64 columns for each 64 rows here
+#pragma unroll
+            for (int j = 0; j < 8; ++j)
+              sts16(s1 + (r >> 6) * (CHUNK / 2) + (g * 8 + j) * 128 + (((r & 63) * 2) ^ (j << 4)), v[j]);
           }
         }
-        if (it.phase != UPDATE && row >= col0 && row < col0 + 32) {  // this row's diagonal element
-#pragma unroll
-          for (int j = 0; j < 32; ++j)
-            if (col0 + j == row) {
-              if (row_in) {
-                if (it.phase == GRAM)
-                  a.da[row_all] = v[j];
-                else
-                  a.db[row_all] = sc.poly_p * d + sc.poly_q * (__uint_as_float(acc[j]) + d * d);
-              }
-              v[j] = 0.0f;
-            }
-        }
-        if (last) {
-          const int inside = row_in ? a.n - col0 : 0;
-          if (dead) {
-#pragma unroll
-            for (int j = 0; j < 32; ++j) v[j] = __int_as_float(0x7fffffff);
-          }
-          if (inside > 0) store_result(a, it.mat, row, col0, v, inside);
-        } else {
-#pragma unroll
-          for (int g = 0; g < 4; ++g) {
-            const unsigned at = r * 128 + ((part * 64 + g * 16) ^ swizzle);
-            unsigned w[4];
-#pragma unroll
-            for (int k = 0; k < 4; ++k) w[k] = packed(v[8 * g + 2 * k], v[8 * g + 2 * k + 1]);
-            sts128(s0 + at, make_uint4(w[0], w[1], w[2], w[3]));
-            if (it.phase == UPDATE) {
-#pragma unroll
-              for (int k = 0; k < 4; ++k) {
-                const float2 h = halves(w[k]);
-                w[k] = packed(v[8 * g + 2 * k] - h.x, v[8 * g + 2 * k + 1] - h.y);
-              }
-              sts128(s1 + at, make_uint4(w[0], w[1], w[2], w[3]));
-            }
-          }
-          if (mirror) {  // rows and columns exchanged: a box for each 64 rows
-#pragma unroll
-            for (int j = 0; j < 32; ++j) {
-              const unsigned cc = part * 32 + j;
-              sts16(s1 + (r >> 6) * BOX + cc * 128 + (((r & 63) * 2) ^ ((cc & 7) << 4)), v[j]);
-            }
-          }
-          asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-        }
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
         __syncwarp();
         if (lane == 0) bar_arrive(&side_done[b]);
+      }
+      e += chunks;
+      if (!waited) wait_acc();
+      asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+      __syncwarp();
+      if (lane == 0 && !dead) {  // the accumulator is free
+        const unsigned bar = CTAS == 1 ? smem_u32(&acc_empty[c & 1]) : in_block(smem_u32(&acc_empty[c & 1]), 0);
+        asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
       }
     }
   } else if (warp == LOADER) {
@@ -616,17 +602,16 @@ __global__ void __launch_bounds__(THREADS, 1)
             break;
           }
           const unsigned s0 = smem_u32(side) + b * (2 * CHUNK), bar = smem_u32(&side_full[b]);
-          const int col = it.col * BN + ch * 64;
+          const int col = it.col * BN + ch * CHUNK_COLS;
           if (it.phase == GRAM) {
             bar_arrive(&side_full[b]);
           } else if (it.phase == POLY) {
             bar_expect(&side_full[b], CHUNK);
-            for (int h = 0; h < 2; ++h) box_load(&maps.m[MAP_A], s0 + h * BOX, bar, col, row + 64 * h, it.mat);
+            box_load(&maps.m[CHUNK_A], s0, bar, col, row, it.mat);
           } else {
             bar_expect(&side_full[b], 2 * CHUNK);
-            const CUtensorMap* x = &maps.m[MAP_X + (it.step & 1)];
-            for (int h = 0; h < 2; ++h) box_load(x, s0 + h * BOX, bar, col, row + 64 * h, it.mat);
-            for (int h = 0; h < 2; ++h) box_load(&maps.m[MAP_LO], s0 + CHUNK + h * BOX, bar, col, row + 64 * h, it.mat);
+            box_load(&maps.m[CHUNK_X + (it.step & 1)], s0, bar, col, row, it.mat);
+            box_load(&maps.m[CHUNK_LO], s0 + CHUNK, bar, col, row, it.mat);
           }
         }
       }
@@ -642,7 +627,8 @@ __global__ void __launch_bounds__(THREADS, 1)
         const bool mirror = it.phase != UPDATE && it.col / TILE::RATIO != it.row;
         const int row = it.row * TILE::M + rank * 128;
         const CUtensorMap* to =
-            &maps.m[it.phase == GRAM ? MAP_A : it.phase == POLY ? MAP_B : MAP_X + ((it.step + 1) & 1)];
+            &maps.m[it.phase == GRAM ? CHUNK_A : it.phase == POLY ? CHUNK_B : CHUNK_X + ((it.step + 1) & 1)];
+        const CUtensorMap* turned = &maps.m[it.phase == GRAM ? TURNED_A : TURNED_B];
         for (int ch = 0; ch < chunks; ++ch, ++e) {
           const int b = e % SIDES;
           if (!bar_wait(&side_done[b], (e / SIDES) & 1, gave_up)) {
@@ -657,13 +643,13 @@ __global__ void __launch_bounds__(THREADS, 1)
           }
           if (!last) {
             const unsigned s0 = smem_u32(side) + b * (2 * CHUNK), s1 = s0 + CHUNK;
-            const int col = it.col * BN + ch * 64;
+            const int col = it.col * BN + ch * CHUNK_COLS;
+            if (row < a.m) {
+              box_store(to, s0, col, row, it.mat);
+              if (it.phase == UPDATE) box_store(&maps.m[CHUNK_LO], s1, col, row, it.mat);
+            }
             for (int h = 0; h < 2; ++h)
-              if (row + 64 * h < a.m) {
-                box_store(to, s0 + h * BOX, col, row + 64 * h, it.mat);
-                if (it.phase == UPDATE) box_store(&maps.m[MAP_LO], s1 + h * BOX, col, row + 64 * h, it.mat);
-                if (mirror) box_store(to, s1 + h * BOX, row + 64 * h, col, it.mat);
-              }
+              if (mirror && row + 64 * h < a.m) box_store(turned, s1 + h * (CHUNK / 2), row + 64 * h, col, it.mat);
             asm volatile("cp.async.bulk.commit_group;" ::: "memory");
             asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
           }
@@ -710,6 +696,8 @@ struct LoadArgs {
   float eps, scale;
   double* part;
   __half *hi, *lo;
+  int* err;
+  unsigned* ready;
 };
 
 // V adjacent elements of a run.
@@ -724,12 +712,17 @@ __device__ __forceinline__ void load_run(const LoadArgs& a, const T* p, float (&
   }
 }
 
-// A share of a matrix's sum of squares, in 64 bits: no scale of the update overflows.
+// A share of a matrix's sum of squares, in 64 bits: no scale of the update
+// overflows.  Clears the counters of the products on the way.
 template <typename T, int V>
 __global__ void __launch_bounds__(256) ns_norm(const __grid_constant__ LoadArgs a) {
   constexpr int U = 4;  // loads in flight
   __shared__ double buf[8];
   const long long mat = blockIdx.y;
+  if (blockIdx.x == 0 && threadIdx.x == 0) {
+    a.ready[mat] = 0;
+    if (mat == 0) *a.err = 0;
+  }
   const T* g = static_cast<const T*>(a.g) + mat * a.batch;
   const unsigned per = a.inner / V;
   const long long total = static_cast<long long>(a.outer) * per, step = static_cast<long long>(gridDim.x) * 256;
@@ -747,13 +740,24 @@ __global__ void __launch_bounds__(256) ns_norm(const __grid_constant__ LoadArgs 
         for (int j = 0; j < V; ++j) x[u][j] = 0.0f;
       }
     }
+    // squares of a few in 32 bits where that can neither overflow nor vanish
+    // (conversions to 64 bits would take longer than the loads: 88 us for 200 MB)
+    float q = 0.0f;
 #pragma unroll
     for (int u = 0; u < U; ++u)
 #pragma unroll
-      for (int j = 0; j < V; ++j) {
-        const double y = x[u][j];
-        s = fma(y, y, s);
-      }
+      for (int j = 0; j < V; ++j) q = fmaf(x[u][j], x[u][j], q);
+    if (q > 1e-25f && q < 1e37f) {
+      s += q;
+    } else {
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+#pragma unroll
+        for (int j = 0; j < V; ++j) {
+          const double y = x[u][j];
+          s = fma(y, y, s);
+        }
+    }
   }
 #pragma unroll
   for (int o = 16; o; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
@@ -855,7 +859,7 @@ Layout plan(long long count, long long rows, long long cols) {
     at += (bytes + 255) / 256 * 256;
     return here;
   };
-  l.head = take(256 + 4ull * count);  // the error word, then the counters: zeros at the start
+  l.head = take(256 + 4ull * count);  // the error word, then the counters
   l.part = take(sizeof(double) * NORM_BLOCKS * count);
   for (size_t& t : l.hi) t = take(2ull * count * l.m * l.ldx);
   l.lo = take(2ull * count * l.m * l.ldx);
@@ -907,13 +911,16 @@ Scales scales_for(int steps, const float* coef) {
   return s;
 }
 
-// The list's tiles for one tile size, and its time in clocks as estimated from
-// the cost of 64 elements of K and of a wait for another block's tile: the work
-// shared by all blocks, or one matrix's products one after the other.
+// The list's tiles for one tile size, and a step's time in us as estimated from
+// measured costs of a tile's 64 elements of K and of a product's start and end:
+// the work shared by all blocks, or one matrix's products one after the other.
+// What a block can bring from L2 (70 to 80 GB/s) bounds the first, so that a
+// large tile costs hardly more than a small one and is taken where there are
+// enough of them.
 struct Tiling {
   long long sym, up;
   int row_tiles, sym_cols;
-  double clocks;
+  double us;
 };
 template <typename TILE>
 Tiling tiling(long long count, long long m, long long n, int workers, double per_kblock) {
@@ -926,8 +933,8 @@ Tiling tiling(long long count, long long m, long long n, int workers, double per
   const double kn = static_cast<double>((n + BK - 1) / BK), km = static_cast<double>((m + BK - 1) / BK);
   const double shared = per_kblock * count * (t.sym * (kn + km) + t.up * km) / workers;
   auto rounds = [&](long long tiles) { return static_cast<double>((tiles + workers - 1) / workers); };
-  const double alone = per_kblock * (rounds(t.sym) * (kn + km) + rounds(t.up) * km) + 3 * 3500.0;
-  t.clocks = std::fmax(shared, alone);
+  const double alone = per_kblock * (rounds(t.sym) * (kn + km) + rounds(t.up) * km) + 3 * 6.0;
+  t.us = std::fmax(shared, alone);
   return t;
 }
 
@@ -1013,11 +1020,11 @@ extern "C" int ad_orthogonalize(int device, int dtype, const void* g, int64_t co
   la.lo = reinterpret_cast<__half*>(w + l.lo);
   const bool vec = la.inner_stride == 1 && la.inner % 4 == 0 && la.outer_stride % 4 == 0 && batch_stride % 4 == 0 &&
                    aligned(g, 4 * elem_size(dtype));
-  cudaError_t e = cudaMemsetAsync(w, 0, 256 + 4ull * count, st);
-  if (e == cudaSuccess)
-    e = dtype == AD_F32    ? (vec ? load<float, 4>(la, num, st) : load<float, 1>(la, num, st))
-        : dtype == AD_BF16 ? (vec ? load<__nv_bfloat16, 4>(la, num, st) : load<__nv_bfloat16, 1>(la, num, st))
-                           : (vec ? load<__half, 4>(la, num, st) : load<__half, 1>(la, num, st));
+  la.err = reinterpret_cast<int*>(w);
+  la.ready = reinterpret_cast<unsigned*>(w + 256);
+  cudaError_t e = dtype == AD_F32    ? (vec ? load<float, 4>(la, num, st) : load<float, 1>(la, num, st))
+                  : dtype == AD_BF16 ? (vec ? load<__nv_bfloat16, 4>(la, num, st) : load<__nv_bfloat16, 1>(la, num, st))
+                                     : (vec ? load<__half, 4>(la, num, st) : load<__half, 1>(la, num, st));
   if (e != cudaSuccess) return fail("ad_orthogonalize: %s", cudaGetErrorString(e));
 
   NsArgs s = {};
@@ -1027,8 +1034,7 @@ extern "C" int ad_orthogonalize(int device, int dtype, const void* g, int64_t co
   s.lo = la.lo;
   s.da = reinterpret_cast<float*>(w + l.da);
   s.db = reinterpret_cast<float*>(w + l.db);
-  s.err = reinterpret_cast<int*>(w);
-  s.ready = reinterpret_cast<unsigned*>(w + 256);
+  s.err = la.err, s.ready = la.ready;
   s.out = out, s.out_type = out_dtype;
   s.out_batch = out_batch_stride;
   s.out_row = tall ? out_col_stride : out_row_stride, s.out_col = tall ? out_row_stride : out_col_stride;
@@ -1048,19 +1054,31 @@ extern "C" int ad_orthogonalize(int device, int dtype, const void* g, int64_t co
                  static_cast<float>(a * up), static_cast<float>(up / sb)};
   }
   Maps maps;
-  const void* const base[MAPS] = {s.hi[0], s.hi[1], s.lo, w + l.a, w + l.b, s.hi[0], s.hi[1], w + l.a, w + l.b};
-  for (int k = 0; k < MAPS; ++k) {
-    const bool of_x = k <= MAP_LO || k == WIDE_X || k == WIDE_X + 1;
-    if (ad_b200_internal::tmap_3d_16(base[k], count, m, of_x ? n : m, of_x ? l.ldx : l.lda, k < WIDE_X ? 64 : 128, BK, &maps.m[k]))
-      return 1;
+  void* const xh[2] = {w + l.hi[0], w + l.hi[1]};
+  void* const ab[2] = {w + l.a, w + l.b};
+  int bad = 0;
+  auto map = [&](int k, const void* base, bool of_x, int box_rows, int box_cols, int swizzle) {
+    bad |= ad_b200_internal::tmap_3d_16(base, count, m, of_x ? n : m, of_x ? l.ldx : l.lda, box_rows, box_cols, swizzle,
+                                        &maps.m[k]);
+  };
+  for (int k = 0; k < 2; ++k) {
+    map(WIDE_X + k, xh[k], true, 128, BK, 128);
+    map(WIDE_A + k, ab[k], false, 128, BK, 128);
+    map(NARROW_X + k, xh[k], true, 64, BK, 128);
+    map(CHUNK_X + k, xh[k], true, 128, CHUNK_COLS, 2 * CHUNK_COLS);
+    map(CHUNK_A + k, ab[k], false, 128, CHUNK_COLS, 2 * CHUNK_COLS);
+    map(TURNED_A + k, ab[k], false, CHUNK_COLS, 64, 128);
   }
+  map(NARROW_A, ab[0], false, 64, BK, 128);
+  map(CHUNK_LO, s.lo, true, 128, CHUNK_COLS, 2 * CHUNK_COLS);
+  if (bad) return 1;
 
   const int sms = sm_count(guard.device());
   if (!sms) return fail("ad_orthogonalize: no device properties");
-  const Tiling big = tiling<Tile<2, 256>>(count, m, n, sms / 2, 512.0);
-  const Tiling mid = tiling<Tile<1, 128>>(count, m, n, sms, 307.0);
-  const Tiling small = tiling<Tile<1, 64>>(count, m, n, sms, 192.0);
-  const Tiling& best = big.clocks <= mid.clocks && big.clocks <= small.clocks ? big : mid.clocks <= small.clocks ? mid : small;
+  const Tiling big = tiling<Tile<2, 256>>(count, m, n, sms / 2, 0.45);
+  const Tiling mid = tiling<Tile<1, 128>>(count, m, n, sms, 0.37);
+  const Tiling small = tiling<Tile<1, 64>>(count, m, n, sms, 0.35);
+  const Tiling& best = big.us <= mid.us && big.us <= small.us ? big : mid.us <= small.us ? mid : small;
   if (steps * count * (2 * best.sym + best.up) > 0x3fffffffll) return fail("ad_orthogonalize: too many tiles in one call");
   e = &best == &big   ? start<2, 256>(maps, s, best, sms, guard.device(), st)
       : &best == &mid ? start<1, 128>(maps, s, best, sms, guard.device(), st)

@@ -176,7 +176,7 @@ namespace ad_b200_internal {
 void set_error(const char* msg) { g_err = msg; }
 
 int tmap_3d_16(const void* base, uint64_t count, uint64_t rows, uint64_t cols, uint64_t ld, uint32_t box_rows,
-               uint32_t box_cols, void* out128) {
+               uint32_t box_cols, int swizzle_bytes, void* out128) {
   if (driver()) return 1;
   cuuint64_t dims[3] = {cols, rows, count};
   cuuint64_t strides[2] = {2 * ld, 2 * ld * rows};
@@ -184,7 +184,8 @@ int tmap_3d_16(const void* base, uint64_t count, uint64_t rows, uint64_t cols, u
   cuuint32_t estr[3] = {1, 1, 1};
   CUresult r = g_drv.tensorMapEncodeTiled(
       reinterpret_cast<CUtensorMap*>(out128), CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 3, const_cast<void*>(base), dims,
-      strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+      strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+      swizzle_bytes == 64 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_128B,
       CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   if (r != CUDA_SUCCESS) return cu_fail(r, "cuTensorMapEncodeTiled");
   return 0;

@@ -6,9 +6,12 @@
 // are (x[i], x[i + rotary/2]) in the half layout and (x[2i], x[2i+1]) in the
 // interleaved one; the rest of the head is copied.
 //
-// Bound by memory: three operations a value.  One block takes one token, its
-// threads the vectors of a head (x) and the heads (y), so that a thread reads
-// its cosines and sines once and keeps them for all its heads.
+// Bound by memory: three operations a value.  A thread takes the same vector of
+// several heads of one token, so that it reads its cosines and sines once and
+// keeps them for all of these heads; the heads' loads are in flight before the
+// token's position and its row of the tables are asked for.
+#include <algorithm>
+
 #include "ops_common.cuh"
 
 namespace {
@@ -26,90 +29,153 @@ struct RotaryArgs {
   long long pos_seq, pos_tok;
   int pos64;
   long long table_rows;
-  long long tokens;
+  long long rows, tokens;  // sequences x tokens, tokens
   int dim, half;
+  unsigned head_groups;  // a thread takes every so-many-th head
   float sign;
 };
 
-// V: elements a load moves; 1 where sizes or addresses allow no more.
-template <typename T, int V, bool HALF>
-__global__ void __launch_bounds__(256) rotary_kernel(const __grid_constant__ RotaryArgs a) {
-  const long long row = blockIdx.x;
-  const long long b = row / a.tokens, t = row - b * a.tokens;
-  const long long at = b * a.pos_seq + t * a.pos_tok;
-  const long long p =
-      a.pos64 ? static_cast<const long long*>(a.positions)[at] : static_cast<const int*>(a.positions)[at];
-  const bool known = p >= 0 && p < a.table_rows;
-  const float nan = __int_as_float(0x7fffffff);
-  // Units of a head: pair units first, then units of copied elements.
-  constexpr int PV = HALF ? V : (V > 1 ? V / 2 : 1);  // pairs of a unit
-  const int pair_units = a.half / PV;
-  const int units = pair_units + (a.dim - 2 * a.half) / V;
-  const int heads = a.heads[0] + a.heads[1];
-  for (int u = threadIdx.x; u < units; u += blockDim.x) {
-    const bool turned = u < pair_units;
-    float c[PV], s[PV];
-    if (turned) {
+// A group of threads, one for each unit of a head, works on a token's every
+// so-many-th head; a block has as many groups as 256 threads make.
+// HALVES: a unit is two vectors, one from each half of the rotated part, whose
+//   halves are whole vectors.
+// PAIRS: a unit is a vector; interleaved pairs lie within it.
+// ACROSS: a unit is a vector of the half layout whose halves are not whole
+//   vectors; its elements' partners are read one by one (from L1: their own
+//   thread reads them too), all of a round's before any result is stored, so
+//   that the result may be the operand.
+enum Units { HALVES, PAIRS, ACROSS };
+
+// Heads whose loads a thread has in flight together: four vectors, or what fits
+// the registers of 1024 threads a multiprocessor.
+template <Units U>
+__host__ __device__ constexpr int heads_at_once() {
+  return U == PAIRS ? 4 : 2;
+}
+
+template <typename T, int V, Units U>
+__global__ void __launch_bounds__(256, 4) rotary_kernel(const __grid_constant__ RotaryArgs a) {
+  constexpr int N = heads_at_once<U>();
+  constexpr int C = U == PAIRS ? V / 2 : V;
+  const unsigned group = blockIdx.x * blockDim.y + threadIdx.y;
+  const unsigned row = group / a.head_groups, h0 = group - row * a.head_groups;
+  const bool here = row < static_cast<unsigned>(a.rows);
+  const unsigned tokens = static_cast<unsigned>(a.tokens), seq = here ? row / tokens : 0;
+  const long long b = seq, t = here ? row - seq * tokens : 0;
+  const unsigned heads = a.heads[0] + a.heads[1];
+  const int i = threadIdx.x * V;  // the unit's first element
+  const int rot = 2 * a.half;
+  const bool copies = U == HALVES ? i >= a.half : i >= rot;
+  const int at = U == HALVES && copies ? i + a.half : i;
+  float c[C], s[C];
+  Vec<T, V> xu[N], xv[U == HALVES ? N : 1];
+  float other[U == ACROSS ? N : 1][V];
 #pragma unroll
-      for (int j = 0; j < PV; ++j) {
-        c[j] = known ? a.cos[p * a.half + u * PV + j] : nan;
-        s[j] = known ? a.sign * a.sin[p * a.half + u * PV + j] : nan;
+  for (int n = 0; n < N; ++n) {
+    const unsigned h = h0 + n * a.head_groups;
+    if (!here || h >= heads) continue;
+    const int w = h >= static_cast<unsigned>(a.heads[0]);
+    const T* x = static_cast<const T*>(a.in[w]) + b * a.is[w][0] + t * a.is[w][1] +
+                 static_cast<long long>(w ? h - a.heads[0] : h) * a.is[w][2];
+    xu[n] = load_vec<T, V>(x + at);
+    if (U == HALVES && !copies) xv[n] = load_vec<T, V>(x + at + a.half);
+    if (U == ACROSS) {
+#pragma unroll
+      for (int j = 0; j < V; ++j) {
+        const int e = i + j;
+        other[n][j] = e < rot ? to_float(x[e < a.half ? e + a.half : e - a.half]) : 0.0f;
       }
     }
+  }
+  if (here) {  // behind the heads' loads
+    const long long pa = b * a.pos_seq + t * a.pos_tok;
+    const long long p =
+        a.pos64 ? static_cast<const long long*>(a.positions)[pa] : static_cast<const int*>(a.positions)[pa];
+    const bool known = p >= 0 && p < a.table_rows;
+    const long long at_row = known ? p * a.half : 0;
+#pragma unroll
+    for (int j = 0; j < C; ++j) {
+      const int e = U == PAIRS ? i / 2 + j : i + j;
+      const int k = U == ACROSS && e >= a.half ? e - a.half : e;
+      const bool turned = known && (U == ACROSS ? e < rot : e < a.half);
+      c[j] = turned ? __ldg(a.cos + at_row + k) : __int_as_float(0x7fffffff);
+      s[j] = turned ? a.sign * __ldg(a.sin + at_row + k) : __int_as_float(0x7fffffff);
+      if (U == ACROSS && e < a.half) s[j] = -s[j];
+    }
+  }
+  if (U == ACROSS) __syncthreads();
+#pragma unroll
+  for (int n = 0; n < N; ++n) {
+    const unsigned h = h0 + n * a.head_groups;
+    if (!here || h >= heads) continue;
+    const int w = h >= static_cast<unsigned>(a.heads[0]);
+    T* y = static_cast<T*>(a.out[w]) + b * a.os[w][0] + t * a.os[w][1] +
+           static_cast<long long>(w ? h - a.heads[0] : h) * a.os[w][2];
+    if (copies) {
+      store_vec<T, V>(y + at, xu[n]);
+    } else if (U == HALVES) {
+      Vec<T, V> yu, yv;
+#pragma unroll
+      for (int j = 0; j < V; ++j) {
+        const float fu = to_float(xu[n].v[j]), fv = to_float(xv[n].v[j]);
+        yu.v[j] = from_float<T>(fu * c[j] - fv * s[j]);
+        yv.v[j] = from_float<T>(fv * c[j] + fu * s[j]);
+      }
+      store_vec<T, V>(y + at, yu);
+      store_vec<T, V>(y + at + a.half, yv);
+    } else if (U == PAIRS) {
+#pragma unroll
+      for (int j = 0; j < C; ++j) {
+        const float fu = to_float(xu[n].v[2 * j]), fv = to_float(xu[n].v[2 * j + 1]);
+        if (i + 2 * j < rot) {
+          xu[n].v[2 * j] = from_float<T>(fu * c[j] - fv * s[j]);
+          xu[n].v[2 * j + 1] = from_float<T>(fv * c[j] + fu * s[j]);
+        }
+      }
+      store_vec<T, V>(y + at, xu[n]);
+    } else {
+#pragma unroll
+      for (int j = 0; j < V; ++j)
+        if (i + j < rot) xu[n].v[j] = from_float<T>(to_float(xu[n].v[j]) * c[j] + other[n][j] * s[j]);
+      store_vec<T, V>(y + at, xu[n]);
+    }
+  }
+}
+
+// The same an element and its partner at a time, whatever the alignment; a
+// block takes one token.
+template <typename T, bool HALF>
+__global__ void __launch_bounds__(256) rotary_single_kernel(const __grid_constant__ RotaryArgs a) {
+  const long long row = blockIdx.x;
+  const long long b = row / a.tokens, t = row - b * a.tokens;
+  const long long pa = b * a.pos_seq + t * a.pos_tok;
+  const long long p =
+      a.pos64 ? static_cast<const long long*>(a.positions)[pa] : static_cast<const int*>(a.positions)[pa];
+  const bool known = p >= 0 && p < a.table_rows;
+  const int units = a.dim - a.half, heads = a.heads[0] + a.heads[1];  // pairs, then what is copied
+  for (int u = threadIdx.x; u < units; u += blockDim.x) {
+    const bool turned = u < a.half;
+    const float c = turned && known ? a.cos[p * a.half + u] : __int_as_float(0x7fffffff);
+    const float s = turned && known ? a.sign * a.sin[p * a.half + u] : __int_as_float(0x7fffffff);
     for (int h = threadIdx.y; h < heads; h += blockDim.y) {
       const int w = h >= a.heads[0];
-      const int hh = w ? h - a.heads[0] : h;
+      const long long hh = w ? h - a.heads[0] : h;
       const T* x = static_cast<const T*>(a.in[w]) + b * a.is[w][0] + t * a.is[w][1] + hh * a.is[w][2];
       T* y = static_cast<T*>(a.out[w]) + b * a.os[w][0] + t * a.os[w][1] + hh * a.os[w][2];
       if (!turned) {
-        const int i = 2 * a.half + (u - pair_units) * V;
-        store_vec<T, V>(y + i, load_vec<T, V>(x + i));
-      } else if (HALF || V == 1) {
-        const int i = HALF ? u * V : 2 * u, k = HALF ? i + a.half : i + 1;
-        const Vec<T, V> xu = load_vec<T, V>(x + i), xv = load_vec<T, V>(x + k);
-        Vec<T, V> yu, yv;
-#pragma unroll
-        for (int j = 0; j < V; ++j) {
-          const float fu = to_float(xu.v[j]), fv = to_float(xv.v[j]);
-          yu.v[j] = from_float<T>(fu * c[j] - fv * s[j]);
-          yv.v[j] = from_float<T>(fv * c[j] + fu * s[j]);
-        }
-        store_vec<T, V>(y + i, yu);
-        store_vec<T, V>(y + k, yv);
+        y[u + a.half] = x[u + a.half];
       } else {
-        const Vec<T, V> xx = load_vec<T, V>(x + u * V);
-        Vec<T, V> yy;
-#pragma unroll
-        for (int j = 0; j < PV; ++j) {
-          const float fu = to_float(xx.v[(2 * j) % V]), fv = to_float(xx.v[(2 * j + 1) % V]);
-          yy.v[(2 * j) % V] = from_float<T>(fu * c[j] - fv * s[j]);
-          yy.v[(2 * j + 1) % V] = from_float<T>(fv * c[j] + fu * s[j]);
-        }
-        store_vec<T, V>(y + u * V, yy);
+        const int i = HALF ? u : 2 * u, k = HALF ? u + a.half : 2 * u + 1;
+        const float fu = to_float(x[i]), fv = to_float(x[k]);
+        y[i] = from_float<T>(fu * c - fv * s);
+        y[k] = from_float<T>(fv * c + fu * s);
       }
     }
   }
 }
 
-template <typename T, int V>
-cudaError_t launch(const RotaryArgs& a, int layout, long long rows, cudaStream_t s) {
-  const int pv = layout == 0 ? V : (V > 1 ? V / 2 : 1);
-  const int units = a.half / pv + (a.dim - 2 * a.half) / V;
-  const int bx = units < 256 ? units : 256;
-  const int heads = a.heads[0] + a.heads[1];
-  int by = 256 / bx;
-  if (by > heads) by = heads;
-  const dim3 block(bx, by);
-  if (layout == 0)
-    rotary_kernel<T, V, true><<<static_cast<unsigned>(rows), block, 0, s>>>(a);
-  else
-    rotary_kernel<T, V, false><<<static_cast<unsigned>(rows), block, 0, s>>>(a);
-  return cudaGetLastError();
-}
-
-// Whether every vector of V elements that the kernel moves is aligned.
-bool fits(const RotaryArgs& a, int layout, int v, int size) {
-  if (layout == 0 ? a.half % v : (2 * a.half) % v) return false;
+// Whether heads start at multiples of v elements and are made of so many.
+bool whole(const RotaryArgs& a, int v, int size) {
   if (a.dim % v) return false;
   for (int w = 0; w < 2; ++w) {
     if (!a.heads[w]) continue;
@@ -120,12 +186,40 @@ bool fits(const RotaryArgs& a, int layout, int v, int size) {
   return true;
 }
 
+template <typename T, int V, Units U>
+cudaError_t launch(RotaryArgs a, cudaStream_t s) {
+  const int units = (U == HALVES ? a.dim - a.half : a.dim) / V;
+  const int heads = a.heads[0] + a.heads[1];
+  a.head_groups = static_cast<unsigned>((heads + heads_at_once<U>() - 1) / heads_at_once<U>());
+  const long long groups = a.rows * a.head_groups;
+  if (groups > 0x7fffffffll) return cudaErrorInvalidValue;
+  const int by = 256 / units;
+  rotary_kernel<T, V, U><<<static_cast<unsigned>((groups + by - 1) / by), dim3(units, by), 0, s>>>(a);
+  return cudaGetLastError();
+}
+
+template <typename T, int V>
+bool try_vectors(const RotaryArgs& a, int layout, cudaStream_t s, cudaError_t& e) {
+  if (a.dim / V > 256 || !whole(a, V, sizeof(T))) return false;
+  e = layout == 1          ? launch<T, V, PAIRS>(a, s)
+      : a.half % V == 0    ? launch<T, V, HALVES>(a, s)
+                           : launch<T, V, ACROSS>(a, s);
+  return true;
+}
+
+// 16-byte vectors where the heads allow them, else 8 bytes, else single elements.
 template <typename T>
-cudaError_t dispatch(const RotaryArgs& a, int layout, long long rows, cudaStream_t s) {
-  constexpr int S = sizeof(T), M = 16 / S;
-  if (fits(a, layout, M, S)) return launch<T, M>(a, layout, rows, s);
-  if (fits(a, layout, M / 2, S)) return launch<T, M / 2>(a, layout, rows, s);
-  return launch<T, 1>(a, layout, rows, s);
+cudaError_t dispatch(const RotaryArgs& a, int layout, cudaStream_t s) {
+  constexpr int M = 16 / sizeof(T);
+  cudaError_t e;
+  if (try_vectors<T, M>(a, layout, s, e) || try_vectors<T, M / 2>(a, layout, s, e)) return e;
+  const int units = a.dim - a.half, bx = std::min(units, 256);
+  const int by = std::max(1, std::min(256 / bx, a.heads[0] + a.heads[1]));
+  if (layout == 0)
+    rotary_single_kernel<T, true><<<static_cast<unsigned>(a.rows), dim3(bx, by), 0, s>>>(a);
+  else
+    rotary_single_kernel<T, false><<<static_cast<unsigned>(a.rows), dim3(bx, by), 0, s>>>(a);
+  return cudaGetLastError();
 }
 
 }  // namespace
@@ -169,6 +263,7 @@ extern "C" int ad_rotary(int device, int dtype, const void* q, const int64_t* q_
   a.pos_tok = pos_tok_stride;
   a.pos64 = pos64;
   a.table_rows = table_rows;
+  a.rows = rows;
   a.tokens = tokens;
   a.dim = dim;
   a.half = rotary / 2;
@@ -176,9 +271,9 @@ extern "C" int ad_rotary(int device, int dtype, const void* q, const int64_t* q_
   DeviceGuard g(device);
   if (g.error() != cudaSuccess) return fail("ad_rotary: %s", cudaGetErrorString(g.error()));
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  const cudaError_t e = dtype == AD_F32    ? dispatch<float>(a, layout, rows, s)
-                        : dtype == AD_BF16 ? dispatch<__nv_bfloat16>(a, layout, rows, s)
-                                           : dispatch<__half>(a, layout, rows, s);
+  const cudaError_t e = dtype == AD_F32    ? dispatch<float>(a, layout, s)
+                        : dtype == AD_BF16 ? dispatch<__nv_bfloat16>(a, layout, s)
+                                           : dispatch<__half>(a, layout, s);
   if (e != cudaSuccess) return fail("ad_rotary: %s", cudaGetErrorString(e));
   return 0;
 }

@@ -10,6 +10,7 @@
 #include <cstdarg>
 #include <cstdint>
 #include <cstdio>
+#include <cstring>
 
 #include "../../include/ad_b200.h"
 
@@ -90,13 +91,32 @@ template <typename T, int V>
 struct alignas(sizeof(T) * V) Vec {
   T v[V];
 };
+// One instruction each: a copy of 16-bit elements as a structure can fall apart
+// into single ones (rotary positions of 16-bit heads ran at half their speed).
+template <int BYTES>
+struct Word;
+template <>
+struct Word<2> { typedef unsigned short type; };
+template <>
+struct Word<4> { typedef unsigned type; };
+template <>
+struct Word<8> { typedef uint2 type; };
+template <>
+struct Word<16> { typedef uint4 type; };
 template <typename T, int V>
 __device__ __forceinline__ Vec<T, V> load_vec(const T* p) {
-  return *reinterpret_cast<const Vec<T, V>*>(p);
+  typedef typename Word<sizeof(T) * V>::type W;
+  const W w = *reinterpret_cast<const W*>(p);
+  Vec<T, V> x;
+  memcpy(&x, &w, sizeof(w));
+  return x;
 }
 template <typename T, int V>
 __device__ __forceinline__ void store_vec(T* p, const Vec<T, V>& x) {
-  *reinterpret_cast<Vec<T, V>*>(p) = x;
+  typedef typename Word<sizeof(T) * V>::type W;
+  W w;
+  memcpy(&w, &x, sizeof(w));
+  *reinterpret_cast<W*>(p) = w;
 }
 
 // Element i of an array whose type (AD_F32, AD_BF16, AD_F16) is known at run

@@ -31,6 +31,7 @@ struct RotaryArgs {
   long long table_rows;
   long long rows, tokens;  // sequences x tokens, tokens
   int dim, half;
+  int table_vec;         // rows of the tables are whole 16-byte vectors
   unsigned head_groups;  // a thread takes every so-many-th head
   float sign;
 };
@@ -38,23 +39,22 @@ struct RotaryArgs {
 // A group of threads, one for each unit of a head, works on a token's every
 // so-many-th head; a block has as many groups as 256 threads make.
 // HALVES: a unit is two vectors, one from each half of the rotated part, whose
-//   halves are whole vectors.
+//   halves are whole vectors, or two of what is copied.
 // PAIRS: a unit is a vector; interleaved pairs lie within it.
 // ACROSS: a unit is a vector of the half layout whose halves are not whole
-//   vectors; its elements' partners are read one by one (from L1: their own
-//   thread reads them too), all of a round's before any result is stored, so
-//   that the result may be the operand.
+//   vectors; the group puts its heads into shared memory, where each thread
+//   finds its elements' partners.
 enum Units { HALVES, PAIRS, ACROSS };
 
 // Heads whose loads a thread has in flight together: four vectors, or what fits
 // the registers of 1024 threads a multiprocessor.
 template <Units U>
 __host__ __device__ constexpr int heads_at_once() {
-  return U == PAIRS ? 4 : 2;
+  return U == HALVES ? 2 : 4;
 }
 
 template <typename T, int V, Units U>
-__global__ void __launch_bounds__(256, 4) rotary_kernel(const __grid_constant__ RotaryArgs a) {
+__global__ void __launch_bounds__(256, U == HALVES ? 4 : 5) rotary_kernel(const __grid_constant__ RotaryArgs a) {
   constexpr int N = heads_at_once<U>();
   constexpr int C = U == PAIRS ? V / 2 : V;
   const unsigned group = blockIdx.x * blockDim.y + threadIdx.y;
@@ -66,10 +66,15 @@ __global__ void __launch_bounds__(256, 4) rotary_kernel(const __grid_constant__ 
   const int i = threadIdx.x * V;  // the unit's first element
   const int rot = 2 * a.half;
   const bool copies = U == HALVES ? i >= a.half : i >= rot;
+  // HALVES: where the unit's two vectors start; what is copied is shared out by twos as well
+  const int left = (a.dim - rot) / V, spread = (left + 1) / 2 * V;
   const int at = U == HALVES && copies ? i + a.half : i;
+  const int at2 = copies ? at + spread : at + a.half;
+  const bool two = U == HALVES && at2 < a.dim;
   float c[C], s[C];
   Vec<T, V> xu[N], xv[U == HALVES ? N : 1];
-  float other[U == ACROSS ? N : 1][V];
+  extern __shared__ __align__(16) unsigned char raw[];
+  T* const mine = reinterpret_cast<T*>(raw) + threadIdx.y * N * a.dim;  // ACROSS: the group's heads
 #pragma unroll
   for (int n = 0; n < N; ++n) {
     const unsigned h = h0 + n * a.head_groups;
@@ -78,14 +83,8 @@ __global__ void __launch_bounds__(256, 4) rotary_kernel(const __grid_constant__ 
     const T* x = static_cast<const T*>(a.in[w]) + b * a.is[w][0] + t * a.is[w][1] +
                  static_cast<long long>(w ? h - a.heads[0] : h) * a.is[w][2];
     xu[n] = load_vec<T, V>(x + at);
-    if (U == HALVES && !copies) xv[n] = load_vec<T, V>(x + at + a.half);
-    if (U == ACROSS) {
-#pragma unroll
-      for (int j = 0; j < V; ++j) {
-        const int e = i + j;
-        other[n][j] = e < rot ? to_float(x[e < a.half ? e + a.half : e - a.half]) : 0.0f;
-      }
-    }
+    if (two) xv[n] = load_vec<T, V>(x + at2);
+    if (U == ACROSS) store_vec<T, V>(mine + n * a.dim + i, xu[n]);
   }
   if (here) {  // behind the heads' loads
     const long long pa = b * a.pos_seq + t * a.pos_tok;
@@ -93,14 +92,25 @@ __global__ void __launch_bounds__(256, 4) rotary_kernel(const __grid_constant__ 
         a.pos64 ? static_cast<const long long*>(a.positions)[pa] : static_cast<const int*>(a.positions)[pa];
     const bool known = p >= 0 && p < a.table_rows;
     const long long at_row = known ? p * a.half : 0;
+    const int first = U == PAIRS ? i / 2 : i;
+    if (U != ACROSS && C % 4 == 0 && a.table_vec && known && first + C <= a.half) {
 #pragma unroll
-    for (int j = 0; j < C; ++j) {
-      const int e = U == PAIRS ? i / 2 + j : i + j;
-      const int k = U == ACROSS && e >= a.half ? e - a.half : e;
-      const bool turned = known && (U == ACROSS ? e < rot : e < a.half);
-      c[j] = turned ? __ldg(a.cos + at_row + k) : __int_as_float(0x7fffffff);
-      s[j] = turned ? a.sign * __ldg(a.sin + at_row + k) : __int_as_float(0x7fffffff);
-      if (U == ACROSS && e < a.half) s[j] = -s[j];
+      for (int j = 0; j < C; j += 4) {
+        const float4 w = __ldg(reinterpret_cast<const float4*>(a.cos + at_row + first + j));
+        const float4 z = __ldg(reinterpret_cast<const float4*>(a.sin + at_row + first + j));
+        c[j % C] = w.x, c[(j + 1) % C] = w.y, c[(j + 2) % C] = w.z, c[(j + 3) % C] = w.w;
+        s[j % C] = a.sign * z.x, s[(j + 1) % C] = a.sign * z.y, s[(j + 2) % C] = a.sign * z.z, s[(j + 3) % C] = a.sign * z.w;
+      }
+    } else {
+#pragma unroll
+      for (int j = 0; j < C; ++j) {
+        const int e = first + j;
+        const int k = U == ACROSS && e >= a.half ? e - a.half : e;
+        const bool turned = known && (U == ACROSS ? e < rot : e < a.half);
+        c[j] = turned ? __ldg(a.cos + at_row + k) : __int_as_float(0x7fffffff);
+        s[j] = turned ? a.sign * __ldg(a.sin + at_row + k) : __int_as_float(0x7fffffff);
+        if (U == ACROSS && e < a.half) s[j] = -s[j];
+      }
     }
   }
   if (U == ACROSS) __syncthreads();
@@ -113,6 +123,7 @@ __global__ void __launch_bounds__(256, 4) rotary_kernel(const __grid_constant__ 
            static_cast<long long>(w ? h - a.heads[0] : h) * a.os[w][2];
     if (copies) {
       store_vec<T, V>(y + at, xu[n]);
+      if (two) store_vec<T, V>(y + at2, xv[n]);
     } else if (U == HALVES) {
       Vec<T, V> yu, yv;
 #pragma unroll
@@ -122,7 +133,7 @@ __global__ void __launch_bounds__(256, 4) rotary_kernel(const __grid_constant__ 
         yv.v[j] = from_float<T>(fv * c[j] + fu * s[j]);
       }
       store_vec<T, V>(y + at, yu);
-      store_vec<T, V>(y + at + a.half, yv);
+      store_vec<T, V>(y + at2, yv);
     } else if (U == PAIRS) {
 #pragma unroll
       for (int j = 0; j < C; ++j) {
@@ -135,8 +146,12 @@ __global__ void __launch_bounds__(256, 4) rotary_kernel(const __grid_constant__ 
       store_vec<T, V>(y + at, xu[n]);
     } else {
 #pragma unroll
-      for (int j = 0; j < V; ++j)
-        if (i + j < rot) xu[n].v[j] = from_float<T>(to_float(xu[n].v[j]) * c[j] + other[n][j] * s[j]);
+      for (int j = 0; j < V; ++j) {
+        const int e = i + j;
+        if (e >= rot) break;
+        const float other = to_float(mine[n * a.dim + (e < a.half ? e + a.half : e - a.half)]);
+        xu[n].v[j] = from_float<T>(to_float(xu[n].v[j]) * c[j] + other * s[j]);
+      }
       store_vec<T, V>(y + at, xu[n]);
     }
   }
@@ -188,13 +203,14 @@ bool whole(const RotaryArgs& a, int v, int size) {
 
 template <typename T, int V, Units U>
 cudaError_t launch(RotaryArgs a, cudaStream_t s) {
-  const int units = (U == HALVES ? a.dim - a.half : a.dim) / V;
+  const int units = U == HALVES ? a.half / V + ((a.dim - 2 * a.half) / V + 1) / 2 : a.dim / V;
   const int heads = a.heads[0] + a.heads[1];
   a.head_groups = static_cast<unsigned>((heads + heads_at_once<U>() - 1) / heads_at_once<U>());
   const long long groups = a.rows * a.head_groups;
   if (groups > 0x7fffffffll) return cudaErrorInvalidValue;
   const int by = 256 / units;
-  rotary_kernel<T, V, U><<<static_cast<unsigned>((groups + by - 1) / by), dim3(units, by), 0, s>>>(a);
+  rotary_kernel<T, V, U><<<static_cast<unsigned>((groups + by - 1) / by), dim3(units, by),
+                          U == ACROSS ? by * heads_at_once<U>() * a.dim * sizeof(T) : 0, s>>>(a);
   return cudaGetLastError();
 }
 
@@ -267,6 +283,7 @@ extern "C" int ad_rotary(int device, int dtype, const void* q, const int64_t* q_
   a.tokens = tokens;
   a.dim = dim;
   a.half = rotary / 2;
+  a.table_vec = a.half % 4 == 0 && aligned(cos, 16) && aligned(sin, 16);
   a.sign = inverse ? -1.0f : 1.0f;
   DeviceGuard g(device);
   if (g.error() != cudaSuccess) return fail("ad_rotary: %s", cudaGetErrorString(g.error()));

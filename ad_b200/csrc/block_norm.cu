@@ -1,5 +1,8 @@
 // The entry points of the norms around a block, and the kernel that adds up the
 // gradient's column sums; block_norm.cuh has the formulas and the row kernels.
+#include <algorithm>
+#include <initializer_list>
+
 #include "block_norm.cuh"
 
 namespace {
@@ -40,23 +43,24 @@ __global__ void __launch_bounds__(256) norm_finish_kernel(const __grid_constant_
   }
 }
 
-// How the gradient's rows are shared out, about two blocks a multiprocessor:
-// consecutive rows to a block; where a gate is shared by rows, either several
+// How the gradient's rows are shared out: consecutive rows to a block; where a gate is shared by rows, either several
 // blocks to a run of such rows or whole runs to a block.
 struct Split {
   long long run, blocks_per_run, rows_per_block, blocks;
 };
-Split split_rows(long long rows, long long rows_per_gate, int sms) {
+Split split_rows(long long rows, long long rows_per_gate, int width, int sms) {
   Split s;
   s.run = rows_per_gate > 1 ? rows_per_gate : rows;
-  const long long runs = rows / s.run, want = 2ll * sms;
+  // 512 threads with eight elements each to a multiprocessor, in as many blocks as that makes
+  const int per_sm = std::max(1, std::min(16, 4096 / width));
+  const long long runs = rows / s.run, want = static_cast<long long>(per_sm) * sms;
   if (runs >= want) {
     s.blocks_per_run = 0;
     s.rows_per_block = (runs + want - 1) / want * s.run;
     s.blocks = (rows + s.rows_per_block - 1) / s.rows_per_block;
     return s;
   }
-  long long per = (want + runs - 1) / runs;
+  long long per = want / runs;  // no more blocks than are resident at a time
   if (per > s.run) per = s.run;
   s.rows_per_block = (s.run + per - 1) / per;
   s.blocks_per_run = (s.run + s.rows_per_block - 1) / s.rows_per_block;
@@ -70,12 +74,14 @@ bool fits(const void* p, long long ld, int size) {
 
 // The checks and the variant that both directions share.
 int check(const char* who, int dtype, int wtype, int kind, const void* x, const void* z, const void* gate,
-          int64_t rows_per_gate, int64_t rows, int width, float eps) {
+          int64_t rows_per_gate, int64_t rows, int width, float eps, std::initializer_list<int64_t> lds) {
   if (dtype < AD_F32 || dtype > AD_F16) return fail("%s: unknown element type %d", who, dtype);
   if (wtype != AD_F32 && wtype != dtype) return fail("%s: weights of type %d beside elements of type %d", who, wtype, dtype);
   if (kind != 0 && kind != 1) return fail("%s: unknown norm %d", who, kind);
   if (rows < 0 || width < 1 || width > 32768) return fail("%s: %lld rows of %d elements (1 to 32768)", who, (long long)rows, width);
   if (rows > 0x7fffffffll) return fail("%s: %lld rows in one call", who, (long long)rows);
+  for (int64_t ld : lds)
+    if (ld < 0 || ld > 0x7fffffffll) return fail("%s: rows %lld elements apart", who, (long long)ld);
   if (!(eps >= 0.0f)) return fail("%s: eps %g", who, eps);
   if (rows && (!x || !z)) return fail("%s: null operand", who);
   if (gate && rows && (rows_per_gate < 1 || rows % rows_per_gate))
@@ -83,10 +89,10 @@ int check(const char* who, int dtype, int wtype, int kind, const void* x, const 
   return 0;
 }
 
-cudaError_t start_any(const NormArgs& a, int dtype, bool grad, bool gen, bool vec, unsigned blocks, cudaStream_t s) {
-  return dtype == AD_F32    ? start_norm_f32(a, grad, gen, vec, blocks, s)
-         : dtype == AD_BF16 ? start_norm_bf16(a, grad, gen, vec, blocks, s)
-                            : start_norm_f16(a, grad, gen, vec, blocks, s);
+cudaError_t start_any(const NormArgs& a, int dtype, bool grad, bool gen, bool vec, unsigned blocks, int sms, cudaStream_t s) {
+  return dtype == AD_F32    ? start_norm_f32(a, grad, gen, vec, blocks, sms, s)
+         : dtype == AD_BF16 ? start_norm_bf16(a, grad, gen, vec, blocks, sms, s)
+                            : start_norm_f16(a, grad, gen, vec, blocks, sms, s);
 }
 
 }  // namespace
@@ -96,7 +102,7 @@ extern "C" int ad_block_norm(int device, int dtype, int wtype, int kind, const v
                              const void* wa, const void* ba, const void* wb, const void* bb, float scale, float eps,
                              int64_t rows, int width, void* h, int64_t ldh, void* y, int64_t ldy, float* stats,
                              void* stream) {
-  if (check("ad_block_norm", dtype, wtype, kind, x, z, gate, rows_per_gate, rows, width, eps)) return 1;
+  if (check("ad_block_norm", dtype, wtype, kind, x, z, gate, rows_per_gate, rows, width, eps, {ldx, ldz, ldg, ldh, ldy})) return 1;
   if (rows == 0) return 0;
   if (!h || (wb && !y) || !stats || !aligned(stats, 16)) return fail("ad_block_norm: null or unaligned result");
   if ((ba && !wa) || (bb && !wb)) return fail("ad_block_norm: a bias without its weight");
@@ -118,9 +124,7 @@ extern "C" int ad_block_norm(int device, int dtype, int wtype, int kind, const v
   if (g.error() != cudaSuccess) return fail("ad_block_norm: %s", cudaGetErrorString(g.error()));
   const int sms = sm_count(g.device());
   if (!sms) return fail("ad_block_norm: no device properties");
-  const long long most = 8ll * sms;
-  const cudaError_t e = start_any(a, dtype, false, kind || ba || bb, vec,
-                                  static_cast<unsigned>(rows < most ? rows : most), static_cast<cudaStream_t>(stream));
+  const cudaError_t e = start_any(a, dtype, false, kind || ba || bb, vec, 0, sms, static_cast<cudaStream_t>(stream));
   if (e != cudaSuccess) return fail("ad_block_norm: %s", cudaGetErrorString(e));
   return 0;
 }
@@ -133,7 +137,7 @@ extern "C" int ad_block_norm_grad_workspace(int device, int64_t rows, int width,
   const int sms = g.error() == cudaSuccess ? sm_count(g.device()) : 0;
   if (!sms) return fail("ad_block_norm_grad_workspace: no device properties");
   if (rows_per_gate && rows % rows_per_gate) return fail("ad_block_norm_grad_workspace: rows cannot share gates so");
-  *bytes = sizeof(float) * SUMS * static_cast<size_t>(split_rows(rows, rows_per_gate, sms).blocks) * width;
+  *bytes = sizeof(float) * SUMS * static_cast<size_t>(split_rows(rows, rows_per_gate, width, sms).blocks) * width;
   return 0;
 }
 
@@ -144,7 +148,8 @@ extern "C" int ad_block_norm_grad(int device, int dtype, int wtype, int kind, co
                                   const float* stats, int64_t rows, int width, void* dx, int64_t lddx, void* dz,
                                   int64_t lddz, void* dgate, int64_t lddg, void* dwa, void* dba, void* dwb, void* dbb,
                                   void* workspace, size_t workspace_bytes, void* stream) {
-  if (check("ad_block_norm_grad", dtype, wtype, kind, x, z, gate, rows_per_gate, rows, width, 0.0f)) return 1;
+  if (check("ad_block_norm_grad", dtype, wtype, kind, x, z, gate, rows_per_gate, rows, width, 0.0f,
+            {lddh, lddy, ldx, ldz, ldg, lddx, lddz, lddg})) return 1;
   if ((ba && !wa) || (bb && !wb)) return fail("ad_block_norm_grad: a bias without its weight");
   if ((wa && !dwa) || (wb && !dwb) || (ba && !dba) || (bb && !dbb))
     return fail("ad_block_norm_grad: a weight without room for its gradient");
@@ -166,7 +171,7 @@ extern "C" int ad_block_norm_grad(int device, int dtype, int wtype, int kind, co
     return fail("ad_block_norm_grad: null or unaligned operand");
   const int sms = sm_count(g.device());
   if (!sms) return fail("ad_block_norm_grad: no device properties");
-  const Split split = split_rows(rows, gate ? rows_per_gate : 0, sms);
+  const Split split = split_rows(rows, gate ? rows_per_gate : 0, width, sms);
   const size_t need = sizeof(float) * SUMS * static_cast<size_t>(split.blocks) * width;
   if (!workspace || !aligned(workspace, 16) || workspace_bytes < need)
     return fail("ad_block_norm_grad: needs %zu bytes of workspace, 16-byte aligned", need);
@@ -187,7 +192,7 @@ extern "C" int ad_block_norm_grad(int device, int dtype, int wtype, int kind, co
   const bool vec = width % (16 / size) == 0 && fits(x, ldx, size) && fits(z, ldz, size) && fits(gate, ldg, size) &&
                    fits(dh, lddh, size) && fits(dy, lddy, size) && fits(dx, lddx, size) && fits(dz, lddz, size) &&
                    fits(dgate, lddg, size) && fits(wa, 0, 1) && fits(ba, 0, 1) && fits(wb, 0, 1) && fits(bb, 0, 1);
-  cudaError_t e = start_any(a, dtype, true, kind || ba || bb, vec, static_cast<unsigned>(split.blocks), s);
+  cudaError_t e = start_any(a, dtype, true, kind || ba || bb, vec, static_cast<unsigned>(split.blocks), sms, s);
   if (e != cudaSuccess) return fail("ad_block_norm_grad: %s", cudaGetErrorString(e));
   FinishArgs f = {};
   f.part = a.part;
@@ -200,7 +205,7 @@ extern "C" int ad_block_norm_grad(int device, int dtype, int wtype, int kind, co
   f.out[SUM_GATE] = shared ? dgate : nullptr;
   f.type[SUM_GATE] = dtype;
   f.ldg = lddg;
-  const long long gates = shared ? rows / rows_per_gate : 0;  // fewer than two a multiprocessor
+  const long long gates = shared ? rows / rows_per_gate : 0;  // fewer than blocks
   if (f.out[SUM_WA] || f.out[SUM_WB] || shared) {
     norm_finish_kernel<<<dim3((width + 31) / 32, static_cast<unsigned>(4 + gates)), dim3(32, 8), 0, s>>>(f);
     e = cudaGetLastError();

@@ -25,6 +25,8 @@
 // consecutive rows, written out once a block (a gate's as soon as its rows end
 // where a block has whole runs of them), and added in the blocks' order by a
 // second kernel, so that results do not depend on scheduling.
+#include <algorithm>
+
 #include "ops_common.cuh"
 
 namespace adops {
@@ -43,48 +45,81 @@ struct NormArgs {
   // a run (0: a block has whole runs), rows of a block
   long long run, blocks_per_run, rows_per_block;
   int width, sigmoid, layer;
+  int staged;  // bytes of weights and biases kept in shared memory
   float scale, eps;
 };
 
-__device__ __forceinline__ float act_of(float g, int sigmoid) {
-  return sigmoid ? 1.0f / (1.0f + __expf(-g)) : g;
+// rows fit 32 bits: a short division
+__device__ __forceinline__ long long gate_row(const NormArgs& a, long long row) {
+  return a.rows_per_gate == 1 ? row : static_cast<unsigned>(row) / static_cast<unsigned>(a.rows_per_gate);
+}
+
+// Offset of a row: both factors fit 32 bits, one instruction.
+__device__ __forceinline__ unsigned long long at(long long row, long long ld) {
+  return static_cast<unsigned long long>(static_cast<unsigned>(row)) * static_cast<unsigned>(ld);
+}
+
+// exp and quotient to about 2 units in the last place of 32 bits
+template <int E>
+__device__ __forceinline__ void activate(float (&g)[E], int sigmoid) {
+  if (!sigmoid) return;
+#pragma unroll
+  for (int i = 0; i < E; ++i) g[i] = __fdividef(1.0f, 1.0f + __expf(-g[i]));
 }
 
 // Sums over the block of N values a thread; every thread gets them.  `buf`
 // alternates between two areas so that one barrier a call is enough.
 template <int N>
 __device__ __forceinline__ void block_sum(float (&v)[N], float* smem, int& flip) {
+  static_assert(N == 1 || N == 2, "");
+  const int lane = threadIdx.x & 31, warps = blockDim.x >> 5;
+  float s;
+  if (N == 1) {
+    s = warp_sum(v[0]);
+  } else {  // each half of the warp adds up one of the two
+    const bool up = lane & 16;
+    s = (up ? v[N - 1] : v[0]) + __shfl_xor_sync(0xffffffffu, up ? v[0] : v[N - 1], 16);
 #pragma unroll
-  for (int k = 0; k < N; ++k) v[k] = warp_sum(v[k]);
-  const int warps = blockDim.x >> 5;
-  if (warps == 1) return;
+    for (int o = 8; o; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+  }
   float* buf = smem + flip * (2 * 32);
   flip ^= 1;
-  if ((threadIdx.x & 31) == 0) {
-#pragma unroll
-    for (int k = 0; k < N; ++k) buf[k * 32 + (threadIdx.x >> 5)] = v[k];
-  }
+  if ((lane & (N == 1 ? 31 : 15)) == 0) buf[lane * 2 + (threadIdx.x >> 5)] = s;  // the second value from 32 on
   __syncthreads();
-  const int lane = threadIdx.x & 31;
 #pragma unroll
-  for (int k = 0; k < N; ++k) v[k] = warp_sum(lane < warps ? buf[k * 32 + lane] : 0.0f);
-}
-
-template <typename T, int V, int NV>
-__device__ __forceinline__ void load_row(const T* p, int width, float (&o)[NV * V]) {
+  for (int k = 0; k < N; ++k) v[k] = 0.0f;
+  for (int w = 0; w < warps; w += 4) {  // areas past the warps hold zeros
 #pragma unroll
-  for (int n = 0; n < NV; ++n) {
-    const int c = (n * blockDim.x + threadIdx.x) * V;
-    if (c < width) {
-      const Vec<T, V> r = load_vec<T, V>(p + c);
-#pragma unroll
-      for (int j = 0; j < V; ++j) o[n * V + j] = to_float(r.v[j]);
-    } else {
-#pragma unroll
-      for (int j = 0; j < V; ++j) o[n * V + j] = 0.0f;
+    for (int k = 0; k < N; ++k) {
+      const float4 q = *reinterpret_cast<const float4*>(buf + k * 32 + w);
+      v[k] += (q.x + q.y) + (q.z + q.w);
     }
   }
 }
+
+// A thread's share of a row; zeros past the width.
+template <typename T, int V, int NV>
+struct Raw {
+  Vec<T, V> q[NV];
+  __device__ __forceinline__ void load(const T* p, int width) {
+#pragma unroll
+    for (int n = 0; n < NV; ++n) {
+      const int c = (n * blockDim.x + threadIdx.x) * V;
+      if (c < width) {
+        q[n] = load_vec<T, V>(p + c);
+      } else {
+#pragma unroll
+        for (int j = 0; j < V; ++j) q[n].v[j] = from_float<T>(0.0f);
+      }
+    }
+  }
+  __device__ __forceinline__ void floats(float (&o)[NV * V]) const {
+#pragma unroll
+    for (int n = 0; n < NV; ++n)
+#pragma unroll
+      for (int j = 0; j < V; ++j) o[n * V + j] = to_float(q[n].v[j]);
+  }
+};
 template <typename T, int V, int NV>
 __device__ __forceinline__ void store_row(T* p, int width, const float (&o)[NV * V]) {
 #pragma unroll
@@ -92,8 +127,7 @@ __device__ __forceinline__ void store_row(T* p, int width, const float (&o)[NV *
     const int c = (n * blockDim.x + threadIdx.x) * V;
     if (c < width) {
       Vec<T, V> r;
-#pragma unroll
-      for (int j = 0; j < V; ++j) r.v[j] = from_float<T>(o[n * V + j]);
+      round_to<T, V>(o + n * V, r);
       store_vec<T, V>(p + c, r);
     }
   }
@@ -132,9 +166,64 @@ __device__ __forceinline__ void load_weights(const void* p, int wtype, int width
       }
     }
   } else {
-    load_row<T, V, NV>(static_cast<const T*>(p), width, o);
+    Raw<T, V, NV> r;
+    r.load(static_cast<const T*>(p), width);
+    r.floats(o);
   }
 }
+
+// The four vectors in shared memory for the block's life: loads of them between
+// the rows' would queue behind those for a microsecond each.  Quads of a vector's
+// elements lie in planes, so that neighbouring threads read neighbouring words.
+enum { W_WA = 0, W_WB = 1, W_BA = 2, W_BB = 3 };
+template <int V>
+__host__ __device__ constexpr int quad() {
+  return V < 4 ? V : 4;
+}
+template <typename T, int V, int NV, bool GEN>
+struct Weights {
+  const NormArgs& a;
+  float* sm;
+  int vecs;
+  __device__ __forceinline__ Weights(const NormArgs& args, float* shared) : a(args), sm(shared) {
+    vecs = (a.width + V - 1) / V;
+    if (!a.staged) return;
+    const void* from[4] = {a.wa, a.wb, a.ba, a.bb};
+#pragma unroll
+    for (int k = 0; k < (GEN ? 4 : 2); ++k) {
+      if (!from[k]) continue;
+      float o[NV * V];
+      load_weights<T, V, NV>(from[k], a.wtype, a.width, o);
+#pragma unroll
+      for (int n = 0; n < NV; ++n) {
+        const int v = n * blockDim.x + threadIdx.x;
+        if (v < vecs) {
+#pragma unroll
+          for (int j = 0; j < V; ++j) sm[((k * (V / quad<V>()) + j / 4) * vecs + v) * quad<V>() + j % 4] = o[n * V + j];
+        }
+      }
+    }
+    // a thread reads what it wrote: no barrier
+  }
+  __device__ __forceinline__ void get(int k, float (&o)[NV * V]) const {
+    if (!a.staged) {
+      load_weights<T, V, NV>(k == W_WA ? a.wa : k == W_WB ? a.wb : k == W_BA ? a.ba : a.bb, a.wtype, a.width, o);
+      return;
+    }
+    constexpr int Q = quad<V>();
+#pragma unroll
+    for (int n = 0; n < NV; ++n) {
+      const int v = n * blockDim.x + threadIdx.x;
+#pragma unroll
+      for (int p = 0; p < V / Q; ++p) {
+        Vec<float, Q> r = {};
+        if (v < vecs) r = load_vec<float, Q>(sm + ((k * (V / Q) + p) * vecs + v) * Q);
+#pragma unroll
+        for (int j = 0; j < Q; ++j) o[n * V + p * Q + j] = r.v[j];
+      }
+    }
+  }
+};
 
 // Mean and reciprocal deviation of a row held by the block; elements past the
 // width are zero on entry.
@@ -166,49 +255,125 @@ __device__ __forceinline__ void moments(const float (&v)[NV * V], bool layer, in
   r = 1.0f / sqrtf(s[0] / width + eps);
 }
 
+// The rows to come of K operands, brought into shared memory while earlier ones
+// are worked on.  A thread copies and reads its own vectors only, so there is
+// nothing to wait for but its own copies.  (Kept in registers instead, the next
+// row was waited for all the same: 888 us for 65535 x 2048 bf16 gradients.)
+// Single elements (V = 1) are too small for such copies and rows of over 8192
+// elements too large: they are read when due.
+template <typename T, int V, int NV, int K>
+struct Ahead {
+  // rows: what 512 threads' shares of five operands leave room for
+  static constexpr int S = (sizeof(T) == 4 ? 2 : 4) / (V * NV <= 8 ? 1 : 2);
+  static constexpr bool DIRECT = V == 1 || V * NV > 16;
+  unsigned base;
+  int width;
+  __device__ __forceinline__ Ahead(void* shared, int w)
+      : base(static_cast<unsigned>(__cvta_generic_to_shared(shared))), width(w) {}
+  __device__ __forceinline__ unsigned slot(int stage, int k, int n) const {
+    return base + (((stage * K + k) * NV + n) * blockDim.x + threadIdx.x) * 16;
+  }
+  __device__ __forceinline__ void copy(int stage, int k, const T* row) const {
+    if (DIRECT) return;
+#pragma unroll
+    for (int n = 0; n < NV; ++n) {
+      const int c = (n * blockDim.x + threadIdx.x) * V;
+      if (c < width) asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(slot(stage, k, n)), "l"(row + c));
+    }
+  }
+  __device__ __forceinline__ void commit() const { asm volatile("cp.async.commit_group;" ::: "memory"); }
+  // The oldest row's copies are done.
+  __device__ __forceinline__ void wait() const { asm volatile("cp.async.wait_group %0;" ::"n"(S - 1) : "memory"); }
+  __device__ __forceinline__ void read(int stage, int k, const T* row, float (&o)[NV * V]) const {
+    if (DIRECT) {
+      Raw<T, V, NV> r;
+      r.load(row, width);
+      r.floats(o);
+      return;
+    }
+#pragma unroll
+    for (int n = 0; n < NV; ++n) {
+      uint4 q = make_uint4(0, 0, 0, 0);
+      if ((n * blockDim.x + threadIdx.x) * V < width)
+        asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];"
+                     : "=r"(q.x), "=r"(q.y), "=r"(q.z), "=r"(q.w)
+                     : "r"(slot(stage, k, n))
+                     : "memory");
+      T e[V];
+      memcpy(e, &q, sizeof(T) * V < 16 ? sizeof(T) * V : 16);
+#pragma unroll
+      for (int j = 0; j < V; ++j) o[n * V + j] = to_float(e[j]);
+    }
+  }
+  static int bytes(int threads) { return DIRECT ? 0 : S * K * NV * threads * 16; }
+};
+
 // GEN: with a LayerNorm's means or with biases; without it both are known to be
 // absent.  MAXT: threads a block may have; with 256 of them several blocks share
 // a multiprocessor.
 template <typename T, int V, int NV, int MAXT, bool GEN>
-__global__ void __launch_bounds__(MAXT, MAXT == 256 ? 4 : 1) norm_kernel(const __grid_constant__ NormArgs a) {
-  __shared__ float smem[2 * 2 * 32];
+__global__ void __launch_bounds__(MAXT, MAXT == 256 ? (V * NV <= 8 ? 4 : 2) : 1)
+    norm_kernel(const __grid_constant__ NormArgs a) {
+  __shared__ __align__(16) float smem[2 * 2 * 32];
+  for (int i = threadIdx.x; i < 2 * 2 * 32; i += blockDim.x) smem[i] = 0.0f;
+  __syncthreads();
+  extern __shared__ __align__(16) float staged[];
   int flip = 0;
   constexpr int E = NV * V;
+  const Ahead<T, V, NV, 3> ahead(staged + a.staged / 4, a.width);
+  auto pz = [&](long long row) { return static_cast<const T*>(a.z) + at(row, a.ldz); };
+  auto px = [&](long long row) { return static_cast<const T*>(a.x) + at(row, a.ldx); };
+  auto pg = [&](long long row) { return static_cast<const T*>(a.gate) + at(gate_row(a, row), a.ldg); };
+  auto fetch = [&](int stage, long long row) {
+    if (row < a.rows) {
+      ahead.copy(stage, 0, pz(row));
+      ahead.copy(stage, 1, px(row));
+      if (a.gate) ahead.copy(stage, 2, pg(row));
+    }
+    ahead.commit();
+  };
+  for (int k = 0; k < ahead.S; ++k) fetch(k, blockIdx.x + static_cast<long long>(k) * gridDim.x);
+  const Weights<T, V, NV, GEN> weights(a, staged);
+  int stage = 0;
   for (long long row = blockIdx.x; row < a.rows; row += gridDim.x) {
-    float x[E], u[E], w[E];
-    load_row<T, V, NV>(static_cast<const T*>(a.x) + row * a.ldx, a.width, x);
-    load_row<T, V, NV>(static_cast<const T*>(a.z) + row * a.ldz, a.width, u);
+    float x[E], u[E], act[E], w[E];
+    ahead.wait();
+    ahead.read(stage, 0, pz(row), u);
+    ahead.read(stage, 1, px(row), x);
+    if (a.gate) ahead.read(stage, 2, pg(row), act);
+    fetch(stage, row + static_cast<long long>(ahead.S) * gridDim.x);
+    stage = stage + 1 == ahead.S ? 0 : stage + 1;
     float mz = 0.0f, rz = 1.0f, mh = 0.0f, rh = 1.0f;
     if (a.wa) {
       moments<V, NV>(u, GEN && a.layer, a.width, a.eps, smem, flip, mz, rz);
-      load_weights<T, V, NV>(a.wa, a.wtype, a.width, w);
+      weights.get(W_WA, w);
 #pragma unroll
       for (int i = 0; i < E; ++i) u[i] = (u[i] - mz) * rz * w[i];
       if (GEN && a.ba) {
-        load_weights<T, V, NV>(a.ba, a.wtype, a.width, w);
+        weights.get(W_BA, w);
 #pragma unroll
         for (int i = 0; i < E; ++i) u[i] += w[i];
       }
     }
     if (a.gate) {
-      load_row<T, V, NV>(static_cast<const T*>(a.gate) + row / a.rows_per_gate * a.ldg, a.width, w);
+      activate<E>(act, a.sigmoid);
 #pragma unroll
-      for (int i = 0; i < E; ++i) u[i] *= act_of(w[i], a.sigmoid);
+      for (int i = 0; i < E; ++i) u[i] *= act[i];
     }
 #pragma unroll
     for (int i = 0; i < E; ++i) x[i] = fmaf(a.scale, x[i], u[i]);
-    store_row<T, V, NV>(static_cast<T*>(a.h) + row * a.ldh, a.width, x);
+    store_row<T, V, NV>(static_cast<T*>(a.h) + at(row, a.ldh), a.width, x);
     if (a.wb) {
       moments<V, NV>(x, GEN && a.layer, a.width, a.eps, smem, flip, mh, rh);
-      load_weights<T, V, NV>(a.wb, a.wtype, a.width, w);
+      weights.get(W_WB, w);
 #pragma unroll
       for (int i = 0; i < E; ++i) x[i] = (x[i] - mh) * rh * w[i];
       if (GEN && a.bb) {
-        load_weights<T, V, NV>(a.bb, a.wtype, a.width, w);
+        weights.get(W_BB, w);
 #pragma unroll
         for (int i = 0; i < E; ++i) x[i] += w[i];
       }
-      store_row<T, V, NV>(static_cast<T*>(a.y) + row * a.ldy, a.width, x);
+      store_row<T, V, NV>(static_cast<T*>(a.y) + at(row, a.ldy), a.width, x);
     }
     if (threadIdx.x == 0)
       reinterpret_cast<float4*>(a.stats)[row] = make_float4(mz, rz, mh, rh);
@@ -220,8 +385,11 @@ enum { SUM_WA = 0, SUM_WB = 1, SUM_BA = 2, SUM_BB = 3, SUM_GATE = 4, SUMS = 5 };
 
 // SHARED: the gate's rows are shared, its gradient is a sum over rows.
 template <typename T, int V, int NV, int MAXT, bool GEN, bool SHARED>
-__global__ void __launch_bounds__(MAXT, MAXT == 256 ? 2 : 1) norm_grad_kernel(const __grid_constant__ NormArgs a) {
-  __shared__ float smem[2 * 2 * 32];
+__global__ void __launch_bounds__(MAXT, MAXT == 256 && V * NV <= 8 ? 2 : 1) norm_grad_kernel(const __grid_constant__ NormArgs a) {
+  __shared__ __align__(16) float smem[2 * 2 * 32];
+  for (int i = threadIdx.x; i < 2 * 2 * 32; i += blockDim.x) smem[i] = 0.0f;
+  __syncthreads();
+  extern __shared__ __align__(16) float staged[];
   int flip = 0;
   constexpr int E = NV * V;
   float swa[E], swb[E], sba[E], sbb[E], sg[E];
@@ -237,43 +405,67 @@ __global__ void __launch_bounds__(MAXT, MAXT == 256 ? 2 : 1) norm_grad_kernel(co
   long long left = a.run;  // rows of the run to come
   const bool layer = GEN && a.layer;
   const float inv = 1.0f / a.width;
-  for (long long row = r0; row < r1; ++row) {
-    const float4 st = reinterpret_cast<const float4*>(a.stats)[row];
-    const float mz = st.x, rz = st.y, mh = st.z, rh = st.w;
-    float nz[E], u[E], act[E], slope[E], t[E], w[E];
-    load_row<T, V, NV>(static_cast<const T*>(a.z) + row * a.ldz, a.width, nz);
-    if (a.gate) {
-      load_row<T, V, NV>(static_cast<const T*>(a.gate) + row / a.rows_per_gate * a.ldg, a.width, act);
-#pragma unroll
-      for (int i = 0; i < E; ++i) {
-        act[i] = act_of(act[i], a.sigmoid);
-        slope[i] = a.sigmoid ? act[i] * (1.0f - act[i]) : 1.0f;
+  const Ahead<T, V, NV, 5> ahead(staged + a.staged / 4, a.width);
+  auto pz = [&](long long row) { return static_cast<const T*>(a.z) + at(row, a.ldz); };
+  auto px = [&](long long row) { return static_cast<const T*>(a.x) + at(row, a.ldx); };
+  auto pg = [&](long long row) { return static_cast<const T*>(a.gate) + at(gate_row(a, row), a.ldg); };
+  auto pdh = [&](long long row) { return static_cast<const T*>(a.dh) + at(row, a.lddh); };
+  auto pdy = [&](long long row) { return static_cast<const T*>(a.dy) + at(row, a.lddy); };
+  auto fetch = [&](int stage, long long row) {
+    if (row < r1) {
+      ahead.copy(stage, 0, pz(row));
+      if (a.gate) ahead.copy(stage, 1, pg(row));
+      if (a.wb) {
+        ahead.copy(stage, 2, px(row));
+        ahead.copy(stage, 3, pdy(row));
       }
+      ahead.copy(stage, 4, pdh(row));
+    }
+    ahead.commit();
+  };
+  for (int k = 0; k < ahead.S; ++k) fetch(k, r0 + k);
+  const Weights<T, V, NV, GEN> weights(a, staged);
+  int stage = 0;
+  float4 rst = r0 < r1 ? reinterpret_cast<const float4*>(a.stats)[r0] : make_float4(0, 0, 0, 0);
+  for (long long row = r0; row < r1; ++row) {
+    const float4 st = rst;
+    const float mz = st.x, rz = st.y, mh = st.z, rh = st.w;
+    float nz[E], u[E], act[E], t[E], w[E], nh[E], d[E];
+    ahead.wait();
+    ahead.read(stage, 0, pz(row), nz);
+    ahead.read(stage, 4, pdh(row), t);
+    if (a.wb) {
+      ahead.read(stage, 2, px(row), nh);
+      ahead.read(stage, 3, pdy(row), d);
+    }
+    if (a.gate) {
+      ahead.read(stage, 1, pg(row), act);
+      activate<E>(act, a.sigmoid);
     } else {
 #pragma unroll
-      for (int i = 0; i < E; ++i) act[i] = slope[i] = 1.0f;
+      for (int i = 0; i < E; ++i) act[i] = 1.0f;
     }
+    fetch(stage, row + ahead.S);
+    stage = stage + 1 == ahead.S ? 0 : stage + 1;
+    if (row + 1 < r1) rst = reinterpret_cast<const float4*>(a.stats)[row + 1];
 #pragma unroll
     for (int i = 0; i < E; ++i) u[i] = nz[i];
     if (a.wa) {
-      load_weights<T, V, NV>(a.wa, a.wtype, a.width, w);
+      weights.get(W_WA, w);
 #pragma unroll
       for (int i = 0; i < E; ++i) {
         nz[i] = (nz[i] - mz) * rz;
         u[i] = nz[i] * w[i];
       }
       if (GEN && a.ba) {
-        load_weights<T, V, NV>(a.ba, a.wtype, a.width, w);
+        weights.get(W_BA, w);
 #pragma unroll
         for (int i = 0; i < E; ++i) u[i] += w[i];
       }
     }
-    load_row<T, V, NV>(static_cast<const T*>(a.dh) + row * a.lddh, a.width, t);
     if (a.wb) {
-      float nh[E], d[E], q[2] = {0.0f, 0.0f};
-      load_row<T, V, NV>(static_cast<const T*>(a.x) + row * a.ldx, a.width, nh);
-      load_row<T, V, NV>(static_cast<const T*>(a.dy) + row * a.lddy, a.width, d);
-      load_weights<T, V, NV>(a.wb, a.wtype, a.width, w);
+      float q[2] = {0.0f, 0.0f};
+      weights.get(W_WB, w);
 #pragma unroll
       for (int i = 0; i < E; ++i) {
         nh[i] = (fmaf(a.scale, nh[i], act[i] * u[i]) - mh) * rh;
@@ -283,27 +475,35 @@ __global__ void __launch_bounds__(MAXT, MAXT == 256 ? 2 : 1) norm_grad_kernel(co
         q[0] = fmaf(d[i], nh[i], q[0]);
         if (layer) q[1] += d[i];
       }
-      block_sum<2>(q, smem, flip);
+      if (GEN)
+        block_sum<2>(q, smem, flip);
+      else
+        block_sum<1>(reinterpret_cast<float(&)[1]>(q), smem, flip);
 #pragma unroll
       for (int i = 0; i < E; ++i) t[i] += rh * (d[i] - nh[i] * (q[0] * inv) - (layer ? q[1] * inv : 0.0f));
     }
     float o[E];
 #pragma unroll
     for (int i = 0; i < E; ++i) o[i] = a.scale * t[i];
-    store_row<T, V, NV>(static_cast<T*>(a.dx) + row * a.lddx, a.width, o);
+    store_row<T, V, NV>(static_cast<T*>(a.dx) + at(row, a.lddx), a.width, o);
     if (a.gate) {
 #pragma unroll
-      for (int i = 0; i < E; ++i) {
-        o[i] = t[i] * u[i] * slope[i];
-        if (SHARED) sg[i] += o[i];
+      for (int i = 0; i < E; ++i) o[i] = t[i] * u[i];
+      if (a.sigmoid) {
+#pragma unroll
+        for (int i = 0; i < E; ++i) o[i] *= act[i] * (1.0f - act[i]);
       }
-      if (!SHARED) store_row<T, V, NV>(static_cast<T*>(a.dgate) + row * a.lddg, a.width, o);
+      if (SHARED) {
+#pragma unroll
+        for (int i = 0; i < E; ++i) sg[i] += o[i];
+      }
+      if (!SHARED) store_row<T, V, NV>(static_cast<T*>(a.dgate) + at(row, a.lddg), a.width, o);
     }
 #pragma unroll
     for (int i = 0; i < E; ++i) t[i] *= act[i];
     if (a.wa) {
       float q[2] = {0.0f, 0.0f};
-      load_weights<T, V, NV>(a.wa, a.wtype, a.width, w);
+      weights.get(W_WA, w);
 #pragma unroll
       for (int i = 0; i < E; ++i) {
         swa[i] = fmaf(t[i], nz[i], swa[i]);
@@ -312,11 +512,14 @@ __global__ void __launch_bounds__(MAXT, MAXT == 256 ? 2 : 1) norm_grad_kernel(co
         q[0] = fmaf(t[i], nz[i], q[0]);
         if (layer) q[1] += t[i];
       }
-      block_sum<2>(q, smem, flip);
+      if (GEN)
+        block_sum<2>(q, smem, flip);
+      else
+        block_sum<1>(reinterpret_cast<float(&)[1]>(q), smem, flip);
 #pragma unroll
       for (int i = 0; i < E; ++i) t[i] = rz * (t[i] - nz[i] * (q[0] * inv) - (layer ? q[1] * inv : 0.0f));
     }
-    store_row<T, V, NV>(static_cast<T*>(a.dz) + row * a.lddz, a.width, t);
+    store_row<T, V, NV>(static_cast<T*>(a.dz) + at(row, a.lddz), a.width, t);
     if (SHARED && whole && --left == 0) {
       store_row<T, V, NV>(static_cast<T*>(a.dgate) + row / a.run * a.lddg, a.width, sg);
 #pragma unroll
@@ -334,52 +537,69 @@ __global__ void __launch_bounds__(MAXT, MAXT == 256 ? 2 : 1) norm_grad_kernel(co
   if (SHARED && !whole) store_sums<V, NV>(part + SUM_GATE * a.width, a.width, sg);
 }
 
-template <typename T, int V, int NV, int MAXT>
-cudaError_t start_norm(const NormArgs& a, bool grad, bool gen, unsigned blocks, int threads, cudaStream_t s) {
-  const bool shared = a.gate && a.rows_per_gate > 1;
-  if (!grad) {
-    if (gen)
-      norm_kernel<T, V, NV, MAXT, true><<<blocks, threads, 0, s>>>(a);
-    else
-      norm_kernel<T, V, NV, MAXT, false><<<blocks, threads, 0, s>>>(a);
-  } else if (gen) {
-    if (shared)
-      norm_grad_kernel<T, V, NV, MAXT, true, true><<<blocks, threads, 0, s>>>(a);
-    else
-      norm_grad_kernel<T, V, NV, MAXT, true, false><<<blocks, threads, 0, s>>>(a);
-  } else {
-    if (shared)
-      norm_grad_kernel<T, V, NV, MAXT, false, true><<<blocks, threads, 0, s>>>(a);
-    else
-      norm_grad_kernel<T, V, NV, MAXT, false, false><<<blocks, threads, 0, s>>>(a);
+// `ahead`: bytes of the rows to come; `blocks` 0: as many as are resident at a
+// time, each with every so-many-th row.
+template <typename K>
+cudaError_t run_norm(K kernel, NormArgs a, bool gen, int v, int ahead, unsigned blocks, int sms, int threads,
+                     cudaStream_t s) {
+  a.staged = ((gen ? 4 : 2) * 4 * ((a.width + v - 1) / v * v) + 15) / 16 * 16;
+  if (a.staged > 64 * 1024) a.staged = 0;
+  const int bytes = a.staged + ahead;
+  if (bytes + 1024 > 48 * 1024) {  // beside what the kernel declares
+    const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+    if (e != cudaSuccess) return e;
   }
+  if (!blocks) {
+    int per = 1;
+    const cudaError_t e = cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per, kernel, threads, bytes);
+    if (e != cudaSuccess) return e;
+    blocks = static_cast<unsigned>(std::min(a.rows, 1ll * std::max(per, 1) * sms));
+  }
+  kernel<<<blocks, threads, bytes, s>>>(a);
   return cudaGetLastError();
 }
 
-// Eight elements a thread while the row fits 1024 threads so, else 32.  `vec`:
-// all addresses and sizes allow 16-byte vectors.
-template <typename T>
-cudaError_t start_norm_typed(const NormArgs& a, bool grad, bool gen, bool vec, unsigned blocks, cudaStream_t s) {
-  constexpr int V = 16 / static_cast<int>(sizeof(T));
-  const int per = a.width <= 8192 ? 8 : 32;
-  const int threads = ((a.width + per - 1) / per + 31) / 32 * 32;
-  if (per == 8) {
-    if (threads <= 256)
-      return vec ? start_norm<T, V, 8 / V, 256>(a, grad, gen, blocks, threads, s)
-                 : start_norm<T, 1, 8, 256>(a, grad, gen, blocks, threads, s);
-    if (threads <= 512)
-      return vec ? start_norm<T, V, 8 / V, 512>(a, grad, gen, blocks, threads, s)
-                 : start_norm<T, 1, 8, 512>(a, grad, gen, blocks, threads, s);
-    return vec ? start_norm<T, V, 8 / V, 1024>(a, grad, gen, blocks, threads, s)
-               : start_norm<T, 1, 8, 1024>(a, grad, gen, blocks, threads, s);
-  }
-  return vec ? start_norm<T, V, 32 / V, 1024>(a, grad, gen, blocks, threads, s)
-             : start_norm<T, 1, 32, 1024>(a, grad, gen, blocks, threads, s);
+template <typename T, int V, int NV, int MAXT>
+cudaError_t start_norm(const NormArgs& a, bool grad, bool gen, unsigned blocks, int sms, int threads, cudaStream_t s) {
+  const bool shared = a.gate && a.rows_per_gate > 1;
+  const int f = Ahead<T, V, NV, 3>::bytes(threads), g = Ahead<T, V, NV, 5>::bytes(threads);
+  if (!grad)
+    return gen ? run_norm(norm_kernel<T, V, NV, MAXT, true>, a, gen, V, f, 0, sms, threads, s)
+               : run_norm(norm_kernel<T, V, NV, MAXT, false>, a, gen, V, f, 0, sms, threads, s);
+  if (gen)
+    return shared ? run_norm(norm_grad_kernel<T, V, NV, MAXT, true, true>, a, gen, V, g, blocks, sms, threads, s)
+                  : run_norm(norm_grad_kernel<T, V, NV, MAXT, true, false>, a, gen, V, g, blocks, sms, threads, s);
+  return shared ? run_norm(norm_grad_kernel<T, V, NV, MAXT, false, true>, a, gen, V, g, blocks, sms, threads, s)
+                : run_norm(norm_grad_kernel<T, V, NV, MAXT, false, false>, a, gen, V, g, blocks, sms, threads, s);
 }
 
-cudaError_t start_norm_f32(const NormArgs& a, bool grad, bool gen, bool vec, unsigned blocks, cudaStream_t s);
-cudaError_t start_norm_bf16(const NormArgs& a, bool grad, bool gen, bool vec, unsigned blocks, cudaStream_t s);
-cudaError_t start_norm_f16(const NormArgs& a, bool grad, bool gen, bool vec, unsigned blocks, cudaStream_t s);
+// Eight elements of a row to a thread while 512 threads are enough for it (what
+// a row costs each warp besides its elements is two sums over the block), 16
+// while 512 are, else 32 to each of up to 1024.  `vec`: all addresses and sizes
+// allow 16-byte vectors; single elements else.
+template <typename T>
+cudaError_t start_norm_typed(const NormArgs& a, bool grad, bool gen, bool vec, unsigned blocks, int sms, cudaStream_t s) {
+  constexpr int V = 16 / static_cast<int>(sizeof(T));
+  auto threads_for = [&](int per) { return ((a.width + per - 1) / per + 31) / 32 * 32; };
+  int t = threads_for(8);
+  if (t <= 256)
+    return vec ? start_norm<T, V, 8 / V, 256>(a, grad, gen, blocks, sms, t, s)
+               : start_norm<T, 1, 8, 256>(a, grad, gen, blocks, sms, t, s);
+  if (t <= 512)
+    return vec ? start_norm<T, V, 8 / V, 512>(a, grad, gen, blocks, sms, t, s)
+               : start_norm<T, 1, 8, 512>(a, grad, gen, blocks, sms, t, s);
+  t = threads_for(16);
+  if (t <= 512)
+    return vec ? start_norm<T, V, 16 / V, 512>(a, grad, gen, blocks, sms, t, s)
+               : start_norm<T, 1, 16, 512>(a, grad, gen, blocks, sms, t, s);
+  t = threads_for(32);
+  return vec ? start_norm<T, V, 32 / V, 1024>(a, grad, gen, blocks, sms, t, s)
+             : start_norm<T, 1, 32, 1024>(a, grad, gen, blocks, sms, t, s);
+}
+
+cudaError_t start_norm_f32(const NormArgs& a, bool grad, bool gen, bool vec, unsigned blocks, int sms, cudaStream_t s);
+cudaError_t start_norm_bf16(const NormArgs& a, bool grad, bool gen, bool vec, unsigned blocks, int sms, cudaStream_t s);
+cudaError_t start_norm_f16(const NormArgs& a, bool grad, bool gen, bool vec, unsigned blocks, int sms, cudaStream_t s);
 
 }  // namespace adops
 

@@ -11,6 +11,7 @@
 #include <cstdint>
 #include <cstdio>
 #include <cstring>
+#include <type_traits>
 
 #include "../../include/ad_b200.h"
 
@@ -117,6 +118,28 @@ __device__ __forceinline__ void store_vec(T* p, const Vec<T, V>& x) {
   W w;
   memcpy(&w, &x, sizeof(w));
   *reinterpret_cast<W*>(p) = w;
+}
+
+// V values rounded to elements, two by one instruction where there are two.
+template <typename T, int V>
+__device__ __forceinline__ void round_to(const float* x, Vec<T, V>& y) {
+  if constexpr (sizeof(T) == 2 && V % 2 == 0) {
+#pragma unroll
+    for (int j = 0; j < V; j += 2) {
+      unsigned w;
+      if constexpr (std::is_same<T, __half>::value) {
+        const __half2 h = __floats2half2_rn(x[j], x[j + 1]);
+        memcpy(&w, &h, 4);
+      } else {
+        const __nv_bfloat162 h = __floats2bfloat162_rn(x[j], x[j + 1]);
+        memcpy(&w, &h, 4);
+      }
+      memcpy(&y.v[j], &w, 4);
+    }
+  } else {
+#pragma unroll
+    for (int j = 0; j < V; ++j) y.v[j] = from_float<T>(x[j]);
+  }
 }
 
 // Element i of an array whose type (AD_F32, AD_BF16, AD_F16) is known at run

@@ -20,16 +20,17 @@ struct FinishArgs {
 };
 
 // Columns' sums over the blocks, in their order: 32 columns a block of
-// threads, 8 rows of threads each taking a consecutive share of the blocks.
-__global__ void __launch_bounds__(256) norm_finish_kernel(const __grid_constant__ FinishArgs a) {
-  __shared__ float buf[8][33];
+// threads, 32 rows of threads each taking a consecutive share of the blocks.
+constexpr int FINISH_ROWS = 32;
+__global__ void __launch_bounds__(32 * FINISH_ROWS) norm_finish_kernel(const __grid_constant__ FinishArgs a) {
+  __shared__ float buf[FINISH_ROWS][33];
   const int c = blockIdx.x * 32 + threadIdx.x;
   const int sum = blockIdx.y < 4 ? blockIdx.y : SUM_GATE;
   if (!a.out[sum]) return;
   const long long gate = sum == SUM_GATE ? blockIdx.y - 4 : 0;
   const long long b0 = sum == SUM_GATE ? gate * a.blocks_per_run : 0;
   const long long n = sum == SUM_GATE ? a.blocks_per_run : a.blocks;
-  const long long share = (n + 7) / 8;
+  const long long share = (n + FINISH_ROWS - 1) / FINISH_ROWS;
   float s = 0.0f;
   if (c < a.width) {
     const long long e = min(n, (threadIdx.y + 1) * share);
@@ -38,7 +39,7 @@ __global__ void __launch_bounds__(256) norm_finish_kernel(const __grid_constant_
   buf[threadIdx.y][threadIdx.x] = s;
   __syncthreads();
   if (threadIdx.y == 0 && c < a.width) {
-    for (int k = 1; k < 8; ++k) s += buf[k][threadIdx.x];
+    for (int k = 1; k < FINISH_ROWS; ++k) s += buf[k][threadIdx.x];
     store_any(a.out[sum], a.type[sum], (sum == SUM_GATE ? gate * a.ldg : 0) + c, s);
   }
 }
@@ -207,7 +208,7 @@ extern "C" int ad_block_norm_grad(int device, int dtype, int wtype, int kind, co
   f.ldg = lddg;
   const long long gates = shared ? rows / rows_per_gate : 0;  // fewer than blocks
   if (f.out[SUM_WA] || f.out[SUM_WB] || shared) {
-    norm_finish_kernel<<<dim3((width + 31) / 32, static_cast<unsigned>(4 + gates)), dim3(32, 8), 0, s>>>(f);
+    norm_finish_kernel<<<dim3((width + 31) / 32, static_cast<unsigned>(4 + gates)), dim3(32, FINISH_ROWS), 0, s>>>(f);
     e = cudaGetLastError();
     if (e != cudaSuccess) return fail("ad_block_norm_grad: %s", cudaGetErrorString(e));
   }

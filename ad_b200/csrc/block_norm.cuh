@@ -180,8 +180,8 @@ template <int V>
 __host__ __device__ constexpr int quad() {
   return V < 4 ? V : 4;
 }
-template <typename T, int V, int NV, bool GEN>
-struct Weights {
+template <typename T, int V, int NV, int N>
+struct Weights {  // the first N of them
   const NormArgs& a;
   float* sm;
   int vecs;
@@ -190,7 +190,7 @@ struct Weights {
     if (!a.staged) return;
     const void* from[4] = {a.wa, a.wb, a.ba, a.bb};
 #pragma unroll
-    for (int k = 0; k < (GEN ? 4 : 2); ++k) {
+    for (int k = 0; k < N; ++k) {
       if (!from[k]) continue;
       float o[NV * V];
       load_weights<T, V, NV>(from[k], a.wtype, a.width, o);
@@ -263,8 +263,9 @@ __device__ __forceinline__ void moments(const float (&v)[NV * V], bool layer, in
 // elements too large: they are read when due.
 template <typename T, int V, int NV, int K>
 struct Ahead {
-  // rows: what 512 threads' shares of five operands leave room for
-  static constexpr int S = (sizeof(T) == 4 ? 2 : 4) / (V * NV <= 8 ? 1 : 2);
+  // rows: what 512 threads' shares of five operands leave room for; of the forward
+  // pass's three a few, so that more blocks fit a multiprocessor
+  static constexpr int S = K == 3 ? 2 : (sizeof(T) == 4 ? 2 : 4) / (V * NV <= 8 ? 1 : 2);
   static constexpr bool DIRECT = V == 1 || V * NV > 16;
   unsigned base;
   int width;
@@ -333,7 +334,7 @@ __global__ void __launch_bounds__(MAXT, MAXT == 256 ? (V * NV <= 8 ? 4 : 2) : 1)
     ahead.commit();
   };
   for (int k = 0; k < ahead.S; ++k) fetch(k, blockIdx.x + static_cast<long long>(k) * gridDim.x);
-  const Weights<T, V, NV, GEN> weights(a, staged);
+  const Weights<T, V, NV, GEN ? 4 : 2> weights(a, staged);
   int stage = 0;
   for (long long row = blockIdx.x; row < a.rows; row += gridDim.x) {
     float x[E], u[E], act[E], w[E];
@@ -424,7 +425,7 @@ __global__ void __launch_bounds__(MAXT, MAXT == 256 && V * NV <= 8 ? 2 : 1) norm
     ahead.commit();
   };
   for (int k = 0; k < ahead.S; ++k) fetch(k, r0 + k);
-  const Weights<T, V, NV, GEN> weights(a, staged);
+  const Weights<T, V, NV, GEN ? 3 : 2> weights(a, staged);
   int stage = 0;
   float4 rst = r0 < r1 ? reinterpret_cast<const float4*>(a.stats)[r0] : make_float4(0, 0, 0, 0);
   for (long long row = r0; row < r1; ++row) {
@@ -540,9 +541,9 @@ __global__ void __launch_bounds__(MAXT, MAXT == 256 && V * NV <= 8 ? 2 : 1) norm
 // `ahead`: bytes of the rows to come; `blocks` 0: as many as are resident at a
 // time, each with every so-many-th row.
 template <typename K>
-cudaError_t run_norm(K kernel, NormArgs a, bool gen, int v, int ahead, unsigned blocks, int sms, int threads,
+cudaError_t run_norm(K kernel, NormArgs a, int vectors, int v, int ahead, unsigned blocks, int sms, int threads,
                      cudaStream_t s) {
-  a.staged = ((gen ? 4 : 2) * 4 * ((a.width + v - 1) / v * v) + 15) / 16 * 16;
+  a.staged = (vectors * 4 * ((a.width + v - 1) / v * v) + 15) / 16 * 16;
   if (a.staged > 64 * 1024) a.staged = 0;
   const int bytes = a.staged + ahead;
   if (bytes + 1024 > 48 * 1024) {  // beside what the kernel declares
@@ -564,24 +565,27 @@ cudaError_t start_norm(const NormArgs& a, bool grad, bool gen, unsigned blocks, 
   const bool shared = a.gate && a.rows_per_gate > 1;
   const int f = Ahead<T, V, NV, 3>::bytes(threads), g = Ahead<T, V, NV, 5>::bytes(threads);
   if (!grad)
-    return gen ? run_norm(norm_kernel<T, V, NV, MAXT, true>, a, gen, V, f, 0, sms, threads, s)
-               : run_norm(norm_kernel<T, V, NV, MAXT, false>, a, gen, V, f, 0, sms, threads, s);
+    return gen ? run_norm(norm_kernel<T, V, NV, MAXT, true>, a, 4, V, f, 0, sms, threads, s)
+               : run_norm(norm_kernel<T, V, NV, MAXT, false>, a, 2, V, f, 0, sms, threads, s);
   if (gen)
-    return shared ? run_norm(norm_grad_kernel<T, V, NV, MAXT, true, true>, a, gen, V, g, blocks, sms, threads, s)
-                  : run_norm(norm_grad_kernel<T, V, NV, MAXT, true, false>, a, gen, V, g, blocks, sms, threads, s);
-  return shared ? run_norm(norm_grad_kernel<T, V, NV, MAXT, false, true>, a, gen, V, g, blocks, sms, threads, s)
-                : run_norm(norm_grad_kernel<T, V, NV, MAXT, false, false>, a, gen, V, g, blocks, sms, threads, s);
+    return shared ? run_norm(norm_grad_kernel<T, V, NV, MAXT, true, true>, a, 3, V, g, blocks, sms, threads, s)
+                  : run_norm(norm_grad_kernel<T, V, NV, MAXT, true, false>, a, 3, V, g, blocks, sms, threads, s);
+  return shared ? run_norm(norm_grad_kernel<T, V, NV, MAXT, false, true>, a, 2, V, g, blocks, sms, threads, s)
+                : run_norm(norm_grad_kernel<T, V, NV, MAXT, false, false>, a, 2, V, g, blocks, sms, threads, s);
 }
 
-// Eight elements of a row to a thread while 512 threads are enough for it (what
-// a row costs each warp besides its elements is two sums over the block), 16
-// while 512 are, else 32 to each of up to 1024.  `vec`: all addresses and sizes
+// Eight elements of a row to a thread while 512 threads are enough for it, 16
+// while 512 are, else 32 to each of up to 1024; 16 in the forward pass of rows
+// wide enough for two warps, because what a row costs each warp besides its
+// elements (two sums over the block, addresses) is as much as eight elements do.  `vec`: all addresses and sizes
 // allow 16-byte vectors; single elements else.
 template <typename T>
 cudaError_t start_norm_typed(const NormArgs& a, bool grad, bool gen, bool vec, unsigned blocks, int sms, cudaStream_t s) {
   constexpr int V = 16 / static_cast<int>(sizeof(T));
   auto threads_for = [&](int per) { return ((a.width + per - 1) / per + 31) / 32 * 32; };
-  int t = threads_for(8);
+  int t = threads_for(16);
+  if (!grad && vec && t >= 64 && t <= 256) return start_norm<T, V, 16 / V, 256>(a, grad, gen, blocks, sms, t, s);
+  t = threads_for(8);
   if (t <= 256)
     return vec ? start_norm<T, V, 8 / V, 256>(a, grad, gen, blocks, sms, t, s)
                : start_norm<T, 1, 8, 256>(a, grad, gen, blocks, sms, t, s);

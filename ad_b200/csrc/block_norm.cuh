@@ -550,7 +550,9 @@ cudaError_t run_norm(K kernel, NormArgs a, int vectors, int v, int ahead, unsign
     const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
     if (e != cudaSuccess) return e;
   }
-  if (!blocks) {
+  if (!blocks && a.rows <= sms) {
+    blocks = static_cast<unsigned>(a.rows);
+  } else if (!blocks) {
     int per = 1;
     const cudaError_t e = cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per, kernel, threads, bytes);
     if (e != cudaSuccess) return e;

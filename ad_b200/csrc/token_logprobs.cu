@@ -43,37 +43,55 @@ __device__ __forceinline__ float exp2_approx(float x) {
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
-// max that keeps a NaN
-__device__ __forceinline__ float max_nan(float a, float b) {
-  float y;
-  asm("max.NaN.f32 %0, %1, %2;" : "=f"(y) : "f"(a), "f"(b));
-  return y;
-}
+// Logits beyond this (masks of a type's lowest value, where nothing larger is
+// left) are compared before they are multiplied: their product overflows.
+constexpr float HUGE_LOGIT = 1e30f;
 
-// Running softmax statistics: largest value, sum and sum weighted with the
-// exponent to base 2, both relative to the largest.  -FLT_MAX rather than -inf
-// at the start: -inf values then lie infinitely below it and count for nothing.
+// Running softmax statistics: largest value m, sum and sum weighted with the
+// exponent to base 2, both relative to the offset o = m k (rounded; all that
+// follows goes by the rounded one).  -FLT_MAX rather than -inf at the start:
+// -inf values then lie infinitely below it and count for nothing.
 struct Soft {
-  float m = -FLT_MAX, s = 0.0f, w = 0.0f;
+  float m = -FLT_MAX, o = 0.0f, s = 0.0f, w = 0.0f;
+  __device__ __forceinline__ static bool huge(float m) { return fabsf(m) > HUGE_LOGIT; }
+  // rounded for good: contracted into a later difference it would not be the offset
+  __device__ __forceinline__ static float offset(float m, float k) { return __fmul_rn(m, k); }
+  __device__ __forceinline__ static float below(float m, float o, float to, float to_o, float k) {
+    return fmaxf(huge(m) || huge(to) ? (m - to) * k : o - to_o, GONE);
+  }
   __device__ __forceinline__ void raise(float to, float k) {
-    const float d = max_nan((m - to) * k, GONE), f = exp2_approx(d);
+    const float to_o = offset(to, k), d = below(m, o, to, to_o, k), f = exp2_approx(d);
     w = f * fmaf(d, s, w);
     s *= f;
     m = to;
+    o = to_o;
   }
+  template <bool HUGE>
   __device__ __forceinline__ void add(float x, float k) {
-    const float d = max_nan((x - m) * k, GONE), e = exp2_approx(d);
-    s += e;
-    w = fmaf(e, d, w);
+    const float d = HUGE ? (x - m) * k : fmaf(x, k, -o), e = exp2_approx(d);
+    s += e;  // a NaN stays here
+    w = fmaf(e, fmaxf(d, GONE), w);
   }
   __device__ __forceinline__ void join(float om, float os, float ow, float k) {
     const float to = fmaxf(m, om);
     raise(to, k);
-    Soft o;
-    o.m = om, o.s = os, o.w = ow;
-    o.raise(to, k);
-    s += o.s;
-    w += o.w;
+    Soft other;
+    other.m = om, other.o = offset(om, k), other.s = os, other.w = ow;
+    other.raise(to, k);
+    s += other.s;
+    w += other.w;
+  }
+  __device__ __forceinline__ void join_lanes(float k) {
+#pragma unroll
+    for (int i = 16; i; i >>= 1) {
+      const float om = __shfl_xor_sync(0xffffffffu, m, i), os = __shfl_xor_sync(0xffffffffu, s, i),
+                  ow = __shfl_xor_sync(0xffffffffu, w, i);
+      join(om, os, ow, k);
+    }
+  }
+  // Natural logarithm of a value's share, given that of the sum.
+  __device__ __forceinline__ float log_share(float x, float k, float scale, float ln_s) const {
+    return (huge(m) ? (x - m) * scale : LN2 * fmaf(x, k, -o)) - ln_s;
   }
 };
 
@@ -90,12 +108,14 @@ __device__ __forceinline__ u64 entry_of(float x, unsigned index) {
   return static_cast<u64>(order_of(x)) << 32 | (0xffffffffu - index);
 }
 
-__device__ __forceinline__ u64 exchange(u64 v, int o, bool keep_larger) {
-  const u64 other = __shfl_xor_sync(0xffffffffu, v, o);
+template <typename U>
+__device__ __forceinline__ U exchange(U v, int o, bool keep_larger) {
+  const U other = __shfl_xor_sync(0xffffffffu, v, o);
   return (v > other) == keep_larger ? v : other;
 }
 // Largest first over the lanes of a warp.
-__device__ __forceinline__ u64 sort_warp(u64 v) {
+template <typename U>
+__device__ __forceinline__ U sort_warp(U v) {
   const int lane = threadIdx.x & 31;
 #pragma unroll
   for (int size = 2; size <= 32; size <<= 1)
@@ -175,7 +195,7 @@ struct Shared {
 
 template <typename T, bool TOP>
 __global__ void __launch_bounds__(512) logprob_kernel(const __grid_constant__ LogprobArgs a) {
-  constexpr int V = 16 / sizeof(T), U = 4;  // vectors in flight
+  constexpr int V = 16 / sizeof(T), U = 2;  // vectors in work; as many are under way
   __shared__ Shared sh;
   cg::cluster_group cluster = cg::this_cluster();
   const int parts = cluster.num_blocks(), part = cluster.block_rank();
@@ -197,35 +217,54 @@ __global__ void __launch_bounds__(512) logprob_kernel(const __grid_constant__ Lo
   Best best;
   u64* queue = sh.queue[warp];
 
-  // warp-uniform trip count: the lanes of a warp stay together for the votes
-  for (int base = v0 + warp * 32; base < v1; base += blockDim.x * U) {
-    Vec<T, V> r[U];
+  // The lanes of a warp stay together for the votes; the next vectors are on
+  // their way while these are worked on.
+  Vec<T, V> next[U];
+  const int step = blockDim.x * U;
+  auto fetch = [&](int base) {
 #pragma unroll
     for (int q = 0; q < U; ++q) {
       const int v = base + q * blockDim.x + lane;
       if (v < v1) {
-        r[q] = load_vec<T, V>(x + head + static_cast<long long>(v) * V);
+        next[q] = load_vec<T, V>(x + head + static_cast<long long>(v) * V);
       } else {
 #pragma unroll
-        for (int j = 0; j < V; ++j) r[q].v[j] = from_float<T>(-INFINITY);
+        for (int j = 0; j < V; ++j) next[q].v[j] = from_float<T>(-INFINITY);
       }
     }
+  };
+  int base = v0 + warp * 32;
+  fetch(base);
+  for (bool start = true; start || base < v1; start = false, base += step) {
+    Vec<T, V> r[U];
+#pragma unroll
+    for (int q = 0; q < U; ++q) r[q] = next[q];
+    if (base + step < v1) fetch(base + step);
     float big = -FLT_MAX;
 #pragma unroll
     for (int q = 0; q < U; ++q)
 #pragma unroll
       for (int j = 0; j < V; ++j) big = fmaxf(big, to_float(r[q].v[j]));
     if (big > soft.m) soft.raise(big, k);
+    if (Soft::huge(soft.m)) {
 #pragma unroll
-    for (int q = 0; q < U; ++q)
+      for (int q = 0; q < U; ++q)
 #pragma unroll
-      for (int j = 0; j < V; ++j) soft.add(to_float(r[q].v[j]), k);
+        for (int j = 0; j < V; ++j) soft.add<true>(to_float(r[q].v[j]), k);
+    } else {
+#pragma unroll
+      for (int q = 0; q < U; ++q)
+#pragma unroll
+        for (int j = 0; j < V; ++j) soft.add<false>(to_float(r[q].v[j]), k);
+    }
     if (TOP) {
-      // The first values: the wanted number of lanes' maxima reach `seed`, so no
-      // alternative lies below it.
-      if (best.bar == 0) {
-        const unsigned seed = __shfl_sync(0xffffffffu, static_cast<unsigned>(sort_warp(order_of(big))), a.top - 1);
-        if (seed > order_of(-FLT_MAX)) best.bar = static_cast<u64>(seed) << 32;
+      // The first values: the wanted number of a warp's lanes' maxima reach
+      // `seed`, so no alternative lies below it, nor below the largest seed.
+      if (start) {
+        const unsigned seed = __shfl_sync(0xffffffffu, sort_warp(order_of(big)), a.top - 1);
+        if (lane == 0 && seed > order_of(-FLT_MAX)) atomicMax(&sh.bar, static_cast<u64>(seed) << 32);
+        __syncthreads();
+        best.bar = *reinterpret_cast<volatile u64*>(&sh.bar);
       }
       const float bar = best.bar ? value_of(static_cast<unsigned>(best.bar >> 32)) : -INFINITY;
       if (__any_sync(0xffffffffu, big >= bar || best.bar == 0)) {
@@ -234,7 +273,7 @@ __global__ void __launch_bounds__(512) logprob_kernel(const __grid_constant__ Lo
         for (int q = 0; q < U; ++q)
 #pragma unroll
           for (int j = 0; j < V; ++j)
-            if (base + q * blockDim.x + lane < v1 && to_float(r[q].v[j]) >= bar) pass |= 1u << (q * V + j);
+            if (base + q * static_cast<int>(blockDim.x) + lane < v1 && to_float(r[q].v[j]) >= bar) pass |= 1u << (q * V + j);
         // one a lane at a time, read again: registers cannot be indexed
         while (__any_sync(0xffffffffu, pass != 0)) {
           const int bit = __ffs(pass) - 1;
@@ -253,41 +292,57 @@ __global__ void __launch_bounds__(512) logprob_kernel(const __grid_constant__ Lo
     const float xi = has ? to_float(x[i]) : -INFINITY;
     if (has) {
       if (xi > soft.m) soft.raise(xi, k);
-      soft.add(xi, k);
+      if (Soft::huge(soft.m))
+        soft.add<true>(xi, k);
+      else
+        soft.add<false>(xi, k);
     }
     if (TOP) best.offer(xi, i, has, queue, &sh.bar, a.top);
   }
-  // Lanes, warps, blocks.
-#pragma unroll
-  for (int o = 16; o; o >>= 1) {
-    const float m = __shfl_xor_sync(0xffffffffu, soft.m, o), s = __shfl_xor_sync(0xffffffffu, soft.s, o),
-                w = __shfl_xor_sync(0xffffffffu, soft.w, o);
-    soft.join(m, s, w, k);
-  }
+  // Lanes, warps, blocks; lists by pairs.
+  soft.join_lanes(k);
   if (lane == 0) sh.m[warp] = soft.m, sh.s[warp] = soft.s, sh.w[warp] = soft.w;
   if (TOP) {
     while (best.queued) best.flush(queue, &sh.bar, a.top);
     sh.list[warp][lane] = best.list;
   }
   __syncthreads();
+  if (TOP)
+    for (int n = 1; n < warps; n *= 2) {
+      if (warp % (2 * n) == 0 && warp + n < warps) sh.list[warp][lane] = merge_warp(sh.list[warp][lane], sh.list[warp + n][lane]);
+      __syncthreads();
+    }
   if (warp == 0) {
-    Soft t;
-    for (int i = 0; i < warps; ++i) t.join(sh.m[i], sh.s[i], sh.w[i], k);
-    if (TOP)
-      for (int i = 1; i < warps; ++i) best.list = merge_warp(best.list, sh.list[i][lane]);
-    soft = t;
+    soft = Soft();
+    if (lane < warps) soft.m = sh.m[lane], soft.o = Soft::offset(soft.m, k), soft.s = sh.s[lane], soft.w = sh.w[lane];
+    soft.join_lanes(k);
+    if (TOP) best.list = sh.list[0][lane];
     if (parts > 1) {
-      if (lane == 0) sh.bm = t.m, sh.bs = t.s, sh.bw = t.w;
+      if (lane == 0) sh.bm = soft.m, sh.bs = soft.s, sh.bw = soft.w;
       if (TOP) sh.blist[lane] = best.list;
     }
   }
   if (parts > 1) {
     cluster.sync();
-    if (part == 0 && warp == 0) {
-      for (int i = 1; i < parts; ++i) {
-        const Shared* o = cluster.map_shared_rank(&sh, i);
-        soft.join(o->bm, o->bs, o->bw, k);
-        if (TOP) best.list = merge_warp(best.list, o->blist[lane]);
+    if (part == 0) {
+      if (TOP) {
+        if (warp < parts) sh.list[warp][lane] = cluster.map_shared_rank(&sh, warp)->blist[lane];
+        for (int i = warps + warp; i < parts; i += warps) sh.list[i][lane] = cluster.map_shared_rank(&sh, i)->blist[lane];
+        __syncthreads();
+        for (int n = 1; n < parts; n *= 2) {
+          for (int i = 2 * n * warp; i + n < parts; i += 2 * n * warps)
+            sh.list[i][lane] = merge_warp(sh.list[i][lane], sh.list[i + n][lane]);
+          __syncthreads();
+        }
+      }
+      if (warp == 0) {
+        soft = Soft();
+        if (lane < parts) {
+          const Shared* other = cluster.map_shared_rank(&sh, lane);
+          soft.m = other->bm, soft.o = Soft::offset(soft.m, k), soft.s = other->bs, soft.w = other->bw;
+        }
+        soft.join_lanes(k);
+        if (TOP) best.list = sh.list[0][lane];
       }
     }
     cluster.sync();  // no block ends while its shared memory is read
@@ -302,16 +357,16 @@ __global__ void __launch_bounds__(512) logprob_kernel(const __grid_constant__ Lo
       if (t >= a.vocab)
         lp = __int_as_float(0x7fffffff);
       else if (t >= 0)
-        lp = empty ? -INFINITY : (to_float(x[t]) - soft.m) * a.scale - ln_s;
+        lp = empty ? -INFINITY : soft.log_share(to_float(x[t]), k, a.scale, ln_s);
       const float h = empty ? 0.0f : ln_s - LN2 * (soft.w / soft.s);
       a.logp[row] = lp;
       a.entropy[row] = h;
       reinterpret_cast<float4*>(a.stats)[row] =
-          make_float4(soft.m, soft.s, h, empty ? -INFINITY : fmaf(soft.m, a.scale, ln_s));
+          make_float4(soft.m, soft.s, h, empty ? -INFINITY : (Soft::huge(soft.m) ? soft.m * a.scale : LN2 * soft.o) + ln_s);
     }
     if (TOP && lane < a.top) {
       const float v = value_of(static_cast<unsigned>(best.list >> 32));
-      a.top_logp[row * a.top + lane] = empty ? -INFINITY : (v - soft.m) * a.scale - ln_s;
+      a.top_logp[row * a.top + lane] = empty ? -INFINITY : soft.log_share(v, k, a.scale, ln_s);
       a.top_index[row * a.top + lane] =
           best.list ? static_cast<long long>(0xffffffffu - static_cast<unsigned>(best.list)) : -1ll;
     }
@@ -358,32 +413,36 @@ __global__ void __launch_bounds__(GRAD_THREADS) logprob_grad_kernel(const __grid
   // with l = k (x - m): -k p (g + e (l - ln s + H)) = q exp(l) (g' + e l)
   const float k = a.scale * LOG2E, el = e * LN2;
   const float c = empty ? 0.0f : -a.scale / st.y, b = empty ? 0.0f : g + e * (st.z - logf(st.y));
-  auto grad = [&](float v) {
-    const float d = max_nan((v - st.x) * k, GONE);
-    return c * exp2_approx(d) * fmaf(el, d, b);
-  };
+  const bool huge = Soft::huge(st.x);
+  const float o = Soft::offset(st.x, k);
+  auto grad = [&](float d) { return c * exp2_approx(d) * fmaf(el, fmaxf(d, GONE), b); };
 #pragma unroll
   for (int q = 0; q < GRAD_VECS; ++q) {
     const int v = first + q * GRAD_THREADS;
     if (v >= vecs) continue;
     const int i = head + v * V;
-    float o[V];
+    float z[V];
+    if (huge) {
 #pragma unroll
-    for (int j = 0; j < V; ++j) o[j] = grad(to_float(r[q].v[j]));
+      for (int j = 0; j < V; ++j) z[j] = grad((to_float(r[q].v[j]) - st.x) * k);
+    } else {
+#pragma unroll
+      for (int j = 0; j < V; ++j) z[j] = grad(fmaf(to_float(r[q].v[j]), k, -o));
+    }
     if (t >= i && t < i + V) {
 #pragma unroll
       for (int j = 0; j < V; ++j)
-        if (t == i + j) o[j] += hot;
+        if (t == i + j) z[j] += hot;
     }
     Vec<T, V> w;
-#pragma unroll
-    for (int j = 0; j < V; ++j) w.v[j] = from_float<T>(o[j]);
+    round_to<T, V>(z, w);
     store_vec<T, V>(y + i, w);
   }
   const int rest = head + (a.vocab - tail0);
   if (seg == 0 && static_cast<int>(threadIdx.x) < rest) {
     const int i = static_cast<int>(threadIdx.x) < head ? threadIdx.x : tail0 + (threadIdx.x - head);
-    y[i] = from_float<T>(grad(to_float(x[i])) + (t == i ? hot : 0.0f));
+    const float xi = to_float(x[i]);
+    y[i] = from_float<T>(grad(huge ? (xi - st.x) * k : fmaf(xi, k, -o)) + (t == i ? hot : 0.0f));
   }
 }
 

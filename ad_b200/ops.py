@@ -114,6 +114,33 @@ def _device(x, name):
     return d
 
 
+# What the checks of a call found, by the layouts of its operands (shapes, strides, types, devices)
+# and its options: a program makes the same calls again and again.
+_checked: dict = {}
+
+
+def _layout(x):
+    return None if x is None else (x.shape, x.stride(), x.dtype, x.get_device())
+
+
+def _remember(key, found):
+    if len(_checked) >= 4096:
+        _checked.clear()
+    _checked[key] = found
+    return found
+
+
+_lib = None
+
+
+def _entry(name):
+    """A function of the library, bound once."""
+    global _lib
+    if _lib is None:
+        _lib = rt.lib()
+    return getattr(_lib, name)
+
+
 _torch = None
 
 
@@ -140,6 +167,11 @@ def _stream(device, stream, x, allocates):
 
 def _empty(shape, like, dtype=None):
     return _torch.empty(shape, dtype=like.dtype if dtype is None else getattr(_torch, dtype), device=like.device)
+
+
+def _empty_rows(x):
+    """A row-major array like x."""
+    return _torch.empty_like(x) if x.is_contiguous() else _empty(x.shape, x)
 
 
 def _rows(x, name):
@@ -246,13 +278,7 @@ def _heads(x, name, sequences=None, tokens=None, dim=None):
     return b, t, h, d, _Strides(st[0], st[1], st[2])
 
 
-def rotary(q, k, cos, sin, positions, *, layout: str = "half", inverse: bool = False, out=None, stream=None):
-    """Rotary positions of queries ``q`` and keys ``k`` ([sequences, tokens, heads, dim] or [tokens,
-    heads, dim], any strides with a head's elements adjacent; ``k`` may be None).  ``cos`` and ``sin``:
-    float32 tables [table rows, rotary / 2] (``rotary_table``); the first ``rotary`` elements of each
-    head turn, the others are copied.  ``positions``: int64 or int32, [sequences, tokens] or [tokens]
-    for all sequences; outside the table they make NaNs.  ``inverse`` turns back, which is also the
-    gradient.  ``out``: (q, k) to write, which may be the operands themselves.  Returns (q, k)."""
+def _rotary_operands(q, k, cos, sin, positions, layout):
     if layout not in _LAYOUTS:
         raise ValueError(f"layout: {layout!r} is not one of {list(_LAYOUTS)}")
     dt = _float(q, "q")
@@ -281,6 +307,24 @@ def rotary(q, k, cos, sin, positions, *, layout: str = "half", inverse: bool = F
         _typed(k, dt, "k")
         _on(dev, k, "k")
         _, _, hk, _, sk = _heads(k, "k", b, t, d)
+    return dev, dt, b, t, hq, hk, d, sq, sk, half, p64, p_seq, p_tok
+
+
+def rotary(q, k, cos, sin, positions, *, layout: str = "half", inverse: bool = False, out=None, stream=None):
+    """Rotary positions of queries ``q`` and keys ``k`` ([sequences, tokens, heads, dim] or [tokens,
+    heads, dim], any strides with a head's elements adjacent; ``k`` may be None).  ``cos`` and ``sin``:
+    float32 tables [table rows, rotary / 2] (``rotary_table``); the first ``rotary`` elements of each
+    head turn, the others are copied.  ``positions``: int64 or int32, [sequences, tokens] or [tokens]
+    for all sequences; outside the table they make NaNs.  ``inverse`` turns back, which is also the
+    gradient.  ``out``: (q, k) to write, which may be the operands themselves.  Returns (q, k)."""
+    try:
+        key = (layout, _layout(q), _layout(k), _layout(cos), _layout(sin), _layout(positions))
+        found = _checked.get(key)
+    except (AttributeError, TypeError):  # not all of them device arrays: refused below
+        key = found = None
+    if found is None:
+        found = _remember(key, _rotary_operands(q, k, cos, sin, positions, layout))
+    dev, dt, b, t, hq, hk, d, sq, sk, half, p64, p_seq, p_tok = found
     s = _stream(dev, stream, q, out is None)
     if out is None:
         yq = _torch.empty_like(q)
@@ -296,9 +340,9 @@ def rotary(q, k, cos, sin, positions, *, layout: str = "half", inverse: bool = F
             _on(dev, y, name)
             if any(n > 1 and not m for n, m in zip(y.shape, y.stride())):
                 raise ValueError(f"{name}: elements share memory (strides {tuple(y.stride())})")
-    oq = _heads(yq, "out for q")[4]
-    ok = _heads(yk, "out for k")[4] if yk is not None else None
-    rt.check(rt.lib().ad_rotary(
+    oq = sq if yq.stride() == q.stride() else _heads(yq, "out for q")[4]
+    ok = None if yk is None else sk if yk.stride() == k.stride() else _heads(yk, "out for k")[4]
+    rt.check(_entry("ad_rotary")(
         dev, dt, q.data_ptr(), sq, yq.data_ptr(), oq, hq, k.data_ptr() if k is not None else None, sk,
         yk.data_ptr() if yk is not None else None, ok, hk, b, t, d, 2 * half, _LAYOUTS[layout], inverse,
         cos.data_ptr(), sin.data_ptr(), cos.shape[0], positions.data_ptr(), p64, p_seq, p_tok, s))
@@ -311,6 +355,16 @@ _KINDS = {"rms": 0, "layer": 1}
 
 
 def _norm_operands(x, z, after, before, gate, after_bias, before_bias, kind):
+    try:
+        key = (kind, _layout(x), _layout(z), _layout(after), _layout(before), _layout(gate), _layout(after_bias),
+               _layout(before_bias))
+        found = _checked.get(key)
+    except (AttributeError, TypeError):  # not all of them device arrays: refused below
+        key = found = None
+    return found or _remember(key, _check_norm_operands(x, z, after, before, gate, after_bias, before_bias, kind))
+
+
+def _check_norm_operands(x, z, after, before, gate, after_bias, before_bias, kind):
     """Checks what both directions take: (device, dtype, wtype, rows, width, ldx, ldz, ldg, rows a gate)."""
     if kind not in _KINDS:
         raise ValueError(f"kind: {kind!r} is not one of {list(_KINDS)}")
@@ -366,9 +420,9 @@ def block_norm(x, z, after_weight, before_weight, *, gate=None, after_bias=None,
         x, z, after_weight, before_weight, gate, after_bias, before_bias, kind)
     s = _stream(dev, stream, x, out is None)
     if out is None:
-        h = _empty(x.shape, x)
-        y = None if before_weight is None else _empty(x.shape, x)
-        stats = _empty((rows, 4), x, "float32")
+        h = _empty_rows(x)
+        y = None if before_weight is None else _empty_rows(x)
+        stats = _torch.empty((rows, 4), dtype=_torch.float32, device=x.device)
         ldh = ldy = width
     else:
         h, y, stats = out
@@ -388,7 +442,7 @@ def block_norm(x, z, after_weight, before_weight, *, gate=None, after_bias=None,
         _typed(stats, F32, "out stats")
         _flat(stats, rows * 4, "out stats")
         _on(dev, stats, "out stats")
-    rt.check(rt.lib().ad_block_norm(
+    rt.check(_entry("ad_block_norm")(
         dev, dt, wt, _KINDS[kind], x.data_ptr(), ldx, z.data_ptr(), ldz, _ptr(gate), ldg, per, gate_sigmoid,
         _ptr(after_weight), _ptr(after_bias), _ptr(before_weight), _ptr(before_bias), residual_scale, eps, rows, width,
         h.data_ptr(), ldh, _ptr(y), ldy, stats.data_ptr(), s))
@@ -440,9 +494,8 @@ def block_norm_grad(dh, dy, x, z, after_weight, before_weight, stats, *, gate=No
     s = _stream(dev, stream, x, out is None or workspace is None)
     weights = (after_weight, before_weight, after_bias, before_bias)
     if out is None:
-        g = BlockNormGrads(_empty(x.shape, x), _empty(x.shape, x),
-                           None if gate is None else _empty(gate.shape, gate),
-                           *(None if v is None else _empty(v.shape, v) for v in weights))
+        g = BlockNormGrads(_empty_rows(x), _empty_rows(x), None if gate is None else _empty_rows(gate),
+                           *(None if v is None else _empty_rows(v) for v in weights))
         lddx = lddz = lddg = width
     else:
         g = BlockNormGrads(*out)
@@ -470,7 +523,7 @@ def block_norm_grad(dh, dy, x, z, after_weight, before_weight, stats, *, gate=No
     else:
         _on(dev, workspace, "workspace")
         have = _nbytes(workspace, "workspace")
-    rt.check(rt.lib().ad_block_norm_grad(
+    rt.check(_entry("ad_block_norm_grad")(
         dev, dt, wt, _KINDS[kind], dh.data_ptr(), lds[0], _ptr(dy), lds[1], x.data_ptr(), ldx, z.data_ptr(), ldz,
         _ptr(gate), ldg, per, gate_sigmoid, _ptr(after_weight), _ptr(after_bias), _ptr(before_weight),
         _ptr(before_bias), residual_scale, stats.data_ptr(), rows, width, g.x.data_ptr(), lddx, g.z.data_ptr(), lddz,
@@ -506,6 +559,17 @@ class TokenLogprobs(NamedTuple):
 
 
 def _logit_operands(logits, tokens, scale):
+    if not 0 < scale < math.inf:
+        raise ValueError(f"scale: {scale} is not a positive number")
+    try:
+        key = (_layout(logits), _layout(tokens))
+        found = _checked.get(key)
+    except (AttributeError, TypeError):  # not both of them device arrays: refused below
+        key = found = None
+    return found or _remember(key, _check_logit_operands(logits, tokens))
+
+
+def _check_logit_operands(logits, tokens):
     dt = _float(logits, "logits")
     dev = _device(logits, "logits")
     rows, vocab, ld = _rows(logits, "logits")
@@ -515,8 +579,6 @@ def _logit_operands(logits, tokens, scale):
     _on(dev, tokens, "tokens")
     if vocab < 1:
         raise ValueError("logits: an empty vocabulary")
-    if not 0 < scale < math.inf:
-        raise ValueError(f"scale: {scale} is not a positive number")
     return dev, dt, rows, vocab, ld, t64
 
 
@@ -532,11 +594,11 @@ def token_logprobs(logits, tokens, *, top: int = 0, scale: float = 1.0, out=None
         raise ValueError(f"top: {top} alternatives of {vocab} (at most 32)")
     s = _stream(dev, stream, logits, out is None)
     if out is None:
-        shape = logits.shape[:-1]
-        r = TokenLogprobs(_empty(shape, logits, "float32"), _empty(shape, logits, "float32"),
-                          _empty((rows, 4), logits, "float32"),
-                          _empty((*shape, top), logits, "float32") if top else None,
-                          _empty((*shape, top), logits, "int64") if top else None)
+        shape, device, f32 = logits.shape[:-1], logits.device, _torch.float32
+        r = TokenLogprobs(_torch.empty(shape, dtype=f32, device=device), _torch.empty(shape, dtype=f32, device=device),
+                          _torch.empty((rows, 4), dtype=f32, device=device),
+                          _torch.empty((*shape, top), dtype=f32, device=device) if top else None,
+                          _torch.empty((*shape, top), dtype=_torch.int64, device=device) if top else None)
     else:
         r = TokenLogprobs(*out)
         for v, n, name in ((r.logp, 1, "logp"), (r.entropy, 1, "entropy"), (r.stats, 4, "stats"),
@@ -551,7 +613,7 @@ def token_logprobs(logits, tokens, *, top: int = 0, scale: float = 1.0, out=None
                     _typed(v, F32, "out " + name)
                 _flat(v, rows * n, "out " + name)
                 _on(dev, v, "out " + name)
-    rt.check(rt.lib().ad_token_logprobs(
+    rt.check(_entry("ad_token_logprobs")(
         dev, dt, logits.data_ptr(), ld, rows, vocab, tokens.data_ptr(), t64, scale, top, r.logp.data_ptr(),
         r.entropy.data_ptr(), r.stats.data_ptr(), _ptr(r.top_logp) if top else None,
         _ptr(r.top_index) if top else None, s))
@@ -571,7 +633,7 @@ def token_logprobs_grad(logits, tokens, stats, g_logp=None, g_entropy=None, *, s
             _on(dev, v, name)
     s = _stream(dev, stream, logits, out is None)
     if out is None:
-        out = _empty(logits.shape, logits)
+        out = _empty_rows(logits)
         ldo = vocab
     else:
         _typed(out, dt, "out")
@@ -579,7 +641,7 @@ def token_logprobs_grad(logits, tokens, stats, g_logp=None, g_entropy=None, *, s
         _on(dev, out, "out")
         ldo = _rows(out, "out")[2]
         _apart(ldo, rows, vocab, "out")
-    rt.check(rt.lib().ad_token_logprobs_grad(
+    rt.check(_entry("ad_token_logprobs_grad")(
         dev, dt, logits.data_ptr(), ld, rows, vocab, tokens.data_ptr(), t64, scale, stats.data_ptr(), _ptr(g_logp),
         _ptr(g_entropy), out.data_ptr(), ldo, s))
     return out
@@ -640,7 +702,7 @@ def orthogonalize(g, *, steps: int = 5, coefficients=NEWTON_SCHULZ, eps: float =
     else:
         _on(dev, workspace, "workspace")
         have = _nbytes(workspace, "workspace")
-    rt.check(rt.lib().ad_orthogonalize(
+    rt.check(_entry("ad_orthogonalize")(
         dev, dt, g.data_ptr(), count, rows, cols, sb, sr, sc, steps, (rt.c_float * max(1, len(coef)))(*coef), eps, ot,
         out.data_ptr(), so[0] if len(so) == 3 else 0, so[-2], so[-1], workspace.data_ptr(), have, s))
     return out

@@ -300,10 +300,10 @@ struct Ahead {
                      : "=r"(q.x), "=r"(q.y), "=r"(q.z), "=r"(q.w)
                      : "r"(slot(stage, k, n))
                      : "memory");
-      T e[V];
-      memcpy(e, &q, sizeof(T) * V < 16 ? sizeof(T) * V : 16);
+      float e[16 / sizeof(T)];
+      unpack<T>(q, e);
 #pragma unroll
-      for (int j = 0; j < V; ++j) o[n * V + j] = to_float(e[j]);
+      for (int j = 0; j < V; ++j) o[n * V + j] = e[j];
     }
   }
   static int bytes(int threads) { return DIRECT ? 0 : S * K * NV * threads * 16; }

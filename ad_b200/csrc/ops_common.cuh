@@ -120,6 +120,26 @@ __device__ __forceinline__ void store_vec(T* p, const Vec<T, V>& x) {
   *reinterpret_cast<W*>(p) = w;
 }
 
+// The elements of 16 bytes as floats: an instruction each (two for a pair of
+// halves); taken out of a structure of 16-bit elements they cost two.
+template <typename T>
+__device__ __forceinline__ void unpack(const uint4& q, float* o) {
+  const unsigned w[4] = {q.x, q.y, q.z, q.w};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    if constexpr (sizeof(T) == 4) {
+      o[i] = __uint_as_float(w[i]);
+    } else if constexpr (std::is_same<T, __half>::value) {
+      const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w[i]));
+      o[2 * i] = f.x;
+      o[2 * i + 1] = f.y;
+    } else {
+      o[2 * i] = __uint_as_float(w[i] << 16);
+      o[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+    }
+  }
+}
+
 // V values rounded to elements, two by one instruction where there are two.
 template <typename T, int V>
 __device__ __forceinline__ void round_to(const float* x, Vec<T, V>& y) {

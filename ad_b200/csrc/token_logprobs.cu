@@ -12,7 +12,7 @@
 //
 // Bound by memory: the row is read once, every thread keeping a running
 // maximum, sum and weighted sum that are rescaled together when the maximum
-// grows (once for several vectors, not once a value).  Few rows over a large
+// grows (once for some vectors, not once a value).  Few rows over a large
 // vocabulary are split over a cluster of blocks that join through distributed
 // shared memory.  The best alternatives come from the same pass: a warp keeps
 // its 32 best in registers, one a lane, sorted; values above the worst of the
@@ -25,6 +25,7 @@
 // nothing but -inf has logp = -inf, entropy 0 and no gradient.
 #include <cooperative_groups.h>
 
+#include <algorithm>
 #include <cfloat>
 
 #include "ops_common.cuh"
@@ -66,6 +67,11 @@ struct Soft {
     m = to;
     o = to_o;
   }
+  __device__ __forceinline__ static void plus(float x, float k, float o, float& s, float& w) {
+    const float d = fmaf(x, k, -o), e = exp2_approx(d);
+    s += e;
+    w = fmaf(e, fmaxf(d, GONE), w);
+  }
   template <bool HUGE>
   __device__ __forceinline__ void add(float x, float k) {
     const float d = HUGE ? (x - m) * k : fmaf(x, k, -o), e = exp2_approx(d);
@@ -94,6 +100,38 @@ struct Soft {
     return (huge(m) ? (x - m) * scale : LN2 * fmaf(x, k, -o)) - ln_s;
   }
 };
+
+// The largest of a thread's values, -FLT_MAX at least; NaNs do not count.
+template <typename T, int U>
+__device__ __forceinline__ float largest(const uint4 (&r)[U]) {
+  if constexpr (sizeof(T) == 2) {  // two by one instruction
+    typedef typename std::conditional<std::is_same<T, __half>::value, __half2, __nv_bfloat162>::type T2;
+    T2 big[U * 4];
+#pragma unroll
+    for (int q = 0; q < U; ++q) memcpy(big + q * 4, &r[q], sizeof(r[q]));
+#pragma unroll
+    for (int n = U * 2; n; n /= 2)
+#pragma unroll
+      for (int i = 0; i < n; ++i) big[i] = __hmax2(big[i], big[i + n]);
+    return fmaxf(fmaxf(to_float(big[0].x), to_float(big[0].y)), -FLT_MAX);
+  } else {
+    float big = -FLT_MAX;
+#pragma unroll
+    for (int q = 0; q < U; ++q) {
+      float e[4];
+      unpack<T>(r[q], e);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) big = fmaxf(big, e[j]);
+    }
+    return big;
+  }
+}
+// 16 bytes of -inf
+template <typename T>
+__device__ __forceinline__ uint4 nothing() {
+  const unsigned w = sizeof(T) == 4 ? 0xff800000u : std::is_same<T, __half>::value ? 0xfc00fc00u : 0xff80ff80u;
+  return make_uint4(w, w, w, w);
+}
 
 // Alternatives order by this: larger logit first, then lower index.
 __device__ __forceinline__ unsigned order_of(float x) {
@@ -182,6 +220,7 @@ struct Best {
 };
 
 constexpr int MAX_WARPS = 16;
+constexpr int VECS = 4, AHEAD = 2;  // vectors of a round, rounds under way
 
 struct Shared {
   float m[MAX_WARPS], s[MAX_WARPS], w[MAX_WARPS];
@@ -195,7 +234,7 @@ struct Shared {
 
 template <typename T, bool TOP>
 __global__ void __launch_bounds__(512) logprob_kernel(const __grid_constant__ LogprobArgs a) {
-  constexpr int V = 16 / sizeof(T), U = 2;  // vectors in work; as many are under way
+  constexpr int V = 16 / sizeof(T), U = VECS;
   __shared__ Shared sh;
   cg::cluster_group cluster = cg::this_cluster();
   const int parts = cluster.num_blocks(), part = cluster.block_rank();
@@ -217,45 +256,60 @@ __global__ void __launch_bounds__(512) logprob_kernel(const __grid_constant__ Lo
   Best best;
   u64* queue = sh.queue[warp];
 
-  // The lanes of a warp stay together for the votes; the next vectors are on
-  // their way while these are worked on.
-  Vec<T, V> next[U];
+  // The lanes of a warp stay together for the votes.  Vectors to come are copied
+  // into the thread's own places in shared memory, AHEAD rounds before they are
+  // worked on: there is nothing to wait for but its own copies.
+  typedef uint4 Set[U];
+  extern __shared__ __align__(16) unsigned char ring[];
+  const unsigned places = static_cast<unsigned>(__cvta_generic_to_shared(ring)) + threadIdx.x * 16;
   const int step = blockDim.x * U;
-  auto fetch = [&](int base) {
-#pragma unroll
-    for (int q = 0; q < U; ++q) {
-      const int v = base + q * blockDim.x + lane;
-      if (v < v1) {
-        next[q] = load_vec<T, V>(x + head + static_cast<long long>(v) * V);
-      } else {
-#pragma unroll
-        for (int j = 0; j < V; ++j) next[q].v[j] = from_float<T>(-INFINITY);
-      }
-    }
-  };
   int base = v0 + warp * 32;
-  fetch(base);
-  for (bool start = true; start || base < v1; start = false, base += step) {
-    Vec<T, V> r[U];
-#pragma unroll
-    for (int q = 0; q < U; ++q) r[q] = next[q];
-    if (base + step < v1) fetch(base + step);
-    float big = -FLT_MAX;
+  auto fetch = [&](int stage, int base) {
+    const T* p = x + head + static_cast<long long>(base + lane) * V;
 #pragma unroll
     for (int q = 0; q < U; ++q)
+      if (base + q * static_cast<int>(blockDim.x) + lane < v1)
+        asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(places + (stage * U + q) * blockDim.x * 16),
+                     "l"(p + static_cast<long long>(q * blockDim.x) * V));
+    asm volatile("cp.async.commit_group;" ::: "memory");
+  };
+  auto take = [&](Set& r, int stage, int base) {
+    asm volatile("cp.async.wait_group %0;" ::"n"(AHEAD - 1) : "memory");
 #pragma unroll
-      for (int j = 0; j < V; ++j) big = fmaxf(big, to_float(r[q].v[j]));
+    for (int q = 0; q < U; ++q) {
+      r[q] = nothing<T>();
+      if (base + q * static_cast<int>(blockDim.x) + lane < v1)
+        asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];"
+                     : "=r"(r[q].x), "=r"(r[q].y), "=r"(r[q].z), "=r"(r[q].w)
+                     : "r"(places + (stage * U + q) * blockDim.x * 16)
+                     : "memory");
+    }
+  };
+  auto work = [&](const Set& r, int base, bool start) {
+    const float big = largest<T, U>(r);
     if (big > soft.m) soft.raise(big, k);
     if (Soft::huge(soft.m)) {
 #pragma unroll
-      for (int q = 0; q < U; ++q)
+      for (int q = 0; q < U; ++q) {
+        float e[V];
+        unpack<T>(r[q], e);
 #pragma unroll
-        for (int j = 0; j < V; ++j) soft.add<true>(to_float(r[q].v[j]), k);
+        for (int j = 0; j < V; ++j) soft.add<true>(e[j], k);
+      }
     } else {
+      float s2 = 0.0f, w2 = 0.0f;  // two chains of sums
 #pragma unroll
-      for (int q = 0; q < U; ++q)
+      for (int q = 0; q < U; ++q) {
+        float e[V];
+        unpack<T>(r[q], e);
 #pragma unroll
-        for (int j = 0; j < V; ++j) soft.add<false>(to_float(r[q].v[j]), k);
+        for (int j = 0; j < V; j += 2) {
+          soft.add<false>(e[j], k);
+          Soft::plus(e[j + 1], k, soft.o, s2, w2);
+        }
+      }
+      soft.s += s2;
+      soft.w += w2;
     }
     if (TOP) {
       // The first values: the wanted number of a warp's lanes' maxima reach
@@ -270,10 +324,15 @@ __global__ void __launch_bounds__(512) logprob_kernel(const __grid_constant__ Lo
       if (__any_sync(0xffffffffu, big >= bar || best.bar == 0)) {
         unsigned pass = 0;
 #pragma unroll
-        for (int q = 0; q < U; ++q)
+        for (int q = 0; q < U; ++q) {
+          float e[V];
+          unpack<T>(r[q], e);
+          if (base + q * static_cast<int>(blockDim.x) + lane < v1) {
 #pragma unroll
-          for (int j = 0; j < V; ++j)
-            if (base + q * static_cast<int>(blockDim.x) + lane < v1 && to_float(r[q].v[j]) >= bar) pass |= 1u << (q * V + j);
+            for (int j = 0; j < V; ++j)
+              if (e[j] >= bar) pass |= 1u << (q * V + j);
+          }
+        }
         // one a lane at a time, read again: registers cannot be indexed
         while (__any_sync(0xffffffffu, pass != 0)) {
           const int bit = __ffs(pass) - 1;
@@ -283,6 +342,17 @@ __global__ void __launch_bounds__(512) logprob_kernel(const __grid_constant__ Lo
         }
       }
     }
+  };
+#pragma unroll
+  for (int i = 0; i < AHEAD; ++i) fetch(i, base + i * step);
+  int stage = 0;
+  for (bool start = true; start || base < v1; start = false) {
+    Set r;
+    take(r, stage, base);
+    fetch(stage, base + AHEAD * step);
+    stage = stage + 1 == AHEAD ? 0 : stage + 1;
+    work(r, base, start);
+    base += step;
   }
   // Head and tail: fewer than a vector each, by the first block's first warp.
   if (part == 0 && warp == 0) {
@@ -422,12 +492,19 @@ __global__ void __launch_bounds__(GRAD_THREADS) logprob_grad_kernel(const __grid
     if (v >= vecs) continue;
     const int i = head + v * V;
     float z[V];
+    if constexpr (V == 1) {
+      z[0] = to_float(r[q].v[0]);
+    } else {
+      uint4 w;
+      memcpy(&w, &r[q], sizeof(w));
+      unpack<T>(w, z);
+    }
     if (huge) {
 #pragma unroll
-      for (int j = 0; j < V; ++j) z[j] = grad((to_float(r[q].v[j]) - st.x) * k);
+      for (int j = 0; j < V; ++j) z[j] = grad((z[j] - st.x) * k);
     } else {
 #pragma unroll
-      for (int j = 0; j < V; ++j) z[j] = grad(fmaf(to_float(r[q].v[j]), k, -o));
+      for (int j = 0; j < V; ++j) z[j] = grad(fmaf(z[j], k, -o));
     }
     if (t >= i && t < i + V) {
 #pragma unroll
@@ -449,15 +526,27 @@ __global__ void __launch_bounds__(GRAD_THREADS) logprob_grad_kernel(const __grid
 template <typename T>
 cudaError_t forward(const LogprobArgs& a, int sms, cudaStream_t s) {
   const int vecs = a.vocab / (16 / static_cast<int>(sizeof(T)));
-  // Threads for four vectors each, blocks of a cluster while the rows leave
-  // multiprocessors without work and a block keeps a vector a thread.
+  // Threads for four vectors each; where there are rows enough for all
+  // multiprocessors not so many that joining them costs more than it saves.
+  // Blocks of a cluster while the rows leave multiprocessors without work and a
+  // block keeps a vector a thread.
+  const int most = a.rows >= 4ll * sms ? 256 : 512;
   int threads = 64;
-  while (threads < 512 && threads * 4 < vecs) threads *= 2;
+  while (threads < most && threads * 4 < vecs) threads *= 2;
   int parts = 1;
   while (parts < 8 && a.rows * parts * 2 <= sms && parts * 2 * threads <= vecs) parts *= 2;
+  const int share = (vecs + parts - 1) / parts, rounds = (share + threads * VECS - 1) / (threads * VECS);
+  const int bytes = threads * VECS * 16 * std::min(std::max(rounds, 1), AHEAD);
+  const void* kernel = a.top ? reinterpret_cast<const void*>(logprob_kernel<T, true>)
+                             : reinterpret_cast<const void*>(logprob_kernel<T, false>);
+  if (bytes + static_cast<int>(sizeof(Shared)) + 1024 > 48 * 1024) {
+    const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+    if (e != cudaSuccess) return e;
+  }
   cudaLaunchConfig_t c = {};
   c.gridDim = dim3(static_cast<unsigned>(a.rows * parts));
   c.blockDim = dim3(threads);
+  c.dynamicSmemBytes = bytes;
   c.stream = s;
   cudaLaunchAttribute at[1];
   at[0].id = cudaLaunchAttributeClusterDimension;

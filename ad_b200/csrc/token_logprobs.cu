@@ -237,8 +237,9 @@ __global__ void __launch_bounds__(512) logprob_kernel(const __grid_constant__ Lo
   constexpr int V = 16 / sizeof(T), U = VECS;
   __shared__ Shared sh;
   cg::cluster_group cluster = cg::this_cluster();
-  const int parts = cluster.num_blocks(), part = cluster.block_rank();
-  const long long row = blockIdx.x / parts;
+  const unsigned parts_u = cluster.num_blocks();
+  const int parts = parts_u, part = cluster.block_rank();
+  const long long row = blockIdx.x / parts_u;
   const T* x = static_cast<const T*>(a.logits) + row * a.ld;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
   const float k = a.scale * LOG2E;
@@ -459,8 +460,9 @@ constexpr int GRAD_THREADS = 256, GRAD_VECS = 4;  // a block's share of a row: s
 // V = 1 where rows of the result are not aligned as those of the logits are.
 template <typename T, int V>
 __global__ void __launch_bounds__(GRAD_THREADS) logprob_grad_kernel(const __grid_constant__ LogprobGradArgs a) {
-  const long long row = blockIdx.x / a.segments;
-  const int seg = static_cast<int>(blockIdx.x - row * a.segments);
+  const unsigned row_u = blockIdx.x / static_cast<unsigned>(a.segments);
+  const long long row = row_u;
+  const int seg = blockIdx.x - row_u * a.segments;
   const T* x = static_cast<const T*>(a.logits) + row * a.ld;
   T* y = static_cast<T*>(a.out) + row * a.ldo;
   const int off = static_cast<int>((reinterpret_cast<uintptr_t>(x) & 15) / sizeof(T));
@@ -530,7 +532,7 @@ cudaError_t forward(const LogprobArgs& a, int sms, cudaStream_t s) {
   // multiprocessors not so many that joining them costs more than it saves.
   // Blocks of a cluster while the rows leave multiprocessors without work and a
   // block keeps a vector a thread.
-  const int most = a.rows >= 4ll * sms ? 256 : 512;
+  const int most = a.rows >= 8ll * sms ? 128 : a.rows >= 4ll * sms ? 256 : 512;
   int threads = 64;
   while (threads < most && threads * 4 < vecs) threads *= 2;
   int parts = 1;

@@ -277,6 +277,12 @@ __device__ __forceinline__ int chunks_of(const NsArgs& a, const Item& i) {
   const int width = (i.phase == UPDATE ? a.n : a.m) - i.col * TILE::N;
   return min(TILE::N, width + CHUNK_COLS - 1) / CHUNK_COLS;
 }
+// Whether the right operand is (part of) the left one: tiles on the diagonal of
+// A A^T.  What a block brings from L2 bounds these products, so it comes once.
+template <typename TILE>
+__device__ __forceinline__ bool on_diagonal(const Item& i) {
+  return i.phase != UPDATE && i.col / TILE::RATIO == i.row;
+}
 // Tiles of its matrix that have to be finished before an item's operands are there.
 __device__ __forceinline__ unsigned needed(const NsArgs& a, const Item& i, int ctas) {
   return static_cast<unsigned>(ctas) * (i.step * (2 * a.sym + a.up) + i.phase * a.sym);
@@ -365,6 +371,7 @@ __global__ void __launch_bounds__(THREADS, 1)
         const int kblocks = ((it.phase == GRAM ? a.n : a.m) + BK - 1) / BK;
         const int p0 = it.row * TILE::M + rank * 128;
         const int q0 = it.col * BN + rank * TILE::QN;
+        const bool once = on_diagonal<TILE>(it);
         bool stop = false;
         for (int kb = 0; kb < kblocks; ++kb, ++n) {
           const int i = n % STAGES;
@@ -377,7 +384,8 @@ __global__ void __launch_bounds__(THREADS, 1)
           unsigned char* st = smem + i * TILE::STAGE;
           unsigned bar = smem_u32(&full[i]);
           if (rank == 0)
-            asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(CTAS * TILE::STAGE)
+            asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar),
+                         "r"(CTAS * (once ? TILE::P_BYTES : TILE::STAGE))
                          : "memory");
           if (CTAS == 2) bar = in_block(bar, 0);
           auto load = [&](const CUtensorMap* map, unsigned char* to, int x0, int y0) {
@@ -399,7 +407,7 @@ __global__ void __launch_bounds__(THREADS, 1)
           if (it.phase == UPDATE) {
 #pragma unroll
             for (int h = 0; h < TILE::QN / 64; ++h) load(q, sq + h * BOX, q0 + h * 64, kb * BK);
-          } else {
+          } else if (!once) {
             load(q, sq, kb * BK, q0);
           }
         }
@@ -423,6 +431,7 @@ __global__ void __launch_bounds__(THREADS, 1)
         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
         const unsigned acc = tmem + (c & 1) * BN;
         const unsigned idesc = IDESC | (it.phase == UPDATE ? 1u << 16 : 0u);
+        const int q_at = on_diagonal<TILE>(it) ? it.col % TILE::RATIO * (TILE::QN * BK * 2) : TILE::P_BYTES;
         const unsigned long long q_step = it.phase == UPDATE ? (16 * 128) >> 4 : 32 >> 4;
         bool stop = false;
         for (int kb = 0; kb < kblocks; ++kb, ++n) {
@@ -436,7 +445,7 @@ __global__ void __launch_bounds__(THREADS, 1)
           asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
           unsigned char* st = smem + i * TILE::STAGE;
           const unsigned long long pd = desc_k(st);
-          const unsigned long long qd = it.phase == UPDATE ? desc_n(st + TILE::P_BYTES) : desc_k(st + TILE::P_BYTES);
+          const unsigned long long qd = it.phase == UPDATE ? desc_n(st + q_at) : desc_k(st + q_at);
 #pragma unroll
           for (int k = 0; k < BK / 16; ++k) {
             const unsigned more = (kb > 0 || k > 0) ? 1u : 0u;
@@ -484,7 +493,7 @@ __global__ void __launch_bounds__(THREADS, 1)
       const bool row_in = row < a.m;
       const long long row_all = static_cast<long long>(it.mat) * a.m + row;
       const bool last = it.phase == UPDATE && it.step + 1 == a.steps;
-      const bool mirror = it.phase != UPDATE && it.col / TILE::RATIO != it.row;
+      const bool mirror = it.phase != UPDATE && !on_diagonal<TILE>(it);
       // X = p X + q (acc + d X_hi);  B = p A + q (acc + (d_row + d_col) A);  A = q acc
       const StepScale& sc = a.step[it.step];
       const float p = it.phase == UPDATE ? sc.up_p : sc.poly_p;
@@ -624,7 +633,7 @@ __global__ void __launch_bounds__(THREADS, 1)
         const Item it = item_of<TILE>(a, t);
         const int chunks = chunks_of<TILE>(a, it);
         const bool last = it.phase == UPDATE && it.step + 1 == a.steps;
-        const bool mirror = it.phase != UPDATE && it.col / TILE::RATIO != it.row;
+        const bool mirror = it.phase != UPDATE && !on_diagonal<TILE>(it);
         const int row = it.row * TILE::M + rank * 128;
         const CUtensorMap* to =
             &maps.m[it.phase == GRAM ? CHUNK_A : it.phase == POLY ? CHUNK_B : CHUNK_X + ((it.step + 1) & 1)];

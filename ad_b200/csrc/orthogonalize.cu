@@ -860,8 +860,9 @@ Layout plan(long long count, long long rows, long long cols) {
   Layout l;
   l.m = rows < cols ? rows : cols;
   l.n = rows < cols ? cols : rows;
-  l.ldx = (l.n + 7) / 8 * 8;
-  l.lda = (l.m + 7) / 8 * 8;
+  // rows start on 128-byte lines, or a box's rows would touch two each
+  l.ldx = (l.n + 63) / 64 * 64;
+  l.lda = (l.m + 63) / 64 * 64;
   size_t at = 0;
   auto take = [&](size_t bytes) {
     const size_t here = at;
@@ -922,10 +923,10 @@ Scales scales_for(int steps, const float* coef) {
 
 // The list's tiles for one tile size, and a step's time in us as estimated from
 // measured costs of a tile's 64 elements of K and of a product's start and end:
-// the work shared by all blocks, or one matrix's products one after the other.
-// What a block can bring from L2 (70 to 80 GB/s) bounds the first, so that a
-// large tile costs hardly more than a small one and is taken where there are
-// enough of them.
+// each product in as many rounds as its tiles make for the blocks.  What a block
+// can bring from L2 (70 to 80 GB/s) bounds the first, so that a large tile costs
+// hardly more than a small one: small ones are for matrices that leave most
+// blocks without a large one.
 struct Tiling {
   long long sym, up;
   int row_tiles, sym_cols;
@@ -940,10 +941,8 @@ Tiling tiling(long long count, long long m, long long n, int workers, double per
   for (int i = 0; i < t.row_tiles; ++i) t.sym += std::min(static_cast<long long>(i + 1) * TILE::RATIO, static_cast<long long>(t.sym_cols));
   t.up = t.row_tiles * ((n + TILE::N - 1) / TILE::N);
   const double kn = static_cast<double>((n + BK - 1) / BK), km = static_cast<double>((m + BK - 1) / BK);
-  const double shared = per_kblock * count * (t.sym * (kn + km) + t.up * km) / workers;
-  auto rounds = [&](long long tiles) { return static_cast<double>((tiles + workers - 1) / workers); };
-  const double alone = per_kblock * (rounds(t.sym) * (kn + km) + rounds(t.up) * km) + 3 * 6.0;
-  t.us = std::fmax(shared, alone);
+  auto rounds = [&](long long tiles) { return static_cast<double>((count * tiles + workers - 1) / workers); };
+  t.us = per_kblock * (rounds(t.sym) * (kn + km) + rounds(t.up) * km) + 3 * 6.0;
   return t;
 }
 
@@ -1085,8 +1084,8 @@ extern "C" int ad_orthogonalize(int device, int dtype, const void* g, int64_t co
   const int sms = sm_count(guard.device());
   if (!sms) return fail("ad_orthogonalize: no device properties");
   const Tiling big = tiling<Tile<2, 256>>(count, m, n, sms / 2, 0.45);
-  const Tiling mid = tiling<Tile<1, 128>>(count, m, n, sms, 0.37);
-  const Tiling small = tiling<Tile<1, 64>>(count, m, n, sms, 0.35);
+  const Tiling mid = tiling<Tile<1, 128>>(count, m, n, sms, 0.47);
+  const Tiling small = tiling<Tile<1, 64>>(count, m, n, sms, 0.40);
   const Tiling& best = big.us <= mid.us && big.us <= small.us ? big : mid.us <= small.us ? mid : small;
   if (steps * count * (2 * best.sym + best.up) > 0x3fffffffll) return fail("ad_orthogonalize: too many tiles in one call");
   e = &best == &big   ? start<2, 256>(maps, s, best, sms, guard.device(), st)

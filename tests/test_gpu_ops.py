@@ -732,3 +732,56 @@ def test_orthogonalize_large(ops, count, rows, cols):
     g = update(gen, count, rows, cols, "decay", "float32")
     g += 1e-5 * torch.randn(g.shape, device="cuda", generator=torch.Generator("cuda").manual_seed(1))
     check_orthogonal(ops.orthogonalize(g), orthogonal64(g, 5, [ops.NEWTON_SCHULZ] * 5, 1e-7), 5, "bfloat16")
+
+
+# ------------------------------------------------------------------ together
+
+def test_language_model_step(ops):
+    """The example's gradients against the same model in plain 64-bit torch, and its loss over 40 steps:
+    it starts above that of guessing (ln 61 = 4.1) and all but the second token can be foretold."""
+    import importlib.util
+    import os
+    path = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "examples", "lm_step.py")
+    spec = importlib.util.spec_from_file_location("lm_step", path)
+    lm = importlib.util.module_from_spec(spec)
+    spec.loader.exec_module(lm)
+    model = lm.Model(vocab=61, width=64, heads=4, hidden=128, layers=2, length=16)
+    tokens = torch.randint(0, 61, (5, 16), device="cuda", generator=torch.Generator("cuda").manual_seed(3))
+    model.loss(tokens).backward()
+
+    def plain(p):  # the parameters in 64 bits
+        def norm(v, w):
+            return v * torch.rsqrt(v.square().mean(-1, keepdim=True) + 1e-5) * w
+
+        def turn(v):
+            u, w = v[..., :8], v[..., 8:]
+            c, s = model.cos.double()[:16, None], model.sin.double()[:16, None]
+            return torch.cat((u * c - w * s, w * c + u * s), -1)
+
+        x = p["embedding"][tokens].reshape(80, 64)
+        y = norm(x, p["first"])
+        for m, v6 in zip(p["matrices"], p["vectors"]):
+            q, k, v = (t.reshape(5, 16, 4, 16) for t in (y @ m["qkv"].T).chunk(3, -1))
+            s = torch.einsum("bthd,bshd->bhts", turn(q), turn(k)) / 4 + model.mask.double()
+            z = torch.einsum("bhts,bshd->bthd", s.softmax(-1), v).reshape(80, 64) @ m["out"].T
+            x = x + torch.sigmoid(v6[4]) * norm(z, v6[0])
+            y = norm(x, v6[1])
+            x = x + torch.sigmoid(v6[5]) * norm(torch.relu(y @ m["up"].T) @ m["down"].T, v6[2])
+            y = norm(x, v6[3])
+        lp = torch.log_softmax(y @ p["embedding"].T, -1).reshape(5, 16, 61)[:, :-1]
+        return -lp.gather(-1, tokens[:, 1:, None]).sum() / 75
+
+    p = dict(embedding=model.embedding, first=model.first, matrices=model.matrices, vectors=model.vectors)
+    double = lambda t: t.detach().double().requires_grad_()  # noqa: E731
+    p64 = dict(embedding=double(p["embedding"]), first=double(p["first"]),
+               matrices=[{k: double(v) for k, v in m.items()} for m in p["matrices"]],
+               vectors=[[double(v) for v in layer] for layer in p["vectors"]])
+    plain(p64).backward()
+    pairs = [(p["embedding"], p64["embedding"]), (p["first"], p64["first"])]
+    pairs += [(a[k], b[k]) for a, b in zip(p["matrices"], p64["matrices"]) for k in a]
+    pairs += [(a, b) for x, y in zip(p["vectors"], p64["vectors"]) for a, b in zip(x, y)]
+    for a, b in pairs:
+        # two layers of products and norms in 32 bits: some thousand roundings on the way, norm-wise
+        assert float((a.grad.double() - b.grad).norm()) <= 2000 * E * float(b.grad.norm())
+    losses = lm.main(40)
+    assert losses[0] > 4.0 and losses[-1] < 0.5 * losses[0]

@@ -349,7 +349,7 @@ __global__ void __launch_bounds__(MAXT, MAXT == 256 ? (V * NV <= 8 ? 4 : 2) : 1)
       moments<V, NV>(u, GEN && a.layer, a.width, a.eps, smem, flip, mz, rz);
       weights.get(W_WA, w);
 #pragma unroll
-      for (int i = 0; i < E; ++i) u[i] = (u[i] - mz) * rz * w[i];
+      for (int i = 0; i < E; ++i) u[i] = (GEN ? u[i] - mz : u[i]) * rz * w[i];
       if (GEN && a.ba) {
         weights.get(W_BA, w);
 #pragma unroll
@@ -368,7 +368,7 @@ __global__ void __launch_bounds__(MAXT, MAXT == 256 ? (V * NV <= 8 ? 4 : 2) : 1)
       moments<V, NV>(x, GEN && a.layer, a.width, a.eps, smem, flip, mh, rh);
       weights.get(W_WB, w);
 #pragma unroll
-      for (int i = 0; i < E; ++i) x[i] = (x[i] - mh) * rh * w[i];
+      for (int i = 0; i < E; ++i) x[i] = (GEN ? x[i] - mh : x[i]) * rh * w[i];
       if (GEN && a.bb) {
         weights.get(W_BB, w);
 #pragma unroll
@@ -455,7 +455,7 @@ __global__ void __launch_bounds__(MAXT, MAXT == 256 && V * NV <= 8 ? 2 : 1) norm
       weights.get(W_WA, w);
 #pragma unroll
       for (int i = 0; i < E; ++i) {
-        nz[i] = (nz[i] - mz) * rz;
+        nz[i] = (GEN ? nz[i] - mz : nz[i]) * rz;
         u[i] = nz[i] * w[i];
       }
       if (GEN && a.ba) {
@@ -469,7 +469,8 @@ __global__ void __launch_bounds__(MAXT, MAXT == 256 && V * NV <= 8 ? 2 : 1) norm
       weights.get(W_WB, w);
 #pragma unroll
       for (int i = 0; i < E; ++i) {
-        nh[i] = (fmaf(a.scale, nh[i], act[i] * u[i]) - mh) * rh;
+        nh[i] = fmaf(a.scale, nh[i], act[i] * u[i]);
+        nh[i] = (GEN ? nh[i] - mh : nh[i]) * rh;
         swb[i] = fmaf(d[i], nh[i], swb[i]);
         if (GEN) sbb[i] += d[i];
         d[i] *= w[i];

@@ -949,30 +949,35 @@ Tiling tiling(long long count, long long m, long long n, int workers, double per
 template <int CTAS, int BN>
 cudaError_t start(const Maps& maps, NsArgs& a, const Tiling& t, int sms, int device, cudaStream_t st) {
   using TILE = Tile<CTAS, BN>;
-  static bool ready[64] = {};
-  if (device >= 64 || !ready[device]) {
-    const cudaError_t e =
-        cudaFuncSetAttribute(ns_kernel<CTAS, BN>, cudaFuncAttributeMaxDynamicSharedMemorySize, TILE::SMEM);
-    if (e != cudaSuccess) return e;
-    if (device < 64) ready[device] = true;
-  }
-  a.sym = static_cast<int>(t.sym), a.up = static_cast<int>(t.up);
-  a.row_tiles = t.row_tiles, a.sym_cols = t.sym_cols;
-  const long long most = a.count * std::max(t.sym, t.up);  // tiles of one product
-  const int workers = static_cast<int>(std::min<long long>(sms / CTAS, most));
   cudaLaunchConfig_t c = {};
-  c.gridDim = dim3(workers * CTAS);
   c.blockDim = dim3(THREADS);
   c.dynamicSmemBytes = TILE::SMEM;
   c.stream = st;
   cudaLaunchAttribute at[2];
-  at[0].id = cudaLaunchAttributeCooperative;  // blocks wait for one another: all of them have to be resident
-  at[0].val.cooperative = 1;
-  at[1].id = cudaLaunchAttributeClusterDimension;
-  at[1].val.clusterDim.x = CTAS;
-  at[1].val.clusterDim.y = at[1].val.clusterDim.z = 1;
+  at[0].id = cudaLaunchAttributeClusterDimension;
+  at[0].val.clusterDim.x = CTAS;
+  at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
+  at[1].id = cudaLaunchAttributeCooperative;  // blocks wait for one another: all of them have to be resident
+  at[1].val.cooperative = 1;
   c.attrs = at;
-  c.numAttrs = CTAS == 1 ? 1 : 2;
+  static int resident[64] = {};  // blocks or pairs of them at a time, asked for once
+  int most_workers = device < 64 ? resident[device] : 0;
+  if (!most_workers) {
+    cudaError_t e = cudaFuncSetAttribute(ns_kernel<CTAS, BN>, cudaFuncAttributeMaxDynamicSharedMemorySize, TILE::SMEM);
+    if (e != cudaSuccess) return e;
+    c.gridDim = dim3(sms / CTAS * CTAS);
+    c.numAttrs = 1;
+    e = cudaOccupancyMaxActiveClusters(&most_workers, ns_kernel<CTAS, BN>, &c);
+    if (e != cudaSuccess) return e;
+    most_workers = std::min(most_workers, sms / CTAS);
+    if (most_workers < 1) return cudaErrorCooperativeLaunchTooLarge;
+    if (device < 64) resident[device] = most_workers;
+  }
+  a.sym = static_cast<int>(t.sym), a.up = static_cast<int>(t.up);
+  a.row_tiles = t.row_tiles, a.sym_cols = t.sym_cols;
+  const long long most = a.count * std::max(t.sym, t.up);  // tiles of one product
+  c.gridDim = dim3(static_cast<unsigned>(std::min<long long>(most_workers, most)) * CTAS);
+  c.numAttrs = 2;
   return cudaLaunchKernelEx(&c, ns_kernel<CTAS, BN>, maps, a);
 }
 

@@ -422,7 +422,7 @@ def block_norm(x, z, after_weight, before_weight, *, gate=None, after_bias=None,
     if out is None:
         h = _empty_rows(x)
         y = None if before_weight is None else _empty_rows(x)
-        stats = _torch.empty((rows, 4), dtype=_torch.float32, device=x.device)
+        stats = x.new_empty((rows, 4), dtype=_torch.float32)
         ldh = ldy = width
     else:
         h, y, stats = out
@@ -594,11 +594,11 @@ def token_logprobs(logits, tokens, *, top: int = 0, scale: float = 1.0, out=None
         raise ValueError(f"top: {top} alternatives of {vocab} (at most 32)")
     s = _stream(dev, stream, logits, out is None)
     if out is None:
-        shape, device, f32 = logits.shape[:-1], logits.device, _torch.float32
-        r = TokenLogprobs(_torch.empty(shape, dtype=f32, device=device), _torch.empty(shape, dtype=f32, device=device),
-                          _torch.empty((rows, 4), dtype=f32, device=device),
-                          _torch.empty((*shape, top), dtype=f32, device=device) if top else None,
-                          _torch.empty((*shape, top), dtype=_torch.int64, device=device) if top else None)
+        shape, new, f32 = logits.shape[:-1], logits.new_empty, _torch.float32
+        stats = new((rows, 4), dtype=f32)
+        r = TokenLogprobs(new(shape, dtype=f32), new(shape, dtype=f32), stats,
+                          new((*shape, top), dtype=f32) if top else None,
+                          new((*shape, top), dtype=_torch.int64) if top else None)
     else:
         r = TokenLogprobs(*out)
         for v, n, name in ((r.logp, 1, "logp"), (r.entropy, 1, "entropy"), (r.stats, 4, "stats"),

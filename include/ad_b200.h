@@ -244,7 +244,9 @@ int ad_token_logprobs_grad(int device, int dtype, const void* logits, int64_t ld
  * take operands of 11 bits and accumulate in 32: the result is within about
  * 1e-3 (norm-wise) of the exact iteration.  Coefficients that let a singular
  * value grow past 1024 are refused.  A zero matrix gives zeros, one with NaN or
- * infinity NaNs.  The workspace is 256-byte aligned. */
+ * infinity NaNs.  Blocks wait for one another inside the one cooperative
+ * kernel; a wait that runs out (2 s) leaves NaNs in the result.  The workspace
+ * is 256-byte aligned. */
 int ad_orthogonalize_workspace(int64_t count, int64_t rows, int64_t cols, size_t* bytes);
 int ad_orthogonalize(int device, int dtype, const void* g, int64_t count, int64_t rows,
                      int64_t cols, int64_t batch_stride, int64_t row_stride, int64_t col_stride,

@@ -49,11 +49,11 @@ __global__ void __launch_bounds__(32 * FINISH_ROWS) norm_finish_kernel(const __g
 struct Split {
   long long run, blocks_per_run, rows_per_block, blocks;
 };
-Split split_rows(long long rows, long long rows_per_gate, int width, int sms) {
+Split split_rows(long long rows, long long rows_per_gate, int width, bool slim, int sms) {
   Split s;
   s.run = rows_per_gate > 1 ? rows_per_gate : rows;
-  // 512 threads with eight elements each to a multiprocessor, in as many blocks as that makes
-  const int per_sm = std::max(1, std::min(16, 4096 / width));
+  // 512 or 768 threads with eight elements each to a multiprocessor, in as many blocks as that makes
+  const int per_sm = std::max(1, std::min(16, (slim ? 6144 : 4096) / width));
   const long long runs = rows / s.run, want = static_cast<long long>(per_sm) * sms;
   if (runs >= want) {
     s.blocks_per_run = 0;
@@ -138,7 +138,8 @@ extern "C" int ad_block_norm_grad_workspace(int device, int64_t rows, int width,
   const int sms = g.error() == cudaSuccess ? sm_count(g.device()) : 0;
   if (!sms) return fail("ad_block_norm_grad_workspace: no device properties");
   if (rows_per_gate && rows % rows_per_gate) return fail("ad_block_norm_grad_workspace: rows cannot share gates so");
-  *bytes = sizeof(float) * SUMS * static_cast<size_t>(split_rows(rows, rows_per_gate, width, sms).blocks) * width;
+  // for the kernels with the most blocks
+  *bytes = sizeof(float) * SUMS * static_cast<size_t>(split_rows(rows, rows_per_gate, width, true, sms).blocks) * width;
   return 0;
 }
 
@@ -172,7 +173,8 @@ extern "C" int ad_block_norm_grad(int device, int dtype, int wtype, int kind, co
     return fail("ad_block_norm_grad: null or unaligned operand");
   const int sms = sm_count(g.device());
   if (!sms) return fail("ad_block_norm_grad: no device properties");
-  const Split split = split_rows(rows, gate ? rows_per_gate : 0, width, sms);
+  const Split split = split_rows(rows, gate ? rows_per_gate : 0, width,
+                                 elem_size(dtype) == 2 && !kind && !ba && !bb, sms);
   const size_t need = sizeof(float) * SUMS * static_cast<size_t>(split.blocks) * width;
   if (!workspace || !aligned(workspace, 16) || workspace_bytes < need)
     return fail("ad_block_norm_grad: needs %zu bytes of workspace, 16-byte aligned", need);

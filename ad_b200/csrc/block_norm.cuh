@@ -255,17 +255,14 @@ __device__ __forceinline__ void moments(const float (&v)[NV * V], bool layer, in
   r = 1.0f / sqrtf(s[0] / width + eps);
 }
 
-// The rows to come of K operands, brought into shared memory while earlier ones
+// The S rows to come of K operands, brought into shared memory while earlier ones
 // are worked on.  A thread copies and reads its own vectors only, so there is
 // nothing to wait for but its own copies.  (Kept in registers instead, the next
 // row was waited for all the same: 888 us for 65535 x 2048 bf16 gradients.)
 // Single elements (V = 1) are too small for such copies and rows of over 8192
 // elements too large: they are read when due.
-template <typename T, int V, int NV, int K>
+template <typename T, int V, int NV, int K, int S>
 struct Ahead {
-  // rows: what 512 threads' shares of five operands leave room for; of the forward
-  // pass's three a few, so that more blocks fit a multiprocessor
-  static constexpr int S = K == 3 ? 2 : (sizeof(T) == 4 ? 2 : 4) / (V * NV <= 8 ? 1 : 2);
   static constexpr bool DIRECT = V == 1 || V * NV > 16;
   unsigned base;
   int width;
@@ -309,6 +306,22 @@ struct Ahead {
   static int bytes(int threads) { return DIRECT ? 0 : S * K * NV * threads * 16; }
 };
 
+constexpr int FORWARD_ROWS = 2;
+// Whether the gradient's registers are held down so that 768 threads fit a
+// multiprocessor rather than 512: without means and biases, for 16-bit elements,
+// that costs nothing (65535 x 2048 bf16: 723 -> 671 us); else the sums spill
+// (16384 x 1024 fp32 LayerNorm: 163 -> 211 us).
+template <typename T, bool GEN>
+__host__ __device__ constexpr bool slim() {
+  return sizeof(T) == 2 && !GEN;
+}
+// Rows that the gradient copies ahead: what the threads' shares of five operands
+// leave room for.
+template <typename T, int V, int NV, int MAXT, bool GEN>
+__host__ __device__ constexpr int grad_rows() {
+  return sizeof(T) == 4 ? (MAXT == 768 || V * NV > 8 ? 1 : 2) : (MAXT == 768 || V * NV > 8 || slim<T, GEN>() ? 2 : 4);
+}
+
 // GEN: with a LayerNorm's means or with biases; without it both are known to be
 // absent.  MAXT: threads a block may have; with 256 of them several blocks share
 // a multiprocessor.
@@ -321,7 +334,7 @@ __global__ void __launch_bounds__(MAXT, MAXT == 256 ? (V * NV <= 8 ? 4 : 2) : 1)
   extern __shared__ __align__(16) float staged[];
   int flip = 0;
   constexpr int E = NV * V;
-  const Ahead<T, V, NV, 3> ahead(staged + a.staged / 4, a.width);
+  const Ahead<T, V, NV, 3, FORWARD_ROWS> ahead(staged + a.staged / 4, a.width);
   auto pz = [&](long long row) { return static_cast<const T*>(a.z) + at(row, a.ldz); };
   auto px = [&](long long row) { return static_cast<const T*>(a.x) + at(row, a.ldx); };
   auto pg = [&](long long row) { return static_cast<const T*>(a.gate) + at(gate_row(a, row), a.ldg); };
@@ -333,7 +346,7 @@ __global__ void __launch_bounds__(MAXT, MAXT == 256 ? (V * NV <= 8 ? 4 : 2) : 1)
     }
     ahead.commit();
   };
-  for (int k = 0; k < ahead.S; ++k) fetch(k, blockIdx.x + static_cast<long long>(k) * gridDim.x);
+  for (int k = 0; k < FORWARD_ROWS; ++k) fetch(k, blockIdx.x + static_cast<long long>(k) * gridDim.x);
   const Weights<T, V, NV, GEN ? 4 : 2> weights(a, staged);
   int stage = 0;
   for (long long row = blockIdx.x; row < a.rows; row += gridDim.x) {
@@ -342,8 +355,8 @@ __global__ void __launch_bounds__(MAXT, MAXT == 256 ? (V * NV <= 8 ? 4 : 2) : 1)
     ahead.read(stage, 0, pz(row), u);
     ahead.read(stage, 1, px(row), x);
     if (a.gate) ahead.read(stage, 2, pg(row), act);
-    fetch(stage, row + static_cast<long long>(ahead.S) * gridDim.x);
-    stage = stage + 1 == ahead.S ? 0 : stage + 1;
+    fetch(stage, row + static_cast<long long>(FORWARD_ROWS) * gridDim.x);
+    stage = stage + 1 == FORWARD_ROWS ? 0 : stage + 1;
     float mz = 0.0f, rz = 1.0f, mh = 0.0f, rh = 1.0f;
     if (a.wa) {
       moments<V, NV>(u, GEN && a.layer, a.width, a.eps, smem, flip, mz, rz);
@@ -386,7 +399,7 @@ enum { SUM_WA = 0, SUM_WB = 1, SUM_BA = 2, SUM_BB = 3, SUM_GATE = 4, SUMS = 5 };
 
 // SHARED: the gate's rows are shared, its gradient is a sum over rows.
 template <typename T, int V, int NV, int MAXT, bool GEN, bool SHARED>
-__global__ void __launch_bounds__(MAXT, MAXT == 256 && V * NV <= 8 ? 2 : 1) norm_grad_kernel(const __grid_constant__ NormArgs a) {
+__global__ void __launch_bounds__(MAXT, MAXT != 256 || V * NV > 8 ? 1 : slim<T, GEN>() ? 3 : 2) norm_grad_kernel(const __grid_constant__ NormArgs a) {
   __shared__ __align__(16) float smem[2 * 2 * 32];
   for (int i = threadIdx.x; i < 2 * 2 * 32; i += blockDim.x) smem[i] = 0.0f;
   __syncthreads();
@@ -406,7 +419,8 @@ __global__ void __launch_bounds__(MAXT, MAXT == 256 && V * NV <= 8 ? 2 : 1) norm
   long long left = a.run;  // rows of the run to come
   const bool layer = GEN && a.layer;
   const float inv = 1.0f / a.width;
-  const Ahead<T, V, NV, 5> ahead(staged + a.staged / 4, a.width);
+  constexpr int S = grad_rows<T, V, NV, MAXT, GEN>();
+  const Ahead<T, V, NV, 5, S> ahead(staged + a.staged / 4, a.width);
   auto pz = [&](long long row) { return static_cast<const T*>(a.z) + at(row, a.ldz); };
   auto px = [&](long long row) { return static_cast<const T*>(a.x) + at(row, a.ldx); };
   auto pg = [&](long long row) { return static_cast<const T*>(a.gate) + at(gate_row(a, row), a.ldg); };
@@ -424,7 +438,7 @@ __global__ void __launch_bounds__(MAXT, MAXT == 256 && V * NV <= 8 ? 2 : 1) norm
     }
     ahead.commit();
   };
-  for (int k = 0; k < ahead.S; ++k) fetch(k, r0 + k);
+  for (int k = 0; k < S; ++k) fetch(k, r0 + k);
   const Weights<T, V, NV, GEN ? 3 : 2> weights(a, staged);
   int stage = 0;
   float4 rst = r0 < r1 ? reinterpret_cast<const float4*>(a.stats)[r0] : make_float4(0, 0, 0, 0);
@@ -446,8 +460,8 @@ __global__ void __launch_bounds__(MAXT, MAXT == 256 && V * NV <= 8 ? 2 : 1) norm
 #pragma unroll
       for (int i = 0; i < E; ++i) act[i] = 1.0f;
     }
-    fetch(stage, row + ahead.S);
-    stage = stage + 1 == ahead.S ? 0 : stage + 1;
+    fetch(stage, row + S);
+    stage = stage + 1 == S ? 0 : stage + 1;
     if (row + 1 < r1) rst = reinterpret_cast<const float4*>(a.stats)[row + 1];
 #pragma unroll
     for (int i = 0; i < E; ++i) u[i] = nz[i];
@@ -566,7 +580,9 @@ cudaError_t run_norm(K kernel, NormArgs a, int vectors, int v, int ahead, unsign
 template <typename T, int V, int NV, int MAXT>
 cudaError_t start_norm(const NormArgs& a, bool grad, bool gen, unsigned blocks, int sms, int threads, cudaStream_t s) {
   const bool shared = a.gate && a.rows_per_gate > 1;
-  const int f = Ahead<T, V, NV, 3>::bytes(threads), g = Ahead<T, V, NV, 5>::bytes(threads);
+  const int f = Ahead<T, V, NV, 3, FORWARD_ROWS>::bytes(threads);
+  const int g = gen ? Ahead<T, V, NV, 5, grad_rows<T, V, NV, MAXT, true>()>::bytes(threads)
+                    : Ahead<T, V, NV, 5, grad_rows<T, V, NV, MAXT, false>()>::bytes(threads);
   if (!grad)
     return gen ? run_norm(norm_kernel<T, V, NV, MAXT, true>, a, 4, V, f, 0, sms, threads, s)
                : run_norm(norm_kernel<T, V, NV, MAXT, false>, a, 2, V, f, 0, sms, threads, s);
@@ -577,8 +593,9 @@ cudaError_t start_norm(const NormArgs& a, bool grad, bool gen, unsigned blocks, 
                 : run_norm(norm_grad_kernel<T, V, NV, MAXT, false, false>, a, 2, V, g, blocks, sms, threads, s);
 }
 
-// Eight elements of a row to a thread while 512 threads are enough for it, 16
-// while 512 are, else 32 to each of up to 1024; 16 in the forward pass of rows
+// Eight elements of a row to a thread while 512 threads are enough for it (768
+// in the gradient, whose sums for 16 do not fit a thread's registers), 16 while
+// 512 are, else 32 to each of up to 1024; 16 in the forward pass of rows
 // wide enough for two warps, because what a row costs each warp besides its
 // elements (two sums over the block, addresses) is as much as eight elements do.  `vec`: all addresses and sizes
 // allow 16-byte vectors; single elements else.
@@ -595,6 +612,7 @@ cudaError_t start_norm_typed(const NormArgs& a, bool grad, bool gen, bool vec, u
   if (t <= 512)
     return vec ? start_norm<T, V, 8 / V, 512>(a, grad, gen, blocks, sms, t, s)
                : start_norm<T, 1, 8, 512>(a, grad, gen, blocks, sms, t, s);
+  if (grad && vec && t <= 768) return start_norm<T, V, 8 / V, 768>(a, grad, gen, blocks, sms, t, s);
   t = threads_for(16);
   if (t <= 512)
     return vec ? start_norm<T, V, 16 / V, 512>(a, grad, gen, blocks, sms, t, s)

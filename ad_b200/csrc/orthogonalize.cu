@@ -146,11 +146,13 @@ __device__ __forceinline__ unsigned load_acquire(const unsigned* p) {
   return v;
 }
 __device__ __noinline__ bool count_wait(const unsigned* p, unsigned need, volatile int* gave_up) {
+  if (load_acquire(p) >= need) return true;
   const unsigned long long t0 = now();
-  while (load_acquire(p) < need) {
+  while (true) {
+    for (int i = 0; i < 32; ++i)
+      if (load_acquire(p) >= need) return true;
     if (*gave_up || now() - t0 > PATIENCE) return false;
   }
-  return true;
 }
 
 // Shared-memory descriptors, 128-byte swizzle.  K-major: 8 rows of 128 bytes
@@ -363,7 +365,7 @@ __global__ void __launch_bounds__(THREADS, 1)
           break;
         }
         // what others wrote through the generic proxy is read through the async one
-        asm volatile("fence.proxy.async;" ::: "memory");
+        asm volatile("fence.proxy.async.global;" ::: "memory");
         const int x = it.step & 1;
         const CUtensorMap* p = &maps.m[it.phase == GRAM ? WIDE_X + x : it.phase == POLY ? WIDE_A : WIDE_B];
         const CUtensorMap* q = it.phase == UPDATE ? &maps.m[NARROW_X + x]
@@ -601,7 +603,7 @@ __global__ void __launch_bounds__(THREADS, 1)
           atomicExch(a.err, 6);
           break;
         }
-        asm volatile("fence.proxy.async;" ::: "memory");
+        asm volatile("fence.proxy.async.global;" ::: "memory");
         const int row = it.row * TILE::M + rank * 128;
         for (int ch = 0; ch < chunks; ++ch, ++e) {
           const int b = e % SIDES;
@@ -668,7 +670,7 @@ __global__ void __launch_bounds__(THREADS, 1)
         if (!stop && !last) {
           // written, and there for other blocks' copies
           asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
-          asm volatile("fence.proxy.async;" ::: "memory");
+          asm volatile("fence.proxy.async.global;" ::: "memory");
           asm volatile("red.release.gpu.global.add.u32 [%0], 1;" ::"l"(a.ready + it.mat) : "memory");
         }
       }

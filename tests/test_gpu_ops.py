@@ -785,3 +785,49 @@ def test_language_model_step(ops):
         assert float((a.grad.double() - b.grad).norm()) <= 2000 * E * float(b.grad.norm())
     losses = lm.main(40)
     assert losses[0] > 4.0 and losses[-1] < 0.5 * losses[0]
+
+
+# ------------------------------------------------------------------ far apart and many
+
+def test_offsets_past_32_bits(ops):
+    """Rows (tokens, matrices) 2^31 elements apart give the bits of rows side by side."""
+    far = 2 ** 31
+    store = torch.empty(far + 70000, dtype=torch.bfloat16, device="cuda")
+    gen = seeded(77)
+    near = rand(gen, (2, 1000), "bfloat16", 2.0)
+    x = store.as_strided((2, 1000), (far, 1))
+    x.copy_(near)
+    tok = torch.tensor([3, 999], device="cuda")
+    a, b = ops.token_logprobs(x, tok, top=4), ops.token_logprobs(near, tok, top=4)
+    assert all(torch.equal(u, v) for u, v in zip(a, b))
+    g = torch.ones(2, device="cuda")
+    assert torch.equal(ops.token_logprobs_grad(x, tok, a.stats, g), ops.token_logprobs_grad(near, tok, b.stats, g))
+    cos, sin = (torch.from_numpy(v).cuda() for v in ops.rotary_table(8, 40))
+    q, pos = x.view(1, 2, 1, 1000)[..., :40], torch.tensor([2, 5], device="cuda")
+    assert torch.equal(ops.rotary(q, None, cos, sin, pos)[0], ops.rotary(q.contiguous(), None, cos, sin, pos)[0])
+    m = store.as_strided((2, 20, 50), (far, 50, 1))
+    assert torch.equal(ops.orthogonalize(m), ops.orthogonalize(m.contiguous()))
+    rows = store.as_strided((2, 1000), (far - 8, 1))
+    rows.copy_(near)
+    w = torch.ones(1000, device="cuda")
+    h, y, st = ops.block_norm(rows, near, w, w)
+    h2, y2, st2 = ops.block_norm(near, near, w, w)
+    assert torch.equal(h, h2) and torch.equal(y, y2)
+    dg, dg2 = (ops.block_norm_grad(near, near, v, near, w, w, s) for v, s in ((rows, st), (near, st2)))
+    assert all(u is None or torch.equal(u, v) for u, v in zip(dg, dg2))
+
+
+def test_many_short_rows(ops):
+    """More rows than a grid's second axis holds."""
+    gen = seeded(78)
+    logits = rand(gen, (70001, 9), "float32", 2.0)
+    tok = torch.randint(-1, 9, (70001,), generator=gen).cuda()
+    check_logprobs(ops, logits, tok, 1.0, 2, "float32", torch.ones(70001, device="cuda"), torch.ones(70001, device="cuda"))
+    d = block_operands(ops, 70002, 8, "float32", "float32", "rms", "many")
+    check_block(ops, d, "float32", "float32", "rms", False, 1.0)
+    cos, sin = (torch.from_numpy(v).cuda() for v in ops.rotary_table(4, 4))
+    q = rand(gen, (70001, 1, 1, 4), "float16")
+    pos = torch.randint(0, 4, (70001, 1), generator=gen)
+    y, _ = ops.rotary(q, None, cos, sin, pos.cuda())
+    want, mag = rotary64(q.cpu(), cos.cpu(), sin.cpu(), pos, 2, "half", False)
+    within(y.cpu(), want, mag, 3, "float16")

@@ -34,6 +34,7 @@ __global__ void __launch_bounds__(32 * FINISH_ROWS) norm_finish_kernel(const __g
   float s = 0.0f;
   if (c < a.width) {
     const long long e = min(n, (threadIdx.y + 1) * share);
+#pragma unroll 8
     for (long long b = threadIdx.y * share; b < e; ++b) s += a.part[((b0 + b) * SUMS + sum) * a.width + c];
   }
   buf[threadIdx.y][threadIdx.x] = s;

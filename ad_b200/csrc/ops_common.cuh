@@ -7,6 +7,7 @@
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
 
+#include <atomic>
 #include <cstdarg>
 #include <cstdint>
 #include <cstdio>
@@ -63,7 +64,7 @@ class DeviceGuard {
 
 // Multiprocessors of a device, asked for once; 0 with an error set on failure.
 inline int sm_count(int device) {
-  static int known[64] = {};
+  static std::atomic<int> known[64];
   if (device >= 0 && device < 64 && known[device]) return known[device];
   int n = 0;
   if (cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, device) != cudaSuccess) return 0;

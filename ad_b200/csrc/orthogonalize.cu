@@ -37,8 +37,8 @@
 // bus as 2 + 2 bytes in each direction.
 //
 // Measured, five steps: 12 x 4096 x 1024 1257 us (666 TFLOP/s of the halves that
-// symmetry leaves), 4096 x 4096 1450 us (945), 512 x 512 121 us, where every
-// product is a wait of 7.6 us.  A block's operands come from L2 at 60 to 80 GB/s,
+// symmetry leaves), 4096 x 4096 1450 us (945), 512 x 512 119 us, where every
+// product is a wait of 7.4 us.  A block's operands come from L2 at 60 to 80 GB/s,
 // which bounds the large cases.
 #include <cuda.h>
 
@@ -635,7 +635,7 @@ __global__ void __launch_bounds__(THREADS, 1)
     }
   } else {
     if (lane == 0) {  // their results
-      int e = 0;
+      int e = 0, under_way = -1;  // chunks used so far; the buffer of a store not yet waited for
       bool stop = false;
       for (int t = first; t < items && !stop; t += stride) {
         const Item it = item_of<TILE>(a, t);
@@ -668,15 +668,22 @@ __global__ void __launch_bounds__(THREADS, 1)
             for (int h = 0; h < 2; ++h)
               if (mirror && row + 64 * h < a.m) box_store(turned, s1 + h * (CHUNK / 2), row + 64 * h, col, it.mat);
             asm volatile("cp.async.bulk.commit_group;" ::: "memory");
-            asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
+            if (under_way >= 0) {  // the one before has been read
+              asm volatile("cp.async.bulk.wait_group.read 1;" ::: "memory");
+              bar_arrive(&side_empty[under_way]);
+            }
+            under_way = b;
+          } else {
+            bar_arrive(&side_empty[b]);
           }
-          bar_arrive(&side_empty[b]);
         }
         if (!stop && !last) {
           // written, and there for other blocks' copies
           asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
           asm volatile("fence.proxy.async.global;" ::: "memory");
           asm volatile("red.release.gpu.global.add.u32 [%0], 1;" ::"l"(a.ready + it.mat) : "memory");
+          bar_arrive(&side_empty[under_way]);
+          under_way = -1;
         }
       }
       asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
@@ -968,8 +975,8 @@ cudaError_t start(const Maps& maps, NsArgs& a, const Tiling& t, int sms, int dev
   at[1].id = cudaLaunchAttributeCooperative;  // blocks wait for one another: all of them have to be resident
   at[1].val.cooperative = 1;
   c.attrs = at;
-  static int resident[64] = {};  // blocks or pairs of them at a time, asked for once
-  int most_workers = device < 64 ? resident[device] : 0;
+  static std::atomic<int> resident[64];  // blocks or pairs of them at a time, asked for once
+  int most_workers = device < 64 ? resident[device].load() : 0;
   if (!most_workers) {
     cudaError_t e = cudaFuncSetAttribute(ns_kernel<CTAS, BN>, cudaFuncAttributeMaxDynamicSharedMemorySize, TILE::SMEM);
     if (e != cudaSuccess) return e;

@@ -937,7 +937,8 @@ Scales scales_for(int steps, const float* coef) {
 }
 
 // The list's tiles for one tile size, and a step's time in us as estimated from
-// measured costs of a tile's 64 elements of K and of a product's start and end:
+// measured costs of a tile's 64 elements of K and of a product's start and end
+// (4.6 us, and 1.4 for each 64 columns of the last tile's epilogue):
 // each product in as many rounds as its tiles make for the blocks.  What a block
 // can bring from L2 (70 to 80 GB/s) bounds the first, so that a large tile costs
 // hardly more than a small one: small ones are for matrices that leave most
@@ -957,7 +958,7 @@ Tiling tiling(long long count, long long m, long long n, int workers, double per
   t.up = t.row_tiles * ((n + TILE::N - 1) / TILE::N);
   const double kn = static_cast<double>((n + BK - 1) / BK), km = static_cast<double>((m + BK - 1) / BK);
   auto rounds = [&](long long tiles) { return static_cast<double>((count * tiles + workers - 1) / workers); };
-  t.us = per_kblock * (rounds(t.sym) * (kn + km) + rounds(t.up) * km) + 3 * 6.0;
+  t.us = per_kblock * (rounds(t.sym) * (kn + km) + rounds(t.up) * km) + 3 * (4.6 + 1.4 * TILE::N / 64);
   return t;
 }
 

@@ -48,21 +48,28 @@ __device__ __forceinline__ float exp2_approx(float x) {
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
-// Logits beyond this (masks of a type's lowest value, where nothing larger is
-// left) are compared before they are multiplied: their product overflows.
-constexpr float HUGE_LOGIT = 1e30f;
+// An offset m k beyond this (a mask of -1e10 or of a type's lowest value, where
+// nothing larger is left) is not used: its rounding, of 2^-24 its size, would be a
+// factor on the sum that grows out of range.  Differences from m are taken before
+// they are multiplied instead, an instruction more for each value.
+constexpr float MOST_OFFSET = 1048576.0f;
 
 // Running softmax statistics: largest value m, sum and sum weighted with the
 // exponent to base 2, both relative to the offset o = m k (rounded; all that
-// follows goes by the rounded one).  -FLT_MAX rather than -inf at the start:
-// -inf values then lie infinitely below it and count for nothing.
+// follows goes by the rounded one), or to m k itself where the offset is huge.
+// -FLT_MAX rather than -inf at the start: -inf values then lie infinitely below
+// it and count for nothing.
 struct Soft {
-  float m = -FLT_MAX, o = 0.0f, s = 0.0f, w = 0.0f;
-  __device__ __forceinline__ static bool huge(float m) { return fabsf(m) > HUGE_LOGIT; }
+  float m = -FLT_MAX, o, s = 0.0f, w = 0.0f;
+  __device__ __forceinline__ explicit Soft(float k) : o(offset(m, k)) {}
+  __device__ __forceinline__ static bool huge(float o) { return !(fabsf(o) <= MOST_OFFSET); }
+  __device__ __forceinline__ bool huge() const { return huge(o); }
   // rounded for good: contracted into a later difference it would not be the offset
   __device__ __forceinline__ static float offset(float m, float k) { return __fmul_rn(m, k); }
+  // The distance of what sums are relative to, from (m, o) to (to, to_o).
   __device__ __forceinline__ static float below(float m, float o, float to, float to_o, float k) {
-    return fmaxf(huge(m) || huge(to) ? (m - to) * k : o - to_o, GONE);
+    const float d = huge(o) ? (huge(to_o) ? (m - to) * k : fmaf(m, k, -to_o)) : huge(to_o) ? -fmaf(to, k, -o) : o - to_o;
+    return fmaxf(d, GONE);
   }
   __device__ __forceinline__ void raise(float to, float k) {
     const float to_o = offset(to, k), d = below(m, o, to, to_o, k), f = exp2_approx(d);
@@ -85,7 +92,7 @@ struct Soft {
   __device__ __forceinline__ void join(float om, float os, float ow, float k) {
     const float to = fmaxf(m, om);
     raise(to, k);
-    Soft other;
+    Soft other(k);
     other.m = om, other.o = offset(om, k), other.s = os, other.w = ow;
     other.raise(to, k);
     s += other.s;
@@ -101,7 +108,7 @@ struct Soft {
   }
   // Natural logarithm of a value's share, given that of the sum.
   __device__ __forceinline__ float log_share(float x, float k, float scale, float ln_s) const {
-    return (huge(m) ? (x - m) * scale : LN2 * fmaf(x, k, -o)) - ln_s;
+    return (huge() ? (x - m) * scale : LN2 * fmaf(x, k, -o)) - ln_s;
   }
 };
 
@@ -257,7 +264,7 @@ __global__ void __launch_bounds__(512) logprob_kernel(const __grid_constant__ Lo
   const int vecs = (a.vocab - head) / V, tail0 = head + vecs * V;
   const int share = (vecs + parts - 1) / parts;
   const int v0 = min(vecs, part * share), v1 = min(vecs, v0 + share);
-  Soft soft;
+  Soft soft(k);
   Best best;
   u64* queue = sh.queue[warp];
 
@@ -293,7 +300,7 @@ __global__ void __launch_bounds__(512) logprob_kernel(const __grid_constant__ Lo
   auto work = [&](const Set& r, int base, bool start) {
     const float big = largest<T, U>(r);
     if (big > soft.m) soft.raise(big, k);
-    if (Soft::huge(soft.m)) {
+    if (soft.huge()) {
 #pragma unroll
       for (int q = 0; q < U; ++q) {
         float e[V];
@@ -367,7 +374,7 @@ __global__ void __launch_bounds__(512) logprob_kernel(const __grid_constant__ Lo
     const float xi = has ? to_float(x[i]) : -INFINITY;
     if (has) {
       if (xi > soft.m) soft.raise(xi, k);
-      if (Soft::huge(soft.m))
+      if (soft.huge())
         soft.add<true>(xi, k);
       else
         soft.add<false>(xi, k);
@@ -388,7 +395,7 @@ __global__ void __launch_bounds__(512) logprob_kernel(const __grid_constant__ Lo
       __syncthreads();
     }
   if (warp == 0) {
-    soft = Soft();
+    soft = Soft(k);
     if (lane < warps) soft.m = sh.m[lane], soft.o = Soft::offset(soft.m, k), soft.s = sh.s[lane], soft.w = sh.w[lane];
     soft.join_lanes(k);
     if (TOP) best.list = sh.list[0][lane];
@@ -411,7 +418,7 @@ __global__ void __launch_bounds__(512) logprob_kernel(const __grid_constant__ Lo
         }
       }
       if (warp == 0) {
-        soft = Soft();
+        soft = Soft(k);
         if (lane < parts) {
           const Shared* other = cluster.map_shared_rank(&sh, lane);
           soft.m = other->bm, soft.o = Soft::offset(soft.m, k), soft.s = other->bs, soft.w = other->bw;
@@ -437,7 +444,7 @@ __global__ void __launch_bounds__(512) logprob_kernel(const __grid_constant__ Lo
       a.logp[row] = lp;
       a.entropy[row] = h;
       reinterpret_cast<float4*>(a.stats)[row] =
-          make_float4(soft.m, soft.s, h, empty ? -INFINITY : (Soft::huge(soft.m) ? soft.m * a.scale : LN2 * soft.o) + ln_s);
+          make_float4(soft.m, soft.s, h, empty ? -INFINITY : (soft.huge() ? soft.m * a.scale : LN2 * soft.o) + ln_s);
     }
     if (TOP && lane < a.top) {
       const float v = value_of(static_cast<unsigned>(best.list >> 32));
@@ -489,8 +496,8 @@ __global__ void __launch_bounds__(GRAD_THREADS) logprob_grad_kernel(const __grid
   // with l = k (x - m): -k p (g + e (l - ln s + H)) = q exp(l) (g' + e l)
   const float k = a.scale * LOG2E, el = e * LN2;
   const float c = empty ? 0.0f : -a.scale / st.y, b = empty ? 0.0f : g + e * (st.z - logf(st.y));
-  const bool huge = Soft::huge(st.x);
   const float o = Soft::offset(st.x, k);
+  const bool huge = Soft::huge(o);
   auto grad = [&](float d) { return c * exp2_approx(d) * fmaf(el, fmaxf(d, GONE), b); };
 #pragma unroll
   for (int q = 0; q < GRAD_VECS; ++q) {

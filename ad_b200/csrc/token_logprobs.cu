@@ -106,9 +106,15 @@ struct Soft {
       join(om, os, ow, k);
     }
   }
-  // Natural logarithm of a value's share, given that of the sum.
+  // Natural logarithm of a value's share, given that of the sum.  A value far
+  // below the maximum (masked with the type's lowest value) may leave the range of
+  // 32 bits when it is multiplied by k, where its distance times the factor does
+  // not; and the distance may, where the products with the factor do not.
   __device__ __forceinline__ float log_share(float x, float k, float scale, float ln_s) const {
-    return (huge() ? (x - m) * scale : LN2 * fmaf(x, k, -o)) - ln_s;
+    const float d = fmaf(x, k, -o);
+    if (!huge() && !isinf(d)) return LN2 * d - ln_s;
+    const float far = x - m;
+    return (isinf(far) ? fmaf(x, scale, -(m * scale)) : far * scale) - ln_s;
   }
 };
 

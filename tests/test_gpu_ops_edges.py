@@ -44,3 +44,29 @@ def test_token_logprobs_of_large_logits(ops, t, scale, base, vocab):
     r, _ = check_logprobs(ops, logits, tokens.cuda(), scale, 7, t, g, e)
     lse = logprobs64(logits, tokens, scale, 0)["lse"]
     within(r.stats[:, 3].cpu(), lse, lse.abs() + 4 + math.log(vocab), N_SOFT, "float32")
+
+
+@pytest.mark.parametrize("t", ["float32", "bfloat16", "float16"])
+@pytest.mark.parametrize("scale", [0.6, 1.0, 1.25])
+@pytest.mark.parametrize("vocab", [40, 3000])
+def test_token_logprobs_of_lowest_values(ops, t, scale, vocab):
+    """Tokens masked with the type's lowest value that are asked for, and alternatives that reach such
+    values: finite where 32 bits hold them."""
+    gen = seeded(vocab, len(t), 10 * scale)
+    low = torch.finfo(dtype(t)).min
+    logits = rand(gen, (6, vocab), t, 2.0)
+    logits[:, 4:] = low                  # four values left
+    logits[1, :4] += 1000                # a larger maximum
+    logits[2, 5] = -math.inf
+    if t != "float16":
+        logits[3, 0] = 1e30              # far above everything
+        logits[4, 0] = -low              # the largest there is
+    tokens = torch.tensor([vocab - 1, 17, 5, 9, 20, 0])
+    r = ops.token_logprobs(logits, tokens.cuda(), top=10, scale=scale)
+    w = logprobs64(logits, tokens, scale, 10)
+    for got, want in ((r.logp, w["logp"]), (r.top_logp, w["top"])):
+        want = want.float().double()     # past the range of 32 bits: infinite
+        within(got.cpu(), want, want.abs().nan_to_num(posinf=0.0) + 4 + math.log(vocab), N_SOFT, "float32")
+    assert torch.equal(r.top_index[[0, 1, 3, 4, 5]].cpu(), w["index"][[0, 1, 3, 4, 5]])
+    if t == "float16" or scale <= 1.0:
+        assert torch.isfinite(r.logp[[0, 1]]).all()

@@ -494,7 +494,7 @@ __global__ void __launch_bounds__(GRAD_THREADS) logprob_grad_kernel(const __grid
   }
   const float4 st = reinterpret_cast<const float4*>(a.stats)[row];
   const long long t = a.tok64 ? static_cast<const long long*>(a.tokens)[row] : static_cast<const int*>(a.tokens)[row];
-  const bool empty = st.w == -INFINITY;
+  const bool empty = st.y == 0.0f;  // the log of the sum may be past 32 bits for another reason
   float g = t >= 0 && a.g_logp ? a.g_logp[row] : 0.0f;
   const float e = a.g_entropy ? a.g_entropy[row] : 0.0f;
   if (t >= a.vocab) g *= __int_as_float(0x7fffffff);

@@ -70,3 +70,18 @@ def test_token_logprobs_of_lowest_values(ops, t, scale, vocab):
     assert torch.equal(r.top_index[[0, 1, 3, 4, 5]].cpu(), w["index"][[0, 1, 3, 4, 5]])
     if t == "float16" or scale <= 1.0:
         assert torch.isfinite(r.logp[[0, 1]]).all()
+
+
+@pytest.mark.parametrize("t", ["float32", "bfloat16"])
+@pytest.mark.parametrize("scale", [1.0, 1.25])
+def test_token_logprobs_grad_of_rows_at_the_lowest_value(ops, t, scale):
+    """A row whose values are all the type's lowest has a gradient like any row of equal values, also
+    where the log of its sum lies past the range of 32 bits; one of -inf has none."""
+    vocab = 70
+    logits = torch.full((3, vocab), torch.finfo(dtype(t)).min, device="cuda", dtype=dtype(t))
+    logits[1] = 0.5
+    logits[2] = -math.inf
+    tokens = torch.tensor([3, 3, 3], device="cuda")
+    g, e = torch.full((3,), -0.5, device="cuda"), torch.full((3,), 0.25, device="cuda")
+    _, d = check_logprobs(ops, logits, tokens, scale, 2, t, g, e)
+    assert d[:2].all() and not d[2].any()

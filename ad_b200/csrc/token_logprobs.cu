@@ -60,6 +60,9 @@ constexpr float MOST_OFFSET = 1048576.0f;
 // -FLT_MAX rather than -inf at the start: -inf values then lie infinitely below
 // it and count for nothing.
 struct Soft {
+  // The factor to base 2.  It stays a number for the largest factors: infinite, it
+  // would make a NaN of a value's distance of 0 from itself.
+  __device__ __forceinline__ static float factor(float scale) { return fminf(scale * LOG2E, FLT_MAX); }
   float m = -FLT_MAX, o, s = 0.0f, w = 0.0f;
   __device__ __forceinline__ explicit Soft(float k) : o(offset(m, k)) {}
   __device__ __forceinline__ static bool huge(float o) { return !(fabsf(o) <= MOST_OFFSET); }
@@ -259,7 +262,7 @@ __global__ void __launch_bounds__(512) logprob_kernel(const __grid_constant__ Lo
   const long long row = blockIdx.x / parts_u;
   const T* x = static_cast<const T*>(a.logits) + row * a.ld;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
-  const float k = a.scale * LOG2E;
+  const float k = Soft::factor(a.scale);
   if (TOP) {
     if (threadIdx.x == 0) sh.bar = 0;
     __syncthreads();
@@ -500,7 +503,7 @@ __global__ void __launch_bounds__(GRAD_THREADS) logprob_grad_kernel(const __grid
   if (t >= a.vocab) g *= __int_as_float(0x7fffffff);
   const float hot = empty ? 0.0f : g * a.scale;
   // with l = k (x - m): -k p (g + e (l - ln s + H)) = q exp(l) (g' + e l)
-  const float k = a.scale * LOG2E, el = e * LN2;
+  const float k = Soft::factor(a.scale), el = e * LN2;
   const float c = empty ? 0.0f : -a.scale / st.y, b = empty ? 0.0f : g + e * (st.z - logf(st.y));
   const float o = Soft::offset(st.x, k);
   const bool huge = Soft::huge(o);

@@ -85,3 +85,19 @@ def test_token_logprobs_grad_of_rows_at_the_lowest_value(ops, t, scale):
     g, e = torch.full((3,), -0.5, device="cuda"), torch.full((3,), 0.25, device="cuda")
     _, d = check_logprobs(ops, logits, tokens, scale, 2, t, g, e)
     assert d[:2].all() and not d[2].any()
+
+
+def test_token_logprobs_largest_scale(ops):
+    """Factors up to the largest number of 32 bits: equal values share, a larger one takes all."""
+    logits = torch.zeros(4, 100, device="cuda")
+    logits[1, 7] = 1.0
+    logits[2] = -3.0
+    logits[3] = 1e-30
+    logits[3, 9] = 2e-30
+    for scale in (1e30, 2.3e38, 2.4e38, 3.4e38):
+        r = ops.token_logprobs(logits, torch.tensor([7, 7, 0, 9], device="cuda"), top=1, scale=scale)
+        want = torch.tensor([-math.log(100), 0.0, -math.log(100), 0.0], dtype=torch.float64)
+        if scale < 1e31:  # the fourth row's values lie 1 apart
+            want[3] = 1.0 - math.log(math.e + 99)
+        within(r.logp.cpu(), want, torch.full((4,), 5.0, dtype=torch.float64), N_SOFT, "float32")
+        assert r.top_index[:, 0].tolist() == [0, 7, 0, 9]

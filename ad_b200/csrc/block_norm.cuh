@@ -558,25 +558,23 @@ __global__ void __launch_bounds__(MAXT, MAXT != 256 || V * NV > 8 ? 1 : slim<T, 
 
 // `ahead`: bytes of the rows to come; `blocks` 0: as many as are resident at a
 // time, each with every so-many-th row.
-template <typename K>
-cudaError_t run_norm(K kernel, NormArgs a, int vectors, int v, int ahead, unsigned blocks, int sms, int threads,
-                     cudaStream_t s) {
+template <auto KERNEL>
+cudaError_t run_norm(NormArgs a, int vectors, int v, int ahead, unsigned blocks, int sms, int threads, cudaStream_t s) {
   a.staged = (vectors * 4 * ((a.width + v - 1) / v * v) + 15) / 16 * 16;
   if (a.staged > 64 * 1024) a.staged = 0;
   const int bytes = a.staged + ahead;
-  if (bytes + 1024 > 48 * 1024) {  // beside what the kernel declares
-    const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
-    if (e != cudaSuccess) return e;
-  }
+  int room = 0;
+  cudaError_t e = shared_room<KERNEL>(&room);
+  if (e != cudaSuccess) return e;
   if (!blocks && a.rows <= sms) {
     blocks = static_cast<unsigned>(a.rows);
   } else if (!blocks) {
     int per = 1;
-    const cudaError_t e = cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per, kernel, threads, bytes);
+    e = cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per, KERNEL, threads, bytes);
     if (e != cudaSuccess) return e;
     blocks = static_cast<unsigned>(std::min(a.rows, 1ll * std::max(per, 1) * sms));
   }
-  kernel<<<blocks, threads, bytes, s>>>(a);
+  KERNEL<<<blocks, threads, bytes, s>>>(a);
   return cudaGetLastError();
 }
 
@@ -587,13 +585,13 @@ cudaError_t start_norm(const NormArgs& a, bool grad, bool gen, unsigned blocks, 
   const int g = gen ? Ahead<T, V, NV, 5, grad_rows<T, V, NV, MAXT, true>()>::bytes(threads)
                     : Ahead<T, V, NV, 5, grad_rows<T, V, NV, MAXT, false>()>::bytes(threads);
   if (!grad)
-    return gen ? run_norm(norm_kernel<T, V, NV, MAXT, true>, a, 4, V, f, 0, sms, threads, s)
-               : run_norm(norm_kernel<T, V, NV, MAXT, false>, a, 2, V, f, 0, sms, threads, s);
+    return gen ? run_norm<norm_kernel<T, V, NV, MAXT, true>>(a, 4, V, f, 0, sms, threads, s)
+               : run_norm<norm_kernel<T, V, NV, MAXT, false>>(a, 2, V, f, 0, sms, threads, s);
   if (gen)
-    return shared ? run_norm(norm_grad_kernel<T, V, NV, MAXT, true, true>, a, 3, V, g, blocks, sms, threads, s)
-                  : run_norm(norm_grad_kernel<T, V, NV, MAXT, true, false>, a, 3, V, g, blocks, sms, threads, s);
-  return shared ? run_norm(norm_grad_kernel<T, V, NV, MAXT, false, true>, a, 2, V, g, blocks, sms, threads, s)
-                : run_norm(norm_grad_kernel<T, V, NV, MAXT, false, false>, a, 2, V, g, blocks, sms, threads, s);
+    return shared ? run_norm<norm_grad_kernel<T, V, NV, MAXT, true, true>>(a, 3, V, g, blocks, sms, threads, s)
+                  : run_norm<norm_grad_kernel<T, V, NV, MAXT, true, false>>(a, 3, V, g, blocks, sms, threads, s);
+  return shared ? run_norm<norm_grad_kernel<T, V, NV, MAXT, false, true>>(a, 2, V, g, blocks, sms, threads, s)
+                : run_norm<norm_grad_kernel<T, V, NV, MAXT, false, false>>(a, 2, V, g, blocks, sms, threads, s);
 }
 
 // Eight elements of a row to a thread while 512 threads are enough for it (768

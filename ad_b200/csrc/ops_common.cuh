@@ -72,6 +72,26 @@ inline int sm_count(int device) {
   return n;
 }
 
+// Dynamic shared memory that a block of KERNEL can have on the current device.  It
+// is allowed to the kernel once and for good: set to what each launch asks for, the
+// limit could be lowered by another thread's launch before this one's.
+template <auto KERNEL>
+cudaError_t shared_room(int* room) {
+  static std::atomic<int> known[64];
+  int device = 0, most = 0;
+  cudaError_t e = cudaGetDevice(&device);
+  if (e != cudaSuccess) return e;
+  if (device < 64 && (*room = known[device])) return cudaSuccess;
+  cudaFuncAttributes f;
+  e = cudaFuncGetAttributes(&f, KERNEL);
+  if (e == cudaSuccess) e = cudaDeviceGetAttribute(&most, cudaDevAttrMaxSharedMemoryPerBlockOptin, device);
+  if (e != cudaSuccess) return e;
+  *room = most - static_cast<int>(f.sharedSizeBytes);
+  e = cudaFuncSetAttribute(KERNEL, cudaFuncAttributeMaxDynamicSharedMemorySize, *room);
+  if (e == cudaSuccess && device < 64) known[device] = *room;
+  return e;
+}
+
 inline int elem_size(int dtype) { return dtype == AD_F32 ? 4 : 2; }
 inline bool aligned(const void* p, size_t n) { return (reinterpret_cast<uintptr_t>(p) & (n - 1)) == 0; }
 

@@ -1,10 +1,11 @@
 """Operators of language models at the edges of what they take (B200 only).  The 64-bit
 implementations and the bounds' derivation are those of test_gpu_ops."""
 import math
+import threading
 
 import pytest
 
-from .test_gpu_ops import N_SOFT, check_logprobs, dtype, logprobs64, rand, seeded, within
+from .test_gpu_ops import N_SOFT, block_operands, check_logprobs, dtype, logprobs64, rand, seeded, within
 
 pytestmark = pytest.mark.gpu
 
@@ -101,3 +102,38 @@ def test_token_logprobs_largest_scale(ops):
             want[3] = 1.0 - math.log(math.e + 99)
         within(r.logp.cpu(), want, torch.full((4,), 5.0, dtype=torch.float64), N_SOFT, "float32")
         assert r.top_index[:, 0].tolist() == [0, 7, 0, 9]
+
+
+def test_block_norm_threads_of_different_widths(ops):
+    """Widths that share a kernel but not its amount of shared memory, launched from threads side by side
+    (the library's calls leave Python's lock to the others)."""
+    from ad_b200 import runtime as rt
+    L, failed = rt.lib(), []
+
+    def loop(width, calls):
+        try:
+            stream = torch.cuda.Stream()
+            d = block_operands(ops, 2, width, "bfloat16", "bfloat16", "rms", "none")
+            h, y, st = ops.block_norm(d["x"], d["z"], d["wa"], d["wb"])
+            want = ops.block_norm_grad(d["dh"], d["dy"], d["x"], d["z"], d["wa"], d["wb"], st)
+            g = [torch.empty_like(v) for v in want if v is not None]
+            ws = torch.empty(ops.block_norm_grad_workspace(2, width), dtype=torch.uint8, device="cuda")
+            torch.cuda.synchronize()
+            p = {k: None if v is None else v.data_ptr() for k, v in d.items()}
+            args = (0, ops.BF16, ops.BF16, 0, p["dh"], width, p["dy"], width, p["x"], width, p["z"], width, None, 0, 0, 0,
+                    p["wa"], None, p["wb"], None, 1.0, st.data_ptr(), 2, width, g[0].data_ptr(), width, g[1].data_ptr(),
+                    width, None, 0, g[2].data_ptr(), None, g[3].data_ptr(), None, ws.data_ptr(), ws.numel(),
+                    stream.cuda_stream)
+            for _ in range(calls):
+                rt.check(L.ad_block_norm_grad(*args))
+            stream.synchronize()
+            assert all(torch.equal(u, v) for u, v in zip(g, [v for v in want if v is not None]))
+        except BaseException as e:  # noqa: BLE001  (handed to the test's own thread)
+            failed.append(e)
+
+    threads = [threading.Thread(target=loop, args=(w, 20000)) for w in (4096, 2304, 3200, 2560)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not failed, failed

@@ -561,11 +561,12 @@ __global__ void __launch_bounds__(MAXT, MAXT != 256 || V * NV > 8 ? 1 : slim<T, 
 template <auto KERNEL>
 cudaError_t run_norm(NormArgs a, int vectors, int v, int ahead, unsigned blocks, int sms, int threads, cudaStream_t s) {
   a.staged = (vectors * 4 * ((a.width + v - 1) / v * v) + 15) / 16 * 16;
-  if (a.staged > 64 * 1024) a.staged = 0;
-  const int bytes = a.staged + ahead;
   int room = 0;
   cudaError_t e = shared_room<KERNEL>(&room);
   if (e != cudaSuccess) return e;
+  // rows to come go before weights, which are read again for each row where both do not fit
+  if (a.staged > 64 * 1024 || a.staged + ahead > room) a.staged = 0;
+  const int bytes = a.staged + ahead;
   if (!blocks && a.rows <= sms) {
     blocks = static_cast<unsigned>(a.rows);
   } else if (!blocks) {

@@ -5,7 +5,7 @@ import threading
 
 import pytest
 
-from .test_gpu_ops import N_SOFT, block_operands, check_logprobs, dtype, logprobs64, rand, seeded, within
+from .test_gpu_ops import N_SOFT, block_operands, check_block, check_logprobs, dtype, logprobs64, rand, seeded, within
 
 pytestmark = pytest.mark.gpu
 
@@ -137,3 +137,19 @@ def test_block_norm_threads_of_different_widths(ops):
     for t in threads:
         t.join()
     assert not failed, failed
+
+
+@pytest.mark.parametrize("t,wt", [("float32", "float32"), ("bfloat16", "float32"), ("float16", "float16")])
+@pytest.mark.parametrize("kind", ["rms", "layer"])
+@pytest.mark.parametrize("width,gate", [(6145, "none"), (6400, "three"), (7168, "none"), (7172, "row"), (7680, "three"),
+                                        (8192, "none"), (8192, "row"), (8193, "three")])
+def test_block_norm_wide_rows(ops, t, wt, kind, width, gate):
+    """Widths whose weights and rows to come would not all fit a multiprocessor's shared memory, and
+    those whose gradients give 16 or 32 elements to a thread."""
+    d = block_operands(ops, 6, width, t, wt, kind, gate)
+    check_block(ops, d, t, wt, kind, gate == "row", 1.0)
+
+
+def test_block_norm_wide_rows_of_many_blocks(ops):
+    d = block_operands(ops, 700, 8192, "float32", "float32", "rms", "many")
+    check_block(ops, d, "float32", "float32", "rms", True, 0.5)

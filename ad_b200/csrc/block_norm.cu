@@ -123,11 +123,11 @@ extern "C" int ad_block_norm(int device, int dtype, int wtype, int kind, const v
                    fits(h, ldh, size) && fits(y, ldy, size) && fits(wa, 0, 1) && fits(ba, 0, 1) && fits(wb, 0, 1) &&
                    fits(bb, 0, 1);
   DeviceGuard g(device);
-  if (g.error() != cudaSuccess) return fail("ad_block_norm: %s", cudaGetErrorString(g.error()));
+  if (g.error() != cudaSuccess) return fail_cuda("ad_block_norm", g.error());
   const int sms = sm_count(g.device());
   if (!sms) return fail("ad_block_norm: no device properties");
   const cudaError_t e = start_any(a, dtype, false, kind || ba || bb, vec, 0, sms, static_cast<cudaStream_t>(stream));
-  if (e != cudaSuccess) return fail("ad_block_norm: %s", cudaGetErrorString(e));
+  if (e != cudaSuccess) return fail_cuda("ad_block_norm", e);
   return 0;
 }
 
@@ -157,7 +157,7 @@ extern "C" int ad_block_norm_grad(int device, int dtype, int wtype, int kind, co
   if ((wa && !dwa) || (wb && !dwb) || (ba && !dba) || (bb && !dbb))
     return fail("ad_block_norm_grad: a weight without room for its gradient");
   DeviceGuard g(device);
-  if (g.error() != cudaSuccess) return fail("ad_block_norm_grad: %s", cudaGetErrorString(g.error()));
+  if (g.error() != cudaSuccess) return fail_cuda("ad_block_norm_grad", g.error());
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   const int wsize = elem_size(wtype);
   if (rows == 0) {  // sums of nothing
@@ -166,7 +166,7 @@ extern "C" int ad_block_norm_grad(int device, int dtype, int wtype, int kind, co
     for (int k = 0; k < 4; ++k)
       if (of[k]) {
         const cudaError_t e = cudaMemsetAsync(sums[k], 0, static_cast<size_t>(width) * wsize, s);
-        if (e != cudaSuccess) return fail("ad_block_norm_grad: %s", cudaGetErrorString(e));
+        if (e != cudaSuccess) return fail_cuda("ad_block_norm_grad", e);
       }
     return 0;
   }
@@ -197,7 +197,7 @@ extern "C" int ad_block_norm_grad(int device, int dtype, int wtype, int kind, co
                    fits(dh, lddh, size) && fits(dy, lddy, size) && fits(dx, lddx, size) && fits(dz, lddz, size) &&
                    fits(dgate, lddg, size) && fits(wa, 0, 1) && fits(ba, 0, 1) && fits(wb, 0, 1) && fits(bb, 0, 1);
   cudaError_t e = start_any(a, dtype, true, kind || ba || bb, vec, static_cast<unsigned>(split.blocks), sms, s);
-  if (e != cudaSuccess) return fail("ad_block_norm_grad: %s", cudaGetErrorString(e));
+  if (e != cudaSuccess) return fail_cuda("ad_block_norm_grad", e);
   FinishArgs f = {};
   f.part = a.part;
   f.blocks = split.blocks, f.blocks_per_run = split.blocks_per_run;
@@ -211,9 +211,8 @@ extern "C" int ad_block_norm_grad(int device, int dtype, int wtype, int kind, co
   f.ldg = lddg;
   const long long gates = shared ? rows / rows_per_gate : 0;  // fewer than blocks
   if (f.out[SUM_WA] || f.out[SUM_WB] || shared) {
-    norm_finish_kernel<<<dim3((width + 31) / 32, static_cast<unsigned>(4 + gates)), dim3(32, FINISH_ROWS), 0, s>>>(f);
-    e = cudaGetLastError();
-    if (e != cudaSuccess) return fail("ad_block_norm_grad: %s", cudaGetErrorString(e));
+    e = launch<norm_finish_kernel>(dim3((width + 31) / 32, static_cast<unsigned>(4 + gates)), dim3(32, FINISH_ROWS), 0, s, f);
+    if (e != cudaSuccess) return fail_cuda("ad_block_norm_grad", e);
   }
   return 0;
 }

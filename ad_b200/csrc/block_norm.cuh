@@ -575,8 +575,7 @@ cudaError_t run_norm(NormArgs a, int vectors, int v, int ahead, unsigned blocks,
     if (e != cudaSuccess) return e;
     blocks = static_cast<unsigned>(std::min(a.rows, 1ll * std::max(per, 1) * sms));
   }
-  KERNEL<<<blocks, threads, bytes, s>>>(a);
-  return cudaGetLastError();
+  return launch<KERNEL>(blocks, threads, bytes, s, a);
 }
 
 template <typename T, int V, int NV, int MAXT>

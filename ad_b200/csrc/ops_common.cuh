@@ -38,6 +38,24 @@ inline int fail(const char* fmt, ...) {
   return 1;
 }
 
+// The same for an error of the CUDA runtime, which remembers it for the thread's
+// next call that asks: it is forgotten here, having been reported.
+inline int fail_cuda(const char* who, cudaError_t e) {
+  cudaGetLastError();
+  return fail("%s: %s", who, cudaGetErrorString(e));
+}
+
+// A launch's own status: the last error may be an earlier call's.
+template <auto KERNEL, typename A>
+cudaError_t launch(dim3 grid, dim3 block, int bytes, cudaStream_t s, const A& a) {
+  cudaLaunchConfig_t c = {};
+  c.gridDim = grid;
+  c.blockDim = block;
+  c.dynamicSmemBytes = bytes;
+  c.stream = s;
+  return cudaLaunchKernelEx(&c, KERNEL, a);
+}
+
 // Makes `device` current for one call (-1: the current one) and puts the
 // caller's device back at its end.
 class DeviceGuard {
@@ -67,7 +85,10 @@ inline int sm_count(int device) {
   static std::atomic<int> known[64];
   if (device >= 0 && device < 64 && known[device]) return known[device];
   int n = 0;
-  if (cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, device) != cudaSuccess) return 0;
+  if (cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, device) != cudaSuccess) {
+    cudaGetLastError();  // reported by the caller
+    return 0;
+  }
   if (device >= 0 && device < 64) known[device] = n;
   return n;
 }

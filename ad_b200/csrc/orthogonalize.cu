@@ -850,9 +850,9 @@ __global__ void __launch_bounds__(256) ns_load(const __grid_constant__ LoadArgs 
 
 template <typename T, int V>
 cudaError_t load(const LoadArgs& a, int count, cudaStream_t st) {
-  ns_norm<T, V><<<dim3(NORM_BLOCKS, count), 256, 0, st>>>(a);
-  ns_load<T, V><<<dim3((a.inner + 63) / 64, (a.outer + 63) / 64, count), 256, 0, st>>>(a);
-  return cudaGetLastError();
+  const cudaError_t e = launch<ns_norm<T, V>>(dim3(NORM_BLOCKS, count), 256, 0, st, a);
+  if (e != cudaSuccess) return e;
+  return launch<ns_load<T, V>>(dim3((a.inner + 63) / 64, (a.outer + 63) / 64, count), 256, 0, st, a);
 }
 
 // No steps: the normalised matrix itself.
@@ -1030,7 +1030,7 @@ extern "C" int ad_orthogonalize(int device, int dtype, const void* g, int64_t co
   const Scales sc = scales_for(steps, coefficients);
   if (!sc.ok) return fail("ad_orthogonalize: these coefficients let singular values grow past 1024");
   DeviceGuard guard(device);
-  if (guard.error() != cudaSuccess) return fail("ad_orthogonalize: %s", cudaGetErrorString(guard.error()));
+  if (guard.error() != cudaSuccess) return fail_cuda("ad_orthogonalize", guard.error());
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   unsigned char* w = static_cast<unsigned char*>(workspace);
   const bool tall = rows > cols;
@@ -1054,7 +1054,7 @@ extern "C" int ad_orthogonalize(int device, int dtype, const void* g, int64_t co
   cudaError_t e = dtype == AD_F32    ? (vec ? load<float, 4>(la, num, st) : load<float, 1>(la, num, st))
                   : dtype == AD_BF16 ? (vec ? load<__nv_bfloat16, 4>(la, num, st) : load<__nv_bfloat16, 1>(la, num, st))
                                      : (vec ? load<__half, 4>(la, num, st) : load<__half, 1>(la, num, st));
-  if (e != cudaSuccess) return fail("ad_orthogonalize: %s", cudaGetErrorString(e));
+  if (e != cudaSuccess) return fail_cuda("ad_orthogonalize", e);
 
   NsArgs s = {};
   s.count = num, s.m = m, s.n = n, s.steps = steps;
@@ -1071,9 +1071,8 @@ extern "C" int ad_orthogonalize(int device, int dtype, const void* g, int64_t co
   const int per16 = 16 / elem_size(out_dtype);
   s.out_vec = s.out_col == 1 && s.out_row % per16 == 0 && s.out_batch % per16 == 0 && aligned(out, 16);
   if (steps == 0) {
-    ns_copy<<<dim3(256, num), 256, 0, st>>>(s);
-    e = cudaGetLastError();
-    if (e != cudaSuccess) return fail("ad_orthogonalize: %s", cudaGetErrorString(e));
+    e = launch<ns_copy>(dim3(256, num), 256, 0, st, s);
+    if (e != cudaSuccess) return fail_cuda("ad_orthogonalize", e);
     return 0;
   }
   for (int k = 0; k < steps; ++k) {
@@ -1112,6 +1111,6 @@ extern "C" int ad_orthogonalize(int device, int dtype, const void* g, int64_t co
   e = &best == &big   ? start<2, 256>(maps, s, best, sms, guard.device(), st)
       : &best == &mid ? start<1, 128>(maps, s, best, sms, guard.device(), st)
                       : start<1, 64>(maps, s, best, sms, guard.device(), st);
-  if (e != cudaSuccess) return fail("ad_orthogonalize: %s", cudaGetErrorString(e));
+  if (e != cudaSuccess) return fail_cuda("ad_orthogonalize", e);
   return 0;
 }

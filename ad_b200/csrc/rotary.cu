@@ -206,24 +206,23 @@ bool whole(const RotaryArgs& a, int v, int size) {
 }
 
 template <typename T, int V, Units U>
-cudaError_t launch(RotaryArgs a, cudaStream_t s) {
+cudaError_t start(RotaryArgs a, cudaStream_t s) {
   const int units = U == HALVES ? a.half / V + ((a.dim - 2 * a.half) / V + 1) / 2 : a.dim / V;
   const int heads = a.heads[0] + a.heads[1];
   a.head_groups = static_cast<unsigned>((heads + heads_at_once<U>() - 1) / heads_at_once<U>());
   const long long groups = a.rows * a.head_groups;
   if (groups > 0x7fffffffll) return cudaErrorInvalidValue;
   const int by = 256 / units;
-  rotary_kernel<T, V, U><<<static_cast<unsigned>((groups + by - 1) / by), dim3(units, by),
-                          U == ACROSS ? by * heads_at_once<U>() * a.dim * sizeof(T) : 0, s>>>(a);
-  return cudaGetLastError();
+  const int bytes = U == ACROSS ? by * heads_at_once<U>() * a.dim * static_cast<int>(sizeof(T)) : 0;
+  return launch<rotary_kernel<T, V, U>>(static_cast<unsigned>((groups + by - 1) / by), dim3(units, by), bytes, s, a);
 }
 
 template <typename T, int V>
 bool try_vectors(const RotaryArgs& a, int layout, cudaStream_t s, cudaError_t& e) {
   if (a.dim / V > 256 || !whole(a, V, sizeof(T))) return false;
-  e = layout == 1          ? launch<T, V, PAIRS>(a, s)
-      : a.half % V == 0    ? launch<T, V, HALVES>(a, s)
-                           : launch<T, V, ACROSS>(a, s);
+  e = layout == 1          ? start<T, V, PAIRS>(a, s)
+      : a.half % V == 0    ? start<T, V, HALVES>(a, s)
+                           : start<T, V, ACROSS>(a, s);
   return true;
 }
 
@@ -235,11 +234,9 @@ cudaError_t dispatch(const RotaryArgs& a, int layout, cudaStream_t s) {
   if (try_vectors<T, M>(a, layout, s, e) || try_vectors<T, M / 2>(a, layout, s, e)) return e;
   const int units = a.dim - a.half, bx = std::min(units, 256);
   const int by = std::max(1, std::min(256 / bx, a.heads[0] + a.heads[1]));
-  if (layout == 0)
-    rotary_single_kernel<T, true><<<static_cast<unsigned>(a.rows), dim3(bx, by), 0, s>>>(a);
-  else
-    rotary_single_kernel<T, false><<<static_cast<unsigned>(a.rows), dim3(bx, by), 0, s>>>(a);
-  return cudaGetLastError();
+  const unsigned blocks = static_cast<unsigned>(a.rows);
+  return layout == 0 ? launch<rotary_single_kernel<T, true>>(blocks, dim3(bx, by), 0, s, a)
+                     : launch<rotary_single_kernel<T, false>>(blocks, dim3(bx, by), 0, s, a);
 }
 
 }  // namespace
@@ -290,11 +287,11 @@ extern "C" int ad_rotary(int device, int dtype, const void* q, const int64_t* q_
   a.table_vec = a.half % 4 == 0 && aligned(cos, 16) && aligned(sin, 16);
   a.sign = inverse ? -1.0f : 1.0f;
   DeviceGuard g(device);
-  if (g.error() != cudaSuccess) return fail("ad_rotary: %s", cudaGetErrorString(g.error()));
+  if (g.error() != cudaSuccess) return fail_cuda("ad_rotary", g.error());
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   const cudaError_t e = dtype == AD_F32    ? dispatch<float>(a, layout, s)
                         : dtype == AD_BF16 ? dispatch<__nv_bfloat16>(a, layout, s)
                                            : dispatch<__half>(a, layout, s);
-  if (e != cudaSuccess) return fail("ad_rotary: %s", cudaGetErrorString(e));
+  if (e != cudaSuccess) return fail_cuda("ad_rotary", e);
   return 0;
 }

@@ -588,11 +588,8 @@ cudaError_t backward(LogprobGradArgs a, cudaStream_t s) {
   a.segments = static_cast<int>((a.vocab + per - 1) / per);
   const long long blocks = a.rows * a.segments;
   if (blocks > 0x7fffffffll) return cudaErrorInvalidValue;
-  if (same)
-    logprob_grad_kernel<T, V><<<static_cast<unsigned>(blocks), GRAD_THREADS, 0, s>>>(a);
-  else
-    logprob_grad_kernel<T, 1><<<static_cast<unsigned>(blocks), GRAD_THREADS, 0, s>>>(a);
-  return cudaGetLastError();
+  return same ? launch<logprob_grad_kernel<T, V>>(static_cast<unsigned>(blocks), GRAD_THREADS, 0, s, a)
+              : launch<logprob_grad_kernel<T, 1>>(static_cast<unsigned>(blocks), GRAD_THREADS, 0, s, a);
 }
 
 int check(const char* who, int dtype, const void* logits, int64_t ld, int64_t rows, int64_t vocab, const void* tokens,
@@ -619,7 +616,7 @@ extern "C" int ad_token_logprobs(int device, int dtype, const void* logits, int6
   if (!logp || !entropy || !stats || !aligned(stats, 16) || (top && (!top_logp || !top_index)))
     return fail("ad_token_logprobs: null or unaligned result");
   DeviceGuard g(device);
-  if (g.error() != cudaSuccess) return fail("ad_token_logprobs: %s", cudaGetErrorString(g.error()));
+  if (g.error() != cudaSuccess) return fail_cuda("ad_token_logprobs", g.error());
   const int sms = sm_count(g.device());
   if (!sms) return fail("ad_token_logprobs: no device properties");
   LogprobArgs a = {};
@@ -631,7 +628,7 @@ extern "C" int ad_token_logprobs(int device, int dtype, const void* logits, int6
   const cudaError_t e = dtype == AD_F32    ? forward<float>(a, sms, s)
                         : dtype == AD_BF16 ? forward<__nv_bfloat16>(a, sms, s)
                                            : forward<__half>(a, sms, s);
-  if (e != cudaSuccess) return fail("ad_token_logprobs: %s", cudaGetErrorString(e));
+  if (e != cudaSuccess) return fail_cuda("ad_token_logprobs", e);
   return 0;
 }
 
@@ -645,7 +642,7 @@ extern "C" int ad_token_logprobs_grad(int device, int dtype, const void* logits,
     return fail("ad_token_logprobs_grad: null or unaligned operand");
   if (rows > 1 && ld_grad < vocab) return fail("ad_token_logprobs_grad: rows of the gradient overlap");
   DeviceGuard g(device);
-  if (g.error() != cudaSuccess) return fail("ad_token_logprobs_grad: %s", cudaGetErrorString(g.error()));
+  if (g.error() != cudaSuccess) return fail_cuda("ad_token_logprobs_grad", g.error());
   LogprobGradArgs a = {};
   a.logits = logits, a.out = grad, a.ld = ld, a.ldo = ld_grad, a.rows = rows, a.vocab = static_cast<int>(vocab);
   a.tokens = tokens, a.tok64 = tok64, a.scale = scale;
@@ -654,6 +651,6 @@ extern "C" int ad_token_logprobs_grad(int device, int dtype, const void* logits,
   const cudaError_t e = dtype == AD_F32    ? backward<float>(a, s)
                         : dtype == AD_BF16 ? backward<__nv_bfloat16>(a, s)
                                            : backward<__half>(a, s);
-  if (e != cudaSuccess) return fail("ad_token_logprobs_grad: %s", cudaGetErrorString(e));
+  if (e != cudaSuccess) return fail_cuda("ad_token_logprobs_grad", e);
   return 0;
 }

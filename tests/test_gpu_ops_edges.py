@@ -153,3 +153,29 @@ def test_block_norm_wide_rows(ops, t, wt, kind, width, gate):
 def test_block_norm_wide_rows_of_many_blocks(ops):
     d = block_operands(ops, 700, 8192, "float32", "float32", "rms", "many")
     check_block(ops, d, "float32", "float32", "rms", True, 0.5)
+
+
+def test_a_refused_call_leaves_nothing_to_the_next(ops):
+    """The error of one call is not reported by the next one, which works."""
+    import ctypes
+    from ad_b200 import runtime as rt
+    x, w = torch.randn(5, 64, device="cuda"), torch.ones(64, device="cuda")
+    q = torch.randn(1, 5, 2, 32, device="cuda")
+    cos, sin = (torch.from_numpy(v).cuda() for v in ops.rotary_table(8, 32))
+    pos = torch.arange(5, device="cuda")
+    tok = torch.arange(5, device="cuda")
+    stats = ops.block_norm(x, x, w, w)[2]
+    calls = [lambda: ops.rotary(q, None, cos, sin, pos), lambda: ops.rotary(q, None, cos, sin, pos, layout="interleaved"),
+             lambda: ops.rotary(q[..., 1:31], None, cos[:, :15].contiguous(), sin[:, :15].contiguous(), pos),
+             lambda: ops.block_norm(x, x, w, w), lambda: ops.block_norm_grad(x, x, x, x, w, w, stats),
+             lambda: ops.token_logprobs(x, tok),
+             lambda: ops.token_logprobs_grad(x, tok, ops.token_logprobs(x, tok).stats),
+             lambda: ops.orthogonalize(x), lambda: ops.orthogonalize(x, steps=0)]
+    L = rt.lib()
+    st = (ctypes.c_int64 * 3)(64, 64, 32)
+    for call in calls:
+        refused = L.ad_rotary(99, 0, q.data_ptr(), st, q.data_ptr(), st, 2, None, None, None, None, 0, 1, 5, 32, 32, 0, 0,
+                              cos.data_ptr(), sin.data_ptr(), 8, pos.data_ptr(), 1, 0, 1, None)
+        assert refused and b"ad_rotary" in L.ad_last_error()
+        call()
+    torch.cuda.synchronize()

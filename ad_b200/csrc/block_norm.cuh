@@ -64,12 +64,24 @@ __device__ __forceinline__ unsigned long long at(long long row, long long ld) {
   return static_cast<unsigned long long>(static_cast<unsigned>(row)) * static_cast<unsigned>(ld);
 }
 
-// exp and quotient to about 2 units in the last place of 32 bits
-template <int E>
-__device__ __forceinline__ void activate(float (&g)[E], int sigmoid) {
-  if (!sigmoid) return;
-#pragma unroll
-  for (int i = 0; i < E; ++i) g[i] = __fdividef(1.0f, 1.0f + __expf(-g[i]));
+// 32-bit elements: to 2 units in the last place.  16-bit ones: to 2 + 1.2 |x|, at
+// most 107 where the result is neither 0 nor infinite, which is 2^-17 of it and
+// far below their own rounding.
+template <typename T>
+__device__ __forceinline__ float exponential(float x) {
+  return sizeof(T) == 4 ? expf(x) : __expf(x);
+}
+template <typename T>
+__device__ __forceinline__ float sigmoid(float g) {
+  return __fdividef(1.0f, 1.0f + exponential<T>(-g));
+}
+// With its slope: shares 1 / (1 + e) and e / (1 + e), without a difference that
+// could cancel; the sigmoid is one of them by g's sign, its slope their product.
+template <typename T>
+__device__ __forceinline__ float sigmoid(float g, float& slope) {
+  const float e = exponential<T>(-fabsf(g)), large = __fdividef(1.0f, 1.0f + e), small = e * large;
+  slope = large * small;
+  return g >= 0.0f ? large : small;
 }
 
 // Sums over the block of N values a thread; every thread gets them.  `buf`
@@ -373,7 +385,10 @@ __global__ void __launch_bounds__(MAXT, MAXT == 256 ? (V * NV <= 8 ? 4 : 2) : 1)
       }
     }
     if (a.gate) {
-      activate<E>(act, a.sigmoid);
+      if (a.sigmoid) {
+#pragma unroll
+        for (int i = 0; i < E; ++i) act[i] = sigmoid<T>(act[i]);
+      }
 #pragma unroll
       for (int i = 0; i < E; ++i) u[i] *= act[i];
     }
@@ -458,7 +473,6 @@ __global__ void __launch_bounds__(MAXT, MAXT != 256 || V * NV > 8 ? 1 : slim<T, 
     }
     if (a.gate) {
       ahead.read(stage, 1, pg(row), act);
-      activate<E>(act, a.sigmoid);
     } else {
 #pragma unroll
       for (int i = 0; i < E; ++i) act[i] = 1.0f;
@@ -481,12 +495,24 @@ __global__ void __launch_bounds__(MAXT, MAXT != 256 || V * NV > 8 ? 1 : slim<T, 
         for (int i = 0; i < E; ++i) u[i] += w[i];
       }
     }
+    // h in nh; from here on u is the gate's part of its own gradient
+    if (a.sigmoid && a.gate) {
+#pragma unroll
+      for (int i = 0; i < E; ++i) {
+        float slope;
+        act[i] = sigmoid<T>(act[i], slope);
+        nh[i] = a.wb ? fmaf(a.scale, nh[i], act[i] * u[i]) : 0.0f;
+        u[i] *= slope;
+      }
+    } else if (a.wb) {
+#pragma unroll
+      for (int i = 0; i < E; ++i) nh[i] = fmaf(a.scale, nh[i], act[i] * u[i]);
+    }
     if (a.wb) {
       float q[2] = {0.0f, 0.0f};
       weights.get(W_WB, w);
 #pragma unroll
       for (int i = 0; i < E; ++i) {
-        nh[i] = fmaf(a.scale, nh[i], act[i] * u[i]);
         nh[i] = (GEN ? nh[i] - mh : nh[i]) * rh;
         swb[i] = fmaf(d[i], nh[i], swb[i]);
         if (GEN) sbb[i] += d[i];
@@ -508,10 +534,6 @@ __global__ void __launch_bounds__(MAXT, MAXT != 256 || V * NV > 8 ? 1 : slim<T, 
     if (a.gate) {
 #pragma unroll
       for (int i = 0; i < E; ++i) o[i] = t[i] * u[i];
-      if (a.sigmoid) {
-#pragma unroll
-        for (int i = 0; i < E; ++i) o[i] *= act[i] * (1.0f - act[i]);
-      }
       if (SHARED) {
 #pragma unroll
         for (int i = 0; i < E; ++i) sg[i] += o[i];

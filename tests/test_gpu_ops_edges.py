@@ -179,3 +179,35 @@ def test_a_refused_call_leaves_nothing_to_the_next(ops):
         assert refused and b"ad_rotary" in L.ad_last_error()
         call()
     torch.cuda.synchronize()
+
+
+# Of a sigmoid's share: exp to 2 ulp (4 E), 1 + exp (4 E carried on and a rounding), the quotient to 2 ulp,
+# a product: 14 E.  Its slope is the product of two shares, times two factors: 32 E.  16-bit elements
+# take an exp of 2 + 1.2 |x| ulp, 50 at most here: 100 E more a share, far below their own rounding.
+@pytest.mark.parametrize("t,n_act,n_slope", [("float32", 14, 32), ("bfloat16", 114, 232), ("float16", 114, 232)])
+@pytest.mark.parametrize("shape", [(12, 256), (12, 100), (6, 333)])
+def test_block_norm_saturated_gates(ops, t, n_act, n_slope, shape):
+    """h = sigmoid(gate) z alone, and the gate's gradient, relative to their own size."""
+    rows, width = shape
+    gen = seeded(rows, width, len(t))
+    signs = torch.tensor([12.0, -12.0, 20.0, -20.0, 5.0, -40.0])
+    gate = (signs.repeat(rows * width)[:rows * width].reshape(rows, width) + torch.rand(rows, width, generator=gen)).to(dtype(t)).cuda()
+    z, dh = rand(gen, shape, t, 1.0, 3.0), rand(gen, shape, t, 1.0, 3.0)
+    opts = dict(gate=gate, gate_sigmoid=True, residual_scale=0.0)
+    x = torch.zeros_like(z)
+    h, _, st = ops.block_norm(x, z, None, None, **opts)
+    g = ops.block_norm_grad(dh, None, x, z, None, None, st, **opts)
+    big = gate.double()
+    act, rest = torch.sigmoid(big), torch.sigmoid(-big)
+    within(h, act * z.double(), act * z.double().abs(), n_act, t)
+    within(g.z, act * dh.double(), act * dh.double().abs(), n_act, t)
+    slope = act * rest * z.double() * dh.double()
+    within(g.gate, slope, slope.abs(), n_slope, t)
+    shared = ops.block_norm_grad(dh, None, x, z, None, None, st, gate=gate[:1], gate_sigmoid=True, residual_scale=0.0)
+    slope = (act * rest)[:1] * z.double() * dh.double()
+    within(shared.gate, slope.sum(0, keepdim=True), slope.abs().sum(0, keepdim=True), n_slope + rows, t)
+    gate[0] = math.inf
+    gate[1] = -math.inf
+    h, _, st = ops.block_norm(x, z, None, None, **opts)
+    g = ops.block_norm_grad(dh, None, x, z, None, None, st, **opts)
+    assert torch.equal(h[0], z[0]) and not h[1].any() and not g.gate[:2].any() and torch.equal(g.z[0], dh[0])

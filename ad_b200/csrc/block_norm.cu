@@ -144,6 +144,18 @@ extern "C" int ad_block_norm_grad_workspace(int device, int64_t rows, int width,
   return 0;
 }
 
+extern "C" int ad_clear_rows(int device, void* p, int64_t row_stride, int64_t row_bytes, int64_t rows, void* stream) {
+  if (row_bytes < 0 || rows < 0 || (rows > 1 && row_stride < row_bytes))
+    return fail("ad_clear_rows: %lld rows of %lld bytes, %lld apart", (long long)rows, (long long)row_bytes, (long long)row_stride);
+  if (rows == 0 || row_bytes == 0) return 0;
+  if (!p) return fail("ad_clear_rows: null operand");
+  DeviceGuard g(device);
+  if (g.error() != cudaSuccess) return fail_cuda("ad_clear_rows", g.error());
+  const cudaError_t e = cudaMemset2DAsync(p, std::max(row_stride, row_bytes), 0, row_bytes, rows, static_cast<cudaStream_t>(stream));
+  if (e != cudaSuccess) return fail_cuda("ad_clear_rows", e);
+  return 0;
+}
+
 extern "C" int ad_block_norm_grad(int device, int dtype, int wtype, int kind, const void* dh, int64_t lddh,
                                   const void* dy, int64_t lddy, const void* x, int64_t ldx, const void* z, int64_t ldz,
                                   const void* gate, int64_t ldg, int64_t rows_per_gate, int gate_sigmoid,

@@ -529,6 +529,9 @@ def block_norm_grad(dh, dy, x, z, after_weight, before_weight, stats, *, gate=No
         _ptr(before_bias), residual_scale, stats.data_ptr(), rows, width, g.x.data_ptr(), lddx, g.z.data_ptr(), lddz,
         _ptr(g.gate), lddg, _ptr(g.after_weight), _ptr(g.after_bias), _ptr(g.before_weight), _ptr(g.before_bias),
         workspace.data_ptr(), have, s))
+    if rows == 0 and gate is not None:  # a sum over no rows for each row of the gate
+        groups, _, lddg = _rows(g.gate, "out gate")
+        rt.check(_entry("ad_clear_rows")(dev, g.gate.data_ptr(), lddg * _SIZES[dt], width * _SIZES[dt], groups, s))
     return g
 
 

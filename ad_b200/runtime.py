@@ -88,6 +88,7 @@ SIGNATURES = {
                                    c_void_p, c_float, c_void_p, c_i64, c_int, c_void_p, c_i64, c_void_p, c_i64,
                                    c_void_p, c_i64, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_size_t,
                                    c_void_p]),
+    "ad_clear_rows": (c_int, [c_int, c_void_p, c_i64, c_i64, c_i64, c_void_p]),
     "ad_token_logprobs": (c_int, [c_int, c_int, c_void_p, c_i64, c_i64, c_i64, c_void_p, c_int, c_float, c_int,
                                   c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p]),
     "ad_token_logprobs_grad": (c_int, [c_int, c_int, c_void_p, c_i64, c_i64, c_i64, c_void_p, c_int, c_float,

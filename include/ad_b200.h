@@ -209,7 +209,9 @@ int ad_block_norm(int device, int dtype, int wtype, int kind, const void* x, int
 int ad_block_norm_grad_workspace(int device, int64_t rows, int width, int64_t rows_per_gate,
                                  size_t* bytes);
 /* The gradients of ad_block_norm's operands from those of h and y: dx, dz, the
- * gate's (of its shape) and, of type wtype, the weights' and biases'. */
+ * gate's (of its shape) and, of type wtype, the weights' and biases'.  With no
+ * rows those of the weights and biases are zeros; how many rows the gate has is
+ * not known then, and its gradient is left to ad_clear_rows. */
 int ad_block_norm_grad(int device, int dtype, int wtype, int kind, const void* dh, int64_t lddh,
                        const void* dy, int64_t lddy, const void* x, int64_t ldx, const void* z,
                        int64_t ldz, const void* gate, int64_t ldg, int64_t rows_per_gate,
@@ -218,6 +220,9 @@ int ad_block_norm_grad(int device, int dtype, int wtype, int kind, const void* d
                        void* dx, int64_t lddx, void* dz, int64_t lddz, void* dgate, int64_t lddg,
                        void* dwa, void* dba, void* dwb, void* dbb, void* workspace,
                        size_t workspace_bytes, void* stream);
+/* Zeros in `rows` rows of row_bytes bytes, row_stride bytes apart. */
+int ad_clear_rows(int device, void* p, int64_t row_stride, int64_t row_bytes, int64_t rows,
+                  void* stream);
 
 /* Of each row of scale * logits: the log probability of its token (0 for a
  * negative token, NaN for one past the vocabulary), the entropy of its

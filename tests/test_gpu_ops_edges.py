@@ -211,3 +211,33 @@ def test_block_norm_saturated_gates(ops, t, n_act, n_slope, shape):
     h, _, st = ops.block_norm(x, z, None, None, **opts)
     g = ops.block_norm_grad(dh, None, x, z, None, None, st, **opts)
     assert torch.equal(h[0], z[0]) and not h[1].any() and not g.gate[:2].any() and torch.equal(g.z[0], dh[0])
+
+
+@pytest.mark.parametrize("shape", [(16,), (1, 16), (3, 16)])
+@pytest.mark.parametrize("t", ["float32", "bfloat16"])
+def test_block_norm_grad_of_a_gate_without_rows(ops, shape, t):
+    """A gate shared by no rows has a gradient of zeros, whatever was in its memory."""
+    x = torch.ones((0, 16), device="cuda", dtype=dtype(t))
+    w, gate = torch.ones(16, device="cuda"), torch.ones(shape, device="cuda", dtype=dtype(t))
+    h, y, stats = ops.block_norm(x, x, w, w, gate=gate)
+    torch.full((1 << 16,), math.nan, device="cuda")  # what the allocator may hand out again
+    g = ops.block_norm_grad(x, x, x, x, w, w, stats, gate=gate)
+    assert g.gate.shape == shape and not g.gate.any()
+    wide = torch.full((shape[0] if len(shape) > 1 else 1, 40), math.nan, device="cuda", dtype=dtype(t))
+    room = wide[:, 5:21].reshape(shape) if len(shape) == 1 else wide[:, 5:21]
+    out = ops.BlockNormGrads(x, x, room, *(torch.full((16,), math.nan, device="cuda") for _ in range(2)), None, None)
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    ops.block_norm_grad(x, x, x, x, w, w, stats, gate=gate, out=out, workspace=torch.empty(0, device="cuda"), stream=s)
+    s.synchronize()
+    assert not room.any() and not out.after_weight.any() and not out.before_weight.any()
+    assert torch.isnan(wide[:, :5]).all() and torch.isnan(wide[:, 21:]).all()
+
+
+def test_clear_rows_refuses(ops):
+    from ad_b200 import runtime as rt
+    x = torch.ones(4, 8, device="cuda")
+    for args in ((16, 32, 4), (32, -1, 4), (32, 32, -1)):
+        with pytest.raises(rt.ADError, match="ad_clear_rows"):
+            rt.check(rt.lib().ad_clear_rows(0, x.data_ptr(), *args, None))
+    assert x.all()

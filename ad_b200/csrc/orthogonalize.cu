@@ -798,7 +798,7 @@ __global__ void __launch_bounds__(256) ns_norm(const __grid_constant__ LoadArgs 
 template <typename T, int V>
 __global__ void __launch_bounds__(256) ns_load(const __grid_constant__ LoadArgs a) {
   __shared__ float t[64][65];
-  __shared__ float factor;
+  __shared__ double factor;
   const long long mat = gridDim.z - 1 - blockIdx.z;
   const T* g = static_cast<const T*>(a.g) + mat * a.batch;
   const int i0 = blockIdx.x * 64, o0 = blockIdx.y * 64;  // along a run, of runs
@@ -820,7 +820,7 @@ __global__ void __launch_bounds__(256) ns_load(const __grid_constant__ LoadArgs 
     for (int k = threadIdx.x; k < NORM_BLOCKS; k += 32) s += a.part[mat * NORM_BLOCKS + k];
 #pragma unroll
     for (int o = 16; o; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
-    if (threadIdx.x == 0) factor = static_cast<float>(a.scale / (sqrt(s) + a.eps));
+    if (threadIdx.x == 0) factor = s == 0.0 ? 0.0 : a.scale / (sqrt(s) + a.eps);  // zeros stay zeros, whatever eps is
   }
 #pragma unroll
   for (int k = 0; k < N; ++k) {
@@ -829,7 +829,10 @@ __global__ void __launch_bounds__(256) ns_load(const __grid_constant__ LoadArgs 
     for (int j = 0; j < V; ++j) t[a.turned ? i + j : o][a.turned ? o : i + j] = x[k][j];
   }
   __syncthreads();
-  const float f = factor;
+  // Norms under 5e-35 have a factor past the range of 32 bits, though not its
+  // products: these are taken in 64 then.
+  const float f = static_cast<float>(factor);
+  const bool wide = factor > 1e37;
   const int r0 = a.turned ? i0 : o0, c0 = a.turned ? o0 : i0;
 #pragma unroll
   for (int k = 0; k < 2; ++k) {  // 8 adjacent elements of a row of X
@@ -838,7 +841,7 @@ __global__ void __launch_bounds__(256) ns_load(const __grid_constant__ LoadArgs 
     Vec<__half, 8> h, l;
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
-      const float y = t[r][c + j] * f;
+      const float y = wide ? static_cast<float>(t[r][c + j] * factor) : t[r][c + j] * f;
       h.v[j] = __float2half_rn(y);
       l.v[j] = __float2half_rn(y - __half2float(h.v[j]));
     }

@@ -5,7 +5,8 @@ import threading
 
 import pytest
 
-from .test_gpu_ops import N_SOFT, block_operands, check_block, check_logprobs, dtype, logprobs64, rand, seeded, within
+from .test_gpu_ops import (N_SOFT, block_operands, check_block, check_logprobs, check_orthogonal, dtype, logprobs64,
+                           orthogonal64, rand, seeded, update, within)
 
 pytestmark = pytest.mark.gpu
 
@@ -241,3 +242,25 @@ def test_clear_rows_refuses(ops):
         with pytest.raises(rt.ADError, match="ad_clear_rows"):
             rt.check(rt.lib().ad_clear_rows(0, x.data_ptr(), *args, None))
     assert x.all()
+
+
+@pytest.mark.parametrize("eps", [0.0, 1e-38, 1e-7])
+def test_orthogonalize_zero_matrices(ops, eps):
+    g = update(seeded(50), 3, 70, 100, "noise", "float32")
+    g[1] = 0
+    y = ops.orthogonalize(g, eps=eps)
+    assert not y[1].any() and torch.isfinite(y).all() and y[0].any() and y[2].any()
+    assert not ops.orthogonalize(g[1:2], eps=eps, steps=0).any()
+
+
+@pytest.mark.parametrize("norm", [1e-42, 1e-40, 1e-36, 3e-35, 1e-34, 1e-30, 1e30, 1e38])
+@pytest.mark.parametrize("rows,cols", [(60, 50), (33, 129)])
+def test_orthogonalize_any_scale(ops, norm, rows, cols):
+    """Scales at which the reciprocal of the norm does not fit 32 bits, or only as a subnormal number."""
+    gen = seeded(51, rows, cols)
+    g = torch.randn(2, rows, cols, generator=gen, dtype=torch.float64)
+    g[0] = torch.linalg.qr(g[0]).Q if rows >= cols else torch.linalg.qr(g[0].T).Q.T
+    g *= norm / g.square().sum((1, 2), keepdim=True).sqrt()
+    g[1, 0, 0] = norm      # one value that 32 bits hold however small the others are
+    g = g.float().cuda()
+    check_orthogonal(ops.orthogonalize(g, eps=0.0), orthogonal64(g, 5, [ops.NEWTON_SCHULZ] * 5, 0.0), 5, "bfloat16")

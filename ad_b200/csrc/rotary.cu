@@ -256,7 +256,8 @@ extern "C" int ad_rotary(int device, int dtype, const void* q, const int64_t* q_
   if (rows == 0 || q_heads + k_heads == 0 || dim == 0) return 0;
   if (rows > 0x7fffffffll) return fail("ad_rotary: %lld tokens in one call", rows);
   if ((q_heads && (!q || !q_out || !q_strides || !q_out_strides)) ||
-      (k_heads && (!k || !k_out || !k_strides || !k_out_strides)) || !positions || (rotary && (!cos || !sin)))
+      (k_heads && (!k || !k_out || !k_strides || !k_out_strides)) || !positions ||
+      (rotary && table_rows > 0 && (!cos || !sin)))  // an empty table has no address; every position lies outside it
     return fail("ad_rotary: null operand");
   RotaryArgs a;
   const void* in[2] = {q, k};

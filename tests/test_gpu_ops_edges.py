@@ -264,3 +264,13 @@ def test_orthogonalize_any_scale(ops, norm, rows, cols):
     g[1, 0, 0] = norm      # one value that 32 bits hold however small the others are
     g = g.float().cuda()
     check_orthogonal(ops.orthogonalize(g, eps=0.0), orthogonal64(g, 5, [ops.NEWTON_SCHULZ] * 5, 0.0), 5, "bfloat16")
+
+
+@pytest.mark.parametrize("layout", ["half", "interleaved"])
+@pytest.mark.parametrize("d,r", [(32, 16), (32, 32), (33, 18), (32, 12)])
+def test_rotary_empty_tables(ops, layout, d, r):
+    """With tables of no rows every position lies outside them."""
+    q = torch.ones(1, 3, 2, d, device="cuda")
+    none = torch.empty(0, r // 2, device="cuda")
+    y, _ = ops.rotary(q, None, none, none, torch.arange(3, device="cuda"), layout=layout)
+    assert torch.isnan(y[..., :r]).all() and torch.equal(y[..., r:], q[..., r:])

@@ -108,6 +108,8 @@ extern "C" int ad_block_norm(int device, int dtype, int wtype, int kind, const v
   if (rows == 0) return 0;
   if (!h || (wb && !y) || !stats || !aligned(stats, 16)) return fail("ad_block_norm: null or unaligned result");
   if ((ba && !wa) || (bb && !wb)) return fail("ad_block_norm: a bias without its weight");
+  if (!aligned({x, z, gate, h, y}, elem_size(dtype)) || !aligned({wa, ba, wb, bb}, elem_size(wtype)))
+    return fail("ad_block_norm: an operand is not aligned to its elements");
   NormArgs a = {};
   a.x = x, a.z = z, a.gate = gate;
   a.ldx = ldx, a.ldz = ldz, a.ldg = ldg;
@@ -166,6 +168,9 @@ extern "C" int ad_block_norm_grad(int device, int dtype, int wtype, int kind, co
   if (check("ad_block_norm_grad", dtype, wtype, kind, x, z, gate, rows_per_gate, rows, width, 0.0f,
             {lddh, lddy, ldx, ldz, ldg, lddx, lddz, lddg})) return 1;
   if ((ba && !wa) || (bb && !wb)) return fail("ad_block_norm_grad: a bias without its weight");
+  if (!aligned({dh, dy, x, z, gate, dx, dz, dgate}, elem_size(dtype)) ||
+      !aligned({wa, ba, wb, bb, dwa, dba, dwb, dbb}, elem_size(wtype)))
+    return fail("ad_block_norm_grad: an operand is not aligned to its elements");
   if ((wa && !dwa) || (wb && !dwb) || (ba && !dba) || (bb && !dbb))
     return fail("ad_block_norm_grad: a weight without room for its gradient");
   DeviceGuard g(device);

@@ -12,6 +12,7 @@
 #include <cstdint>
 #include <cstdio>
 #include <cstring>
+#include <initializer_list>
 #include <type_traits>
 
 #include "../../include/ad_b200.h"
@@ -115,6 +116,12 @@ cudaError_t shared_room(int* room) {
 
 inline int elem_size(int dtype) { return dtype == AD_F32 ? 4 : 2; }
 inline bool aligned(const void* p, size_t n) { return (reinterpret_cast<uintptr_t>(p) & (n - 1)) == 0; }
+// A load or store of an element elsewhere would be a fault of the device.
+inline bool aligned(std::initializer_list<const void*> all, size_t n) {
+  for (const void* p : all)
+    if (!aligned(p, n)) return false;
+  return true;
+}
 
 // ---------------------------------------------------------------- elements
 __device__ __forceinline__ float to_float(float x) { return x; }

@@ -1026,6 +1026,8 @@ extern "C" int ad_orthogonalize(int device, int dtype, const void* g, int64_t co
   const Layout l = plan(count, rows, cols);
   if (count * l.n > 0x7fffffffll) return fail("ad_orthogonalize: too many rows in one call");
   if (!g || !out) return fail("ad_orthogonalize: null operand");
+  if (!aligned(g, elem_size(dtype)) || !aligned(out, elem_size(out_dtype)))
+    return fail("ad_orthogonalize: an operand is not aligned to its elements");
   if (!workspace || !aligned(workspace, 256) || workspace_bytes < l.total)
     return fail("ad_orthogonalize: needs %zu bytes of workspace, 256-byte aligned", l.total);
   for (int i = 0; i < 3 * steps; ++i)

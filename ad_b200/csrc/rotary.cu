@@ -259,6 +259,8 @@ extern "C" int ad_rotary(int device, int dtype, const void* q, const int64_t* q_
       (k_heads && (!k || !k_out || !k_strides || !k_out_strides)) || !positions ||
       (rotary && table_rows > 0 && (!cos || !sin)))  // an empty table has no address; every position lies outside it
     return fail("ad_rotary: null operand");
+  if (!aligned({q, q_out, k, k_out}, elem_size(dtype)) || !aligned({cos, sin}, 4) || !aligned(positions, pos64 ? 8 : 4))
+    return fail("ad_rotary: an operand is not aligned to its elements");
   RotaryArgs a;
   const void* in[2] = {q, k};
   void* out[2] = {q_out, k_out};

@@ -593,7 +593,7 @@ cudaError_t backward(LogprobGradArgs a, cudaStream_t s) {
 }
 
 int check(const char* who, int dtype, const void* logits, int64_t ld, int64_t rows, int64_t vocab, const void* tokens,
-          float scale) {
+          int tok64, float scale) {
   if (dtype < AD_F32 || dtype > AD_F16) return fail("%s: unknown element type %d", who, dtype);
   if (rows < 0 || vocab < 1 || vocab > 0x7fff0000ll) return fail("%s: %lld rows of %lld logits", who, (long long)rows, (long long)vocab);
   if (rows > 0x0fffffffll) return fail("%s: %lld rows in one call", who, (long long)rows);
@@ -601,6 +601,7 @@ int check(const char* who, int dtype, const void* logits, int64_t ld, int64_t ro
   if (rows && (!logits || !tokens)) return fail("%s: null operand", who);
   if (rows > 1 && ld < vocab) return fail("%s: rows overlap", who);
   if (!aligned(logits, elem_size(dtype))) return fail("%s: unaligned logits", who);
+  if (!aligned(tokens, tok64 ? 8 : 4)) return fail("%s: unaligned tokens", who);
   return 0;
 }
 
@@ -609,11 +610,12 @@ int check(const char* who, int dtype, const void* logits, int64_t ld, int64_t ro
 extern "C" int ad_token_logprobs(int device, int dtype, const void* logits, int64_t ld, int64_t rows, int64_t vocab,
                                  const void* tokens, int tok64, float scale, int top, float* logp, float* entropy,
                                  float* stats, float* top_logp, int64_t* top_index, void* stream) {
-  if (check("ad_token_logprobs", dtype, logits, ld, rows, vocab, tokens, scale)) return 1;
+  if (check("ad_token_logprobs", dtype, logits, ld, rows, vocab, tokens, tok64, scale)) return 1;
   if (top < 0 || top > MAX_TOP || top > vocab)
     return fail("ad_token_logprobs: %d alternatives (at most %d, and no more than logits)", top, MAX_TOP);
   if (rows == 0) return 0;
-  if (!logp || !entropy || !stats || !aligned(stats, 16) || (top && (!top_logp || !top_index)))
+  if (!logp || !entropy || !stats || !aligned(stats, 16) || !aligned({logp, entropy}, 4) ||
+      (top && (!top_logp || !top_index || !aligned(top_logp, 4) || !aligned(top_index, 8))))
     return fail("ad_token_logprobs: null or unaligned result");
   DeviceGuard g(device);
   if (g.error() != cudaSuccess) return fail_cuda("ad_token_logprobs", g.error());
@@ -636,9 +638,9 @@ extern "C" int ad_token_logprobs_grad(int device, int dtype, const void* logits,
                                       int64_t vocab, const void* tokens, int tok64, float scale, const float* stats,
                                       const float* g_logp, const float* g_entropy, void* grad, int64_t ld_grad,
                                       void* stream) {
-  if (check("ad_token_logprobs_grad", dtype, logits, ld, rows, vocab, tokens, scale)) return 1;
+  if (check("ad_token_logprobs_grad", dtype, logits, ld, rows, vocab, tokens, tok64, scale)) return 1;
   if (rows == 0) return 0;
-  if (!stats || !aligned(stats, 16) || !grad || !aligned(grad, elem_size(dtype)))
+  if (!stats || !aligned(stats, 16) || !grad || !aligned(grad, elem_size(dtype)) || !aligned({g_logp, g_entropy}, 4))
     return fail("ad_token_logprobs_grad: null or unaligned operand");
   if (rows > 1 && ld_grad < vocab) return fail("ad_token_logprobs_grad: rows of the gradient overlap");
   DeviceGuard g(device);

@@ -184,9 +184,11 @@ def _rows(x, name):
     if width > 1 and st[-1] != 1:
         raise ValueError(f"{name}: a row's elements have to be adjacent (stride {st[-1]})")
     if n == 2:
-        return shape[0], width, st[0]
+        return shape[0], width, st[0] if shape[0] > 1 else width
     if n == 1:
         return 1, width, width
+    if 0 in shape:  # no elements: strides say nothing
+        return math.prod(shape[:-1]), width, width
     rows, ld = 1, None
     for i in range(n - 2, -1, -1):
         if shape[i] != 1:

@@ -63,3 +63,20 @@ def test_device_arrays_refuse_unaligned_addresses():
             ops.rotary(**rotary_args(**kw))
     with pytest.raises(rt.ADError, match="aligned"):
         ops.orthogonalize(arr((4, 8), "bfloat16", ptr=P + 1), out=arr((4, 8), "bfloat16"), workspace=arr((1 << 20,)))
+
+
+def test_arrays_without_elements_and_single_rows():
+    """Strides that nothing follows are not looked at."""
+    for shape, strides, want in (((2, 0, 8), (8, 8, 1), (0, 8, 8)), ((0, 3, 8), (24, 8, 1), (0, 8, 8)),
+                                 ((3, 0, 2, 8), (16, 16, 8, 1), (0, 8, 8)), ((2, 0, 5, 8), (1, 7, 3, 1), (0, 8, 8)),
+                                 ((1, 8), (2 ** 40, 1), (1, 8, 8)), ((1, 1, 8), (3, 2 ** 40, 1), (1, 8, 8)),
+                                 ((2, 3, 0), (3, 1, 1), (6, 0, 0))):
+        assert ops._rows(arr(shape, strides=strides), "x") == want
+    x = arr((2, 0, 8), strides=(8, 8, 1))
+    h, y, _ = ops.block_norm(x, x, arr((8,)), arr((8,)), gate=x, out=(x, x, arr((0, 4))))
+    assert h is x and y is x
+    none = arr((2, 0), strides=(1, 1))
+    out = ops.TokenLogprobs(none, none, arr((0, 4)), None, None)
+    r = ops.token_logprobs(x, arr((2, 0), "int64", strides=(1, 1)), out=out)
+    assert r.logp is none
+    assert ops.token_logprobs_grad(x, arr((2, 0), "int64", strides=(1, 1)), arr((0, 4)), out=x) is x

@@ -286,6 +286,8 @@ def _rotary_operands(q, k, cos, sin, positions, layout):
     dt = _float(q, "q")
     dev = _device(q, "q")
     b, t, hq, d, sq = _heads(q, "q")
+    _typed(cos, F32, "cos")
+    _typed(sin, F32, "sin")
     half = cos.shape[1] if len(cos.shape) == 2 else -1
     if half < 0 or tuple(cos.shape) != tuple(sin.shape):
         raise ValueError(f"cos, sin: shapes {tuple(cos.shape)} and {tuple(sin.shape)}, expected [rows, rotary / 2] twice")
@@ -300,7 +302,6 @@ def _rotary_operands(q, k, cos, sin, positions, layout):
     else:
         raise ValueError(f"positions: shape {tuple(ps)}, expected {(b, t)} or {(t,)}")
     for x, name in ((cos, "cos"), (sin, "sin")):
-        _typed(x, F32, name)
         _flat(x, cos.shape[0] * half, name)
         _on(dev, x, name)
     _on(dev, positions, "positions")
@@ -373,8 +374,8 @@ def _check_norm_operands(x, z, after, before, gate, after_bias, before_bias, kin
     dt = _float(x, "x")
     dev = _device(x, "x")
     rows, width, ldx = _rows(x, "x")
-    _same_shape(z, x.shape, "z")
     _typed(z, dt, "z")
+    _same_shape(z, x.shape, "z")
     _on(dev, z, "z")
     ldz = _rows(z, "z")[2]
     wt = None
@@ -431,6 +432,7 @@ def block_norm(x, z, after_weight, before_weight, *, gate=None, after_bias=None,
         if (y is None) != (before_weight is None):
             raise ValueError("out: y goes with before_weight")
         ldh = ldy = 0
+        _typed(h, dt, "out h")
         for v, name in ((h, "out h"), (y, "out y")):
             if v is not None:
                 _typed(v, dt, name)
@@ -483,7 +485,7 @@ def block_norm_grad(dh, dy, x, z, after_weight, before_weight, stats, *, gate=No
         raise ValueError("dy goes with before_weight")
     lds = []
     for v, name in ((dh, "dh"), (dy, "dy")):
-        if v is None:
+        if v is None and name == "dy":
             lds.append(0)
             continue
         _typed(v, dt, name)
@@ -523,8 +525,8 @@ def block_norm_grad(dh, dy, x, z, after_weight, before_weight, stats, *, gate=No
         workspace = _empty((need,), x, "uint8")
         have = need
     else:
-        _on(dev, workspace, "workspace")
         have = _nbytes(workspace, "workspace")
+        _on(dev, workspace, "workspace")
     rt.check(_entry("ad_block_norm_grad")(
         dev, dt, wt, _KINDS[kind], dh.data_ptr(), lds[0], _ptr(dy), lds[1], x.data_ptr(), ldx, z.data_ptr(), ldz,
         _ptr(gate), ldg, per, gate_sigmoid, _ptr(after_weight), _ptr(after_bias), _ptr(before_weight),
@@ -539,6 +541,7 @@ def block_norm_grad(dh, dy, x, z, after_weight, before_weight, stats, *, gate=No
 
 def _nbytes(x, name):
     """Bytes of an array of adjacent elements of any type."""
+    _code(x, name)
     n = 1
     for s in x.shape:
         n *= s
@@ -705,8 +708,8 @@ def orthogonalize(g, *, steps: int = 5, coefficients=NEWTON_SCHULZ, eps: float =
         workspace = _empty((need,), g, "uint8")
         have = need
     else:
-        _on(dev, workspace, "workspace")
         have = _nbytes(workspace, "workspace")
+        _on(dev, workspace, "workspace")
     rt.check(_entry("ad_orthogonalize")(
         dev, dt, g.data_ptr(), count, rows, cols, sb, sr, sc, steps, (rt.c_float * max(1, len(coef)))(*coef), eps, ot,
         out.data_ptr(), so[0] if len(so) == 3 else 0, so[-2], so[-1], workspace.data_ptr(), have, s))

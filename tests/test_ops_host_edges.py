@@ -7,7 +7,7 @@ import pytest
 from ad_b200 import ops
 from ad_b200 import runtime as rt
 
-from .test_ops_host import arr, refused, rotary_args
+from .test_ops_host import arr, norm_args, refused, rotary_args
 
 P = 4096
 
@@ -80,3 +80,35 @@ def test_arrays_without_elements_and_single_rows():
     r = ops.token_logprobs(x, arr((2, 0), "int64", strides=(1, 1)), out=out)
     assert r.logp is none
     assert ops.token_logprobs_grad(x, arr((2, 0), "int64", strides=(1, 1)), arr((0, 4)), out=x) is x
+
+
+@pytest.mark.parametrize("what", [None, 3, "text", [1.0], object()])
+def test_operands_that_are_no_arrays(what):
+    """A TypeError that names the operand, wherever one has to be given."""
+    def no(name, call, **kw):
+        with pytest.raises(TypeError, match=name + ": expected a device array"):
+            call(**kw)
+
+    for name in ("q", "cos", "sin", "positions"):
+        no(name, ops.rotary, **rotary_args(**{name: what}))
+    for name in ("x", "z"):
+        no(name, ops.block_norm, **norm_args(**{name: what}))
+    no("out h", ops.block_norm, **norm_args(out=(what, arr((6, 8)), arr((6, 4)))))
+    no("out stats", ops.block_norm, **norm_args(out=(arr((6, 8)), arr((6, 8)), what)))
+    grads = (arr((6, 8)), arr((6, 8)), None, arr((8,)), arr((8,)), None, None)
+    args = dict(dh=arr((6, 8)), dy=arr((6, 8)), x=arr((6, 8)), z=arr((6, 8)), after_weight=arr((8,)),
+                before_weight=arr((8,)), stats=arr((6, 4)), workspace=arr((1 << 20,)), out=grads)
+    for name in ("dh", "x", "z", "stats"):
+        no(name, ops.block_norm_grad, **{**args, name: what})
+    for name in ("logits", "tokens"):
+        no(name, ops.token_logprobs, **{**dict(logits=arr((4, 10)), tokens=arr((4,), "int64")), name: what})
+    for name in ("logits", "tokens", "stats"):
+        no(name, ops.token_logprobs_grad,
+           **{**dict(logits=arr((4, 10)), tokens=arr((4,), "int64"), stats=arr((4, 4)), out=arr((4, 10))), name: what})
+    no("g", ops.orthogonalize, g=what)
+    if what is not None:
+        no("k", ops.rotary, **rotary_args(k=what))
+        no("gate", ops.block_norm, **norm_args(gate=what))
+        no("before_weight", ops.block_norm, **norm_args(before_weight=what))
+        no("dy", ops.block_norm_grad, **{**args, "dy": what})
+        no("workspace", ops.orthogonalize, g=arr((4, 8)), out=arr((4, 8)), workspace=what)

@@ -600,20 +600,23 @@ cudaError_t run_norm(NormArgs a, int vectors, int v, int ahead, unsigned blocks,
   return launch<KERNEL>(blocks, threads, bytes, s, a);
 }
 
-template <typename T, int V, int NV, int MAXT>
-cudaError_t start_norm(const NormArgs& a, bool grad, bool gen, unsigned blocks, int sms, int threads, cudaStream_t s) {
-  const bool shared = a.gate && a.rows_per_gate > 1;
-  const int f = Ahead<T, V, NV, 3, FORWARD_ROWS>::bytes(threads);
-  const int g = gen ? Ahead<T, V, NV, 5, grad_rows<T, V, NV, MAXT, true>()>::bytes(threads)
-                    : Ahead<T, V, NV, 5, grad_rows<T, V, NV, MAXT, false>()>::bytes(threads);
-  if (!grad)
+// GRAD: which of the two directions; each is built for the sizes below that take it.
+template <bool GRAD, typename T, int V, int NV, int MAXT>
+cudaError_t start_norm(const NormArgs& a, bool gen, unsigned blocks, int sms, int threads, cudaStream_t s) {
+  if constexpr (!GRAD) {
+    const int f = Ahead<T, V, NV, 3, FORWARD_ROWS>::bytes(threads);
     return gen ? run_norm<norm_kernel<T, V, NV, MAXT, true>>(a, 4, V, f, 0, sms, threads, s)
                : run_norm<norm_kernel<T, V, NV, MAXT, false>>(a, 2, V, f, 0, sms, threads, s);
-  if (gen)
-    return shared ? run_norm<norm_grad_kernel<T, V, NV, MAXT, true, true>>(a, 3, V, g, blocks, sms, threads, s)
-                  : run_norm<norm_grad_kernel<T, V, NV, MAXT, true, false>>(a, 3, V, g, blocks, sms, threads, s);
-  return shared ? run_norm<norm_grad_kernel<T, V, NV, MAXT, false, true>>(a, 2, V, g, blocks, sms, threads, s)
-                : run_norm<norm_grad_kernel<T, V, NV, MAXT, false, false>>(a, 2, V, g, blocks, sms, threads, s);
+  } else {
+    const bool shared = a.gate && a.rows_per_gate > 1;
+    const int g = gen ? Ahead<T, V, NV, 5, grad_rows<T, V, NV, MAXT, true>()>::bytes(threads)
+                      : Ahead<T, V, NV, 5, grad_rows<T, V, NV, MAXT, false>()>::bytes(threads);
+    if (gen)
+      return shared ? run_norm<norm_grad_kernel<T, V, NV, MAXT, true, true>>(a, 3, V, g, blocks, sms, threads, s)
+                    : run_norm<norm_grad_kernel<T, V, NV, MAXT, true, false>>(a, 3, V, g, blocks, sms, threads, s);
+    return shared ? run_norm<norm_grad_kernel<T, V, NV, MAXT, false, true>>(a, 2, V, g, blocks, sms, threads, s)
+                  : run_norm<norm_grad_kernel<T, V, NV, MAXT, false, false>>(a, 2, V, g, blocks, sms, threads, s);
+  }
 }
 
 // Eight elements of a row to a thread while 512 threads are enough for it (768
@@ -626,23 +629,30 @@ template <typename T>
 cudaError_t start_norm_typed(const NormArgs& a, bool grad, bool gen, bool vec, unsigned blocks, int sms, cudaStream_t s) {
   constexpr int V = 16 / static_cast<int>(sizeof(T));
   auto threads_for = [&](int per) { return ((a.width + per - 1) / per + 31) / 32 * 32; };
-  int t = threads_for(16);
-  if (!grad && vec && t >= 64 && t <= 256) return start_norm<T, V, 16 / V, 256>(a, grad, gen, blocks, sms, t, s);
-  t = threads_for(8);
-  if (t <= 256)
-    return vec ? start_norm<T, V, 8 / V, 256>(a, grad, gen, blocks, sms, t, s)
-               : start_norm<T, 1, 8, 256>(a, grad, gen, blocks, sms, t, s);
-  if (t <= 512)
-    return vec ? start_norm<T, V, 8 / V, 512>(a, grad, gen, blocks, sms, t, s)
-               : start_norm<T, 1, 8, 512>(a, grad, gen, blocks, sms, t, s);
-  if (grad && vec && t <= 768) return start_norm<T, V, 8 / V, 768>(a, grad, gen, blocks, sms, t, s);
-  t = threads_for(16);
-  if (t <= 512)
-    return vec ? start_norm<T, V, 16 / V, 512>(a, grad, gen, blocks, sms, t, s)
-               : start_norm<T, 1, 16, 512>(a, grad, gen, blocks, sms, t, s);
-  t = threads_for(32);
-  return vec ? start_norm<T, V, 32 / V, 1024>(a, grad, gen, blocks, sms, t, s)
-             : start_norm<T, 1, 32, 1024>(a, grad, gen, blocks, sms, t, s);
+  const int t8 = threads_for(8), t16 = threads_for(16), t32 = threads_for(32);
+  if (!grad) {
+    if (vec) {
+      if (t16 < 64) return start_norm<false, T, V, 8 / V, 256>(a, gen, blocks, sms, t8, s);
+      if (t16 <= 256) return start_norm<false, T, V, 16 / V, 256>(a, gen, blocks, sms, t16, s);
+      if (t16 <= 512) return start_norm<false, T, V, 16 / V, 512>(a, gen, blocks, sms, t16, s);
+      return start_norm<false, T, V, 32 / V, 1024>(a, gen, blocks, sms, t32, s);
+    }
+    if (t8 <= 256) return start_norm<false, T, 1, 8, 256>(a, gen, blocks, sms, t8, s);
+    if (t8 <= 512) return start_norm<false, T, 1, 8, 512>(a, gen, blocks, sms, t8, s);
+    if (t16 <= 512) return start_norm<false, T, 1, 16, 512>(a, gen, blocks, sms, t16, s);
+    return start_norm<false, T, 1, 32, 1024>(a, gen, blocks, sms, t32, s);
+  }
+  if (vec) {
+    if (t8 <= 256) return start_norm<true, T, V, 8 / V, 256>(a, gen, blocks, sms, t8, s);
+    if (t8 <= 512) return start_norm<true, T, V, 8 / V, 512>(a, gen, blocks, sms, t8, s);
+    if (t8 <= 768) return start_norm<true, T, V, 8 / V, 768>(a, gen, blocks, sms, t8, s);
+    if (t16 <= 512) return start_norm<true, T, V, 16 / V, 512>(a, gen, blocks, sms, t16, s);
+    return start_norm<true, T, V, 32 / V, 1024>(a, gen, blocks, sms, t32, s);
+  }
+  if (t8 <= 256) return start_norm<true, T, 1, 8, 256>(a, gen, blocks, sms, t8, s);
+  if (t8 <= 512) return start_norm<true, T, 1, 8, 512>(a, gen, blocks, sms, t8, s);
+  if (t16 <= 512) return start_norm<true, T, 1, 16, 512>(a, gen, blocks, sms, t16, s);
+  return start_norm<true, T, 1, 32, 1024>(a, gen, blocks, sms, t32, s);
 }
 
 cudaError_t start_norm_f32(const NormArgs& a, bool grad, bool gen, bool vec, unsigned blocks, int sms, cudaStream_t s);

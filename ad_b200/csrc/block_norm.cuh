@@ -27,9 +27,18 @@
 // second kernel, so that results do not depend on scheduling.
 //
 // Measured, forward and gradient: 16384 x 1024 fp32 LayerNorm with a shared gate
-// 60 + 92 us (4.1 TB/s over both), 65535 x 2048 bf16 RMS with a sigmoid gate
-// 227 + 451 us (5.2 TB/s); 65536 x 1023 bf16, whose rows allow single elements
-// only, 680 us (2.0 TB/s).
+// 58 + 102 us (4.2 TB/s over both), 65535 x 2048 bf16 RMS with a sigmoid gate
+// 224 + 459 us (5.1 TB/s), 545 with one gate row for all; 65536 x 1023 bf16, whose
+// rows allow single elements only, 689 us (2.0 TB/s).
+//
+// Wide rows: the gradient's sums and row do not fit the registers.  Spilled stores
+// a thread: 224 to 744 bytes with 16 elements a thread (6145 to 8192 wide, single
+// elements from 4097), 3 to 5.3 KB with 32 (beyond), up to 276 with 768 threads
+// (4097 to 6144; none for 16-bit RMS rows without a shared gate).  RMS in bf16:
+// 16384 x 4096 95 + 232 us (4.3 TB/s over both), 8192 x 8192 107 + 332 (3.1), 4096
+// x 16384 193 + 1280 (0.9), 2048 x 32768 220 + 1650 (0.7).  fp32 RMS rows of 7172 to
+// 8192 read their weights again for each row: 8192 x 7168 170 us forward, 8192 x
+// 8192 195 (5.5 TB/s both).
 #include <algorithm>
 
 #include "ops_common.cuh"
@@ -324,8 +333,9 @@ struct Ahead {
 constexpr int FORWARD_ROWS = 2;
 // Whether the gradient's registers are held down so that 768 threads fit a
 // multiprocessor rather than 512: without means and biases, for 16-bit elements,
-// that costs nothing (65535 x 2048 bf16: 723 -> 671 us); else the sums spill
-// (16384 x 1024 fp32 LayerNorm: 163 -> 211 us).
+// vectors then spill nothing (65535 x 2048 bf16: 723 -> 671 us both directions), or
+// 64 bytes with a shared gate and up to 104 where elements are single; else the sums
+// spill more (16384 x 1024 fp32 LayerNorm: 163 -> 211 us).
 template <typename T, bool GEN>
 __host__ __device__ constexpr bool slim() {
   return sizeof(T) == 2 && !GEN;

@@ -36,10 +36,13 @@
 // the sum of two f16 numbers, the larger of which is the operand: X crosses the
 // bus as 2 + 2 bytes in each direction.
 //
-// Measured, five steps: 12 x 4096 x 1024 1257 us (666 TFLOP/s of the halves that
-// symmetry leaves), 4096 x 4096 1450 us (945), 512 x 512 119 us, where every
-// product is a wait of 7.4 us.  A block's operands come from L2 at 60 to 80 GB/s,
-// which bounds the large cases.
+// Measured, five steps: 12 x 4096 x 1024 1290 us (649 TFLOP/s of the halves that
+// symmetry leaves), 4096 x 4096 1400 to 1600 us (860 to 980), 512 x 512 119 us,
+// where every product is a wait of 7.4 us.  A block's operands come from L2 at 60 to
+// 80 GB/s, which accounts for half of the large case: its 6.5 GB of operands take
+// 595 us at that rate, the epilogues' 2.4 GB 217, norm and load 103.  The rest, some
+// 370 us, is not accounted for; the epilogues' reads of tensor memory, 8 columns
+// at a time, and items of unequal cost dealt out in turn have not been measured apart.
 #include <cuda.h>
 
 #include <cmath>

@@ -18,6 +18,13 @@ with a ``cuda_stream`` attribute); on a stream that is not the current one, and 
 operands, all results (and the workspace, where there is one) have to be given, because torch's
 allocator hands out memory for its current stream.  Sums are held in 32 bits or more and results do
 not depend on scheduling.
+
+Results are not recorded for automatic differentiation, also where operands require gradients: a
+training step calls the gradients' entry points itself, or from ``torch.autograd.Function``s as
+``examples/lm_step.py`` does.  The streams of a ``runtime.Context`` neither wait for the legacy default
+stream, on which calls with ``DeviceArray`` operands go by default, nor it for them: such a program
+waits with ``Context.sync`` before a call that reads what the context wrote, and for the stream of the
+call before the context goes on.
 """
 import ctypes
 import math
@@ -316,7 +323,7 @@ def _rotary_operands(q, k, cos, sin, positions, layout):
 def rotary(q, k, cos, sin, positions, *, layout: str = "half", inverse: bool = False, out=None, stream=None):
     """Rotary positions of queries ``q`` and keys ``k`` ([sequences, tokens, heads, dim] or [tokens,
     heads, dim], any strides with a head's elements adjacent; ``k`` may be None).  ``cos`` and ``sin``:
-    float32 tables [table rows, rotary / 2] (``rotary_table``); the first ``rotary`` elements of each
+    float32 tables [table rows, rotary / 2] (``rotary_table``; rows may be none); the first ``rotary`` elements of each
     head turn, the others are copied.  ``positions``: int64 or int32, [sequences, tokens] or [tokens]
     for all sequences; outside the table they make NaNs.  ``inverse`` turns back, which is also the
     gradient.  ``out``: (q, k) to write, which may be the operands themselves.  Returns (q, k)."""
@@ -477,8 +484,9 @@ def block_norm_grad(dh, dy, x, z, after_weight, before_weight, stats, *, gate=No
                     out=None, workspace=None, stream=None):
     """The gradients of ``block_norm``'s operands from those of its results (``dy`` is None without a
     ``before_weight``), its operands and its ``stats``: a ``BlockNormGrads``, gradients of weights and
-    biases in their type (``eps`` went into ``stats``).  ``out``: a ``BlockNormGrads`` to write; ``workspace``: adjacent elements of
-    any type, ``block_norm_grad_workspace`` bytes or more."""
+    biases in their type (``eps`` went into ``stats``), zeros where there are no rows.  ``out``: a
+    ``BlockNormGrads`` to write; ``workspace``: adjacent elements of any type,
+    ``block_norm_grad_workspace`` bytes or more."""
     dev, dt, wt, rows, width, ldx, ldz, ldg, per = _norm_operands(
         x, z, after_weight, before_weight, gate, after_bias, before_bias, kind)
     if (dy is None) != (before_weight is None):
@@ -595,7 +603,8 @@ def token_logprobs(logits, tokens, *, top: int = 0, scale: float = 1.0, out=None
     log probability of its entry of ``tokens`` (int64 or int32; 0 for a negative one, NaN for one past
     the vocabulary), the entropy of the row's distribution, and the ``top`` (at most 32) most likely
     tokens with their log probabilities, the lower index first among equal logits.  Logits of -inf are
-    masked; a row with nothing else has log probabilities of -inf, entropy 0 and no gradient.
+    masked; a row with nothing else has log probabilities of -inf, entropy 0 and no gradient.  Any other
+    mask has a probability of 0 beside larger logits, and a finite log probability while 32 bits hold it.
     ``out``: a ``TokenLogprobs`` to write."""
     dev, dt, rows, vocab, ld, t64 = _logit_operands(logits, tokens, scale)
     if not 0 <= top <= min(32, vocab):
@@ -673,9 +682,11 @@ def orthogonalize(g, *, steps: int = 5, coefficients=NEWTON_SCHULZ, eps: float =
     rows, cols], any strides), X = G / (|G| + eps), then ``steps`` times X = a X + (b A + c A A) X with
     A = X X^T (taken from the side with fewer rows).  ``coefficients``: (a, b, c), or one such triple a
     step.  Products have operands of 11 bits and sums of 32, so the result is within about 1e-3
-    (norm-wise) of the exact iteration; it is bfloat16, or of ``out``'s type.  A zero matrix gives
-    zeros, one with a NaN or an infinity NaNs.  ``workspace``: adjacent elements at a 256-byte
-    boundary, ``orthogonalize_workspace`` bytes or more."""
+    (norm-wise) of the exact iteration, in float32 too; it is bfloat16, or of ``out``'s type.  A zero
+    matrix gives zeros, whatever ``eps`` is, one with a NaN or an infinity NaNs.  X's elements are held to
+    about 2e-12, which is more than 1e-3 of a matrix with a norm below 1e-6 ``eps``.  ``workspace``:
+    adjacent elements at a 256-byte boundary, ``orthogonalize_workspace`` bytes or more.  Blocks of the kernel wait
+    for one another; where such a wait took longer than 2 s the result is NaNs, and no error is raised."""
     dt = _float(g, "g")
     dev = _device(g, "g")
     shape, st = g.shape, g.stride()

@@ -165,7 +165,8 @@ int ad_dot_tf32x3_noalloc(const float* A, const float* B, float* C, int M, int N
 /* ---- Operators of language models (no reference counterpart: the reference
  * composes such steps from its elementwise, reduce and dot nodes) ------------
  *
- * They work on the caller's device memory, allocate nothing, launch on
+ * They work on the caller's device memory (addresses are multiples of the
+ * elements' size), allocate nothing, launch on
  * `stream` (a cudaStream_t; NULL = the legacy default stream) and return
  * without waiting.  `device`: the device that the memory and the stream belong
  * to, or -1 for the current one.  Element types are AD_F32, AD_BF16, AD_F16;
@@ -183,7 +184,7 @@ int ad_dot_tf32x3_noalloc(const float* A, const float* B, float* C, int M, int N
  * (x[2i], x[2i+1]) with layout 1; pair (u, v) becomes (u c - v s, v c + u s)
  * with c, s from row positions[token] of the [table_rows][rotary / 2] tables
  * (s negated when `inverse`: also the gradient).  A position outside the
- * tables makes NaNs.  Positions are of 64 bits when pos64, else of 32. */
+ * tables (of 0 rows, too) makes NaNs.  Positions are of 64 bits when pos64, else of 32. */
 int ad_rotary(int device, int dtype, const void* q, const int64_t* q_strides, void* q_out,
               const int64_t* q_out_strides, int q_heads, const void* k, const int64_t* k_strides,
               void* k_out, const int64_t* k_out_strides, int k_heads, int64_t sequences,
@@ -230,7 +231,9 @@ int ad_clear_rows(int device, void* p, int64_t row_stride, int64_t row_bytes, in
  * probabilities, the lower index first among equal logits (-1 where fewer than
  * `top` logits are numbers).  Tokens are of 64 bits when tok64, else of 32.
  * stats: rows * 4 floats (16-byte aligned): the largest logit, the sum of
- * exp(scale (x - largest)), the entropy, the log of the sum of exp(scale x). */
+ * exp(scale (x - largest)) but for the rounding of scale times the largest, which
+ * the gradient knows (0: a row of -inf alone), the entropy, the log of the sum of
+ * exp(scale x). */
 int ad_token_logprobs(int device, int dtype, const void* logits, int64_t ld, int64_t rows,
                       int64_t vocab, const void* tokens, int tok64, float scale, int top,
                       float* logp, float* entropy, float* stats, float* top_logp,
@@ -248,8 +251,8 @@ int ad_token_logprobs_grad(int device, int dtype, const void* logits, int64_t ld
  * side with fewer rows.  Any strides; the result must not overlap G.  Products
  * take operands of 11 bits and accumulate in 32: the result is within about
  * 1e-3 (norm-wise) of the exact iteration.  Coefficients that let a singular
- * value grow past 1024 are refused.  A zero matrix gives zeros, one with NaN or
- * infinity NaNs.  Blocks wait for one another inside the one cooperative
+ * value grow past 1024 are refused.  A zero matrix gives zeros, whatever eps is,
+ * one with NaN or infinity NaNs.  Blocks wait for one another inside the one cooperative
  * kernel; a wait that runs out (2 s) leaves NaNs in the result.  The workspace
  * is 256-byte aligned. */
 int ad_orthogonalize_workspace(int64_t count, int64_t rows, int64_t cols, size_t* bytes);

@@ -28,12 +28,12 @@
 //
 // Measured, forward and gradient: 16384 x 1024 fp32 LayerNorm with a shared gate
 // 58 + 102 us (4.2 TB/s over both), 65535 x 2048 bf16 RMS with a sigmoid gate
-// 224 + 459 us (5.1 TB/s), 545 with one gate row for all; 65536 x 1023 bf16, whose
+// 224 + 459 us (5.1 TB/s), gradient 500 with one gate row for all; 65536 x 1023 bf16, whose
 // rows allow single elements only, 689 us (2.0 TB/s).
 //
 // Wide rows: the gradient's sums and row do not fit the registers.  Spilled stores
-// a thread: 224 to 744 bytes with 16 elements a thread (6145 to 8192 wide, single
-// elements from 4097), 3 to 5.3 KB with 32 (beyond), up to 276 with 768 threads
+// a thread: 224 to 752 bytes with 16 elements a thread (6145 to 8192 wide, single
+// elements from 4097), 3 to 5.5 KB with 32 (beyond), up to 272 with 768 threads
 // (4097 to 6144; none for 16-bit RMS rows without a shared gate).  RMS in bf16:
 // 16384 x 4096 95 + 232 us (4.3 TB/s over both), 8192 x 8192 107 + 332 (3.1), 4096
 // x 16384 193 + 1280 (0.9), 2048 x 32768 220 + 1650 (0.7).  fp32 RMS rows of 7172 to
@@ -334,7 +334,7 @@ constexpr int FORWARD_ROWS = 2;
 // Whether the gradient's registers are held down so that 768 threads fit a
 // multiprocessor rather than 512: without means and biases, for 16-bit elements,
 // vectors then spill nothing (65535 x 2048 bf16: 723 -> 671 us both directions), or
-// 64 bytes with a shared gate and up to 104 where elements are single; else the sums
+// 88 bytes with a shared gate and up to 104 where elements are single; else the sums
 // spill more (16384 x 1024 fp32 LayerNorm: 163 -> 211 us).
 template <typename T, bool GEN>
 __host__ __device__ constexpr bool slim() {
@@ -466,6 +466,17 @@ __global__ void __launch_bounds__(MAXT, MAXT != 256 || V * NV > 8 ? 1 : slim<T, 
     }
     ahead.commit();
   };
+  auto slopes = [&](long long row) {  // of the row's gate, onto its sums
+    if (!a.sigmoid) return;
+    Raw<T, V, NV> g;
+    g.load(pg(row), a.width);
+#pragma unroll
+    for (int i = 0; i < E; ++i) {
+      float slope;
+      sigmoid<T>(to_float(g.q[i / V].v[i % V]), slope);
+      sg[i] *= slope;
+    }
+  };
   for (int k = 0; k < S; ++k) fetch(k, r0 + k);
   const Weights<T, V, NV, GEN ? 3 : 2> weights(a, staged);
   int stage = 0;
@@ -505,12 +516,13 @@ __global__ void __launch_bounds__(MAXT, MAXT != 256 || V * NV > 8 ? 1 : slim<T, 
         for (int i = 0; i < E; ++i) u[i] += w[i];
       }
     }
-    // h in nh; from here on u is the gate's part of its own gradient
+    // h in nh; from here on u is the gate's part of its own gradient (but for the
+    // slope of a shared gate, which its sum is multiplied with)
     if (a.sigmoid && a.gate) {
 #pragma unroll
       for (int i = 0; i < E; ++i) {
-        float slope;
-        act[i] = sigmoid<T>(act[i], slope);
+        float slope = 1.0f;
+        act[i] = SHARED ? sigmoid<T>(act[i]) : sigmoid<T>(act[i], slope);
         nh[i] = a.wb ? fmaf(a.scale, nh[i], act[i] * u[i]) : 0.0f;
         u[i] *= slope;
       }
@@ -572,12 +584,14 @@ __global__ void __launch_bounds__(MAXT, MAXT != 256 || V * NV > 8 ? 1 : slim<T, 
     }
     store_row<T, V, NV>(static_cast<T*>(a.dz) + at(row, a.lddz), a.width, t);
     if (SHARED && whole && --left == 0) {
+      slopes(row);
       store_row<T, V, NV>(static_cast<T*>(a.dgate) + row / a.run * a.lddg, a.width, sg);
 #pragma unroll
       for (int i = 0; i < E; ++i) sg[i] = 0.0f;
       left = a.run;
     }
   }
+  if (SHARED && !whole) slopes(r0);
   float* part = a.part + static_cast<long long>(blockIdx.x) * SUMS * a.width;
   store_sums<V, NV>(part + SUM_WA * a.width, a.width, swa);
   store_sums<V, NV>(part + SUM_WB * a.width, a.width, swb);

@@ -16,9 +16,10 @@ ROOT = os.path.dirname(PKG)
 LIB = os.path.join(PKG, "libad_b200.so")
 SOURCES = [os.path.join(PKG, "csrc", f) for f in (
     "runtime.cu", "noalloc.cu", "rotary.cu", "block_norm.cu", "block_norm_f32.cu", "block_norm_bf16.cu",
-    "block_norm_f16.cu", "token_logprobs.cu", "orthogonalize.cu")]
+    "block_norm_f16.cu", "token_logprobs.cu", "orthogonalize.cu", "gemm16.cu", "linear_logprobs.cu",
+    "feed_forward.cu", "embed.cu", "clip_norm.cu")]
 HEADERS = [os.path.join(ROOT, "include", "ad_b200.h"), os.path.join(PKG, "csrc", "ops_common.cuh"),
-           os.path.join(PKG, "csrc", "block_norm.cuh")]
+           os.path.join(PKG, "csrc", "block_norm.cuh"), os.path.join(PKG, "csrc", "gemm16.cuh")]
 NVCC = os.environ.get("NVCC", "/usr/local/cuda/bin/nvcc")
 
 

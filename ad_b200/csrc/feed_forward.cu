@@ -1,0 +1,449 @@
+// A gated feed-forward block and its gradient: ad_feed_forward, ad_feed_forward_grad.
+//
+//   g = x Wg^T;  u = x Wu^T;  h = act(g) u;  y = h Wd^T
+//   dh = dy Wd;  du = dh act(g);  dg = dh u act'(g)
+//   dx = dg Wg + du Wu;  dWg = dg^T x;  dWu = du^T x;  dWd = dy^T h
+//
+// Bound by the tensor cores (gemm16.cuh) where there are many rows.  One kernel
+// makes g, u and h: a tile's operands are rows of both matrices, half its columns
+// each, so that x comes once and the activation and the product are its epilogue's;
+// g and u go to memory only when the gradient will want them.  Backward, dh never
+// leaves the tile: its epilogue reads g and u and writes dg, du and h, made again
+// from g and u.  dx is one product over both K's, dWg and dWu are one launch.
+// What lies between products (h, g, u, dg, du) is rounded to the operands' type:
+// half a step of 16 bits for values that are then summed over hundreds of others.
+#include <cmath>
+
+#include "gemm16.cuh"
+
+namespace {
+
+using namespace adgemm;
+
+enum Act { SILU = 0, GELU = 1, GELU_TANH = 2, RELU = 3, ACTS = 4 };
+
+constexpr float SQRT_HALF = 0.70710678118654752f;     // 1 / sqrt(2)
+constexpr float DENSITY = 0.39894228040143268f;       // 1 / sqrt(2 pi)
+constexpr float TANH_SCALE = 1.5957691216057308f;     // 2 sqrt(2 / pi)
+constexpr float TANH_CUBE = 0.044715f;
+
+// The activation, and with SLOPE its derivative.  1 + tanh(z) is twice the
+// logistic function of 2 z, which keeps the precision of what tanh brings near 0.
+template <int ACT, bool SLOPE>
+__device__ __forceinline__ float activate(float z, float* slope) {
+  if (ACT == RELU) {
+    if (SLOPE) *slope = z > 0.0f ? 1.0f : z == z ? 0.0f : z;
+    return z > 0.0f ? z : z == z ? 0.0f : z;
+  }
+  if (ACT == GELU) {
+    const float p = 0.5f * erfcf(-z * SQRT_HALF);
+    if (SLOPE) *slope = fmaf(z * DENSITY, __expf(-0.5f * z * z), p);
+    return z * p;
+  }
+  float q = 1.0f, w = z;  // the logistic function's argument and its derivative
+  if (ACT == GELU_TANH) {
+    w = TANH_SCALE * z * fmaf(TANH_CUBE * z, z, 1.0f);
+    q = TANH_SCALE * fmaf(3.0f * TANH_CUBE * z, z, 1.0f);
+  }
+  const float e = __expf(-fabsf(w));  // no overflow on either side
+  const float r = __fdividef(1.0f, 1.0f + e);
+  const float p = w >= 0.0f ? r : e * r, other = w >= 0.0f ? e * r : r;
+  if (SLOPE) *slope = z == z ? fmaf(fabsf(z) < 1e18f ? z * q * p : 0.0f, other, p) : z;
+  return z * p;
+}
+
+// h of 32 columns from accumulators of both products.
+struct Gated {
+  static constexpr bool DUAL = true;
+  struct Params {
+    unsigned short *h, *gate, *up;  // gate, up: NULL when not kept
+    long long ldh, ldg, ldu;
+    int vec_h, vec_g, vec_u, act;
+  };
+  struct State {
+    __device__ State(const Params&, const Shape&, const Spot&, int, int, int) {}
+    __device__ void end(const Params&, const Shape&, const Spot&, int) {}
+    template <int ACT>
+    __device__ static void gated(float (&g)[32], const float (&u)[32]) {
+#pragma unroll
+      for (int j = 0; j < 32; ++j) g[j] = activate<ACT, false>(g[j], nullptr) * u[j];
+    }
+    __device__ static void round(const float (&v)[32], unsigned (&w)[16], int half) {
+      if (half) {
+#pragma unroll
+        for (int j = 0; j < 16; ++j) w[j] = pack2(v[2 * j], v[2 * j + 1], 1);
+      } else {
+#pragma unroll
+        for (int j = 0; j < 16; ++j) w[j] = pack2(v[2 * j], v[2 * j + 1], 0);
+      }
+    }
+    __device__ void chunk(const Params& p, const Shape& a, const Spot& s, int col0, unsigned acc, int cols) {
+      unsigned q[32], t[32], w[16];
+      float g[32], u[32];
+      tmem_issue32(acc, q);
+      tmem_issue32(acc + cols, t);
+      tmem_wait32(q);
+      tmem_wait32(t);
+#pragma unroll
+      for (int j = 0; j < 32; ++j) {
+        g[j] = s.dead ? __int_as_float(0x7fffffff) : __uint_as_float(q[j]);
+        u[j] = __uint_as_float(t[j]);
+      }
+      if (p.gate) {
+        round(g, w, a.half);
+        put16(s, w, p.gate, p.ldg, a.m, a.n, col0, p.vec_g);
+        round(u, w, a.half);
+        put16(s, w, p.up, p.ldu, a.m, a.n, col0, p.vec_u);
+      }
+      switch (p.act) {
+        case SILU: gated<SILU>(g, u); break;
+        case GELU: gated<GELU>(g, u); break;
+        case GELU_TANH: gated<GELU_TANH>(g, u); break;
+        default: gated<RELU>(g, u);
+      }
+      round(g, w, a.half);
+      put16(s, w, p.h, p.ldh, a.m, a.n, col0, p.vec_h);
+    }
+  };
+};
+
+// dg, du and h from an accumulator of dh, eight columns of a row a lane.
+struct GatedGrad {
+  static constexpr bool DUAL = false;
+  struct Params {
+    const unsigned short *gate, *up;
+    long long ldg, ldu;
+    int vec;  // of g and u
+    unsigned short *dg, *du, *h;
+    long long ld;  // of these, whose rows are aligned
+    int act;
+  };
+  struct State {
+    __device__ State(const Params&, const Shape&, const Spot&, int, int, int) {}
+    __device__ void end(const Params&, const Shape&, const Spot&, int) {}
+    template <int ACT>
+    __device__ static void one(float dh, float g, float u, float& dg, float& du, float& h) {
+      float slope;
+      const float act = activate<ACT, true>(g, &slope);
+      dg = dh * u * slope, du = dh * act, h = act * u;
+    }
+    template <int ACT>
+    __device__ static void eight(const float (&dh)[8], const uint4& g, const uint4& u, uint4& dg, uint4& du, uint4& h,
+                                 int half) {
+      const unsigned gs[4] = {g.x, g.y, g.z, g.w}, us[4] = {u.x, u.y, u.z, u.w};
+      unsigned a[4], b[4], c[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const float2 gg = unpack2(gs[j], half), uu = unpack2(us[j], half);
+        float x[2], y[2], z[2];
+        one<ACT>(dh[2 * j], gg.x, uu.x, x[0], y[0], z[0]);
+        one<ACT>(dh[2 * j + 1], gg.y, uu.y, x[1], y[1], z[1]);
+        a[j] = pack2(x[0], x[1], half), b[j] = pack2(y[0], y[1], half), c[j] = pack2(z[0], z[1], half);
+      }
+      dg = make_uint4(a[0], a[1], a[2], a[3]), du = make_uint4(b[0], b[1], b[2], b[3]), h = make_uint4(c[0], c[1], c[2], c[3]);
+    }
+    template <int ACT>
+    __device__ static void part(const Params& p, const Shape& a, const Spot& s, int col0, const uint4 (&g)[4],
+                                const uint4 (&u)[4]) {
+      const int q = s.lane & 3;
+#pragma unroll 1
+      for (int i = 0; i < 4; ++i) {
+        const int r = i * 8 + (s.lane >> 2);
+        const float4 x = staged(s, r, 2 * q), y = staged(s, r, 2 * q + 1);
+        const float dh[8] = {x.x, x.y, x.z, x.w, y.x, y.y, y.z, y.w};
+        uint4 dg, du, h, gi = g[0], ui = u[0];
+#pragma unroll
+        for (int k = 1; k < 4; ++k)
+          if (i == k) gi = g[k], ui = u[k];
+        eight<ACT>(dh, gi, ui, dg, du, h, a.half);
+        if (s.row0 + r < a.m) {
+          const long long at = (s.row0 + r) * p.ld + col0 + q * 8;
+          *reinterpret_cast<uint4*>(p.dg + at) = dg;
+          *reinterpret_cast<uint4*>(p.du + at) = du;
+          *reinterpret_cast<uint4*>(p.h + at) = h;
+        }
+      }
+    }
+    template <int ACT>
+    __device__ static void columns(const Params& p, const Shape& a, const Spot& s, int col0) {
+      const int col = col0 + s.lane;
+      if (col >= a.n) return;
+      for (int r = 0; r < 32 && s.row0 + r < a.m; ++r) {
+        float dh;
+        asm volatile("ld.shared.f32 %0, [%1];"
+                     : "=f"(dh)
+                     : "r"(s.side + r * 128 + (((s.lane >> 2) ^ (r & 7)) << 4) + (s.lane & 3) * 4)
+                     : "memory");
+        const int type = a.half ? AD_F16 : AD_BF16;
+        const long long row = s.row0 + r;
+        float dg, du, h;
+        one<ACT>(dh, load_any(p.gate, type, row * p.ldg + col), load_any(p.up, type, row * p.ldu + col), dg, du, h);
+        store_any(p.dg, type, row * p.ld + col, dg);
+        store_any(p.du, type, row * p.ld + col, du);
+        store_any(p.h, type, row * p.ld + col, h);
+      }
+    }
+    __device__ void chunk(const Params& p, const Shape& a, const Spot& s, int col0, unsigned acc, int) {
+      const bool fast = p.vec && col0 + CHUNK <= a.n;
+      uint4 g[4], u[4];
+      if (fast) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const long long row = s.row0 + i * 8 + (s.lane >> 2);
+          g[i] = u[i] = make_uint4(0, 0, 0, 0);
+          if (row < a.m) {
+            g[i] = *reinterpret_cast<const uint4*>(p.gate + row * p.ldg + col0 + (s.lane & 3) * 8);
+            u[i] = *reinterpret_cast<const uint4*>(p.up + row * p.ldu + col0 + (s.lane & 3) * 8);
+          }
+        }
+      }
+      float v[32];
+      tmem_ld32(acc, v);
+      if (s.dead) {
+#pragma unroll
+        for (int j = 0; j < 32; ++j) v[j] = __int_as_float(0x7fffffff);
+      }
+      stage32(s, v);
+      if (fast) {
+        switch (p.act) {
+          case SILU: part<SILU>(p, a, s, col0, g, u); break;
+          case GELU: part<GELU>(p, a, s, col0, g, u); break;
+          case GELU_TANH: part<GELU_TANH>(p, a, s, col0, g, u); break;
+          default: part<RELU>(p, a, s, col0, g, u);
+        }
+      } else {
+        switch (p.act) {
+          case SILU: columns<SILU>(p, a, s, col0); break;
+          case GELU: columns<GELU>(p, a, s, col0); break;
+          case GELU_TANH: columns<GELU_TANH>(p, a, s, col0); break;
+          default: columns<RELU>(p, a, s, col0);
+        }
+      }
+    }
+  };
+};
+
+// ------------------------------------------------------------------ host
+
+struct Operand {
+  const void* p;
+  long long ld, rows, cols;
+};
+
+struct Layout {
+  size_t pack[5], h, dg, du, partial, total;
+  long long ld;  // of h, dg, du
+  Plan hidden, y, dh, dx, dw, dd;
+};
+
+Problem hidden_of(int device, int half, long long rows, long long width, long long hidden) {
+  Problem p = {};
+  p.device = device, p.half = half;
+  p.m = rows, p.n = hidden, p.k = p.k0 = width, p.groups = 1;
+  return p;
+}
+Problem y_of(int device, int half, long long rows, long long width, long long hidden) {
+  Problem p = hidden_of(device, half, rows, hidden, width);
+  return p;
+}
+Problem dh_of(int device, int half, long long rows, long long width, long long hidden) {
+  Problem p = hidden_of(device, half, rows, width, hidden);
+  p.b_turned = true;
+  return p;
+}
+Problem dx_of(int device, int half, long long rows, long long width, long long hidden) {
+  Problem p = {};
+  p.device = device, p.half = half;
+  p.m = rows, p.n = width, p.k = 2 * hidden, p.k0 = hidden, p.groups = 1;
+  p.b_turned = true;
+  return p;
+}
+Problem dw_of(int device, int half, long long rows, long long m, long long n, int groups) {
+  Problem p = {};
+  p.device = device, p.half = half;
+  p.m = m, p.n = n, p.k = p.k0 = rows, p.groups = groups;
+  p.a_turned = p.b_turned = true;
+  return p;
+}
+
+// ops: x, Wg, Wu, Wd and, for the gradient, dy.
+Layout plan(int device, const Operand* ops, int count, long long rows, long long width, long long hidden, int sms) {
+  Layout l = {};
+  size_t at = 0;
+  auto take = [&](size_t bytes) {
+    const size_t here = at;
+    at += room(bytes);
+    return here;
+  };
+  for (int i = 0; i < count; ++i)
+    if (!tma_ready(ops[i].p, ops[i].ld, ops[i].rows)) l.pack[i] = take(2ull * ops[i].rows * round_up(ops[i].cols, 64));
+  l.ld = round_up(hidden, 64);
+  l.h = take(2ull * rows * l.ld);
+  const long long kblocks = (width + BK - 1) / BK;
+  if (count == 4) {
+    l.hidden = plan_for(rows, hidden, kblocks, 1, true, false, sms);
+    const Problem y = y_of(device, 0, rows, width, hidden);
+    l.y = store_plan(y, sms);
+    l.partial = take(partial_bytes(y, l.y, false));
+  } else {
+    l.dg = take(2ull * rows * l.ld);
+    l.du = take(2ull * rows * l.ld);
+    l.dh = plan_for(rows, hidden, kblocks, 1, false, false, sms);
+    const Problem x = dx_of(device, 0, rows, width, hidden), w = dw_of(device, 0, rows, hidden, width, 2),
+                  d = dw_of(device, 0, rows, width, hidden, 1);
+    l.dx = store_plan(x, sms), l.dw = store_plan(w, sms), l.dd = store_plan(d, sms);
+    l.partial = take(std::max({partial_bytes(x, l.dx, false), partial_bytes(w, l.dw, false), partial_bytes(d, l.dd, false)}));
+  }
+  l.total = at;
+  return l;
+}
+
+int check(const char* who, int dtype, int64_t rows, int64_t width, int64_t hidden, int act, const Operand* ops, int count) {
+  if (dtype != AD_BF16 && dtype != AD_F16) return fail("%s: unknown element type %d (AD_BF16 or AD_F16)", who, dtype);
+  if (rows < 0 || width < 1 || hidden < 1) return fail("%s: %lld rows of %lld, %lld hidden", who, (long long)rows, (long long)width, (long long)hidden);
+  if (rows > (1 << 24) || width > (1 << 20) || hidden > (1 << 20)) return fail("%s: at most 2^24 rows of 2^20 elements", who);
+  if (act < 0 || act >= ACTS) return fail("%s: unknown activation %d", who, act);
+  for (int i = 0; i < count; ++i) {
+    if (ops[i].rows > 1 && ops[i].ld < ops[i].cols) return fail("%s: rows overlap", who);
+    if (!aligned(ops[i].p, 2)) return fail("%s: an operand is not aligned to its elements", who);
+  }
+  return 0;
+}
+
+// An operand as TMA reads it: itself, or its copy.
+int ready(const char* who, const Operand& o, unsigned char* copy, cudaStream_t st, Mat* m) {
+  *m = Mat{o.p, o.ld};
+  if (tma_ready(o.p, o.ld, o.rows)) return 0;
+  *m = Mat{copy, round_up(o.cols, 64)};
+  return pack_rows(who, o.p, o.ld, o.rows, o.cols, copy, m->ld, st);
+}
+
+bool vec16(const void* p, long long ld, long long rows) { return aligned(p, 16) && (rows <= 1 || ld % 8 == 0); }
+
+}  // namespace
+
+extern "C" int ad_feed_forward_workspace(int device, int dtype, const void* x, int64_t ldx, const void* w_gate,
+                                         int64_t ld_gate, const void* w_up, int64_t ld_up, const void* w_down,
+                                         int64_t ld_down, const void* dy, int64_t lddy, int64_t rows, int64_t width,
+                                         int64_t hidden, int grad, size_t* bytes) {
+  const char* who = "ad_feed_forward_workspace";
+  if (!bytes) return fail("%s: null operand", who);
+  const Operand ops[5] = {{x, ldx, rows, width}, {w_gate, ld_gate, hidden, width}, {w_up, ld_up, hidden, width},
+                          {w_down, ld_down, width, hidden}, {dy, lddy, rows, width}};
+  const int count = grad ? 5 : 4;
+  if (check(who, dtype, rows, width, hidden, 0, ops, count)) return 1;
+  *bytes = 0;
+  if (!rows) return 0;
+  DeviceGuard guard(device);
+  if (guard.error() != cudaSuccess) return fail_cuda(who, guard.error());
+  const int sms = sm_count(guard.device());
+  if (!sms) return fail("%s: no device properties", who);
+  *bytes = plan(guard.device(), ops, count, rows, width, hidden, sms).total;
+  return 0;
+}
+
+extern "C" int ad_feed_forward(int device, int dtype, int act, const void* x, int64_t ldx, const void* w_gate,
+                               int64_t ld_gate, const void* w_up, int64_t ld_up, const void* w_down, int64_t ld_down,
+                               int64_t rows, int64_t width, int64_t hidden, void* y, int64_t ldy, void* gate, int64_t ldg,
+                               void* up, int64_t ldu, void* workspace, size_t workspace_bytes, void* stream) {
+  const char* who = "ad_feed_forward";
+  const Operand ops[4] = {{x, ldx, rows, width}, {w_gate, ld_gate, hidden, width}, {w_up, ld_up, hidden, width},
+                          {w_down, ld_down, width, hidden}};
+  if (check(who, dtype, rows, width, hidden, act, ops, 4)) return 1;
+  if ((gate == nullptr) != (up == nullptr) && rows) return fail("%s: gate and up are kept together", who);
+  if (rows > 1 && (ldy < width || (gate && (ldg < hidden || ldu < hidden)))) return fail("%s: rows overlap", who);
+  if (!rows) return 0;
+  if (!x || !w_gate || !w_up || !w_down || !y) return fail("%s: null operand", who);
+  if (!aligned({y, gate, up}, 2)) return fail("%s: an operand is not aligned to its elements", who);
+  DeviceGuard guard(device);
+  if (guard.error() != cudaSuccess) return fail_cuda(who, guard.error());
+  const int dev = guard.device(), half = dtype == AD_F16, sms = sm_count(dev);
+  if (!sms) return fail("%s: no device properties", who);
+  const Layout l = plan(dev, ops, 4, rows, width, hidden, sms);
+  if (!workspace || !aligned(workspace, 256) || workspace_bytes < l.total)
+    return fail("%s: needs %zu bytes of workspace, 256-byte aligned", who, l.total);
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  unsigned char* ws = static_cast<unsigned char*>(workspace);
+  Mat m[4];
+  for (int i = 0; i < 4; ++i)
+    if (ready(who, ops[i], ws + l.pack[i], st, &m[i])) return 1;
+  Problem p = hidden_of(dev, half, rows, width, hidden);
+  p.a[0] = m[0], p.b[0] = m[1], p.b[1] = m[2];
+  Gated::Params q = {};
+  q.h = reinterpret_cast<unsigned short*>(ws + l.h), q.ldh = l.ld, q.vec_h = 1;
+  q.gate = static_cast<unsigned short*>(gate), q.up = static_cast<unsigned short*>(up);
+  q.ldg = ldg, q.ldu = ldu, q.vec_g = vec16(gate, ldg, rows), q.vec_u = vec16(up, ldu, rows);
+  q.act = act;
+  if (start<Gated>(who, p, l.hidden, q, sms, st)) return 1;
+  p = y_of(dev, half, rows, width, hidden);
+  p.a[0] = Mat{ws + l.h, l.ld}, p.b[0] = m[3];
+  const Out out = {y, ldy};
+  return store_product(who, p, l.y, dtype, &out, false, nullptr, reinterpret_cast<float*>(ws + l.partial), nullptr, sms, st);
+}
+
+extern "C" int ad_feed_forward_grad(int device, int dtype, int act, const void* dy, int64_t lddy, const void* x,
+                                    int64_t ldx, const void* w_gate, int64_t ld_gate, const void* w_up, int64_t ld_up,
+                                    const void* w_down, int64_t ld_down, const void* gate, int64_t ldg, const void* up,
+                                    int64_t ldu, int64_t rows, int64_t width, int64_t hidden, void* dx, int64_t lddx,
+                                    int dw_type, void* dw_gate, int64_t lddw_gate, void* dw_up, int64_t lddw_up,
+                                    void* dw_down, int64_t lddw_down, int accumulate, void* workspace,
+                                    size_t workspace_bytes, void* stream) {
+  const char* who = "ad_feed_forward_grad";
+  const Operand ops[5] = {{x, ldx, rows, width}, {w_gate, ld_gate, hidden, width}, {w_up, ld_up, hidden, width},
+                          {w_down, ld_down, width, hidden}, {dy, lddy, rows, width}};
+  if (check(who, dtype, rows, width, hidden, act, ops, 5)) return 1;
+  if (dw_type != dtype && dw_type != AD_F32) return fail("%s: unknown type %d of the weights' gradients", who, dw_type);
+  const size_t es = elem_size(dw_type);
+  if (!dw_gate || !dw_up || !dw_down || !aligned({dw_gate, dw_up, dw_down}, es))
+    return fail("%s: an operand is null or not aligned to its elements", who);
+  if ((rows > 1 && (lddx < width || ldg < hidden || ldu < hidden)) ||
+      (hidden > 1 && (lddw_gate < width || lddw_up < width)) || (width > 1 && lddw_down < hidden))
+    return fail("%s: rows overlap", who);
+  if (!rows) {
+    if (accumulate) return 0;
+    return ad_clear_rows(device, dw_gate, lddw_gate * es, width * es, hidden, stream) ||
+           ad_clear_rows(device, dw_up, lddw_up * es, width * es, hidden, stream) ||
+           ad_clear_rows(device, dw_down, lddw_down * es, hidden * es, width, stream);
+  }
+  if (!dy || !x || !w_gate || !w_up || !w_down || !gate || !up || !dx) return fail("%s: null operand", who);
+  if (!aligned({gate, up, dx}, 2)) return fail("%s: an operand is not aligned to its elements", who);
+  DeviceGuard guard(device);
+  if (guard.error() != cudaSuccess) return fail_cuda(who, guard.error());
+  const int dev = guard.device(), half = dtype == AD_F16, sms = sm_count(dev);
+  if (!sms) return fail("%s: no device properties", who);
+  const Layout l = plan(dev, ops, 5, rows, width, hidden, sms);
+  if (!workspace || !aligned(workspace, 256) || workspace_bytes < l.total)
+    return fail("%s: needs %zu bytes of workspace, 256-byte aligned", who, l.total);
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  unsigned char* ws = static_cast<unsigned char*>(workspace);
+  float* partial = reinterpret_cast<float*>(ws + l.partial);
+  Mat m[5];
+  for (int i = 0; i < 5; ++i)
+    if (ready(who, ops[i], ws + l.pack[i], st, &m[i])) return 1;
+  const Mat h = {ws + l.h, l.ld}, dg = {ws + l.dg, l.ld}, du = {ws + l.du, l.ld};
+
+  Problem p = dh_of(dev, half, rows, width, hidden);
+  p.a[0] = m[4], p.b[0] = m[3];
+  GatedGrad::Params q = {};
+  q.gate = static_cast<const unsigned short*>(gate), q.up = static_cast<const unsigned short*>(up);
+  q.ldg = ldg, q.ldu = ldu, q.vec = vec16(gate, ldg, rows) && vec16(up, ldu, rows);
+  q.dg = reinterpret_cast<unsigned short*>(ws + l.dg), q.du = reinterpret_cast<unsigned short*>(ws + l.du);
+  q.h = reinterpret_cast<unsigned short*>(ws + l.h), q.ld = l.ld;
+  q.act = act;
+  if (start<GatedGrad>(who, p, l.dh, q, sms, st)) return 1;
+
+  p = dx_of(dev, half, rows, width, hidden);
+  p.a[0] = dg, p.a[1] = du, p.b[0] = m[1], p.b[1] = m[2];
+  Out out[2] = {{dx, lddx}, {}};
+  if (store_product(who, p, l.dx, dtype, out, false, nullptr, partial, nullptr, sms, st)) return 1;
+
+  p = dw_of(dev, half, rows, hidden, width, 2);
+  p.a[0] = dg, p.a[1] = du, p.b[0] = p.b[1] = m[0];
+  out[0] = {dw_gate, lddw_gate}, out[1] = {dw_up, lddw_up};
+  if (store_product(who, p, l.dw, dw_type, out, accumulate != 0, nullptr, partial, nullptr, sms, st)) return 1;
+
+  p = dw_of(dev, half, rows, width, hidden, 1);
+  p.a[0] = m[4], p.b[0] = h;
+  out[0] = {dw_down, lddw_down};
+  return store_product(who, p, l.dd, dw_type, out, accumulate != 0, nullptr, partial, nullptr, sms, st);
+}

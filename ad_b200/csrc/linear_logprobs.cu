@@ -1,0 +1,423 @@
+// Log probabilities of given tokens under softmax(scale x W^T) over a large
+// vocabulary, without its logits in memory: ad_linear_logprobs and its gradient.
+//
+//   z = x W^T;  lse = log sum_v exp(scale z_v);  logp = scale z_t - lse
+//   dz = scale ((g_lse - g_logp) p + g_logp [v = t]),  p = exp(scale z - lse)
+//   dx = dz W,  dW = dz^T x
+//
+// Bound by the tensor cores (gemm16.cuh).  Forward: a tile's epilogue reduces each
+// row of its logits to their largest and the sum of exponents from there, one pass
+// over the accumulator with a running maximum; a small kernel joins the tiles'
+// pairs.  Backward: pieces of the vocabulary, of each of which the logits are made
+// again (a product of three instead of two; kept they would be rows x vocab), turned
+// into dz in the epilogue, rounded to the operands' type and used twice: as rows for
+// dx, which is summed over the pieces in 32 bits, and across for the piece's rows of dW.
+//
+// dz in f16 is held times a power of two that puts the largest gradient of a row
+// at 2^14: what it loses is below 2^-38 of that.
+//
+#include <cfloat>
+#include <cmath>
+
+#include "gemm16.cuh"
+
+namespace {
+
+using namespace adgemm;
+
+constexpr float LOG2E = 1.4426950408889634f;
+
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+__device__ __forceinline__ long long token_at(const void* tokens, int tok64, long long i) {
+  return tok64 ? static_cast<const long long*>(tokens)[i] : static_cast<const int*>(tokens)[i];
+}
+
+// A row's largest logit and the sum of exponents from there, over a tile's columns.
+struct Sum {
+  static constexpr bool DUAL = false;
+  struct Params {
+    float2* part;   // [2 x column tiles][rows]
+    float* target;  // [rows]
+    const void* tokens;
+    int tok64;
+    float k;  // scale log2(e)
+  };
+  struct State {
+    float top, sum;
+    int token;  // -1: not in reach
+    __device__ State(const Params& p, const Shape& a, const Spot& s, int, int, int) {
+      top = -INFINITY, sum = 0.0f, token = -1;
+      const int row = s.row0 + s.lane;
+      if (row < a.m) {
+        const long long t = token_at(p.tokens, p.tok64, row);
+        if (t >= 0 && t < a.n) token = static_cast<int>(t);
+      }
+    }
+    __device__ void chunk(const Params& p, const Shape& a, const Spot& s, int col0, unsigned acc, int) {
+      float v[32];
+      tmem_ld32(acc, v);
+      if (col0 + CHUNK > a.n) {
+#pragma unroll
+        for (int j = 0; j < 32; ++j)
+          if (col0 + j >= a.n) v[j] = -INFINITY;
+      }
+      const unsigned at = static_cast<unsigned>(token - col0);
+      if (__any_sync(0xffffffffu, at < 32u)) {
+        float z = 0.0f;
+#pragma unroll
+        for (int j = 0; j < 32; ++j)
+          if (at == j) z = v[j];
+        if (at < 32u) p.target[s.row0 + s.lane] = z;
+      }
+      float most = v[0];
+#pragma unroll
+      for (int j = 1; j < 32; ++j) most = fmaxf(most, v[j]);
+      most = fmaxf(most, top);
+      const float from = most == -INFINITY ? 0.0f : most;
+      // the difference first: scale times a large logit would lose what tells logits apart
+      float part[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+      for (int j = 0; j < 32; ++j) part[j & 3] += ex2((v[j] - from) * p.k);
+      sum = sum * ex2((top - from) * p.k) + ((part[0] + part[1]) + (part[2] + part[3]));
+      top = most;
+    }
+    __device__ void end(const Params& p, const Shape& a, const Spot& s, int part) {
+      const int row = s.row0 + s.lane;
+      if (s.dead) sum = __int_as_float(0x7fffffff);
+      if (row < a.m) p.part[(2ll * s.unit_col + part) * a.m + row] = make_float2(top, sum);
+    }
+  };
+};
+
+struct FinishArgs {
+  const float2* part;
+  const float* target;
+  const void* tokens;
+  int tok64, parts, rows;
+  long long vocab;
+  float scale, k;
+  float *logp, *lse;
+  float2* stats;
+};
+
+// Joins the tiles' pairs: 32 rows a block, 16 warps over the tiles.
+constexpr int FINISH_WARPS = 16;
+__global__ void __launch_bounds__(32 * FINISH_WARPS) finish_kernel(const __grid_constant__ FinishArgs a) {
+  __shared__ float2 buf[FINISH_WARPS][32];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int row = blockIdx.x * 32 + lane;
+  float top = -INFINITY, sum = 0.0f;
+  auto join = [&](float2 x) {
+    const float most = fmaxf(top, x.x), from = most == -INFINITY ? 0.0f : most;
+    sum = sum * ex2((top - from) * a.k) + x.y * ex2((x.x - from) * a.k);
+    top = most;
+  };
+  if (row < a.rows) {
+#pragma unroll 4
+    for (int i = warp; i < a.parts; i += FINISH_WARPS) join(a.part[static_cast<long long>(i) * a.rows + row]);
+  }
+  buf[warp][lane] = make_float2(top, sum);
+  __syncthreads();
+  if (warp || row >= a.rows) return;
+  for (int w = 1; w < FINISH_WARPS; ++w) join(buf[w][lane]);
+  const long long t = token_at(a.tokens, a.tok64, row);
+  const float log_sum = logf(sum);
+  a.lse[row] = a.scale * top + log_sum;
+  a.logp[row] = t < 0          ? 0.0f
+                : t >= a.vocab ? __int_as_float(0x7fffffff)
+                               : a.scale * (a.target[row] - top) - log_sum;
+  a.stats[row] = make_float2(top, sum);
+}
+
+// The power of two for f16 (factor[0]) and its reciprocal (factor[1]).
+struct RangeArgs {
+  const float *g_logp, *g_lse;
+  int rows;
+  float scale;
+  float* factor;
+};
+__global__ void __launch_bounds__(1024) range_kernel(const __grid_constant__ RangeArgs a) {
+  __shared__ float buf[32];
+  float most = 0.0f;
+  for (int i = threadIdx.x; i < a.rows; i += 1024)
+    most = fmaxf(most, (a.g_logp ? 2.0f * fabsf(a.g_logp[i]) : 0.0f) + (a.g_lse ? fabsf(a.g_lse[i]) : 0.0f));
+#pragma unroll
+  for (int o = 16; o; o >>= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, o));
+  if ((threadIdx.x & 31) == 0) buf[threadIdx.x >> 5] = most;
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    for (int w = 1; w < 32; ++w) most = fmaxf(most, buf[w]);
+    most *= a.scale;
+    int e = 0;
+    if (most > 0.0f && most < INFINITY) e = max(-100, min(100, 14 - ilogbf(most)));
+    a.factor[0] = ldexpf(1.0f, e);
+    a.factor[1] = ldexpf(1.0f, -e);
+  }
+}
+
+// dz of a piece of the vocabulary.
+struct Slope {
+  static constexpr bool DUAL = false;
+  struct Params {
+    const float2* stats;
+    const void* tokens;
+    int tok64;
+    const float *g_logp, *g_lse;
+    const float* factor;
+    long long vocab, first;  // of all; the piece's first column
+    float k, scale;
+    unsigned short* out;
+    long long ld;
+  };
+  struct State {
+    float top, of_p, of_hot;
+    int hot;  // the token's column in the piece
+    __device__ State(const Params& p, const Shape& a, const Spot& s, int, int, int) {
+      top = 0.0f, of_p = 0.0f, of_hot = 0.0f, hot = -1;
+      const int row = s.row0 + s.lane;
+      if (row >= a.m) return;
+      const float2 st = p.stats[row];
+      const long long t = token_at(p.tokens, p.tok64, row);
+      const float f = p.factor ? *p.factor : 1.0f;
+      const float gp = p.g_logp && t >= 0 ? p.g_logp[row] : 0.0f, gl = p.g_lse ? p.g_lse[row] : 0.0f;
+      top = st.x;
+      of_p = t >= p.vocab ? __int_as_float(0x7fffffff) : p.scale * (gl - gp) * f / st.y;
+      of_hot = p.scale * gp * f;
+      if (t >= p.first && t < p.first + a.n) hot = static_cast<int>(t - p.first);
+    }
+    __device__ void chunk(const Params& p, const Shape& a, const Spot& s, int col0, unsigned acc, int) {
+      float v[32];
+      tmem_ld32(acc, v);
+#pragma unroll
+      for (int j = 0; j < 32; ++j) v[j] = s.dead ? __int_as_float(0x7fffffff) : ex2((v[j] - top) * p.k) * of_p;
+      const unsigned at = static_cast<unsigned>(hot - col0);
+      if (__any_sync(0xffffffffu, at < 32u)) {
+#pragma unroll
+        for (int j = 0; j < 32; ++j)
+          if (at == j) v[j] += of_hot;
+      }
+      unsigned w[16];
+      if (a.half) {
+#pragma unroll
+        for (int j = 0; j < 16; ++j) w[j] = pack2(v[2 * j], v[2 * j + 1], 1);
+      } else {
+#pragma unroll
+        for (int j = 0; j < 16; ++j) w[j] = pack2(v[2 * j], v[2 * j + 1], 0);
+      }
+      put16(s, w, p.out, p.ld, a.m, a.n, col0, 1);
+    }
+    __device__ void end(const Params&, const Shape&, const Spot&, int) {}
+  };
+};
+
+// ------------------------------------------------------------------ host
+
+constexpr long long PIECE = 1ll << 28;  // elements of dz at a time: half a gigabyte
+
+struct Layout {
+  bool pack_x, pack_w;
+  long long ld_packed;
+  Plan forward, slope, dx, dw;
+  long long piece, pieces;
+  size_t x, w, part, target, factor, dz, sum_dx, sum_dw, total;
+};
+
+Problem logits(int device, int half, long long rows, long long width, long long vocab) {
+  Problem p = {};
+  p.device = device, p.half = half;
+  p.m = rows, p.n = vocab, p.k = p.k0 = width, p.groups = 1;
+  return p;
+}
+Problem dx_of(int device, int half, long long rows, long long width, long long piece) {
+  Problem p = {};
+  p.device = device, p.half = half;
+  p.m = rows, p.n = width, p.k = p.k0 = piece, p.groups = 1;
+  p.b_turned = true;
+  return p;
+}
+Problem dw_of(int device, int half, long long rows, long long width, long long piece) {
+  Problem p = {};
+  p.device = device, p.half = half;
+  p.m = piece, p.n = width, p.k = p.k0 = rows, p.groups = 1;
+  p.a_turned = p.b_turned = true;
+  return p;
+}
+
+Layout plan(int device, const void* x, long long ldx, const void* w, long long ldw, long long rows, long long width,
+            long long vocab, bool grad, int sms) {
+  Layout l = {};
+  l.pack_x = !tma_ready(x, ldx, rows), l.pack_w = !tma_ready(w, ldw, vocab);
+  l.ld_packed = round_up(width, 64);
+  size_t at = 0;
+  auto take = [&](size_t bytes) {
+    const size_t here = at;
+    at += room(bytes);
+    return here;
+  };
+  if (l.pack_x) l.x = take(2ull * rows * l.ld_packed);
+  if (l.pack_w) l.w = take(2ull * vocab * l.ld_packed);
+  const long long kblocks = (width + BK - 1) / BK;
+  if (!grad) {
+    l.forward = plan_for(rows, vocab, kblocks, 1, false, false, sms);
+    const long long cols = l.forward.tile == 0 ? 256 : l.forward.tile == 1 ? 128 : 64;
+    l.part = take(sizeof(float2) * 2 * ((vocab + cols - 1) / cols) * rows);
+    l.target = take(sizeof(float) * rows);
+  } else {
+    l.pieces = (vocab * rows + PIECE - 1) / PIECE;
+    // at least 1024 columns, so that the products with a piece do not fall apart
+    l.pieces = std::max(1ll, std::min(l.pieces, (vocab + 1023) / 1024));
+    l.piece = std::min(round_up((vocab + l.pieces - 1) / l.pieces, 256), round_up(vocab, 8));
+    l.pieces = (vocab + l.piece - 1) / l.piece;
+    const long long first = std::min(l.piece, vocab);
+    l.slope = plan_for(rows, first, kblocks, 1, false, false, sms);
+    const Problem px = dx_of(device, 0, rows, width, first), pw = dw_of(device, 0, rows, width, first);
+    l.dx = store_plan(px, sms), l.dw = store_plan(pw, sms);
+    l.factor = take(2 * sizeof(float));
+    l.dz = take(2ull * rows * l.piece);
+    l.sum_dx = take(partial_bytes(px, l.dx, l.pieces > 1));
+    l.sum_dw = take(partial_bytes(pw, l.dw, false));
+  }
+  l.total = at;
+  return l;
+}
+
+int check(const char* who, int dtype, const void* x, int64_t ldx, const void* w, int64_t ldw, int64_t rows, int64_t width,
+          int64_t vocab) {
+  if (dtype != AD_BF16 && dtype != AD_F16) return fail("%s: unknown element type %d (AD_BF16 or AD_F16)", who, dtype);
+  if (rows < 0 || width < 1 || vocab < 1) return fail("%s: %lld rows of %lld, %lld tokens", who, (long long)rows, (long long)width, (long long)vocab);
+  if (rows > (1 << 24) || width > (1 << 20) || vocab > (1 << 24))
+    return fail("%s: at most 2^24 rows and tokens, of 2^20 elements", who);
+  if ((rows > 1 && ldx < width) || (vocab > 1 && ldw < width)) return fail("%s: rows overlap", who);
+  if (!aligned({x, w}, 2)) return fail("%s: an operand is not aligned to its elements", who);
+  return 0;
+}
+
+}  // namespace
+
+extern "C" int ad_linear_logprobs_workspace(int device, int dtype, const void* x, int64_t ldx, const void* weight,
+                                            int64_t ldw, int64_t rows, int64_t width, int64_t vocab, int grad,
+                                            size_t* bytes) {
+  const char* who = "ad_linear_logprobs_workspace";
+  if (!bytes) return fail("%s: null operand", who);
+  if (check(who, dtype, x, ldx, weight, ldw, rows, width, vocab)) return 1;
+  *bytes = 0;
+  if (!rows) return 0;
+  DeviceGuard guard(device);
+  if (guard.error() != cudaSuccess) return fail_cuda(who, guard.error());
+  const int sms = sm_count(guard.device());
+  if (!sms) return fail("%s: no device properties", who);
+  *bytes = plan(guard.device(), x, ldx, weight, ldw, rows, width, vocab, grad != 0, sms).total;
+  return 0;
+}
+
+extern "C" int ad_linear_logprobs(int device, int dtype, const void* x, int64_t ldx, const void* weight, int64_t ldw,
+                                  int64_t rows, int64_t width, int64_t vocab, const void* tokens, int tok64, float scale,
+                                  float* logp, float* lse, float* stats, void* workspace, size_t workspace_bytes,
+                                  void* stream) {
+  const char* who = "ad_linear_logprobs";
+  if (check(who, dtype, x, ldx, weight, ldw, rows, width, vocab)) return 1;
+  if (!(scale > 0.0f && scale <= FLT_MAX)) return fail("%s: scale %g", who, scale);
+  if (!rows) return 0;
+  if (!x || !weight || !tokens || !logp || !lse || !stats) return fail("%s: null operand", who);
+  if (!aligned(tokens, tok64 ? 8 : 4) || !aligned({logp, lse}, 4) || !aligned(stats, 8))
+    return fail("%s: an operand is not aligned to its elements", who);
+  DeviceGuard guard(device);
+  if (guard.error() != cudaSuccess) return fail_cuda(who, guard.error());
+  const int sms = sm_count(guard.device());
+  if (!sms) return fail("%s: no device properties", who);
+  const Layout l = plan(guard.device(), x, ldx, weight, ldw, rows, width, vocab, false, sms);
+  if (!workspace || !aligned(workspace, 256) || workspace_bytes < l.total)
+    return fail("%s: needs %zu bytes of workspace, 256-byte aligned", who, l.total);
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  unsigned char* ws = static_cast<unsigned char*>(workspace);
+  Problem p = logits(guard.device(), dtype == AD_F16, rows, width, vocab);
+  p.a[0] = l.pack_x ? Mat{ws + l.x, l.ld_packed} : Mat{x, ldx};
+  p.b[0] = l.pack_w ? Mat{ws + l.w, l.ld_packed} : Mat{weight, ldw};
+  if (l.pack_x && pack_rows(who, x, ldx, rows, width, ws + l.x, l.ld_packed, st)) return 1;
+  if (l.pack_w && pack_rows(who, weight, ldw, vocab, width, ws + l.w, l.ld_packed, st)) return 1;
+  Sum::Params q = {};
+  q.part = reinterpret_cast<float2*>(ws + l.part);
+  q.target = reinterpret_cast<float*>(ws + l.target);
+  q.tokens = tokens, q.tok64 = tok64;
+  q.k = std::min(scale * LOG2E, FLT_MAX);
+  if (start<Sum>(who, p, l.forward, q, sms, st)) return 1;
+  const long long cols = l.forward.tile == 0 ? 256 : l.forward.tile == 1 ? 128 : 64;
+  FinishArgs f = {};
+  f.part = q.part, f.target = q.target, f.tokens = tokens, f.tok64 = tok64;
+  f.parts = static_cast<int>(2 * ((vocab + cols - 1) / cols)), f.rows = static_cast<int>(rows);
+  f.vocab = vocab, f.scale = scale, f.k = q.k;
+  f.logp = logp, f.lse = lse, f.stats = reinterpret_cast<float2*>(stats);
+  const cudaError_t e = launch<finish_kernel>(dim3(static_cast<unsigned>((rows + 31) / 32)), 32 * FINISH_WARPS, 0, st, f);
+  return e == cudaSuccess ? 0 : fail_cuda(who, e);
+}
+
+extern "C" int ad_linear_logprobs_grad(int device, int dtype, const void* x, int64_t ldx, const void* weight, int64_t ldw,
+                                       int64_t rows, int64_t width, int64_t vocab, const void* tokens, int tok64,
+                                       float scale, const float* stats, const float* g_logp, const float* g_lse, void* dx,
+                                       int64_t lddx, int dw_type, void* dw, int64_t lddw, int accumulate, void* workspace,
+                                       size_t workspace_bytes, void* stream) {
+  const char* who = "ad_linear_logprobs_grad";
+  if (check(who, dtype, x, ldx, weight, ldw, rows, width, vocab)) return 1;
+  if (dw_type != dtype && dw_type != AD_F32) return fail("%s: unknown type %d of the weight's gradient", who, dw_type);
+  if (!(scale > 0.0f && scale <= FLT_MAX)) return fail("%s: scale %g", who, scale);
+  if (!dw || !aligned(dw, elem_size(dw_type))) return fail("%s: an operand is null or not aligned to its elements", who);
+  if ((rows > 1 && lddx < width) || (vocab > 1 && lddw < width)) return fail("%s: rows overlap", who);
+  const size_t es = elem_size(dw_type);
+  if (!rows) return accumulate ? 0 : ad_clear_rows(device, dw, lddw * es, width * es, vocab, stream);
+  if (!x || !weight || !tokens || !stats || !dx) return fail("%s: null operand", who);
+  if (!aligned(tokens, tok64 ? 8 : 4) || !aligned({g_logp, g_lse}, 4) || !aligned(stats, 8) || !aligned(dx, 2))
+    return fail("%s: an operand is not aligned to its elements", who);
+  DeviceGuard guard(device);
+  if (guard.error() != cudaSuccess) return fail_cuda(who, guard.error());
+  const int sms = sm_count(guard.device());
+  if (!sms) return fail("%s: no device properties", who);
+  const int dev = guard.device(), half = dtype == AD_F16;
+  const Layout l = plan(dev, x, ldx, weight, ldw, rows, width, vocab, true, sms);
+  if (!workspace || !aligned(workspace, 256) || workspace_bytes < l.total)
+    return fail("%s: needs %zu bytes of workspace, 256-byte aligned", who, l.total);
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  unsigned char* ws = static_cast<unsigned char*>(workspace);
+  const Mat mx = l.pack_x ? Mat{ws + l.x, l.ld_packed} : Mat{x, ldx};
+  const Mat mw = l.pack_w ? Mat{ws + l.w, l.ld_packed} : Mat{weight, ldw};
+  if (l.pack_x && pack_rows(who, x, ldx, rows, width, ws + l.x, l.ld_packed, st)) return 1;
+  if (l.pack_w && pack_rows(who, weight, ldw, vocab, width, ws + l.w, l.ld_packed, st)) return 1;
+  float* factor = half ? reinterpret_cast<float*>(ws + l.factor) : nullptr;
+  if (half) {
+    const RangeArgs r = {g_logp, g_lse, static_cast<int>(rows), scale, factor};
+    const cudaError_t e = launch<range_kernel>(1, 1024, 0, st, r);
+    if (e != cudaSuccess) return fail_cuda(who, e);
+  }
+  const Mat dz = {ws + l.dz, l.piece};
+  for (long long i = 0; i < l.pieces; ++i) {
+    const long long v0 = i * l.piece, n = std::min(l.piece, vocab - v0);
+    const Mat w = {static_cast<const unsigned short*>(mw.p) + v0 * mw.ld, mw.ld};
+    Problem p = logits(dev, half, rows, width, n);
+    p.a[0] = mx, p.b[0] = w;
+    Slope::Params q = {};
+    q.stats = reinterpret_cast<const float2*>(stats);
+    q.tokens = tokens, q.tok64 = tok64;
+    q.g_logp = g_logp, q.g_lse = g_lse, q.factor = factor;
+    q.vocab = vocab, q.first = v0;
+    q.k = std::min(scale * LOG2E, FLT_MAX), q.scale = scale;
+    q.out = reinterpret_cast<unsigned short*>(ws + l.dz), q.ld = l.piece;
+    if (start<Slope>(who, p, l.slope, q, sms, st)) return 1;
+    Problem px = dx_of(dev, half, rows, width, n);
+    px.a[0] = dz, px.b[0] = w;
+    const Out ox = {dx, lddx};
+    const Sums sums = {i == 0, i + 1 == l.pieces};
+    if (store_product(who, px, l.dx, dtype, &ox, false, factor ? factor + 1 : nullptr, reinterpret_cast<float*>(ws + l.sum_dx),
+                      &sums, sms, st))
+      return 1;
+    Problem pw = dw_of(dev, half, rows, width, n);
+    pw.a[0] = dz, pw.b[0] = mx;
+    const Out ow = {static_cast<unsigned char*>(dw) + v0 * lddw * es, lddw};
+    if (store_product(who, pw, l.dw, dw_type, &ow, accumulate != 0, factor ? factor + 1 : nullptr,
+                      reinterpret_cast<float*>(ws + l.sum_dw), nullptr, sms, st))
+      return 1;
+  }
+  return 0;
+}

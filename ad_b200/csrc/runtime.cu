@@ -190,6 +190,21 @@ int tmap_3d_16(const void* base, uint64_t count, uint64_t rows, uint64_t cols, u
   if (r != CUDA_SUCCESS) return cu_fail(r, "cuTensorMapEncodeTiled");
   return 0;
 }
+
+int tmap_2d_16(const void* base, uint64_t rows, uint64_t cols, uint64_t ld, uint32_t box_rows, uint32_t box_cols,
+               void* out128) {
+  if (driver()) return 1;
+  cuuint64_t dims[2] = {cols, rows};
+  cuuint64_t strides[1] = {rows > 1 ? 2 * ld : (2 * cols + 15) / 16 * 16};  // one row has no next one
+  cuuint32_t box[2] = {box_cols, box_rows};
+  cuuint32_t estr[2] = {1, 1};
+  CUresult r = g_drv.tensorMapEncodeTiled(
+      reinterpret_cast<CUtensorMap*>(out128), CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 2, const_cast<void*>(base), dims,
+      strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+      CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS) return cu_fail(r, "cuTensorMapEncodeTiled");
+  return 0;
+}
 }  // namespace ad_b200_internal
 
 // ---------------------------------------------------------------- objects

@@ -725,3 +725,491 @@ def orthogonalize(g, *, steps: int = 5, coefficients=NEWTON_SCHULZ, eps: float =
         dev, dt, g.data_ptr(), count, rows, cols, sb, sr, sc, steps, (rt.c_float * max(1, len(coef)))(*coef), eps, ot,
         out.data_ptr(), so[0] if len(so) == 3 else 0, so[-2], so[-1], workspace.data_ptr(), have, s))
     return out
+
+
+# ------------------------------------------------------------------ products of 16-bit matrices
+
+def _half_type(x, name):
+    c = _float(x, name)
+    if c == F32:
+        raise TypeError(f"{name}: expected bfloat16 or float16 elements, got {x.dtype}")
+    return c
+
+
+def _matrix(x, rows, cols, code, device, name):
+    """Elements from row to row of a [rows, cols] operand."""
+    _typed(x, code, name)
+    _same_shape(x, (rows, cols), name)
+    _on(device, x, name)
+    ld = _rows(x, name)[2]
+    _apart(ld, rows, cols, name)
+    return ld
+
+
+def _weight_grads(out, like, code, device, accumulate, names):
+    """(type code, elements from row to row of each) of weights' gradients given by the caller."""
+    types, lds = set(), []
+    for v, w, name in zip(out, like, names):
+        c = _float(v, name)
+        if c not in (F32, code):
+            raise TypeError(f"{name}: expected float32 elements or the weight's, got {v.dtype}")
+        types.add(c)
+        lds.append(_matrix(v, *w.shape, c, device, name))
+    if len(types) > 1:
+        raise TypeError(f"{', '.join(names)}: gradients of one type are wanted")
+    return types.pop(), lds
+
+
+def _scratch(need, workspace, device, like):
+    """(workspace, its bytes), a new one where none is given."""
+    if workspace is None:
+        return _empty((need,), like, "uint8"), need
+    have = _nbytes(workspace, "workspace")
+    _on(device, workspace, "workspace")
+    return workspace, have
+
+
+class LinearLogprobs(NamedTuple):
+    """Results of ``linear_logprobs``: float32 [rows] twice, float32 [rows, 2] for the gradient."""
+    logp: object
+    lse: object
+    stats: object
+
+
+class LinearLogprobsGrads(NamedTuple):
+    """Gradients of ``linear_logprobs``'s operands."""
+    x: object
+    weight: object
+
+
+def _linear_operands(x, weight, tokens, scale):
+    if not 0 < scale < math.inf:
+        raise ValueError(f"scale: {scale} is not a positive number")
+    try:
+        key = ("linear", _layout(x), _layout(weight), _layout(tokens))
+        found = _checked.get(key)
+    except (AttributeError, TypeError):  # not all of them device arrays: refused below
+        key = found = None
+    return found or _remember(key, _check_linear_operands(x, weight, tokens))
+
+
+def _check_linear_operands(x, weight, tokens):
+    dt = _half_type(x, "x")
+    dev = _device(x, "x")
+    rows, width, ldx = _rows(x, "x")
+    _apart(ldx, rows, width, "x")
+    _typed(weight, dt, "weight")
+    if len(weight.shape) != 2:
+        raise ValueError(f"weight: expected [vocab, width], got {tuple(weight.shape)}")
+    vocab = weight.shape[0]
+    if width < 1 or vocab < 1:
+        raise ValueError(f"weight: an empty vocabulary or width ({tuple(weight.shape)})")
+    ldw = _matrix(weight, vocab, width, dt, dev, "weight")
+    t64 = _integer(tokens, "tokens")
+    _flat(tokens, rows, "tokens")
+    _on(dev, tokens, "tokens")
+    return dev, dt, rows, width, vocab, ldx, ldw, t64
+
+
+def _linear_workspace(dev, dt, x, ldx, weight, ldw, rows, width, vocab, grad):
+    n = rt.c_size_t()
+    rt.check(_entry("ad_linear_logprobs_workspace")(dev, dt, x.data_ptr(), ldx, weight.data_ptr(), ldw, rows, width,
+                                                    vocab, grad, ctypes.byref(n)))
+    return n.value
+
+
+def linear_logprobs_workspace(x, weight, grad: bool = False) -> int:
+    """Bytes of workspace that ``linear_logprobs`` (or its gradient) needs for these operands."""
+    dt = _half_type(x, "x")
+    dev = _device(x, "x")
+    rows, width, ldx = _rows(x, "x")
+    ldw = _matrix(weight, weight.shape[0], width, dt, dev, "weight")
+    return _linear_workspace(dev, dt, x, ldx, weight, ldw, rows, width, weight.shape[0], grad)
+
+
+def linear_logprobs(x, weight, tokens, *, scale: float = 1.0, out=None, workspace=None, stream=None) -> LinearLogprobs:
+    """For each row of ``x`` ([..., width]) the log probability of its entry of ``tokens`` (int64 or int32; 0
+    for a negative one, NaN for one past the vocabulary) under softmax(scale * x weight^T), and the log of the
+    sum of exp(scale * logits), without keeping the logits: what ``token_logprobs`` gives for ``x @ weight.T``
+    ([vocab, width]), at the memory of neither.  Operands are bfloat16 or float16, products are accumulated
+    in 32 bits (tensor cores, which truncate: about 2^-26 of a logit's terms for each 16 of the width).
+    ``out``: a ``LinearLogprobs`` to write; ``workspace``: adjacent elements at a 256-byte boundary,
+    ``linear_logprobs_workspace`` bytes or more."""
+    dev, dt, rows, width, vocab, ldx, ldw, t64 = _linear_operands(x, weight, tokens, scale)
+    s = _stream(dev, stream, x, out is None or workspace is None)
+    if out is None:
+        shape, new, f32 = x.shape[:-1], x.new_empty, _torch.float32
+        r = LinearLogprobs(new(shape, dtype=f32), new(shape, dtype=f32), new((rows, 2), dtype=f32))
+    else:
+        r = LinearLogprobs(*out)
+        for v, n, name in zip(r, (1, 1, 2), LinearLogprobs._fields):
+            _typed(v, F32, "out " + name)
+            _flat(v, rows * n, "out " + name)
+            _on(dev, v, "out " + name)
+    workspace, have = _scratch(_linear_workspace(dev, dt, x, ldx, weight, ldw, rows, width, vocab, 0)
+                               if workspace is None else 0, workspace, dev, x)
+    rt.check(_entry("ad_linear_logprobs")(
+        dev, dt, x.data_ptr(), ldx, weight.data_ptr(), ldw, rows, width, vocab, tokens.data_ptr(), t64, scale,
+        r.logp.data_ptr(), r.lse.data_ptr(), r.stats.data_ptr(), workspace.data_ptr(), have, s))
+    return r
+
+
+def linear_logprobs_grad(x, weight, tokens, stats, g_logp=None, g_lse=None, *, scale: float = 1.0,
+                         accumulate: bool = False, out=None, workspace=None, stream=None) -> LinearLogprobsGrads:
+    """The gradients of ``x`` and ``weight`` from those of ``linear_logprobs``'s ``logp`` and ``lse``
+    (float32, one a row; None: zeros; a negative token has none by its ``logp``), its operands and its
+    ``stats``.  Logits are made again a piece of the vocabulary at a time; their gradients are rounded to
+    the operands' type (float16: held to 2^-38 of the largest) and summed in 32 bits.  ``out``: a
+    ``LinearLogprobsGrads`` to write, the weight's of its type or float32, to which the gradient is added
+    with ``accumulate``; ``workspace``: as for ``linear_logprobs``."""
+    dev, dt, rows, width, vocab, ldx, ldw, t64 = _linear_operands(x, weight, tokens, scale)
+    for v, n, name in ((stats, 2, "stats"), (g_logp, 1, "g_logp"), (g_lse, 1, "g_lse")):
+        if v is not None or n == 2:
+            _typed(v, F32, name)
+            _flat(v, rows * n, name)
+            _on(dev, v, name)
+    if accumulate and out is None:
+        raise ValueError("accumulate: out has to be given")
+    s = _stream(dev, stream, x, out is None or workspace is None)
+    if out is None:
+        g = LinearLogprobsGrads(_empty_rows(x), _empty_rows(weight))
+        lddx = lddw = width
+        wt = dt
+    else:
+        g = LinearLogprobsGrads(*out)
+        _typed(g.x, dt, "out x")
+        _same_shape(g.x, x.shape, "out x")
+        _on(dev, g.x, "out x")
+        lddx = _rows(g.x, "out x")[2]
+        _apart(lddx, rows, width, "out x")
+        wt, (lddw,) = _weight_grads((g.weight,), (weight,), dt, dev, accumulate, ("out weight",))
+    workspace, have = _scratch(_linear_workspace(dev, dt, x, ldx, weight, ldw, rows, width, vocab, 1)
+                               if workspace is None else 0, workspace, dev, x)
+    rt.check(_entry("ad_linear_logprobs_grad")(
+        dev, dt, x.data_ptr(), ldx, weight.data_ptr(), ldw, rows, width, vocab, tokens.data_ptr(), t64, scale,
+        stats.data_ptr(), _ptr(g_logp), _ptr(g_lse), g.x.data_ptr(), lddx, wt, g.weight.data_ptr(), lddw, accumulate,
+        workspace.data_ptr(), have, s))
+    return g
+
+
+# ------------------------------------------------------------------ gated feed-forward blocks
+
+_ACTS = {"silu": 0, "gelu": 1, "gelu_tanh": 2, "relu": 3}
+
+
+class FeedForward(NamedTuple):
+    """Results of ``feed_forward``: y [..., width], and x w_gate^T and x w_up^T [rows, hidden] or None."""
+    y: object
+    gate: object
+    up: object
+
+
+class FeedForwardGrads(NamedTuple):
+    """Gradients of ``feed_forward``'s operands."""
+    x: object
+    w_gate: object
+    w_up: object
+    w_down: object
+
+
+def _ffn_operands(x, w_gate, w_up, w_down, act):
+    if act not in _ACTS:
+        raise ValueError(f"act: {act!r} is not one of {list(_ACTS)}")
+    try:
+        key = ("ffn", _layout(x), _layout(w_gate), _layout(w_up), _layout(w_down))
+        found = _checked.get(key)
+    except (AttributeError, TypeError):  # not all of them device arrays: refused below
+        key = found = None
+    return found or _remember(key, _check_ffn_operands(x, w_gate, w_up, w_down))
+
+
+def _check_ffn_operands(x, w_gate, w_up, w_down):
+    dt = _half_type(x, "x")
+    dev = _device(x, "x")
+    rows, width, ldx = _rows(x, "x")
+    _apart(ldx, rows, width, "x")
+    _typed(w_gate, dt, "w_gate")
+    if len(w_gate.shape) != 2:
+        raise ValueError(f"w_gate: expected [hidden, width], got {tuple(w_gate.shape)}")
+    hidden = w_gate.shape[0]
+    if width < 1 or hidden < 1:
+        raise ValueError(f"w_gate: an empty width or hidden size ({tuple(w_gate.shape)})")
+    return (dev, dt, rows, width, hidden, ldx, _matrix(w_gate, hidden, width, dt, dev, "w_gate"),
+            _matrix(w_up, hidden, width, dt, dev, "w_up"), _matrix(w_down, width, hidden, dt, dev, "w_down"))
+
+
+def _ffn_workspace(dev, dt, operands, dy, lddy, rows, width, hidden, grad):
+    n = rt.c_size_t()
+    rt.check(_entry("ad_feed_forward_workspace")(dev, dt, *operands, dy, lddy, rows, width, hidden, grad,
+                                                 ctypes.byref(n)))
+    return n.value
+
+
+def feed_forward_workspace(x, w_gate, w_up, w_down, dy=None) -> int:
+    """Bytes of workspace that ``feed_forward`` (with ``dy``: its gradient) needs for these operands."""
+    dev, dt, rows, width, hidden, ldx, ldg, ldu, ldd = _ffn_operands(x, w_gate, w_up, w_down, "silu")
+    operands = (x.data_ptr(), ldx, w_gate.data_ptr(), ldg, w_up.data_ptr(), ldu, w_down.data_ptr(), ldd)
+    return _ffn_workspace(dev, dt, operands, _ptr(dy), 0 if dy is None else _rows(dy, "dy")[2], rows, width, hidden,
+                          dy is not None)
+
+
+def feed_forward(x, w_gate, w_up, w_down, *, act: str = "silu", keep: bool = False, out=None, workspace=None,
+                 stream=None) -> FeedForward:
+    """A gated feed-forward block over rows of ``x`` ([..., width]; ``w_gate`` and ``w_up``: [hidden, width],
+    ``w_down``: [width, hidden])::
+
+        h = act(x w_gate^T) * (x w_up^T)
+        y = h w_down^T
+
+    ``act``: "silu", "gelu", "gelu_tanh" or "relu".  Operands are bfloat16 or float16; products are accumulated
+    in 32 bits, the activation is taken of them, and ``h`` is rounded to the operands' type.  ``keep`` keeps
+    both products before the activation for ``feed_forward_grad``.  ``out``: a ``FeedForward`` to write;
+    ``workspace``: adjacent elements at a 256-byte boundary, ``feed_forward_workspace`` bytes or more."""
+    dev, dt, rows, width, hidden, ldx, ldwg, ldwu, ldwd = _ffn_operands(x, w_gate, w_up, w_down, act)
+    s = _stream(dev, stream, x, out is None or workspace is None)
+    ldg = ldu = 0
+    if out is None:
+        gate = up = None
+        if keep:  # rows that start on 16-byte boundaries, whatever the hidden size is
+            ldg = ldu = (hidden + 7) // 8 * 8
+            gate, up = (_empty((rows, ldg), x)[:, :hidden] for _ in range(2))
+        r = FeedForward(_empty_rows(x), gate, up)
+        ldy = width
+    else:
+        r = FeedForward(*out)
+        _typed(r.y, dt, "out y")
+        _same_shape(r.y, x.shape, "out y")
+        _on(dev, r.y, "out y")
+        ldy = _rows(r.y, "out y")[2]
+        _apart(ldy, rows, width, "out y")
+        if (r.gate is None) != (not keep) or (r.up is None) != (not keep):
+            raise ValueError("out: gate and up go with keep")
+        if keep:
+            ldg = _matrix(r.gate, rows, hidden, dt, dev, "out gate")
+            ldu = _matrix(r.up, rows, hidden, dt, dev, "out up")
+    operands = (x.data_ptr(), ldx, w_gate.data_ptr(), ldwg, w_up.data_ptr(), ldwu, w_down.data_ptr(), ldwd)
+    workspace, have = _scratch(_ffn_workspace(dev, dt, operands, None, 0, rows, width, hidden, 0)
+                               if workspace is None else 0, workspace, dev, x)
+    rt.check(_entry("ad_feed_forward")(
+        dev, dt, _ACTS[act], *operands, rows, width, hidden, r.y.data_ptr(), ldy, _ptr(r.gate), ldg, _ptr(r.up), ldu,
+        workspace.data_ptr(), have, s))
+    return r
+
+
+def feed_forward_grad(dy, x, w_gate, w_up, w_down, gate, up, *, act: str = "silu", accumulate: bool = False, out=None,
+                      workspace=None, stream=None) -> FeedForwardGrads:
+    """The gradients of ``feed_forward``'s operands from that of ``y``, its operands and the ``gate`` and
+    ``up`` that it kept.  What lies between the products is rounded to the operands' type, sums are held in
+    32 bits.  ``out``: a ``FeedForwardGrads`` to write, the weights' all of the operands' type or all float32, to
+    which the gradients are added with ``accumulate``; ``workspace``: as for ``feed_forward``, with ``dy``."""
+    dev, dt, rows, width, hidden, ldx, ldwg, ldwu, ldwd = _ffn_operands(x, w_gate, w_up, w_down, act)
+    _typed(dy, dt, "dy")
+    _same_shape(dy, x.shape, "dy")
+    _on(dev, dy, "dy")
+    lddy = _rows(dy, "dy")[2]
+    _apart(lddy, rows, width, "dy")
+    ldg = _matrix(gate, rows, hidden, dt, dev, "gate")
+    ldu = _matrix(up, rows, hidden, dt, dev, "up")
+    if accumulate and out is None:
+        raise ValueError("accumulate: out has to be given")
+    s = _stream(dev, stream, x, out is None or workspace is None)
+    if out is None:
+        g = FeedForwardGrads(_empty_rows(x), *(_empty_rows(w) for w in (w_gate, w_up, w_down)))
+        lddx, wt, lds = width, dt, (width, width, hidden)
+    else:
+        g = FeedForwardGrads(*out)
+        _typed(g.x, dt, "out x")
+        _same_shape(g.x, x.shape, "out x")
+        _on(dev, g.x, "out x")
+        lddx = _rows(g.x, "out x")[2]
+        _apart(lddx, rows, width, "out x")
+        wt, lds = _weight_grads(g[1:], (w_gate, w_up, w_down), dt, dev, accumulate,
+                                tuple("out " + n for n in FeedForwardGrads._fields[1:]))
+    operands = (x.data_ptr(), ldx, w_gate.data_ptr(), ldwg, w_up.data_ptr(), ldwu, w_down.data_ptr(), ldwd)
+    workspace, have = _scratch(_ffn_workspace(dev, dt, operands, dy.data_ptr(), lddy, rows, width, hidden, 1)
+                               if workspace is None else 0, workspace, dev, x)
+    rt.check(_entry("ad_feed_forward_grad")(
+        dev, dt, _ACTS[act], dy.data_ptr(), lddy, *operands, gate.data_ptr(), ldg, up.data_ptr(), ldu, rows, width,
+        hidden, g.x.data_ptr(), lddx, wt, g.w_gate.data_ptr(), lds[0], g.w_up.data_ptr(), lds[1], g.w_down.data_ptr(),
+        lds[2], accumulate, workspace.data_ptr(), have, s))
+    return g
+
+
+# ------------------------------------------------------------------ embeddings
+
+def _embed_operands(tokens, table):
+    try:
+        key = ("embed", _layout(tokens), _layout(table))
+        found = _checked.get(key)
+    except (AttributeError, TypeError):  # not both of them device arrays: refused below
+        key = found = None
+    return found or _remember(key, _check_embed_operands(tokens, table))
+
+
+def _check_embed_operands(tokens, table):
+    dt = _float(table, "table")
+    dev = _device(table, "table")
+    if len(table.shape) != 2 or table.shape[0] < 1:
+        raise ValueError(f"table: expected [vocab, width] with a token or more, got {tuple(table.shape)}")
+    vocab, width, ldt = _rows(table, "table")
+    t64 = _integer(tokens, "tokens")
+    rows = math.prod(tokens.shape)
+    _flat(tokens, rows, "tokens")
+    _on(dev, tokens, "tokens")
+    return dev, dt, rows, vocab, width, ldt, t64
+
+
+def _finite(scale):
+    if not -math.inf < scale < math.inf:
+        raise ValueError(f"scale: {scale} is not a finite number")
+
+
+def embed(tokens, table, *, scale: float = 1.0, out=None, stream=None):
+    """``scale`` times the row of ``table`` ([vocab, width]) of each of ``tokens`` (int64 or int32, any
+    shape), [..., width] of the table's type: zeros for a negative token (padding), NaNs for one past the
+    vocabulary.  ``out``: the array to write."""
+    dev, dt, rows, vocab, width, ldt, t64 = _embed_operands(tokens, table)
+    _finite(scale)
+    s = _stream(dev, stream, table, out is None)
+    shape = (*tokens.shape, width)
+    if out is None:
+        out = _empty(shape, table)
+        ldo = width
+    else:
+        _typed(out, dt, "out")
+        _same_shape(out, shape, "out")
+        _on(dev, out, "out")
+        ldo = _rows(out, "out")[2]
+        _apart(ldo, rows, width, "out")
+    rt.check(_entry("ad_embed")(dev, dt, tokens.data_ptr(), t64, rows, table.data_ptr(), ldt, vocab, width, scale,
+                                out.data_ptr(), ldo, s))
+    return out
+
+
+def embed_grad_workspace(rows: int, vocab: int, width: int) -> int:
+    """Bytes of workspace that ``embed_grad`` needs."""
+    n = rt.c_size_t()
+    rt.check(_entry("ad_embed_grad_workspace")(rows, vocab, width, ctypes.byref(n)), "ad_embed_grad_workspace")
+    return n.value
+
+
+def embed_grad(dy, tokens, vocab: int, *, scale: float = 1.0, accumulate: bool = False, out=None, workspace=None,
+               stream=None):
+    """The gradient of ``embed``'s table, [vocab, width], from that of its result: ``scale`` times the sum of
+    the rows of ``dy`` ([..., width]) of each token, held in 32 bits in an order that the tokens alone set.
+    Tokens outside of the vocabulary have no part in it.  ``out``: the array to write, of ``dy``'s type or
+    float32; with ``accumulate`` the sums are added to it and rows of other tokens are left alone (a table that is
+    the output layer's too has two gradients).  ``workspace``: adjacent elements at a 256-byte boundary,
+    ``embed_grad_workspace`` bytes or more."""
+    dt = _float(dy, "dy")
+    dev = _device(dy, "dy")
+    rows, width, lddy = _rows(dy, "dy")
+    t64 = _integer(tokens, "tokens")
+    _same_shape(tokens, dy.shape[:-1], "tokens")
+    _flat(tokens, rows, "tokens")
+    _on(dev, tokens, "tokens")
+    _finite(scale)
+    if vocab < 1:
+        raise ValueError(f"vocab: {vocab} tokens")
+    if accumulate and out is None:
+        raise ValueError("accumulate: out has to be given")
+    s = _stream(dev, stream, dy, out is None or workspace is None)
+    if out is None:
+        out = _empty((vocab, width), dy)
+        ot, ldo = dt, width
+    else:
+        ot = _float(out, "out")
+        if ot not in (dt, F32):
+            raise TypeError(f"out: expected float32 elements or dy's, got {out.dtype}")
+        ldo = _matrix(out, vocab, width, ot, dev, "out")
+    workspace, have = _scratch(embed_grad_workspace(rows, vocab, width) if workspace is None else 0, workspace, dev, dy)
+    rt.check(_entry("ad_embed_grad")(
+        dev, dt, dy.data_ptr(), lddy, tokens.data_ptr(), t64, rows, vocab, width, scale, ot, out.data_ptr(), ldo,
+        accumulate, workspace.data_ptr(), have, s))
+    return out
+
+
+# ------------------------------------------------------------------ clipping
+
+def clip_norm_workspace(count: int) -> int:
+    """Bytes of workspace that ``clip_norm`` needs for ``count`` arrays."""
+    n = rt.c_size_t()
+    rt.check(_entry("ad_clip_norm_workspace")(count, ctypes.byref(n)), "ad_clip_norm_workspace")
+    return n.value
+
+
+def _dense(x, name):
+    """Elements of an array that fills its memory, its axes in any order."""
+    n = 1
+    for st, size in sorted((st, size) for st, size in zip(x.stride(), x.shape) if size != 1):
+        if size and st != n:
+            raise ValueError(f"{name}: elements have to be adjacent (shape {tuple(x.shape)}, strides {tuple(x.stride())})")
+        n *= size
+    return n
+
+
+def _clip_operands(arrays, name, device):
+    """(type codes, element counts) of arrays on a device."""
+    found = []
+    for i, x in enumerate(arrays):
+        try:
+            key = _layout(x)
+            f = _checked.get(key)
+        except (AttributeError, TypeError):  # not a device array: refused below
+            key = f = None
+        if f is None:
+            label = f"{name}[{i}]"
+            code = _float(x, label)
+            _device(x, label)
+            n = 0 if 0 in x.shape else _dense(x, label)
+            f = _remember(key, (code, n, x.get_device()))
+        if f[2] != device:
+            raise ValueError(f"{name}[{i}]: on device {f[2]}, not on device {device}")
+        found.append(f)
+    return [f[0] for f in found], [f[1] for f in found]
+
+
+def clip_norm(grads, max_norm: float, *, out=None, norm=None, workspace=None, stream=None):
+    """Scales the arrays of ``grads`` (a list; of any types, shapes and order of axes, their elements adjacent)
+    by ``max_norm`` over the norm of all their elements together, where that norm is larger, and returns the norm
+    as it was, float32 [1].  ``max_norm`` of infinity gives the norm alone.  A norm that is infinite or NaN
+    leaves the arrays as they are: what to do then is the caller's.  Sums are held in 64 bits.  The arrays themselves are
+    written, or those of ``out``, of the same types, shapes and strides; none of them may overlap another one.
+    ``norm``: the array for the result; ``workspace``: adjacent elements at a 256-byte boundary,
+    ``clip_norm_workspace`` bytes or more."""
+    grads = list(grads)
+    if not grads:
+        raise ValueError("grads: no arrays")
+    if not max_norm >= 0:
+        raise ValueError(f"max_norm: {max_norm}")
+    if not hasattr(grads[0], "get_device"):
+        _float(grads[0], "grads[0]")
+    dev = _device(grads[0], "grads[0]")
+    types, counts = _clip_operands(grads, "grads", dev)
+    to = grads
+    if out is not None:
+        to = list(out)
+        if len(to) != len(grads):
+            raise ValueError(f"out: {len(to)} arrays for {len(grads)}")
+        for i, (x, y) in enumerate(zip(grads, to)):
+            if not hasattr(y, "data_ptr"):
+                _float(y, f"out[{i}]")
+            if x.shape != y.shape or x.stride() != y.stride() or x.dtype != y.dtype:
+                raise ValueError(f"out[{i}]: {y.dtype} of shape {tuple(y.shape)} and strides {tuple(y.stride())}, expected "
+                                 f"{x.dtype}, {tuple(x.shape)}, {tuple(x.stride())}")
+            _on(dev, y, f"out[{i}]")
+    s = _stream(dev, stream, grads[0], norm is None or workspace is None)
+    if norm is None:
+        norm = grads[0].new_empty((1,), dtype=_torch.float32)
+    else:
+        _typed(norm, F32, "norm")
+        _flat(norm, 1, "norm")
+        _on(dev, norm, "norm")
+    n = len(grads)
+    workspace, have = _scratch(clip_norm_workspace(n) if workspace is None else 0, workspace, dev, grads[0])
+    pointers, longs = ctypes.c_void_p * n, ctypes.c_int64 * n
+    at = pointers(*[x.data_ptr() for x in grads])
+    rt.check(_entry("ad_clip_norm")(dev, n, at, at if out is None else pointers(*[y.data_ptr() for y in to]),
+                                    longs(*counts), (ctypes.c_int * n)(*types), max_norm, norm.data_ptr(),
+                                    workspace.data_ptr(), have, s))
+    return norm

@@ -96,6 +96,31 @@ SIGNATURES = {
     "ad_orthogonalize_workspace": (c_int, [c_i64, c_i64, c_i64, ctypes.POINTER(c_size_t)]),
     "ad_orthogonalize": (c_int, [c_int, c_int, c_void_p, c_i64, c_i64, c_i64, c_i64, c_i64, c_i64, c_int, c_void_p,
                                  c_float, c_int, c_void_p, c_i64, c_i64, c_i64, c_void_p, c_size_t, c_void_p]),
+    "ad_linear_logprobs_workspace": (c_int, [c_int, c_int, c_void_p, c_i64, c_void_p, c_i64, c_i64, c_i64, c_i64,
+                                             c_int, ctypes.POINTER(c_size_t)]),
+    "ad_linear_logprobs": (c_int, [c_int, c_int, c_void_p, c_i64, c_void_p, c_i64, c_i64, c_i64, c_i64, c_void_p,
+                                   c_int, c_float, c_void_p, c_void_p, c_void_p, c_void_p, c_size_t, c_void_p]),
+    "ad_linear_logprobs_grad": (c_int, [c_int, c_int, c_void_p, c_i64, c_void_p, c_i64, c_i64, c_i64, c_i64,
+                                        c_void_p, c_int, c_float, c_void_p, c_void_p, c_void_p, c_void_p, c_i64,
+                                        c_int, c_void_p, c_i64, c_int, c_void_p, c_size_t, c_void_p]),
+    "ad_feed_forward_workspace": (c_int, [c_int, c_int, c_void_p, c_i64, c_void_p, c_i64, c_void_p, c_i64, c_void_p,
+                                          c_i64, c_void_p, c_i64, c_i64, c_i64, c_i64, c_int,
+                                          ctypes.POINTER(c_size_t)]),
+    "ad_feed_forward": (c_int, [c_int, c_int, c_int, c_void_p, c_i64, c_void_p, c_i64, c_void_p, c_i64, c_void_p,
+                                c_i64, c_i64, c_i64, c_i64, c_void_p, c_i64, c_void_p, c_i64, c_void_p, c_i64,
+                                c_void_p, c_size_t, c_void_p]),
+    "ad_feed_forward_grad": (c_int, [c_int, c_int, c_int, c_void_p, c_i64, c_void_p, c_i64, c_void_p, c_i64,
+                                     c_void_p, c_i64, c_void_p, c_i64, c_void_p, c_i64, c_void_p, c_i64, c_i64,
+                                     c_i64, c_i64, c_void_p, c_i64, c_int, c_void_p, c_i64, c_void_p, c_i64,
+                                     c_void_p, c_i64, c_int, c_void_p, c_size_t, c_void_p]),
+    "ad_embed": (c_int, [c_int, c_int, c_void_p, c_int, c_i64, c_void_p, c_i64, c_i64, c_i64, c_float, c_void_p, c_i64,
+                         c_void_p]),
+    "ad_embed_grad_workspace": (c_int, [c_i64, c_i64, c_i64, ctypes.POINTER(c_size_t)]),
+    "ad_embed_grad": (c_int, [c_int, c_int, c_void_p, c_i64, c_void_p, c_int, c_i64, c_i64, c_i64, c_float, c_int,
+                              c_void_p, c_i64, c_int, c_void_p, c_size_t, c_void_p]),
+    "ad_clip_norm_workspace": (c_int, [c_i64, ctypes.POINTER(c_size_t)]),
+    "ad_clip_norm": (c_int, [c_int, c_i64, c_void_p, c_void_p, c_void_p, c_void_p, ctypes.c_double, c_void_p, c_void_p,
+                             c_size_t, c_void_p]),
 }
 
 

@@ -262,6 +262,83 @@ int ad_orthogonalize(int device, int dtype, const void* g, int64_t count, int64_
                      int64_t out_batch_stride, int64_t out_row_stride, int64_t out_col_stride,
                      void* workspace, size_t workspace_bytes, void* stream);
 
+/* Log probabilities of given tokens under softmax(scale x W^T), x of rows x
+ * width, W of vocab x width, without the logits in memory.  dtype is AD_BF16 or
+ * AD_F16; products are accumulated in 32 bits.  logp: 0 for a negative token, NaN
+ * for one past the vocabulary.  lse: the log of the sum of exp(scale logits).
+ * stats: rows * 2 floats (8-byte aligned) for the gradient: the largest logit
+ * and the sum of exp(scale (logit - largest)).  Tokens are of 64 bits when tok64,
+ * else of 32.  The workspace is 256-byte aligned; how much a call needs depends
+ * on its operands' sizes and on whether their rows are aligned to 16 bytes. */
+int ad_linear_logprobs_workspace(int device, int dtype, const void* x, int64_t ldx, const void* weight,
+                                 int64_t ldw, int64_t rows, int64_t width, int64_t vocab, int grad,
+                                 size_t* bytes);
+int ad_linear_logprobs(int device, int dtype, const void* x, int64_t ldx, const void* weight,
+                       int64_t ldw, int64_t rows, int64_t width, int64_t vocab, const void* tokens,
+                       int tok64, float scale, float* logp, float* lse, float* stats, void* workspace,
+                       size_t workspace_bytes, void* stream);
+/* The gradients of x (of dtype) and W (of dw_type: dtype or AD_F32) from those of
+ * logp and lse (rows floats each; NULL: zeros); W's is added to what dw holds when
+ * `accumulate`.  Logits are made again a piece of the vocabulary at a time, and
+ * their gradients rounded to dtype as operands (AD_F16: times a power of two that
+ * puts the largest at 2^14; they are held to 2^-38 of it). */
+int ad_linear_logprobs_grad(int device, int dtype, const void* x, int64_t ldx, const void* weight,
+                            int64_t ldw, int64_t rows, int64_t width, int64_t vocab,
+                            const void* tokens, int tok64, float scale, const float* stats,
+                            const float* g_logp, const float* g_lse, void* dx, int64_t lddx,
+                            int dw_type, void* dw, int64_t lddw, int accumulate, void* workspace,
+                            size_t workspace_bytes, void* stream);
+
+/* A gated feed-forward block: g = x Wg^T, u = x Wu^T, h = act(g) u, y = h Wd^T;
+ * x and y of rows x width, Wg and Wu of hidden x width, Wd of width x hidden, all
+ * of dtype (AD_BF16 or AD_F16).  act: 0 silu, 1 gelu, 2 gelu by tanh, 3 relu.
+ * Products are accumulated in 32 bits; h is rounded to dtype.  gate and up, of
+ * rows x hidden: g and u for the gradient, or both NULL. */
+int ad_feed_forward_workspace(int device, int dtype, const void* x, int64_t ldx, const void* w_gate,
+                              int64_t ld_gate, const void* w_up, int64_t ld_up, const void* w_down,
+                              int64_t ld_down, const void* dy, int64_t lddy, int64_t rows,
+                              int64_t width, int64_t hidden, int grad, size_t* bytes);
+int ad_feed_forward(int device, int dtype, int act, const void* x, int64_t ldx, const void* w_gate,
+                    int64_t ld_gate, const void* w_up, int64_t ld_up, const void* w_down,
+                    int64_t ld_down, int64_t rows, int64_t width, int64_t hidden, void* y, int64_t ldy,
+                    void* gate, int64_t ldg, void* up, int64_t ldu, void* workspace,
+                    size_t workspace_bytes, void* stream);
+/* The gradients of x (of dtype) and the weights (of dw_type: dtype or AD_F32; added
+ * to what is there when `accumulate`; with no rows zeros or left alone). */
+int ad_feed_forward_grad(int device, int dtype, int act, const void* dy, int64_t lddy, const void* x,
+                         int64_t ldx, const void* w_gate, int64_t ld_gate, const void* w_up,
+                         int64_t ld_up, const void* w_down, int64_t ld_down, const void* gate,
+                         int64_t ldg, const void* up, int64_t ldu, int64_t rows, int64_t width,
+                         int64_t hidden, void* dx, int64_t lddx, int dw_type, void* dw_gate,
+                         int64_t lddw_gate, void* dw_up, int64_t lddw_up, void* dw_down,
+                         int64_t lddw_down, int accumulate, void* workspace, size_t workspace_bytes,
+                         void* stream);
+
+/* y[r] = scale table[tokens[r]], rows x width; zeros for a negative token, NaNs
+ * for one past the vocabulary.  Tokens are of 64 bits when tok64, else of 32. */
+int ad_embed(int device, int dtype, const void* tokens, int tok64, int64_t rows, const void* table,
+             int64_t ldt, int64_t vocab, int64_t width, float scale, void* y, int64_t ldy, void* stream);
+/* The table's gradient, vocab x width of out_type (dtype or AD_F32): scale times
+ * the sum of the rows of dy of each token, in the order of their positions;
+ * tokens outside of the vocabulary have no part in it.  Added to what is there
+ * when `accumulate` (other rows are left alone), else rows without a token are
+ * zeros.  The workspace is 256-byte aligned. */
+int ad_embed_grad_workspace(int64_t rows, int64_t vocab, int64_t width, size_t* bytes);
+int ad_embed_grad(int device, int dtype, const void* dy, int64_t lddy, const void* tokens, int tok64,
+                  int64_t rows, int64_t vocab, int64_t width, float scale, int out_type, void* out,
+                  int64_t ldo, int accumulate, void* workspace, size_t workspace_bytes, void* stream);
+
+/* *norm (device memory): the square root of the sum of squares over `count` arrays
+ * of adjacent elements, in[i] of counts[i] elements of dtypes[i] (lists in host
+ * memory); out[i] = in[i] min(1, max_norm / norm), where out[i] may be in[i].
+ * A norm that is infinite or no number leaves the arrays as they are (copied to
+ * out[i]).  Sums are held in 64 bits.  Arrays that are written may overlap nothing else:
+ * an array that is given twice is refused.  The workspace is 256-byte aligned. */
+int ad_clip_norm_workspace(int64_t count, size_t* bytes);
+int ad_clip_norm(int device, int64_t count, const void* const* in, void* const* out,
+                 const int64_t* counts, const int* dtypes, double max_norm, float* norm, void* workspace,
+                 size_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

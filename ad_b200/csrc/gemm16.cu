@@ -23,14 +23,14 @@ struct Store {
     unsigned char* out;
     long long ld;
     float alpha;
-    __device__ State(const Params& p, const Shape&, const Spot& s, int, int, int) {
+    __device__ State(const Params& p, const Shape&, const Spot& s) {
       const int g = p.split_stride ? 0 : s.group;
       ld = p.ld[g];
       out = static_cast<unsigned char*>(p.out[g]) +
             (p.split_stride ? 4 * (s.split * p.split_stride + s.group * p.group_stride) : 0);
       alpha = p.alpha ? *p.alpha : 1.0f;
     }
-    __device__ void end(const Params&, const Shape&, const Spot&, int) {}
+    __device__ void end(const Params&, const Shape&, const Spot&) {}
     __device__ void chunk(const Params& p, const Shape& a, const Spot& s, int col0, unsigned acc, int) {
       float v[32];
       tmem_ld32(acc, v);
@@ -74,11 +74,7 @@ struct Store {
       const int col = col0 + s.lane;
       if (col >= a.n) return;
       for (int r = 0; r < 32 && s.row0 + r < a.m; ++r) {
-        float x;
-        asm volatile("ld.shared.f32 %0, [%1];"
-                     : "=f"(x)
-                     : "r"(s.side + r * 128 + (((s.lane >> 2) ^ (r & 7)) << 4) + (s.lane & 3) * 4)
-                     : "memory");
+        float x = staged1(s, r);
         const long long at = (s.row0 + r) * ld + col;
         if (p.accumulate) x += load_any(out, p.type, at);
         store_any(out, p.type, at, x);

@@ -12,7 +12,7 @@
 // x 256, so that 32 KB a block serve 4.2 MFLOP; single blocks on 128 x 128 or 128 x
 // 64 are for products with too few large tiles.  Blocks stay resident and take
 // every so-many-th tile; in a block one warp brings operands by TMA, one issues
-// the products into one of two accumulators, eight work on the other, so that a
+// the products into one of two accumulators, sixteen work on the other, so that a
 // tile's epilogue is hidden behind the next tile's products.  Tiles are walked in
 // bands of rows, so that the tiles under way at a time share operands in L2.
 // Few tiles with a long K are split over K: partial sums go to memory in 32 bits
@@ -39,7 +39,7 @@ using namespace adops;
 
 constexpr int BK = 64;            // elements of K a stage: 128 bytes, the swizzle's width
 constexpr int BOX = 64 * BK * 2;  // bytes of a box of 64 x 64
-constexpr int EPI_WARPS = 8;
+constexpr int EPI_WARPS = 16, PARTS = EPI_WARPS / 4;  // warps that share 32 rows, each with every fourth chunk
 constexpr int THREADS = 32 * (2 + EPI_WARPS);
 constexpr int CHUNK = 32;                  // columns that an epilogue takes at a time
 constexpr int SIDE = 32 * CHUNK * 4;       // bytes of shared memory of an epilogue warp: 32 rows of them
@@ -194,7 +194,8 @@ __device__ __forceinline__ float2 unpack2(unsigned w, int half) {
 // What a warp's epilogue knows of its tile: 32 rows from row0 on, of which the
 // thread's accumulator row is row0 + lane, and where it may keep 4 KB.
 struct Spot {
-  int lane, row0, unit_col, group, split;
+  int lane, quad, part, row0, unit_col, group, split;
+  int odd;        // every other tile of the block
   unsigned side;
   bool dead;  // a wait ran out: results are NaNs
 };
@@ -248,11 +249,40 @@ __device__ __forceinline__ float4 staged(const Spot& s, int r, int p) {
   return make_float4(__uint_as_float(x.x), __uint_as_float(x.y), __uint_as_float(x.z), __uint_as_float(x.w));
 }
 
+// The lane's column of row r of them.
+__device__ __forceinline__ float staged1(const Spot& s, int r) {
+  float x;
+  asm volatile("ld.shared.f32 %0, [%1];"
+               : "=f"(x)
+               : "r"(s.side + r * 128 + (((s.lane >> 2) ^ (r & 7)) << 4) + (s.lane & 3) * 4)
+               : "memory");
+  return x;
+}
+
+// A warp's 32 x 32 values in 32 bits to memory.
+__device__ __forceinline__ void put32(const Spot& s, const float (&v)[32], float* out, long long ld, int m, int n, int col0,
+                                      int vec) {
+  stage32(s, v);
+  if (vec && col0 + CHUNK <= n) {
+    const int q = s.lane & 7;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const int r = i * 4 + (s.lane >> 3);
+      const float4 x = staged(s, r, q);
+      if (s.row0 + r < m) *reinterpret_cast<float4*>(out + (s.row0 + r) * ld + col0 + q * 4) = x;
+    }
+  } else {  // a column a lane
+    const int col = col0 + s.lane;
+    if (col < n)
+      for (int r = 0; r < 32 && s.row0 + r < m; ++r) out[(s.row0 + r) * ld + col] = staged1(s, r);
+  }
+}
+
 // ------------------------------------------------------------------ the kernel
 
 // EPI: static constexpr bool DUAL (B's tiles hold half their columns of each of
 // two operands); Params; a State that is constructed for a tile (loads that need
-// no accumulator) and whose chunk(ch, acc) takes 32 columns.
+// no accumulator), whose chunk() takes 32 columns, and whose end() all warps call.
 template <typename TILE, typename EPI>
 __global__ void __launch_bounds__(THREADS, 1)
     gemm_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Shape a,
@@ -435,9 +465,9 @@ __global__ void __launch_bounds__(THREADS, 1)
       }
     }
   } else {  // epilogues
-    const int quad = warp & 3, part = (warp - 2) >> 2;  // 32 rows; every other chunk
+    const int quad = warp & 3, part = (warp - 2) >> 2;  // 32 rows; which of their chunks
     Spot s;
-    s.lane = lane;
+    s.lane = lane, s.quad = quad, s.part = part;
     s.side = smem_u32(side) + (warp - 2) * SIDE;
     s.dead = false;
     int c = 0;
@@ -446,7 +476,7 @@ __global__ void __launch_bounds__(THREADS, 1)
       s.row0 = t.row * TILE::M + rank * 128 + quad * 32;
       s.unit_col = t.col, s.group = t.group, s.split = t.split;
       const int chunks = (min(COLS, a.n - t.col * COLS) + CHUNK - 1) / CHUNK;
-      typename EPI::State e(params, a, s, t.col * COLS, part, chunks);
+      typename EPI::State e(params, a, s);
       if (!s.dead && !bar_wait(&acc_full[c & 1], (c / 2) & 1, gave_up)) {
         s.dead = true;
         *gave_up = 1;
@@ -455,14 +485,15 @@ __global__ void __launch_bounds__(THREADS, 1)
       const unsigned acc = tmem + (static_cast<unsigned>(quad * 32) << 16) + (c & 1) * BN;
       // a warp without a row of the result still has to say that it is done
       if (s.row0 < a.m)
-        for (int ch = part; ch < chunks; ch += 2) e.chunk(params, a, s, t.col * COLS + ch * CHUNK, acc + ch * CHUNK, COLS);
+        for (int ch = part; ch < chunks; ch += PARTS) e.chunk(params, a, s, t.col * COLS + ch * CHUNK, acc + ch * CHUNK, COLS);
       asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
       __syncwarp();
       if (lane == 0 && !s.dead) {  // the accumulator is free
         const unsigned bar = CTAS == 1 ? smem_u32(&acc_empty[c & 1]) : in_block(smem_u32(&acc_empty[c & 1]), 0);
         asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
       }
-      if (s.row0 < a.m) e.end(params, a, s, part);
+      s.odd = c & 1;
+      e.end(params, a, s);
     }
   }
   __syncwarp();

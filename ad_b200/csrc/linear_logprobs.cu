@@ -40,7 +40,7 @@ __device__ __forceinline__ long long token_at(const void* tokens, int tok64, lon
 struct Sum {
   static constexpr bool DUAL = false;
   struct Params {
-    float2* part;   // [2 x column tiles][rows]
+    float2* part;   // [column tiles][rows]
     float* target;  // [rows]
     const void* tokens;
     int tok64;
@@ -49,7 +49,7 @@ struct Sum {
   struct State {
     float top, sum;
     int token;  // -1: not in reach
-    __device__ State(const Params& p, const Shape& a, const Spot& s, int, int, int) {
+    __device__ State(const Params& p, const Shape& a, const Spot& s) {
       top = -INFINITY, sum = 0.0f, token = -1;
       const int row = s.row0 + s.lane;
       if (row < a.m) {
@@ -85,10 +85,24 @@ struct Sum {
       sum = sum * ex2((top - from) * p.k) + ((part[0] + part[1]) + (part[2] + part[3]));
       top = most;
     }
-    __device__ void end(const Params& p, const Shape& a, const Spot& s, int part) {
+    // The four warps of 32 rows join their pairs.  A warp's place for them is
+    // used again two tiles later, when all have met once more.
+    __device__ void end(const Params& p, const Shape& a, const Spot& s) {
       const int row = s.row0 + s.lane;
       if (s.dead) sum = __int_as_float(0x7fffffff);
-      if (row < a.m) p.part[(2ll * s.unit_col + part) * a.m + row] = make_float2(top, sum);
+      const unsigned at = s.side + s.odd * 256 + s.lane * 8;
+      if (s.part) asm volatile("st.shared.v2.f32 [%0], {%1, %2};" ::"r"(at), "f"(top), "f"(sum) : "memory");
+      asm volatile("bar.sync %0, %1;" ::"r"(1 + s.quad), "r"(32 * PARTS) : "memory");
+      if (s.part) return;
+#pragma unroll
+      for (int i = 1; i < PARTS; ++i) {
+        float t, u;
+        asm volatile("ld.shared.v2.f32 {%0, %1}, [%2];" : "=f"(t), "=f"(u) : "r"(at + i * 4 * SIDE) : "memory");
+        const float most = fmaxf(top, t), from = most == -INFINITY ? 0.0f : most;
+        sum = sum * ex2((top - from) * p.k) + u * ex2((t - from) * p.k);
+        top = most;
+      }
+      if (row < a.m) p.part[static_cast<long long>(s.unit_col) * a.m + row] = make_float2(top, sum);
     }
   };
 };
@@ -104,12 +118,12 @@ struct FinishArgs {
   float2* stats;
 };
 
-// Joins the tiles' pairs: 32 rows a block, 16 warps over the tiles.
-constexpr int FINISH_WARPS = 16;
+// Joins the tiles' pairs: 8 rows a block, 4 lanes of each of 16 warps a row.
+constexpr int FINISH_WARPS = 16, FINISH_ROWS = 8;
 __global__ void __launch_bounds__(32 * FINISH_WARPS) finish_kernel(const __grid_constant__ FinishArgs a) {
-  __shared__ float2 buf[FINISH_WARPS][32];
+  __shared__ float2 buf[FINISH_WARPS][FINISH_ROWS];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int row = blockIdx.x * 32 + lane;
+  const int row = blockIdx.x * FINISH_ROWS + (lane & (FINISH_ROWS - 1));
   float top = -INFINITY, sum = 0.0f;
   auto join = [&](float2 x) {
     const float most = fmaxf(top, x.x), from = most == -INFINITY ? 0.0f : most;
@@ -118,11 +132,14 @@ __global__ void __launch_bounds__(32 * FINISH_WARPS) finish_kernel(const __grid_
   };
   if (row < a.rows) {
 #pragma unroll 4
-    for (int i = warp; i < a.parts; i += FINISH_WARPS) join(a.part[static_cast<long long>(i) * a.rows + row]);
+    for (int i = warp * 4 + lane / FINISH_ROWS; i < a.parts; i += FINISH_WARPS * 4) join(a.part[static_cast<long long>(i) * a.rows + row]);
   }
-  buf[warp][lane] = make_float2(top, sum);
+#pragma unroll
+  for (int o = FINISH_ROWS; o < 32; o <<= 1)
+    join(make_float2(__shfl_xor_sync(0xffffffffu, top, o), __shfl_xor_sync(0xffffffffu, sum, o)));
+  if (lane < FINISH_ROWS) buf[warp][lane] = make_float2(top, sum);
   __syncthreads();
-  if (warp || row >= a.rows) return;
+  if (warp || lane >= FINISH_ROWS || row >= a.rows) return;
   for (int w = 1; w < FINISH_WARPS; ++w) join(buf[w][lane]);
   const long long t = token_at(a.tokens, a.tok64, row);
   const float log_sum = logf(sum);
@@ -176,7 +193,7 @@ struct Slope {
   struct State {
     float top, of_p, of_hot;
     int hot;  // the token's column in the piece
-    __device__ State(const Params& p, const Shape& a, const Spot& s, int, int, int) {
+    __device__ State(const Params& p, const Shape& a, const Spot& s) {
       top = 0.0f, of_p = 0.0f, of_hot = 0.0f, hot = -1;
       const int row = s.row0 + s.lane;
       if (row >= a.m) return;
@@ -210,7 +227,7 @@ struct Slope {
       }
       put16(s, w, p.out, p.ld, a.m, a.n, col0, 1);
     }
-    __device__ void end(const Params&, const Shape&, const Spot&, int) {}
+    __device__ void end(const Params&, const Shape&, const Spot&) {}
   };
 };
 
@@ -264,7 +281,7 @@ Layout plan(int device, const void* x, long long ldx, const void* w, long long l
   if (!grad) {
     l.forward = plan_for(rows, vocab, kblocks, 1, false, false, sms);
     const long long cols = l.forward.tile == 0 ? 256 : l.forward.tile == 1 ? 128 : 64;
-    l.part = take(sizeof(float2) * 2 * ((vocab + cols - 1) / cols) * rows);
+    l.part = take(sizeof(float2) * ((vocab + cols - 1) / cols) * rows);
     l.target = take(sizeof(float) * rows);
   } else {
     l.pieces = (vocab * rows + PIECE - 1) / PIECE;
@@ -348,10 +365,10 @@ extern "C" int ad_linear_logprobs(int device, int dtype, const void* x, int64_t 
   const long long cols = l.forward.tile == 0 ? 256 : l.forward.tile == 1 ? 128 : 64;
   FinishArgs f = {};
   f.part = q.part, f.target = q.target, f.tokens = tokens, f.tok64 = tok64;
-  f.parts = static_cast<int>(2 * ((vocab + cols - 1) / cols)), f.rows = static_cast<int>(rows);
+  f.parts = static_cast<int>((vocab + cols - 1) / cols), f.rows = static_cast<int>(rows);
   f.vocab = vocab, f.scale = scale, f.k = q.k;
   f.logp = logp, f.lse = lse, f.stats = reinterpret_cast<float2*>(stats);
-  const cudaError_t e = launch<finish_kernel>(dim3(static_cast<unsigned>((rows + 31) / 32)), 32 * FINISH_WARPS, 0, st, f);
+  const cudaError_t e = launch<finish_kernel>(dim3(static_cast<unsigned>((rows + FINISH_ROWS - 1) / FINISH_ROWS)), 32 * FINISH_WARPS, 0, st, f);
   return e == cudaSuccess ? 0 : fail_cuda(who, e);
 }
 

@@ -898,7 +898,7 @@ _ACTS = {"silu": 0, "gelu": 1, "gelu_tanh": 2, "relu": 3}
 
 
 class FeedForward(NamedTuple):
-    """Results of ``feed_forward``: y [..., width], and x w_gate^T and x w_up^T [rows, hidden] or None."""
+    """Results of ``feed_forward``: y [..., width], and x w_gate^T and x w_up^T, float32 [rows, hidden], or None."""
     y: object
     gate: object
     up: object
@@ -963,7 +963,7 @@ def feed_forward(x, w_gate, w_up, w_down, *, act: str = "silu", keep: bool = Fal
 
     ``act``: "silu", "gelu", "gelu_tanh" or "relu".  Operands are bfloat16 or float16; products are accumulated
     in 32 bits, the activation is taken of them, and ``h`` is rounded to the operands' type.  ``keep`` keeps
-    both products before the activation for ``feed_forward_grad``.  ``out``: a ``FeedForward`` to write;
+    both products before the activation, in 32 bits, for ``feed_forward_grad``.  ``out``: a ``FeedForward`` to write;
     ``workspace``: adjacent elements at a 256-byte boundary, ``feed_forward_workspace`` bytes or more."""
     dev, dt, rows, width, hidden, ldx, ldwg, ldwu, ldwd = _ffn_operands(x, w_gate, w_up, w_down, act)
     s = _stream(dev, stream, x, out is None or workspace is None)
@@ -971,8 +971,8 @@ def feed_forward(x, w_gate, w_up, w_down, *, act: str = "silu", keep: bool = Fal
     if out is None:
         gate = up = None
         if keep:  # rows that start on 16-byte boundaries, whatever the hidden size is
-            ldg = ldu = (hidden + 7) // 8 * 8
-            gate, up = (_empty((rows, ldg), x)[:, :hidden] for _ in range(2))
+            ldg = ldu = (hidden + 3) // 4 * 4
+            gate, up = (_empty((rows, ldg), x, "float32")[:, :hidden] for _ in range(2))
         r = FeedForward(_empty_rows(x), gate, up)
         ldy = width
     else:
@@ -985,8 +985,8 @@ def feed_forward(x, w_gate, w_up, w_down, *, act: str = "silu", keep: bool = Fal
         if (r.gate is None) != (not keep) or (r.up is None) != (not keep):
             raise ValueError("out: gate and up go with keep")
         if keep:
-            ldg = _matrix(r.gate, rows, hidden, dt, dev, "out gate")
-            ldu = _matrix(r.up, rows, hidden, dt, dev, "out up")
+            ldg = _matrix(r.gate, rows, hidden, F32, dev, "out gate")
+            ldu = _matrix(r.up, rows, hidden, F32, dev, "out up")
     operands = (x.data_ptr(), ldx, w_gate.data_ptr(), ldwg, w_up.data_ptr(), ldwu, w_down.data_ptr(), ldwd)
     workspace, have = _scratch(_ffn_workspace(dev, dt, operands, None, 0, rows, width, hidden, 0)
                                if workspace is None else 0, workspace, dev, x)
@@ -999,8 +999,7 @@ def feed_forward(x, w_gate, w_up, w_down, *, act: str = "silu", keep: bool = Fal
 def feed_forward_grad(dy, x, w_gate, w_up, w_down, gate, up, *, act: str = "silu", accumulate: bool = False, out=None,
                       workspace=None, stream=None) -> FeedForwardGrads:
     """The gradients of ``feed_forward``'s operands from that of ``y``, its operands and the ``gate`` and
-    ``up`` that it kept.  What lies between the products is rounded to the operands' type, sums are held in
-    32 bits.  ``out``: a ``FeedForwardGrads`` to write, the weights' all of the operands' type or all float32, to
+    ``up`` that it kept.  What enters a product is rounded to the operands' type, sums are held in 32 bits.  ``out``: a ``FeedForwardGrads`` to write, the weights' all of the operands' type or all float32, to
     which the gradients are added with ``accumulate``; ``workspace``: as for ``feed_forward``, with ``dy``."""
     dev, dt, rows, width, hidden, ldx, ldwg, ldwu, ldwd = _ffn_operands(x, w_gate, w_up, w_down, act)
     _typed(dy, dt, "dy")
@@ -1008,8 +1007,8 @@ def feed_forward_grad(dy, x, w_gate, w_up, w_down, gate, up, *, act: str = "silu
     _on(dev, dy, "dy")
     lddy = _rows(dy, "dy")[2]
     _apart(lddy, rows, width, "dy")
-    ldg = _matrix(gate, rows, hidden, dt, dev, "gate")
-    ldu = _matrix(up, rows, hidden, dt, dev, "up")
+    ldg = _matrix(gate, rows, hidden, F32, dev, "gate")
+    ldu = _matrix(up, rows, hidden, F32, dev, "up")
     if accumulate and out is None:
         raise ValueError("accumulate: out has to be given")
     s = _stream(dev, stream, x, out is None or workspace is None)

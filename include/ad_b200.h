@@ -293,7 +293,7 @@ int ad_linear_logprobs_grad(int device, int dtype, const void* x, int64_t ldx, c
  * x and y of rows x width, Wg and Wu of hidden x width, Wd of width x hidden, all
  * of dtype (AD_BF16 or AD_F16).  act: 0 silu, 1 gelu, 2 gelu by tanh, 3 relu.
  * Products are accumulated in 32 bits; h is rounded to dtype.  gate and up, of
- * rows x hidden: g and u for the gradient, or both NULL. */
+ * rows x hidden in 32 bits: g and u for the gradient, or both NULL. */
 int ad_feed_forward_workspace(int device, int dtype, const void* x, int64_t ldx, const void* w_gate,
                               int64_t ld_gate, const void* w_up, int64_t ld_up, const void* w_down,
                               int64_t ld_down, const void* dy, int64_t lddy, int64_t rows,
@@ -301,14 +301,14 @@ int ad_feed_forward_workspace(int device, int dtype, const void* x, int64_t ldx,
 int ad_feed_forward(int device, int dtype, int act, const void* x, int64_t ldx, const void* w_gate,
                     int64_t ld_gate, const void* w_up, int64_t ld_up, const void* w_down,
                     int64_t ld_down, int64_t rows, int64_t width, int64_t hidden, void* y, int64_t ldy,
-                    void* gate, int64_t ldg, void* up, int64_t ldu, void* workspace,
+                    float* gate, int64_t ldg, float* up, int64_t ldu, void* workspace,
                     size_t workspace_bytes, void* stream);
 /* The gradients of x (of dtype) and the weights (of dw_type: dtype or AD_F32; added
  * to what is there when `accumulate`; with no rows zeros or left alone). */
 int ad_feed_forward_grad(int device, int dtype, int act, const void* dy, int64_t lddy, const void* x,
                          int64_t ldx, const void* w_gate, int64_t ld_gate, const void* w_up,
-                         int64_t ld_up, const void* w_down, int64_t ld_down, const void* gate,
-                         int64_t ldg, const void* up, int64_t ldu, int64_t rows, int64_t width,
+                         int64_t ld_up, const void* w_down, int64_t ld_down, const float* gate,
+                         int64_t ldg, const float* up, int64_t ldu, int64_t rows, int64_t width,
                          int64_t hidden, void* dx, int64_t lddx, int dw_type, void* dw_gate,
                          int64_t lddw_gate, void* dw_up, int64_t lddw_up, void* dw_down,
                          int64_t lddw_down, int accumulate, void* workspace, size_t workspace_bytes,

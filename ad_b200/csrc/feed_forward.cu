@@ -64,6 +64,8 @@ __device__ __forceinline__ float activate(float z, float* slope) {
 // h of 32 columns from accumulators of both products.
 struct Gated {
   static constexpr bool DUAL = true;
+  static constexpr int WARPS = 16, SIDE = 4096;
+  using Units = ByNumber;
   struct Params {
     unsigned short* h;
     float *gate, *up;  // NULL when not kept
@@ -94,14 +96,16 @@ struct Gated {
       tmem_issue32(acc + cols, t);
       tmem_wait32(q);
       tmem_wait32(t);
+      if (s.last) accumulator_read(s);
 #pragma unroll
-      for (int j = 0; j < 32; ++j) {
-        g[j] = s.dead ? __int_as_float(0x7fffffff) : __uint_as_float(q[j]);
-        u[j] = __uint_as_float(t[j]);
+      for (int j = 0; j < 32; ++j) g[j] = __uint_as_float(q[j]), u[j] = __uint_as_float(t[j]);
+      if (s.dead) {
+#pragma unroll
+        for (int j = 0; j < 32; ++j) g[j] = u[j] = __int_as_float(0x7fffffff);
       }
       if (p.gate) {
-        put32(s, g, p.gate, p.ldg, a.m, a.n, col0, p.vec_g);
-        put32(s, u, p.up, p.ldu, a.m, a.n, col0, p.vec_u);
+        put32(s, g, p.gate, p.ldg, s.m, s.n, col0, p.vec_g);
+        put32(s, u, p.up, p.ldu, s.m, s.n, col0, p.vec_u);
       }
       switch (p.act) {
         case SILU: gated<SILU>(g, u); break;
@@ -110,7 +114,7 @@ struct Gated {
         default: gated<RELU>(g, u);
       }
       round(g, w, a.half);
-      put16(s, w, p.h, p.ldh, a.m, a.n, col0, p.vec_h);
+      put16(s, w, p.h, p.ldh, s.m, s.n, col0, p.vec_h);
     }
   };
 };
@@ -118,6 +122,8 @@ struct Gated {
 // dg, du and h from an accumulator of dh, eight columns of a row a lane.
 struct GatedGrad {
   static constexpr bool DUAL = false;
+  static constexpr int WARPS = 16, SIDE = 4096;
+  using Units = ByNumber;
   struct Params {
     const float *gate, *up;
     long long ldg, ldu;
@@ -145,15 +151,16 @@ struct GatedGrad {
 #pragma unroll
       for (int j = 0; j < 2; ++j) {
         k.g[j] = k.u[j] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-        if (row < a.m) {
+        if (row < s.m) {
           k.g[j] = reinterpret_cast<const float4*>(p.gate + row * p.ldg + col)[j];
           k.u[j] = reinterpret_cast<const float4*>(p.up + row * p.ldu + col)[j];
         }
       }
     }
-    template <int ACT>
+    template <int ACT, int HALF>
     __device__ static void part(const Params& p, const Shape& a, const Spot& s, int col0, Kept (&k)[2]) {
       const int q = s.lane & 3;
+      long long at = (s.row0 + (s.lane >> 2)) * p.ld + col0 + q * 8;
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         const int r = i * 8 + (s.lane >> 2);
@@ -167,24 +174,31 @@ struct GatedGrad {
           one<ACT>(d.y, c.g[j].y, c.u[j].y, x[1], y[1], z[1]);
           one<ACT>(d.z, c.g[j].z, c.u[j].z, x[2], y[2], z[2]);
           one<ACT>(d.w, c.g[j].w, c.u[j].w, x[3], y[3], z[3]);
-          dg[2 * j] = pack2(x[0], x[1], a.half), dg[2 * j + 1] = pack2(x[2], x[3], a.half);
-          du[2 * j] = pack2(y[0], y[1], a.half), du[2 * j + 1] = pack2(y[2], y[3], a.half);
-          h[2 * j] = pack2(z[0], z[1], a.half), h[2 * j + 1] = pack2(z[2], z[3], a.half);
+          dg[2 * j] = pack2(x[0], x[1], HALF), dg[2 * j + 1] = pack2(x[2], x[3], HALF);
+          du[2 * j] = pack2(y[0], y[1], HALF), du[2 * j + 1] = pack2(y[2], y[3], HALF);
+          h[2 * j] = pack2(z[0], z[1], HALF), h[2 * j + 1] = pack2(z[2], z[3], HALF);
         }
         if (i + 2 < 4) fetch(p, a, s, col0, i + 2, k[i & 1]);
-        if (s.row0 + r < a.m) {
-          const long long at = (s.row0 + r) * p.ld + col0 + q * 8;
+        if (s.row0 + r < s.m) {
           *reinterpret_cast<uint4*>(p.dg + at) = make_uint4(dg[0], dg[1], dg[2], dg[3]);
           *reinterpret_cast<uint4*>(p.du + at) = make_uint4(du[0], du[1], du[2], du[3]);
           *reinterpret_cast<uint4*>(p.h + at) = make_uint4(h[0], h[1], h[2], h[3]);
         }
+        at += 8 * p.ld;
       }
+    }
+    template <int ACT>
+    __device__ static void part(const Params& p, const Shape& a, const Spot& s, int col0, Kept (&k)[2]) {
+      if (a.half)
+        part<ACT, 1>(p, a, s, col0, k);
+      else
+        part<ACT, 0>(p, a, s, col0, k);
     }
     template <int ACT>
     __device__ static void columns(const Params& p, const Shape& a, const Spot& s, int col0) {
       const int col = col0 + s.lane;
-      if (col >= a.n) return;
-      for (int r = 0; r < 32 && s.row0 + r < a.m; ++r) {
+      if (col >= s.n) return;
+      for (int r = 0; r < 32 && s.row0 + r < s.m; ++r) {
         const float dh = staged1(s, r);
         const int type = a.half ? AD_F16 : AD_BF16;
         const long long row = s.row0 + r;
@@ -196,18 +210,14 @@ struct GatedGrad {
       }
     }
     __device__ void chunk(const Params& p, const Shape& a, const Spot& s, int col0, unsigned acc, int) {
-      const bool fast = p.vec && col0 + CHUNK <= a.n;
+      const bool fast = p.vec && col0 + CHUNK <= s.n;
       Kept k[2];
       if (fast) {
         fetch(p, a, s, col0, 0, k[0]);
         fetch(p, a, s, col0, 1, k[1]);
       }
       float v[32];
-      tmem_ld32(acc, v);
-      if (s.dead) {
-#pragma unroll
-        for (int j = 0; j < 32; ++j) v[j] = __int_as_float(0x7fffffff);
-      }
+      take32(s, acc, v);
       stage32(s, v);
       if (fast) {
         switch (p.act) {
@@ -238,41 +248,11 @@ struct Operand {
 struct Layout {
   size_t pack[5], h, dg, du, partial, total;
   long long ld;  // of h, dg, du
-  Plan hidden, y, dh, dx, dw, dd;
+  int tiling;    // of the product with an epilogue of its own
 };
 
-Problem hidden_of(int device, int half, long long rows, long long width, long long hidden) {
-  Problem p = {};
-  p.device = device, p.half = half;
-  p.m = rows, p.n = hidden, p.k = p.k0 = width, p.groups = 1;
-  return p;
-}
-Problem y_of(int device, int half, long long rows, long long width, long long hidden) {
-  Problem p = hidden_of(device, half, rows, hidden, width);
-  return p;
-}
-Problem dh_of(int device, int half, long long rows, long long width, long long hidden) {
-  Problem p = hidden_of(device, half, rows, width, hidden);
-  p.b_turned = true;
-  return p;
-}
-Problem dx_of(int device, int half, long long rows, long long width, long long hidden) {
-  Problem p = {};
-  p.device = device, p.half = half;
-  p.m = rows, p.n = width, p.k = 2 * hidden, p.k0 = hidden, p.groups = 1;
-  p.b_turned = true;
-  return p;
-}
-Problem dw_of(int device, int half, long long rows, long long m, long long n, int groups) {
-  Problem p = {};
-  p.device = device, p.half = half;
-  p.m = m, p.n = n, p.k = p.k0 = rows, p.groups = groups;
-  p.a_turned = p.b_turned = true;
-  return p;
-}
-
 // ops: x, Wg, Wu, Wd and, for the gradient, dy.
-Layout plan(int device, const Operand* ops, int count, long long rows, long long width, long long hidden, int sms) {
+Layout plan(const Device& d, const Operand* ops, int count, long long rows, long long width, long long hidden) {
   Layout l = {};
   size_t at = 0;
   auto take = [&](size_t bytes) {
@@ -284,21 +264,12 @@ Layout plan(int device, const Operand* ops, int count, long long rows, long long
     if (!tma_ready(ops[i].p, ops[i].ld, ops[i].rows)) l.pack[i] = take(2ull * ops[i].rows * round_up(ops[i].cols, 64));
   l.ld = round_up(hidden, 64);
   l.h = take(2ull * rows * l.ld);
-  const long long kblocks = (width + BK - 1) / BK;
-  if (count == 4) {
-    l.hidden = plan_for(rows, hidden, kblocks, 1, true, false, sms);
-    const Problem y = y_of(device, 0, rows, width, hidden);
-    l.y = store_plan(y, sms);
-    l.partial = take(partial_bytes(y, l.y, false));
-  } else {
+  if (count == 5) {
     l.dg = take(2ull * rows * l.ld);
     l.du = take(2ull * rows * l.ld);
-    l.dh = plan_for(rows, hidden, kblocks, 1, false, false, sms);
-    const Problem x = dx_of(device, 0, rows, width, hidden), w = dw_of(device, 0, rows, hidden, width, 2),
-                  d = dw_of(device, 0, rows, width, hidden, 1);
-    l.dx = store_plan(x, sms), l.dw = store_plan(w, sms), l.dd = store_plan(d, sms);
-    l.partial = take(std::max({partial_bytes(x, l.dx, false), partial_bytes(w, l.dw, false), partial_bytes(d, l.dd, false)}));
   }
+  l.tiling = tiling_for(rows, hidden, (width + BK - 1) / BK, count == 4, d.sms);
+  l.partial = take(partial_bytes(d));
   l.total = at;
   return l;
 }
@@ -341,9 +312,9 @@ extern "C" int ad_feed_forward_workspace(int device, int dtype, const void* x, i
   if (!rows) return 0;
   DeviceGuard guard(device);
   if (guard.error() != cudaSuccess) return fail_cuda(who, guard.error());
-  const int sms = sm_count(guard.device());
-  if (!sms) return fail("%s: no device properties", who);
-  *bytes = plan(guard.device(), ops, count, rows, width, hidden, sms).total;
+  const Device d = {guard.device(), sm_count(guard.device())};
+  if (!d.sms) return fail("%s: no device properties", who);
+  *bytes = plan(d, ops, count, rows, width, hidden).total;
   return 0;
 }
 
@@ -362,9 +333,10 @@ extern "C" int ad_feed_forward(int device, int dtype, int act, const void* x, in
   if (!aligned(y, 2) || !aligned({gate, up}, 4)) return fail("%s: an operand is not aligned to its elements", who);
   DeviceGuard guard(device);
   if (guard.error() != cudaSuccess) return fail_cuda(who, guard.error());
-  const int dev = guard.device(), half = dtype == AD_F16, sms = sm_count(dev);
-  if (!sms) return fail("%s: no device properties", who);
-  const Layout l = plan(dev, ops, 4, rows, width, hidden, sms);
+  const Device d = {guard.device(), sm_count(guard.device())};
+  if (!d.sms) return fail("%s: no device properties", who);
+  const int half = dtype == AD_F16;
+  const Layout l = plan(d, ops, 4, rows, width, hidden);
   if (!workspace || !aligned(workspace, 256) || workspace_bytes < l.total)
     return fail("%s: needs %zu bytes of workspace, 256-byte aligned", who, l.total);
   cudaStream_t st = static_cast<cudaStream_t>(stream);
@@ -372,18 +344,16 @@ extern "C" int ad_feed_forward(int device, int dtype, int act, const void* x, in
   Mat m[4];
   for (int i = 0; i < 4; ++i)
     if (ready(who, ops[i], ws + l.pack[i], st, &m[i])) return 1;
-  Problem p = hidden_of(dev, half, rows, width, hidden);
-  p.a[0] = m[0], p.b[0] = m[1], p.b[1] = m[2];
+  const Problem p = {rows, hidden, width, width, false, false, {m[0], {}}, {m[1], m[2]}};
   Gated::Params q = {};
   q.h = reinterpret_cast<unsigned short*>(ws + l.h), q.ldh = l.ld, q.vec_h = 1;
   q.gate = gate, q.up = up;
   q.ldg = ldg, q.ldu = ldu, q.vec_g = vec32(gate, ldg, rows), q.vec_u = vec32(up, ldu, rows);
   q.act = act;
-  if (start<Gated>(who, p, l.hidden, q, sms, st)) return 1;
-  p = y_of(dev, half, rows, width, hidden);
-  p.a[0] = Mat{ws + l.h, l.ld}, p.b[0] = m[3];
-  const Out out = {y, ldy};
-  return store_product(who, p, l.y, dtype, &out, false, nullptr, reinterpret_cast<float*>(ws + l.partial), nullptr, sms, st);
+  if (start<Gated>(who, d, p, half, l.tiling, q, st)) return 1;
+  const Problem product = {rows, width, hidden, hidden, false, false, {{ws + l.h, l.ld}, {}}, {m[3], {}}};
+  const Result result = {y, ldy, dtype, false, nullptr, 0, nullptr};
+  return store_products(who, d, half, &product, &result, 1, reinterpret_cast<float*>(ws + l.partial), st);
 }
 
 extern "C" int ad_feed_forward_grad(int device, int dtype, int act, const void* dy, int64_t lddy, const void* x,
@@ -414,41 +384,36 @@ extern "C" int ad_feed_forward_grad(int device, int dtype, int act, const void* 
   if (!aligned(dx, 2) || !aligned({gate, up}, 4)) return fail("%s: an operand is not aligned to its elements", who);
   DeviceGuard guard(device);
   if (guard.error() != cudaSuccess) return fail_cuda(who, guard.error());
-  const int dev = guard.device(), half = dtype == AD_F16, sms = sm_count(dev);
-  if (!sms) return fail("%s: no device properties", who);
-  const Layout l = plan(dev, ops, 5, rows, width, hidden, sms);
+  const Device d = {guard.device(), sm_count(guard.device())};
+  if (!d.sms) return fail("%s: no device properties", who);
+  const int half = dtype == AD_F16;
+  const Layout l = plan(d, ops, 5, rows, width, hidden);
   if (!workspace || !aligned(workspace, 256) || workspace_bytes < l.total)
     return fail("%s: needs %zu bytes of workspace, 256-byte aligned", who, l.total);
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   unsigned char* ws = static_cast<unsigned char*>(workspace);
-  float* partial = reinterpret_cast<float*>(ws + l.partial);
   Mat m[5];
   for (int i = 0; i < 5; ++i)
     if (ready(who, ops[i], ws + l.pack[i], st, &m[i])) return 1;
   const Mat h = {ws + l.h, l.ld}, dg = {ws + l.dg, l.ld}, du = {ws + l.du, l.ld};
 
-  Problem p = dh_of(dev, half, rows, width, hidden);
-  p.a[0] = m[4], p.b[0] = m[3];
+  const Problem p = {rows, hidden, width, width, false, true, {m[4], {}}, {m[3], {}}};
   GatedGrad::Params q = {};
   q.gate = gate, q.up = up;
   q.ldg = ldg, q.ldu = ldu, q.vec = vec32(gate, ldg, rows) && vec32(up, ldu, rows);
   q.dg = reinterpret_cast<unsigned short*>(ws + l.dg), q.du = reinterpret_cast<unsigned short*>(ws + l.du);
   q.h = reinterpret_cast<unsigned short*>(ws + l.h), q.ld = l.ld;
   q.act = act;
-  if (start<GatedGrad>(who, p, l.dh, q, sms, st)) return 1;
+  if (start<GatedGrad>(who, d, p, half, l.tiling, q, st)) return 1;
 
-  p = dx_of(dev, half, rows, width, hidden);
-  p.a[0] = dg, p.a[1] = du, p.b[0] = m[1], p.b[1] = m[2];
-  Out out[2] = {{dx, lddx}, {}};
-  if (store_product(who, p, l.dx, dtype, out, false, nullptr, partial, nullptr, sms, st)) return 1;
-
-  p = dw_of(dev, half, rows, hidden, width, 2);
-  p.a[0] = dg, p.a[1] = du, p.b[0] = p.b[1] = m[0];
-  out[0] = {dw_gate, lddw_gate}, out[1] = {dw_up, lddw_up};
-  if (store_product(who, p, l.dw, dw_type, out, accumulate != 0, nullptr, partial, nullptr, sms, st)) return 1;
-
-  p = dw_of(dev, half, rows, width, hidden, 1);
-  p.a[0] = m[4], p.b[0] = h;
-  out[0] = {dw_down, lddw_down};
-  return store_product(who, p, l.dd, dw_type, out, accumulate != 0, nullptr, partial, nullptr, sms, st);
+  const bool more = accumulate != 0;
+  const Problem products[4] = {{rows, width, 2 * hidden, hidden, false, true, {dg, du}, {m[1], m[2]}},
+                               {hidden, width, rows, rows, true, true, {dg, {}}, {m[0], {}}},
+                               {hidden, width, rows, rows, true, true, {du, {}}, {m[0], {}}},
+                               {width, hidden, rows, rows, true, true, {m[4], {}}, {h, {}}}};
+  const Result results[4] = {{dx, lddx, dtype, false, nullptr, 0, nullptr},
+                             {dw_gate, lddw_gate, dw_type, more, nullptr, 0, nullptr},
+                             {dw_up, lddw_up, dw_type, more, nullptr, 0, nullptr},
+                             {dw_down, lddw_down, dw_type, more, nullptr, 0, nullptr}};
+  return store_products(who, d, half, products, results, 4, reinterpret_cast<float*>(ws + l.partial), st);
 }

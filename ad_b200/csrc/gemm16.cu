@@ -1,121 +1,207 @@
 // Products of 16-bit matrices to memory (gemm16.cuh): results in 16 or 32 bits,
-// sums over several products, splits of a long K, and copies of operands whose
+// added to others, several products in one launch, and copies of operands whose
 // rows are not aligned to the 16 bytes that TMA asks for.
+//
+// Up to 2048 tiles are dealt out from a list that the host makes: whole tiles, the
+// longest first, each to the blocks that are done first, and those that would stick
+// out above the others cut along K so that all end together (where that saves more than the partial
+// sums' way through memory costs).  The list goes with the kernel's parameters.  What
+// it gains: dx, dWg, dWu and dWd of a feed-forward block of 4095 x 512 x 2048 took 88 us
+// as three launches with equal splits and their joins, XXX in one.
+#include <cstdlib>
+
 #include "gemm16.cuh"
 
 namespace adgemm {
 
 namespace {
 
+constexpr int MAX_WORKERS = 256;
+constexpr int SMALL_LIST = 256, LARGE_LIST = 2048;  // units of a launch: 3 and 25 KB of parameters
+constexpr int LEAST = 6;                            // 64 elements of K that a part of a tile has at least
+
+struct Listed {
+  unsigned where;  // group, row and column of the tile
+  unsigned short kb0, kb1;
+};
+__host__ __device__ __forceinline__ unsigned pack_where(int group, int row, int col) {
+  return static_cast<unsigned>(group) << 30 | static_cast<unsigned>(row) << 15 | static_cast<unsigned>(col);
+}
+template <int N>
+struct List {
+  Listed unit[N];
+  short slot[N];
+  short first[MAX_WORKERS + 1];  // of each worker's units
+};
+template <>
+struct List<0> {};
+
+template <int N>
+struct ByList {
+  template <typename P>
+  __device__ static void range(const P& p, const Shape&, int worker, int, int& first, int& end, int& step) {
+    first = p.list.first[worker], end = p.list.first[worker + 1], step = 1;
+  }
+  template <typename P>
+  __device__ static Unit unit(const P& p, const Shape&, int u) {
+    const Listed l = p.list.unit[u];
+    return {static_cast<int>(l.where >> 30), static_cast<int>(l.where >> 15 & 0x7fff), static_cast<int>(l.where & 0x7fff),
+            l.kb0, l.kb1, p.list.slot[u]};
+  }
+};
+
+struct Target {
+  void* out;
+  const float* addend;
+  const float* alpha;
+  long long ld, ld_addend;
+  int type, accumulate;
+  int vec;  // four elements at a time are aligned, and eight of 16 bits
+};
+struct Targets {
+  Target t[MAX_GROUPS];
+  float* partial;
+};
+
+// Four adjacent elements.
+__device__ __forceinline__ void load4(const void* p, int type, long long at, float (&x)[4]) {
+  if (type == AD_F32) {
+    const float4 v = *reinterpret_cast<const float4*>(static_cast<const float*>(p) + at);
+    x[0] = v.x, x[1] = v.y, x[2] = v.z, x[3] = v.w;
+  } else {
+    const uint2 v = *reinterpret_cast<const uint2*>(static_cast<const unsigned short*>(p) + at);
+    const float2 a = unpack2(v.x, type == AD_F16), b = unpack2(v.y, type == AD_F16);
+    x[0] = a.x, x[1] = a.y, x[2] = b.x, x[3] = b.y;
+  }
+}
+__device__ __forceinline__ void store4(void* p, int type, long long at, const float (&x)[4]) {
+  if (type == AD_F32)
+    *reinterpret_cast<float4*>(static_cast<float*>(p) + at) = make_float4(x[0], x[1], x[2], x[3]);
+  else
+    *reinterpret_cast<uint2*>(static_cast<unsigned short*>(p) + at) =
+        make_uint2(pack2(x[0], x[1], type == AD_F16), pack2(x[2], x[3], type == AD_F16));
+}
+// alpha (x + addend) + what is there, to the result.
+__device__ __forceinline__ void finish4(const Target& t, float alpha, long long row, int col, float4 v) {
+  float x[4] = {v.x, v.y, v.z, v.w}, y[4];
+  if (t.addend) {
+    load4(t.addend, AD_F32, row * t.ld_addend + col, y);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) x[j] += y[j];
+  }
+#pragma unroll
+  for (int j = 0; j < 4; ++j) x[j] *= alpha;
+  if (t.accumulate) {
+    load4(t.out, t.type, row * t.ld + col, y);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) x[j] += y[j];
+  }
+  store4(t.out, t.type, row * t.ld + col, x);
+}
+__device__ __forceinline__ void finish1(const Target& t, float alpha, long long row, int col, float x) {
+  if (t.addend) x += t.addend[row * t.ld_addend + col];
+  x *= alpha;
+  if (t.accumulate) x += load_any(t.out, t.type, row * t.ld + col);
+  store_any(t.out, t.type, row * t.ld + col, x);
+}
+
+// N: the list's room, 0 for units by number.
+template <int N>
 struct Store {
   static constexpr bool DUAL = false;
+  static constexpr int WARPS = 8, SIDE = 4096;
+  using Units = std::conditional_t<N == 0, ByNumber, ByList<N>>;
   struct Params {
-    void* out[MAX_GROUPS];
-    long long ld[MAX_GROUPS];
-    long long split_stride;  // elements between the partial sums of two splits
-    long long group_stride;  // and of two groups
-    int type;                // AD_F32, or the operands'
-    int vec;                 // 16-byte stores are aligned
-    int accumulate;
-    const float* alpha;
+    Targets to;
+    int tile_m, tile_n;
+    List<N> list;
   };
   struct State {
-    unsigned char* out;
-    long long ld;
     float alpha;
     __device__ State(const Params& p, const Shape&, const Spot& s) {
-      const int g = p.split_stride ? 0 : s.group;
-      ld = p.ld[g];
-      out = static_cast<unsigned char*>(p.out[g]) +
-            (p.split_stride ? 4 * (s.split * p.split_stride + s.group * p.group_stride) : 0);
-      alpha = p.alpha ? *p.alpha : 1.0f;
+      const float* a = p.to.t[s.unit.group].alpha;
+      alpha = a ? *a : 1.0f;
     }
     __device__ void end(const Params&, const Shape&, const Spot&) {}
     __device__ void chunk(const Params& p, const Shape& a, const Spot& s, int col0, unsigned acc, int) {
       float v[32];
-      tmem_ld32(acc, v);
-#pragma unroll
-      for (int j = 0; j < 32; ++j) v[j] = s.dead ? __int_as_float(0x7fffffff) : v[j] * alpha;
-      if (p.type != AD_F32 && !p.accumulate) {
+      take32(s, acc, v);
+      if (s.unit.slot >= 0) {  // partial sums: tiles of their own
+        float* base = p.to.partial + static_cast<long long>(s.unit.slot) * p.tile_m * p.tile_n -
+                      static_cast<long long>(s.unit.row) * p.tile_m * p.tile_n - s.unit.col * p.tile_n;
+        put32(s, v, base, p.tile_n, s.m, 0x7fffffff, col0, 1);
+        return;
+      }
+      const Target& t = p.to.t[s.unit.group];
+      if (t.type != AD_F32 && !t.accumulate && !t.addend) {
         unsigned w[16];
         if (a.half) {
 #pragma unroll
-          for (int j = 0; j < 16; ++j) w[j] = pack2(v[2 * j], v[2 * j + 1], 1);
+          for (int j = 0; j < 16; ++j) w[j] = pack2(v[2 * j] * alpha, v[2 * j + 1] * alpha, 1);
         } else {
 #pragma unroll
-          for (int j = 0; j < 16; ++j) w[j] = pack2(v[2 * j], v[2 * j + 1], 0);
+          for (int j = 0; j < 16; ++j) w[j] = pack2(v[2 * j] * alpha, v[2 * j + 1] * alpha, 0);
         }
-        put16(s, w, reinterpret_cast<unsigned short*>(out), ld, a.m, a.n, col0, p.vec);
+        put16(s, w, static_cast<unsigned short*>(t.out), t.ld, s.m, s.n, col0, t.vec);
         return;
       }
       stage32(s, v);
-      if (p.type == AD_F32) {
-        float* o = reinterpret_cast<float*>(out);
-        const int q = s.lane & 7, col = col0 + q * 4;
-        if (p.vec && col0 + CHUNK <= a.n) {
-          float4 old[8];
-#pragma unroll
-          for (int i = 0; i < 8; ++i) {
-            const int r = i * 4 + (s.lane >> 3);
-            old[i] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-            if (p.accumulate && s.row0 + r < a.m) old[i] = *reinterpret_cast<const float4*>(o + (s.row0 + r) * ld + col);
-          }
-#pragma unroll
-          for (int i = 0; i < 8; ++i) {
-            const int r = i * 4 + (s.lane >> 3);
-            const float4 x = staged(s, r, q);
-            old[i].x += x.x, old[i].y += x.y, old[i].z += x.z, old[i].w += x.w;
-            if (s.row0 + r < a.m) *reinterpret_cast<float4*>(o + (s.row0 + r) * ld + col) = old[i];
-          }
-          return;
+      if (t.vec && col0 + CHUNK <= s.n) {
+        const int q = s.lane & 7;
+#pragma unroll 4
+        for (int i = 0; i < 8; ++i) {
+          const int r = i * 4 + (s.lane >> 3);
+          const float4 x = staged(s, r, q);
+          if (s.row0 + r < s.m) finish4(t, alpha, s.row0 + r, col0 + q * 4, x);
         }
-      }
-      // a column a lane
-      const int col = col0 + s.lane;
-      if (col >= a.n) return;
-      for (int r = 0; r < 32 && s.row0 + r < a.m; ++r) {
-        float x = staged1(s, r);
-        const long long at = (s.row0 + r) * ld + col;
-        if (p.accumulate) x += load_any(out, p.type, at);
-        store_any(out, p.type, at, x);
+      } else {  // a column a lane
+        const int col = col0 + s.lane;
+        if (col < s.n)
+          for (int r = 0; r < 32 && s.row0 + r < s.m; ++r) finish1(t, alpha, s.row0 + r, col, staged1(s, r));
       }
     }
   };
 };
 
-struct JoinArgs {
-  const float* part;
-  long long split_stride, group_stride, ld_part;
-  int splits, type, accumulate;
-  int m, n;
-  void* out[MAX_GROUPS];
-  long long ld[MAX_GROUPS];
-  const float* alpha;
+// Tiles that were cut: the sums of their parts, in order, to the result.
+struct Cut {
+  unsigned where;
+  short slot, parts;
 };
+struct JoinArgs {
+  Targets to;
+  Group group[MAX_GROUPS];
+  int tile_m, tile_n;
+  Cut cut[MAX_WORKERS];
+};
+constexpr int JOIN_ROWS = 16;  // of a tile a block
 
-// Partial sums, in order, to the result.  Bound by memory.
 __global__ void __launch_bounds__(256) join_kernel(const __grid_constant__ JoinArgs a) {
-  const int g = blockIdx.z;
-  const int per = (a.n + 3) / 4;
-  const long long total = static_cast<long long>(a.m) * per;
-  const float alpha = a.alpha ? *a.alpha : 1.0f;
-  for (long long i = blockIdx.x * 256ll + threadIdx.x; i < total; i += gridDim.x * 256ll) {
-    const int r = static_cast<int>(i / per), c = static_cast<int>(i - static_cast<long long>(r) * per) * 4;
-    const float* p = a.part + g * a.group_stride + r * a.ld_part + c;
+  const Cut c = a.cut[blockIdx.y];
+  const int g = c.where >> 30, row0 = (c.where >> 15 & 0x7fff) * a.tile_m + blockIdx.x * JOIN_ROWS,
+            col0 = (c.where & 0x7fff) * a.tile_n;
+  const int m = a.group[g].m, n = a.group[g].n;
+  const Target& t = a.to.t[g];
+  const float alpha = t.alpha ? *t.alpha : 1.0f;
+  const long long size = static_cast<long long>(a.tile_m) * a.tile_n;
+  const float* part = a.to.partial + c.slot * size + static_cast<long long>(blockIdx.x) * JOIN_ROWS * a.tile_n;
+  const int per = a.tile_n / 4;
+  for (int i = threadIdx.x; i < JOIN_ROWS * per; i += 256) {
+    const int r = i / per, q = (i - r * per) * 4;
+    if (row0 + r >= m || col0 + q >= n) continue;
+    const float* p = part + r * a.tile_n + q;
     float4 x = *reinterpret_cast<const float4*>(p);
-    for (int s = 1; s < a.splits; ++s) {
-      const float4 y = *reinterpret_cast<const float4*>(p + s * a.split_stride);
+#pragma unroll 4
+    for (int k = 1; k < c.parts; ++k) {
+      const float4 y = *reinterpret_cast<const float4*>(p + k * size);
       x.x += y.x, x.y += y.y, x.z += y.z, x.w += y.w;
     }
-    const float v[4] = {x.x, x.y, x.z, x.w};
-    const long long at = r * a.ld[g] + c;
-#pragma unroll
-    for (int j = 0; j < 4; ++j)
-      if (c + j < a.n) {
-        float y = v[j] * alpha;
-        if (a.accumulate) y += load_any(a.out[g], a.type, at + j);
-        store_any(a.out[g], a.type, at + j, y);
-      }
+    if (t.vec && col0 + q + 4 <= n) {
+      finish4(t, alpha, row0 + r, col0 + q, x);
+    } else {
+      const float v[4] = {x.x, x.y, x.z, x.w};
+      for (int j = 0; j < 4 && col0 + q + j < n; ++j) finish1(t, alpha, row0 + r, col0 + q + j, v[j]);
+    }
   }
 }
 
@@ -131,46 +217,221 @@ __global__ void __launch_bounds__(256) pack_kernel(const __grid_constant__ PackA
     for (int c = threadIdx.x; c < a.cols; c += 256) a.to[r * a.ld_to + c] = a.p[r * a.ld + c];
 }
 
+// ------------------------------------------------------------------ the list
+
+struct Schedule {
+  int tiling, workers, units, cuts;
+  double us;
+  Listed unit[LARGE_LIST];
+  short slot[LARGE_LIST], first[MAX_WORKERS + 1];
+  Cut cut[MAX_WORKERS];
+};
+
+// Deals the tiles of all products out to `workers`; false when there are too many.
+bool make_schedule(const Problem* p, int count, int tiling, int workers, Schedule& s) {
+  const Tiling& t = TILINGS[tiling];
+  workers = std::min(workers, MAX_WORKERS);
+  s.tiling = tiling, s.workers = workers, s.cuts = 0;
+  long long all = 0, total = 0;
+  int order[MAX_GROUPS], rows[MAX_GROUPS], cols[MAX_GROUPS], kb[MAX_GROUPS];
+  for (int g = 0; g < count; ++g) {
+    const long long r = (p[g].m + t.m - 1) / t.m, c = (p[g].n + t.n - 1) / t.n;
+    if (r > 0x7fff || c > 0x7fff || p[g].k > 64ll * 65000) return false;
+    rows[g] = static_cast<int>(r), cols[g] = static_cast<int>(c), kb[g] = kblocks_of(p[g]);
+    all += r * c, total += r * c * kb[g];
+    order[g] = g;
+    for (int i = g; i > 0 && kb[order[i]] > kb[order[i - 1]]; --i) std::swap(order[i], order[i - 1]);
+  }
+  if (all + 2 * workers > LARGE_LIST) return false;
+  // a unit's worker, besides what goes to the device
+  static_assert(LARGE_LIST < 0x7fff, "");
+  struct Piece {
+    Listed l;
+    short worker, slot;
+  };
+  Piece piece[LARGE_LIST];
+  int pieces = 0, load[MAX_WORKERS] = {}, most = 0;
+  // Whole tiles, the longest first, to the worker that is done first, as long as
+  // they stay below the height that all would have if work could be dealt out evenly.
+  int height = static_cast<int>((total + all + workers - 1) / workers) + 1;
+  int heap[MAX_WORKERS];  // load and worker in one number
+  for (int w = 0; w < workers; ++w) heap[w] = w;
+  auto later = [](int a, int b) { return a > b; };
+  auto give = [&](unsigned where, int k) {
+    std::pop_heap(heap, heap + workers, later);
+    const int w = heap[workers - 1] % MAX_WORKERS;
+    piece[pieces++] = {{where, 0, static_cast<unsigned short>(k)}, static_cast<short>(w), -1};
+    load[w] += k + 1;
+    most = std::max(most, load[w]);
+    heap[workers - 1] = load[w] * MAX_WORKERS + w;
+    std::push_heap(heap, heap + workers, later);
+  };
+  struct Rest {
+    unsigned where;
+    int k;
+  } rest[LARGE_LIST];
+  int left = 0;
+  for (int i = 0; i < count; ++i) {
+    const int g = order[i], band_rows = t.m == 256 ? 8 : 16;
+    for (int b = 0; b < rows[g]; b += band_rows)
+      for (int c = 0; c < cols[g]; ++c)
+        for (int r = b; r < std::min(b + band_rows, rows[g]); ++r) {
+          const unsigned where = pack_where(g, r, c);
+          if (heap[0] / MAX_WORKERS + kb[g] + 1 <= height)
+            give(where, kb[g]);
+          else
+            rest[left++] = {where, kb[g]};
+        }
+  }
+  const int kept = pieces;
+  int before[MAX_WORKERS], by_load[MAX_WORKERS];
+  for (int w = 0; w < workers; ++w) before[w] = load[w], by_load[w] = w;
+  std::stable_sort(by_load, by_load + workers, [&](int a, int b) { return load[a] < load[b]; });
+  for (int i = 0; i < left; ++i) give(rest[i].where, rest[i].k);  // uncut
+  s.us = most * t.us + 4.0;
+  // Cut, the remaining tiles fill all workers up to one height.
+  const double slot_us = 2.0 * 4 * t.m * t.n / 3e6;  // a part's sums, there and back at 3 TB/s
+  // about one part for each worker
+  bool cut = left > 0 && left < workers && height > LEAST && (most - height) * t.us > 5.0 + slot_us * workers;
+  while (cut) {
+    pieces = kept;
+    s.cuts = 0;
+    int slots = 0, w = 0, filled[MAX_WORKERS];
+    for (int k = 0; k < workers; ++k) filled[k] = before[k];
+    bool fits = true;
+    for (int i = 0; i < left && fits; ++i) {
+      int kb0 = 0;
+      const int from = pieces;
+      while (kb0 < rest[i].k) {
+        while (w < workers && height - filled[by_load[w]] - 1 < LEAST) ++w;
+        if (w == workers) {
+          fits = false;
+          break;
+        }
+        int n = std::min(rest[i].k - kb0, height - filled[by_load[w]] - 1);
+        if (rest[i].k - kb0 - n < LEAST) n = rest[i].k - kb0;  // no crumbs
+        piece[pieces++] = {{rest[i].where, static_cast<unsigned short>(kb0), static_cast<unsigned short>(kb0 + n)},
+                           static_cast<short>(by_load[w]), -1};
+        filled[by_load[w]] += n + 1;
+        kb0 += n;
+      }
+      if (fits && pieces - from > 1) {
+        s.cut[s.cuts++] = {rest[i].where, static_cast<short>(slots), static_cast<short>(pieces - from)};
+        for (int k = from; k < pieces; ++k) piece[k].slot = static_cast<short>(slots++);
+      }
+    }
+    if (fits) {
+      most = 0;
+      for (int k = 0; k < workers; ++k) most = std::max(most, filled[k]);
+      s.us = most * t.us + 4.0 + (s.cuts ? 5.0 + slot_us * slots : 0.0);
+      break;
+    }
+    height += 1 + height / 64;
+  }
+  // each worker's units side by side, in order
+  int counts[MAX_WORKERS + 1] = {};
+  for (int i = 0; i < pieces; ++i) ++counts[piece[i].worker + 1];
+  for (int w = 0; w < workers; ++w) counts[w + 1] += counts[w];
+  for (int w = 0; w <= workers; ++w) s.first[w] = static_cast<short>(counts[w]);
+  for (int i = 0; i < pieces; ++i) {
+    const int to = counts[piece[i].worker]++;
+    s.unit[to] = piece[i].l, s.slot[to] = piece[i].slot;
+  }
+  s.units = pieces;
+  return true;
+}
+
+Target target_of(const Result& r, const Problem& p) {
+  Target t = {r.p, r.addend, r.alpha, r.ld, r.ld_addend, r.type, r.accumulate, 1};
+  const int per = 16 / elem_size(r.type);
+  if (!aligned(r.p, 16) || (p.m > 1 && r.ld % per) || (r.addend && (!aligned(r.addend, 16) || (p.m > 1 && r.ld_addend % 4)))) t.vec = 0;
+  return t;
+}
+
+template <int CTAS, int BN, int N>
+int start_listed(const char* who, const Device& d, int half, const Problem* p, const Targets& to, int count, const Schedule& s,
+                 cudaStream_t st) {
+  using EPI = Store<N>;
+  using TILE = Tile<CTAS, BN, EPI>;
+  Maps maps = {};
+  Shape shape = {};
+  shape.half = half;
+  typename EPI::Params params;
+  params.to = to, params.tile_m = TILE::M, params.tile_n = TILE::BN;
+  int map = 0;
+  for (int g = 0; g < count; ++g) {
+    if (map + 2 > MAX_MAPS) return fail("%s: too many operands in one launch", who);
+    if (make_maps<TILE, false>(p[g], maps, map)) return 1;
+    shape.group[g] = group_of(p[g], map);
+    map += p[g].k0 < p[g].k ? 2 : 1;
+  }
+  memcpy(params.list.unit, s.unit, sizeof(Listed) * s.units);
+  memcpy(params.list.slot, s.slot, sizeof(short) * s.units);
+  memcpy(params.list.first, s.first, sizeof(short) * (s.workers + 1));
+  int workers = 0;
+  cudaError_t e = workers_of<TILE, EPI>(d, &workers);  // its shared memory is allowed on the way
+  if (e == cudaSuccess) e = launch_gemm<TILE, EPI>(maps, shape, params, s.workers, st);
+  if (e != cudaSuccess) return fail_cuda(who, e);
+  if (!s.cuts) return 0;
+  JoinArgs j;
+  j.to = to, j.tile_m = TILE::M, j.tile_n = TILE::BN;
+  for (int g = 0; g < count; ++g) j.group[g] = shape.group[g];
+  memcpy(j.cut, s.cut, sizeof(Cut) * s.cuts);
+  e = launch<join_kernel>(dim3(TILE::M / JOIN_ROWS, s.cuts), 256, 0, st, j);
+  return e == cudaSuccess ? 0 : fail_cuda(who, e);
+}
+template <int CTAS, int BN>
+int start_schedule(const char* who, const Device& d, int half, const Problem* p, const Targets& to, int count, const Schedule& s,
+                   cudaStream_t st) {
+  return s.units <= SMALL_LIST ? start_listed<CTAS, BN, SMALL_LIST>(who, d, half, p, to, count, s, st)
+                               : start_listed<CTAS, BN, LARGE_LIST>(who, d, half, p, to, count, s, st);
+}
+
 }  // namespace
 
-Plan store_plan(const Problem& p, int sms) {
-  const long long kblocks = (p.k0 + BK - 1) / BK + (p.k - p.k0 + BK - 1) / BK;
-  return plan_for(p.m, p.n, kblocks, p.groups, false, true, sms);
+size_t partial_bytes(const Device& d) {
+  // no more parts than workers and cut tiles, of which there are fewer than workers
+  return room(sizeof(float) * 2 * static_cast<size_t>(d.sms / 2) * 256 * 256);
 }
 
-size_t partial_bytes(const Problem& p, const Plan& plan, bool sums) {
-  if (plan.splits == 1 && !sums) return 0;
-  return room(sizeof(float) * static_cast<size_t>(plan.splits) * p.groups * p.m * round_up(p.n, 4));
-}
-
-int store_product(const char* who, const Problem& p, const Plan& plan, int type, const Out* out, bool accumulate,
-                  const float* alpha, float* partial, const Sums* sums, int sms, cudaStream_t st) {
-  Store::Params q = {};
-  const bool parts = plan.splits > 1 || (sums && !(sums->first && sums->last));
-  const long long ld_part = round_up(p.n, 4);
-  JoinArgs j = {};
-  for (int g = 0; g < p.groups; ++g) j.out[g] = out[g].p, j.ld[g] = out[g].ld;
-  if (parts) {
-    q.out[0] = partial, q.ld[0] = ld_part;
-    q.group_stride = p.m * ld_part, q.split_stride = p.groups * q.group_stride;
-    q.type = AD_F32, q.vec = 1;
-    q.accumulate = sums && !sums->first;
-  } else {
-    q.type = type, q.accumulate = accumulate, q.alpha = alpha, q.vec = 1;
-    for (int g = 0; g < p.groups; ++g) {
-      q.out[g] = out[g].p, q.ld[g] = out[g].ld;
-      if (!aligned(out[g].p, 16) || (p.m > 1 && out[g].ld % (16 / elem_size(type)))) q.vec = 0;
+int store_products(const char* who, const Device& d, int half, const Problem* p, const Result* r, int count, float* partial,
+                   cudaStream_t st) {
+  Targets to = {};
+  to.partial = partial;
+  for (int g = 0; g < count; ++g) to.t[g] = target_of(r[g], p[g]);
+  Schedule s[2];
+  int best = -1;
+  for (int i = 0; i < 3; ++i) {
+    const Tiling& t = TILINGS[i];
+    int workers = 0;
+    cudaError_t e = i == 0   ? workers_of<Tile<2, 256, Store<SMALL_LIST>>, Store<SMALL_LIST>>(d, &workers)
+                    : i == 1 ? workers_of<Tile<1, 128, Store<SMALL_LIST>>, Store<SMALL_LIST>>(d, &workers)
+                             : workers_of<Tile<1, 64, Store<SMALL_LIST>>, Store<SMALL_LIST>>(d, &workers);
+    if (e != cudaSuccess) return fail_cuda(who, e);
+    if (best >= 0) {  // not if it could not do better with all its workers busy all the time
+      double work = 0.0;
+      for (int g = 0; g < count; ++g)
+        work += static_cast<double>((p[g].m + t.m - 1) / t.m) * ((p[g].n + t.n - 1) / t.n) * kblocks_of(p[g]);
+      if (work * t.us / workers + 4.0 > s[best].us * 0.97) continue;
     }
+    const int other = best < 0 ? 0 : 1 - best;
+    if (make_schedule(p, count, i, workers, s[other]) && (best < 0 || s[other].us < 0.97 * s[best].us)) best = other;
+    if (best < 0) break;  // too many large tiles: one product at a time, by number
   }
-  if (start<Store>(who, p, plan, q, sms, st)) return 1;
-  if (!parts || (sums && !sums->last)) return 0;
-  j.part = partial, j.split_stride = q.split_stride, j.group_stride = q.group_stride, j.ld_part = ld_part;
-  j.splits = plan.splits, j.type = type, j.accumulate = accumulate, j.alpha = alpha;
-  j.m = static_cast<int>(p.m), j.n = static_cast<int>(p.n);
-  const long long blocks = (p.m * (ld_part / 4) + 255) / 256;
-  const cudaError_t e = launch<join_kernel>(dim3(static_cast<unsigned>(std::min<long long>(blocks, 8 * sms)), 1, p.groups),
-                                            256, 0, st, j);
-  return e == cudaSuccess ? 0 : fail_cuda(who, e);
+  if (best < 0) {
+    if (count > 1) {
+      for (int g = 0; g < count; ++g)
+        if (store_products(who, d, half, p + g, r + g, 1, partial, st)) return 1;
+      return 0;
+    }
+    Store<0>::Params params = {};
+    params.to = to;
+    return start<Store<0>>(who, d, p[0], half, 0, params, st);
+  }
+  const Schedule& b = s[best];
+  return b.tiling == 0   ? start_schedule<2, 256>(who, d, half, p, to, count, b, st)
+         : b.tiling == 1 ? start_schedule<1, 128>(who, d, half, p, to, count, b, st)
+                         : start_schedule<1, 64>(who, d, half, p, to, count, b, st);
 }
 
 int pack_rows(const char* who, const void* p, long long ld, long long rows, long long cols, void* to, long long ld_to,

@@ -15,8 +15,9 @@
 // the products into one of two accumulators, sixteen work on the other, so that a
 // tile's epilogue is hidden behind the next tile's products.  Tiles are walked in
 // bands of rows, so that the tiles under way at a time share operands in L2.
-// Few tiles with a long K are split over K: partial sums go to memory in 32 bits
-// and are joined in order.  Nothing depends on scheduling.
+// Products to memory (gemm16.cu) are dealt out as whole tiles and, where the last round
+// would leave blocks without one, as parts of a tile's K, whose sums are joined in
+// order.  Nothing depends on scheduling.
 #ifndef AD_B200_GEMM16_CUH
 #define AD_B200_GEMM16_CUH
 
@@ -39,53 +40,65 @@ using namespace adops;
 
 constexpr int BK = 64;            // elements of K a stage: 128 bytes, the swizzle's width
 constexpr int BOX = 64 * BK * 2;  // bytes of a box of 64 x 64
-constexpr int EPI_WARPS = 16, PARTS = EPI_WARPS / 4;  // warps that share 32 rows, each with every fourth chunk
-constexpr int THREADS = 32 * (2 + EPI_WARPS);
-constexpr int CHUNK = 32;                  // columns that an epilogue takes at a time
-constexpr int SIDE = 32 * CHUNK * 4;       // bytes of shared memory of an epilogue warp: 32 rows of them
-constexpr int MAX_GROUPS = 3;
+constexpr int CHUNK = 32;         // columns that an epilogue takes at a time
+constexpr int MAX_GROUPS = 4, MAX_MAPS = 6;
 
-// Tiles: CTAS blocks work on one of 128 CTAS rows and BN columns.
-template <int CTAS_, int BN_>
+// Tiles: CTAS blocks work on one of 128 CTAS rows and BN columns.  An epilogue has
+// WARPS warps, and SIDE bytes of shared memory for each of them.
+template <int CTAS_, int BN_, typename EPI>
 struct Tile {
   static constexpr int CTAS = CTAS_, BN = BN_, M = 128 * CTAS;
   static constexpr int QN = BN / CTAS;  // columns whose operand a block holds
   static constexpr int P_BYTES = 128 * BK * 2, Q_BYTES = QN * BK * 2, STAGE = P_BYTES + Q_BYTES;
-  static constexpr int STAGES = (225 * 1024 - EPI_WARPS * SIDE) / STAGE < 8 ? (225 * 1024 - EPI_WARPS * SIDE) / STAGE : 8;
-  static constexpr int SMEM = STAGES * STAGE + EPI_WARPS * SIDE + 1024 + 256;
+  static constexpr int SIDES = EPI::WARPS * EPI::SIDE, MOST = (225 * 1024 - SIDES) / STAGE;
+  static constexpr int STAGES = MOST < 8 ? MOST : 8;
+  static constexpr int SMEM = STAGES * STAGE + SIDES + 1024 + 256;
+  static constexpr int THREADS = 32 * (2 + EPI::WARPS);
   static constexpr int TMEM = 2 * BN;
 };
 
+// One of the products of a launch.
+struct Group {
+  int m, n;
+  int kblocks0;            // of the first operands (the second ones' follow)
+  int a_turned, b_turned;  // operands lie across K
+  int map;                 // its first operands' maps
+};
 struct Shape {
-  int m, n;                        // of each group
-  int kblocks, kblocks0;           // all, and those of the first operands (the others' follow)
-  int row_tiles, col_tiles, groups, splits, per_split;
-  int band;                        // row tiles that share a walk over the columns
-  int units;
-  int a_turned, b_turned;          // operands lie across K
-  int half;                        // f16, else bf16
+  Group group[MAX_GROUPS];
+  int half;  // f16, else bf16
+  // the only group's, where units go by number
+  int kblocks, row_tiles, col_tiles, units;
+  int band;  // row tiles that share a walk over the columns
 };
 struct Maps {
-  CUtensorMap a[MAX_GROUPS], b[MAX_GROUPS];
+  CUtensorMap a[MAX_MAPS], b[MAX_MAPS];
 };
 
+// A tile, or a part of its K.
 struct Unit {
-  int row, col, group, split;
+  int group, row, col, kb0, kb1;
+  int slot;  // where partial sums go, or -1
 };
-__device__ __forceinline__ Unit unit_of(const Shape& s, int u) {
-  Unit t;
-  const int tiles = s.row_tiles * s.col_tiles;
-  const int gs = u / tiles;
-  u -= gs * tiles;
-  t.split = gs / s.groups;
-  t.group = gs - t.split * s.groups;
-  const int per = s.band * s.col_tiles, band = u / per;
-  u -= band * per;
-  const int rows = min(s.band, s.row_tiles - band * s.band);
-  t.col = u / rows;
-  t.row = band * s.band + u - t.col * rows;
-  return t;
-}
+// Whole tiles by number: for epilogues that need whole sums.
+struct ByNumber {
+  template <typename P>
+  __device__ static void range(const P&, const Shape& s, int worker, int workers, int& first, int& end, int& step) {
+    first = worker, end = s.units, step = workers;
+  }
+  template <typename P>
+  __device__ static Unit unit(const P&, const Shape& s, int u) {
+    const int per = s.band * s.col_tiles, band = u / per;
+    u -= band * per;
+    const int rows = min(s.band, s.row_tiles - band * s.band);
+    Unit t;
+    t.group = 0, t.slot = -1;
+    t.col = u / rows;
+    t.row = band * s.band + u - t.col * rows;
+    t.kb0 = 0, t.kb1 = s.kblocks;
+    return t;
+  }
+};
 
 __device__ __forceinline__ unsigned smem_u32(const void* p) {
   return static_cast<unsigned>(__cvta_generic_to_shared(p));
@@ -127,13 +140,40 @@ __device__ __forceinline__ bool bar_wait(unsigned long long* b, unsigned phase, 
 
 // Shared-memory descriptors, 128-byte swizzle.  K-major: 8 rows of 128 bytes
 // make a group.  Across K: 64 columns to a row of 128 bytes, a row for each k;
-// the next 64 columns lie a box further.
-__device__ __forceinline__ unsigned long long desc_k(unsigned at) {
-  return ((at >> 4) & 0x3FFFull) | (1ull << 16) | ((1024ull >> 4) << 32) | (1ull << 46) | (2ull << 61);
+// the next 64 columns lie a box further.  The upper word is the same for both; the lower
+// one has the address, and how far 16 elements of K are.
+constexpr unsigned DESC_UPPER = (1024u >> 4) | (1u << 14) | (2u << 29);
+template <bool TURNED>
+__device__ __forceinline__ unsigned desc_lower(unsigned at) {
+  return (at >> 4) | (TURNED ? static_cast<unsigned>(BOX >> 4) << 16 : 1u << 16);
 }
-__device__ __forceinline__ unsigned long long desc_turned(unsigned at) {
-  return ((at >> 4) & 0x3FFFull) | ((static_cast<unsigned long long>(BOX) >> 4) << 16) | ((1024ull >> 4) << 32) |
-         (1ull << 46) | (2ull << 61);
+template <bool TURNED>
+constexpr unsigned DESC_STEP = TURNED ? (16 * 128) >> 4 : 32 >> 4;
+
+template <int CTAS>
+__device__ __forceinline__ void mma(unsigned acc, unsigned p, unsigned q, unsigned idesc, unsigned more) {
+  if (CTAS == 1)
+    asm volatile(
+        "{\n .reg .pred p;\n .reg .b64 a, b;\n setp.ne.u32 p, %5, 0;\n mov.b64 a, {%1, %3};\n mov.b64 b, {%2, %3};\n"
+        " tcgen05.mma.cta_group::1.kind::f16 [%0], a, b, %4, p;\n}" ::"r"(acc),
+        "r"(p), "r"(q), "n"(DESC_UPPER), "r"(idesc), "r"(more)
+        : "memory");
+  else
+    asm volatile(
+        "{\n .reg .pred p;\n .reg .b64 a, b;\n setp.ne.u32 p, %5, 0;\n mov.b64 a, {%1, %3};\n mov.b64 b, {%2, %3};\n"
+        " tcgen05.mma.cta_group::2.kind::f16 [%0], a, b, %4, p;\n}" ::"r"(acc),
+        "r"(p), "r"(q), "n"(DESC_UPPER), "r"(idesc), "r"(more)
+        : "memory");
+}
+template <int CTAS>
+__device__ __forceinline__ void commit(unsigned bar) {
+  if (CTAS == 1)
+    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
+  else
+    asm volatile(
+        "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(bar),
+        "h"(static_cast<unsigned short>(3))
+        : "memory");
 }
 
 // 32 columns of the thread's row of an accumulator: the load, and the wait for it,
@@ -194,11 +234,33 @@ __device__ __forceinline__ float2 unpack2(unsigned w, int half) {
 // What a warp's epilogue knows of its tile: 32 rows from row0 on, of which the
 // thread's accumulator row is row0 + lane, and where it may keep 4 KB.
 struct Spot {
-  int lane, quad, part, row0, unit_col, group, split;
+  int lane, quad, part, row0, rank;
+  Unit unit;
+  int m, n;       // of the result
   int odd;        // every other tile of the block
   unsigned side;
-  bool dead;  // a wait ran out: results are NaNs
+  unsigned free_bar;  // to arrive at once the accumulator has been read
+  bool last;          // the warp's last chunk of the tile
+  bool dead;          // a wait ran out: results are NaNs
 };
+
+// The warp has read its part of the accumulator.  Relaxed: what is ordered is the
+// reads of tensor memory, by the fence; a release would wait for the warp's stores too.
+__device__ __forceinline__ void accumulator_read(const Spot& s) {
+  asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+  __syncwarp();
+  if (s.lane == 0 && !s.dead)
+    asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];" ::"r"(s.free_bar) : "memory");
+}
+// 32 columns of the warp's rows; the accumulator is given back with the last ones.
+__device__ __forceinline__ void take32(const Spot& s, unsigned acc, float (&v)[32]) {
+  tmem_ld32(acc, v);
+  if (s.last) accumulator_read(s);
+  if (s.dead) {
+#pragma unroll
+    for (int j = 0; j < 32; ++j) v[j] = __int_as_float(0x7fffffff);
+  }
+}
 
 // A warp's 32 x 32 values as 16-bit elements: each thread's row into shared
 // memory (64 bytes a row, 16-byte pieces exchanged so that neither direction meets
@@ -212,11 +274,13 @@ __device__ __forceinline__ void put16(const Spot& s, const unsigned (&w)[16], un
   __syncwarp();
   if (vec && col0 + CHUNK <= n) {
     const int p = s.lane & 3;
+    unsigned short* to = out + (s.row0 + (s.lane >> 2)) * ld + col0 + p * 8;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       const int r = i * 8 + (s.lane >> 2);
       const uint4 x = lds128(s.side + r * 64 + ((p ^ ((r >> 1) & 3)) << 4));
-      if (s.row0 + r < m) *reinterpret_cast<uint4*>(out + (s.row0 + r) * ld + col0 + p * 8) = x;
+      if (s.row0 + r < m) *reinterpret_cast<uint4*>(to) = x;
+      to += 8 * ld;
     }
   } else {  // a column a lane
     const int col = col0 + s.lane, p = s.lane >> 3;
@@ -265,11 +329,13 @@ __device__ __forceinline__ void put32(const Spot& s, const float (&v)[32], float
   stage32(s, v);
   if (vec && col0 + CHUNK <= n) {
     const int q = s.lane & 7;
+    float* to = out + (s.row0 + (s.lane >> 3)) * ld + col0 + q * 4;
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
       const int r = i * 4 + (s.lane >> 3);
       const float4 x = staged(s, r, q);
-      if (s.row0 + r < m) *reinterpret_cast<float4*>(out + (s.row0 + r) * ld + col0 + q * 4) = x;
+      if (s.row0 + r < m) *reinterpret_cast<float4*>(to) = x;
+      to += 4 * ld;
     }
   } else {  // a column a lane
     const int col = col0 + s.lane;
@@ -280,19 +346,30 @@ __device__ __forceinline__ void put32(const Spot& s, const float (&v)[32], float
 
 // ------------------------------------------------------------------ the kernel
 
-// EPI: static constexpr bool DUAL (B's tiles hold half their columns of each of
-// two operands); Params; a State that is constructed for a tile (loads that need
-// no accumulator), whose chunk() takes 32 columns, and whose end() all warps call.
+// A place among the stages, the phase of its barriers, and whether it has been used before.
+template <int STAGES>
+struct Ring {
+  int i = 0;
+  unsigned phase = 0, again = 0;
+  __device__ __forceinline__ void next() {
+    if (++i == STAGES) i = 0, phase ^= 1, again = 1;
+  }
+};
+
+// EPI: DUAL (B's tiles hold half their columns of each of two operands), WARPS,
+// SIDE; Params; Units; a State that is constructed for a tile (loads that need no
+// accumulator), whose chunk() takes 32 columns, and whose end() all warps call.
 template <typename TILE, typename EPI>
-__global__ void __launch_bounds__(THREADS, 1)
+__global__ void __launch_bounds__(TILE::THREADS, 1)
     gemm_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Shape a,
                 const __grid_constant__ typename EPI::Params params) {
   constexpr int CTAS = TILE::CTAS, BN = TILE::BN, STAGES = TILE::STAGES;
   constexpr int COLS = EPI::DUAL ? BN / 2 : BN;  // columns of the result
+  constexpr int PARTS = EPI::WARPS / 4;          // warps that share 32 rows, each with its share of the chunks
   extern __shared__ __align__(1024) unsigned char raw[];
   unsigned char* smem = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~uintptr_t(1023));
   unsigned char* side = smem + STAGES * TILE::STAGE;
-  unsigned long long* full = reinterpret_cast<unsigned long long*>(side + EPI_WARPS * SIDE);
+  unsigned long long* full = reinterpret_cast<unsigned long long*>(side + TILE::SIDES);
   unsigned long long* empty = full + STAGES;
   unsigned long long* acc_full = empty + STAGES;
   unsigned long long* acc_empty = acc_full + 2;
@@ -300,7 +377,8 @@ __global__ void __launch_bounds__(THREADS, 1)
   volatile int* gave_up = reinterpret_cast<volatile int*>(tmem_slot + 1);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int rank = CTAS == 1 ? 0 : blockIdx.x & 1;
-  const int first = blockIdx.x / CTAS, stride = gridDim.x / CTAS;
+  int first, end, step;
+  EPI::Units::range(params, a, blockIdx.x / CTAS, gridDim.x / CTAS, first, end, step);
 
   if (threadIdx.x == 0) {
     for (int i = 0; i < STAGES; ++i) {
@@ -309,7 +387,7 @@ __global__ void __launch_bounds__(THREADS, 1)
     }
     for (int i = 0; i < 2; ++i) {
       asm volatile("mbarrier.init.shared::cta.b64 [%0], 1;" ::"r"(smem_u32(&acc_full[i])));
-      asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(smem_u32(&acc_empty[i])), "r"(CTAS * EPI_WARPS));
+      asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(smem_u32(&acc_empty[i])), "r"(CTAS * EPI::WARPS));
     }
     *gave_up = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -341,126 +419,115 @@ __global__ void __launch_bounds__(THREADS, 1)
     if (lane == 0) {  // operands
       // what earlier kernels wrote is read through the async proxy
       asm volatile("fence.proxy.async.global;" ::: "memory");
-      int n = 0;  // stages used so far
-      bool stop = false;
-      for (int u = first; u < a.units && !stop; u += stride) {
-        const Unit t = unit_of(a, u);
-        const int kb0 = t.split * a.per_split, kb1 = min(a.kblocks, kb0 + a.per_split);
+      Ring<TILE::STAGES> ring;
+      const unsigned leader = CTAS == 2 ? in_block(smem_u32(full), 0) : smem_u32(full);
+      auto load = [&](const CUtensorMap* map, unsigned to, unsigned bar, int x0, int y0) {
+        if (CTAS == 1)
+          asm volatile(
+              "cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], [%2];" ::"r"(
+                  to),
+              "l"(reinterpret_cast<unsigned long long>(map)), "r"(bar), "r"(x0), "r"(y0)
+              : "memory");
+        else
+          asm volatile(
+              "cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], "
+              "[%1, {%3, %4}], [%2];" ::"r"(to),
+              "l"(reinterpret_cast<unsigned long long>(map)), "r"(bar), "r"(x0), "r"(y0)
+              : "memory");
+      };
+      for (int u = first; u < end; u += step) {
+        const Unit t = EPI::Units::unit(params, a, u);
+        const Group g = a.group[t.group];
         const int p0 = t.row * TILE::M + rank * 128;
         const int q0 = EPI::DUAL ? t.col * COLS : t.col * BN + rank * TILE::QN;
-        for (int kb = kb0; kb < kb1; ++kb, ++n) {
-          const int i = n % STAGES;
-          if (n >= STAGES && !bar_wait(&empty[i], (n / STAGES - 1) & 1, gave_up)) {
-            *gave_up = 1;
-            stop = true;
-            break;
-          }
-          const unsigned st = smem_u32(smem) + i * TILE::STAGE;
-          unsigned bar = smem_u32(&full[i]);
-          if (rank == 0)
-            asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(CTAS * TILE::STAGE)
-                         : "memory");
-          if (CTAS == 2) bar = in_block(bar, 0);
-          auto load = [&](const CUtensorMap* map, unsigned to, int x0, int y0) {
-            if (CTAS == 1)
-              asm volatile(
-                  "cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], "
-                  "[%2];" ::"r"(to),
-                  "l"(reinterpret_cast<unsigned long long>(map)), "r"(bar), "r"(x0), "r"(y0)
-                  : "memory");
-            else
-              asm volatile(
-                  "cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], "
-                  "[%1, {%3, %4}], [%2];" ::"r"(to),
-                  "l"(reinterpret_cast<unsigned long long>(map)), "r"(bar), "r"(x0), "r"(y0)
-                  : "memory");
-          };
-          const int second = kb >= a.kblocks0;
-          const int k0 = (second ? kb - a.kblocks0 : kb) * BK, which = t.group + second;
-          const CUtensorMap *pa = &maps.a[which], *pb = &maps.b[which];
-          if (a.a_turned) {
+        // a run of stages with the same operands
+        auto run = [&](auto a_turned, auto b_turned, const CUtensorMap* pa, const CUtensorMap* pb, int kb0, int kb1) {
+          constexpr bool AT = decltype(a_turned)::value, BT = decltype(b_turned)::value;
+          int k0 = kb0 * BK;
+          for (int left = kb1 - kb0; left > 0; --left, ring.next(), k0 += BK) {
+            if (ring.again && !bar_wait(&empty[ring.i], ring.phase ^ 1, gave_up)) return false;
+            const unsigned st = smem_u32(smem) + ring.i * TILE::STAGE, sq = st + TILE::P_BYTES, bar = leader + ring.i * 8;
+            if (rank == 0)
+              asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(smem_u32(&full[ring.i])),
+                           "r"(CTAS * TILE::STAGE)
+                           : "memory");
+            if (AT) {
 #pragma unroll
-            for (int h = 0; h < 2; ++h) load(pa, st + h * BOX, p0 + h * 64, k0);
-          } else {
-            load(pa, st, k0, p0);
-          }
-          const unsigned sq = st + TILE::P_BYTES;
-          if (EPI::DUAL) {
-            if (CTAS == 2) {
-              load(&maps.b[rank], sq, k0, q0);
+              for (int h = 0; h < 2; ++h) load(pa, st + h * BOX, bar, p0 + h * 64, k0);
             } else {
-              load(&maps.b[0], sq, k0, q0);
-              load(&maps.b[1], sq + TILE::Q_BYTES / 2, k0, q0);
+              load(pa, st, bar, k0, p0);
             }
-          } else if (a.b_turned) {
+            if (EPI::DUAL) {
+              if (CTAS == 2) {
+                load(pb + rank, sq, bar, k0, q0);
+              } else {
+                load(pb, sq, bar, k0, q0);
+                load(pb + 1, sq + TILE::Q_BYTES / 2, bar, k0, q0);
+              }
+            } else if (BT) {
 #pragma unroll
-            for (int h = 0; h < TILE::QN / 64; ++h) load(pb, sq + h * BOX, q0 + h * 64, k0);
-          } else {
-            load(pb, sq, k0, q0);
+              for (int h = 0; h < TILE::QN / 64; ++h) load(pb, sq + h * BOX, bar, q0 + h * 64, k0);
+            } else {
+              load(pb, sq, bar, k0, q0);
+            }
           }
+          return true;
+        };
+        auto both = [&](const CUtensorMap* pa, const CUtensorMap* pb, int kb0, int kb1) {
+          const std::true_type yes;
+          const std::false_type no;
+          return g.a_turned ? (g.b_turned ? run(yes, yes, pa, pb, kb0, kb1) : run(yes, no, pa, pb, kb0, kb1))
+                            : (g.b_turned ? run(no, yes, pa, pb, kb0, kb1) : run(no, no, pa, pb, kb0, kb1));
+        };
+        const int turn = g.kblocks0;
+        if (!both(&maps.a[g.map], &maps.b[g.map], t.kb0, min(t.kb1, turn)) ||
+            (t.kb1 > turn && !both(&maps.a[g.map + 1], &maps.b[g.map + 1], max(t.kb0 - turn, 0), t.kb1 - turn))) {
+          *gave_up = 1;
+          break;
         }
       }
     }
   } else if (warp == 1) {
     if (lane == 0 && rank == 0) {  // products
-      // D in 32 bits; operand types (bf16: 1) in bits 7 and 10; across K: bits 15 and 16
-      const unsigned idesc = (1u << 4) | (a.half ? 0u : (1u << 7) | (1u << 10)) | (a.a_turned ? 1u << 15 : 0u) |
-                             (a.b_turned ? 1u << 16 : 0u) | (static_cast<unsigned>(BN >> 3) << 17) |
-                             (static_cast<unsigned>(TILE::M >> 4) << 24);
-      const unsigned long long p_step = a.a_turned ? (16 * 128) >> 4 : 32 >> 4;
-      const unsigned long long q_step = a.b_turned ? (16 * 128) >> 4 : 32 >> 4;
-      int n = 0, c = 0;  // stages, accumulators used so far
-      bool stop = false;
-      for (int u = first; u < a.units && !stop; u += stride, ++c) {
-        const Unit t = unit_of(a, u);
-        const int kb0 = t.split * a.per_split, kb1 = min(a.kblocks, kb0 + a.per_split);
+      Ring<TILE::STAGES> ring;
+      int c = 0;  // accumulators used so far
+      for (int u = first; u < end; u += step, ++c) {
+        const Unit t = EPI::Units::unit(params, a, u);
         if (c >= 2 && !bar_wait(&acc_empty[c & 1], (c / 2 - 1) & 1, gave_up)) {
           *gave_up = 1;
           break;
         }
         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
         const unsigned acc = tmem + (c & 1) * BN;
-        for (int kb = kb0; kb < kb1; ++kb, ++n) {
-          const int i = n % STAGES;
-          if (!bar_wait(&full[i], (n / STAGES) & 1, gave_up)) {
-            *gave_up = 1;
-            stop = true;
-            break;
-          }
-          asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-          const unsigned st = smem_u32(smem) + i * TILE::STAGE;
-          const unsigned long long pd = a.a_turned ? desc_turned(st) : desc_k(st);
-          const unsigned long long qd = a.b_turned ? desc_turned(st + TILE::P_BYTES) : desc_k(st + TILE::P_BYTES);
+        const Group& g = a.group[t.group];
+        auto tile = [&](auto a_turned, auto b_turned) {
+          constexpr bool AT = decltype(a_turned)::value, BT = decltype(b_turned)::value;
+          // D in 32 bits; operand types (bf16: 1) in bits 7 and 10; across K: bits 15 and 16
+          const unsigned idesc = (1u << 4) | (a.half ? 0u : (1u << 7) | (1u << 10)) | (AT ? 1u << 15 : 0u) |
+                                 (BT ? 1u << 16 : 0u) | (static_cast<unsigned>(BN >> 3) << 17) |
+                                 (static_cast<unsigned>(TILE::M >> 4) << 24);
+          unsigned more = 0;
+          for (int left = t.kb1 - t.kb0; left > 0; --left, ring.next()) {
+            if (!bar_wait(&full[ring.i], ring.phase, gave_up)) return false;
+            asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+            const unsigned st = smem_u32(smem) + ring.i * TILE::STAGE;
+            const unsigned p = desc_lower<AT>(st), q = desc_lower<BT>(st + TILE::P_BYTES);
 #pragma unroll
-          for (int k = 0; k < BK / 16; ++k) {
-            const unsigned more = (kb > kb0 || k > 0) ? 1u : 0u;
-            if (CTAS == 1)
-              asm volatile(
-                  "{\n .reg .pred p;\n setp.ne.u32 p, %4, 0;\n"
-                  " tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}" ::"r"(acc),
-                  "l"(pd + k * p_step), "l"(qd + k * q_step), "r"(idesc), "r"(more)
-                  : "memory");
-            else
-              asm volatile(
-                  "{\n .reg .pred p;\n setp.ne.u32 p, %4, 0;\n"
-                  " tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n}" ::"r"(acc),
-                  "l"(pd + k * p_step), "l"(qd + k * q_step), "r"(idesc), "r"(more)
-                  : "memory");
+            for (int k = 0; k < BK / 16; ++k) {
+              mma<CTAS>(acc, p + k * DESC_STEP<AT>, q + k * DESC_STEP<BT>, idesc, more);
+              more = 1;
+            }
+            commit<CTAS>(smem_u32(&empty[ring.i]));
           }
-          auto commit = [&](unsigned long long* bar) {
-            if (CTAS == 1)
-              asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(
-                               smem_u32(bar))
-                           : "memory");
-            else
-              asm volatile(
-                  "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], "
-                  "%1;" ::"r"(smem_u32(bar)),
-                  "h"(static_cast<unsigned short>(3))
-                  : "memory");
-          };
-          commit(&empty[i]);
-          if (kb + 1 == kb1) commit(&acc_full[c & 1]);
+          commit<CTAS>(smem_u32(&acc_full[c & 1]));
+          return true;
+        };
+        const std::true_type yes;
+        const std::false_type no;
+        const bool fine = g.a_turned ? (g.b_turned ? tile(yes, yes) : tile(yes, no)) : g.b_turned ? tile(no, yes) : tile(no, no);
+        if (!fine) {
+          *gave_up = 1;
+          break;
         }
       }
     }
@@ -468,14 +535,15 @@ __global__ void __launch_bounds__(THREADS, 1)
     const int quad = warp & 3, part = (warp - 2) >> 2;  // 32 rows; which of their chunks
     Spot s;
     s.lane = lane, s.quad = quad, s.part = part;
-    s.side = smem_u32(side) + (warp - 2) * SIDE;
+    s.side = smem_u32(side) + (warp - 2) * EPI::SIDE;
+    s.rank = rank;
     s.dead = false;
     int c = 0;
-    for (int u = first; u < a.units; u += stride, ++c) {
-      const Unit t = unit_of(a, u);
+    for (int u = first; u < end; u += step, ++c) {
+      const Unit t = EPI::Units::unit(params, a, u);
       s.row0 = t.row * TILE::M + rank * 128 + quad * 32;
-      s.unit_col = t.col, s.group = t.group, s.split = t.split;
-      const int chunks = (min(COLS, a.n - t.col * COLS) + CHUNK - 1) / CHUNK;
+      s.unit = t, s.m = a.group[t.group].m, s.n = a.group[t.group].n;
+      const int chunks = (min(COLS, s.n - t.col * COLS) + CHUNK - 1) / CHUNK;
       typename EPI::State e(params, a, s);
       if (!s.dead && !bar_wait(&acc_full[c & 1], (c / 2) & 1, gave_up)) {
         s.dead = true;
@@ -483,14 +551,15 @@ __global__ void __launch_bounds__(THREADS, 1)
       }
       asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
       const unsigned acc = tmem + (static_cast<unsigned>(quad * 32) << 16) + (c & 1) * BN;
-      // a warp without a row of the result still has to say that it is done
-      if (s.row0 < a.m)
-        for (int ch = part; ch < chunks; ch += PARTS) e.chunk(params, a, s, t.col * COLS + ch * CHUNK, acc + ch * CHUNK, COLS);
-      asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
-      __syncwarp();
-      if (lane == 0 && !s.dead) {  // the accumulator is free
-        const unsigned bar = CTAS == 1 ? smem_u32(&acc_empty[c & 1]) : in_block(smem_u32(&acc_empty[c & 1]), 0);
-        asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
+      s.free_bar = CTAS == 1 ? smem_u32(&acc_empty[c & 1]) : in_block(smem_u32(&acc_empty[c & 1]), 0);
+      // a warp without a row of the result, or a chunk of it, still has to say that it is done
+      if (s.row0 < s.m && part < chunks) {
+        for (int ch = part; ch < chunks; ch += PARTS) {
+          s.last = ch + PARTS >= chunks;
+          e.chunk(params, a, s, t.col * COLS + ch * CHUNK, acc + ch * CHUNK, COLS);
+        }
+      } else {
+        accumulator_read(s);
       }
       s.odd = c & 1;
       e.end(params, a, s);
@@ -531,131 +600,151 @@ inline bool tma_ready(const void* p, long long ld, long long rows) {
 inline long long round_up(long long x, long long to) { return (x + to - 1) / to * to; }
 inline size_t room(size_t bytes) { return (bytes + 255) / 256 * 256; }
 
+// A product C = A B^T of 16-bit operands: m x n over k.
 struct Problem {
-  int device, half;
   long long m, n, k, k0;  // k0: K of the first operands when there are two in a row (else k)
-  int groups;             // products of one shape in one launch
   bool a_turned, b_turned;
-  Mat a[MAX_GROUPS], b[MAX_GROUPS];
+  Mat a[2], b[2];
+};
+struct Device {
+  int device, sms;
 };
 
-// How a problem is laid out over the device: the tile with the smallest estimated
-// time, from measured costs of 64 elements of K (a pair of blocks on 256 x 256: 0.45
-// us, single blocks on 128 x 128: 0.47 and 128 x 64: 0.40, all of them L2's rate) and
-// 4 us for a product's start and its last epilogue; each tile is a wave's part.  A
-// split costs its partial sums' way to memory and back at 4 TB/s, and a launch of 4 us.
-struct Plan {
-  int tile;  // 0: 2 x 256, 1: 128, 2: 64
-  int splits;
+// The three tilings: rows and columns, blocks, and measured us for 64 elements of K
+// (with the clocks that large products leave).
+struct Tiling {
+  int m, n, ctas;
   double us;
 };
-inline Plan plan_for(long long m, long long n, long long kblocks, int groups, bool dual, bool may_split, int sms) {
-  struct { int m, n, workers; double us; } const tiles[3] = {{256, 256, sms / 2, 0.45}, {128, 128, sms, 0.47}, {128, 64, sms, 0.40}};
-  Plan best = {0, 1, 1e30};
+constexpr Tiling TILINGS[3] = {{256, 256, 2, 0.43}, {128, 128, 1, 0.47}, {128, 64, 1, 0.40}};
+
+inline int kblocks_of(const Problem& p) { return static_cast<int>((p.k0 + BK - 1) / BK + (p.k - p.k0 + BK - 1) / BK); }
+
+// The tiling for whole tiles: the one whose rounds take least.
+inline int tiling_for(long long m, long long n, long long kblocks, bool dual, int sms) {
+  int best = 0;
+  double least = 1e30;
   for (int i = 0; i < 3; ++i) {
-    const int cols = dual ? tiles[i].n / 2 : tiles[i].n;
-    const long long count = groups * ((m + tiles[i].m - 1) / tiles[i].m) * ((n + cols - 1) / cols);
-    for (int s = 1; s <= (may_split ? 16 : 1); ++s) {
-      const long long per = (kblocks + s - 1) / s;
-      if (s > 1 && (per < 8 || (kblocks + per - 1) / per != s)) continue;
-      const double rounds = static_cast<double>((count * s + tiles[i].workers - 1) / tiles[i].workers);
-      double us = rounds * per * tiles[i].us + 4.0;
-      if (s > 1) us += 4.0 + 8e-6 * s * groups * static_cast<double>(m) * n / 4.0;
-      if (us < best.us * 0.97) best = {i, s, us};
-    }
+    const Tiling& t = TILINGS[i];
+    const int cols = dual ? t.n / 2 : t.n, workers = sms / t.ctas;
+    const long long count = ((m + t.m - 1) / t.m) * ((n + cols - 1) / cols);
+    const double us = static_cast<double>((count + workers - 1) / workers) * kblocks * t.us + 4.0;
+    if (us < least * 0.97) best = i, least = us;
   }
   return best;
 }
 
-template <typename TILE, typename EPI>
-cudaError_t start_tile(const Problem& p, Shape s, const typename EPI::Params& params, int sms, cudaStream_t st, int* bad) {
-  Maps maps = {};
-  const int cols = EPI::DUAL ? TILE::BN / 2 : TILE::BN;
-  s.row_tiles = static_cast<int>((p.m + TILE::M - 1) / TILE::M);
-  s.col_tiles = static_cast<int>((p.n + cols - 1) / cols);
-  // about as many rows as columns under way at a time
-  s.band = TILE::M == 256 ? 8 : 16;
-  const long long units = static_cast<long long>(s.row_tiles) * s.col_tiles * s.groups * s.splits;
-  *bad = units > 0x3fffffffll ? fail("too many tiles in one product") : 0;
-  s.units = static_cast<int>(units);
-  const int operands = EPI::DUAL ? 2 : std::max(s.groups, s.kblocks0 < s.kblocks ? 2 : 1);
-  for (int i = 0; i < operands && !*bad; ++i) {
-    const long long k = s.kblocks0 == s.kblocks ? p.k : i ? p.k - p.k0 : p.k0;
-    if (!EPI::DUAL || i == 0)
-      *bad |= p.a_turned ? ad_b200_internal::tmap_2d_16(p.a[i].p, k, p.m, p.a[i].ld, 64, 64, &maps.a[i])
-                         : ad_b200_internal::tmap_2d_16(p.a[i].p, p.m, k, p.a[i].ld, 128, 64, &maps.a[i]);
-    const int rows = EPI::DUAL && TILE::CTAS == 1 ? TILE::QN / 2 : TILE::QN;
-    *bad |= p.b_turned ? ad_b200_internal::tmap_2d_16(p.b[i].p, k, p.n, p.b[i].ld, 64, 64, &maps.b[i])
-                       : ad_b200_internal::tmap_2d_16(p.b[i].p, p.n, k, p.b[i].ld, rows, 64, &maps.b[i]);
+// Maps of a group's operands, at `map` of them.  1 with an error set.
+template <typename TILE, bool DUAL>
+int make_maps(const Problem& p, Maps& maps, int map) {
+  const int operands = DUAL || p.k0 < p.k ? 2 : 1;
+  for (int i = 0; i < operands; ++i) {
+    const long long k = DUAL || p.k0 == p.k ? p.k : i ? p.k - p.k0 : p.k0;
+    if (!DUAL || i == 0) {
+      if (p.a_turned ? ad_b200_internal::tmap_2d_16(p.a[i].p, k, p.m, p.a[i].ld, 64, 64, &maps.a[map + i])
+                     : ad_b200_internal::tmap_2d_16(p.a[i].p, p.m, k, p.a[i].ld, 128, 64, &maps.a[map + i]))
+        return 1;
+    }
+    const int rows = DUAL && TILE::CTAS == 1 ? TILE::QN / 2 : TILE::QN;
+    if (p.b_turned ? ad_b200_internal::tmap_2d_16(p.b[i].p, k, p.n, p.b[i].ld, 64, 64, &maps.b[map + i])
+                   : ad_b200_internal::tmap_2d_16(p.b[i].p, p.n, k, p.b[i].ld, rows, 64, &maps.b[map + i]))
+      return 1;
   }
-  if (*bad) return cudaSuccess;
+  return 0;
+}
+inline Group group_of(const Problem& p, int map) {
+  return {static_cast<int>(p.m), static_cast<int>(p.n), static_cast<int>((p.k0 + BK - 1) / BK), p.a_turned, p.b_turned, map};
+}
+
+// Blocks or pairs of them at a time: more would start when others have ended, with
+// a whole share of the units each.
+template <typename TILE, typename EPI>
+cudaError_t workers_of(const Device& d, int* workers) {
+  static std::atomic<int> known[64];
+  if (d.device < 64 && (*workers = known[d.device])) return cudaSuccess;
   int room = 0;
   cudaError_t e = shared_room<gemm_kernel<TILE, EPI>>(&room);
   if (e != cudaSuccess) return e;
   if (room < TILE::SMEM) return cudaErrorInvalidConfiguration;
   cudaLaunchConfig_t c = {};
-  c.blockDim = dim3(THREADS);
-  c.dynamicSmemBytes = TILE::SMEM;
-  c.stream = st;
   cudaLaunchAttribute at[1];
   at[0].id = cudaLaunchAttributeClusterDimension;
   at[0].val.clusterDim.x = TILE::CTAS;
   at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
-  c.attrs = at;
-  c.numAttrs = 1;
-  // blocks or pairs of them at a time: more would start when others have ended, with a whole share of the units each
-  static std::atomic<int> resident[64];
-  int workers = p.device < 64 ? resident[p.device].load() : 0;
-  if (!workers) {
-    c.gridDim = dim3(sms / TILE::CTAS * TILE::CTAS);
-    e = cudaOccupancyMaxActiveClusters(&workers, gemm_kernel<TILE, EPI>, &c);
-    if (e != cudaSuccess) return e;
-    workers = std::max(1, std::min(workers, sms / TILE::CTAS));
-    if (p.device < 64) resident[p.device] = workers;
-  }
-  c.gridDim = dim3(std::min(s.units, workers) * TILE::CTAS);
+  c.gridDim = dim3(d.sms / TILE::CTAS * TILE::CTAS);
+  c.blockDim = dim3(TILE::THREADS);
+  c.dynamicSmemBytes = TILE::SMEM;
+  c.attrs = at, c.numAttrs = 1;
+  e = cudaOccupancyMaxActiveClusters(workers, gemm_kernel<TILE, EPI>, &c);
+  if (e != cudaSuccess) return e;
+  *workers = std::max(1, std::min(*workers, d.sms / TILE::CTAS));
+  if (d.device < 64) known[d.device] = *workers;
+  return cudaSuccess;
+}
+
+template <typename TILE, typename EPI>
+cudaError_t launch_gemm(const Maps& maps, const Shape& s, const typename EPI::Params& params, int workers, cudaStream_t st) {
+  cudaLaunchConfig_t c = {};
+  cudaLaunchAttribute at[1];
+  at[0].id = cudaLaunchAttributeClusterDimension;
+  at[0].val.clusterDim.x = TILE::CTAS;
+  at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
+  c.gridDim = dim3(workers * TILE::CTAS);
+  c.blockDim = dim3(TILE::THREADS);
+  c.dynamicSmemBytes = TILE::SMEM;
+  c.stream = st;
+  c.attrs = at, c.numAttrs = 1;
   return cudaLaunchKernelEx(&c, gemm_kernel<TILE, EPI>, maps, s, params);
 }
 
-// Launches a problem under a plan.  0, or 1 with an error set.
-template <typename EPI>
-int start(const char* who, const Problem& p, const Plan& plan, const typename EPI::Params& params, int sms, cudaStream_t st) {
+template <typename TILE, typename EPI>
+int start_tile(const char* who, const Device& d, const Problem& p, int half, const typename EPI::Params& params, cudaStream_t st) {
+  Maps maps = {};
   Shape s = {};
-  s.m = static_cast<int>(p.m), s.n = static_cast<int>(p.n);
-  s.kblocks0 = static_cast<int>((p.k0 + BK - 1) / BK);
-  s.kblocks = s.kblocks0 + static_cast<int>((p.k - p.k0 + BK - 1) / BK);
-  s.groups = p.groups;
-  s.per_split = (s.kblocks + plan.splits - 1) / plan.splits;
-  s.splits = (s.kblocks + s.per_split - 1) / s.per_split;  // none without a share: nothing would end its wait
-  s.a_turned = p.a_turned, s.b_turned = p.b_turned, s.half = p.half;
-  int bad = 0;
-  cudaError_t e = plan.tile == 0   ? start_tile<Tile<2, 256>, EPI>(p, s, params, sms, st, &bad)
-                  : plan.tile == 1 ? start_tile<Tile<1, 128>, EPI>(p, s, params, sms, st, &bad)
-                                   : start_tile<Tile<1, 64>, EPI>(p, s, params, sms, st, &bad);
-  if (bad) return 1;
-  if (e != cudaSuccess) return fail_cuda(who, e);
-  return 0;
+  const int cols = EPI::DUAL ? TILE::BN / 2 : TILE::BN;
+  s.group[0] = group_of(p, 0);
+  s.half = half;
+  s.kblocks = kblocks_of(p);
+  s.row_tiles = static_cast<int>((p.m + TILE::M - 1) / TILE::M);
+  s.col_tiles = static_cast<int>((p.n + cols - 1) / cols);
+  // about as many rows as columns under way at a time
+  s.band = TILE::M == 256 ? 8 : 16;
+  const long long units = static_cast<long long>(s.row_tiles) * s.col_tiles;
+  if (units > 0x3fffffffll) return fail("%s: too many tiles in one product", who);
+  s.units = static_cast<int>(units);
+  if (make_maps<TILE, EPI::DUAL>(p, maps, 0)) return 1;
+  int workers = 0;
+  cudaError_t e = workers_of<TILE, EPI>(d, &workers);
+  if (e == cudaSuccess) e = launch_gemm<TILE, EPI>(maps, s, params, std::min(workers, s.units), st);
+  return e == cudaSuccess ? 0 : fail_cuda(who, e);
+}
+
+// Launches a product with an epilogue.  0, or 1 with an error set.
+template <typename EPI>
+int start(const char* who, const Device& d, const Problem& p, int half, int tiling, const typename EPI::Params& params,
+          cudaStream_t st) {
+  return tiling == 0   ? start_tile<Tile<2, 256, EPI>, EPI>(who, d, p, half, params, st)
+         : tiling == 1 ? start_tile<Tile<1, 128, EPI>, EPI>(who, d, p, half, params, st)
+                       : start_tile<Tile<1, 64, EPI>, EPI>(who, d, p, half, params, st);
 }
 
 // ------------------------------------------------------------------ products to memory (gemm16.cu)
 
-// A result: m x n of a type (AD_F32 or the operands'), added to what it holds
-// when `accumulate`.
-struct Out {
+// result = alpha (product + addend) + (accumulate ? result : 0)
+struct Result {
   void* p;
   long long ld;
+  int type;  // AD_F32 or the operands'
+  bool accumulate;
+  const float* addend;  // of the result's shape, in 32 bits; NULL: none.  May be the result itself
+  long long ld_addend;
+  const float* alpha;  // device memory; NULL: 1
 };
-// The products of a problem, times *alpha (device memory; NULL: 1), to out[group].
-// `partial`: at least partial_bytes() of memory, 16-byte aligned.  With `sums`, a
-// first or later part of a sum over products (one group): the partial sums stay in
-// `partial` and only the `last` part's call writes the result.
-struct Sums {
-  bool first, last;
-};
-Plan store_plan(const Problem& p, int sms);
-size_t partial_bytes(const Problem& p, const Plan& plan, bool sums);
-int store_product(const char* who, const Problem& p, const Plan& plan, int type, const Out* out, bool accumulate,
-                  const float* alpha, float* partial, const Sums* sums, int sms, cudaStream_t st);
+// Up to MAX_GROUPS products in one go, independent of one another.  `partial`:
+// partial_bytes() of memory, 16-byte aligned.
+size_t partial_bytes(const Device& d);
+int store_products(const char* who, const Device& d, int half, const Problem* p, const Result* r, int count, float* partial,
+                   cudaStream_t st);
 // A copy of a 16-bit matrix whose rows TMA can read.
 int pack_rows(const char* who, const void* p, long long ld, long long rows, long long cols, void* to, long long ld_to,
               cudaStream_t st);

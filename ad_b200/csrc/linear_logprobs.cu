@@ -39,6 +39,8 @@ __device__ __forceinline__ long long token_at(const void* tokens, int tok64, lon
 // A row's largest logit and the sum of exponents from there, over a tile's columns.
 struct Sum {
   static constexpr bool DUAL = false;
+  static constexpr int WARPS = 8, SIDE = 512;
+  using Units = ByNumber;
   struct Params {
     float2* part;   // [column tiles][rows]
     float* target;  // [rows]
@@ -49,21 +51,21 @@ struct Sum {
   struct State {
     float top, sum;
     int token;  // -1: not in reach
-    __device__ State(const Params& p, const Shape& a, const Spot& s) {
+    __device__ State(const Params& p, const Shape&, const Spot& s) {
       top = -INFINITY, sum = 0.0f, token = -1;
       const int row = s.row0 + s.lane;
-      if (row < a.m) {
+      if (row < s.m) {
         const long long t = token_at(p.tokens, p.tok64, row);
-        if (t >= 0 && t < a.n) token = static_cast<int>(t);
+        if (t >= 0 && t < s.n) token = static_cast<int>(t);
       }
     }
-    __device__ void chunk(const Params& p, const Shape& a, const Spot& s, int col0, unsigned acc, int) {
+    __device__ void chunk(const Params& p, const Shape&, const Spot& s, int col0, unsigned acc, int) {
       float v[32];
-      tmem_ld32(acc, v);
-      if (col0 + CHUNK > a.n) {
+      take32(s, acc, v);
+      if (col0 + CHUNK > s.n) {
 #pragma unroll
         for (int j = 0; j < 32; ++j)
-          if (col0 + j >= a.n) v[j] = -INFINITY;
+          if (col0 + j >= s.n) v[j] = -INFINITY;
       }
       const unsigned at = static_cast<unsigned>(token - col0);
       if (__any_sync(0xffffffffu, at < 32u)) {
@@ -85,9 +87,10 @@ struct Sum {
       sum = sum * ex2((top - from) * p.k) + ((part[0] + part[1]) + (part[2] + part[3]));
       top = most;
     }
-    // The four warps of 32 rows join their pairs.  A warp's place for them is
+    static constexpr int PARTS = WARPS / 4;
+    // The warps of the same 32 rows join their pairs.  A warp's place for them is
     // used again two tiles later, when all have met once more.
-    __device__ void end(const Params& p, const Shape& a, const Spot& s) {
+    __device__ void end(const Params& p, const Shape&, const Spot& s) {
       const int row = s.row0 + s.lane;
       if (s.dead) sum = __int_as_float(0x7fffffff);
       const unsigned at = s.side + s.odd * 256 + s.lane * 8;
@@ -102,7 +105,7 @@ struct Sum {
         sum = sum * ex2((top - from) * p.k) + u * ex2((t - from) * p.k);
         top = most;
       }
-      if (row < a.m) p.part[static_cast<long long>(s.unit_col) * a.m + row] = make_float2(top, sum);
+      if (row < s.m) p.part[static_cast<long long>(s.unit.col) * s.m + row] = make_float2(top, sum);
     }
   };
 };
@@ -179,6 +182,8 @@ __global__ void __launch_bounds__(1024) range_kernel(const __grid_constant__ Ran
 // dz of a piece of the vocabulary.
 struct Slope {
   static constexpr bool DUAL = false;
+  static constexpr int WARPS = 16, SIDE = 2048;
+  using Units = ByNumber;
   struct Params {
     const float2* stats;
     const void* tokens;
@@ -193,10 +198,10 @@ struct Slope {
   struct State {
     float top, of_p, of_hot;
     int hot;  // the token's column in the piece
-    __device__ State(const Params& p, const Shape& a, const Spot& s) {
+    __device__ State(const Params& p, const Shape&, const Spot& s) {
       top = 0.0f, of_p = 0.0f, of_hot = 0.0f, hot = -1;
       const int row = s.row0 + s.lane;
-      if (row >= a.m) return;
+      if (row >= s.m) return;
       const float2 st = p.stats[row];
       const long long t = token_at(p.tokens, p.tok64, row);
       const float f = p.factor ? *p.factor : 1.0f;
@@ -204,13 +209,13 @@ struct Slope {
       top = st.x;
       of_p = t >= p.vocab ? __int_as_float(0x7fffffff) : p.scale * (gl - gp) * f / st.y;
       of_hot = p.scale * gp * f;
-      if (t >= p.first && t < p.first + a.n) hot = static_cast<int>(t - p.first);
+      if (t >= p.first && t < p.first + s.n) hot = static_cast<int>(t - p.first);
     }
     __device__ void chunk(const Params& p, const Shape& a, const Spot& s, int col0, unsigned acc, int) {
       float v[32];
-      tmem_ld32(acc, v);
+      take32(s, acc, v);
 #pragma unroll
-      for (int j = 0; j < 32; ++j) v[j] = s.dead ? __int_as_float(0x7fffffff) : ex2((v[j] - top) * p.k) * of_p;
+      for (int j = 0; j < 32; ++j) v[j] = ex2((v[j] - top) * p.k) * of_p;
       const unsigned at = static_cast<unsigned>(hot - col0);
       if (__any_sync(0xffffffffu, at < 32u)) {
 #pragma unroll
@@ -225,7 +230,7 @@ struct Slope {
 #pragma unroll
         for (int j = 0; j < 16; ++j) w[j] = pack2(v[2 * j], v[2 * j + 1], 0);
       }
-      put16(s, w, p.out, p.ld, a.m, a.n, col0, 1);
+      put16(s, w, p.out, p.ld, s.m, s.n, col0, 1);
     }
     __device__ void end(const Params&, const Shape&, const Spot&) {}
   };
@@ -238,34 +243,15 @@ constexpr long long PIECE = 1ll << 28;  // elements of dz at a time: half a giga
 struct Layout {
   bool pack_x, pack_w;
   long long ld_packed;
-  Plan forward, slope, dx, dw;
+  int tiling;  // of the product with an epilogue of its own
   long long piece, pieces;
-  size_t x, w, part, target, factor, dz, sum_dx, sum_dw, total;
+  size_t x, w, part, target, factor, dz, sum, partial, total;
 };
 
-Problem logits(int device, int half, long long rows, long long width, long long vocab) {
-  Problem p = {};
-  p.device = device, p.half = half;
-  p.m = rows, p.n = vocab, p.k = p.k0 = width, p.groups = 1;
-  return p;
-}
-Problem dx_of(int device, int half, long long rows, long long width, long long piece) {
-  Problem p = {};
-  p.device = device, p.half = half;
-  p.m = rows, p.n = width, p.k = p.k0 = piece, p.groups = 1;
-  p.b_turned = true;
-  return p;
-}
-Problem dw_of(int device, int half, long long rows, long long width, long long piece) {
-  Problem p = {};
-  p.device = device, p.half = half;
-  p.m = piece, p.n = width, p.k = p.k0 = rows, p.groups = 1;
-  p.a_turned = p.b_turned = true;
-  return p;
-}
+long long parts_of(int tiling, long long vocab) { return (vocab + TILINGS[tiling].n - 1) / TILINGS[tiling].n; }
 
-Layout plan(int device, const void* x, long long ldx, const void* w, long long ldw, long long rows, long long width,
-            long long vocab, bool grad, int sms) {
+Layout plan(const Device& d, const void* x, long long ldx, const void* w, long long ldw, long long rows, long long width,
+            long long vocab, bool grad) {
   Layout l = {};
   l.pack_x = !tma_ready(x, ldx, rows), l.pack_w = !tma_ready(w, ldw, vocab);
   l.ld_packed = round_up(width, 64);
@@ -279,9 +265,8 @@ Layout plan(int device, const void* x, long long ldx, const void* w, long long l
   if (l.pack_w) l.w = take(2ull * vocab * l.ld_packed);
   const long long kblocks = (width + BK - 1) / BK;
   if (!grad) {
-    l.forward = plan_for(rows, vocab, kblocks, 1, false, false, sms);
-    const long long cols = l.forward.tile == 0 ? 256 : l.forward.tile == 1 ? 128 : 64;
-    l.part = take(sizeof(float2) * ((vocab + cols - 1) / cols) * rows);
+    l.tiling = tiling_for(rows, vocab, kblocks, false, d.sms);
+    l.part = take(sizeof(float2) * parts_of(l.tiling, vocab) * rows);
     l.target = take(sizeof(float) * rows);
   } else {
     l.pieces = (vocab * rows + PIECE - 1) / PIECE;
@@ -289,14 +274,11 @@ Layout plan(int device, const void* x, long long ldx, const void* w, long long l
     l.pieces = std::max(1ll, std::min(l.pieces, (vocab + 1023) / 1024));
     l.piece = std::min(round_up((vocab + l.pieces - 1) / l.pieces, 256), round_up(vocab, 8));
     l.pieces = (vocab + l.piece - 1) / l.piece;
-    const long long first = std::min(l.piece, vocab);
-    l.slope = plan_for(rows, first, kblocks, 1, false, false, sms);
-    const Problem px = dx_of(device, 0, rows, width, first), pw = dw_of(device, 0, rows, width, first);
-    l.dx = store_plan(px, sms), l.dw = store_plan(pw, sms);
+    l.tiling = tiling_for(rows, std::min(l.piece, vocab), kblocks, false, d.sms);
     l.factor = take(2 * sizeof(float));
     l.dz = take(2ull * rows * l.piece);
-    l.sum_dx = take(partial_bytes(px, l.dx, l.pieces > 1));
-    l.sum_dw = take(partial_bytes(pw, l.dw, false));
+    if (l.pieces > 1) l.sum = take(sizeof(float) * rows * round_up(width, 4));
+    l.partial = take(partial_bytes(d));
   }
   l.total = at;
   return l;
@@ -325,9 +307,9 @@ extern "C" int ad_linear_logprobs_workspace(int device, int dtype, const void* x
   if (!rows) return 0;
   DeviceGuard guard(device);
   if (guard.error() != cudaSuccess) return fail_cuda(who, guard.error());
-  const int sms = sm_count(guard.device());
-  if (!sms) return fail("%s: no device properties", who);
-  *bytes = plan(guard.device(), x, ldx, weight, ldw, rows, width, vocab, grad != 0, sms).total;
+  const Device d = {guard.device(), sm_count(guard.device())};
+  if (!d.sms) return fail("%s: no device properties", who);
+  *bytes = plan(d, x, ldx, weight, ldw, rows, width, vocab, grad != 0).total;
   return 0;
 }
 
@@ -344,14 +326,14 @@ extern "C" int ad_linear_logprobs(int device, int dtype, const void* x, int64_t 
     return fail("%s: an operand is not aligned to its elements", who);
   DeviceGuard guard(device);
   if (guard.error() != cudaSuccess) return fail_cuda(who, guard.error());
-  const int sms = sm_count(guard.device());
-  if (!sms) return fail("%s: no device properties", who);
-  const Layout l = plan(guard.device(), x, ldx, weight, ldw, rows, width, vocab, false, sms);
+  const Device d = {guard.device(), sm_count(guard.device())};
+  if (!d.sms) return fail("%s: no device properties", who);
+  const Layout l = plan(d, x, ldx, weight, ldw, rows, width, vocab, false);
   if (!workspace || !aligned(workspace, 256) || workspace_bytes < l.total)
     return fail("%s: needs %zu bytes of workspace, 256-byte aligned", who, l.total);
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   unsigned char* ws = static_cast<unsigned char*>(workspace);
-  Problem p = logits(guard.device(), dtype == AD_F16, rows, width, vocab);
+  Problem p = {rows, vocab, width, width, false, false, {}, {}};
   p.a[0] = l.pack_x ? Mat{ws + l.x, l.ld_packed} : Mat{x, ldx};
   p.b[0] = l.pack_w ? Mat{ws + l.w, l.ld_packed} : Mat{weight, ldw};
   if (l.pack_x && pack_rows(who, x, ldx, rows, width, ws + l.x, l.ld_packed, st)) return 1;
@@ -361,11 +343,10 @@ extern "C" int ad_linear_logprobs(int device, int dtype, const void* x, int64_t 
   q.target = reinterpret_cast<float*>(ws + l.target);
   q.tokens = tokens, q.tok64 = tok64;
   q.k = std::min(scale * LOG2E, FLT_MAX);
-  if (start<Sum>(who, p, l.forward, q, sms, st)) return 1;
-  const long long cols = l.forward.tile == 0 ? 256 : l.forward.tile == 1 ? 128 : 64;
+  if (start<Sum>(who, d, p, dtype == AD_F16, l.tiling, q, st)) return 1;
   FinishArgs f = {};
   f.part = q.part, f.target = q.target, f.tokens = tokens, f.tok64 = tok64;
-  f.parts = static_cast<int>((vocab + cols - 1) / cols), f.rows = static_cast<int>(rows);
+  f.parts = static_cast<int>(parts_of(l.tiling, vocab)), f.rows = static_cast<int>(rows);
   f.vocab = vocab, f.scale = scale, f.k = q.k;
   f.logp = logp, f.lse = lse, f.stats = reinterpret_cast<float2*>(stats);
   const cudaError_t e = launch<finish_kernel>(dim3(static_cast<unsigned>((rows + FINISH_ROWS - 1) / FINISH_ROWS)), 32 * FINISH_WARPS, 0, st, f);
@@ -390,10 +371,10 @@ extern "C" int ad_linear_logprobs_grad(int device, int dtype, const void* x, int
     return fail("%s: an operand is not aligned to its elements", who);
   DeviceGuard guard(device);
   if (guard.error() != cudaSuccess) return fail_cuda(who, guard.error());
-  const int sms = sm_count(guard.device());
-  if (!sms) return fail("%s: no device properties", who);
-  const int dev = guard.device(), half = dtype == AD_F16;
-  const Layout l = plan(dev, x, ldx, weight, ldw, rows, width, vocab, true, sms);
+  const Device d = {guard.device(), sm_count(guard.device())};
+  if (!d.sms) return fail("%s: no device properties", who);
+  const int half = dtype == AD_F16;
+  const Layout l = plan(d, x, ldx, weight, ldw, rows, width, vocab, true);
   if (!workspace || !aligned(workspace, 256) || workspace_bytes < l.total)
     return fail("%s: needs %zu bytes of workspace, 256-byte aligned", who, l.total);
   cudaStream_t st = static_cast<cudaStream_t>(stream);
@@ -412,8 +393,7 @@ extern "C" int ad_linear_logprobs_grad(int device, int dtype, const void* x, int
   for (long long i = 0; i < l.pieces; ++i) {
     const long long v0 = i * l.piece, n = std::min(l.piece, vocab - v0);
     const Mat w = {static_cast<const unsigned short*>(mw.p) + v0 * mw.ld, mw.ld};
-    Problem p = logits(dev, half, rows, width, n);
-    p.a[0] = mx, p.b[0] = w;
+    Problem p = {rows, n, width, width, false, false, {mx, {}}, {w, {}}};
     Slope::Params q = {};
     q.stats = reinterpret_cast<const float2*>(stats);
     q.tokens = tokens, q.tok64 = tok64;
@@ -421,20 +401,18 @@ extern "C" int ad_linear_logprobs_grad(int device, int dtype, const void* x, int
     q.vocab = vocab, q.first = v0;
     q.k = std::min(scale * LOG2E, FLT_MAX), q.scale = scale;
     q.out = reinterpret_cast<unsigned short*>(ws + l.dz), q.ld = l.piece;
-    if (start<Slope>(who, p, l.slope, q, sms, st)) return 1;
-    Problem px = dx_of(dev, half, rows, width, n);
-    px.a[0] = dz, px.b[0] = w;
-    const Out ox = {dx, lddx};
-    const Sums sums = {i == 0, i + 1 == l.pieces};
-    if (store_product(who, px, l.dx, dtype, &ox, false, factor ? factor + 1 : nullptr, reinterpret_cast<float*>(ws + l.sum_dx),
-                      &sums, sms, st))
-      return 1;
-    Problem pw = dw_of(dev, half, rows, width, n);
-    pw.a[0] = dz, pw.b[0] = mx;
-    const Out ow = {static_cast<unsigned char*>(dw) + v0 * lddw * es, lddw};
-    if (store_product(who, pw, l.dw, dw_type, &ow, accumulate != 0, factor ? factor + 1 : nullptr,
-                      reinterpret_cast<float*>(ws + l.sum_dw), nullptr, sms, st))
-      return 1;
+    if (start<Slope>(who, d, p, half, l.tiling, q, st)) return 1;
+    const Problem products[2] = {{rows, width, n, n, false, true, {dz, {}}, {w, {}}},
+                                 {n, width, rows, rows, true, true, {dz, {}}, {mx, {}}}};
+    // dx: sums over the pieces stay in 32 bits until the last one's
+    float* sum = reinterpret_cast<float*>(ws + l.sum);
+    const long long ld_sum = round_up(width, 4);
+    const bool first = i == 0, last = i + 1 == l.pieces;
+    const float* alpha = factor ? factor + 1 : nullptr;
+    const Result results[2] = {
+        {last ? dx : sum, last ? lddx : ld_sum, last ? dtype : AD_F32, false, first ? nullptr : sum, ld_sum, last ? alpha : nullptr},
+        {static_cast<unsigned char*>(dw) + v0 * lddw * es, lddw, dw_type, accumulate != 0, nullptr, 0, alpha}};
+    if (store_products(who, d, half, products, results, 2, reinterpret_cast<float*>(ws + l.partial), st)) return 1;
   }
   return 0;
 }

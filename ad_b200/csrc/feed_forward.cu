@@ -132,8 +132,18 @@ struct GatedGrad {
     long long ld;  // of these, whose rows are aligned
     int act;
   };
+  // Eight columns of g and u in a row of a chunk.
+  struct Kept {
+    float4 g[2], u[2];
+  };
   struct State {
-    __device__ State(const Params&, const Shape&, const Spot&) {}
+    Kept kept[2];  // what comes next, under way
+    // the warp's first chunk, ahead of the wait for the accumulator
+    __device__ State(const Params& p, const Shape&, const Spot& s) {
+      const int col0 = s.unit.col * s.width + s.part * CHUNK;
+      if (fast(p, s, col0)) fetch(p, s, col0, 0, kept[0]), fetch(p, s, col0, 1, kept[1]);
+    }
+    __device__ static bool fast(const Params& p, const Spot& s, int col0) { return p.vec && col0 + CHUNK <= s.n; }
     __device__ void end(const Params&, const Shape&, const Spot&) {}
     template <int ACT>
     __device__ static void one(float dh, float g, float u, float& dg, float& du, float& h) {
@@ -141,11 +151,7 @@ struct GatedGrad {
       const float act = activate<ACT, true>(g, &slope);
       dg = dh * u * slope, du = dh * act, h = act * u;
     }
-    // Eight columns of g and u in a row of the chunk.
-    struct Kept {
-      float4 g[2], u[2];
-    };
-    __device__ static void fetch(const Params& p, const Shape& a, const Spot& s, int col0, int i, Kept& k) {
+    __device__ static void fetch(const Params& p, const Spot& s, int col0, int i, Kept& k) {
       const long long row = s.row0 + i * 8 + (s.lane >> 2);
       const int col = col0 + (s.lane & 3) * 8;
 #pragma unroll
@@ -158,13 +164,19 @@ struct GatedGrad {
       }
     }
     template <int ACT, int HALF>
-    __device__ static void part(const Params& p, const Shape& a, const Spot& s, int col0, Kept (&k)[2]) {
+    __device__ __forceinline__ void part(const Params& p, const Spot& s, int col0) {
+      const int next = col0 + s.stride;
+      const bool more = !s.last && fast(p, s, next);
       const int q = s.lane & 3;
       long long at = (s.row0 + (s.lane >> 2)) * p.ld + col0 + q * 8;
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         const int r = i * 8 + (s.lane >> 2);
-        const Kept& c = k[i & 1];
+        const Kept c = kept[i & 1];
+        if (i + 2 < 4)
+          fetch(p, s, col0, i + 2, kept[i & 1]);
+        else if (more)
+          fetch(p, s, next, i - 2, kept[i & 1]);
         unsigned dg[4], du[4], h[4];
 #pragma unroll
         for (int j = 0; j < 2; ++j) {
@@ -178,7 +190,6 @@ struct GatedGrad {
           du[2 * j] = pack2(y[0], y[1], HALF), du[2 * j + 1] = pack2(y[2], y[3], HALF);
           h[2 * j] = pack2(z[0], z[1], HALF), h[2 * j + 1] = pack2(z[2], z[3], HALF);
         }
-        if (i + 2 < 4) fetch(p, a, s, col0, i + 2, k[i & 1]);
         if (s.row0 + r < s.m) {
           *reinterpret_cast<uint4*>(p.dg + at) = make_uint4(dg[0], dg[1], dg[2], dg[3]);
           *reinterpret_cast<uint4*>(p.du + at) = make_uint4(du[0], du[1], du[2], du[3]);
@@ -188,11 +199,11 @@ struct GatedGrad {
       }
     }
     template <int ACT>
-    __device__ static void part(const Params& p, const Shape& a, const Spot& s, int col0, Kept (&k)[2]) {
+    __device__ __forceinline__ void part(const Params& p, const Shape& a, const Spot& s, int col0) {
       if (a.half)
-        part<ACT, 1>(p, a, s, col0, k);
+        part<ACT, 1>(p, s, col0);
       else
-        part<ACT, 0>(p, a, s, col0, k);
+        part<ACT, 0>(p, s, col0);
     }
     template <int ACT>
     __device__ static void columns(const Params& p, const Shape& a, const Spot& s, int col0) {
@@ -210,21 +221,15 @@ struct GatedGrad {
       }
     }
     __device__ void chunk(const Params& p, const Shape& a, const Spot& s, int col0, unsigned acc, int) {
-      const bool fast = p.vec && col0 + CHUNK <= s.n;
-      Kept k[2];
-      if (fast) {
-        fetch(p, a, s, col0, 0, k[0]);
-        fetch(p, a, s, col0, 1, k[1]);
-      }
       float v[32];
       take32(s, acc, v);
       stage32(s, v);
-      if (fast) {
+      if (fast(p, s, col0)) {
         switch (p.act) {
-          case SILU: part<SILU>(p, a, s, col0, k); break;
-          case GELU: part<GELU>(p, a, s, col0, k); break;
-          case GELU_TANH: part<GELU_TANH>(p, a, s, col0, k); break;
-          default: part<RELU>(p, a, s, col0, k);
+          case SILU: part<SILU>(p, a, s, col0); break;
+          case GELU: part<GELU>(p, a, s, col0); break;
+          case GELU_TANH: part<GELU_TANH>(p, a, s, col0); break;
+          default: part<RELU>(p, a, s, col0);
         }
       } else {
         switch (p.act) {
@@ -237,6 +242,137 @@ struct GatedGrad {
     }
   };
 };
+
+// ------------------------------------------------------------------ a few rows
+
+// Up to eight rows are bound by the weights, which are read once: a warp takes
+// a row of them (of both matrices for h), 16 bytes a lane at a time, against all
+// rows of x, on the CUDA cores; WARPS warps of a block share a row of the weights where
+// it is long and there are few.
+struct RowsArgs {
+  const unsigned short *x, *w0, *w1;
+  long long ldx, ld0, ld1;
+  int rows, n, k, act;
+  unsigned short* out;
+  long long ldo;
+  float *gate, *up;
+  long long ldg, ldu;
+};
+
+// V elements as they are loaded, and their values.
+template <int V>
+using Raw = typename Word<2 * V>::type;
+template <int V>
+__device__ __forceinline__ Raw<V> raw_row(const unsigned short* p) {
+  return *reinterpret_cast<const Raw<V>*>(p);
+}
+template <int V>
+__device__ __forceinline__ void open_row(const Raw<V>& r, int half, float (&v)[V]) {
+  if constexpr (V == 8) {
+    const unsigned w[4] = {r.x, r.y, r.z, r.w};
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const float2 f = unpack2(w[j], half);
+      v[2 * j] = f.x, v[2 * j + 1] = f.y;
+    }
+  } else {
+    v[0] = unpack2(r, half).x;
+  }
+}
+
+template <int T, int V, int HALF, bool DUAL>
+__global__ void __launch_bounds__(256) rows_kernel(const __grid_constant__ RowsArgs a, int shared_by) {
+  __shared__ float buf[8][2 * T];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int row = blockIdx.x * (8 / shared_by) + warp / shared_by, share = warp % shared_by;
+  float s[2][T];
+#pragma unroll
+  for (int t = 0; t < T; ++t) s[0][t] = s[1][t] = 0.0f;
+  if (row < a.n) {
+    const unsigned short *w0 = a.w0 + row * a.ld0, *w1 = DUAL ? a.w1 + row * a.ld1 : nullptr;
+    const int step = 32 * V * shared_by;
+    constexpr int U = 4;  // loads of weights under way
+    for (int k0 = (share * 32 + lane) * V; k0 < a.k; k0 += U * step) {
+      Raw<V> p[U], q[U];
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+        if (k0 + u * step < a.k) {
+          p[u] = raw_row<V>(w0 + k0 + u * step);
+          if (DUAL) q[u] = raw_row<V>(w1 + k0 + u * step);
+        }
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        const int k = k0 + u * step;
+        if (k >= a.k) break;
+        float pv[V], qv[V], x[V];
+        open_row<V>(p[u], HALF, pv);
+        if (DUAL) open_row<V>(q[u], HALF, qv);
+#pragma unroll
+        for (int t = 0; t < T; ++t) {
+          if (t >= a.rows) break;
+          open_row<V>(raw_row<V>(a.x + t * a.ldx + k), HALF, x);
+#pragma unroll
+          for (int j = 0; j < V; ++j) {
+            s[0][t] = fmaf(pv[j], x[j], s[0][t]);
+            if (DUAL) s[1][t] = fmaf(qv[j], x[j], s[1][t]);
+          }
+        }
+      }
+    }
+  }
+#pragma unroll
+  for (int t = 0; t < T; ++t) {
+    s[0][t] = warp_sum(s[0][t]);
+    if (DUAL) s[1][t] = warp_sum(s[1][t]);
+  }
+  if (lane == 0) {
+#pragma unroll
+    for (int t = 0; t < T; ++t) buf[warp][2 * t] = s[0][t], buf[warp][2 * t + 1] = s[1][t];
+  }
+  __syncthreads();
+  if (row >= a.n || share || lane >= a.rows) return;
+  float g = buf[warp][2 * lane], u = buf[warp][2 * lane + 1];
+  for (int i = 1; i < shared_by; ++i) g += buf[warp + i][2 * lane], u += buf[warp + i][2 * lane + 1];
+  if (DUAL) {
+    if (a.gate) {
+      a.gate[lane * a.ldg + row] = g;
+      a.up[lane * a.ldu + row] = u;
+    }
+    switch (a.act) {
+      case SILU: g = activate<SILU, false>(g, nullptr); break;
+      case GELU: g = activate<GELU, false>(g, nullptr); break;
+      case GELU_TANH: g = activate<GELU_TANH, false>(g, nullptr); break;
+      default: g = activate<RELU, false>(g, nullptr);
+    }
+    g *= u;
+  }
+  const unsigned w = pack2(g, 0.0f, HALF);
+  a.out[lane * a.ldo + row] = static_cast<unsigned short>(w);
+}
+
+constexpr int FEW = 8;
+
+template <int T, bool DUAL>
+cudaError_t start_rows(const RowsArgs& a, int half, int sms, cudaStream_t st) {
+  auto fits = [](const void* p, long long ld, long long rows) { return aligned(p, 16) && (rows <= 1 || ld % 8 == 0); };
+  const bool vec = a.k % 8 == 0 && fits(a.x, a.ldx, a.rows) && fits(a.w0, a.ld0, a.n) && (!DUAL || fits(a.w1, a.ld1, a.n));
+  // warps for all of the device, as long as each has 512 elements of a row
+  int shared_by = 1;
+  while (shared_by < 8 && a.n * shared_by < 16 * sms && a.k / (2 * shared_by) >= 512) shared_by *= 2;
+  cudaLaunchConfig_t c = {};
+  c.gridDim = dim3((a.n + 8 / shared_by - 1) / (8 / shared_by));
+  c.blockDim = dim3(256);
+  c.stream = st;
+  return vec ? (half ? cudaLaunchKernelEx(&c, rows_kernel<T, 8, 1, DUAL>, a, shared_by) : cudaLaunchKernelEx(&c, rows_kernel<T, 8, 0, DUAL>, a, shared_by))
+             : (half ? cudaLaunchKernelEx(&c, rows_kernel<T, 1, 1, DUAL>, a, shared_by) : cudaLaunchKernelEx(&c, rows_kernel<T, 1, 0, DUAL>, a, shared_by));
+}
+template <bool DUAL>
+cudaError_t few_rows(const RowsArgs& a, int half, int sms, cudaStream_t st) {
+  return a.rows == 1   ? start_rows<1, DUAL>(a, half, sms, st)
+         : a.rows == 2 ? start_rows<2, DUAL>(a, half, sms, st)
+         : a.rows <= 4 ? start_rows<4, DUAL>(a, half, sms, st)
+                       : start_rows<FEW, DUAL>(a, half, sms, st);
+}
 
 // ------------------------------------------------------------------ host
 
@@ -260,6 +396,12 @@ Layout plan(const Device& d, const Operand* ops, int count, long long rows, long
     at += room(bytes);
     return here;
   };
+  if (count == 4 && rows <= FEW) {  // h alone
+    l.ld = round_up(hidden, 64);
+    l.h = take(2ull * rows * l.ld);
+    l.total = at;
+    return l;
+  }
   for (int i = 0; i < count; ++i)
     if (!tma_ready(ops[i].p, ops[i].ld, ops[i].rows)) l.pack[i] = take(2ull * ops[i].rows * round_up(ops[i].cols, 64));
   l.ld = round_up(hidden, 64);
@@ -286,12 +428,18 @@ int check(const char* who, int dtype, int64_t rows, int64_t width, int64_t hidde
   return 0;
 }
 
-// An operand as TMA reads it: itself, or its copy.
-int ready(const char* who, const Operand& o, unsigned char* copy, cudaStream_t st, Mat* m) {
-  *m = Mat{o.p, o.ld};
-  if (tma_ready(o.p, o.ld, o.rows)) return 0;
-  *m = Mat{copy, round_up(o.cols, 64)};
-  return pack_rows(who, o.p, o.ld, o.rows, o.cols, copy, m->ld, st);
+// Operands as TMA reads them: themselves, or their copies.
+int ready(const char* who, const Device& d, const Operand* ops, int count, const size_t* copies, unsigned char* ws, Mat* m,
+          cudaStream_t st) {
+  Pack packs[MAX_PACKS];
+  int n = 0;
+  for (int i = 0; i < count; ++i) {
+    m[i] = Mat{ops[i].p, ops[i].ld};
+    if (tma_ready(ops[i].p, ops[i].ld, ops[i].rows)) continue;
+    m[i] = Mat{ws + copies[i], round_up(ops[i].cols, 64)};
+    packs[n++] = {ops[i].p, ws + copies[i], ops[i].rows, ops[i].cols, ops[i].ld, m[i].ld};
+  }
+  return pack_rows(who, d, packs, n, st);
 }
 
 bool vec32(const void* p, long long ld, long long rows) { return aligned(p, 16) && (rows <= 1 || ld % 4 == 0); }
@@ -341,9 +489,19 @@ extern "C" int ad_feed_forward(int device, int dtype, int act, const void* x, in
     return fail("%s: needs %zu bytes of workspace, 256-byte aligned", who, l.total);
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   unsigned char* ws = static_cast<unsigned char*>(workspace);
+  if (rows <= FEW) {
+    auto half_ptr = [](const void* q) { return static_cast<const unsigned short*>(q); };
+    unsigned short* h = reinterpret_cast<unsigned short*>(ws + l.h);
+    RowsArgs r = {half_ptr(x), half_ptr(w_gate), half_ptr(w_up), ldx, ld_gate, ld_up, static_cast<int>(rows),
+                  static_cast<int>(hidden), static_cast<int>(width), act, h, l.ld, gate, up, ldg, ldu};
+    cudaError_t e = few_rows<true>(r, half, d.sms, st);
+    r = {h, half_ptr(w_down), nullptr, l.ld, ld_down, 0, static_cast<int>(rows), static_cast<int>(width),
+         static_cast<int>(hidden), act, static_cast<unsigned short*>(y), ldy, nullptr, nullptr, 0, 0};
+    if (e == cudaSuccess) e = few_rows<false>(r, half, d.sms, st);
+    return e == cudaSuccess ? 0 : fail_cuda(who, e);
+  }
   Mat m[4];
-  for (int i = 0; i < 4; ++i)
-    if (ready(who, ops[i], ws + l.pack[i], st, &m[i])) return 1;
+  if (ready(who, d, ops, 4, l.pack, ws, m, st)) return 1;
   const Problem p = {rows, hidden, width, width, false, false, {m[0], {}}, {m[1], m[2]}};
   Gated::Params q = {};
   q.h = reinterpret_cast<unsigned short*>(ws + l.h), q.ldh = l.ld, q.vec_h = 1;
@@ -393,8 +551,7 @@ extern "C" int ad_feed_forward_grad(int device, int dtype, int act, const void* 
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   unsigned char* ws = static_cast<unsigned char*>(workspace);
   Mat m[5];
-  for (int i = 0; i < 5; ++i)
-    if (ready(who, ops[i], ws + l.pack[i], st, &m[i])) return 1;
+  if (ready(who, d, ops, 5, l.pack, ws, m, st)) return 1;
   const Mat h = {ws + l.h, l.ld}, dg = {ws + l.dg, l.ld}, du = {ws + l.du, l.ld};
 
   const Problem p = {rows, hidden, width, width, false, true, {m[4], {}}, {m[3], {}}};

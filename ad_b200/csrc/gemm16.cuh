@@ -237,6 +237,7 @@ struct Spot {
   int lane, quad, part, row0, rank;
   Unit unit;
   int m, n;       // of the result
+  int width, stride;  // of a tile; columns from a chunk of the warp's to its next
   int odd;        // every other tile of the block
   unsigned side;
   unsigned free_bar;  // to arrive at once the accumulator has been read
@@ -282,16 +283,28 @@ __device__ __forceinline__ void put16(const Spot& s, const unsigned (&w)[16], un
       if (s.row0 + r < m) *reinterpret_cast<uint4*>(to) = x;
       to += 8 * ld;
     }
-  } else {  // a column a lane
-    const int col = col0 + s.lane, p = s.lane >> 3;
-    if (col < n) {
-      for (int r = 0; r < 32 && s.row0 + r < m; ++r) {
-        unsigned short x;
-        asm volatile("ld.shared.u16 %0, [%1];"
-                     : "=h"(x)
-                     : "r"(s.side + r * 64 + ((p ^ ((r >> 1) & 3)) << 4) + (s.lane & 7) * 2)
-                     : "memory");
-        out[(s.row0 + r) * ld + col] = x;
+  } else {
+    // two rows at a time, half a warp each, two columns a lane: words where they are
+    // aligned, else words from the second column on and the first and last one apart
+    const int h = s.lane >> 4, l = s.lane & 15;
+    auto at = [&](int r, int c) {
+      unsigned short x;
+      asm volatile("ld.shared.u16 %0, [%1];"
+                   : "=h"(x)
+                   : "r"(s.side + r * 64 + (((c >> 3) ^ ((r >> 1) & 3)) << 4) + (c & 7) * 2)
+                   : "memory");
+      return x;
+    };
+    for (int r = h; r < 32 && s.row0 + r < m; r += 2) {
+      unsigned short* row = out + (s.row0 + r) * ld + col0;
+      const int shift = (reinterpret_cast<uintptr_t>(row) >> 1) & 1;
+      const int c0 = 2 * l + shift, c1 = c0 + 1 < 32 ? c0 + 1 : 0;  // of the last lane: the first column
+      const unsigned short x0 = at(r, c0), x1 = at(r, c1);
+      if (c1 && col0 + c1 < n) {
+        *reinterpret_cast<unsigned*>(row + c0) = x0 | static_cast<unsigned>(x1) << 16;
+      } else {
+        if (col0 + c0 < n) row[c0] = x0;
+        if (!c1) row[0] = x1;
       }
     }
   }
@@ -536,7 +549,7 @@ __global__ void __launch_bounds__(TILE::THREADS, 1)
     Spot s;
     s.lane = lane, s.quad = quad, s.part = part;
     s.side = smem_u32(side) + (warp - 2) * EPI::SIDE;
-    s.rank = rank;
+    s.rank = rank, s.width = COLS, s.stride = PARTS * CHUNK;
     s.dead = false;
     int c = 0;
     for (int u = first; u < end; u += step, ++c) {
@@ -745,9 +758,15 @@ struct Result {
 size_t partial_bytes(const Device& d);
 int store_products(const char* who, const Device& d, int half, const Problem* p, const Result* r, int count, float* partial,
                    cudaStream_t st);
-// A copy of a 16-bit matrix whose rows TMA can read.
-int pack_rows(const char* who, const void* p, long long ld, long long rows, long long cols, void* to, long long ld_to,
-              cudaStream_t st);
+// Copies of 16-bit matrices whose rows TMA can read (16-byte aligned, of a multiple
+// of 8 elements), up to MAX_PACKS of them in one go.
+constexpr int MAX_PACKS = 5;
+struct Pack {
+  const void* from;
+  void* to;
+  long long rows, cols, ld, ld_to;
+};
+int pack_rows(const char* who, const Device& d, const Pack* packs, int count, cudaStream_t st);
 
 }  // namespace adgemm
 

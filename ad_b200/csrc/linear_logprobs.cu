@@ -284,6 +284,16 @@ Layout plan(const Device& d, const void* x, long long ldx, const void* w, long l
   return l;
 }
 
+// Copies of the operands that TMA cannot read as they are.
+int pack(const char* who, const Device& d, const Layout& l, const void* x, long long ldx, const void* w, long long ldw,
+         long long rows, long long width, long long vocab, unsigned char* ws, cudaStream_t st) {
+  Pack packs[2];
+  int n = 0;
+  if (l.pack_x) packs[n++] = {x, ws + l.x, rows, width, ldx, l.ld_packed};
+  if (l.pack_w) packs[n++] = {w, ws + l.w, vocab, width, ldw, l.ld_packed};
+  return pack_rows(who, d, packs, n, st);
+}
+
 int check(const char* who, int dtype, const void* x, int64_t ldx, const void* w, int64_t ldw, int64_t rows, int64_t width,
           int64_t vocab) {
   if (dtype != AD_BF16 && dtype != AD_F16) return fail("%s: unknown element type %d (AD_BF16 or AD_F16)", who, dtype);
@@ -336,8 +346,7 @@ extern "C" int ad_linear_logprobs(int device, int dtype, const void* x, int64_t 
   Problem p = {rows, vocab, width, width, false, false, {}, {}};
   p.a[0] = l.pack_x ? Mat{ws + l.x, l.ld_packed} : Mat{x, ldx};
   p.b[0] = l.pack_w ? Mat{ws + l.w, l.ld_packed} : Mat{weight, ldw};
-  if (l.pack_x && pack_rows(who, x, ldx, rows, width, ws + l.x, l.ld_packed, st)) return 1;
-  if (l.pack_w && pack_rows(who, weight, ldw, vocab, width, ws + l.w, l.ld_packed, st)) return 1;
+  if (pack(who, d, l, x, ldx, weight, ldw, rows, width, vocab, ws, st)) return 1;
   Sum::Params q = {};
   q.part = reinterpret_cast<float2*>(ws + l.part);
   q.target = reinterpret_cast<float*>(ws + l.target);
@@ -381,8 +390,7 @@ extern "C" int ad_linear_logprobs_grad(int device, int dtype, const void* x, int
   unsigned char* ws = static_cast<unsigned char*>(workspace);
   const Mat mx = l.pack_x ? Mat{ws + l.x, l.ld_packed} : Mat{x, ldx};
   const Mat mw = l.pack_w ? Mat{ws + l.w, l.ld_packed} : Mat{weight, ldw};
-  if (l.pack_x && pack_rows(who, x, ldx, rows, width, ws + l.x, l.ld_packed, st)) return 1;
-  if (l.pack_w && pack_rows(who, weight, ldw, vocab, width, ws + l.w, l.ld_packed, st)) return 1;
+  if (pack(who, d, l, x, ldx, weight, ldw, rows, width, vocab, ws, st)) return 1;
   float* factor = half ? reinterpret_cast<float*>(ws + l.factor) : nullptr;
   if (half) {
     const RangeArgs r = {g_logp, g_lse, static_cast<int>(rows), scale, factor};

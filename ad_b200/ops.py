@@ -1147,25 +1147,38 @@ def _dense(x, name):
     return n
 
 
-def _clip_operands(arrays, name, device):
-    """(type codes, element counts) of arrays on a device."""
-    found = []
-    for i, x in enumerate(arrays):
+def _dense_array(x, name):
+    """(type code, elements, device) of an array that fills its memory."""
+    code = _float(x, name)
+    return code, 0 if 0 in x.shape else _dense(x, name), _device(x, name)
+
+
+def _clip_operands(grads, out):
+    """(device, type codes, element counts) of the arrays; ``out`` has the same layouts."""
+    types, counts, device = [], [], None
+    for i, x in enumerate(grads):
         try:
             key = _layout(x)
-            f = _checked.get(key)
+            found = _checked.get(key)
         except (AttributeError, TypeError):  # not a device array: refused below
-            key = f = None
-        if f is None:
-            label = f"{name}[{i}]"
-            code = _float(x, label)
-            _device(x, label)
-            n = 0 if 0 in x.shape else _dense(x, label)
-            f = _remember(key, (code, n, x.get_device()))
-        if f[2] != device:
-            raise ValueError(f"{name}[{i}]: on device {f[2]}, not on device {device}")
-        found.append(f)
-    return [f[0] for f in found], [f[1] for f in found]
+            key = found = None
+        if found is None:
+            found = _remember(key, _dense_array(x, f"grads[{i}]"))
+        code, n, on = found
+        if on != device:
+            if device is not None:
+                raise ValueError(f"grads[{i}]: on device {on}, not on device {device}")
+            device = on
+        types.append(code)
+        counts.append(n)
+        if out is not None:
+            y = out[i]
+            if not hasattr(y, "data_ptr"):
+                _float(y, f"out[{i}]")
+            if _layout(y) != key:
+                raise ValueError(f"out[{i}]: {y.dtype} of shape {tuple(y.shape)} and strides {tuple(y.stride())} on device "
+                                 f"{y.get_device()}, expected {x.dtype}, {tuple(x.shape)}, {tuple(x.stride())} on {device}")
+    return device, types, counts
 
 
 def clip_norm(grads, max_norm: float, *, out=None, norm=None, workspace=None, stream=None):
@@ -1181,22 +1194,12 @@ def clip_norm(grads, max_norm: float, *, out=None, norm=None, workspace=None, st
         raise ValueError("grads: no arrays")
     if not max_norm >= 0:
         raise ValueError(f"max_norm: {max_norm}")
-    if not hasattr(grads[0], "get_device"):
-        _float(grads[0], "grads[0]")
-    dev = _device(grads[0], "grads[0]")
-    types, counts = _clip_operands(grads, "grads", dev)
-    to = grads
+    to = None
     if out is not None:
         to = list(out)
         if len(to) != len(grads):
             raise ValueError(f"out: {len(to)} arrays for {len(grads)}")
-        for i, (x, y) in enumerate(zip(grads, to)):
-            if not hasattr(y, "data_ptr"):
-                _float(y, f"out[{i}]")
-            if x.shape != y.shape or x.stride() != y.stride() or x.dtype != y.dtype:
-                raise ValueError(f"out[{i}]: {y.dtype} of shape {tuple(y.shape)} and strides {tuple(y.stride())}, expected "
-                                 f"{x.dtype}, {tuple(x.shape)}, {tuple(x.stride())}")
-            _on(dev, y, f"out[{i}]")
+    dev, types, counts = _clip_operands(grads, to)
     s = _stream(dev, stream, grads[0], norm is None or workspace is None)
     if norm is None:
         norm = grads[0].new_empty((1,), dtype=_torch.float32)
@@ -1208,7 +1211,7 @@ def clip_norm(grads, max_norm: float, *, out=None, norm=None, workspace=None, st
     workspace, have = _scratch(clip_norm_workspace(n) if workspace is None else 0, workspace, dev, grads[0])
     pointers, longs = ctypes.c_void_p * n, ctypes.c_int64 * n
     at = pointers(*[x.data_ptr() for x in grads])
-    rt.check(_entry("ad_clip_norm")(dev, n, at, at if out is None else pointers(*[y.data_ptr() for y in to]),
+    rt.check(_entry("ad_clip_norm")(dev, n, at, at if to is None else pointers(*[y.data_ptr() for y in to]),
                                     longs(*counts), (ctypes.c_int * n)(*types), max_norm, norm.data_ptr(),
                                     workspace.data_ptr(), have, s))
     return norm

@@ -25,40 +25,97 @@ using namespace adgemm;
 
 enum Act { SILU = 0, GELU = 1, GELU_TANH = 2, RELU = 3, ACTS = 4 };
 
-constexpr float SQRT_HALF = 0.70710678118654752f;     // 1 / sqrt(2)
-constexpr float DENSITY = 0.39894228040143268f;       // 1 / sqrt(2 pi)
-constexpr float TANH_SCALE = 1.5957691216057308f;     // 2 sqrt(2 / pi)
+// Two values that one instruction works on.
+typedef unsigned long long Two;
+__device__ __forceinline__ Two two(float a, float b) {
+  Two r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ float2 apart(Two x) {
+  float2 r;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(x));
+  return r;
+}
+__device__ __forceinline__ unsigned rounded(Two x, int half) {
+  const float2 v = apart(x);
+  return pack2(v.x, v.y, half);
+}
+__device__ __forceinline__ Two fma2(Two a, Two b, Two c) {
+  Two r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+__device__ __forceinline__ Two mul2(Two a, Two b) {
+  Two r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ Two fma2(Two a, float b, float c) { return fma2(a, two(b, b), two(c, c)); }
+__device__ __forceinline__ Two mul2(Two a, float b) { return mul2(a, two(b, b)); }
+__device__ __forceinline__ Two exp2_2(Two x) {
+  float2 v = apart(x);
+  asm("ex2.approx.f32 %0, %0;" : "+f"(v.x));
+  asm("ex2.approx.f32 %0, %0;" : "+f"(v.y));
+  return two(v.x, v.y);
+}
+__device__ __forceinline__ Two reciprocal2(Two x) {
+  float2 v = apart(x);
+  asm("rcp.approx.f32 %0, %0;" : "+f"(v.x));
+  asm("rcp.approx.f32 %0, %0;" : "+f"(v.y));
+  return two(v.x, v.y);
+}
+
+constexpr float LOG2E = 1.4426950408889634f;
+constexpr float DENSITY = 0.39894228040143268f;    // 1 / sqrt(2 pi)
+constexpr float TANH_SCALE = 1.5957691216057308f;  // 2 sqrt(2 / pi)
 constexpr float TANH_CUBE = 0.044715f;
 
-// The activation, and with SLOPE its derivative.  1 + tanh(z) is twice the
-// logistic function of 2 z, which keeps the precision of what tanh brings near 0.
+// What act(z) = z p is z times, and with SLOPE the derivative, of two values; where
+// these say nothing else, errors are a few of 32 bits.
 template <int ACT, bool SLOPE>
-__device__ __forceinline__ float activate(float z, float* slope) {
+__device__ __forceinline__ Two share(Two z, Two& slope) {
+  const float2 v = apart(z);
   if (ACT == RELU) {
-    if (SLOPE) *slope = z > 0.0f ? 1.0f : z == z ? 0.0f : z;
-    return z > 0.0f ? z : z == z ? 0.0f : z;
+    const Two p = two(v.x > 0.0f ? 1.0f : v.x == v.x ? 0.0f : v.x, v.y > 0.0f ? 1.0f : v.y == v.y ? 0.0f : v.y);
+    slope = p;
+    return p;
   }
   if (ACT == GELU) {
-    // Abramowitz and Stegun 7.1.26: erfc(x) = (a1 t + ... + a5 t^5) exp(-x^2), t = 1 / (1 + 0.3275911 x),
-    // for x >= 0, within 1.5e-7; erfcf took the block's small training case from 196 to XXX us
-    const float e = __expf(-0.5f * z * z);
-    const float t = __fdividef(1.0f, fmaf(0.3275911f * SQRT_HALF, fabsf(z), 1.0f));
-    const float poly = t * fmaf(t, fmaf(t, fmaf(t, fmaf(t, 1.061405429f, -1.453152027f), 1.421413741f), -0.284496736f), 0.254829592f);
-    const float tail = 0.5f * poly * e;
-    const float p = z >= 0.0f ? 1.0f - tail : z == z ? tail : z;
-    if (SLOPE) *slope = fmaf(z * DENSITY, e, p);
-    return z * p;
+    // the normal distribution's sum by Abramowitz and Stegun 7.1.26: erfc(x) = (a1 t + ... + a5 t^5) exp(-x^2),
+    // t = 1 / (1 + 0.3275911 x), x = |z| / sqrt(2), within 1.5e-7 (with erfcf: 43 us instead of 40 for 4095 x 512 x
+    // 2048); half of it is what lies beyond |z|
+    const Two e = exp2_2(mul2(mul2(z, z), -0.5f * LOG2E));
+    const Two t = reciprocal2(fma2(two(fabsf(v.x), fabsf(v.y)), 0.3275911f * 0.70710678f, 1.0f));
+    Two poly = fma2(t, 0.5f * 1.061405429f, 0.5f * -1.453152027f);
+    poly = fma2(poly, t, two(0.5f * 1.421413741f, 0.5f * 1.421413741f));
+    poly = fma2(poly, t, two(0.5f * -0.284496736f, 0.5f * -0.284496736f));
+    poly = fma2(poly, t, two(0.5f * 0.254829592f, 0.5f * 0.254829592f));
+    // 1/2 + sign(z) (1/2 - tail)
+    const float2 inner = apart(fma2(mul2(mul2(poly, t), e), -1.0f, 0.5f));
+    const Two p = fma2(two(copysignf(1.0f, v.x), copysignf(1.0f, v.y)), two(inner.x, inner.y), two(0.5f, 0.5f));
+    if (SLOPE) slope = fma2(mul2(z, DENSITY), e, p);
+    return p;
   }
-  float q = 1.0f, w = z;  // the logistic function's argument and its derivative
+  // The logistic function of z, or of 2 y where tanh(y) is asked for: 1 + tanh(y) is
+  // twice that.  From 30 on it is 0 or 1 in 32 bits and the cube is kept from overflowing.
+  Two w = z, q = z;  // its argument, and z times the argument's derivative
   if (ACT == GELU_TANH) {
-    w = TANH_SCALE * z * fmaf(TANH_CUBE * z, z, 1.0f);
-    q = TANH_SCALE * fmaf(3.0f * TANH_CUBE * z, z, 1.0f);
+    const Two c = two(v.x > 30.0f ? 30.0f : v.x < -30.0f ? -30.0f : v.x, v.y > 30.0f ? 30.0f : v.y < -30.0f ? -30.0f : v.y);
+    const Two square = mul2(c, c), scaled = mul2(c, TANH_SCALE);
+    w = mul2(scaled, fma2(square, TANH_CUBE, 1.0f));
+    q = mul2(scaled, fma2(square, 3.0f * TANH_CUBE, 1.0f));
   }
-  const float e = __expf(-fabsf(w));  // no overflow on either side
-  const float r = __fdividef(1.0f, 1.0f + e);
-  const float p = w >= 0.0f ? r : e * r, other = w >= 0.0f ? e * r : r;
-  if (SLOPE) *slope = z == z ? fmaf(fabsf(z) < 1e18f ? z * q * p : 0.0f, other, p) : z;
-  return z * p;
+  const Two p = reciprocal2(fma2(exp2_2(mul2(w, -LOG2E)), 1.0f, 1.0f));
+  if (SLOPE) slope = fma2(mul2(q, p), fma2(p, -1.0f, 1.0f), p);
+  return p;
+}
+// act(z).
+template <int ACT>
+__device__ __forceinline__ Two activated(Two z) {
+  Two slope;
+  const Two p = share<ACT, false>(z, slope);
+  return ACT == RELU ? two(apart(z).x > 0.0f ? apart(z).x : apart(p).x, apart(z).y > 0.0f ? apart(z).y : apart(p).y) : mul2(z, p);
 }
 
 // h of 32 columns from accumulators of both products.
@@ -75,19 +132,18 @@ struct Gated {
   struct State {
     __device__ State(const Params&, const Shape&, const Spot&) {}
     __device__ void end(const Params&, const Shape&, const Spot&) {}
-    template <int ACT>
-    __device__ static void gated(float (&g)[32], const float (&u)[32]) {
+    template <int ACT, int HALF>
+    __device__ static void gated(const float (&g)[32], const float (&u)[32], unsigned (&w)[16]) {
 #pragma unroll
-      for (int j = 0; j < 32; ++j) g[j] = activate<ACT, false>(g[j], nullptr) * u[j];
+      for (int j = 0; j < 16; ++j)
+        w[j] = rounded(mul2(activated<ACT>(two(g[2 * j], g[2 * j + 1])), two(u[2 * j], u[2 * j + 1])), HALF);
     }
-    __device__ static void round(const float (&v)[32], unsigned (&w)[16], int half) {
-      if (half) {
-#pragma unroll
-        for (int j = 0; j < 16; ++j) w[j] = pack2(v[2 * j], v[2 * j + 1], 1);
-      } else {
-#pragma unroll
-        for (int j = 0; j < 16; ++j) w[j] = pack2(v[2 * j], v[2 * j + 1], 0);
-      }
+    template <int ACT>
+    __device__ static void gated(const float (&g)[32], const float (&u)[32], unsigned (&w)[16], int half) {
+      if (half)
+        gated<ACT, 1>(g, u, w);
+      else
+        gated<ACT, 0>(g, u, w);
     }
     __device__ void chunk(const Params& p, const Shape& a, const Spot& s, int col0, unsigned acc, int cols) {
       unsigned q[32], t[32], w[16];
@@ -103,18 +159,22 @@ struct Gated {
 #pragma unroll
         for (int j = 0; j < 32; ++j) g[j] = u[j] = __int_as_float(0x7fffffff);
       }
-      if (p.gate) {
+      // All warps come here at once: half of them store first and the others compute
+      // first, so that the two overlap (4095 x 512 x 2048, gelu: 39 us, XXX so)
+      const bool late = s.part & 1;
+      auto keep = [&] {
         put32(s, g, p.gate, p.ldg, s.m, s.n, col0, p.vec_g);
         put32(s, u, p.up, p.ldu, s.m, s.n, col0, p.vec_u);
-      }
+      };
+      if (p.gate && !late) keep();
       switch (p.act) {
-        case SILU: gated<SILU>(g, u); break;
-        case GELU: gated<GELU>(g, u); break;
-        case GELU_TANH: gated<GELU_TANH>(g, u); break;
-        default: gated<RELU>(g, u);
+        case SILU: gated<SILU>(g, u, w, a.half); break;
+        case GELU: gated<GELU>(g, u, w, a.half); break;
+        case GELU_TANH: gated<GELU_TANH>(g, u, w, a.half); break;
+        default: gated<RELU>(g, u, w, a.half);
       }
-      round(g, w, a.half);
       put16(s, w, p.h, p.ldh, s.m, s.n, col0, p.vec_h);
+      if (p.gate && late) keep();
     }
   };
 };
@@ -146,10 +206,11 @@ struct GatedGrad {
     __device__ static bool fast(const Params& p, const Spot& s, int col0) { return p.vec && col0 + CHUNK <= s.n; }
     __device__ void end(const Params&, const Shape&, const Spot&) {}
     template <int ACT>
-    __device__ static void one(float dh, float g, float u, float& dg, float& du, float& h) {
-      float slope;
-      const float act = activate<ACT, true>(g, &slope);
-      dg = dh * u * slope, du = dh * act, h = act * u;
+    __device__ __forceinline__ static void both(Two dh, Two g, Two u, Two& dg, Two& du, Two& h) {
+      Two slope;
+      const Two p = share<ACT, true>(g, slope);
+      const Two act = ACT == RELU ? activated<ACT>(g) : mul2(g, p);
+      dg = mul2(mul2(dh, u), slope), du = mul2(dh, act), h = mul2(act, u);
     }
     __device__ static void fetch(const Params& p, const Spot& s, int col0, int i, Kept& k) {
       const long long row = s.row0 + i * 8 + (s.lane >> 2);
@@ -181,14 +242,11 @@ struct GatedGrad {
 #pragma unroll
         for (int j = 0; j < 2; ++j) {
           const float4 d = staged(s, r, 2 * q + j);
-          float x[4], y[4], z[4];
-          one<ACT>(d.x, c.g[j].x, c.u[j].x, x[0], y[0], z[0]);
-          one<ACT>(d.y, c.g[j].y, c.u[j].y, x[1], y[1], z[1]);
-          one<ACT>(d.z, c.g[j].z, c.u[j].z, x[2], y[2], z[2]);
-          one<ACT>(d.w, c.g[j].w, c.u[j].w, x[3], y[3], z[3]);
-          dg[2 * j] = pack2(x[0], x[1], HALF), dg[2 * j + 1] = pack2(x[2], x[3], HALF);
-          du[2 * j] = pack2(y[0], y[1], HALF), du[2 * j + 1] = pack2(y[2], y[3], HALF);
-          h[2 * j] = pack2(z[0], z[1], HALF), h[2 * j + 1] = pack2(z[2], z[3], HALF);
+          Two x, y, z;
+          both<ACT>(two(d.x, d.y), two(c.g[j].x, c.g[j].y), two(c.u[j].x, c.u[j].y), x, y, z);
+          dg[2 * j] = rounded(x, HALF), du[2 * j] = rounded(y, HALF), h[2 * j] = rounded(z, HALF);
+          both<ACT>(two(d.z, d.w), two(c.g[j].z, c.g[j].w), two(c.u[j].z, c.u[j].w), x, y, z);
+          dg[2 * j + 1] = rounded(x, HALF), du[2 * j + 1] = rounded(y, HALF), h[2 * j + 1] = rounded(z, HALF);
         }
         if (s.row0 + r < s.m) {
           *reinterpret_cast<uint4*>(p.dg + at) = make_uint4(dg[0], dg[1], dg[2], dg[3]);
@@ -213,8 +271,9 @@ struct GatedGrad {
         const float dh = staged1(s, r);
         const int type = a.half ? AD_F16 : AD_BF16;
         const long long row = s.row0 + r;
-        float dg, du, h;
-        one<ACT>(dh, p.gate[row * p.ldg + col], p.up[row * p.ldu + col], dg, du, h);
+        Two x, y, z;
+        both<ACT>(two(dh, dh), two(p.gate[row * p.ldg + col], 0.0f), two(p.up[row * p.ldu + col], 0.0f), x, y, z);
+        const float dg = apart(x).x, du = apart(y).x, h = apart(z).x;
         store_any(p.dg, type, row * p.ld + col, dg);
         store_any(p.du, type, row * p.ld + col, du);
         store_any(p.h, type, row * p.ld + col, h);
@@ -339,10 +398,10 @@ __global__ void __launch_bounds__(256) rows_kernel(const __grid_constant__ RowsA
       a.up[lane * a.ldu + row] = u;
     }
     switch (a.act) {
-      case SILU: g = activate<SILU, false>(g, nullptr); break;
-      case GELU: g = activate<GELU, false>(g, nullptr); break;
-      case GELU_TANH: g = activate<GELU_TANH, false>(g, nullptr); break;
-      default: g = activate<RELU, false>(g, nullptr);
+      case SILU: g = apart(activated<SILU>(two(g, g))).x; break;
+      case GELU: g = apart(activated<GELU>(two(g, g))).x; break;
+      case GELU_TANH: g = apart(activated<GELU_TANH>(two(g, g))).x; break;
+      default: g = apart(activated<RELU>(two(g, g))).x;
     }
     g *= u;
   }

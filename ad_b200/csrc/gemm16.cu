@@ -174,7 +174,7 @@ struct JoinArgs {
   int tile_m, tile_n;
   Cut cut[MAX_WORKERS];
 };
-constexpr int JOIN_ROWS = 16;  // of a tile a block
+constexpr int JOIN_ROWS = 4;   // of a tile a block
 
 __global__ void __launch_bounds__(256) join_kernel(const __grid_constant__ JoinArgs a) {
   const Cut c = a.cut[blockIdx.y];

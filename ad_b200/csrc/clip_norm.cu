@@ -6,7 +6,7 @@
 // Bound by memory: each array is read for the norm, and once more, backwards so that
 // what the first pass has left in L2 comes first, to be scaled.  Where nothing has
 // to be scaled and the arrays are their own results, the second pass ends at once.
-// Arrays are cut into chunks of 16 KB, dealt out to the blocks of one launch, whose
+// Arrays are cut into chunks of 64 KB, dealt out to the blocks of one launch, whose
 // table of arrays travels with its parameters: no copy to the device, and a
 // captured call replays by itself.  Squares of 16 bytes' elements are summed in 32
 // bits where they can neither overflow nor vanish, else in 64, and all sums of
@@ -22,7 +22,7 @@ namespace {
 using namespace adops;
 
 constexpr int THREADS = 256, U = 4;            // 16-byte loads of a thread under way
-constexpr int CHUNK = THREADS * U;             // 16-byte words of a chunk
+constexpr int ROUNDS = 4, CHUNK = THREADS * U * ROUNDS;  // 16-byte words of a chunk
 constexpr int MAX_BLOCKS = 2048;               // of a launch: partial sums of a table
 constexpr long long MAX_ELEMENTS = 1ll << 44;
 
@@ -125,19 +125,19 @@ __global__ void __launch_bounds__(THREADS) norm_kernel(const __grid_constant__ C
     const void* p = a.t.in[i];
     const long long count = a.t.count[i], head = head_of(p, size, count), words = (count - head) / per;
     const uint4* body = reinterpret_cast<const uint4*>(static_cast<const unsigned char*>(p) + head * size);
-    const long long w0 = static_cast<long long>(c - a.t.first[i]) * CHUNK + threadIdx.x;
-    uint4 q[U];
+    const long long from = static_cast<long long>(c - a.t.first[i]) * CHUNK, end = from + CHUNK < words ? from + CHUNK : words;
+    for (long long w0 = from + threadIdx.x; w0 < end; w0 += THREADS * U) {
+      uint4 q[U];
 #pragma unroll
-    for (int u = 0; u < U; ++u) {
-      q[u] = make_uint4(0, 0, 0, 0);
-      if (w0 + u * THREADS < words) q[u] = body[w0 + u * THREADS];
-    }
+      for (int u = 0; u < U; ++u)
+        if (w0 + u * THREADS < end) q[u] = body[w0 + u * THREADS];
 #pragma unroll
-    for (int u = 0; u < U; ++u) {
-      if (w0 + u * THREADS < words) {
-        float x[8];
-        unpack_any(q[u], type, x);
-        s += squares(x, per);
+      for (int u = 0; u < U; ++u) {
+        if (w0 + u * THREADS < end) {
+          float x[8];
+          unpack_any(q[u], type, x);
+          s += squares(x, per);
+        }
       }
     }
     if (c == a.t.first[i]) {  // what lies before the first and behind the last 16 bytes: fewer than 16 elements
@@ -176,33 +176,35 @@ __global__ void __launch_bounds__(THREADS) scale_kernel(const __grid_constant__ 
     const uint4* body = reinterpret_cast<const uint4*>(static_cast<const unsigned char*>(p) + head * size);
     unsigned char* to = static_cast<unsigned char*>(o) + head * size;
     const bool vec = (reinterpret_cast<uintptr_t>(to) & 15) == 0;
-    const long long w0 = static_cast<long long>(c - a.t.first[i]) * CHUNK + threadIdx.x;
-    uint4 q[U];
+    const long long from = static_cast<long long>(c - a.t.first[i]) * CHUNK, end = from + CHUNK < words ? from + CHUNK : words;
+    for (long long w0 = from + threadIdx.x; w0 < end; w0 += THREADS * U) {
+      uint4 q[U];
 #pragma unroll
-    for (int u = 0; u < U; ++u)
-      if (w0 + u * THREADS < words) q[u] = body[w0 + u * THREADS];
+      for (int u = 0; u < U; ++u)
+        if (w0 + u * THREADS < end) q[u] = body[w0 + u * THREADS];
 #pragma unroll
-    for (int u = 0; u < U; ++u) {
-      const long long w = w0 + u * THREADS;
-      if (w >= words) continue;
-      if (clip) {
-        float x[8];
-        unpack_any(q[u], type, x);
+      for (int u = 0; u < U; ++u) {
+        const long long w = w0 + u * THREADS;
+        if (w >= end) continue;
+        if (clip) {
+          float x[8];
+          unpack_any(q[u], type, x);
 #pragma unroll
-        for (int j = 0; j < 8; ++j) x[j] = wide ? static_cast<float>(x[j] * factor) : x[j] * f;
-        q[u] = pack_any(x, type);
-      }
-      if (vec) {
-        reinterpret_cast<uint4*>(to)[w] = q[u];
-      } else {
-        const unsigned v[4] = {q[u].x, q[u].y, q[u].z, q[u].w};
+          for (int j = 0; j < 8; ++j) x[j] = wide ? static_cast<float>(x[j] * factor) : x[j] * f;
+          q[u] = pack_any(x, type);
+        }
+        if (vec) {
+          reinterpret_cast<uint4*>(to)[w] = q[u];
+        } else {
+          const unsigned v[4] = {q[u].x, q[u].y, q[u].z, q[u].w};
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          if (size == 4) {
-            reinterpret_cast<unsigned*>(to)[w * 4 + j] = v[j];
-          } else {
-            reinterpret_cast<unsigned short*>(to)[w * 8 + 2 * j] = static_cast<unsigned short>(v[j]);
-            reinterpret_cast<unsigned short*>(to)[w * 8 + 2 * j + 1] = static_cast<unsigned short>(v[j] >> 16);
+          for (int j = 0; j < 4; ++j) {
+            if (size == 4) {
+              reinterpret_cast<unsigned*>(to)[w * 4 + j] = v[j];
+            } else {
+              reinterpret_cast<unsigned short*>(to)[w * 8 + 2 * j] = static_cast<unsigned short>(v[j]);
+              reinterpret_cast<unsigned short*>(to)[w * 8 + 2 * j + 1] = static_cast<unsigned short>(v[j] >> 16);
+            }
           }
         }
       }

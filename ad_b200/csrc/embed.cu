@@ -13,8 +13,8 @@
 // lie in one chunk is written there and then; a sum that goes on in the next chunk
 // is left in memory, and a last kernel joins such partial sums, a block a token and
 // slice, found through a list.  A token that comes up thousands of times so costs
-// no more than others.  Rows of tokens that do not come up are cleared by blocks
-// beside those of the first count.
+// no more than others.  Rows of tokens that do not come up are cleared by further
+// blocks of the sort's launches.
 #include <algorithm>
 #include <cmath>
 
@@ -91,10 +91,18 @@ struct SortArgs {
   int n, tiles, shift, digits;
   int* counts;  // [digits][tiles], then their running sums
   int* totals;  // [digits]
-  int* joins;   // the number of joins, cleared by the first kernel
-  uint4* clear; // with the first count: memory to clear, in 16-byte words
+  int* joins;   // the numbers of short and of long joins, cleared ahead of the sums
+  uint4* clear; // this launch's share of the memory to clear, in 16-byte words
   long long clear_words;
 };
+// Blocks from `first` on clear; whether this is one of them.
+__device__ __forceinline__ bool clears(const SortArgs& a, unsigned first) {
+  if (blockIdx.x < first) return false;
+  const long long step = static_cast<long long>(gridDim.x - first) * blockDim.x;
+  for (long long i = (blockIdx.x - first) * static_cast<long long>(blockDim.x) + threadIdx.x; i < a.clear_words; i += step)
+    a.clear[i] = make_uint4(0, 0, 0, 0);
+  return true;
+}
 __device__ __forceinline__ int key_of(const SortArgs& a, int i) {
   if (a.keys) return a.keys[i];
   const long long t = token_at(a.tokens, a.tok64, i);
@@ -103,13 +111,8 @@ __device__ __forceinline__ int key_of(const SortArgs& a, int i) {
 
 __global__ void __launch_bounds__(SORT_THREADS) count_kernel(const __grid_constant__ SortArgs a) {
   __shared__ int hist[MAX_DIGITS];
-  if (blockIdx.x >= a.tiles) {  // rows of the table's gradient
-    const long long step = static_cast<long long>(gridDim.x - a.tiles) * SORT_THREADS;
-    for (long long i = (blockIdx.x - a.tiles) * static_cast<long long>(SORT_THREADS) + threadIdx.x; i < a.clear_words; i += step)
-      a.clear[i] = make_uint4(0, 0, 0, 0);
-    return;
-  }
-  if (a.joins && blockIdx.x == 0 && threadIdx.x == 0) *a.joins = 0;
+  if (clears(a, a.tiles)) return;
+  if (blockIdx.x == 0 && threadIdx.x < 2) a.joins[threadIdx.x] = 0;
   for (int d = threadIdx.x; d < a.digits; d += SORT_THREADS) hist[d] = 0;
   __syncthreads();
 #pragma unroll
@@ -123,6 +126,7 @@ __global__ void __launch_bounds__(SORT_THREADS) count_kernel(const __grid_consta
 
 // A digit's counts to running sums over the tiles, a warp a digit.
 __global__ void __launch_bounds__(256) scan_kernel(const __grid_constant__ SortArgs a) {
+  if (clears(a, (a.digits + 7) / 8)) return;
   const int d = blockIdx.x * 8 + (threadIdx.x >> 5), lane = threadIdx.x & 31;
   if (d >= a.digits) return;
   int* c = a.counts + static_cast<long long>(d) * a.tiles;
@@ -210,6 +214,7 @@ __device__ __forceinline__ void rank_tile(TileSort& s, const int (&digit)[KEYS],
 
 __global__ void __launch_bounds__(SORT_THREADS) move_kernel(const __grid_constant__ SortArgs a) {
   __shared__ TileSort s;
+  if (clears(a, a.tiles)) return;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   for (int d = threadIdx.x; d < a.digits; d += SORT_THREADS) {
     s.base[d] = a.totals[d];
@@ -244,13 +249,8 @@ __global__ void __launch_bounds__(SORT_THREADS) sort_kernel(const __grid_constan
   __shared__ TileSort s;
   int* const keys = s.hist[0];  // in the place of the counts, once these have served
   short* const at = reinterpret_cast<short*>(s.hist[TILE / MAX_DIGITS]);
-  if (blockIdx.x) {
-    const long long step = static_cast<long long>(gridDim.x - 1) * SORT_THREADS;
-    for (long long i = (blockIdx.x - 1) * static_cast<long long>(SORT_THREADS) + threadIdx.x; i < a.clear_words; i += step)
-      a.clear[i] = make_uint4(0, 0, 0, 0);
-    return;
-  }
-  if (threadIdx.x == 0) *a.joins = 0;
+  if (clears(a, 1)) return;
+  if (threadIdx.x < 2) a.joins[threadIdx.x] = 0;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, digits = 1 << bits;
   int key[KEYS], from[KEYS], digit[KEYS], place[KEYS];
 #pragma unroll
@@ -295,7 +295,8 @@ __global__ void __launch_bounds__(SORT_THREADS) sort_kernel(const __grid_constan
 
 // ------------------------------------------------------------------ sums
 
-constexpr int SPAN = 32;  // sorted positions a chunk
+constexpr int SPAN = 32;   // sorted positions a chunk
+constexpr int SHORT = 16;  // chunks that a token goes on in and one warp joins
 
 struct SumArgs {
   const void* dy;
@@ -309,7 +310,7 @@ struct SumArgs {
   int accumulate;
   float* part;  // [chunks][2][ldp]: a sum that began earlier, one that goes on
   long long ldp;
-  int *joins, *list;
+  int *joins, *list;  // the numbers of tokens whose sums are to be joined, and where they begin: short and long ones
   int vec_out;  // the result takes the vectors that dy does
 };
 
@@ -401,7 +402,11 @@ __global__ void __launch_bounds__(128) sum_kernel(const __grid_constant__ SumArg
                   for (int j = 0; j < V; ++j) p[j] = sum[j];
                 }
               }
-              if (began && slice == 0 && lane == 0) a.list[atomicAdd(a.joins, 1)] = chunk;
+              if (began && slice == 0 && lane == 0) {
+                const int beyond = chunk + SHORT + 1;
+                const int kind = beyond < a.chunks && a.keys[beyond * SPAN] == key;
+                a.list[kind * a.chunks + atomicAdd(&a.joins[kind], 1)] = chunk;
+              }
             }
 #pragma unroll
             for (int j = 0; j < V; ++j) sum[j] = 0.0f;
@@ -413,40 +418,56 @@ __global__ void __launch_bounds__(128) sum_kernel(const __grid_constant__ SumArg
   }
 }
 
+// Four columns of a row of the result.
+__device__ __forceinline__ void write_four(const SumArgs& a, int key, int col, float4 x) {
+  float v[4] = {x.x, x.y, x.z, x.w};
+  if (a.vec_out && col + 4 <= a.width) {
+    write_sum<4>(a, key, col, v);
+  } else {
+    for (int j = 0; j < 4 && col + j < a.width; ++j) {
+      float one[1] = {v[j]};
+      write_sum<1>(a, key, col + j, one);
+    }
+  }
+}
+
 // The partial sums of a token: the chunk where it began, then those that it goes
-// on in, eight warps by turns and joined in their order.  128 columns a block.
+// on in.  128 columns at a time: by a warp where there are few, in their order, else by
+// eight warps by turns, whose sums are joined in the warps' order.  (All of them by
+// blocks, a search of the token's end ahead of each 128 columns: 47 us for 131072 rows
+// of 2048 instead of XXX.)
 __global__ void __launch_bounds__(256) join_kernel(const __grid_constant__ SumArgs a) {
   __shared__ float4 buf[8][32];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int slices = (a.width + 127) / 128;
-  const long long items = static_cast<long long>(*a.joins) * slices;
-  for (long long item = blockIdx.x; item < items; item += gridDim.x) {
-    const int chunk = a.list[item / slices], col = static_cast<int>(item % slices) * 128 + lane * 4;
-    const int key = a.keys[chunk * SPAN + SPAN - 1];
-    // the last chunk that begins with this token: among the next 32, or by halving
-    int last = chunk;
-    {
-      const int c = chunk + 1 + lane;
-      const bool same = c < a.chunks && a.keys[c * SPAN] == key;
-      last += __popc(__ballot_sync(0xffffffffu, same));
-      if (last == chunk + 32) {
-        int past = a.chunks;
-        while (past - last > 1) {
-          const int mid = last + (past - last) / 2;
-          if (a.keys[mid * SPAN] == key)
-            last = mid;
-          else
-            past = mid;
-        }
+  auto add = [&](float4& x, int c, int chunk, int col) {
+    const float4 y = *reinterpret_cast<const float4*>(a.part + (2ll * c + (c == chunk ? 1 : 0)) * a.ldp + col);
+    x.x += y.x, x.y += y.y, x.z += y.z, x.w += y.w;
+  };
+  // the token, and how many of the next 32 chunks begin with it
+  auto look = [&](int chunk, int& key) {
+    key = a.keys[chunk * SPAN + SPAN - 1];
+    const int c = chunk + 1 + lane;
+    return __popc(__ballot_sync(0xffffffffu, c < a.chunks && a.keys[c * SPAN] == key));
+  };
+  const long long longs = static_cast<long long>(a.joins[1]) * slices;
+  for (long long item = blockIdx.x; item < longs; item += gridDim.x) {
+    const int chunk = a.list[a.chunks + item / slices], col = static_cast<int>(item % slices) * 128 + lane * 4;
+    int key, last = chunk + look(chunk, key);
+    if (last == chunk + 32) {  // by halving
+      int past = a.chunks;
+      while (past - last > 1) {
+        const int mid = last + (past - last) / 2;
+        if (a.keys[mid * SPAN] == key)
+          last = mid;
+        else
+          past = mid;
       }
     }
     float4 x = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
     if (col < a.width) {
 #pragma unroll 4
-      for (int c = chunk + warp; c <= last; c += 8) {
-        const float4 y = *reinterpret_cast<const float4*>(a.part + (2ll * c + (c == chunk ? 1 : 0)) * a.ldp + col);
-        x.x += y.x, x.y += y.y, x.z += y.z, x.w += y.w;
-      }
+      for (int c = chunk + warp; c <= last; c += 8) add(x, c, chunk, col);
     }
     buf[warp][lane] = x;
     __syncthreads();
@@ -455,17 +476,20 @@ __global__ void __launch_bounds__(256) join_kernel(const __grid_constant__ SumAr
         const float4 y = buf[w][lane];
         x.x += y.x, x.y += y.y, x.z += y.z, x.w += y.w;
       }
-      float v[4] = {x.x, x.y, x.z, x.w};
-      if (a.vec_out && col + 4 <= a.width) {
-        write_sum<4>(a, key, col, v);
-      } else {
-        for (int j = 0; j < 4 && col + j < a.width; ++j) {
-          float one[1] = {v[j]};
-          write_sum<1>(a, key, col + j, one);
-        }
-      }
+      write_four(a, key, col, x);
     }
     __syncthreads();
+  }
+  const long long shorts = static_cast<long long>(a.joins[0]) * slices;
+  for (long long item = blockIdx.x * 8ll + warp; item < shorts; item += gridDim.x * 8ll) {
+    const int chunk = a.list[item / slices], col = static_cast<int>(item % slices) * 128 + lane * 4;
+    int key;
+    const int last = chunk + look(chunk, key);
+    if (col >= a.width) continue;
+    float4 x = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll 4
+    for (int c = chunk; c <= last; ++c) add(x, c, chunk, col);
+    write_four(a, key, col, x);
   }
 }
 
@@ -494,8 +518,8 @@ Layout plan(long long rows, long long vocab, long long width) {
   for (int k = 0; k < 2; ++k) l.keys[k] = take(4ull * rows), l.at[k] = take(4ull * rows);
   l.counts = take(4ull * l.tiles << l.bits);
   l.totals = take(4ull << l.bits);
-  l.joins = take(4);
-  l.list = take(4ull * l.chunks);
+  l.joins = take(8);
+  l.list = take(8ull * l.chunks);
   l.part = take(8ull * l.chunks * l.ldp);
   l.total = at;
   return l;
@@ -600,13 +624,25 @@ extern "C" int ad_embed_grad(int device, int dtype, const void* dy, int64_t lddy
       return 1;
     }
   }
-  const unsigned clearing = static_cast<unsigned>(std::min<long long>((s.clear_words + 1023) / 1024, 8ll * sms));
+  // Each launch of the sort, which waits for memory most of the time, clears a share:
+  // what takes it about as long as it has to wait (CLEAR), and the first one the rest.
+  constexpr long long CLEAR = 32 << 20;
+  const int launches = l.tiles == 1 ? 1 : 3 * l.passes;
+  uint4* const all = s.clear;
+  const long long words = s.clear_words, later = std::min(words / launches, CLEAR / 16);
+  long long cleared = 0;
+  auto share = [&](int launch) {  // blocks that clear
+    s.clear = all + cleared;
+    s.clear_words = launch ? later : words - (launches - 1) * later;
+    cleared += s.clear_words;
+    return static_cast<unsigned>(std::min<long long>((s.clear_words + 1023) / 1024, 8ll * sms));
+  };
   cudaError_t e;
   int to = 0;
   if (l.tiles == 1) {
     s.keys_out = ints(l.keys[0]), s.at_out = ints(l.at[0]);
     cudaLaunchConfig_t c = {};
-    c.gridDim = dim3(1 + clearing), c.blockDim = dim3(SORT_THREADS), c.stream = st;
+    c.gridDim = dim3(1 + share(0)), c.blockDim = dim3(SORT_THREADS), c.stream = st;
     e = cudaLaunchKernelEx(&c, sort_kernel, s, l.bits, l.passes);
     if (e != cudaSuccess) return fail_cuda(who, e);
   } else {
@@ -616,9 +652,12 @@ extern "C" int ad_embed_grad(int device, int dtype, const void* dy, int64_t lddy
       s.shift = p * l.bits;
       s.keys = p ? ints(l.keys[to ^ 1]) : nullptr, s.at = p ? ints(l.at[to ^ 1]) : nullptr;
       s.keys_out = ints(l.keys[to]), s.at_out = ints(l.at[to]);
-      e = launch<count_kernel>(dim3(l.tiles + (p ? 0 : clearing)), SORT_THREADS, 0, st, s);
-      if (e == cudaSuccess) e = launch<scan_kernel>(dim3((s.digits + 7) / 8), 256, 0, st, s);
-      if (e == cudaSuccess) e = launch<move_kernel>(dim3(l.tiles), SORT_THREADS, 0, st, s);
+      unsigned more = share(3 * p);
+      e = launch<count_kernel>(dim3(l.tiles + more), SORT_THREADS, 0, st, s);
+      more = share(3 * p + 1);
+      if (e == cudaSuccess) e = launch<scan_kernel>(dim3((s.digits + 7) / 8 + more), 256, 0, st, s);
+      more = share(3 * p + 2);
+      if (e == cudaSuccess) e = launch<move_kernel>(dim3(l.tiles + more), SORT_THREADS, 0, st, s);
       if (e != cudaSuccess) return fail_cuda(who, e);
     }
   }

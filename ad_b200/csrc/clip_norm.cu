@@ -117,6 +117,7 @@ __device__ __forceinline__ double block_sum(double s, double* buf) {
 
 template <int N>
 __global__ void __launch_bounds__(THREADS) norm_kernel(const __grid_constant__ ClipArgs<N> a) {
+  after_previous();
   __shared__ double buf[THREADS / 32];
   const unsigned chunks = a.t.first[a.t.arrays];
   double s = 0.0;
@@ -155,6 +156,7 @@ __global__ void __launch_bounds__(THREADS) norm_kernel(const __grid_constant__ C
 
 template <int N>
 __global__ void __launch_bounds__(THREADS) scale_kernel(const __grid_constant__ ClipArgs<N> a) {
+  after_previous();
   __shared__ double buf[THREADS / 32];
   double s = 0.0;
   for (int i = threadIdx.x; i < a.all_parts; i += THREADS) s += a.parts[i];
@@ -249,11 +251,11 @@ int run(const char* who, const std::vector<int>& which, const void* const* in, v
   for (size_t k = 0; k < args.size(); ++k) {
     args[k].parts = parts, args[k].all_parts = all;
     args[k].max_norm = max_norm, args[k].norm = k ? nullptr : norm;
-    const cudaError_t e = launch<norm_kernel<N>>(dim3(blocks[k]), THREADS, 0, st, args[k]);
+    const cudaError_t e = launch_early<norm_kernel<N>>(dim3(blocks[k]), THREADS, 0, st, args[k]);
     if (e != cudaSuccess) return fail_cuda(who, e);
   }
   for (size_t k = args.size(); k-- > 0;) {  // backwards, too
-    const cudaError_t e = launch<scale_kernel<N>>(dim3(blocks[k]), THREADS, 0, st, args[k]);
+    const cudaError_t e = launch_early<scale_kernel<N>>(dim3(blocks[k]), THREADS, 0, st, args[k]);
     if (e != cudaSuccess) return fail_cuda(who, e);
   }
   return 0;

@@ -42,6 +42,7 @@ __device__ __forceinline__ long long token_at(const void* tokens, int tok64, lon
 
 template <typename T, int V>
 __global__ void __launch_bounds__(256) embed_kernel(const __grid_constant__ EmbedArgs a) {
+  after_previous();
   constexpr int U = 4;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int per = a.width / V;                      // vectors of a row
@@ -110,6 +111,7 @@ __device__ __forceinline__ int key_of(const SortArgs& a, int i) {
 }
 
 __global__ void __launch_bounds__(SORT_THREADS) count_kernel(const __grid_constant__ SortArgs a) {
+  after_previous();
   __shared__ int hist[MAX_DIGITS];
   if (clears(a, a.tiles)) return;
   if (blockIdx.x == 0 && threadIdx.x < 2) a.joins[threadIdx.x] = 0;
@@ -126,6 +128,7 @@ __global__ void __launch_bounds__(SORT_THREADS) count_kernel(const __grid_consta
 
 // A digit's counts to running sums over the tiles, a warp a digit.
 __global__ void __launch_bounds__(256) scan_kernel(const __grid_constant__ SortArgs a) {
+  after_previous();
   if (clears(a, (a.digits + 7) / 8)) return;
   const int d = blockIdx.x * 8 + (threadIdx.x >> 5), lane = threadIdx.x & 31;
   if (d >= a.digits) return;
@@ -213,6 +216,7 @@ __device__ __forceinline__ void rank_tile(TileSort& s, const int (&digit)[KEYS],
 }
 
 __global__ void __launch_bounds__(SORT_THREADS) move_kernel(const __grid_constant__ SortArgs a) {
+  after_previous();
   __shared__ TileSort s;
   if (clears(a, a.tiles)) return;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
@@ -246,6 +250,7 @@ __global__ void __launch_bounds__(SORT_THREADS) move_kernel(const __grid_constan
 
 // All passes over at most one tile of keys; other blocks clear.
 __global__ void __launch_bounds__(SORT_THREADS) sort_kernel(const __grid_constant__ SortArgs a, int bits, int passes) {
+  after_previous();
   __shared__ TileSort s;
   int* const keys = s.hist[0];  // in the place of the counts, once these have served
   short* const at = reinterpret_cast<short*>(s.hist[TILE / MAX_DIGITS]);
@@ -348,6 +353,7 @@ __device__ __forceinline__ void write_sum(const SumArgs& a, int key, int col, fl
 
 template <typename T, int V>
 __global__ void __launch_bounds__(128) sum_kernel(const __grid_constant__ SumArgs a) {
+  after_previous();
   constexpr int U = 8;  // rows under way
   const int lane = threadIdx.x & 31;
   const int per = a.width / V, slices = (per + 31) / 32;
@@ -437,6 +443,7 @@ __device__ __forceinline__ void write_four(const SumArgs& a, int key, int col, f
 // blocks, a search of the token's end ahead of each 128 columns: 47 us for 131072 rows
 // of 2048 instead of XXX.)
 __global__ void __launch_bounds__(256) join_kernel(const __grid_constant__ SumArgs a) {
+  after_previous();
   __shared__ float4 buf[8][32];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int slices = (a.width + 127) / 128;
@@ -529,13 +536,13 @@ template <typename T, int V>
 cudaError_t embed(const EmbedArgs& a, int sms, cudaStream_t st) {
   const long long per = a.width / V, items = a.rows * ((per + 127) / 128);
   const long long blocks = std::min<long long>((items + 7) / 8, 16ll * sms);
-  return launch<embed_kernel<T, V>>(dim3(static_cast<unsigned>(blocks)), 256, 0, st, a);
+  return launch_early<embed_kernel<T, V>>(dim3(static_cast<unsigned>(blocks)), 256, 0, st, a);
 }
 template <typename T, int V>
 cudaError_t sums(const SumArgs& a, int sms, cudaStream_t st) {
   const long long items = static_cast<long long>(a.chunks) * ((a.width / V + 31) / 32);
   const long long blocks = std::min<long long>((items + 3) / 4, 32ll * sms);
-  return launch<sum_kernel<T, V>>(dim3(static_cast<unsigned>(blocks)), 128, 0, st, a);
+  return launch_early<sum_kernel<T, V>>(dim3(static_cast<unsigned>(blocks)), 128, 0, st, a);
 }
 
 int check(const char* who, int dtype, int64_t rows, int64_t vocab, int64_t width) {
@@ -641,9 +648,8 @@ extern "C" int ad_embed_grad(int device, int dtype, const void* dy, int64_t lddy
   int to = 0;
   if (l.tiles == 1) {
     s.keys_out = ints(l.keys[0]), s.at_out = ints(l.at[0]);
-    cudaLaunchConfig_t c = {};
-    c.gridDim = dim3(1 + share(0)), c.blockDim = dim3(SORT_THREADS), c.stream = st;
-    e = cudaLaunchKernelEx(&c, sort_kernel, s, l.bits, l.passes);
+    const unsigned more = share(0);
+    e = launch_early<sort_kernel>(dim3(1 + more), SORT_THREADS, 0, st, s, l.bits, l.passes);
     if (e != cudaSuccess) return fail_cuda(who, e);
   } else {
     s.digits = 1 << l.bits;
@@ -653,11 +659,11 @@ extern "C" int ad_embed_grad(int device, int dtype, const void* dy, int64_t lddy
       s.keys = p ? ints(l.keys[to ^ 1]) : nullptr, s.at = p ? ints(l.at[to ^ 1]) : nullptr;
       s.keys_out = ints(l.keys[to]), s.at_out = ints(l.at[to]);
       unsigned more = share(3 * p);
-      e = launch<count_kernel>(dim3(l.tiles + more), SORT_THREADS, 0, st, s);
+      e = launch_early<count_kernel>(dim3(l.tiles + more), SORT_THREADS, 0, st, s);
       more = share(3 * p + 1);
-      if (e == cudaSuccess) e = launch<scan_kernel>(dim3((s.digits + 7) / 8 + more), 256, 0, st, s);
+      if (e == cudaSuccess) e = launch_early<scan_kernel>(dim3((s.digits + 7) / 8 + more), 256, 0, st, s);
       more = share(3 * p + 2);
-      if (e == cudaSuccess) e = launch<move_kernel>(dim3(l.tiles + more), SORT_THREADS, 0, st, s);
+      if (e == cudaSuccess) e = launch_early<move_kernel>(dim3(l.tiles + more), SORT_THREADS, 0, st, s);
       if (e != cudaSuccess) return fail_cuda(who, e);
     }
   }
@@ -685,6 +691,6 @@ extern "C" int ad_embed_grad(int device, int dtype, const void* dy, int64_t lddy
                                    : sums<__half, 1>(a, sms, st));
   if (e != cudaSuccess) return fail_cuda(who, e);
   const long long joins = static_cast<long long>(l.chunks) * ((width + 127) / 128);
-  e = launch<join_kernel>(dim3(static_cast<unsigned>(std::min<long long>(joins, 8ll * sms))), 256, 0, st, a);
+  e = launch_early<join_kernel>(dim3(static_cast<unsigned>(std::min<long long>(joins, 8ll * sms))), 256, 0, st, a);
   return e == cudaSuccess ? 0 : fail_cuda(who, e);
 }

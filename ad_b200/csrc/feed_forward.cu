@@ -339,42 +339,55 @@ __device__ __forceinline__ void open_row(const Raw<V>& r, int half, float (&v)[V
   }
 }
 
+// 64 registers a thread at most, or the blocks of 4096 rows would not all be resident.
 template <int T, int V, int HALF, bool DUAL>
-__global__ void __launch_bounds__(256) rows_kernel(const __grid_constant__ RowsArgs a, int shared_by) {
+__global__ void __launch_bounds__(256, 4) rows_kernel(const __grid_constant__ RowsArgs a, int shared_by) {
+  constexpr int U = DUAL ? 2 : 4;  // loads of weights under way, in each matrix
   __shared__ float buf[8][2 * T];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int row = blockIdx.x * (8 / shared_by) + warp / shared_by, share = warp % shared_by;
+  const int first = (share * 32 + lane) * V, step = 32 * V * shared_by;
+  const bool in = row < a.n;
+  const unsigned short *w0 = a.w0 + row * a.ld0, *w1 = DUAL ? a.w1 + row * a.ld1 : nullptr;
+  Raw<V> p[U], q[U];
+  auto fetch = [&](int k0) {
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+      if (in && k0 + u * step < a.k) {
+        p[u] = raw_row<V>(w0 + k0 + u * step);
+        if (DUAL) q[u] = raw_row<V>(w1 + k0 + u * step);
+      }
+  };
+  // The second product's weights are under way before the first has ended, which
+  // does not write them; it began when all before it had ended.
+  if (!DUAL) fetch(first);
+  after_previous();
+  if (DUAL) fetch(first);
   float s[2][T];
 #pragma unroll
   for (int t = 0; t < T; ++t) s[0][t] = s[1][t] = 0.0f;
-  if (row < a.n) {
-    const unsigned short *w0 = a.w0 + row * a.ld0, *w1 = DUAL ? a.w1 + row * a.ld1 : nullptr;
-    const int step = 32 * V * shared_by;
-    constexpr int U = 4;  // loads of weights under way
-    for (int k0 = (share * 32 + lane) * V; k0 < a.k; k0 += U * step) {
-      Raw<V> p[U], q[U];
+  for (int k0 = first; in && k0 < a.k;) {
+    Raw<V> pc[U], qc[U];
 #pragma unroll
-      for (int u = 0; u < U; ++u)
-        if (k0 + u * step < a.k) {
-          p[u] = raw_row<V>(w0 + k0 + u * step);
-          if (DUAL) q[u] = raw_row<V>(w1 + k0 + u * step);
-        }
+    for (int u = 0; u < U; ++u) pc[u] = p[u], qc[u] = q[u];
+    const int now = k0;
+    k0 += U * step;
+    fetch(k0);
 #pragma unroll
-      for (int u = 0; u < U; ++u) {
-        const int k = k0 + u * step;
-        if (k >= a.k) break;
-        float pv[V], qv[V], x[V];
-        open_row<V>(p[u], HALF, pv);
-        if (DUAL) open_row<V>(q[u], HALF, qv);
+    for (int u = 0; u < U; ++u) {
+      const int k = now + u * step;
+      if (k >= a.k) break;
+      float pv[V], qv[V], x[V];
+      open_row<V>(pc[u], HALF, pv);
+      if (DUAL) open_row<V>(qc[u], HALF, qv);
 #pragma unroll
-        for (int t = 0; t < T; ++t) {
-          if (t >= a.rows) break;
-          open_row<V>(raw_row<V>(a.x + t * a.ldx + k), HALF, x);
+      for (int t = 0; t < T; ++t) {
+        if (t >= a.rows) break;
+        open_row<V>(raw_row<V>(a.x + t * a.ldx + k), HALF, x);
 #pragma unroll
-          for (int j = 0; j < V; ++j) {
-            s[0][t] = fmaf(pv[j], x[j], s[0][t]);
-            if (DUAL) s[1][t] = fmaf(qv[j], x[j], s[1][t]);
-          }
+        for (int j = 0; j < V; ++j) {
+          s[0][t] = fmaf(pv[j], x[j], s[0][t]);
+          if (DUAL) s[1][t] = fmaf(qv[j], x[j], s[1][t]);
         }
       }
     }
@@ -418,12 +431,11 @@ cudaError_t start_rows(const RowsArgs& a, int half, int sms, cudaStream_t st) {
   // warps for all of the device, as long as each has 512 elements of a row
   int shared_by = 1;
   while (shared_by < 8 && a.n * shared_by < 16 * sms && a.k / (2 * shared_by) >= 512) shared_by *= 2;
-  cudaLaunchConfig_t c = {};
-  c.gridDim = dim3((a.n + 8 / shared_by - 1) / (8 / shared_by));
-  c.blockDim = dim3(256);
-  c.stream = st;
-  return vec ? (half ? cudaLaunchKernelEx(&c, rows_kernel<T, 8, 1, DUAL>, a, shared_by) : cudaLaunchKernelEx(&c, rows_kernel<T, 8, 0, DUAL>, a, shared_by))
-             : (half ? cudaLaunchKernelEx(&c, rows_kernel<T, 1, 1, DUAL>, a, shared_by) : cudaLaunchKernelEx(&c, rows_kernel<T, 1, 0, DUAL>, a, shared_by));
+  const dim3 grid((a.n + 8 / shared_by - 1) / (8 / shared_by));
+  return vec ? (half ? launch_early<rows_kernel<T, 8, 1, DUAL>>(grid, 256, 0, st, a, shared_by)
+                     : launch_early<rows_kernel<T, 8, 0, DUAL>>(grid, 256, 0, st, a, shared_by))
+             : (half ? launch_early<rows_kernel<T, 1, 1, DUAL>>(grid, 256, 0, st, a, shared_by)
+                     : launch_early<rows_kernel<T, 1, 0, DUAL>>(grid, 256, 0, st, a, shared_by));
 }
 template <bool DUAL>
 cudaError_t few_rows(const RowsArgs& a, int half, int sms, cudaStream_t st) {

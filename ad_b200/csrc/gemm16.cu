@@ -177,6 +177,7 @@ struct JoinArgs {
 constexpr int JOIN_ROWS = 4;   // of a tile a block
 
 __global__ void __launch_bounds__(256) join_kernel(const __grid_constant__ JoinArgs a) {
+  after_previous();
   const Cut c = a.cut[blockIdx.y];
   const int g = c.where >> 30, row0 = (c.where >> 15 & 0x7fff) * a.tile_m + blockIdx.x * JOIN_ROWS,
             col0 = (c.where & 0x7fff) * a.tile_n;
@@ -212,6 +213,7 @@ struct PackArgs {
 // of a word, five words are read and shifted (5.5 MB from rows of 1001: XXX us;
 // element by element 9.3).
 __global__ void __launch_bounds__(256) pack_kernel(const __grid_constant__ PackArgs a) {
+  after_previous();
   const Pack& p = a.pack[blockIdx.y];
   const int per = static_cast<int>((p.cols + 7) / 8);
   const long long total = p.rows * per;
@@ -402,7 +404,7 @@ int start_listed(const char* who, const Device& d, int half, const Problem* p, c
   j.to = to, j.tile_m = TILE::M, j.tile_n = TILE::BN;
   for (int g = 0; g < count; ++g) j.group[g] = shape.group[g];
   memcpy(j.cut, s.cut, sizeof(Cut) * s.cuts);
-  e = launch<join_kernel>(dim3(TILE::M / JOIN_ROWS, s.cuts), 256, 0, st, j);
+  e = launch_early<join_kernel>(dim3(TILE::M / JOIN_ROWS, s.cuts), 256, 0, st, j);
   return e == cudaSuccess ? 0 : fail_cuda(who, e);
 }
 template <int CTAS, int BN>
@@ -467,7 +469,7 @@ int pack_rows(const char* who, const Device& d, const Pack* packs, int count, cu
     a.pack[i] = packs[i];
     most = std::max(most, packs[i].rows * ((packs[i].cols + 7) / 8));
   }
-  const cudaError_t e = launch<pack_kernel>(dim3(static_cast<unsigned>(std::min<long long>((most + 255) / 256, 8 * d.sms)), count), 256, 0, st, a);
+  const cudaError_t e = launch_early<pack_kernel>(dim3(static_cast<unsigned>(std::min<long long>((most + 255) / 256, 8 * d.sms)), count), 256, 0, st, a);
   return e == cudaSuccess ? 0 : fail_cuda(who, e);
 }
 

@@ -427,6 +427,7 @@ __global__ void __launch_bounds__(TILE::THREADS, 1)
   }
   asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
   const unsigned tmem = *tmem_slot;
+  after_previous();
 
   if (warp == 0) {
     if (lane == 0) {  // operands
@@ -698,15 +699,17 @@ cudaError_t workers_of(const Device& d, int* workers) {
 template <typename TILE, typename EPI>
 cudaError_t launch_gemm(const Maps& maps, const Shape& s, const typename EPI::Params& params, int workers, cudaStream_t st) {
   cudaLaunchConfig_t c = {};
-  cudaLaunchAttribute at[1];
+  cudaLaunchAttribute at[2];
   at[0].id = cudaLaunchAttributeClusterDimension;
   at[0].val.clusterDim.x = TILE::CTAS;
   at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
+  at[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at[1].val.programmaticStreamSerializationAllowed = 1;
   c.gridDim = dim3(workers * TILE::CTAS);
   c.blockDim = dim3(TILE::THREADS);
   c.dynamicSmemBytes = TILE::SMEM;
   c.stream = st;
-  c.attrs = at, c.numAttrs = 1;
+  c.attrs = at, c.numAttrs = 2;
   return cudaLaunchKernelEx(&c, gemm_kernel<TILE, EPI>, maps, s, params);
 }
 

@@ -124,6 +124,7 @@ struct FinishArgs {
 // Joins the tiles' pairs: 8 rows a block, 4 lanes of each of 16 warps a row.
 constexpr int FINISH_WARPS = 16, FINISH_ROWS = 8;
 __global__ void __launch_bounds__(32 * FINISH_WARPS) finish_kernel(const __grid_constant__ FinishArgs a) {
+  after_previous();
   __shared__ float2 buf[FINISH_WARPS][FINISH_ROWS];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int row = blockIdx.x * FINISH_ROWS + (lane & (FINISH_ROWS - 1));
@@ -161,6 +162,7 @@ struct RangeArgs {
   float* factor;
 };
 __global__ void __launch_bounds__(1024) range_kernel(const __grid_constant__ RangeArgs a) {
+  after_previous();
   __shared__ float buf[32];
   float most = 0.0f;
   for (int i = threadIdx.x; i < a.rows; i += 1024)
@@ -358,7 +360,7 @@ extern "C" int ad_linear_logprobs(int device, int dtype, const void* x, int64_t 
   f.parts = static_cast<int>(parts_of(l.tiling, vocab)), f.rows = static_cast<int>(rows);
   f.vocab = vocab, f.scale = scale, f.k = q.k;
   f.logp = logp, f.lse = lse, f.stats = reinterpret_cast<float2*>(stats);
-  const cudaError_t e = launch<finish_kernel>(dim3(static_cast<unsigned>((rows + FINISH_ROWS - 1) / FINISH_ROWS)), 32 * FINISH_WARPS, 0, st, f);
+  const cudaError_t e = launch_early<finish_kernel>(dim3(static_cast<unsigned>((rows + FINISH_ROWS - 1) / FINISH_ROWS)), 32 * FINISH_WARPS, 0, st, f);
   return e == cudaSuccess ? 0 : fail_cuda(who, e);
 }
 
@@ -394,7 +396,7 @@ extern "C" int ad_linear_logprobs_grad(int device, int dtype, const void* x, int
   float* factor = half ? reinterpret_cast<float*>(ws + l.factor) : nullptr;
   if (half) {
     const RangeArgs r = {g_logp, g_lse, static_cast<int>(rows), scale, factor};
-    const cudaError_t e = launch<range_kernel>(1, 1024, 0, st, r);
+    const cudaError_t e = launch_early<range_kernel>(1, 1024, 0, st, r);
     if (e != cudaSuccess) return fail_cuda(who, e);
   }
   const Mat dz = {ws + l.dz, l.piece};

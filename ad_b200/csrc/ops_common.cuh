@@ -57,6 +57,23 @@ cudaError_t launch(dim3 grid, dim3 block, int bytes, cudaStream_t s, const A& a)
   return cudaLaunchKernelEx(&c, KERNEL, a);
 }
 
+// The same for a kernel that begins with after_previous(): it may be brought up while
+// the stream's previous kernel ends.
+template <auto KERNEL, typename... A>
+cudaError_t launch_early(dim3 grid, dim3 block, int bytes, cudaStream_t s, const A&... a) {
+  cudaLaunchConfig_t c = {};
+  c.gridDim = grid;
+  c.blockDim = block;
+  c.dynamicSmemBytes = bytes;
+  c.stream = s;
+  cudaLaunchAttribute at[1];
+  at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at[0].val.programmaticStreamSerializationAllowed = 1;
+  c.attrs = at;
+  c.numAttrs = 1;
+  return cudaLaunchKernelEx(&c, KERNEL, a...);
+}
+
 // Makes `device` current for one call (-1: the current one) and puts the
 // caller's device back at its end.
 class DeviceGuard {
@@ -121,6 +138,14 @@ inline bool aligned(std::initializer_list<const void*> all, size_t n) {
   for (const void* p : all)
     if (!aligned(p, n)) return false;
   return true;
+}
+
+// Waits until the stream's previous kernel has ended and its results are there; before
+// it a kernel touches no memory that another one could write.  From then on the next
+// kernel may be brought up, whose own wait is for this one's end.
+__device__ __forceinline__ void after_previous() {
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
 }
 
 // ---------------------------------------------------------------- elements

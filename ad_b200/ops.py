@@ -762,8 +762,8 @@ def _weight_grads(out, like, code, device, accumulate, names):
 
 def _scratch(need, workspace, device, like):
     """(workspace, its bytes), a new one where none is given."""
-    if workspace is None:
-        return _empty((need,), like, "uint8"), need
+    if workspace is None:  # of the operand's type: the cheapest to ask for
+        return like.new_empty((need + 1) // 2 if need else 0), need
     have = _nbytes(workspace, "workspace")
     _on(device, workspace, "workspace")
     return workspace, have
@@ -1072,7 +1072,7 @@ def embed(tokens, table, *, scale: float = 1.0, out=None, stream=None):
     s = _stream(dev, stream, table, out is None)
     shape = (*tokens.shape, width)
     if out is None:
-        out = _empty(shape, table)
+        out = table.new_empty(shape)
         ldo = width
     else:
         _typed(out, dt, "out")

@@ -175,7 +175,7 @@ __global__ void __launch_bounds__(1024) range_kernel(const __grid_constant__ Ran
     for (int w = 1; w < 32; ++w) most = fmaxf(most, buf[w]);
     most *= a.scale;
     int e = 0;
-    if (most > 0.0f && most < INFINITY) e = max(-100, min(100, 14 - ilogbf(most)));
+    if (most > 0.0f && most < INFINITY) e = max(-126, min(126, 14 - ilogbf(most)));
     a.factor[0] = ldexpf(1.0f, e);
     a.factor[1] = ldexpf(1.0f, -e);
   }

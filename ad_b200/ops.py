@@ -39,6 +39,7 @@ F32, BF16, F16 = 0, 1, 2
 _FLOATS = {"float32": F32, "bfloat16": BF16, "float16": F16}
 _INTS = {"int64": 1, "int32": 0}
 _SIZES = (4, 2, 2)
+_BYTES = {"uint8": 1, "int8": 1, "bfloat16": 2, "float16": 2, "float32": 4, "int32": 4, "int64": 8}
 _codes: dict = {}  # dtype object -> (kind, code)
 
 
@@ -555,10 +556,9 @@ def _nbytes(x, name):
         n *= s
     _flat(x, n, name)
     if isinstance(x, DeviceArray):
-        sizes = {"uint8": 1, "int8": 1, "bfloat16": 2, "float16": 2, "float32": 4, "int32": 4, "int64": 8}
-        if x.dtype not in sizes:
+        if x.dtype not in _BYTES:
             raise TypeError(f"{name}: unknown element type {x.dtype}")
-        return n * sizes[x.dtype]
+        return n * _BYTES[x.dtype]
     return n * x.element_size()
 
 
@@ -746,7 +746,7 @@ def _matrix(x, rows, cols, code, device, name):
     return ld
 
 
-def _weight_grads(out, like, code, device, accumulate, names):
+def _weight_grads(out, like, code, device, names):
     """(type code, elements from row to row of each) of weights' gradients given by the caller."""
     types, lds = set(), []
     for v, w, name in zip(out, like, names):
@@ -767,6 +767,34 @@ def _scratch(need, workspace, device, like):
     have = _nbytes(workspace, "workspace")
     _on(device, workspace, "workspace")
     return workspace, have
+
+
+def _place(x):
+    """(first byte, last byte + 1, bytes from row to row, bytes of a row) of an array; None without elements."""
+    size = _BYTES[x.dtype] if isinstance(x, DeviceArray) else x.element_size()
+    rows, width, ld = _rows(x, "array")
+    if not rows or not width:
+        return None
+    p = x.data_ptr()
+    return p, p + ((rows - 1) * ld + width) * size, ld * size, width * size
+
+
+def _separate(written, read):
+    """Refuses results that share memory with an operand or with one another: pairs of name and array."""
+    places = [(n, _place(x), True) for n, x in written if x is not None]
+    places += [(n, _place(x), False) for n, x in read if x is not None]
+    for i, (n, p, w) in enumerate(places):
+        if p is None or not w:
+            continue
+        for m, q, _ in places[i + 1:]:
+            if q is None or p[1] <= q[0] or q[1] <= p[0]:
+                continue
+            # columns of one array side by side: rows of both start in the same distance
+            if p[2] == q[2]:
+                apart = (q[0] - p[0]) % p[2]
+                if apart >= p[3] and apart + q[3] <= p[2]:
+                    continue
+            raise ValueError(f"{n}: overlaps {m}")
 
 
 class LinearLogprobs(NamedTuple):
@@ -846,6 +874,9 @@ def linear_logprobs(x, weight, tokens, *, scale: float = 1.0, out=None, workspac
             _typed(v, F32, "out " + name)
             _flat(v, rows * n, "out " + name)
             _on(dev, v, "out " + name)
+    if out is not None or workspace is not None:
+        _separate((*(("out " + n, v) for n, v in zip(r._fields, r)), ("workspace", workspace)),
+                  (("x", x), ("weight", weight), ("tokens", tokens)))
     workspace, have = _scratch(_linear_workspace(dev, dt, x, ldx, weight, ldw, rows, width, vocab, 0)
                                if workspace is None else 0, workspace, dev, x)
     rt.check(_entry("ad_linear_logprobs")(
@@ -882,7 +913,10 @@ def linear_logprobs_grad(x, weight, tokens, stats, g_logp=None, g_lse=None, *, s
         _on(dev, g.x, "out x")
         lddx = _rows(g.x, "out x")[2]
         _apart(lddx, rows, width, "out x")
-        wt, (lddw,) = _weight_grads((g.weight,), (weight,), dt, dev, accumulate, ("out weight",))
+        wt, (lddw,) = _weight_grads((g.weight,), (weight,), dt, dev, ("out weight",))
+    if out is not None or workspace is not None:
+        _separate((("out x", g.x), ("out weight", g.weight), ("workspace", workspace)),
+                  (("x", x), ("weight", weight), ("tokens", tokens), ("stats", stats), ("g_logp", g_logp), ("g_lse", g_lse)))
     workspace, have = _scratch(_linear_workspace(dev, dt, x, ldx, weight, ldw, rows, width, vocab, 1)
                                if workspace is None else 0, workspace, dev, x)
     rt.check(_entry("ad_linear_logprobs_grad")(
@@ -987,6 +1021,9 @@ def feed_forward(x, w_gate, w_up, w_down, *, act: str = "silu", keep: bool = Fal
         if keep:
             ldg = _matrix(r.gate, rows, hidden, F32, dev, "out gate")
             ldu = _matrix(r.up, rows, hidden, F32, dev, "out up")
+    if out is not None or workspace is not None:
+        _separate((*(("out " + n, v) for n, v in zip(r._fields, r)), ("workspace", workspace)),
+                  (("x", x), ("w_gate", w_gate), ("w_up", w_up), ("w_down", w_down)))
     operands = (x.data_ptr(), ldx, w_gate.data_ptr(), ldwg, w_up.data_ptr(), ldwu, w_down.data_ptr(), ldwd)
     workspace, have = _scratch(_ffn_workspace(dev, dt, operands, None, 0, rows, width, hidden, 0)
                                if workspace is None else 0, workspace, dev, x)
@@ -1022,8 +1059,11 @@ def feed_forward_grad(dy, x, w_gate, w_up, w_down, gate, up, *, act: str = "silu
         _on(dev, g.x, "out x")
         lddx = _rows(g.x, "out x")[2]
         _apart(lddx, rows, width, "out x")
-        wt, lds = _weight_grads(g[1:], (w_gate, w_up, w_down), dt, dev, accumulate,
+        wt, lds = _weight_grads(g[1:], (w_gate, w_up, w_down), dt, dev,
                                 tuple("out " + n for n in FeedForwardGrads._fields[1:]))
+    if out is not None or workspace is not None:
+        _separate((*(("out " + n, v) for n, v in zip(g._fields, g)), ("workspace", workspace)),
+                  (("dy", dy), ("x", x), ("w_gate", w_gate), ("w_up", w_up), ("w_down", w_down), ("gate", gate), ("up", up)))
     operands = (x.data_ptr(), ldx, w_gate.data_ptr(), ldwg, w_up.data_ptr(), ldwu, w_down.data_ptr(), ldwd)
     workspace, have = _scratch(_ffn_workspace(dev, dt, operands, dy.data_ptr(), lddy, rows, width, hidden, 1)
                                if workspace is None else 0, workspace, dev, x)
@@ -1080,6 +1120,7 @@ def embed(tokens, table, *, scale: float = 1.0, out=None, stream=None):
         _on(dev, out, "out")
         ldo = _rows(out, "out")[2]
         _apart(ldo, rows, width, "out")
+        _separate((("out", out),), (("tokens", tokens), ("table", table)))
     rt.check(_entry("ad_embed")(dev, dt, tokens.data_ptr(), t64, rows, table.data_ptr(), ldt, vocab, width, scale,
                                 out.data_ptr(), ldo, s))
     return out
@@ -1113,6 +1154,7 @@ def embed_grad(dy, tokens, vocab: int, *, scale: float = 1.0, accumulate: bool =
     if accumulate and out is None:
         raise ValueError("accumulate: out has to be given")
     s = _stream(dev, stream, dy, out is None or workspace is None)
+    given = out is not None
     if out is None:
         out = _empty((vocab, width), dy)
         ot, ldo = dt, width
@@ -1121,6 +1163,8 @@ def embed_grad(dy, tokens, vocab: int, *, scale: float = 1.0, accumulate: bool =
         if ot not in (dt, F32):
             raise TypeError(f"out: expected float32 elements or dy's, got {out.dtype}")
         ldo = _matrix(out, vocab, width, ot, dev, "out")
+    if given or workspace is not None:
+        _separate((("out", out), ("workspace", workspace)), (("dy", dy), ("tokens", tokens)))
     workspace, have = _scratch(embed_grad_workspace(rows, vocab, width) if workspace is None else 0, workspace, dev, dy)
     rt.check(_entry("ad_embed_grad")(
         dev, dt, dy.data_ptr(), lddy, tokens.data_ptr(), t64, rows, vocab, width, scale, ot, out.data_ptr(), ldo,
@@ -1184,7 +1228,8 @@ def _clip_operands(grads, out):
 def clip_norm(grads, max_norm: float, *, out=None, norm=None, workspace=None, stream=None):
     """Scales the arrays of ``grads`` (a list; of any types, shapes and order of axes, their elements adjacent)
     by ``max_norm`` over the norm of all their elements together, where that norm is larger, and returns the norm
-    as it was, float32 [1].  ``max_norm`` of infinity gives the norm alone.  A norm that is infinite or NaN
+    as it was, float32 [1] (infinity past that range, which does not keep finite arrays from being scaled).
+    ``max_norm`` of infinity gives the norm alone.  A norm that is infinite or NaN
     leaves the arrays as they are: what to do then is the caller's.  Sums are held in 64 bits.  The arrays themselves are
     written, or those of ``out``, of the same types, shapes and strides; none of them may overlap another one.
     ``norm``: the array for the result; ``workspace``: adjacent elements at a 256-byte boundary,

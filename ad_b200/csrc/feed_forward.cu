@@ -122,6 +122,7 @@ __device__ __forceinline__ Two activated(Two z) {
 struct Gated {
   static constexpr bool DUAL = true;
   static constexpr int WARPS = 16, SIDE = 4096;
+  static constexpr double US[3] = {6.0, 4.5, 3.0};
   using Units = ByNumber;
   struct Params {
     unsigned short* h;
@@ -183,6 +184,7 @@ struct Gated {
 struct GatedGrad {
   static constexpr bool DUAL = false;
   static constexpr int WARPS = 16, SIDE = 4096;
+  static constexpr double US[3] = {11.0, 5.5, 3.2};
   using Units = ByNumber;
   struct Params {
     const float *gate, *up;
@@ -481,7 +483,8 @@ Layout plan(const Device& d, const Operand* ops, int count, long long rows, long
     l.dg = take(2ull * rows * l.ld);
     l.du = take(2ull * rows * l.ld);
   }
-  l.tiling = tiling_for(rows, hidden, (width + BK - 1) / BK, count == 4, d.sms);
+  const long long kblocks = (width + BK - 1) / BK;
+  l.tiling = count == 4 ? tiling_for<Gated>(rows, hidden, kblocks, d.sms) : tiling_for<GatedGrad>(rows, hidden, kblocks, d.sms);
   l.partial = take(partial_bytes(d));
   l.total = at;
   return l;

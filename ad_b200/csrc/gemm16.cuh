@@ -370,7 +370,7 @@ struct Ring {
 };
 
 // EPI: DUAL (B's tiles hold half their columns of each of two operands), WARPS,
-// SIDE; Params; Units; a State that is constructed for a tile (loads that need no
+// SIDE; US (tiling_for); Params; Units; a State that is constructed for a tile (loads that need no
 // accumulator), whose chunk() takes 32 columns, and whose end() all warps call.
 template <typename TILE, typename EPI>
 __global__ void __launch_bounds__(TILE::THREADS, 1)
@@ -625,24 +625,31 @@ struct Device {
 };
 
 // The three tilings: rows and columns, blocks, and measured us for 64 elements of K
-// (with the clocks that large products leave).
+// (with the clocks that large products leave; 2047 x 50001 over 1024 took 152, 250
+// and 453 us).
 struct Tiling {
   int m, n, ctas;
   double us;
 };
-constexpr Tiling TILINGS[3] = {{256, 256, 2, 0.43}, {128, 128, 1, 0.47}, {128, 64, 1, 0.40}};
+constexpr Tiling TILINGS[3] = {{256, 256, 2, 0.38}, {128, 128, 1, 0.36}, {128, 64, 1, 0.33}};
 
 inline int kblocks_of(const Problem& p) { return static_cast<int>((p.k0 + BK - 1) / BK + (p.k - p.k0 + BK - 1) / BK); }
 
-// The tiling for whole tiles: the one whose rounds take least.
-inline int tiling_for(long long m, long long n, long long kblocks, bool dual, int sms) {
+// The tiling for whole tiles: the one whose rounds take least, a round being a
+// tile's products or its epilogue (EPI::US, measured for each tiling), whichever is
+// longer.  A large tile's epilogue bounds short K's: dh of 600 x 2048 over 512 took 19 us on
+// large tiles, 13 on middle ones and 15 on small ones; of 4095 x 2048 35, 35 and 40.
+template <typename EPI>
+int tiling_for(long long m, long long n, long long kblocks, int sms) {
   int best = 0;
   double least = 1e30;
   for (int i = 0; i < 3; ++i) {
     const Tiling& t = TILINGS[i];
-    const int cols = dual ? t.n / 2 : t.n, workers = sms / t.ctas;
+    const int cols = EPI::DUAL ? t.n / 2 : t.n, workers = sms / t.ctas;
     const long long count = ((m + t.m - 1) / t.m) * ((n + cols - 1) / cols);
-    const double us = static_cast<double>((count + workers - 1) / workers) * kblocks * t.us + 4.0;
+    const double products = kblocks * t.us, epilogue = EPI::US[i];
+    const double us = static_cast<double>((count + workers - 1) / workers) * std::max(products, epilogue) +
+                      std::min(products, epilogue) + 4.0;
     if (us < least * 0.97) best = i, least = us;
   }
   return best;

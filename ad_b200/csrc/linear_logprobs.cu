@@ -40,6 +40,7 @@ __device__ __forceinline__ long long token_at(const void* tokens, int tok64, lon
 struct Sum {
   static constexpr bool DUAL = false;
   static constexpr int WARPS = 8, SIDE = 512;
+  static constexpr double US[3] = {4.0, 2.2, 1.5};
   using Units = ByNumber;
   struct Params {
     float2* part;   // [column tiles][rows]
@@ -185,6 +186,7 @@ __global__ void __launch_bounds__(1024) range_kernel(const __grid_constant__ Ran
 struct Slope {
   static constexpr bool DUAL = false;
   static constexpr int WARPS = 16, SIDE = 2048;
+  static constexpr double US[3] = {4.5, 2.5, 1.7};
   using Units = ByNumber;
   struct Params {
     const float2* stats;
@@ -267,7 +269,7 @@ Layout plan(const Device& d, const void* x, long long ldx, const void* w, long l
   if (l.pack_w) l.w = take(2ull * vocab * l.ld_packed);
   const long long kblocks = (width + BK - 1) / BK;
   if (!grad) {
-    l.tiling = tiling_for(rows, vocab, kblocks, false, d.sms);
+    l.tiling = tiling_for<Sum>(rows, vocab, kblocks, d.sms);
     l.part = take(sizeof(float2) * parts_of(l.tiling, vocab) * rows);
     l.target = take(sizeof(float) * rows);
   } else {
@@ -276,7 +278,7 @@ Layout plan(const Device& d, const void* x, long long ldx, const void* w, long l
     l.pieces = std::max(1ll, std::min(l.pieces, (vocab + 1023) / 1024));
     l.piece = std::min(round_up((vocab + l.pieces - 1) / l.pieces, 256), round_up(vocab, 8));
     l.pieces = (vocab + l.piece - 1) / l.piece;
-    l.tiling = tiling_for(rows, std::min(l.piece, vocab), kblocks, false, d.sms);
+    l.tiling = tiling_for<Slope>(rows, std::min(l.piece, vocab), kblocks, d.sms);
     l.factor = take(2 * sizeof(float));
     l.dz = take(2ull * rows * l.piece);
     if (l.pieces > 1) l.sum = take(sizeof(float) * rows * round_up(width, 4));

@@ -14,7 +14,7 @@
 // is left in memory, and a last kernel joins such partial sums, a block a token and
 // slice, found through a list.  A token that comes up thousands of times so costs
 // no more than others.  Rows of tokens that do not come up are cleared by further
-// blocks of the sort's launches.
+// blocks of the sort's launches, once the first two have noted which these are.
 #include <algorithm>
 #include <cmath>
 
@@ -80,6 +80,15 @@ __global__ void __launch_bounds__(256) embed_kernel(const __grid_constant__ Embe
 constexpr int TILE = 2048, SORT_THREADS = 256, SORT_WARPS = 8, KEYS = TILE / SORT_THREADS;
 constexpr int MAX_BITS = 10, MAX_DIGITS = 1 << MAX_BITS;
 
+// Rows of the table's gradient to clear: `units` of `unit` bytes each, by `lanes` lanes,
+// `rows` of them (a power of two up to 8) by a warp.
+struct Clear {
+  unsigned char* p;
+  long long row_stride, from, to;
+  const unsigned char* seen;  // eight rows a byte; NULL: all are cleared
+  int unit, units, lanes, rows;
+};
+
 // Keys and the positions that they came from; the first pass takes them from the
 // tokens themselves, the others from the previous pass.  Tokens outside of the
 // vocabulary have its size as their key and end up last.
@@ -93,15 +102,31 @@ struct SortArgs {
   int* counts;  // [digits][tiles], then their running sums
   int* totals;  // [digits]
   int* joins;   // the numbers of short and of long joins, cleared ahead of the sums
-  uint4* clear; // this launch's share of the memory to clear, in 16-byte words
-  long long clear_words;
+  unsigned* seen;  // a bit for each token that comes up: cleared by the first launch, set by the second
+  int seen_words, noting;  // blocks of the second launch that set them
+  Clear clear;     // this launch's share of the rows to clear
 };
-// Blocks from `first` on clear; whether this is one of them.
-__device__ __forceinline__ bool clears(const SortArgs& a, unsigned first) {
+// Blocks from `first` on clear; whether this is one of them.  A warp takes one to eight
+// rows (whose bits lie in a byte), a group of its lanes a row at a time.
+__device__ __forceinline__ bool clears(const Clear& c, unsigned first) {
   if (blockIdx.x < first) return false;
-  const long long step = static_cast<long long>(gridDim.x - first) * blockDim.x;
-  for (long long i = (blockIdx.x - first) * static_cast<long long>(blockDim.x) + threadIdx.x; i < a.clear_words; i += step)
-    a.clear[i] = make_uint4(0, 0, 0, 0);
+  const long long warps = static_cast<long long>(gridDim.x - first) * (blockDim.x >> 5);
+  const int lane = threadIdx.x & 31, at_once = 32 / c.lanes < c.rows ? 32 / c.lanes : c.rows, l = lane & (c.lanes - 1);
+  if (lane / c.lanes >= at_once) return true;
+  for (long long r0 = c.from + ((blockIdx.x - first) * (blockDim.x >> 5) + (threadIdx.x >> 5)) * static_cast<long long>(c.rows); r0 < c.to;
+       r0 += warps * c.rows) {
+    const unsigned seen = c.seen ? c.seen[r0 >> 3] >> (r0 & 7) : 0u;
+    for (int j = lane / c.lanes; j < c.rows && r0 + j < c.to; j += at_once) {
+      if (seen >> j & 1) continue;
+      unsigned char* p = c.p + (r0 + j) * c.row_stride;
+      if (c.unit == 16)
+        for (int i = l; i < c.units; i += c.lanes) reinterpret_cast<uint4*>(p)[i] = make_uint4(0, 0, 0, 0);
+      else if (c.unit == 4)
+        for (int i = l; i < c.units; i += c.lanes) reinterpret_cast<unsigned*>(p)[i] = 0;
+      else
+        for (int i = l; i < c.units; i += c.lanes) reinterpret_cast<unsigned short*>(p)[i] = 0;
+    }
+  }
   return true;
 }
 __device__ __forceinline__ int key_of(const SortArgs& a, int i) {
@@ -113,14 +138,17 @@ __device__ __forceinline__ int key_of(const SortArgs& a, int i) {
 __global__ void __launch_bounds__(SORT_THREADS) count_kernel(const __grid_constant__ SortArgs a) {
   after_previous();
   __shared__ int hist[MAX_DIGITS];
-  if (clears(a, a.tiles)) return;
+  if (clears(a.clear, a.tiles)) return;
   if (blockIdx.x == 0 && threadIdx.x < 2) a.joins[threadIdx.x] = 0;
   for (int d = threadIdx.x; d < a.digits; d += SORT_THREADS) hist[d] = 0;
+  if (a.seen)
+    for (int i = blockIdx.x * SORT_THREADS + threadIdx.x; i < a.seen_words; i += a.tiles * SORT_THREADS) a.seen[i] = 0;
   __syncthreads();
 #pragma unroll
   for (int j = 0; j < KEYS; ++j) {
     const int i = blockIdx.x * TILE + j * SORT_THREADS + threadIdx.x;
-    if (i < a.n) atomicAdd(&hist[(key_of(a, i) >> a.shift) & (a.digits - 1)], 1);
+    if (i >= a.n) continue;
+    atomicAdd(&hist[(key_of(a, i) >> a.shift) & (a.digits - 1)], 1);
   }
   __syncthreads();
   for (int d = threadIdx.x; d < a.digits; d += SORT_THREADS) a.counts[static_cast<long long>(d) * a.tiles + blockIdx.x] = hist[d];
@@ -129,7 +157,16 @@ __global__ void __launch_bounds__(SORT_THREADS) count_kernel(const __grid_consta
 // A digit's counts to running sums over the tiles, a warp a digit.
 __global__ void __launch_bounds__(256) scan_kernel(const __grid_constant__ SortArgs a) {
   after_previous();
-  if (clears(a, (a.digits + 7) / 8)) return;
+  const unsigned scanning = (a.digits + 7) / 8;
+  if (clears(a.clear, scanning + a.noting)) return;
+  if (blockIdx.x >= scanning) {  // which tokens come up
+    for (int i = (blockIdx.x - scanning) * 256 + threadIdx.x; i < a.n; i += a.noting * 256) {
+      const int key = key_of(a, i);
+      const unsigned bit = 1u << (key & 31);
+      if (key < a.vocab && !(a.seen[key >> 5] & bit)) atomicOr(&a.seen[key >> 5], bit);
+    }
+    return;
+  }
   const int d = blockIdx.x * 8 + (threadIdx.x >> 5), lane = threadIdx.x & 31;
   if (d >= a.digits) return;
   int* c = a.counts + static_cast<long long>(d) * a.tiles;
@@ -218,7 +255,7 @@ __device__ __forceinline__ void rank_tile(TileSort& s, const int (&digit)[KEYS],
 __global__ void __launch_bounds__(SORT_THREADS) move_kernel(const __grid_constant__ SortArgs a) {
   after_previous();
   __shared__ TileSort s;
-  if (clears(a, a.tiles)) return;
+  if (clears(a.clear, a.tiles)) return;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   for (int d = threadIdx.x; d < a.digits; d += SORT_THREADS) {
     s.base[d] = a.totals[d];
@@ -254,7 +291,7 @@ __global__ void __launch_bounds__(SORT_THREADS) sort_kernel(const __grid_constan
   __shared__ TileSort s;
   int* const keys = s.hist[0];  // in the place of the counts, once these have served
   short* const at = reinterpret_cast<short*>(s.hist[TILE / MAX_DIGITS]);
-  if (clears(a, 1)) return;
+  if (clears(a.clear, 1)) return;
   if (threadIdx.x < 2) a.joins[threadIdx.x] = 0;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, digits = 1 << bits;
   int key[KEYS], from[KEYS], digit[KEYS], place[KEYS];
@@ -505,7 +542,7 @@ __global__ void __launch_bounds__(256) join_kernel(const __grid_constant__ SumAr
 struct Layout {
   int bits, passes, tiles, chunks;
   long long ldp;
-  size_t keys[2], at[2], counts, totals, joins, list, part, total;
+  size_t keys[2], at[2], counts, totals, seen, joins, list, part, total;
 };
 Layout plan(long long rows, long long vocab, long long width) {
   Layout l;
@@ -525,6 +562,7 @@ Layout plan(long long rows, long long vocab, long long width) {
   for (int k = 0; k < 2; ++k) l.keys[k] = take(4ull * rows), l.at[k] = take(4ull * rows);
   l.counts = take(4ull * l.tiles << l.bits);
   l.totals = take(4ull << l.bits);
+  l.seen = take((vocab + 31) / 32 * 4);
   l.joins = take(8);
   l.list = take(8ull * l.chunks);
   l.part = take(8ull * l.chunks * l.ldp);
@@ -623,46 +661,52 @@ extern "C" int ad_embed_grad(int device, int dtype, const void* dy, int64_t lddy
   SortArgs s = {};
   s.tokens = tokens, s.tok64 = tok64, s.vocab = vocab, s.n = static_cast<int>(rows), s.tiles = l.tiles;
   s.counts = ints(l.counts), s.totals = ints(l.totals), s.joins = ints(l.joins);
-  if (!accumulate) {
-    const size_t bytes = static_cast<size_t>(vocab) * width * os;
-    if ((ldo == width || vocab == 1) && aligned(out, 16) && bytes % 16 == 0) {
-      s.clear = static_cast<uint4*>(out), s.clear_words = bytes / 16;
-    } else if (ad_clear_rows(guard.device(), out, ldo * os, width * os, vocab, stream)) {
-      return 1;
-    }
-  }
-  // Each launch of the sort, which waits for memory most of the time, clears a share:
-  // what takes it about as long as it has to wait (CLEAR), and the first one the rest.
-  constexpr long long CLEAR = 32 << 20;
-  const int launches = l.tiles == 1 ? 1 : 3 * l.passes;
-  uint4* const all = s.clear;
-  const long long words = s.clear_words, later = std::min(words / launches, CLEAR / 16);
-  long long cleared = 0;
-  auto share = [&](int launch) {  // blocks that clear
-    s.clear = all + cleared;
-    s.clear_words = launch ? later : words - (launches - 1) * later;
-    cleared += s.clear_words;
-    return static_cast<unsigned>(std::min<long long>((s.clear_words + 1023) / 1024, 8ll * sms));
+  // The launches of the sort wait for memory most of the time.  The first two note which
+  // tokens come up; each of the others clears a share of the rows beside its work, and leaves those
+  // to the sums (131072 tokens of as many, rows of 8 KB: 454 us, 509 with all rows cleared; 16288
+  // tokens of 50001, rows of 4 KB: 94 and 93).
+  const bool note = l.tiles > 1 && !accumulate;
+  Clear clear = {};
+  clear.p = static_cast<unsigned char*>(out), clear.row_stride = ldo * os;
+  const long long bytes = width * os;
+  auto whole = [&](int unit) { return bytes % unit == 0 && (vocab == 1 || clear.row_stride % unit == 0) && aligned(out, unit); };
+  clear.unit = whole(16) ? 16 : whole(4) ? 4 : 2;
+  clear.units = static_cast<int>(bytes / clear.unit);
+  for (clear.lanes = 1; clear.lanes < 32 && clear.lanes < clear.units;) clear.lanes *= 2;
+  for (clear.rows = 8; clear.rows > 1 && clear.rows * bytes > 4096;) clear.rows /= 2;  // 4 KB a warp (8: 98 us instead of 94)
+  const int early = note ? 2 : 0, launches = (l.tiles == 1 ? 1 : 3 * l.passes) - early;
+  const long long share = (vocab + 8 * launches - 1) / (8 * launches) * 8;
+  auto clearing = [&](int launch) {  // blocks that clear in one of the launches
+    if (accumulate || launch < early) return 0u;
+    s.clear = clear;
+    s.clear.from = std::min<long long>(vocab, (launch - early) * share), s.clear.to = std::min<long long>(vocab, s.clear.from + share);
+    return static_cast<unsigned>(std::min<long long>((s.clear.to - s.clear.from + 8 * clear.rows - 1) / (8 * clear.rows), 32ll * sms));
   };
   cudaError_t e;
   int to = 0;
   if (l.tiles == 1) {
     s.keys_out = ints(l.keys[0]), s.at_out = ints(l.at[0]);
-    const unsigned more = share(0);
+    const unsigned more = clearing(0);
     e = launch_early<sort_kernel>(dim3(1 + more), SORT_THREADS, 0, st, s, l.bits, l.passes);
     if (e != cudaSuccess) return fail_cuda(who, e);
   } else {
+    if (note) {
+      s.seen = reinterpret_cast<unsigned*>(ws + l.seen), s.seen_words = static_cast<int>((vocab + 31) / 32);
+      clear.seen = ws + l.seen;
+    }
     s.digits = 1 << l.bits;
     for (int p = 0; p < l.passes; ++p) {
       to = p & 1;
       s.shift = p * l.bits;
       s.keys = p ? ints(l.keys[to ^ 1]) : nullptr, s.at = p ? ints(l.at[to ^ 1]) : nullptr;
       s.keys_out = ints(l.keys[to]), s.at_out = ints(l.at[to]);
-      unsigned more = share(3 * p);
+      unsigned more = clearing(3 * p);
       e = launch_early<count_kernel>(dim3(l.tiles + more), SORT_THREADS, 0, st, s);
-      more = share(3 * p + 1);
-      if (e == cudaSuccess) e = launch_early<scan_kernel>(dim3((s.digits + 7) / 8 + more), 256, 0, st, s);
-      more = share(3 * p + 2);
+      more = clearing(3 * p + 1);
+      s.noting = p || !note ? 0 : std::min((s.n + 1023) / 1024, 8 * sms);
+      if (e == cudaSuccess) e = launch_early<scan_kernel>(dim3((s.digits + 7) / 8 + s.noting + more), 256, 0, st, s);
+      s.seen = nullptr;
+      more = clearing(3 * p + 2);
       if (e == cudaSuccess) e = launch_early<move_kernel>(dim3(l.tiles + more), SORT_THREADS, 0, st, s);
       if (e != cudaSuccess) return fail_cuda(who, e);
     }

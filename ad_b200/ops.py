@@ -839,11 +839,26 @@ def _check_linear_operands(x, weight, tokens):
     return dev, dt, rows, width, vocab, ldx, ldw, t64
 
 
+# Bytes of workspace that calls needed, by what they depend on.
+_needs: dict = {}
+
+
 def _linear_workspace(dev, dt, x, ldx, weight, ldw, rows, width, vocab, grad):
+    key = (dev, dt, x.data_ptr() & 15, ldx, weight.data_ptr() & 15, ldw, rows, width, vocab, grad)
+    need = _needs.get(key)
+    if need is not None:
+        return need
     n = rt.c_size_t()
     rt.check(_entry("ad_linear_logprobs_workspace")(dev, dt, x.data_ptr(), ldx, weight.data_ptr(), ldw, rows, width,
                                                     vocab, grad, ctypes.byref(n)))
-    return n.value
+    return _remember_need(key, n.value)
+
+
+def _remember_need(key, need):
+    if len(_needs) >= 4096:
+        _needs.clear()
+    _needs[key] = need
+    return need
 
 
 def linear_logprobs_workspace(x, weight, grad: bool = False) -> int:
@@ -973,10 +988,15 @@ def _check_ffn_operands(x, w_gate, w_up, w_down):
 
 
 def _ffn_workspace(dev, dt, operands, dy, lddy, rows, width, hidden, grad):
+    x, ldx, wg, ldg, wu, ldu, wd, ldd = operands
+    key = (dev, dt, x & 15, ldx, wg & 15, ldg, wu & 15, ldu, wd & 15, ldd, dy and dy & 15, lddy, rows, width, hidden, grad)
+    need = _needs.get(key)
+    if need is not None:
+        return need
     n = rt.c_size_t()
     rt.check(_entry("ad_feed_forward_workspace")(dev, dt, *operands, dy, lddy, rows, width, hidden, grad,
                                                  ctypes.byref(n)))
-    return n.value
+    return _remember_need(key, n.value)
 
 
 def feed_forward_workspace(x, w_gate, w_up, w_down, dy=None) -> int:

@@ -603,6 +603,8 @@ extern "C" int ad_embed(int device, int dtype, const void* tokens, int tok64, in
   if (!tokens || !table || !y) return fail("%s: null operand", who);
   const int es = elem_size(dtype);
   if (!aligned(tokens, tok64 ? 8 : 4) || !aligned({table, y}, es)) return fail("%s: an operand is not aligned to its elements", who);
+  if (overlap({{y, rows, width * es, ldy * es, true}, {table, vocab, width * es, ldt * es, false}, {tokens, 1, rows * (tok64 ? 8 : 4), 0, false}}))
+    return fail("%s: results overlap operands or one another", who);
   DeviceGuard guard(device);
   if (guard.error() != cudaSuccess) return fail_cuda(who, guard.error());
   const int sms = sm_count(guard.device());
@@ -650,6 +652,9 @@ extern "C" int ad_embed_grad(int device, int dtype, const void* dy, int64_t lddy
   const Layout l = plan(rows, vocab, width);
   if (!workspace || !aligned(workspace, 256) || workspace_bytes < l.total)
     return fail("%s: needs %zu bytes of workspace, 256-byte aligned", who, l.total);
+  if (overlap({{out, vocab, width * os, ldo * os, true}, {workspace, 1, static_cast<long long>(l.total), 0, true},
+               {dy, rows, width * es, lddy * es, false}, {tokens, 1, rows * (tok64 ? 8 : 4), 0, false}}))
+    return fail("%s: results overlap operands or one another", who);
   DeviceGuard guard(device);
   if (guard.error() != cudaSuccess) return fail_cuda(who, guard.error());
   const int sms = sm_count(guard.device());

@@ -553,6 +553,11 @@ extern "C" int ad_feed_forward(int device, int dtype, int act, const void* x, in
   if (!rows) return 0;
   if (!x || !w_gate || !w_up || !w_down || !y) return fail("%s: null operand", who);
   if (!aligned(y, 2) || !aligned({gate, up}, 4)) return fail("%s: an operand is not aligned to its elements", who);
+  if (overlap({{y, rows, width * 2, ldy * 2, true}, {gate, rows, hidden * 4, ldg * 4, true}, {up, rows, hidden * 4, ldu * 4, true},
+               {workspace, 1, static_cast<long long>(workspace_bytes), 0, true}, {x, rows, width * 2, ldx * 2, false},
+               {w_gate, hidden, width * 2, ld_gate * 2, false}, {w_up, hidden, width * 2, ld_up * 2, false},
+               {w_down, width, hidden * 2, ld_down * 2, false}}))
+    return fail("%s: results overlap operands or one another", who);
   DeviceGuard guard(device);
   if (guard.error() != cudaSuccess) return fail_cuda(who, guard.error());
   const Device d = {guard.device(), sm_count(guard.device())};
@@ -614,6 +619,13 @@ extern "C" int ad_feed_forward_grad(int device, int dtype, int act, const void* 
   }
   if (!dy || !x || !w_gate || !w_up || !w_down || !gate || !up || !dx) return fail("%s: null operand", who);
   if (!aligned(dx, 2) || !aligned({gate, up}, 4)) return fail("%s: an operand is not aligned to its elements", who);
+  const long long wide = width * es, tall = hidden * es, e = es;
+  if (overlap({{dx, rows, width * 2, lddx * 2, true}, {dw_gate, hidden, wide, lddw_gate * e, true}, {dw_up, hidden, wide, lddw_up * e, true},
+               {dw_down, width, tall, lddw_down * e, true}, {workspace, 1, static_cast<long long>(workspace_bytes), 0, true},
+               {dy, rows, width * 2, lddy * 2, false}, {x, rows, width * 2, ldx * 2, false},
+               {w_gate, hidden, width * 2, ld_gate * 2, false}, {w_up, hidden, width * 2, ld_up * 2, false},
+               {w_down, width, hidden * 2, ld_down * 2, false}, {gate, rows, hidden * 4, ldg * 4, false}, {up, rows, hidden * 4, ldu * 4, false}}))
+    return fail("%s: results overlap operands or one another", who);
   DeviceGuard guard(device);
   if (guard.error() != cudaSuccess) return fail_cuda(who, guard.error());
   const Device d = {guard.device(), sm_count(guard.device())};

@@ -338,6 +338,10 @@ extern "C" int ad_linear_logprobs(int device, int dtype, const void* x, int64_t 
   if (!x || !weight || !tokens || !logp || !lse || !stats) return fail("%s: null operand", who);
   if (!aligned(tokens, tok64 ? 8 : 4) || !aligned({logp, lse}, 4) || !aligned(stats, 8))
     return fail("%s: an operand is not aligned to its elements", who);
+  const long long tokens_bytes = rows * (tok64 ? 8 : 4), ws_bytes = static_cast<long long>(workspace_bytes);
+  if (overlap({{logp, 1, rows * 4, 0, true}, {lse, 1, rows * 4, 0, true}, {stats, 1, rows * 8, 0, true}, {workspace, 1, ws_bytes, 0, true},
+               {x, rows, width * 2, ldx * 2, false}, {weight, vocab, width * 2, ldw * 2, false}, {tokens, 1, tokens_bytes, 0, false}}))
+    return fail("%s: results overlap operands or one another", who);
   DeviceGuard guard(device);
   if (guard.error() != cudaSuccess) return fail_cuda(who, guard.error());
   const Device d = {guard.device(), sm_count(guard.device())};
@@ -382,6 +386,12 @@ extern "C" int ad_linear_logprobs_grad(int device, int dtype, const void* x, int
   if (!x || !weight || !tokens || !stats || !dx) return fail("%s: null operand", who);
   if (!aligned(tokens, tok64 ? 8 : 4) || !aligned({g_logp, g_lse}, 4) || !aligned(stats, 8) || !aligned(dx, 2))
     return fail("%s: an operand is not aligned to its elements", who);
+  const long long tokens_bytes = rows * (tok64 ? 8 : 4), ws_bytes = static_cast<long long>(workspace_bytes);
+  if (overlap({{dx, rows, width * 2, lddx * 2, true}, {dw, vocab, static_cast<long long>(width * es), static_cast<long long>(lddw * es), true},
+               {workspace, 1, ws_bytes, 0, true}, {x, rows, width * 2, ldx * 2, false}, {weight, vocab, width * 2, ldw * 2, false},
+               {tokens, 1, tokens_bytes, 0, false}, {stats, 1, rows * 8, 0, false}, {g_logp, 1, rows * 4, 0, false},
+               {g_lse, 1, rows * 4, 0, false}}))
+    return fail("%s: results overlap operands or one another", who);
   DeviceGuard guard(device);
   if (guard.error() != cudaSuccess) return fail_cuda(who, guard.error());
   const Device d = {guard.device(), sm_count(guard.device())};

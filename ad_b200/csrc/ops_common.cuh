@@ -148,6 +148,32 @@ __device__ __forceinline__ void after_previous() {
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
 }
 
+// Memory of a call: rows of row_bytes bytes, `stride` bytes apart.
+struct Place {
+  const void* p;
+  long long rows, row_bytes, stride;
+  bool written;
+};
+// Whether what is written shares memory with anything else.  Columns of one array
+// side by side (rows of both the same distance apart) do not.
+inline bool overlap(std::initializer_list<Place> all) {
+  for (const Place* a = all.begin(); a != all.end(); ++a) {
+    if (!a->p || a->rows < 1 || a->row_bytes < 1) continue;
+    const intptr_t a0 = reinterpret_cast<intptr_t>(a->p), a1 = a0 + (a->rows - 1) * a->stride + a->row_bytes;
+    for (const Place* b = a + 1; b != all.end(); ++b) {
+      if (!(a->written || b->written) || !b->p || b->rows < 1 || b->row_bytes < 1) continue;
+      const intptr_t b0 = reinterpret_cast<intptr_t>(b->p), b1 = b0 + (b->rows - 1) * b->stride + b->row_bytes;
+      if (a1 <= b0 || b1 <= a0) continue;
+      if (a->stride == b->stride && a->stride > 0) {
+        const long long d = ((b0 - a0) % a->stride + a->stride) % a->stride;
+        if (d >= a->row_bytes && d + b->row_bytes <= a->stride) continue;
+      }
+      return true;
+    }
+  }
+  return false;
+}
+
 // ---------------------------------------------------------------- elements
 __device__ __forceinline__ float to_float(float x) { return x; }
 __device__ __forceinline__ float to_float(__nv_bfloat16 x) { return __bfloat162float(x); }

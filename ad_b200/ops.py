@@ -6,10 +6,15 @@
 * ``token_logprobs`` / ``token_logprobs_grad``: log probabilities of given tokens, entropy and the
   best alternatives of rows of logits
 * ``orthogonalize``: Newton-Schulz orthogonalisation of matrix updates
+* ``embed`` / ``embed_grad``: scaled rows of an embedding table, and its gradient summed by token
+* ``feed_forward`` / ``feed_forward_grad``: a gated feed-forward block, for single tokens too
+* ``linear_logprobs`` / ``linear_logprobs_grad``: log probabilities under the softmax of a linear layer
+  over a large vocabulary, whose logits are not kept
+* ``clip_norm``: the norm of many arrays together, and their scaling down to a largest one
 
 Operands are device arrays: torch CUDA tensors, or ``DeviceArray`` views of memory from
 ``runtime.Context.malloc`` (this module imports no framework by itself).  Elements are float32,
-bfloat16 or float16.  A call checks its arguments (``TypeError``, ``ValueError``), launches and
+bfloat16 or float16 (of ``feed_forward`` and ``linear_logprobs``: the latter two, the tensor cores' own).  A call checks its arguments (``TypeError``, ``ValueError``), launches and
 returns without waiting; errors of the library are ``runtime.ADError``.
 
 Results are new torch tensors unless ``out`` gives arrays to write.  The launch goes to torch's
@@ -21,7 +26,7 @@ not depend on scheduling.
 
 Results are not recorded for automatic differentiation, also where operands require gradients: a
 training step calls the gradients' entry points itself, or from ``torch.autograd.Function``s as
-``examples/lm_step.py`` does.  The streams of a ``runtime.Context`` neither wait for the legacy default
+``examples/lm_step.py`` and ``examples/lm_half.py`` do.  The streams of a ``runtime.Context`` neither wait for the legacy default
 stream, on which calls with ``DeviceArray`` operands go by default, nor it for them: such a program
 waits with ``Context.sync`` before a call that reads what the context wrote, and for the stream of the
 call before the context goes on.

@@ -267,10 +267,8 @@ bool make_schedule(const Problem* p, int count, int tiling, int workers, Schedul
     if (r > 0x7fff || c > 0x7fff || p[g].k > 64ll * 65000) return false;
     rows[g] = static_cast<int>(r), cols[g] = static_cast<int>(c), kb[g] = kblocks_of(p[g]);
     all += r * c, total += r * c * kb[g];
-    order[g] = g;
-    for (int i = g; i > 0 && kb[order[i]] > kb[order[i - 1]]; --i) std::swap(order[i], order[i - 1]);
   }
-  if (all + 2 * workers > LARGE_LIST) return false;
+  if (all + 3 * workers > LARGE_LIST) return false;
   // a unit's worker, besides what goes to the device
   static_assert(LARGE_LIST < 0x7fff, "");
   struct Piece {
@@ -278,18 +276,34 @@ bool make_schedule(const Problem* p, int count, int tiling, int workers, Schedul
     short worker, slot;
   };
   Piece piece[LARGE_LIST];
-  int pieces = 0, load[MAX_WORKERS] = {}, most = 0;
-  // Whole tiles, the longest first, to the worker that is done first, as long as
-  // they stay below the height that all would have if work could be dealt out evenly.
+  int pieces = 0, slots = 0, load[MAX_WORKERS] = {}, most = 0;
+  // The height that all would have if work could be dealt out evenly.
   int height = static_cast<int>((total + all + workers - 1) / workers) + 1;
+  // A few tiles that are longer than that, beside others: all of them in the same parts, so that
+  // those under way at a time share operands in L2 (dx and dW of 2047 x 50001 over 1024, cut at
+  // odd places: 342 us and 1.5 GB from memory; so 303 and 0.5).
+  int parts[MAX_GROUPS], length[MAX_GROUPS];
+  bool in_parts = false;
+  for (int g = 0; g < count; ++g) {
+    const long long tiles = static_cast<long long>(rows[g]) * cols[g];
+    const int n = (kb[g] + 1) * 5 / (height * 3) + 1;
+    const bool few = count > 1 && kb[g] + 1 > height && tiles * n <= workers && kb[g] / n >= 2 * LEAST;
+    parts[g] = few ? n : 1;
+    length[g] = (kb[g] + parts[g] - 1) / parts[g];
+    in_parts |= few;
+    order[g] = g;
+    for (int i = g; i > 0 && length[order[i]] > length[order[i - 1]]; --i) std::swap(order[i], order[i - 1]);
+  }
+  // Tiles, the longest first, to the worker that is done first, as long as they stay
+  // below that height.
   int heap[MAX_WORKERS];  // load and worker in one number
   for (int w = 0; w < workers; ++w) heap[w] = w;
   auto later = [](int a, int b) { return a > b; };
-  auto give = [&](unsigned where, int k) {
+  auto give = [&](unsigned where, int kb0, int kb1, int slot) {
     std::pop_heap(heap, heap + workers, later);
     const int w = heap[workers - 1] % MAX_WORKERS;
-    piece[pieces++] = {{where, 0, static_cast<unsigned short>(k)}, static_cast<short>(w), -1};
-    load[w] += k + 1;
+    piece[pieces++] = {{where, static_cast<unsigned short>(kb0), static_cast<unsigned short>(kb1)}, static_cast<short>(w), static_cast<short>(slot)};
+    load[w] += kb1 - kb0 + 1;
     most = std::max(most, load[w]);
     heap[workers - 1] = load[w] * MAX_WORKERS + w;
     std::push_heap(heap, heap + workers, later);
@@ -300,31 +314,40 @@ bool make_schedule(const Problem* p, int count, int tiling, int workers, Schedul
   } rest[LARGE_LIST];
   int left = 0;
   for (int i = 0; i < count; ++i) {
-    const int g = order[i], band_rows = t.m == 256 ? 8 : 16;
-    for (int b = 0; b < rows[g]; b += band_rows)
-      for (int c = 0; c < cols[g]; ++c)
-        for (int r = b; r < std::min(b + band_rows, rows[g]); ++r) {
-          const unsigned where = pack_where(g, r, c);
-          if (heap[0] / MAX_WORKERS + kb[g] + 1 <= height)
-            give(where, kb[g]);
-          else
-            rest[left++] = {where, kb[g]};
-        }
+    const int g = order[i], first_slot = slots;
+    // rows of tiles under way together: all workers' tiles in one band, or about as many rows as columns
+    const int square = t.m == 256 ? 8 : 16, band_rows = std::max(square, workers / cols[g]);
+    for (int part = 0; part < parts[g]; ++part)
+      for (int b = 0; b < rows[g]; b += band_rows)
+        for (int c = 0; c < cols[g]; ++c)
+          for (int r = b; r < std::min(b + band_rows, rows[g]); ++r) {
+            const unsigned where = pack_where(g, r, c);
+            if (parts[g] > 1) {
+              const int slot = first_slot + (r * cols[g] + c) * parts[g];
+              if (part == 0) s.cut[s.cuts++] = {where, static_cast<short>(slot), static_cast<short>(parts[g])};
+              give(where, part * length[g], std::min(kb[g], (part + 1) * length[g]), slot + part);
+              ++slots;
+            } else if (heap[0] / MAX_WORKERS + kb[g] + 1 <= height) {
+              give(where, 0, kb[g], -1);
+            } else {
+              rest[left++] = {where, kb[g]};
+            }
+          }
   }
   const int kept = pieces;
   int before[MAX_WORKERS], by_load[MAX_WORKERS];
   for (int w = 0; w < workers; ++w) before[w] = load[w], by_load[w] = w;
   std::stable_sort(by_load, by_load + workers, [&](int a, int b) { return load[a] < load[b]; });
-  for (int i = 0; i < left; ++i) give(rest[i].where, rest[i].k);  // uncut
-  s.us = most * t.us + 4.0;
+  for (int i = 0; i < left; ++i) give(rest[i].where, 0, rest[i].k, -1);  // uncut
   // Cut, the remaining tiles fill all workers up to one height.
   const double slot_us = 2.0 * 4 * t.m * t.n / 3e6;  // a part's sums, there and back at 3 TB/s
+  s.us = most * t.us + 4.0 + (slots ? 5.0 + slot_us * slots : 0.0);
   // about one part for each worker
-  bool cut = left > 0 && left < workers && height > LEAST && (most - height) * t.us > 5.0 + slot_us * workers;
+  bool cut = !in_parts && left > 0 && left < workers && height > LEAST && (most - height) * t.us > 5.0 + slot_us * workers;
   while (cut) {
     pieces = kept;
-    s.cuts = 0;
-    int slots = 0, w = 0, filled[MAX_WORKERS];
+    s.cuts = slots = 0;
+    int w = 0, filled[MAX_WORKERS];
     for (int k = 0; k < workers; ++k) filled[k] = before[k];
     bool fits = true;
     for (int i = 0; i < left && fits; ++i) {

@@ -315,8 +315,9 @@ bool make_schedule(const Problem* p, int count, int tiling, int workers, Schedul
   int left = 0;
   for (int i = 0; i < count; ++i) {
     const int g = order[i], first_slot = slots;
-    // rows of tiles under way together: all workers' tiles in one band, or about as many rows as columns
-    const int square = t.m == 256 ? 8 : 16, band_rows = std::max(square, workers / cols[g]);
+    // about as many rows as columns under way at a time (all rows that workers have where there are
+    // eight columns: 1930 us instead of 1890 for the four gradients of 16384 x 2048 x 8192)
+    const int band_rows = t.m == 256 ? 8 : 16;
     for (int part = 0; part < parts[g]; ++part)
       for (int b = 0; b < rows[g]; b += band_rows)
         for (int c = 0; c < cols[g]; ++c)

@@ -336,6 +336,9 @@ __device__ __forceinline__ void open_row(const Raw<V>& r, int half, float (&v)[V
       const float2 f = unpack2(w[j], half);
       v[2 * j] = f.x, v[2 * j + 1] = f.y;
     }
+  } else if constexpr (V == 2) {
+    const float2 f = unpack2(r, half);
+    v[0] = f.x, v[1] = f.y;
   } else {
     v[0] = unpack2(r, half).x;
   }
@@ -428,16 +431,23 @@ constexpr int FEW = 8;
 
 template <int T, bool DUAL>
 cudaError_t start_rows(const RowsArgs& a, int half, int sms, cudaStream_t st) {
-  auto fits = [](const void* p, long long ld, long long rows) { return aligned(p, 16) && (rows <= 1 || ld % 8 == 0); };
-  const bool vec = a.k % 8 == 0 && fits(a.x, a.ldx, a.rows) && fits(a.w0, a.ld0, a.n) && (!DUAL || fits(a.w1, a.ld1, a.n));
+  // 16 bytes at a time where rows allow it, else 4, else an element
+  auto fits = [&](int v) {
+    auto whole = [&](const void* p, long long ld, long long rows) { return aligned(p, 2 * v) && (rows <= 1 || ld % v == 0); };
+    return a.k % v == 0 && whole(a.x, a.ldx, a.rows) && whole(a.w0, a.ld0, a.n) && (!DUAL || whole(a.w1, a.ld1, a.n));
+  };
   // warps for all of the device, as long as each has 512 elements of a row
   int shared_by = 1;
   while (shared_by < 8 && a.n * shared_by < 16 * sms && a.k / (2 * shared_by) >= 512) shared_by *= 2;
   const dim3 grid((a.n + 8 / shared_by - 1) / (8 / shared_by));
-  return vec ? (half ? launch_early<rows_kernel<T, 8, 1, DUAL>>(grid, 256, 0, st, a, shared_by)
-                     : launch_early<rows_kernel<T, 8, 0, DUAL>>(grid, 256, 0, st, a, shared_by))
-             : (half ? launch_early<rows_kernel<T, 1, 1, DUAL>>(grid, 256, 0, st, a, shared_by)
-                     : launch_early<rows_kernel<T, 1, 0, DUAL>>(grid, 256, 0, st, a, shared_by));
+  auto go = [&](auto v) {
+    constexpr int V = decltype(v)::value;
+    return half ? launch_early<rows_kernel<T, V, 1, DUAL>>(grid, 256, 0, st, a, shared_by)
+                : launch_early<rows_kernel<T, V, 0, DUAL>>(grid, 256, 0, st, a, shared_by);
+  };
+  return fits(8)   ? go(std::integral_constant<int, 8>())
+         : fits(2) ? go(std::integral_constant<int, 2>())
+                   : go(std::integral_constant<int, 1>());
 }
 template <bool DUAL>
 cudaError_t few_rows(const RowsArgs& a, int half, int sms, cudaStream_t st) {

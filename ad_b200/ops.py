@@ -844,6 +844,7 @@ def linear_logprobs_workspace(x, weight, grad: bool = False) -> int:
     dt = _half_type(x, "x")
     dev = _device(x, "x")
     rows, width, ldx = _rows(x, "x")
+    _typed(weight, dt, "weight")
     ldw = _matrix(weight, weight.shape[0], width, dt, dev, "weight")
     return _linear_workspace(dev, dt, x, ldx, weight, ldw, rows, width, weight.shape[0], grad)
 
@@ -974,6 +975,8 @@ def _ffn_workspace(dev, dt, operands, dy, lddy, rows, width, hidden, grad):
 def feed_forward_workspace(x, w_gate, w_up, w_down, dy=None) -> int:
     """Bytes of workspace that ``feed_forward`` (with ``dy``: its gradient) needs for these operands."""
     dev, dt, rows, width, hidden, ldx, ldg, ldu, ldd = _ffn_operands(x, w_gate, w_up, w_down, "silu")
+    if dy is not None:
+        _typed(dy, dt, "dy")
     operands = (x.data_ptr(), ldx, w_gate.data_ptr(), ldg, w_up.data_ptr(), ldu, w_down.data_ptr(), ldd)
     return _ffn_workspace(dev, dt, operands, _ptr(dy), 0 if dy is None else _rows(dy, "dy")[2], rows, width, hidden,
                           dy is not None)

@@ -224,7 +224,7 @@ def check_ffn(got, grads, r, t, wt=None):
 @pytest.mark.parametrize("act", ["silu", "gelu", "gelu_tanh", "relu"])
 @pytest.mark.parametrize("t", HALVES)
 @pytest.mark.parametrize("rows,width,hidden", [
-    (1, 1, 1), (1, 64, 64), (2, 8, 24), (3, 1000, 17), (4, 1024, 512), (7, 65, 130), (8, 16, 2000), (9, 16, 64), (17, 65, 33),
+    (1, 1, 1), (1, 64, 64), (2, 8, 24), (3, 1000, 17), (3, 250, 66), (4, 1024, 512), (7, 65, 130), (8, 16, 2000), (9, 16, 64), (17, 65, 33),
     (64, 128, 320), (129, 200, 77), (300, 72, 1000), (1500, 520, 264)])
 def test_feed_forward(ops, act, t, rows, width, hidden):
     x, wg, wu, wd, dy = ffn_operands(t, rows, width, hidden)
@@ -722,6 +722,36 @@ def test_replayed_graphs_follow_their_operands(ops):
         whole.replay()
         for out, (_, call, _, _) in zip(together, graphs):
             assert all(torch.equal(a, b) for a, b in zip(out, call()))
+
+
+@pytest.mark.parametrize("which", range(6))
+def test_first_call_can_be_captured(which):
+    """In a process of its own, with nothing run before."""
+    import os
+    import subprocess
+    import sys
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    code = """
+import torch
+from ad_b200 import ops
+torch.manual_seed(0)
+x, w = torch.randn(40, 64, device="cuda").bfloat16(), torch.randn(96, 64, device="cuda").bfloat16()
+d, t = torch.randn(64, 96, device="cuda").bfloat16(), torch.arange(40, device="cuda")
+kept = torch.randn(2, 40, 96, device="cuda")
+stats = torch.ones(40, 2, device="cuda")
+call = [lambda: ops.embed(t, w), lambda: ops.embed_grad(x, t, 96), lambda: ops.feed_forward(x, w, w, d).y,
+        lambda: ops.feed_forward_grad(x, x, w, w, d, kept[0], kept[1]).w_down, lambda: ops.linear_logprobs(x, w, t).lse,
+        lambda: ops.linear_logprobs_grad(x, w, t, stats, stats[:, 0].contiguous()).weight][%d]
+torch.cuda.synchronize()
+g = torch.cuda.CUDAGraph()
+with torch.cuda.graph(g):
+    y = call()
+for _ in range(2):
+    g.replay()
+assert torch.equal(y, call()) and bool(y.isfinite().all())
+""" % which
+    r = subprocess.run([sys.executable, "-c", code], cwd=root, env={**os.environ, "PYTHONPATH": root}, capture_output=True, text=True, timeout=120)
+    assert r.returncode == 0, r.stderr[-2000:]
 
 
 def test_other_streams_and_threads(ops):

@@ -71,6 +71,15 @@ def test_embed_grad_refuses(kw, error, text):
         ops.embed_grad(**a)
 
 
+def test_workspace_queries_name_what_is_no_array():
+    x, w = far(0, (4, 16)), far(1, (24, 16))
+    for call, name in ((lambda: ops.linear_logprobs_workspace(x, 3), "weight"), (lambda: ops.linear_logprobs_workspace(3, w), "x"),
+                       (lambda: ops.feed_forward_workspace(x, w, w, 3), "w_down"),
+                       (lambda: ops.feed_forward_workspace(x, w, w, far(2, (16, 24)), dy=3), "dy")):
+        with pytest.raises(TypeError, match=f"{name}: expected a device array"):
+            call()
+
+
 def test_embed_grad_workspace_grows():
     sizes = [ops.embed_grad_workspace(n, 1000, 64) for n in (0, 1, 100, 2048, 2049, 100000)]
     assert sizes[0] == 0 and sizes == sorted(sizes) and len(set(sizes)) == len(sizes)

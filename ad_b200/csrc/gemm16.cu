@@ -284,13 +284,14 @@ bool make_schedule(const Problem* p, int count, int tiling, int workers, Schedul
   // odd places: 342 us and 1.5 GB from memory; so 303 and 0.5).
   int parts[MAX_GROUPS], length[MAX_GROUPS];
   bool in_parts = false;
+  int room = workers;  // for parts: no more of them than workers, all groups' together
   for (int g = 0; g < count; ++g) {
     const long long tiles = static_cast<long long>(rows[g]) * cols[g];
     const int n = (kb[g] + 1) * 5 / (height * 3) + 1;
-    const bool few = count > 1 && kb[g] + 1 > height && tiles * n <= workers && kb[g] / n >= 2 * LEAST;
-    parts[g] = few ? n : 1;
-    length[g] = (kb[g] + parts[g] - 1) / parts[g];
-    in_parts |= few;
+    const bool few = count > 1 && kb[g] + 1 > height && tiles * n <= budget && kb[g] / n >= 2 * LEAST;
+    length[g] = few ? (kb[g] + n - 1) / n : kb[g];
+    parts[g] = (kb[g] + length[g] - 1) / length[g];  // none of them empty
+    if (few) in_parts = true, budget -= static_cast<int>(tiles) * parts[g];
     order[g] = g;
     for (int i = g; i > 0 && length[order[i]] > length[order[i - 1]]; --i) std::swap(order[i], order[i - 1]);
   }

@@ -239,7 +239,7 @@ def test_feed_forward(ops, act, t, rows, width, hidden):
 
 
 @pytest.mark.parametrize("t", HALVES)
-@pytest.mark.parametrize("rows,width,hidden", [(5000, 64, 96), (4095, 512, 640), (700, 1001, 2731), (130, 4096, 128), (20000, 40, 16)])
+@pytest.mark.parametrize("rows,width,hidden", [(5000, 64, 96), (4095, 512, 640), (700, 1001, 2731), (130, 4096, 128), (20000, 40, 16), (2467, 385, 1274)])
 def test_feed_forward_products_that_are_cut(ops, t, rows, width, hidden):
     """Sizes whose last round of tiles is cut along K, odd ones among them; results in 32 bits, and added."""
     x, wg, wu, wd, dy = ffn_operands(t, rows, width, hidden)
@@ -405,7 +405,8 @@ def linear_operands(t, rows, width, vocab, lead=()):
 @pytest.mark.parametrize("scale", [1.0, 0.6])
 @pytest.mark.parametrize("rows,width,vocab", [
     (1, 1, 1), (1, 64, 2), (2, 8, 300), (3, 65, 77), (31, 16, 33), (64, 512, 1000), (130, 72, 257), (257, 200, 4099),
-    (1000, 64, 63), (9, 1000, 20000), (600, 1001, 2048)])
+    (1000, 64, 63), (9, 1000, 20000), (600, 1001, 2048),
+    (7, 512, 29204), (2, 128, 28660), (40, 2000, 9000), (200, 300, 31000)])
 def test_linear_logprobs(ops, t, scale, rows, width, vocab):
     x, w, tokens, gp, gl = linear_operands(t, rows, width, vocab)
     want = linear64(x, w, tokens, scale, gp, gl, t)

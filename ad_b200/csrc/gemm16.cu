@@ -284,7 +284,7 @@ bool make_schedule(const Problem* p, int count, int tiling, int workers, Schedul
   // odd places: 342 us and 1.5 GB from memory; so 303 and 0.5).
   int parts[MAX_GROUPS], length[MAX_GROUPS];
   bool in_parts = false;
-  int room = workers;  // for parts: no more of them than workers, all groups' together
+  int budget = workers;  // for parts: no more of them than workers, those of all groups together
   for (int g = 0; g < count; ++g) {
     const long long tiles = static_cast<long long>(rows[g]) * cols[g];
     const int n = (kb[g] + 1) * 5 / (height * 3) + 1;

@@ -285,52 +285,101 @@ __global__ void __launch_bounds__(SORT_THREADS) move_kernel(const __grid_constan
   }
 }
 
-// All passes over at most one tile of keys; other blocks clear.
-__global__ void __launch_bounds__(SORT_THREADS) sort_kernel(const __grid_constant__ SortArgs a, int bits, int passes) {
+// All passes over at most ONE keys, by one block, PER keys a thread; others clear.  A gradient of
+// 5670 tokens of 30000, rows of 1 KB, takes 30 us; in six launches 41.  500 tokens of 1000,
+// rows of 512 bytes: 14.8 us with two keys a thread, 17.0 with eight.
+constexpr int ONE = 8192, ONE_THREADS = 1024, ONE_WARPS = ONE_THREADS / 32;
+struct OneSort {
+  union {
+    unsigned short hist[ONE_WARPS][MAX_DIGITS];  // of the warps, then where their keys go
+    struct {
+      int keys[ONE];
+      short at[ONE];
+    };
+  };
+  int warp_sums[ONE_WARPS];
+};
+template <int PER>
+__global__ void __launch_bounds__(ONE_THREADS) sort_kernel(const __grid_constant__ SortArgs a, int bits, int passes) {
   after_previous();
-  __shared__ TileSort s;
-  int* const keys = s.hist[0];  // in the place of the counts, once these have served
-  short* const at = reinterpret_cast<short*>(s.hist[TILE / MAX_DIGITS]);
+  extern __shared__ __align__(16) unsigned char raw[];
+  OneSort& s = *reinterpret_cast<OneSort*>(raw);
   if (clears(a.clear, 1)) return;
   if (threadIdx.x < 2) a.joins[threadIdx.x] = 0;
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, digits = 1 << bits;
-  int key[KEYS], from[KEYS], digit[KEYS], place[KEYS];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, digits = 1 << bits, d = threadIdx.x;
+  int key[PER], from[PER], digit[PER], place[PER];
 #pragma unroll
-  for (int j = 0; j < KEYS; ++j) {
-    from[j] = warp * (KEYS * 32) + j * 32 + lane;
+  for (int j = 0; j < PER; ++j) {
+    from[j] = warp * (PER * 32) + j * 32 + lane;
     key[j] = from[j] < a.n ? key_of(a, from[j]) : 0;
   }
   for (int p = 0; p < passes; ++p) {
-    for (int d = threadIdx.x; d < digits; d += SORT_THREADS) {
-      s.base[d] = 0;
-#pragma unroll
-      for (int w = 0; w < SORT_WARPS; ++w) s.hist[w][d] = 0;
-    }
+    if (d < digits)
+      for (int w = 0; w < ONE_WARPS; ++w) s.hist[w][d] = 0;
     __syncthreads();
 #pragma unroll
-    for (int j = 0; j < KEYS; ++j) {
-      const bool there = warp * (KEYS * 32) + j * 32 + lane < a.n;
+    for (int j = 0; j < PER; ++j) {  // places among the warp's keys of a digit
+      const bool there = warp * (PER * 32) + j * 32 + lane < a.n;
       digit[j] = there ? (key[j] >> (p * bits)) & (digits - 1) : -1;
-      if (there) atomicAdd(&s.base[digit[j]], 1);
+      const unsigned same = __match_any_sync(0xffffffffu, digit[j]);
+      const int before = __popc(same & ((1u << lane) - 1));
+      const int seen = there ? s.hist[warp][digit[j]] : 0;
+      __syncwarp();
+      if (there && before == 0) s.hist[warp][digit[j]] = static_cast<unsigned short>(seen + __popc(same));
+      __syncwarp();
+      place[j] = seen + before;
     }
     __syncthreads();
-    scan_digits(s.base, digits, s.warp_sums);
-    rank_tile(s, digit, place, digits);
+    // running sums over the digits, of all warps' counts, a digit a thread
+    int mine = 0;
+    if (d < digits)
+      for (int w = 0; w < ONE_WARPS; ++w) mine += s.hist[w][d];
+    int sum = mine;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int x = __shfl_up_sync(0xffffffffu, sum, o);
+      if (lane >= o) sum += x;
+    }
+    if (lane == 31) s.warp_sums[warp] = sum;
+    __syncthreads();
+    if (warp == 0) {
+      int x = s.warp_sums[lane];
+      const int own = x;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const int y = __shfl_up_sync(0xffffffffu, x, o);
+        if (lane >= o) x += y;
+      }
+      s.warp_sums[lane] = x - own;
+    }
+    __syncthreads();
+    if (d < digits) {  // at most 8192: 16 bits hold where they go
+      int run = s.warp_sums[warp] + sum - mine;
+      for (int w = 0; w < ONE_WARPS; ++w) {
+        const int x = s.hist[w][d];
+        s.hist[w][d] = static_cast<unsigned short>(run);
+        run += x;
+      }
+    }
     __syncthreads();
 #pragma unroll
-    for (int j = 0; j < KEYS; ++j)
-      if (digit[j] >= 0) keys[place[j]] = key[j], at[place[j]] = static_cast<short>(from[j]);
+    for (int j = 0; j < PER; ++j)
+      if (digit[j] >= 0) place[j] += s.hist[warp][digit[j]];
+    __syncthreads();  // the counts have served: keys and positions go in their place
+#pragma unroll
+    for (int j = 0; j < PER; ++j)
+      if (digit[j] >= 0) s.keys[place[j]] = key[j], s.at[place[j]] = static_cast<short>(from[j]);
     __syncthreads();
 #pragma unroll
-    for (int j = 0; j < KEYS; ++j) {
-      const int i = warp * (KEYS * 32) + j * 32 + lane;
-      if (i < a.n) key[j] = keys[i], from[j] = at[i];
+    for (int j = 0; j < PER; ++j) {
+      const int i = warp * (PER * 32) + j * 32 + lane;
+      if (i < a.n) key[j] = s.keys[i], from[j] = s.at[i];
     }
     __syncthreads();
   }
 #pragma unroll
-  for (int j = 0; j < KEYS; ++j) {
-    const int i = warp * (KEYS * 32) + j * 32 + lane;
+  for (int j = 0; j < PER; ++j) {
+    const int i = warp * (PER * 32) + j * 32 + lane;
     if (i < a.n) a.keys_out[i] = key[j], a.at_out[i] = from[j];
   }
 }
@@ -540,6 +589,7 @@ __global__ void __launch_bounds__(256) join_kernel(const __grid_constant__ SumAr
 // ------------------------------------------------------------------ host
 
 struct Layout {
+  bool one;  // sorted by one block
   int bits, passes, tiles, chunks;
   long long ldp;
   size_t keys[2], at[2], counts, totals, seen, joins, list, part, total;
@@ -550,6 +600,7 @@ Layout plan(long long rows, long long vocab, long long width) {
   while (vocab >> bits) ++bits;
   l.passes = (bits + MAX_BITS - 1) / MAX_BITS;
   l.bits = (bits + l.passes - 1) / l.passes;
+  l.one = rows <= ONE;
   l.tiles = static_cast<int>((rows + TILE - 1) / TILE);
   l.chunks = static_cast<int>((rows + SPAN - 1) / SPAN);
   l.ldp = (width + 3) / 4 * 4;
@@ -670,7 +721,7 @@ extern "C" int ad_embed_grad(int device, int dtype, const void* dy, int64_t lddy
   // tokens come up; each of the others clears a share of the rows beside its work, and leaves those
   // to the sums (131072 tokens of as many, rows of 8 KB: 454 us, 509 with all rows cleared; 16288
   // tokens of 50001, rows of 4 KB: 94 and 93).
-  const bool note = l.tiles > 1 && !accumulate;
+  const bool note = !l.one && !accumulate;
   Clear clear = {};
   clear.p = static_cast<unsigned char*>(out), clear.row_stride = ldo * os;
   const long long bytes = width * os;
@@ -679,20 +730,27 @@ extern "C" int ad_embed_grad(int device, int dtype, const void* dy, int64_t lddy
   clear.units = static_cast<int>(bytes / clear.unit);
   for (clear.lanes = 1; clear.lanes < 32 && clear.lanes < clear.units;) clear.lanes *= 2;
   for (clear.rows = 8; clear.rows > 1 && clear.rows * bytes > 4096;) clear.rows /= 2;  // 4 KB a warp (8: 98 us instead of 94)
-  const int early = note ? 2 : 0, launches = (l.tiles == 1 ? 1 : 3 * l.passes) - early;
+  const int early = note ? 2 : 0, launches = (l.one ? 1 : 3 * l.passes) - early;
   const long long share = (vocab + 8 * launches - 1) / (8 * launches) * 8;
   auto clearing = [&](int launch) {  // blocks that clear in one of the launches
     if (accumulate || launch < early) return 0u;
     s.clear = clear;
     s.clear.from = std::min<long long>(vocab, (launch - early) * share), s.clear.to = std::min<long long>(vocab, s.clear.from + share);
-    return static_cast<unsigned>(std::min<long long>((s.clear.to - s.clear.from + 8 * clear.rows - 1) / (8 * clear.rows), 32ll * sms));
+    const int per = (l.one ? ONE_WARPS : SORT_WARPS) * clear.rows;  // rows a block
+    return static_cast<unsigned>(std::min<long long>((s.clear.to - s.clear.from + per - 1) / per, (l.one ? 8ll : 32ll) * sms));
   };
   cudaError_t e;
   int to = 0;
-  if (l.tiles == 1) {
+  if (l.one) {
     s.keys_out = ints(l.keys[0]), s.at_out = ints(l.at[0]);
     const unsigned more = clearing(0);
-    e = launch_early<sort_kernel>(dim3(1 + more), SORT_THREADS, 0, st, s, l.bits, l.passes);
+    int most = 0;
+    const bool few = rows <= 2 * ONE_THREADS;
+    e = few ? shared_room<sort_kernel<2>>(&most) : shared_room<sort_kernel<ONE / ONE_THREADS>>(&most);
+    if (e == cudaSuccess && most < static_cast<int>(sizeof(OneSort))) e = cudaErrorInvalidConfiguration;
+    if (e == cudaSuccess)
+      e = few ? launch_early<sort_kernel<2>>(dim3(1 + more), ONE_THREADS, sizeof(OneSort), st, s, l.bits, l.passes)
+              : launch_early<sort_kernel<ONE / ONE_THREADS>>(dim3(1 + more), ONE_THREADS, sizeof(OneSort), st, s, l.bits, l.passes);
     if (e != cudaSuccess) return fail_cuda(who, e);
   } else {
     if (note) {

@@ -9,7 +9,8 @@
 // it gains: dx, dWg, dWu and dWd of a feed-forward block of 4095 x 512 x 2048 took 88 us
 // as three launches with equal splits and their joins, 56 in one (42 since operands are
 // issued as gemm16.cuh says).
-#include <cstdlib>
+#include <memory>
+#include <new>
 
 #include "gemm16.cuh"
 
@@ -394,6 +395,58 @@ bool make_schedule(const Problem* p, int count, int tiling, int workers, Schedul
   return true;
 }
 
+// The best schedule for products of these sizes, or NULL when there are too many
+// tiles for a list.  A program makes the same calls again: a thread keeps the last ones (a
+// schedule takes 2 to 50 us to make).
+struct Sizes {
+  long long m[MAX_GROUPS], n[MAX_GROUPS], k[MAX_GROUPS], k0[MAX_GROUPS];
+  int count, workers[3];
+};
+struct Kept {
+  static constexpr int N = 24;
+  Sizes sizes[N];
+  Schedule schedule[N];
+  bool listed[N];
+  int used = 0, next = 0;
+};
+bool best_schedule(const Problem* p, int count, const int (&workers)[3], Schedule& best) {
+  bool found = false;
+  for (int i = 0; i < 3; ++i) {
+    const Tiling& t = TILINGS[i];
+    if (found) {  // not if it could not do better with all its workers busy all the time
+      double work = 0.0;
+      for (int g = 0; g < count; ++g)
+        work += static_cast<double>((p[g].m + t.m - 1) / t.m) * ((p[g].n + t.n - 1) / t.n) * kblocks_of(p[g]);
+      if (work * t.us / workers[i] + 4.0 > best.us * 0.97) continue;
+    }
+    Schedule s;
+    const bool fits = make_schedule(p, count, i, workers[i], s);
+    if (fits && (!found || s.us < 0.97 * best.us)) best = s, found = true;
+    if (!found) break;  // too many large tiles: one product at a time, by number
+  }
+  return found;
+}
+const Schedule* schedule_for(const Problem* p, int count, const int (&workers)[3], Schedule& room) {
+  thread_local std::unique_ptr<Kept> kept(new (std::nothrow) Kept);
+  Sizes z;
+  memset(&z, 0, sizeof(z));
+  z.count = count;
+  memcpy(z.workers, workers, sizeof(workers));
+  for (int g = 0; g < count; ++g) z.m[g] = p[g].m, z.n[g] = p[g].n, z.k[g] = p[g].k, z.k0[g] = p[g].k0;
+  if (!kept) return best_schedule(p, count, workers, room) ? &room : nullptr;
+  Kept& c = *kept;
+  int at = 0;
+  while (at < c.used && memcmp(&c.sizes[at], &z, sizeof(z))) ++at;
+  if (at == c.used) {
+    at = c.next;
+    c.next = (c.next + 1) % Kept::N;
+    c.used = std::max(c.used, at + 1);
+    c.sizes[at] = z;
+    c.listed[at] = best_schedule(p, count, workers, c.schedule[at]);
+  }
+  return c.listed[at] ? &c.schedule[at] : nullptr;
+}
+
 Target target_of(const Result& r, const Problem& p) {
   Target t = {r.p, r.addend, r.alpha, r.ld, r.ld_addend, r.type, r.accumulate, 1};
   const int per = 16 / elem_size(r.type);
@@ -452,26 +505,14 @@ int store_products(const char* who, const Device& d, int half, const Problem* p,
   Targets to = {};
   to.partial = partial;
   for (int g = 0; g < count; ++g) to.t[g] = target_of(r[g], p[g]);
-  Schedule s[2];
-  int best = -1;
-  for (int i = 0; i < 3; ++i) {
-    const Tiling& t = TILINGS[i];
-    int workers = 0;
-    cudaError_t e = i == 0   ? workers_of<Tile<2, 256, Store<SMALL_LIST>>, Store<SMALL_LIST>>(d, &workers)
-                    : i == 1 ? workers_of<Tile<1, 128, Store<SMALL_LIST>>, Store<SMALL_LIST>>(d, &workers)
-                             : workers_of<Tile<1, 64, Store<SMALL_LIST>>, Store<SMALL_LIST>>(d, &workers);
-    if (e != cudaSuccess) return fail_cuda(who, e);
-    if (best >= 0) {  // not if it could not do better with all its workers busy all the time
-      double work = 0.0;
-      for (int g = 0; g < count; ++g)
-        work += static_cast<double>((p[g].m + t.m - 1) / t.m) * ((p[g].n + t.n - 1) / t.n) * kblocks_of(p[g]);
-      if (work * t.us / workers + 4.0 > s[best].us * 0.97) continue;
-    }
-    const int other = best < 0 ? 0 : 1 - best;
-    if (make_schedule(p, count, i, workers, s[other]) && (best < 0 || s[other].us < 0.97 * s[best].us)) best = other;
-    if (best < 0) break;  // too many large tiles: one product at a time, by number
-  }
-  if (best < 0) {
+  int workers[3];
+  cudaError_t e = workers_of<Tile<2, 256, Store<SMALL_LIST>>, Store<SMALL_LIST>>(d, &workers[0]);
+  if (e == cudaSuccess) e = workers_of<Tile<1, 128, Store<SMALL_LIST>>, Store<SMALL_LIST>>(d, &workers[1]);
+  if (e == cudaSuccess) e = workers_of<Tile<1, 64, Store<SMALL_LIST>>, Store<SMALL_LIST>>(d, &workers[2]);
+  if (e != cudaSuccess) return fail_cuda(who, e);
+  Schedule room;
+  const Schedule* best = schedule_for(p, count, workers, room);
+  if (!best) {
     if (count > 1) {
       for (int g = 0; g < count; ++g)
         if (store_products(who, d, half, p + g, r + g, 1, partial, st)) return 1;
@@ -481,7 +522,7 @@ int store_products(const char* who, const Device& d, int half, const Problem* p,
     params.to = to;
     return start<Store<0>>(who, d, p[0], half, 0, params, st);
   }
-  const Schedule& b = s[best];
+  const Schedule& b = *best;
   return b.tiling == 0   ? start_schedule<2, 256>(who, d, half, p, to, count, b, st)
          : b.tiling == 1 ? start_schedule<1, 128>(who, d, half, p, to, count, b, st)
                          : start_schedule<1, 64>(who, d, half, p, to, count, b, st);

@@ -1001,7 +1001,9 @@ def feed_forward(x, w_gate, w_up, w_down, *, act: str = "silu", keep: bool = Fal
         gate = up = None
         if keep:  # rows that start on 16-byte boundaries, whatever the hidden size is
             ldg = ldu = (hidden + 3) // 4 * 4
-            gate, up = (_empty((rows, ldg), x, "float32")[:, :hidden] for _ in range(2))
+            gate, up = x.new_empty((rows, ldg), dtype=_torch.float32), x.new_empty((rows, ldg), dtype=_torch.float32)
+            if ldg != hidden:
+                gate, up = gate[:, :hidden], up[:, :hidden]
         r = FeedForward(_empty_rows(x), gate, up)
         ldy = width
     else:

@@ -95,7 +95,8 @@ def test_embed_shapes_strides_and_places(ops):
 @pytest.mark.parametrize("t,o", [("float32", "float32"), ("bfloat16", "bfloat16"), ("bfloat16", "float32"), ("float16", "float16")])
 @pytest.mark.parametrize("rows,vocab,width", [
     (1, 1, 1), (1, 7, 64), (31, 3, 5), (32, 1, 128), (33, 1, 128), (2048, 1, 8), (2047, 50, 100), (2049, 1500, 64),
-    (5000, 3, 257), (6000, 1025, 1001), (4100, 70000, 16), (70000, 40, 32), (20000, 2, 2048)])
+    (5000, 3, 257), (6000, 1025, 1001), (4100, 70000, 16), (8192, 9000, 40), (8193, 9000, 40), (70000, 40, 32),
+    (20000, 2, 2048)])
 def test_embed_grad(ops, t, o, rows, vocab, width):
     gen = seeded(rows, vocab, width)
     # some tokens far more frequent than others, some outside of the vocabulary
@@ -321,6 +322,39 @@ def test_feed_forward_of_large_values(ops, act, rows):
     for got, want in ((f.y, a * u), (g.x, slope * u + a * small.double())):
         assert torch.isfinite(got).all()
         assert ((got.double() - want).abs() <= 2.0 ** -6 * want.abs() + 1e-3 * (1 + u.abs())).all()
+
+
+def test_feed_forward_gradients_of_many_sizes_in_turn(ops):
+    # the same bits whatever sizes, devices' streams and threads came before
+    import threading
+
+    gen = seeded(31)
+    x = rand(gen, (70, 64), "bfloat16")
+    weights = [[rand(gen, s, "bfloat16") for s in ((h, 64), (h, 64), (64, h))] for h in range(8, 8 + 33 * 24, 24)]
+
+    def grads(w, stream=None):
+        with torch.cuda.stream(stream or torch.cuda.current_stream()):
+            r = ops.feed_forward(x, *w, keep=True)
+            return r.y, *ops.feed_forward_grad(x, x, *w, r.gate, r.up)
+
+    first = [grads(w) for w in weights]
+    others = {}
+
+    def work(name):
+        stream = torch.cuda.Stream()
+        others[name] = [grads(w, stream) for w in weights[::-1]][::-1]
+        stream.synchronize()
+
+    torch.cuda.synchronize()
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    again = [grads(w) for w in weights]
+    torch.cuda.synchronize()
+    for got in (again, others[0], others[1]):
+        assert all(torch.equal(a, b) for u, v in zip(first, got) for a, b in zip(u, v))
 
 
 @pytest.mark.parametrize("act", ["silu", "gelu", "gelu_tanh"])

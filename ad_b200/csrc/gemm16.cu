@@ -156,10 +156,24 @@ struct Store {
           const float4 x = staged(s, r, q);
           if (s.row0 + r < s.m) finish4(t, alpha, s.row0 + r, col0 + q * 4, x);
         }
-      } else {  // a column a lane
+      } else {  // a column a lane, eight rows read ahead of their stores
         const int col = col0 + s.lane;
-        if (col < s.n)
-          for (int r = 0; r < 32 && s.row0 + r < s.m; ++r) finish1(t, alpha, s.row0 + r, col, staged1(s, r));
+        const long long at = s.row0 * t.ld + col, from = s.row0 * t.ld_addend + col;
+#pragma unroll 1
+        for (int r0 = 0; r0 < 32; r0 += 8) {
+          float x[8], y[8];
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            const bool there = col < s.n && s.row0 + r0 + i < s.m;
+            x[i] = staged1(s, r0 + i);
+            if (t.addend && there) x[i] += t.addend[from + (r0 + i) * t.ld_addend];
+            y[i] = t.accumulate && there ? load_any(t.out, t.type, at + (r0 + i) * t.ld) : 0.0f;
+          }
+#pragma unroll
+          for (int i = 0; i < 8; ++i)
+            if (col < s.n && s.row0 + r0 + i < s.m)
+              store_any(t.out, t.type, at + (r0 + i) * t.ld, t.accumulate ? x[i] * alpha + y[i] : x[i] * alpha);
+        }
       }
     }
   };

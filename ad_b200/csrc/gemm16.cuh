@@ -215,6 +215,11 @@ __device__ __forceinline__ void tmem_ld32(unsigned taddr, float (&v)[32]) {
   for (int j = 0; j < 32; ++j) v[j] = __uint_as_float(q[j]);
 }
 
+__device__ __forceinline__ unsigned lds32(unsigned addr) {
+  unsigned v;
+  asm volatile("ld.shared.u32 %0, [%1];" : "=r"(v) : "r"(addr) : "memory");
+  return v;
+}
 __device__ __forceinline__ uint4 lds128(unsigned addr) {
   uint4 v;
   asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(addr) : "memory");
@@ -291,27 +296,35 @@ __device__ __forceinline__ void put16(const Spot& s, const unsigned (&w)[16], un
       to += 8 * ld;
     }
   } else {
-    // two rows at a time, half a warp each, two columns a lane: words where they are
-    // aligned, else words from the second column on and the first and last one apart
-    const int h = s.lane >> 4, l = s.lane & 15;
-    auto at = [&](int r, int c) {
-      unsigned short x;
-      asm volatile("ld.shared.u16 %0, [%1];"
-                   : "=h"(x)
-                   : "r"(s.side + r * 64 + (((c >> 3) ^ ((r >> 1) & 3)) << 4) + (c & 7) * 2)
-                   : "memory");
-      return x;
-    };
-    for (int r = h; r < 32 && s.row0 + r < m; r += 2) {
-      unsigned short* row = out + (s.row0 + r) * ld + col0;
-      const int shift = (reinterpret_cast<uintptr_t>(row) >> 1) & 1;
-      const int c0 = 2 * l + shift, c1 = c0 + 1 < 32 ? c0 + 1 : 0;  // of the last lane: the first column
-      const unsigned short x0 = at(r, c0), x1 = at(r, c1);
-      if (c1 && col0 + c1 < n) {
-        *reinterpret_cast<unsigned*>(row + c0) = x0 | static_cast<unsigned>(x1) << 16;
-      } else {
-        if (col0 + c0 < n) row[c0] = x0;
-        if (!c1) row[0] = x1;
+    // two rows at a time, half a warp each, a word a lane; where the row starts in the
+    // upper half of one, words from the second column on, and the first and last one
+    // apart by the last lane.  Read ahead of the stores, eight at a time (dW of 62044 x
+    // 3802 over 4: 296 us, 491 one at a time; 142 where rows are aligned).
+    const int h = s.lane >> 4, l = s.lane & 15, left = n - col0;
+    unsigned short* row = out + (s.row0 + h) * ld + col0;
+    const int shift = (reinterpret_cast<uintptr_t>(row) >> 1) & 1;  // of every second row too
+    const int c0 = 2 * l + shift, c1 = (c0 + 1) & 31;
+#pragma unroll 1
+    for (int r0 = h; r0 < 32; r0 += 16) {
+      unsigned x[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const int r = r0 + 2 * i;
+        x[i] = lds32(s.side + r * 64 + (((l >> 2) ^ ((r >> 1) & 3)) << 4) + (l & 3) * 4);
+        const unsigned next = __shfl_sync(0xffffffffu, x[i], (l + 1) & 15, 16);
+        if (shift) x[i] = x[i] >> 16 | next << 16;
+      }
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        if (s.row0 + r0 + 2 * i < m) {
+          if (c1 && c1 < left) {
+            *reinterpret_cast<unsigned*>(row + c0) = x[i];
+          } else {
+            if (c0 < left) row[c0] = static_cast<unsigned short>(x[i]);
+            if (!c1) row[0] = static_cast<unsigned short>(x[i] >> 16);
+          }
+        }
+        row += 2 * ld;
       }
     }
   }

@@ -8,15 +8,17 @@
 // Gradient: the rows of dy that belong to one token are summed in the order of
 // their positions, so that nothing depends on scheduling.  Positions are sorted by
 // token (a stable radix sort of at most 10 bits a pass: counts of each 2048 keys, their
-// running sums, the move); sorted positions are cut into chunks of 32, and a warp walks
+// running sums, the move; up to 16384 keys all in one launch); sorted positions are cut into chunks of 32, and a warp walks
 // a chunk over a slice of columns, with a running sum in 32 bits.  A token whose rows
 // lie in one chunk is written there and then; a sum that goes on in the next chunk
 // is left in memory, and a last kernel joins such partial sums, a block a token and
 // slice, found through a list.  A token that comes up thousands of times so costs
 // no more than others.  Rows of tokens that do not come up are cleared by further
-// blocks of the sort's launches, once the first two have noted which these are.
+// blocks of the sort's launches, once the first two have noted which these are (in one
+// launch: all rows).
 #include <algorithm>
 #include <cmath>
+#include <type_traits>
 
 #include "ops_common.cuh"
 
@@ -215,6 +217,18 @@ __device__ __forceinline__ void scan_digits(int* v, int digits, int* warp_sums) 
   __syncthreads();
 }
 
+// The lanes with this lane's digit (-1: none), bit by bit: __match_any_sync takes longer the more
+// digits differ (8192 tokens sorted by a block: 45 us, 40).
+__device__ __forceinline__ unsigned same_digit(int digit) {
+  unsigned same = __ballot_sync(0xffffffffu, digit >= 0);
+#pragma unroll
+  for (int b = 0; b < MAX_BITS; ++b) {
+    const unsigned set = __ballot_sync(0xffffffffu, digit >> b & 1);
+    same &= digit >> b & 1 ? set : ~set;
+  }
+  return same;
+}
+
 // Where each key of a tile goes: its place among the tile's keys of its digit,
 // from the warps' counts.  `base`: where the tile's first key of each digit goes.
 struct TileSort {
@@ -227,7 +241,7 @@ __device__ __forceinline__ void rank_tile(TileSort& s, const int (&digit)[KEYS],
 #pragma unroll
   for (int j = 0; j < KEYS; ++j) {
     // lanes behind the last key have a digit of -1
-    const unsigned same = __match_any_sync(0xffffffffu, digit[j]);
+    const unsigned same = same_digit(digit[j]);
     const int before = __popc(same & ((1u << lane) - 1));
     int seen = 0;
     if (digit[j] >= 0) seen = s.hist[warp][digit[j]];
@@ -285,10 +299,10 @@ __global__ void __launch_bounds__(SORT_THREADS) move_kernel(const __grid_constan
   }
 }
 
-// All passes over at most ONE keys, by one block, PER keys a thread; others clear.  A gradient of
-// 5670 tokens of 30000, rows of 1 KB, takes 30 us; in six launches 41.  500 tokens of 1000,
-// rows of 512 bytes: 14.8 us with two keys a thread, 17.0 with eight.
-constexpr int ONE = 8192, ONE_THREADS = 1024, ONE_WARPS = ONE_THREADS / 32;
+// All passes over at most ONE keys, by one block, PER keys a thread; others clear.  (Gradients of
+// 2049 tokens of 1000, rows of 512 bytes: 16.5 us, in three launches 23.3.  Of 500 of them: 14.1,
+// 17.0 with eight keys a thread.)
+constexpr int ONE = 4096, ONE_THREADS = 1024, ONE_WARPS = ONE_THREADS / 32;
 struct OneSort {
   union {
     unsigned short hist[ONE_WARPS][MAX_DIGITS];  // of the warps, then where their keys go
@@ -319,9 +333,11 @@ __global__ void __launch_bounds__(ONE_THREADS) sort_kernel(const __grid_constant
     __syncthreads();
 #pragma unroll
     for (int j = 0; j < PER; ++j) {  // places among the warp's keys of a digit
+      digit[j] = -1;
+      if (warp * (PER * 32) + j * 32 >= a.n) continue;
       const bool there = warp * (PER * 32) + j * 32 + lane < a.n;
       digit[j] = there ? (key[j] >> (p * bits)) & (digits - 1) : -1;
-      const unsigned same = __match_any_sync(0xffffffffu, digit[j]);
+      const unsigned same = same_digit(digit[j]);
       const int before = __popc(same & ((1u << lane) - 1));
       const int seen = there ? s.hist[warp][digit[j]] : 0;
       __syncwarp();
@@ -353,7 +369,7 @@ __global__ void __launch_bounds__(ONE_THREADS) sort_kernel(const __grid_constant
       s.warp_sums[lane] = x - own;
     }
     __syncthreads();
-    if (d < digits) {  // at most 8192: 16 bits hold where they go
+    if (d < digits) {
       int run = s.warp_sums[warp] + sum - mine;
       for (int w = 0; w < ONE_WARPS; ++w) {
         const int x = s.hist[w][d];
@@ -381,6 +397,128 @@ __global__ void __launch_bounds__(ONE_THREADS) sort_kernel(const __grid_constant
   for (int j = 0; j < PER; ++j) {
     const int i = warp * (PER * 32) + j * 32 + lane;
     if (i < a.n) a.keys_out[i] = key[j], a.at_out[i] = from[j];
+  }
+}
+
+// All passes over at most MANY keys, by the blocks of one cluster, PER keys a thread; other
+// clusters clear.  The blocks tell one another how often each digit comes up through their
+// shared memory; keys go from pass to pass through L2.
+// (5670 tokens of 30000, rows of 1 KB: 25.8 us; one block 29.7, six launches 41.0.  16288 of 50001,
+// rows of 2 KB: 40 and 61.  With eight keys a thread 16385 of 30000 take 50, in six launches 40: a
+// key's place is anywhere, and a multiprocessor stores 32 bytes a clock.)
+constexpr int CLUSTER = 8, MANY = 2 * ONE_THREADS * CLUSTER;
+struct ManySort {
+  unsigned short hist[ONE_WARPS][MAX_DIGITS];  // of the warps, then where their keys go: less than MANY
+  int total[MAX_DIGITS];                       // of the block
+  int warp_sums[ONE_WARPS];
+};
+static_assert(MANY <= 0x10000, "16 bits hold where a key goes");
+struct Passes {
+  int *keys[2], *at[2];  // pass p writes p & 1
+  int bits, count;
+};
+__device__ __forceinline__ int read_of(const int* mine, int rank) {
+  int v;
+  asm volatile(
+      "{\n\t.reg .u32 there;\n\t"
+      "mapa.shared::cluster.u32 there, %1, %2;\n\t"
+      "ld.shared::cluster.s32 %0, [there];\n\t}"
+      : "=r"(v)
+      : "r"(static_cast<unsigned>(__cvta_generic_to_shared(mine))), "r"(rank)
+      : "memory");
+  return v;
+}
+__device__ __forceinline__ void cluster_sync() {
+  __syncwarp();
+  asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+  asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+template <int PER>
+__global__ void __launch_bounds__(ONE_THREADS) cluster_sort_kernel(const __grid_constant__ SortArgs a, const __grid_constant__ Passes b) {
+  after_previous();
+  extern __shared__ __align__(16) unsigned char raw[];
+  ManySort& s = *reinterpret_cast<ManySort*>(raw);
+  if (clears(a.clear, CLUSTER)) return;  // whole clusters
+  const int rank = blockIdx.x;           // of the first one
+  if (rank == 0 && threadIdx.x < 2) a.joins[threadIdx.x] = 0;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, digits = 1 << b.bits, d = threadIdx.x;
+  const int first = rank * (PER * ONE_THREADS) + warp * (PER * 32) + lane;
+  int key[PER], from[PER], digit[PER], place[PER];
+  for (int p = 0; p < b.count; ++p) {
+    const int in = p & 1 ? 0 : 1;
+#pragma unroll
+    for (int j = 0; j < PER; ++j) {
+      const int i = first + j * 32;
+      key[j] = i >= a.n ? 0 : p ? __ldcg(b.keys[in] + i) : key_of(a, i);
+      from[j] = i >= a.n ? 0 : p ? __ldcg(b.at[in] + i) : i;
+    }
+    if (d < digits)
+      for (int w = 0; w < ONE_WARPS; ++w) s.hist[w][d] = 0;
+    __syncthreads();
+#pragma unroll
+    for (int j = 0; j < PER; ++j) {  // places among the warp's keys of a digit
+      const bool there = first + j * 32 < a.n;
+      digit[j] = there ? (key[j] >> (p * b.bits)) & (digits - 1) : -1;
+      const unsigned same = same_digit(digit[j]);
+      const int before = __popc(same & ((1u << lane) - 1));
+      const int seen = there ? s.hist[warp][digit[j]] : 0;
+      __syncwarp();
+      if (there && before == 0) s.hist[warp][digit[j]] = static_cast<unsigned short>(seen + __popc(same));
+      __syncwarp();
+      place[j] = seen + before;
+    }
+    __syncthreads();
+    int mine = 0;
+    if (d < digits) {
+      for (int w = 0; w < ONE_WARPS; ++w) mine += s.hist[w][d];
+      s.total[d] = mine;
+    }
+    cluster_sync();
+    int all = 0, ahead = 0;  // of the cluster's blocks, and of those before this one
+    if (d < digits) {
+#pragma unroll
+      for (int q = 0; q < CLUSTER; ++q) {
+        const int x = read_of(&s.total[d], q);
+        all += x;
+        if (q < rank) ahead += x;
+      }
+    }
+    int sum = all;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int x = __shfl_up_sync(0xffffffffu, sum, o);
+      if (lane >= o) sum += x;
+    }
+    if (lane == 31) s.warp_sums[warp] = sum;
+    __syncthreads();
+    if (warp == 0) {
+      int x = s.warp_sums[lane];
+      const int own = x;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const int y = __shfl_up_sync(0xffffffffu, x, o);
+        if (lane >= o) x += y;
+      }
+      s.warp_sums[lane] = x - own;
+    }
+    __syncthreads();
+    if (d < digits) {
+      int run = s.warp_sums[warp] + sum - all + ahead;
+      for (int w = 0; w < ONE_WARPS; ++w) {
+        const int x = s.hist[w][d];
+        s.hist[w][d] = static_cast<unsigned short>(run);
+        run += x;
+      }
+    }
+    __syncthreads();
+#pragma unroll
+    for (int j = 0; j < PER; ++j) {
+      if (digit[j] < 0) continue;
+      const int to = place[j] + s.hist[warp][digit[j]];
+      __stcg(b.keys[in ^ 1] + to, key[j]);
+      __stcg(b.at[in ^ 1] + to, from[j]);
+    }
+    cluster_sync();  // what was written is there for all; and no block leaves, or counts again, ahead of the others' reads
   }
 }
 
@@ -589,7 +727,7 @@ __global__ void __launch_bounds__(256) join_kernel(const __grid_constant__ SumAr
 // ------------------------------------------------------------------ host
 
 struct Layout {
-  bool one;  // sorted by one block
+  bool one, many;  // sorted by one block, by a cluster
   int bits, passes, tiles, chunks;
   long long ldp;
   size_t keys[2], at[2], counts, totals, seen, joins, list, part, total;
@@ -600,7 +738,7 @@ Layout plan(long long rows, long long vocab, long long width) {
   while (vocab >> bits) ++bits;
   l.passes = (bits + MAX_BITS - 1) / MAX_BITS;
   l.bits = (bits + l.passes - 1) / l.passes;
-  l.one = rows <= ONE;
+  l.one = rows <= ONE, l.many = !l.one && rows <= MANY;
   l.tiles = static_cast<int>((rows + TILE - 1) / TILE);
   l.chunks = static_cast<int>((rows + SPAN - 1) / SPAN);
   l.ldp = (width + 3) / 4 * 4;
@@ -717,11 +855,11 @@ extern "C" int ad_embed_grad(int device, int dtype, const void* dy, int64_t lddy
   SortArgs s = {};
   s.tokens = tokens, s.tok64 = tok64, s.vocab = vocab, s.n = static_cast<int>(rows), s.tiles = l.tiles;
   s.counts = ints(l.counts), s.totals = ints(l.totals), s.joins = ints(l.joins);
-  // The launches of the sort wait for memory most of the time.  The first two note which
+  // One launch sorts few tokens, and clears all rows beside.  With more,
+  // the launches of the sort wait for memory most of the time.  The first two note which
   // tokens come up; each of the others clears a share of the rows beside its work, and leaves those
-  // to the sums (131072 tokens of as many, rows of 8 KB: 454 us, 509 with all rows cleared; 16288
-  // tokens of 50001, rows of 4 KB: 94 and 93).
-  const bool note = !l.one && !accumulate;
+  // to the sums (131072 tokens of as many, rows of 8 KB: 454 us, 509 with all rows cleared).
+  const bool single = l.one || l.many, note = !single && !accumulate;
   Clear clear = {};
   clear.p = static_cast<unsigned char*>(out), clear.row_stride = ldo * os;
   const long long bytes = width * os;
@@ -730,14 +868,14 @@ extern "C" int ad_embed_grad(int device, int dtype, const void* dy, int64_t lddy
   clear.units = static_cast<int>(bytes / clear.unit);
   for (clear.lanes = 1; clear.lanes < 32 && clear.lanes < clear.units;) clear.lanes *= 2;
   for (clear.rows = 8; clear.rows > 1 && clear.rows * bytes > 4096;) clear.rows /= 2;  // 4 KB a warp (8: 98 us instead of 94)
-  const int early = note ? 2 : 0, launches = (l.one ? 1 : 3 * l.passes) - early;
+  const int early = note ? 2 : 0, launches = (single ? 1 : 3 * l.passes) - early;
   const long long share = (vocab + 8 * launches - 1) / (8 * launches) * 8;
   auto clearing = [&](int launch) {  // blocks that clear in one of the launches
     if (accumulate || launch < early) return 0u;
     s.clear = clear;
     s.clear.from = std::min<long long>(vocab, (launch - early) * share), s.clear.to = std::min<long long>(vocab, s.clear.from + share);
-    const int per = (l.one ? ONE_WARPS : SORT_WARPS) * clear.rows;  // rows a block
-    return static_cast<unsigned>(std::min<long long>((s.clear.to - s.clear.from + per - 1) / per, (l.one ? 8ll : 32ll) * sms));
+    const int per = (single ? ONE_WARPS : SORT_WARPS) * clear.rows;  // rows a block
+    return static_cast<unsigned>(std::min<long long>((s.clear.to - s.clear.from + per - 1) / per, (single ? 8ll : 32ll) * sms));
   };
   cudaError_t e;
   int to = 0;
@@ -745,12 +883,30 @@ extern "C" int ad_embed_grad(int device, int dtype, const void* dy, int64_t lddy
     s.keys_out = ints(l.keys[0]), s.at_out = ints(l.at[0]);
     const unsigned more = clearing(0);
     int most = 0;
-    const bool few = rows <= 2 * ONE_THREADS;
-    e = few ? shared_room<sort_kernel<2>>(&most) : shared_room<sort_kernel<ONE / ONE_THREADS>>(&most);
-    if (e == cudaSuccess && most < static_cast<int>(sizeof(OneSort))) e = cudaErrorInvalidConfiguration;
-    if (e == cudaSuccess)
-      e = few ? launch_early<sort_kernel<2>>(dim3(1 + more), ONE_THREADS, sizeof(OneSort), st, s, l.bits, l.passes)
-              : launch_early<sort_kernel<ONE / ONE_THREADS>>(dim3(1 + more), ONE_THREADS, sizeof(OneSort), st, s, l.bits, l.passes);
+    auto go = [&](auto v) {
+      constexpr int PER = decltype(v)::value;
+      const cudaError_t f = shared_room<sort_kernel<PER>>(&most);
+      if (f != cudaSuccess) return f;
+      if (most < static_cast<int>(sizeof(OneSort))) return cudaErrorInvalidConfiguration;
+      return launch_early<sort_kernel<PER>>(dim3(1 + more), ONE_THREADS, sizeof(OneSort), st, s, l.bits, l.passes);
+    };
+    e = rows <= ONE_THREADS       ? go(std::integral_constant<int, 1>())
+        : rows <= 2 * ONE_THREADS ? go(std::integral_constant<int, 2>())
+                                  : go(std::integral_constant<int, 4>());
+    if (e != cudaSuccess) return fail_cuda(who, e);
+  } else if (l.many) {
+    to = (l.passes - 1) & 1;
+    const Passes b = {{ints(l.keys[0]), ints(l.keys[1])}, {ints(l.at[0]), ints(l.at[1])}, l.bits, l.passes};
+    const unsigned more = (clearing(0) + CLUSTER - 1) / CLUSTER * CLUSTER;
+    int most = 0;
+    auto go = [&](auto v) {
+      constexpr int PER = decltype(v)::value;
+      const cudaError_t f = shared_room<cluster_sort_kernel<PER>>(&most);
+      if (f != cudaSuccess) return f;
+      if (most < static_cast<int>(sizeof(ManySort))) return cudaErrorInvalidConfiguration;
+      return launch_early_cluster<cluster_sort_kernel<PER>>(CLUSTER, dim3(CLUSTER + more), ONE_THREADS, sizeof(ManySort), st, s, b);
+    };
+    e = rows <= ONE_THREADS * CLUSTER ? go(std::integral_constant<int, 1>()) : go(std::integral_constant<int, 2>());
     if (e != cudaSuccess) return fail_cuda(who, e);
   } else {
     if (note) {

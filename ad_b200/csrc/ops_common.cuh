@@ -73,6 +73,23 @@ cudaError_t launch_early(dim3 grid, dim3 block, int bytes, cudaStream_t s, const
   c.numAttrs = 1;
   return cudaLaunchKernelEx(&c, KERNEL, a...);
 }
+// And in clusters of blocks.
+template <auto KERNEL, typename... A>
+cudaError_t launch_early_cluster(int cluster, dim3 grid, dim3 block, int bytes, cudaStream_t s, const A&... a) {
+  cudaLaunchConfig_t c = {};
+  c.gridDim = grid;
+  c.blockDim = block;
+  c.dynamicSmemBytes = bytes;
+  c.stream = s;
+  cudaLaunchAttribute at[2];
+  at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at[0].val.programmaticStreamSerializationAllowed = 1;
+  at[1].id = cudaLaunchAttributeClusterDimension;
+  at[1].val.clusterDim.x = cluster, at[1].val.clusterDim.y = at[1].val.clusterDim.z = 1;
+  c.attrs = at;
+  c.numAttrs = 2;
+  return cudaLaunchKernelEx(&c, KERNEL, a...);
+}
 
 // Makes `device` current for one call (-1: the current one) and puts the
 // caller's device back at its end.

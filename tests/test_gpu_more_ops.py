@@ -95,7 +95,8 @@ def test_embed_shapes_strides_and_places(ops):
 @pytest.mark.parametrize("t,o", [("float32", "float32"), ("bfloat16", "bfloat16"), ("bfloat16", "float32"), ("float16", "float16")])
 @pytest.mark.parametrize("rows,vocab,width", [
     (1, 1, 1), (1, 7, 64), (31, 3, 5), (32, 1, 128), (33, 1, 128), (2048, 1, 8), (2047, 50, 100), (2049, 1500, 64),
-    (5000, 3, 257), (6000, 1025, 1001), (4100, 70000, 16), (8192, 9000, 40), (8193, 9000, 40), (70000, 40, 32),
+    (5000, 3, 257), (6000, 1025, 1001), (4100, 70000, 16), (8192, 9000, 40), (8193, 9000, 40), (16384, 1, 8),
+    (16385, 2000000, 8), (33000, 1500, 33), (65536, 70000, 8), (65536, 1, 8), (65537, 1024, 8), (70000, 40, 32),
     (20000, 2, 2048)])
 def test_embed_grad(ops, t, o, rows, vocab, width):
     gen = seeded(rows, vocab, width)

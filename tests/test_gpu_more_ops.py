@@ -721,10 +721,14 @@ def calls(ops, seed):
     r = ops.linear_logprobs(x, table, t300)
     g = rand(gen, (300,), "float32")
     grads = [rand(gen, (70, 11), "float32"), rand(gen, (999,), "bfloat16")]
+    many, wide = torch.randint(-1, 9000, (20000,), generator=gen).cuda(), rand(gen, (20000, 24), "bfloat16")
     return [
         (lambda: [ops.embed(tokens, table)], table),
         (lambda: [ops.embed_grad(d, tokens, 500)], d),
         (lambda: [ops.embed_grad(d[:200], tokens[:200], 500)], d),
+        (lambda: [ops.embed_grad(wide[:6000], many[:6000], 9000)], wide),
+        (lambda: [ops.embed_grad(wide[:15000], many[:15000], 9000)], wide),
+        (lambda: [ops.embed_grad(wide, many, 9000)], wide),
         (lambda: [ops.feed_forward(x, wg, wu, wd).y], x),
         (lambda: [ops.feed_forward(x[:3], wg, wu, wd).y], x),
         (lambda: list(ops.feed_forward_grad(dy, x, wg, wu, wd, f.gate, f.up)), dy),
@@ -760,7 +764,7 @@ def test_replayed_graphs_follow_their_operands(ops):
             assert all(torch.equal(a, b) for a, b in zip(out, call()))
 
 
-@pytest.mark.parametrize("which", range(6))
+@pytest.mark.parametrize("which", range(7))
 def test_first_call_can_be_captured(which):
     """In a process of its own, with nothing run before."""
     import os
@@ -777,7 +781,8 @@ kept = torch.randn(2, 40, 96, device="cuda")
 stats = torch.ones(40, 2, device="cuda")
 call = [lambda: ops.embed(t, w), lambda: ops.embed_grad(x, t, 96), lambda: ops.feed_forward(x, w, w, d).y,
         lambda: ops.feed_forward_grad(x, x, w, w, d, kept[0], kept[1]).w_down, lambda: ops.linear_logprobs(x, w, t).lse,
-        lambda: ops.linear_logprobs_grad(x, w, t, stats, stats[:, 0].contiguous()).weight][%d]
+        lambda: ops.linear_logprobs_grad(x, w, t, stats, stats[:, 0].contiguous()).weight,
+        lambda: ops.embed_grad(x.repeat(200, 1), t.repeat(200), 96)][%d]
 torch.cuda.synchronize()
 g = torch.cuda.CUDAGraph()
 with torch.cuda.graph(g):

@@ -377,6 +377,15 @@ __device__ __forceinline__ void put32(const Spot& s, const float (&v)[32], float
   }
 }
 
+// Rows of A that a copy brings, where there are m: rows outside of the operand cost time,
+// although they are not read (the loss of 4 rows over 130000 tokens of width 2048: 147 us with
+// copies of 128 rows, 94 of 4; from 32 rows on 96). What then is left in their place
+// in shared memory only goes to rows of the product that there are none of.
+template <int CTAS>
+__host__ __device__ __forceinline__ int rows_of_box(int m) {
+  return CTAS == 1 && m < 128 ? m : 128;
+}
+
 // ------------------------------------------------------------------ the kernel
 
 // A place among the stages, the phase of its barriers, and whether it has been used before.
@@ -483,7 +492,7 @@ __global__ void __launch_bounds__(TILE::THREADS, 1)
             const unsigned st = smem_u32(smem) + ring.i * TILE::STAGE, sq = st + TILE::P_BYTES, bar = leader + ring.i * 8;
             if (rank == 0)
               asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(smem_u32(&full[ring.i])),
-                           "r"(CTAS * TILE::STAGE)
+                           "r"(AT ? CTAS * TILE::STAGE : CTAS * TILE::STAGE - (128 - rows_of_box<CTAS>(g.m)) * 128)
                            : "memory");
             if (AT) {
 #pragma unroll
@@ -683,7 +692,9 @@ int make_maps(const Problem& p, Maps& maps, int map) {
     const long long k = DUAL || p.k0 == p.k ? p.k : i ? p.k - p.k0 : p.k0;
     if (!DUAL || i == 0) {
       if (p.a_turned ? ad_b200_internal::tmap_2d_16(p.a[i].p, k, p.m, p.a[i].ld, 64, 64, &maps.a[map + i])
-                     : ad_b200_internal::tmap_2d_16(p.a[i].p, p.m, k, p.a[i].ld, 128, 64, &maps.a[map + i]))
+                     : ad_b200_internal::tmap_2d_16(p.a[i].p, p.m, k, p.a[i].ld,
+                                                     rows_of_box<TILE::CTAS>(static_cast<int>(std::min(p.m, 128ll))), 64,
+                                                     &maps.a[map + i]))
         return 1;
     }
     const int rows = DUAL && TILE::CTAS == 1 ? TILE::QN / 2 : TILE::QN;

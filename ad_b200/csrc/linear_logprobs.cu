@@ -155,9 +155,14 @@ __global__ void __launch_bounds__(32 * FINISH_WARPS) finish_kernel(const __grid_
   a.stats[row] = make_float2(top, sum);
 }
 
-// The power of two for f16 (factor[0]) and its reciprocal (factor[1]).
+// The power of two for f16 (factor[0]) and its reciprocal (factor[1]), from the rows' gradients as
+// far as they have a part in any: g_logp not where there is no token, and nothing of a row whose
+// token is past the vocabulary, which is NaN whatever the factor is.
 struct RangeArgs {
   const float *g_logp, *g_lse;
+  const void* tokens;
+  int tok64;
+  long long vocab;
   int rows;
   float scale;
   float* factor;
@@ -166,8 +171,11 @@ __global__ void __launch_bounds__(1024) range_kernel(const __grid_constant__ Ran
   after_previous();
   __shared__ float buf[32];
   float most = 0.0f;
-  for (int i = threadIdx.x; i < a.rows; i += 1024)
-    most = fmaxf(most, (a.g_logp ? 2.0f * fabsf(a.g_logp[i]) : 0.0f) + (a.g_lse ? fabsf(a.g_lse[i]) : 0.0f));
+  for (int i = threadIdx.x; i < a.rows; i += 1024) {
+    const long long t = token_at(a.tokens, a.tok64, i);
+    if (t >= a.vocab) continue;
+    most = fmaxf(most, (a.g_logp && t >= 0 ? 2.0f * fabsf(a.g_logp[i]) : 0.0f) + (a.g_lse ? fabsf(a.g_lse[i]) : 0.0f));
+  }
 #pragma unroll
   for (int o = 16; o; o >>= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, o));
   if ((threadIdx.x & 31) == 0) buf[threadIdx.x >> 5] = most;
@@ -417,7 +425,7 @@ extern "C" int ad_linear_logprobs_grad(int device, int dtype, const void* x, int
   if (pack(who, d, l, x, ldx, weight, ldw, rows, width, vocab, ws, st)) return 1;
   float* factor = half ? reinterpret_cast<float*>(ws + l.factor) : nullptr;
   if (half) {
-    const RangeArgs r = {g_logp, g_lse, static_cast<int>(rows), scale, factor};
+    const RangeArgs r = {g_logp, g_lse, tokens, tok64, vocab, static_cast<int>(rows), scale, factor};
     const cudaError_t e = launch_early<range_kernel>(1, 1024, 0, st, r);
     if (e != cudaSuccess) return fail_cuda(who, e);
   }

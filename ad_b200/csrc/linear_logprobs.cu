@@ -157,7 +157,8 @@ __global__ void __launch_bounds__(32 * FINISH_WARPS) finish_kernel(const __grid_
 
 // The power of two for f16 (factor[0]) and its reciprocal (factor[1]), from the rows' gradients as
 // far as they have a part in any: g_logp not where there is no token, and nothing of a row whose
-// token is past the vocabulary, which is NaN whatever the factor is.
+// token is past the vocabulary, which is NaN whatever the factor is; nor of rows whose gradients are
+// infinite or NaN.  In 64 bits: a gradient times the scale may be past 32.
 struct RangeArgs {
   const float *g_logp, *g_lse;
   const void* tokens;
@@ -169,22 +170,23 @@ struct RangeArgs {
 };
 __global__ void __launch_bounds__(1024) range_kernel(const __grid_constant__ RangeArgs a) {
   after_previous();
-  __shared__ float buf[32];
-  float most = 0.0f;
+  __shared__ double buf[32];
+  double most = 0.0;
   for (int i = threadIdx.x; i < a.rows; i += 1024) {
     const long long t = token_at(a.tokens, a.tok64, i);
     if (t >= a.vocab) continue;
-    most = fmaxf(most, (a.g_logp && t >= 0 ? 2.0f * fabsf(a.g_logp[i]) : 0.0f) + (a.g_lse ? fabsf(a.g_lse[i]) : 0.0f));
+    const double gp = a.g_logp && t >= 0 ? a.g_logp[i] : 0.0f, gl = a.g_lse ? a.g_lse[i] : 0.0f;
+    const double size = 2.0 * fabs(gp) + fabs(gl);
+    if (size < INFINITY) most = fmax(most, size);
   }
 #pragma unroll
-  for (int o = 16; o; o >>= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, o));
+  for (int o = 16; o; o >>= 1) most = fmax(most, __shfl_xor_sync(0xffffffffu, most, o));
   if ((threadIdx.x & 31) == 0) buf[threadIdx.x >> 5] = most;
   __syncthreads();
   if (threadIdx.x == 0) {
-    for (int w = 1; w < 32; ++w) most = fmaxf(most, buf[w]);
+    for (int w = 1; w < 32; ++w) most = fmax(most, buf[w]);
     most *= a.scale;
-    int e = 0;
-    if (most > 0.0f && most < INFINITY) e = max(-126, min(126, 14 - ilogbf(most)));
+    const int e = most > 0.0 ? max(-126, min(126, 14 - ilogb(most))) : 0;
     a.factor[0] = ldexpf(1.0f, e);
     a.factor[1] = ldexpf(1.0f, -e);
   }
@@ -216,11 +218,12 @@ struct Slope {
       if (row >= s.m) return;
       const float2 st = p.stats[row];
       const long long t = token_at(p.tokens, p.tok64, row);
-      const float f = p.factor ? *p.factor : 1.0f;
-      const float gp = p.g_logp && t >= 0 ? p.g_logp[row] : 0.0f, gl = p.g_lse ? p.g_lse[row] : 0.0f;
+      // in 64 bits until the factor is on: without it they may be past 32
+      const double f = p.scale * (p.factor ? static_cast<double>(*p.factor) : 1.0);
+      const double gp = p.g_logp && t >= 0 ? p.g_logp[row] : 0.0f, gl = p.g_lse ? p.g_lse[row] : 0.0f;
       top = st.x;
-      of_p = t >= p.vocab ? __int_as_float(0x7fffffff) : p.scale * (gl - gp) * f / st.y;
-      of_hot = p.scale * gp * f;
+      of_p = t >= p.vocab ? __int_as_float(0x7fffffff) : static_cast<float>((gl - gp) * f) / st.y;
+      of_hot = static_cast<float>(gp * f);
       if (t >= p.first && t < p.first + s.n) hot = static_cast<int>(t - p.first);
     }
     __device__ void chunk(const Params& p, const Shape& a, const Spot& s, int col0, unsigned acc, int) {

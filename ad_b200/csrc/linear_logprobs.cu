@@ -13,6 +13,11 @@
 // into dz in the epilogue, rounded to the operands' type and used twice: as rows for
 // dx, which is summed over the pieces in 32 bits, and across for the piece's rows of dW.
 //
+// Logits are what the tensor cores sum, which truncate as they add: where terms have one sign and
+// size, about 1.55e-8 of a logit is missing for each 16 of the width (lse of width 4096: 2.0e-6 of
+// it, norm-wise, over dense states); where the sums fit 24 bits, nothing.  It depends on the data and
+// is left as it is.  (Sums of 512 elements joined on the CUDA cores: 2.2e-7, for 1.5 times the time.)
+//
 // dz in f16 is held times a power of two that puts the largest gradient of a row
 // at 2^14: what it loses is below 2^-38 of that.
 //
@@ -253,15 +258,6 @@ struct Slope {
 
 // ------------------------------------------------------------------ host
 
-// The tensor cores truncate where they add to an accumulator.  What a logit loses so
-// is near LOSS of it for each addition (16 elements of the width) where it grows evenly, as
-// those do that are far ahead and make up lse: half a step of 2^-23 of what is there, with a
-// bit more kept than 24.  It is given back by the factor on logits: lse of width 4096 was
-// off by 2.0e-6, norm-wise, and is by 1.2e-7 (bf16; 3.2e-7 f16).  Sums of 512 elements
-// joined on the CUDA cores gave 2.2e-7, for 1.5 times the time.
-constexpr double LOSS = 1.55e-8;
-float regained(float scale, long long width) { return static_cast<float>(scale * (1.0 + LOSS * static_cast<double>((width + 15) / 16))); }
-
 constexpr long long PIECE = 1ll << 28;  // elements of dz at a time, about: half a gigabyte
 
 struct Layout {
@@ -379,13 +375,12 @@ extern "C" int ad_linear_logprobs(int device, int dtype, const void* x, int64_t 
   q.part = reinterpret_cast<float2*>(ws + l.part);
   q.target = reinterpret_cast<float*>(ws + l.target);
   q.tokens = tokens, q.tok64 = tok64;
-  const float factor = std::min(regained(scale, width), FLT_MAX);
-  q.k = std::min(factor * LOG2E, FLT_MAX);
+  q.k = std::min(scale * LOG2E, FLT_MAX);
   if (start<Sum>(who, d, p, dtype == AD_F16, l.tiling, q, st)) return 1;
   FinishArgs f = {};
   f.part = q.part, f.target = q.target, f.tokens = tokens, f.tok64 = tok64;
   f.parts = static_cast<int>(parts_of(l.tiling, vocab)), f.rows = static_cast<int>(rows);
-  f.vocab = vocab, f.scale = factor, f.k = q.k;
+  f.vocab = vocab, f.scale = scale, f.k = q.k;
   f.logp = logp, f.lse = lse, f.stats = reinterpret_cast<float2*>(stats);
   const cudaError_t e = launch_early<finish_kernel>(dim3(static_cast<unsigned>((rows + FINISH_ROWS - 1) / FINISH_ROWS)), 32 * FINISH_WARPS, 0, st, f);
   return e == cudaSuccess ? 0 : fail_cuda(who, e);
@@ -442,7 +437,7 @@ extern "C" int ad_linear_logprobs_grad(int device, int dtype, const void* x, int
     q.tokens = tokens, q.tok64 = tok64;
     q.g_logp = g_logp, q.g_lse = g_lse, q.factor = factor;
     q.vocab = vocab, q.first = v0;
-    q.k = std::min(std::min(regained(scale, width), FLT_MAX) * LOG2E, FLT_MAX), q.scale = scale;
+    q.k = std::min(scale * LOG2E, FLT_MAX), q.scale = scale;
     q.out = reinterpret_cast<unsigned short*>(ws + l.dz), q.ld = l.piece;
     if (start<Slope>(who, d, p, half, l.tiling, q, st)) return 1;
     const Problem products[2] = {{rows, width, n, n, false, true, {dz, {}}, {w, {}}},

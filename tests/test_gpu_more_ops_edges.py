@@ -90,3 +90,48 @@ def test_linear_logprobs_gradient_of_a_row_that_is_no_number(ops, bad):
     got = ops.linear_logprobs_grad(x, w, tokens, r.stats, gp, gl)
     rest = torch.arange(30) != 5
     assert torch.equal(got.x[rest], want.x[rest]) and not got.x[5].isfinite().any() and want.x[rest].count_nonzero() > 0
+
+
+@pytest.mark.parametrize("t", HALVES)
+@pytest.mark.parametrize("width", [64, 1024, 4096, 16384])
+@pytest.mark.parametrize("place", ["first", "last", "spread"])
+def test_linear_logprobs_of_exact_logits(ops, t, width, place):
+    """Logits of 16 terms, whole numbers that 24 bits hold in any order of addition: nothing is lost, whatever
+    the width is.  One is 16 and more ahead of the others, so the log of the sum is below 500 e^-16 < 2^-14 and off
+    by no more than 2^-22 (an exponential's error and a rounding of a sum that begins with 1); beside it,
+    lse and logp are rounded once."""
+    gen = seeded(width, len(t))
+    at = torch.tensor({"first": list(range(16)), "last": list(range(width - 16, width)),
+                       "spread": list(range(3, width, width // 16))}[place])
+    x, w = torch.zeros(40, width, dtype=torch.double), torch.randint(-4, 5, (500, width), generator=gen).double()
+    x[:, at] = torch.randint(1, 5, (40, 16), generator=gen).double()
+    x[:, at[0]], w[0], w[0, at[0]] = 4.0, 0.0, 64.0
+    x, w = x.to(dtype(t)).cuda(), w.to(dtype(t)).cuda()
+    z = x.double() @ w.double().T
+    top, second = z.topk(2, -1).values.T
+    assert (top == 256).all() and float(second.max()) <= 240
+    tokens = torch.randint(0, 500, (40,), generator=gen).cuda()
+    tokens[:20] = 0
+    r = ops.linear_logprobs(x, w, tokens)
+    lse = torch.logsumexp(z, -1)
+    close(r.lse, lse, 2.0 ** -22, "float32")
+    close(r.logp, z[torch.arange(40, device="cuda"), tokens] - lse, 2.0 ** -22, "float32")
+    assert (r.stats[:, 0] == 256).all()
+
+
+@pytest.mark.parametrize("t", HALVES)
+@pytest.mark.parametrize("width", [1000, 4096])
+def test_linear_logprobs_of_logits_that_grow_evenly(ops, t, width):
+    """Terms of one sign, all along the width: truncation adds up, and takes away only: what lse is above its
+    value comes from the exponents, their sum and the log, linear64's bound without that of logits."""
+    gen = seeded(width)
+    x = (0.5 + torch.rand(40, width, generator=gen)).to(dtype(t)).cuda()
+    w = ((0.5 + torch.rand(300, width, generator=gen)) * 40 / width).to(dtype(t)).cuda()
+    tokens = torch.randint(0, 300, (40,), generator=gen).cuda()
+    want = linear64(x, w, tokens, 1.0)
+    r = ops.linear_logprobs(x, w, tokens)
+    close(r.lse, want["lse"], want["elf"], "float32")
+    close(r.logp, want["logp"], want["elp"], "float32")
+    top = (x.double() @ w.double().T).amax(-1)
+    others = (math.log(300) + 4) * 4 + 300 / 64 + 64 + 4 * (want["lse"] + top)
+    assert ((r.lse.double() - want["lse"]) <= 1.05 * E * others).all()

@@ -82,18 +82,21 @@ __device__ __forceinline__ Two share(Two z, Two& slope) {
     return p;
   }
   if (ACT == GELU) {
-    // the normal distribution's sum by Abramowitz and Stegun 7.1.26: erfc(x) = (a1 t + ... + a5 t^5) exp(-x^2),
-    // t = 1 / (1 + 0.3275911 x), x = |z| / sqrt(2), within 1.5e-7 (with erfcf: 43 us instead of 40 for 4095 x 512 x
-    // 2048); half of it is what lies beyond |z|
+    // What the normal distribution has beyond |z| is exp(-z^2 / 2) R(|z|), and R, which falls from 1/2 like
+    // 1 / |z|, a polynomial in t = 1 / (1 + 0.3 |z|) without a constant, in the manner of Hastings: these
+    // coefficients have the least largest error relative to R (1.2e-7 up to |z| = 13.2, where the exponential
+    // leaves the normal numbers), fitted in 64 bits.  In 32 bits the whole is within (0.75 z^2 + 9) 2^-24 of
+    // itself on the negative side, where it is what z is multiplied by, and 4 2^-24 on the other.  (With
+    // erfcf 43 us instead of 40 for 4095 x 512 x 2048.)
     const Two e = exp2_2(mul2(mul2(z, z), -0.5f * LOG2E));
-    const Two t = reciprocal2(fma2(two(fabsf(v.x), fabsf(v.y)), 0.3275911f * 0.70710678f, 1.0f));
-    Two poly = fma2(t, 0.5f * 1.061405429f, 0.5f * -1.453152027f);
-    poly = fma2(poly, t, two(0.5f * 1.421413741f, 0.5f * 1.421413741f));
-    poly = fma2(poly, t, two(0.5f * -0.284496736f, 0.5f * -0.284496736f));
-    poly = fma2(poly, t, two(0.5f * 0.254829592f, 0.5f * 0.254829592f));
-    // 1/2 + sign(z) (1/2 - tail)
-    const float2 inner = apart(fma2(mul2(mul2(poly, t), e), -1.0f, 0.5f));
-    const Two p = fma2(two(copysignf(1.0f, v.x), copysignf(1.0f, v.y)), two(inner.x, inner.y), two(0.5f, 0.5f));
+    const Two t = reciprocal2(fma2(two(fabsf(v.x), fabsf(v.y)), 0.3f, 1.0f));
+    Two poly = fma2(t, 0.0360888243f, -0.158933669f);
+    constexpr float C[6] = {0.209346309f, -0.0564500354f, 0.130032599f, 0.0994650722f, 0.120826311f, 0.11962454f};
+#pragma unroll
+    for (int i = 0; i < 6; ++i) poly = fma2(poly, t, two(C[i], C[i]));
+    const Two tail = mul2(mul2(poly, t), e);
+    const float2 below = apart(tail), above = apart(fma2(tail, -1.0f, 1.0f));
+    const Two p = two(v.x < 0.0f ? below.x : above.x, v.y < 0.0f ? below.y : above.y);
     if (SLOPE) slope = fma2(mul2(z, DENSITY), e, p);
     return p;
   }

@@ -135,3 +135,48 @@ def test_linear_logprobs_of_logits_that_grow_evenly(ops, t, width):
     top = (x.double() @ w.double().T).amax(-1)
     others = (math.log(300) + 4) * 4 + 300 / 64 + 64 + 4 * (want["lse"] + top)
     assert ((r.lse.double() - want["lse"]) <= 1.05 * E * others).all()
+
+
+# ------------------------------------------------------------------ gated feed-forward blocks
+
+@pytest.mark.parametrize("t", HALVES)
+@pytest.mark.parametrize("act", ["silu", "gelu", "gelu_tanh"])
+@pytest.mark.parametrize("rows", [2, 40])
+def test_feed_forward_activations_relative_to_their_size(ops, t, act, rows):
+    """act(z) u and its gradients one element at a time, far out on the negative side too.  Products have one
+    term each and are exact, so what is left is the activation's share p of z in 32 bits, relative to
+    itself: an exponential whose argument, of size c, is off by 3 E c at most (its own roundings; gelu_tanh's
+    argument is a cubic, 3 E more), 2^-22 for it, and 16 E for the sum and quotient or the polynomial (its
+    fit: 2 E)."""
+    n = 512
+    z = torch.linspace(-9, 9, n).to(dtype(t))
+    x, wu, wd = torch.zeros(rows, n, dtype=dtype(t)), torch.zeros(n, n, dtype=dtype(t)), torch.eye(n, dtype=dtype(t))
+    wg = torch.zeros(n, n, dtype=dtype(t))
+    x[:, 0], wg[:, 0], wu[:, 0] = 1.0, z, 4096.0
+    x, wg, wu, wd = (v.cuda() for v in (x, wg, wu, wd))
+    z = z.double().cuda()
+    if act == "silu":
+        c, p, dp = z.abs(), torch.sigmoid(z), torch.sigmoid(z) * torch.sigmoid(-z)
+    elif act == "gelu":
+        c, p, dp = z * z / 2, torch.exp(torch.special.log_ndtr(z)), torch.exp(-z * z / 2) / math.sqrt(2 * math.pi)
+    else:
+        k = math.sqrt(8 / math.pi)
+        c = k * (z + 0.044715 * z ** 3)
+        p, dp = torch.sigmoid(c), torch.sigmoid(c) * torch.sigmoid(-c) * k * (1 + 3 * 0.044715 * z * z)
+        c = 2 * c.abs()
+    off = (3 * c + 20) * E
+    got = ops.feed_forward(x, wg, wu, wd, act=act, keep=True)
+    assert torch.equal(got.gate[0].double(), z) and (got.up[0] == 4096).all()
+    h = 4096 * z * p
+    close(got.y[0], h, off * h.abs(), t)
+    assert all(torch.equal(got.y[0], v) for v in got.y)
+    dy = torch.zeros_like(x)
+    dy[0] = 1.0
+    out = (torch.empty_like(x), *(torch.empty(n, n, device="cuda") for _ in range(3)))
+    g = ops.feed_forward_grad(dy, x, wg, wu, wd, got.gate, got.up, act=act, out=out)
+    close(g.w_up[:, 0], z * p, off * (z * p).abs() + U[t] * (z * p).abs(), t)
+    slope = 4096 * (p + z * dp)
+    close(g.w_gate[:, 0], slope, off * 4096 * (p + (z * dp).abs()) + U[t] * slope.abs(), t)
+    down = g.w_down.double()
+    assert torch.equal(down, down[:1].expand(n, n))
+    close(g.w_down[0], h, off * h.abs() + U[t] * h.abs(), t)

@@ -124,7 +124,7 @@ __device__ __forceinline__ Two activated(Two z) {
 // h of 32 columns from accumulators of both products.
 struct Gated {
   static constexpr bool DUAL = true;
-  static constexpr int WARPS = 16, SIDE = 4096;
+  static constexpr int WARPS = 16, SIDE = 4096, PART = 0;
   static constexpr double US[3] = {6.0, 4.5, 3.0};
   using Units = ByNumber;
   struct Params {
@@ -186,7 +186,7 @@ struct Gated {
 // dg, du and h from an accumulator of dh, eight columns of a row a lane.
 struct GatedGrad {
   static constexpr bool DUAL = false;
-  static constexpr int WARPS = 16, SIDE = 4096;
+  static constexpr int WARPS = 16, SIDE = 4096, PART = 0;
   static constexpr double US[3] = {11.0, 5.5, 3.2};
   using Units = ByNumber;
   struct Params {

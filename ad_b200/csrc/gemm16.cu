@@ -111,7 +111,7 @@ __device__ __forceinline__ void finish1(const Target& t, float alpha, long long 
 template <int N>
 struct Store {
   static constexpr bool DUAL = false;
-  static constexpr int WARPS = 8, SIDE = 4096;
+  static constexpr int WARPS = 8, SIDE = 4096, PART = 0;
   using Units = std::conditional_t<N == 0, ByNumber, ByList<N>>;
   struct Params {
     Targets to;

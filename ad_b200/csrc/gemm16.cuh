@@ -215,6 +215,24 @@ __device__ __forceinline__ void tmem_ld32(unsigned taddr, float (&v)[32]) {
   for (int j = 0; j < 32; ++j) v[j] = __uint_as_float(q[j]);
 }
 
+// 16 columns, added to sums that are there.
+__device__ __forceinline__ void tmem_add16(unsigned taddr, float* v) {
+  unsigned q[16];
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+      : "=r"(q[0]), "=r"(q[1]), "=r"(q[2]), "=r"(q[3]), "=r"(q[4]), "=r"(q[5]), "=r"(q[6]), "=r"(q[7]), "=r"(q[8]),
+        "=r"(q[9]), "=r"(q[10]), "=r"(q[11]), "=r"(q[12]), "=r"(q[13]), "=r"(q[14]), "=r"(q[15])
+      : "r"(taddr)
+      : "memory");
+  asm volatile("tcgen05.wait::ld.sync.aligned;"
+               : "+r"(q[0]), "+r"(q[1]), "+r"(q[2]), "+r"(q[3]), "+r"(q[4]), "+r"(q[5]), "+r"(q[6]), "+r"(q[7]),
+                 "+r"(q[8]), "+r"(q[9]), "+r"(q[10]), "+r"(q[11]), "+r"(q[12]), "+r"(q[13]), "+r"(q[14]), "+r"(q[15])
+               :
+               : "memory");
+#pragma unroll
+  for (int j = 0; j < 16; ++j) v[j] += __uint_as_float(q[j]);
+}
+
 __device__ __forceinline__ unsigned lds32(unsigned addr) {
   unsigned v;
   asm volatile("ld.shared.u32 %0, [%1];" : "=r"(v) : "r"(addr) : "memory");
@@ -268,6 +286,17 @@ __device__ __forceinline__ void accumulator_read(const Spot& s) {
 // 32 columns of the warp's rows; the accumulator is given back with the last ones.
 __device__ __forceinline__ void take32(const Spot& s, unsigned acc, float (&v)[32]) {
   tmem_ld32(acc, v);
+  if (s.last) accumulator_read(s);
+  if (s.dead) {
+#pragma unroll
+    for (int j = 0; j < 32; ++j) v[j] = __int_as_float(0x7fffffff);
+  }
+}
+
+// The same, added to v.
+__device__ __forceinline__ void add32(const Spot& s, unsigned acc, float (&v)[32]) {
+  tmem_add16(acc, v);
+  tmem_add16(acc + 16, v + 16);
   if (s.last) accumulator_read(s);
   if (s.dead) {
 #pragma unroll
@@ -388,6 +417,13 @@ __host__ __device__ __forceinline__ int rows_of_box(int m) {
 
 // ------------------------------------------------------------------ the kernel
 
+// Parts of a unit's K, and where one of them begins.
+template <typename EPI>
+__device__ __forceinline__ int parts_of_k(const Unit& t) {
+  return EPI::PART ? max(1, (t.kb1 - t.kb0 + EPI::PART / 2) / EPI::PART) : 1;
+}
+__device__ __forceinline__ int part_begin(const Unit& t, int part, int parts) { return (t.kb1 - t.kb0) * part / parts; }
+
 // A place among the stages, the phase of its barriers, and whether it has been used before.
 template <int STAGES>
 struct Ring {
@@ -400,7 +436,10 @@ struct Ring {
 
 // EPI: DUAL (B's tiles hold half their columns of each of two operands), WARPS,
 // SIDE; US (tiling_for); Params; Units; a State that is constructed for a tile (loads that need no
-// accumulator), whose chunk() takes 32 columns, and whose end() all warps call.
+// accumulator), whose chunk() takes 32 columns, and whose end() all warps call.  PART: 0, or about
+// how many stages of K one accumulator sums; a tile's K is then taken in parts of the same length,
+// by turns in both accumulators, and the State's hold() keeps the sums of all but the last, 32 columns for
+// each of the warp's chunks.
 template <typename TILE, typename EPI>
 __global__ void __launch_bounds__(TILE::THREADS, 1)
     gemm_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Shape a,
@@ -534,23 +573,23 @@ __global__ void __launch_bounds__(TILE::THREADS, 1)
     if (lane == 0 && rank == 0) {  // products
       Ring<TILE::STAGES> ring;
       int c = 0;  // accumulators used so far
-      for (int u = first; u < end; u += step, ++c) {
+      for (int u = first; u < end; u += step) {
         const Unit t = EPI::Units::unit(params, a, u);
-        if (c >= 2 && !bar_wait(&acc_empty[c & 1], (c / 2 - 1) & 1, gave_up)) {
-          *gave_up = 1;
-          break;
-        }
-        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-        const unsigned acc = tmem + (c & 1) * BN;
         const Group& g = a.group[t.group];
+        const int parts = parts_of_k<EPI>(t);
+        int part = 0;
         auto tile = [&](auto a_turned, auto b_turned) {
           constexpr bool AT = decltype(a_turned)::value, BT = decltype(b_turned)::value;
           // D in 32 bits; operand types (bf16: 1) in bits 7 and 10; across K: bits 15 and 16
           const unsigned idesc = (1u << 4) | (a.half ? 0u : (1u << 7) | (1u << 10)) | (AT ? 1u << 15 : 0u) |
                                  (BT ? 1u << 16 : 0u) | (static_cast<unsigned>(BN >> 3) << 17) |
                                  (static_cast<unsigned>(TILE::M >> 4) << 24);
+          if (c >= 2 && !bar_wait(&acc_empty[c & 1], (c / 2 - 1) & 1, gave_up)) return false;
+          asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+          const unsigned acc = tmem + (c & 1) * BN;
           unsigned more = 0;
-          for (int left = t.kb1 - t.kb0; left > 0; --left, ring.next()) {
+          const int stages = EPI::PART ? part_begin(t, part + 1, parts) - part_begin(t, part, parts) : t.kb1 - t.kb0;
+          for (int left = stages; left > 0; --left, ring.next()) {
             if (!bar_wait(&full[ring.i], ring.phase, gave_up)) return false;
             asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
             const unsigned st = smem_u32(smem) + ring.i * TILE::STAGE;
@@ -567,7 +606,9 @@ __global__ void __launch_bounds__(TILE::THREADS, 1)
         };
         const std::true_type yes;
         const std::false_type no;
-        const bool fine = g.a_turned ? (g.b_turned ? tile(yes, yes) : tile(yes, no)) : g.b_turned ? tile(no, yes) : tile(no, no);
+        bool fine = true;
+        for (; part < parts && fine; ++part, ++c)
+          fine = g.a_turned ? (g.b_turned ? tile(yes, yes) : tile(yes, no)) : g.b_turned ? tile(no, yes) : tile(no, no);
         if (!fine) {
           *gave_up = 1;
           break;
@@ -580,7 +621,7 @@ __global__ void __launch_bounds__(TILE::THREADS, 1)
     s.lane = lane, s.quad = quad, s.part = part;
     s.side = smem_u32(side) + (warp - 2) * EPI::SIDE;
     s.rank = rank, s.width = COLS, s.stride = PARTS * CHUNK;
-    s.dead = false;
+    s.dead = false, s.odd = 1;
     int c = 0;
     for (int u = first; u < end; u += step, ++c) {
       const Unit t = EPI::Units::unit(params, a, u);
@@ -588,23 +629,44 @@ __global__ void __launch_bounds__(TILE::THREADS, 1)
       s.unit = t, s.m = a.group[t.group].m, s.n = a.group[t.group].n;
       const int chunks = (min(COLS, s.n - t.col * COLS) + CHUNK - 1) / CHUNK;
       typename EPI::State e(params, a, s);
-      if (!s.dead && !bar_wait(&acc_full[c & 1], (c / 2) & 1, gave_up)) {
-        s.dead = true;
-        *gave_up = 1;
-      }
-      asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-      const unsigned acc = tmem + (static_cast<unsigned>(quad * 32) << 16) + (c & 1) * BN;
-      s.free_bar = CTAS == 1 ? smem_u32(&acc_empty[c & 1]) : in_block(smem_u32(&acc_empty[c & 1]), 0);
       // a warp without a row of the result, or a chunk of it, still has to say that it is done
-      if (s.row0 < s.m && part < chunks) {
-        for (int ch = part; ch < chunks; ch += PARTS) {
-          s.last = ch + PARTS >= chunks;
-          e.chunk(params, a, s, t.col * COLS + ch * CHUNK, acc + ch * CHUNK, COLS);
+      const bool some = s.row0 < s.m && part < chunks;
+      unsigned acc;
+      auto filled = [&] {  // the accumulator that comes next
+        if (!s.dead && !bar_wait(&acc_full[c & 1], (c / 2) & 1, gave_up)) {
+          s.dead = true;
+          *gave_up = 1;
         }
+        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+        acc = tmem + (static_cast<unsigned>(quad * 32) << 16) + (c & 1) * BN;
+        s.free_bar = CTAS == 1 ? smem_u32(&acc_empty[c & 1]) : in_block(smem_u32(&acc_empty[c & 1]), 0);
+        if (!some) accumulator_read(s);
+      };
+      if constexpr (EPI::PART != 0) {
+        constexpr int MINE = (COLS / CHUNK + PARTS - 1) / PARTS;  // chunks of a warp, at most: sums that are held stay in registers
+        for (int left = parts_of_k<EPI>(t); left > 0; --left, ++c) {
+          filled();
+#pragma unroll
+          for (int i = 0; i < MINE; ++i) {
+            const int ch = part + i * PARTS;
+            if (!some || ch >= chunks) continue;
+            s.last = ch + PARTS >= chunks;
+            if (left > 1)
+              e.hold(s, acc + ch * CHUNK, i);
+            else
+              e.chunk(params, a, s, t.col * COLS + ch * CHUNK, acc + ch * CHUNK, i);
+          }
+        }
+        --c;
       } else {
-        accumulator_read(s);
+        filled();
+        if (some)
+          for (int ch = part; ch < chunks; ch += PARTS) {
+            s.last = ch + PARTS >= chunks;
+            e.chunk(params, a, s, t.col * COLS + ch * CHUNK, acc + ch * CHUNK, COLS);
+          }
       }
-      s.odd = c & 1;
+      s.odd ^= 1;
       e.end(params, a, s);
     }
   }

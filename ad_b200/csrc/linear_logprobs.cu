@@ -14,9 +14,8 @@
 // dx, which is summed over the pieces in 32 bits, and across for the piece's rows of dW.
 //
 // Logits are what the tensor cores sum, which truncate as they add: where terms have one sign and
-// size, about 1.55e-8 of a logit is missing for each 16 of the width (lse of width 4096: 2.0e-6 of
-// it, norm-wise, over dense states); where the sums fit 24 bits, nothing.  It depends on the data and
-// is left as it is.  (Sums of 512 elements joined on the CUDA cores: 2.2e-7, for 1.5 times the time.)
+// size, 1.55e-8 of a sum for each 16 elements that went into it, where the sums fit 24 bits nothing.  It depends
+// on the data, so it is not given back, but kept small: widths are summed in parts (WHOLE).
 //
 // dz in f16 is held times a power of two that puts the largest gradient of a row
 // at 2^14: what it loses is below 2^-38 of that.
@@ -41,20 +40,56 @@ __device__ __forceinline__ long long token_at(const void* tokens, int tok64, lon
   return tok64 ? static_cast<const long long*>(tokens)[i] : static_cast<const int*>(tokens)[i];
 }
 
+// Logits of a width above WHOLE are summed in parts of about LENGTH (FOLD), joined in registers and
+// rounded to nearest there: what the tensor cores truncate grows with the sum that they add to (lse of width
+// 4096 over dense states: 1.9e-6 of it in one accumulator, 4.4e-7 in four parts; of 1024 4.6e-7).  The same
+// parts forward and backward, or a probability near 1 would be off by the difference.  A part's
+// products take longer than an epilogue, which so stays hidden, and what the joins cost is 3 to 8%: 2047 x 1600 over
+// 50001 tokens takes 274 us forward instead of 254 and 840 backward instead of 793, 2000 x 4096 over 32000
+// 455 and 1345 instead of 433 and 1318.  (Below 1536 parts would be shorter than an epilogue: of 550, 323 us instead
+// of 295.)
+constexpr int LENGTH = 1024, WHOLE = 1536;
+template <bool FOLD, int WARPS>
+struct Held {
+  float held[256 / CHUNK / (WARPS / 4)][CHUNK];  // of each of the warp's chunks
+  __device__ Held() {
+#pragma unroll
+    for (auto& h : held)
+#pragma unroll
+      for (float& x : h) x = 0.0f;
+  }
+  __device__ __forceinline__ void hold(const Spot& s, unsigned acc, int i) { add32(s, acc, held[i]); }
+  // the whole sums of the warp's chunk i
+  __device__ __forceinline__ float (&take(const Spot& s, unsigned acc, int i))[32] {
+    add32(s, acc, held[i]);
+    return held[i];
+  }
+};
+template <int WARPS>
+struct Held<false, WARPS> {
+  float sums[CHUNK];
+  __device__ __forceinline__ float (&take(const Spot& s, unsigned acc, int))[32] {
+    take32(s, acc, sums);
+    return sums;
+  }
+};
+
+struct SumParams {
+  float2* part;   // [column tiles][rows]
+  float* target;  // [rows]
+  const void* tokens;
+  int tok64;
+  float k;  // scale log2(e)
+};
 // A row's largest logit and the sum of exponents from there, over a tile's columns.
+template <bool FOLD>
 struct Sum {
   static constexpr bool DUAL = false;
-  static constexpr int WARPS = 8, SIDE = 512;
+  static constexpr int WARPS = 8, SIDE = 512, PART = FOLD ? LENGTH / BK : 0;
   static constexpr double US[3] = {4.0, 2.2, 1.5};
   using Units = ByNumber;
-  struct Params {
-    float2* part;   // [column tiles][rows]
-    float* target;  // [rows]
-    const void* tokens;
-    int tok64;
-    float k;  // scale log2(e)
-  };
-  struct State {
+  using Params = SumParams;
+  struct State : Held<FOLD, WARPS> {
     float top, sum;
     int token;  // -1: not in reach
     __device__ State(const Params& p, const Shape&, const Spot& s) {
@@ -65,9 +100,8 @@ struct Sum {
         if (t >= 0 && t < s.n) token = static_cast<int>(t);
       }
     }
-    __device__ void chunk(const Params& p, const Shape&, const Spot& s, int col0, unsigned acc, int) {
-      float v[32];
-      take32(s, acc, v);
+    __device__ void chunk(const Params& p, const Shape&, const Spot& s, int col0, unsigned acc, int i) {
+      float(&v)[32] = this->take(s, acc, i);
       if (col0 + CHUNK > s.n) {
 #pragma unroll
         for (int j = 0; j < 32; ++j)
@@ -197,24 +231,26 @@ __global__ void __launch_bounds__(1024) range_kernel(const __grid_constant__ Ran
   }
 }
 
+struct SlopeParams {
+  const float2* stats;
+  const void* tokens;
+  int tok64;
+  const float *g_logp, *g_lse;
+  const float* factor;
+  long long vocab, first;  // of all; the piece's first column
+  float k, scale;
+  unsigned short* out;
+  long long ld;
+};
 // dz of a piece of the vocabulary.
+template <bool FOLD>
 struct Slope {
   static constexpr bool DUAL = false;
-  static constexpr int WARPS = 16, SIDE = 2048;
+  static constexpr int WARPS = 16, SIDE = 2048, PART = FOLD ? LENGTH / BK : 0;
   static constexpr double US[3] = {4.5, 2.5, 1.7};
   using Units = ByNumber;
-  struct Params {
-    const float2* stats;
-    const void* tokens;
-    int tok64;
-    const float *g_logp, *g_lse;
-    const float* factor;
-    long long vocab, first;  // of all; the piece's first column
-    float k, scale;
-    unsigned short* out;
-    long long ld;
-  };
-  struct State {
+  using Params = SlopeParams;
+  struct State : Held<FOLD, WARPS> {
     float top, of_p, of_hot;
     int hot;  // the token's column in the piece
     __device__ State(const Params& p, const Shape&, const Spot& s) {
@@ -231,9 +267,8 @@ struct Slope {
       of_hot = static_cast<float>(gp * f);
       if (t >= p.first && t < p.first + s.n) hot = static_cast<int>(t - p.first);
     }
-    __device__ void chunk(const Params& p, const Shape& a, const Spot& s, int col0, unsigned acc, int) {
-      float v[32];
-      take32(s, acc, v);
+    __device__ void chunk(const Params& p, const Shape& a, const Spot& s, int col0, unsigned acc, int i) {
+      float(&v)[32] = this->take(s, acc, i);
 #pragma unroll
       for (int j = 0; j < 32; ++j) v[j] = ex2((v[j] - top) * p.k) * of_p;
       const unsigned at = static_cast<unsigned>(hot - col0);
@@ -285,7 +320,7 @@ Layout plan(const Device& d, const void* x, long long ldx, const void* w, long l
   if (l.pack_w) l.w = take(2ull * vocab * l.ld_packed);
   const long long kblocks = (width + BK - 1) / BK;
   if (!grad) {
-    l.tiling = tiling_for<Sum>(rows, vocab, kblocks, d.sms);
+    l.tiling = tiling_for<Sum<false>>(rows, vocab, kblocks, d.sms);
     l.part = take(sizeof(float2) * parts_of(l.tiling, vocab) * rows);
     l.target = take(sizeof(float) * rows);
   } else {
@@ -294,7 +329,7 @@ Layout plan(const Device& d, const void* x, long long ldx, const void* w, long l
     l.pieces = std::max(1ll, std::min(l.pieces, (vocab + 1023) / 1024));
     l.piece = std::min(round_up((vocab + l.pieces - 1) / l.pieces, 256), round_up(vocab, 8));
     l.pieces = (vocab + l.piece - 1) / l.piece;
-    l.tiling = tiling_for<Slope>(rows, std::min(l.piece, vocab), kblocks, d.sms);
+    l.tiling = tiling_for<Slope<false>>(rows, std::min(l.piece, vocab), kblocks, d.sms);
     l.factor = take(2 * sizeof(float));
     l.dz = take(2ull * rows * l.piece);
     if (l.pieces > 1) l.sum = take(sizeof(float) * rows * round_up(width, 4));
@@ -371,12 +406,13 @@ extern "C" int ad_linear_logprobs(int device, int dtype, const void* x, int64_t 
   p.a[0] = l.pack_x ? Mat{ws + l.x, l.ld_packed} : Mat{x, ldx};
   p.b[0] = l.pack_w ? Mat{ws + l.w, l.ld_packed} : Mat{weight, ldw};
   if (pack(who, d, l, x, ldx, weight, ldw, rows, width, vocab, ws, st)) return 1;
-  Sum::Params q = {};
+  SumParams q = {};
   q.part = reinterpret_cast<float2*>(ws + l.part);
   q.target = reinterpret_cast<float*>(ws + l.target);
   q.tokens = tokens, q.tok64 = tok64;
   q.k = std::min(scale * LOG2E, FLT_MAX);
-  if (start<Sum>(who, d, p, dtype == AD_F16, l.tiling, q, st)) return 1;
+  const int half = dtype == AD_F16;
+  if (width > WHOLE ? start<Sum<true>>(who, d, p, half, l.tiling, q, st) : start<Sum<false>>(who, d, p, half, l.tiling, q, st)) return 1;
   FinishArgs f = {};
   f.part = q.part, f.target = q.target, f.tokens = tokens, f.tok64 = tok64;
   f.parts = static_cast<int>(parts_of(l.tiling, vocab)), f.rows = static_cast<int>(rows);
@@ -432,14 +468,14 @@ extern "C" int ad_linear_logprobs_grad(int device, int dtype, const void* x, int
     const long long v0 = i * l.piece, n = std::min(l.piece, vocab - v0);
     const Mat w = {static_cast<const unsigned short*>(mw.p) + v0 * mw.ld, mw.ld};
     Problem p = {rows, n, width, width, false, false, {mx, {}}, {w, {}}};
-    Slope::Params q = {};
+    SlopeParams q = {};
     q.stats = reinterpret_cast<const float2*>(stats);
     q.tokens = tokens, q.tok64 = tok64;
     q.g_logp = g_logp, q.g_lse = g_lse, q.factor = factor;
     q.vocab = vocab, q.first = v0;
     q.k = std::min(scale * LOG2E, FLT_MAX), q.scale = scale;
     q.out = reinterpret_cast<unsigned short*>(ws + l.dz), q.ld = l.piece;
-    if (start<Slope>(who, d, p, half, l.tiling, q, st)) return 1;
+    if (width > WHOLE ? start<Slope<true>>(who, d, p, half, l.tiling, q, st) : start<Slope<false>>(who, d, p, half, l.tiling, q, st)) return 1;
     const Problem products[2] = {{rows, width, n, n, false, true, {dz, {}}, {w, {}}},
                                  {n, width, rows, rows, true, true, {dz, {}}, {mx, {}}}};
     // dx: sums over the pieces stay in 32 bits until the last one's

@@ -854,8 +854,8 @@ def linear_logprobs(x, weight, tokens, *, scale: float = 1.0, out=None, workspac
     for a negative one, NaN for one past the vocabulary) under softmax(scale * x weight^T), and the log of the
     sum of exp(scale * logits), without keeping the logits: what ``token_logprobs`` gives for ``x @ weight.T``
     ([vocab, width]), without the memory for them.  Operands are bfloat16 or float16, products are accumulated
-    in 32 bits by the tensor cores, which truncate as they add: up to about 2^-26 of a logit's terms for each 16 of the
-    width, on average where they have one sign, and nothing where 24 bits hold the sums.
+    in 32 bits by the tensor cores, which truncate as they add, in parts of 1536 of the width at most: up to 1.5e-6 of a logit
+    whose terms all have one sign, less of others, and nothing where 24 bits hold the sums.
     ``out``: a ``LinearLogprobs`` to write; ``workspace``: adjacent elements at a 256-byte boundary,
     ``linear_logprobs_workspace`` bytes or more."""
     dev, dt, rows, width, vocab, ldx, ldw, t64 = _linear_operands(x, weight, tokens, scale)

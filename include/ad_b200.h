@@ -265,8 +265,8 @@ int ad_orthogonalize(int device, int dtype, const void* g, int64_t count, int64_
 /* Log probabilities of given tokens under softmax(scale x W^T), x of rows x
  * width, W of vocab x width, without the logits in memory.  dtype is AD_BF16 or
  * AD_F16; products are accumulated in 32 bits by the tensor cores, which truncate as
- * they add (about 2^-26 of a logit whose terms have one sign for each 16 elements of
- * the width; nothing where 24 bits hold the sums).  logp: 0 for a negative token, NaN
+ * they add, in parts of 1536 of the width at most (up to 1.5e-6 of a logit whose terms all
+ * have one sign, nothing where 24 bits hold the sums).  logp: 0 for a negative token, NaN
  * for one past the vocabulary.  lse: the log of the sum of exp(scale logits).
  * stats: rows * 2 floats (8-byte aligned) for the gradient: the largest logit
  * and the sum of exp(scale (logit - largest)).  Tokens are of 64 bits when tok64,

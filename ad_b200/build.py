@@ -19,7 +19,8 @@ SOURCES = [os.path.join(PKG, "csrc", f) for f in (
     "block_norm_f16.cu", "token_logprobs.cu", "orthogonalize.cu", "gemm16.cu", "linear_logprobs.cu",
     "feed_forward.cu", "embed.cu", "clip_norm.cu")]
 HEADERS = [os.path.join(ROOT, "include", "ad_b200.h"), os.path.join(PKG, "csrc", "ops_common.cuh"),
-           os.path.join(PKG, "csrc", "block_norm.cuh"), os.path.join(PKG, "csrc", "gemm16.cuh")]
+           os.path.join(PKG, "csrc", "block_norm.cuh"), os.path.join(PKG, "csrc", "gemm16.cuh"),
+           os.path.join(PKG, "csrc", "schedule.h")]
 NVCC = os.environ.get("NVCC", "/usr/local/cuda/bin/nvcc")
 
 

@@ -33,6 +33,7 @@
 #include <algorithm>
 
 #include "ops_common.cuh"
+#include "schedule.h"
 
 namespace ad_b200_internal {
 // runtime.cu: TMA descriptor of a row-major matrix of 16-bit elements, swizzled
@@ -45,10 +46,9 @@ namespace adgemm {
 
 using namespace adops;
 
-constexpr int BK = 64;            // elements of K a stage: 128 bytes, the swizzle's width
 constexpr int BOX = 64 * BK * 2;  // bytes of a box of 64 x 64
 constexpr int CHUNK = 32;         // columns that an epilogue takes at a time
-constexpr int MAX_GROUPS = 4, MAX_MAPS = 6;
+constexpr int MAX_MAPS = 6;
 
 // Tiles: CTAS blocks work on one of 128 CTAS rows and BN columns.  An epilogue has
 // WARPS warps, and SIDE bytes of shared memory for each of them.
@@ -714,17 +714,6 @@ struct Problem {
 struct Device {
   int device, sms;
 };
-
-// The three tilings: rows and columns, blocks, and measured us for 64 elements of K
-// (with the clocks that large products leave; 2047 x 50001 over 1024 took 152, 250
-// and 453 us).
-struct Tiling {
-  int m, n, ctas;
-  double us;
-};
-constexpr Tiling TILINGS[3] = {{256, 256, 2, 0.38}, {128, 128, 1, 0.36}, {128, 64, 1, 0.33}};
-
-inline int kblocks_of(const Problem& p) { return static_cast<int>((p.k0 + BK - 1) / BK + (p.k - p.k0 + BK - 1) / BK); }
 
 // The tiling for whole tiles: the one whose rounds take least, a round being a
 // tile's products or its epilogue (EPI::US, measured for each tiling), whichever is

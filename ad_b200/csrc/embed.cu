@@ -38,10 +38,6 @@ struct EmbedArgs {
   long long ldy;
 };
 
-__device__ __forceinline__ long long token_at(const void* tokens, int tok64, long long i) {
-  return tok64 ? static_cast<const long long*>(tokens)[i] : static_cast<const int*>(tokens)[i];
-}
-
 template <typename T, int V>
 __global__ void __launch_bounds__(256) embed_kernel(const __grid_constant__ EmbedArgs a) {
   after_previous();

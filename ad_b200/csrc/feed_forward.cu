@@ -497,7 +497,7 @@ Layout plan(const Device& d, const Operand* ops, int count, long long rows, long
     l.du = take(2ull * rows * l.ld);
   }
   const long long kblocks = (width + BK - 1) / BK;
-  l.tiling = count == 4 ? tiling_for<Gated>(rows, hidden, kblocks, d.sms) : tiling_for<GatedGrad>(rows, hidden, kblocks, d.sms);
+  l.tiling = count == 4 ? tiling_for<Gated, true>(rows, hidden, kblocks, d.sms) : tiling_for<GatedGrad>(rows, hidden, kblocks, d.sms);
   l.partial = take(partial_bytes(d));
   l.total = at;
   return l;

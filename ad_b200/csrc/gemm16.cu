@@ -371,7 +371,7 @@ int store_products(const char* who, const Device& d, int half, const Problem* p,
     }
     Store<0>::Params params = {};
     params.to = to;
-    return start<Store<0>>(who, d, p[0], half, 0, params, st);
+    return start_tile<Tile<2, 256, Store<0>>, Store<0>>(who, d, p[0], half, params, st);
   }
   const Schedule& b = *best;
   return b.tiling == 0   ? start_schedule<2, 256>(who, d, half, p, to, count, b, st)

@@ -264,7 +264,7 @@ __device__ __forceinline__ float2 unpack2(unsigned w, int half) {
 // What a warp's epilogue knows of its tile: 32 rows from row0 on, of which the
 // thread's accumulator row is row0 + lane, and where it may keep 4 KB.
 struct Spot {
-  int lane, quad, part, row0, rank;
+  int lane, quad, part, row0;
   Unit unit;
   int m, n;       // of the result
   int width, stride;  // of a tile; columns from a chunk of the warp's to its next
@@ -620,7 +620,7 @@ __global__ void __launch_bounds__(TILE::THREADS, 1)
     Spot s;
     s.lane = lane, s.quad = quad, s.part = part;
     s.side = smem_u32(side) + (warp - 2) * EPI::SIDE;
-    s.rank = rank, s.width = COLS, s.stride = PARTS * CHUNK;
+    s.width = COLS, s.stride = PARTS * CHUNK;
     s.dead = false, s.odd = 1;
     int c = 0;
     for (int u = first; u < end; u += step, ++c) {
@@ -719,13 +719,13 @@ struct Device {
 // tile's products or its epilogue (EPI::US, measured for each tiling), whichever is
 // longer.  A large tile's epilogue bounds short K's: dh of 600 x 2048 over 512 took 19 us on
 // large tiles, 13 on middle ones and 15 on small ones; of 4095 x 2048 35, 35 and 40.
-template <typename EPI>
+template <typename EPI, bool DUAL = false>
 int tiling_for(long long m, long long n, long long kblocks, int sms) {
   int best = 0;
   double least = 1e30;
   for (int i = 0; i < 3; ++i) {
     const Tiling& t = TILINGS[i];
-    const int cols = EPI::DUAL ? t.n / 2 : t.n, workers = sms / t.ctas;
+    const int cols = DUAL ? t.n / 2 : t.n, workers = sms / t.ctas;
     const long long count = ((m + t.m - 1) / t.m) * ((n + cols - 1) / cols);
     const double products = kblocks * t.us, epilogue = EPI::US[i];
     const double us = static_cast<double>((count + workers - 1) / workers) * std::max(products, epilogue) +

@@ -36,9 +36,6 @@ __device__ __forceinline__ float ex2(float x) {
   asm("ex2.approx.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
-__device__ __forceinline__ long long token_at(const void* tokens, int tok64, long long i) {
-  return tok64 ? static_cast<const long long*>(tokens)[i] : static_cast<const int*>(tokens)[i];
-}
 
 // Logits of a width above WHOLE are summed in parts of about LENGTH (FOLD), joined in registers and
 // rounded to nearest there: what the tensor cores truncate grows with the sum that they add to (lse of width
@@ -81,12 +78,15 @@ struct SumParams {
   int tok64;
   float k;  // scale log2(e)
 };
+// us of a tile's epilogue (tiling_for).
+struct SumCosts {
+  static constexpr double US[3] = {4.0, 2.2, 1.5};
+};
 // A row's largest logit and the sum of exponents from there, over a tile's columns.
 template <bool FOLD>
-struct Sum {
+struct Sum : SumCosts {
   static constexpr bool DUAL = false;
   static constexpr int WARPS = 8, SIDE = 512, PART = FOLD ? LENGTH / BK : 0;
-  static constexpr double US[3] = {4.0, 2.2, 1.5};
   using Units = ByNumber;
   using Params = SumParams;
   struct State : Held<FOLD, WARPS> {
@@ -242,12 +242,14 @@ struct SlopeParams {
   unsigned short* out;
   long long ld;
 };
+struct SlopeCosts {
+  static constexpr double US[3] = {4.5, 2.5, 1.7};
+};
 // dz of a piece of the vocabulary.
 template <bool FOLD>
-struct Slope {
+struct Slope : SlopeCosts {
   static constexpr bool DUAL = false;
   static constexpr int WARPS = 16, SIDE = 2048, PART = FOLD ? LENGTH / BK : 0;
-  static constexpr double US[3] = {4.5, 2.5, 1.7};
   using Units = ByNumber;
   using Params = SlopeParams;
   struct State : Held<FOLD, WARPS> {
@@ -320,7 +322,7 @@ Layout plan(const Device& d, const void* x, long long ldx, const void* w, long l
   if (l.pack_w) l.w = take(2ull * vocab * l.ld_packed);
   const long long kblocks = (width + BK - 1) / BK;
   if (!grad) {
-    l.tiling = tiling_for<Sum<false>>(rows, vocab, kblocks, d.sms);
+    l.tiling = tiling_for<SumCosts>(rows, vocab, kblocks, d.sms);
     l.part = take(sizeof(float2) * parts_of(l.tiling, vocab) * rows);
     l.target = take(sizeof(float) * rows);
   } else {
@@ -329,7 +331,7 @@ Layout plan(const Device& d, const void* x, long long ldx, const void* w, long l
     l.pieces = std::max(1ll, std::min(l.pieces, (vocab + 1023) / 1024));
     l.piece = std::min(round_up((vocab + l.pieces - 1) / l.pieces, 256), round_up(vocab, 8));
     l.pieces = (vocab + l.piece - 1) / l.piece;
-    l.tiling = tiling_for<Slope<false>>(rows, std::min(l.piece, vocab), kblocks, d.sms);
+    l.tiling = tiling_for<SlopeCosts>(rows, std::min(l.piece, vocab), kblocks, d.sms);
     l.factor = take(2 * sizeof(float));
     l.dz = take(2ull * rows * l.piece);
     if (l.pieces > 1) l.sum = take(sizeof(float) * rows * round_up(width, 4));

@@ -191,6 +191,11 @@ inline bool overlap(std::initializer_list<Place> all) {
   return false;
 }
 
+// A token of 64 bits, or of 32.
+__device__ __forceinline__ long long token_at(const void* tokens, int tok64, long long i) {
+  return tok64 ? static_cast<const long long*>(tokens)[i] : static_cast<const int*>(tokens)[i];
+}
+
 // ---------------------------------------------------------------- elements
 __device__ __forceinline__ float to_float(float x) { return x; }
 __device__ __forceinline__ float to_float(__nv_bfloat16 x) { return __bfloat162float(x); }

@@ -180,3 +180,39 @@ def test_feed_forward_activations_relative_to_their_size(ops, t, act, rows):
     down = g.w_down.double()
     assert torch.equal(down, down[:1].expand(n, n))
     close(g.w_down[0], h, off * h.abs() + U[t] * h.abs(), t)
+
+
+# ------------------------------------------------------------------ graphs
+
+@pytest.mark.parametrize("which", range(3))
+def test_first_call_of_clipping_can_be_captured(which):
+    """In a process of its own, with nothing run before: few arrays in place and into others, and many."""
+    import os
+    import subprocess
+    import sys
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    code = """
+import torch
+from ad_b200 import ops
+torch.manual_seed(0)
+grads = [torch.randn(70, 11, device="cuda"), torch.randn(999, device="cuda").bfloat16()]
+if %d == 2:
+    grads = [torch.randn(33, device="cuda") for _ in range(100)]
+out = grads if %d == 0 else [torch.empty_like(g) for g in grads]
+kept = [g.clone() for g in grads]
+want = torch.cat([g.double().reshape(-1) for g in grads]).norm()
+torch.cuda.synchronize()
+g = torch.cuda.CUDAGraph()
+with torch.cuda.graph(g):
+    norm = ops.clip_norm(grads, 0.5, out=out)
+for _ in range(2):
+    for a, b in zip(grads, kept):
+        a.copy_(b)
+    g.replay()
+    assert abs(float(norm) / float(want) - 1) < 1e-6
+    for a, b in zip(out, kept):
+        s = (b.double() * (0.5 / want)).to(b.dtype)
+        assert torch.allclose(a, s, rtol=2 * torch.finfo(b.dtype).eps, atol=0)
+""" % (which, which)
+    r = subprocess.run([sys.executable, "-c", code], cwd=root, env={**os.environ, "PYTHONPATH": root}, capture_output=True, text=True, timeout=120)
+    assert r.returncode == 0, r.stderr[-2000:]

@@ -1031,7 +1031,10 @@ def feed_forward(x, w_gate, w_up, w_down, *, act: str = "silu", keep: bool = Fal
 def feed_forward_grad(dy, x, w_gate, w_up, w_down, gate, up, *, act: str = "silu", accumulate: bool = False, out=None,
                       workspace=None, stream=None) -> FeedForwardGrads:
     """The gradients of ``feed_forward``'s operands from that of ``y``, its operands and the ``gate`` and
-    ``up`` that it kept.  What enters a product is rounded to the operands' type, sums are held in 32 bits.  ``out``: a ``FeedForwardGrads`` to write, the weights' all of the operands' type or all float32, to
+    ``up`` that it kept.  What enters a product is rounded to the operands' type, sums are held in 32 bits.  In
+    float16 the gradients of both products before the activation have the range that ``dy`` has (bits are lost
+    below 6e-5, nothing is left below 3e-8), in float32 weights' gradients too: a loss is scaled for it.  ``out``: a
+    ``FeedForwardGrads`` to write, the weights' all of the operands' type or all float32, to
     which the gradients are added with ``accumulate``; ``workspace``: as for ``feed_forward``, with ``dy``."""
     dev, dt, rows, width, hidden, ldx, ldwg, ldwu, ldwd = _ffn_operands(x, w_gate, w_up, w_down, act)
     _typed(dy, dt, "dy")

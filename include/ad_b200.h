@@ -306,7 +306,8 @@ int ad_feed_forward(int device, int dtype, int act, const void* x, int64_t ldx, 
                     float* gate, int64_t ldg, float* up, int64_t ldu, void* workspace,
                     size_t workspace_bytes, void* stream);
 /* The gradients of x (of dtype) and the weights (of dw_type: dtype or AD_F32; added
- * to what is there when `accumulate`; with no rows zeros or left alone). */
+ * to what is there when `accumulate`; with no rows zeros or left alone).  Those of g and u
+ * are rounded to dtype as they are on the way: in AD_F16 they have the range of dy. */
 int ad_feed_forward_grad(int device, int dtype, int act, const void* dy, int64_t lddy, const void* x,
                          int64_t ldx, const void* w_gate, int64_t ld_gate, const void* w_up,
                          int64_t ld_up, const void* w_down, int64_t ld_down, const float* gate,

@@ -295,7 +295,10 @@ struct Slope : SlopeCosts {
 
 // ------------------------------------------------------------------ host
 
-constexpr long long PIECE = 1ll << 28;  // elements of dz at a time, about: half a gigabyte
+// Elements of dz at a time: about half a gigabyte, up to one and a half times that.  Only the vocabulary is
+// cut, and a piece has about 1024 columns or more, so that above 2^18 rows dz takes 2 to 4 KB a row, like operands of
+// that width (and sums of dx, 4 bytes an element).
+constexpr long long PIECE = 1ll << 28;
 
 struct Layout {
   bool pack_x, pack_w;

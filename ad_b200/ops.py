@@ -884,7 +884,9 @@ def linear_logprobs_grad(x, weight, tokens, stats, g_logp=None, g_lse=None, *, s
     ``stats``.  Logits are made again a piece of the vocabulary at a time; their gradients are rounded to
     the operands' type (float16: held to 2^-38 of the largest) and summed in 32 bits.  ``out``: a
     ``LinearLogprobsGrads`` to write, the weight's of its type or float32, to which the gradient is added
-    with ``accumulate``; ``workspace``: as for ``linear_logprobs``."""
+    with ``accumulate``; ``workspace``: as for ``linear_logprobs``.  It holds a piece's gradients (half a gigabyte, up to
+    one and a half times that; above 2^18 rows 2 to 4 KB a row), where there are several pieces the gradient of ``x`` in 32
+    bits, and 39 MB of partial sums."""
     dev, dt, rows, width, vocab, ldx, ldw, t64 = _linear_operands(x, weight, tokens, scale)
     for v, n, name in ((stats, 2, "stats"), (g_logp, 1, "g_logp"), (g_lse, 1, "g_lse")):
         if v is not None or n == 2:

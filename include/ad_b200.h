@@ -283,7 +283,9 @@ int ad_linear_logprobs(int device, int dtype, const void* x, int64_t ldx, const 
  * logp and lse (rows floats each; NULL: zeros); W's is added to what dw holds when
  * `accumulate`.  Logits are made again a piece of the vocabulary at a time, and
  * their gradients rounded to dtype as operands (AD_F16: times a power of two that
- * puts the largest at 2^14; they are held to 2^-38 of it). */
+ * puts the largest at 2^14; they are held to 2^-38 of it; g_logp of rows without a
+ * token has no part in anything).  A piece has about 2^28 logits, up to 1.5 times
+ * that, but about 1024 columns or more: above 2^18 rows its workspace grows by 2 to 4 KB a row. */
 int ad_linear_logprobs_grad(int device, int dtype, const void* x, int64_t ldx, const void* weight,
                             int64_t ldw, int64_t rows, int64_t width, int64_t vocab,
                             const void* tokens, int tok64, float scale, const float* stats,

@@ -216,3 +216,17 @@ for _ in range(2):
 """ % (which, which)
     r = subprocess.run([sys.executable, "-c", code], cwd=root, env={**os.environ, "PYTHONPATH": root}, capture_output=True, text=True, timeout=120)
     assert r.returncode == 0, r.stderr[-2000:]
+
+
+def test_linear_logprobs_workspaces(ops):
+    """As documented: logits' gradients of a piece of the vocabulary, at most 1.5 times 2^28 elements (and a round to 256
+    columns), or 2 KB to 4 KB a row where rows are many; the sums of x's gradient in 32 bits beside several pieces; 2 x
+    74 tiles of partial sums.  Forward: two floats for each row and 256 or fewer tokens."""
+    for rows, width, vocab in ((1, 64, 100), (2047, 1024, 50001), (8192, 2048, 65537), (9000, 24, 50003), (1 << 18, 64, 131072),
+                               (1 << 20, 512, 50000), (1 << 24, 64, 200000), (1 << 24, 64, 1)):
+        x, w = (ops.DeviceArray(1 << 20, s, "bfloat16") for s in ((rows, width), (vocab, width)))
+        dz = min(max(3 * 2 ** 28 + 512 * rows, 4096 * rows), 2 * rows * (vocab + 8))
+        sums = 4 * rows * width if rows * vocab > 2 ** 28 else 0
+        need = ops.linear_logprobs_workspace(x, w, True)
+        assert need <= dz + sums + 2 * 74 * 4 * 256 * 256 + 4096, (rows, width, vocab, need)
+        assert ops.linear_logprobs_workspace(x, w) <= 8 * rows * (vocab // 64 + 2) + 4096

@@ -2,7 +2,8 @@
 // added to others, several products in one launch, and copies of operands whose
 // rows are not aligned to the 16 bytes that TMA asks for.
 //
-// Up to 2048 tiles are dealt out from a list that the host makes: whole tiles, the
+// Tiles are dealt out from a list of up to 2048 units that the host makes (schedule.h; with room
+// for three parts a block, 1826 tiles of pairs, 1604 of single ones; more go by number): whole tiles, the
 // longest first, each to the blocks that are done first, and those that would stick
 // out above the others cut along K so that all end together (where that saves more than the partial
 // sums' way through memory costs).  The list goes with the kernel's parameters.  What

@@ -20,8 +20,8 @@
 // products.  Tiles are walked in bands of rows, so that the tiles under way at a time
 // share operands in L2.  The two issuing threads are the narrowest place: with what they
 // do for 64 elements of K computed as it comes (which stage, which operands, descriptors
-// of 64 bits) 16384 x 2048 over 8192 took 400 to 430 us, with loops that only count 320 to
-// 340 (1.65 PFLOP/s; cuBLAS 359), although loads left out altogether had changed little.
+// of 64 bits) 16384 x 2048 over 8192 took 400 to 430 us, with loops that only count
+// 334 (1.65 PFLOP/s; cuBLAS 359), although loads left out altogether had changed little.
 // Products to memory (gemm16.cu) are dealt out as whole tiles and, where the last round
 // would leave blocks without one, as parts of a tile's K, whose sums are joined in
 // order.  Nothing depends on scheduling.

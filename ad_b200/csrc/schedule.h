@@ -29,7 +29,9 @@ int kblocks_of(const P& p) {
 
 constexpr int MAX_WORKERS = 256;
 constexpr int SMALL_LIST = 256, LARGE_LIST = 2048;  // units of a launch: 3 and 25 KB of parameters
-constexpr int LEAST = 6;                            // 64 elements of K that a part of a tile has at least
+// 64 elements of K that a part of a tile has at least (anything from 2 to 12 takes the same time, within the
+// noise, for gradients of 600 to 8000 rows of 512 to 2048).
+constexpr int LEAST = 6;
 
 struct Listed {
   unsigned where;  // group, row and column of the tile
@@ -82,7 +84,9 @@ bool make_schedule(const P* p, int count, int tiling, int workers, Schedule& s) 
   int height = static_cast<int>((total + all + workers - 1) / workers) + 1;
   // A few tiles that are longer than that, beside others: all of them in the same parts, so that
   // those under way at a time share operands in L2 (dx and dW of 2047 x 50001 over 1024, cut at
-  // odd places: 342 us and 1.5 GB from memory; so 303 and 0.5).
+  // odd places: 342 us and 1.5 GB from memory; so 303 and 0.5).  Parts of at most 3/5 of the height: of
+  // all of it, gradients of 64 x 2048 over 32000 tokens take 135 us instead of 93; of 2/5 the example is not cut in parts
+  // any more, and its gradients take 540 us instead of 473.
   int parts[MAX_GROUPS], length[MAX_GROUPS];
   bool in_parts = false;
   int budget = workers;  // for parts: no more of them than workers, those of all groups together
@@ -143,7 +147,9 @@ bool make_schedule(const P* p, int count, int tiling, int workers, Schedule& s) 
   std::stable_sort(by_load, by_load + workers, [&](int a, int b) { return load[a] < load[b]; });
   for (int i = 0; i < left; ++i) give(rest[i].where, 0, rest[i].k, -1);  // uncut
   // Cut, the remaining tiles fill all workers up to one height.
-  const double slot_us = 2.0 * 4 * t.m * t.n / 3e6;  // a part's sums, there and back at 3 TB/s
+  // a part's sums, there and back at 3 TB/s (at 1, too few tiles are cut: 36 us instead of 28 and 87 instead of
+  // 78 for the gradients of 600 and 4095 x 512 x 2048; at 9 the same as at 3)
+  const double slot_us = 2.0 * 4 * t.m * t.n / 3e6;
   s.us = most * t.us + 4.0 + (slots ? 5.0 + slot_us * slots : 0.0);
   // about one part for each worker
   bool cut = !in_parts && left > 0 && left < workers && height > LEAST && (most - height) * t.us > 5.0 + slot_us * workers;

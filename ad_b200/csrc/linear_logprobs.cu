@@ -41,10 +41,10 @@ __device__ __forceinline__ float ex2(float x) {
 // rounded to nearest there: what the tensor cores truncate grows with the sum that they add to (lse of width
 // 4096 over dense states: 1.9e-6 of it in one accumulator, 4.4e-7 in four parts; of 1024 4.6e-7).  The same
 // parts forward and backward, or a probability near 1 would be off by the difference.  A part's
-// products take longer than an epilogue, which so stays hidden, and what the joins cost is 3 to 8%: 2047 x 1600 over
-// 50001 tokens takes 274 us forward instead of 254 and 840 backward instead of 793, 2000 x 4096 over 32000
-// 455 and 1345 instead of 433 and 1318.  (Below 1536 parts would be shorter than an epilogue: of 550, 323 us instead
-// of 295.)
+// products take longer than an epilogue, which so stays hidden, and what the joins cost is 2 to 8%: 8192 x 2048 over
+// 65537 tokens takes 5430 us backward instead of 5180, 2047 x 1600 over 50001 290 forward instead of 272 and 895
+// backward instead of 860, 2000 x 4096 over 32000 445 and 1435 instead of 430 and 1400 (medians of three runs by turns;
+// forward at 2048 within the noise).  Below 1536 parts would be shorter than an epilogue: of 550, 323 us instead of 295.
 constexpr int LENGTH = 1024, WHOLE = 1536;
 template <bool FOLD, int WARPS>
 struct Held {

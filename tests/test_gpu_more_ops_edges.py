@@ -5,7 +5,7 @@ import math
 
 import pytest
 
-from .test_gpu_more_ops import HALVES, close, linear64, linear_operands
+from .test_gpu_more_ops import HALVES, close, linear64, linear_operands, tc
 from .test_gpu_ops import E, U, dtype, rand, seeded
 
 pytestmark = pytest.mark.gpu
@@ -135,6 +135,52 @@ def test_linear_logprobs_of_logits_that_grow_evenly(ops, t, width):
     top = (x.double() @ w.double().T).amax(-1)
     others = (math.log(300) + 4) * 4 + 300 / 64 + 64 + 4 * (want["lse"] + top)
     assert ((r.lse.double() - want["lse"]) <= 1.05 * E * others).all()
+
+
+@pytest.mark.parametrize("t", HALVES)
+@pytest.mark.parametrize("rows,width,vocab", [(1, 1537, 300), (9, 2500, 40000), (64, 1600, 1000), (130, 1601, 3000), (300, 4100, 700),
+                                              (700, 2111, 9000), (2000, 1700, 20000)])
+def test_linear_logprobs_of_wide_layers(ops, t, rows, width, vocab):
+    """Widths that are summed in parts, on tiles of each size, one and several for a block; the same bits again."""
+    x, w, tokens, gp, gl = linear_operands(t, rows, width, vocab)
+    want = linear64(x, w, tokens, 1.0, gp, gl, t)
+    r = ops.linear_logprobs(x, w, tokens)
+    close(r.logp, want["logp"], want["elp"], "float32")
+    close(r.lse, want["lse"], want["elf"], "float32")
+    g = ops.linear_logprobs_grad(x, w, tokens, r.stats, gp, gl)
+    close(g.x, want["dx"], want["edx"], t)
+    close(g.weight, want["dw"], want["edw"], t)
+    for _ in range(3):
+        q = ops.linear_logprobs(x, w, tokens)
+        h = ops.linear_logprobs_grad(x, w, tokens, q.stats, gp, gl)
+        assert all(torch.equal(a, b) for a, b in zip((*r, *g), (*q, *h)))
+
+
+@pytest.mark.parametrize("t", HALVES)
+@pytest.mark.parametrize("width", [1000, 1536, 1600, 4096])
+def test_linear_logprobs_of_a_row_that_is_sure(ops, t, width):
+    """Logits of the backward pass are those of the forward one, bit for bit: where the token is far ahead, dz is 1 - 1 / sum,
+    where the sum is 1 and the others' exponentials.  That is off by 4 E and by their share of it, which
+    moves by at most twice a logit's error (tc) and by an exponential's (16 E, arguments below 16); p of
+    another token by the same share; both are rounded once."""
+    gen = seeded(width, len(t))
+    w = rand(gen, (400, width), t, width ** -0.5)
+    x = (12.0 * w[:40].double() + 0.01 * rand(gen, (40, width), "float32").double()).to(dtype(t))
+    tokens = torch.arange(40, device="cuda")
+    out = (torch.empty_like(x), torch.empty(w.shape, device="cuda"))
+    r = ops.linear_logprobs(x, w, tokens)
+    g = ops.linear_logprobs_grad(x, w, tokens, r.stats, torch.ones(40, device="cuda"), out=out)
+    x, w = x.double(), w.double()
+    p = torch.softmax(x @ w.T, -1)
+    move = 2 * tc(width) * (x.abs() @ w.abs().T).amax(-1) + 16 * E
+    d, ed = -p, p * move[:, None]
+    rest = p.clone()
+    rest[tokens, tokens] = 0
+    miss = rest.sum(-1)
+    assert 1e-4 < float(miss.min()) and float(miss.max()) < 2e-2
+    d[tokens, tokens], ed[tokens, tokens] = miss, miss * move + 4 * E
+    ed += U[t] * d.abs() + 2.0 ** -38
+    close(g.weight, d.T @ x, ed.T @ x.abs() + tc(40) * (d.abs().T @ x.abs()), "float32")
 
 
 # ------------------------------------------------------------------ gated feed-forward blocks
